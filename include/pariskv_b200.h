@@ -527,6 +527,50 @@ int pk_silu_mul(const pk_tensor* gate_up, const pk_tensor* out, void* stream);
  *   rounded like pk_silu_mul after a separate product.  I a multiple of 8, at most 24576. */
 int pk_gemv(const pk_tensor* weight, const pk_tensor* x, const pk_tensor* out, int gated, void* stream);
 
+/* ---- several tokens a step: a tree of drafts, blocks of the cache, 4-bit weights ------------------------- */
+
+/* Positions follow the device: lengths i32 [bs] holds the rows of the cache per sample (values outside [0, cap] are clamped),
+ * so that a captured step stays valid while the sequences grow.  Rows of 128 bf16 with a unit inner stride, the other strides
+ * multiples of 8 elements, 16-byte aligned.  A query that sees no row gets zeros, and lse = -inf.  What a query does not see
+ * does not reach it, whatever is stored there (NaN and infinities included).  lse (f32 [bs,T,Hq] or NULL) is the log2 of the
+ * softmax denominator, as in pk_sparse_attention.  workspace: device, 256-byte aligned, pk_*_workspace_bytes; nothing in it
+ * has to be cleared and nothing carries over between calls.  No counterpart in the reference.
+ *
+ * pk_tree_attention: T drafted tokens per sequence (at most 256) attend to rows [0, lengths[b]) of the cache and to the drafts that
+ *   tree_mask[b][t] names.  queries bf16 [bs,T,Hq,128], query head h*G+g belonging to KV head h; keys / values bf16
+ *   [bs,H,cap,128]; draft_keys / draft_values bf16 [bs,T,H,128]; tree_mask u8 [1 or bs,T,T], nonzero: token t sees draft j (a
+ *   token sees itself only if its own entry says so); out bf16 [bs,T,Hq,128].
+ * pk_block_bounds: bounds[b,h,j] = (lo, hi), smallest and largest value per channel of the rows j*block .. that are below
+ *   lengths[b] (NULL: cap), bf16 [bs,H,ceil(cap/block),2,128]; block 16, 32, 64 or 128.  n_new >= 0: only the blocks that hold
+ *   the last n_new rows, each from all of its rows (so that rows taken back since leave no trace); -1: all.  Blocks without
+ *   rows are left as they are.  A NaN in a channel makes that channel's bounds NaN.
+ * pk_select_blocks: token t of T is at position lengths[b] - T + t and sees the blocks up to its own.  Of these the n = blocks.shape[3]
+ *   with the largest score are listed in blocks i32 [bs,T,H,n], ascending, -1 behind the last; the first sink_blocks and the
+ *   last local_blocks (>= 1) are always among them.  score = sum over the group's query heads and the channels of
+ *   max(q lo, q hi) (a zero of q adds nothing), summed in 64 bits and rounded once to 32; ties go to the lower block, a NaN score is
+ *   above all others.
+ * pk_block_attention: query (b,t,h*G+g), at the same position, attends to the rows up to it of the listed blocks.  Entries below zero
+ *   and blocks behind the position are skipped; the order is free; a block listed twice counts twice.
+ * pk_gemv_w4: out[T,O] = x[T,I] W^T for up to 16 tokens, fp32 sums.  weight u8 [O,I/2], the low nibble of a byte the even column;
+ *   scales bf16 [O,I/group], group 32, 64 or 128; W = (code - 8) * scale, or code * scale + offset with offsets bf16 like scales.
+ *   gated: weight is [gate; up] stacked, out[T,O/2] = silu(gate x) * (up x), rounded once.  I at most 32768. */
+int64_t pk_tree_attention_workspace_bytes(int64_t bs, int64_t T, int64_t Hq, int64_t H, int64_t cap);
+int pk_tree_attention(const pk_tensor* queries, const pk_tensor* keys, const pk_tensor* values, const pk_tensor* draft_keys,
+                      const pk_tensor* draft_values, const pk_tensor* tree_mask, const pk_tensor* lengths, float scale,
+                      const pk_tensor* out, const pk_tensor* lse, void* workspace, int64_t workspace_bytes, void* stream);
+int pk_block_bounds(const pk_tensor* keys, const pk_tensor* lengths, int64_t block, int64_t n_new, const pk_tensor* bounds,
+                    void* stream);
+int64_t pk_select_blocks_workspace_bytes(int64_t bs, int64_t T, int64_t H, int64_t n_blocks);
+int pk_select_blocks(const pk_tensor* queries, const pk_tensor* bounds, const pk_tensor* lengths, int64_t block,
+                     int64_t sink_blocks, int64_t local_blocks, const pk_tensor* blocks, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+int64_t pk_block_attention_workspace_bytes(int64_t bs, int64_t T, int64_t Hq, int64_t H, int64_t n, int64_t block);
+int pk_block_attention(const pk_tensor* queries, const pk_tensor* keys, const pk_tensor* values, const pk_tensor* blocks,
+                       const pk_tensor* lengths, int64_t block, float scale, const pk_tensor* out, const pk_tensor* lse,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+int pk_gemv_w4(const pk_tensor* weight, const pk_tensor* scales, const pk_tensor* offsets, const pk_tensor* x,
+               const pk_tensor* out, int gated, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

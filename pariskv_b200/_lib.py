@@ -101,6 +101,14 @@ SIGNATURES = {
     "pk_add_rmsnorm": (_INT, [TP, TP, TP, TP, TP, ctypes.c_double, _VP]),
     "pk_silu_mul": (_INT, [TP, TP, _VP]),
     "pk_gemv": (_INT, [TP, TP, TP, _INT, _VP]),
+    "pk_tree_attention_workspace_bytes": (_I64, [_I64] * 5),
+    "pk_tree_attention": (_INT, [TP] * 7 + [_F32, TP, TP, _VP, _I64, _VP]),
+    "pk_block_bounds": (_INT, [TP, TP, _I64, _I64, TP, _VP]),
+    "pk_select_blocks_workspace_bytes": (_I64, [_I64] * 4),
+    "pk_select_blocks": (_INT, [TP, TP, TP, _I64, _I64, _I64, TP, _VP, _I64, _VP]),
+    "pk_block_attention_workspace_bytes": (_I64, [_I64] * 6),
+    "pk_block_attention": (_INT, [TP] * 5 + [_I64, _F32, TP, TP, _VP, _I64, _VP]),
+    "pk_gemv_w4": (_INT, [TP] * 5 + [_INT, _VP]),
 }
 
 _lib = None

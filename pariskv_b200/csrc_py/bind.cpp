@@ -12,6 +12,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -595,6 +596,153 @@ PyObject* py_gemv(PyObject*, PyObject* const* a, Py_ssize_t n) {
   PK_PY_END
 }
 
+// ---- several tokens a step.  Scratch comes from torch's allocator on the current stream for each call: calls on other streams and
+// in captured graphs have their own.  The tensors' device is made current for the launches.
+
+bool same_device(std::initializer_list<const Arg*> args, const at::Tensor& like) {
+  for (const Arg* a : args)
+    if (a->t && a->t->device() != like.device()) {
+      PyErr_SetString(PyExc_RuntimeError, "pariskv_b200: the tensors of a call must be on one device");
+      return false;
+    }
+  return true;
+}
+bool dims(const Arg& a, int n, const char* what) {
+  if (a.d.ndim == n) return true;
+  PyErr_Format(PyExc_RuntimeError, "pariskv_b200: %s must have %d dimensions, has %d", what, n, (int)a.d.ndim);
+  return false;
+}
+// A mask: bool or uint8.
+bool take_mask(PyObject* o, Arg* a) {
+  if (o == Py_None || !THPVariable_Check(o) || THPVariable_Unpack(o).scalar_type() != at::kBool) return need(o, a, CUDA);
+  a->t = &THPVariable_Unpack(o);
+  if (!a->t->is_cuda()) {
+    PyErr_SetString(PyExc_RuntimeError, "pariskv_b200 ops need CUDA tensors; there is no CPU fallback");
+    return false;
+  }
+  const int64_t n = a->t->dim();
+  if (n > PK_MAX_DIMS) return PyErr_SetString(PyExc_ValueError, "too many dimensions"), false;
+  a->d.data = a->t->data_ptr(), a->d.dtype = PK_U8, a->d.ndim = (int32_t)n;
+  for (int64_t i = 0; i < n; i++) a->d.shape[i] = a->t->size(i), a->d.stride[i] = a->t->stride(i);
+  return true;
+}
+
+// (queries, keys, values, draft_keys, draft_values, tree_mask, lengths, scale, out, lse) -> out
+PyObject* py_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 10, "tree_attention")) return nullptr;
+  PK_PY_BEGIN
+  Arg q, k, v, dk, dv, m, len, out, lse;
+  at::Tensor own;
+  double scale;
+  if (!need(a[0], &q, CUDA) || !need(a[1], &k, CUDA) || !need(a[2], &v, CUDA) || !need(a[3], &dk, CUDA) || !need(a[4], &dv, CUDA) ||
+      !take_mask(a[5], &m) || !need(a[6], &len, CUDA) || !to_f64(a[7], &scale) || !take(a[9], &lse, CUDA) ||
+      !dims(q, 4, "queries") || !dims(k, 4, "keys"))
+    return nullptr;
+  const c10::cuda::CUDAGuard guard(q.t->device());
+  if (!output(a[8], &out, &own, *q.t, q.t->sizes(), at::kBFloat16) || !same_device({&k, &v, &dk, &dv, &m, &len, &out, &lse}, *q.t)) return nullptr;
+  if (q.t->numel() == 0) return give(a[8], out);
+  const int64_t bytes = pk_tree_attention_workspace_bytes(q.d.shape[0], q.d.shape[1], q.d.shape[2], k.d.shape[1], k.d.shape[2]);
+  const at::Tensor ws = empty_on(*q.t, {bytes}, at::kByte);
+  void* st = stream_of(*q.t);
+  const int rc = without_gil([&] {
+    return pk_tree_attention(q.p(), k.p(), v.p(), dk.p(), dv.p(), m.p(), len.p(), (float)scale, out.p(), lse.p(), ws.data_ptr(), bytes, st);
+  });
+  if (rc) return raise(rc);
+  return give(a[8], out);
+  PK_PY_END
+}
+
+// (keys, lengths or None, block, n_new, bounds or None) -> bounds
+PyObject* py_block_bounds(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 5, "block_bounds")) return nullptr;
+  PK_PY_BEGIN
+  Arg k, len, out;
+  at::Tensor own;
+  int64_t block, n_new;
+  if (!need(a[0], &k, CUDA) || !take(a[1], &len, CUDA) || !to_i64(a[2], &block) || !to_i64(a[3], &n_new) || !dims(k, 4, "keys")) return nullptr;
+  if (block < 1) return PyErr_SetString(PyExc_RuntimeError, "pariskv_b200: block must be 16, 32, 64 or 128"), nullptr;
+  const c10::cuda::CUDAGuard guard(k.t->device());
+  if (!output(a[4], &out, &own, *k.t, {k.d.shape[0], k.d.shape[1], (k.d.shape[2] + block - 1) / block, 2, 128}, at::kBFloat16) ||
+      !same_device({&len, &out}, *k.t))
+    return nullptr;
+  if (k.t->numel() == 0) return give(a[4], out);
+  void* st = stream_of(*k.t);
+  const int rc = without_gil([&] { return pk_block_bounds(k.p(), len.p(), block, n_new, out.p(), st); });
+  if (rc) return raise(rc);
+  return give(a[4], out);
+  PK_PY_END
+}
+
+// (queries, bounds, lengths, n_select, block, sink_blocks, local_blocks, blocks or None) -> blocks
+PyObject* py_select_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 8, "select_blocks")) return nullptr;
+  PK_PY_BEGIN
+  Arg q, bd, len, out;
+  at::Tensor own;
+  int64_t k, block, sink, local;
+  if (!need(a[0], &q, CUDA) || !need(a[1], &bd, CUDA) || !need(a[2], &len, CUDA) || !to_i64(a[3], &k) || !to_i64(a[4], &block) ||
+      !to_i64(a[5], &sink) || !to_i64(a[6], &local) || !dims(q, 4, "queries") || !dims(bd, 5, "bounds"))
+    return nullptr;
+  if (k < 1) return PyErr_SetString(PyExc_RuntimeError, "pariskv_b200: n_select must be at least 1"), nullptr;
+  const c10::cuda::CUDAGuard guard(q.t->device());
+  if (!output(a[7], &out, &own, *q.t, {q.d.shape[0], q.d.shape[1], bd.d.shape[1], k}, at::kInt) || !same_device({&bd, &len, &out}, *q.t)) return nullptr;
+  if (q.t->numel() == 0) return give(a[7], out);
+  const int64_t bytes = pk_select_blocks_workspace_bytes(q.d.shape[0], q.d.shape[1], bd.d.shape[1], bd.d.shape[2]);
+  const at::Tensor ws = empty_on(*q.t, {bytes}, at::kByte);
+  void* st = stream_of(*q.t);
+  const int rc = without_gil([&] { return pk_select_blocks(q.p(), bd.p(), len.p(), block, sink, local, out.p(), ws.data_ptr(), bytes, st); });
+  if (rc) return raise(rc);
+  return give(a[7], out);
+  PK_PY_END
+}
+
+// (queries, keys, values, blocks, lengths, block, scale, out, lse) -> out
+PyObject* py_block_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 9, "block_attention")) return nullptr;
+  PK_PY_BEGIN
+  Arg q, k, v, ids, len, out, lse;
+  at::Tensor own;
+  int64_t block;
+  double scale;
+  if (!need(a[0], &q, CUDA) || !need(a[1], &k, CUDA) || !need(a[2], &v, CUDA) || !need(a[3], &ids, CUDA) || !need(a[4], &len, CUDA) ||
+      !to_i64(a[5], &block) || !to_f64(a[6], &scale) || !take(a[8], &lse, CUDA) || !dims(q, 4, "queries") || !dims(k, 4, "keys") ||
+      !dims(ids, 4, "blocks"))
+    return nullptr;
+  const c10::cuda::CUDAGuard guard(q.t->device());
+  if (!output(a[7], &out, &own, *q.t, q.t->sizes(), at::kBFloat16) || !same_device({&k, &v, &ids, &len, &out, &lse}, *q.t)) return nullptr;
+  if (q.t->numel() == 0) return give(a[7], out);
+  const int64_t bytes = pk_block_attention_workspace_bytes(q.d.shape[0], q.d.shape[1], q.d.shape[2], k.d.shape[1], ids.d.shape[3], block);
+  const at::Tensor ws = empty_on(*q.t, {bytes}, at::kByte);
+  void* st = stream_of(*q.t);
+  const int rc = without_gil([&] {
+    return pk_block_attention(q.p(), k.p(), v.p(), ids.p(), len.p(), block, (float)scale, out.p(), lse.p(), ws.data_ptr(), bytes, st);
+  });
+  if (rc) return raise(rc);
+  return give(a[7], out);
+  PK_PY_END
+}
+
+// (weight, scales, offsets or None, x, gated) -> [T, O] or [T, O / 2]
+PyObject* py_gemv_w4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 5, "gemv_w4")) return nullptr;
+  PK_PY_BEGIN
+  Arg w, s, m, x, o;
+  at::Tensor own;
+  int64_t gated;
+  if (!need(a[0], &w, CUDA) || !need(a[1], &s, CUDA) || !take(a[2], &m, CUDA) || !need(a[3], &x, CUDA) || !to_i64(a[4], &gated) ||
+      !dims(w, 2, "weight") || !dims(x, 2, "x"))
+    return nullptr;
+  const c10::cuda::CUDAGuard guard(x.t->device());
+  const int64_t O = w.d.shape[0];
+  if (!output(Py_None, &o, &own, *x.t, {x.d.shape[0], gated ? O / 2 : O}, at::kBFloat16) || !same_device({&w, &s, &m}, *x.t)) return nullptr;
+  if (own.numel() == 0) return THPVariable_Wrap(own);
+  void* st = stream_of(*x.t);
+  const int rc = without_gil([&] { return pk_gemv_w4(w.p(), s.p(), m.p(), x.p(), o.p(), gated != 0, st); });
+  if (rc) return raise(rc);
+  return THPVariable_Wrap(own);
+  PK_PY_END
+}
+
 PyObject* py_attention_workspace_bytes(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arity(n, 3, "attention_workspace_bytes")) return nullptr;
   int64_t v[3];
@@ -633,6 +781,11 @@ PyMethodDef methods[] = {
     PK_METHOD("add_rmsnorm", py_add_rmsnorm),
     PK_METHOD("silu_mul", py_silu_mul),
     PK_METHOD("gemv", py_gemv),
+    PK_METHOD("tree_attention", py_tree_attention),
+    PK_METHOD("block_bounds", py_block_bounds),
+    PK_METHOD("select_blocks", py_select_blocks),
+    PK_METHOD("block_attention", py_block_attention),
+    PK_METHOD("gemv_w4", py_gemv_w4),
     PK_METHOD("attention_workspace_bytes", py_attention_workspace_bytes),
     PK_METHOD("retrieve_workspace_bytes", py_retrieve_workspace_bytes),
     {nullptr, nullptr, 0, nullptr}};

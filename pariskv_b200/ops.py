@@ -501,3 +501,51 @@ def gemv(weight, x, gated=False):
     """x [1, I] @ weight[O, I]^T -> [1, O] (bf16, fp32 accumulation) for one token; gated: weight = [gate; up] stacked,
     result [1, O/2] = silu(gate x) * (up x).  See pk_gemv."""
     return L.native().gemv(weight, x, gated)
+
+
+# --------------------------------------------------------------------------------------------------
+# several tokens a step: a tree of drafts, blocks of the cache, 4-bit weights
+# --------------------------------------------------------------------------------------------------
+def tree_attention(queries, keys, values, draft_keys, draft_values, tree_mask, lengths, scale=None, out=None, lse=None):
+    """Attention of T drafted tokens per sequence over the cache and over the drafts themselves.
+    queries bf16 [bs,T,Hq,128]; keys / values bf16 [bs,H,cap,128], of which sample b holds lengths[b] rows (i32 [bs], read on the
+    device); draft_keys / draft_values bf16 [bs,T,H,128]; tree_mask bool or uint8 [1 or bs,T,T]: token t sees draft j (itself
+    included only if the mask says so).  Returns bf16 [bs,T,Hq,128]; lse, if given (f32 [bs,T,Hq]), receives log2 of the softmax
+    denominators.  The verification of a tree needs one call per layer; see pk_tree_attention."""
+    return L.native().tree_attention(queries, keys, values, draft_keys, draft_values, tree_mask, lengths,
+                                     queries.shape[-1] ** -0.5 if scale is None else float(scale), out, lse)
+
+
+def block_bounds(keys, lengths=None, block=64, n_new=None, bounds=None):
+    """Smallest and largest value per channel of every block of `block` keys: keys bf16 [bs,H,cap,128], the first lengths[b] rows
+    (i32 [bs]; None: all) -> bf16 [bs,H,ceil(cap/block),2,128].  With n_new only the blocks of the last n_new rows are made
+    again, in the `bounds` given: what a step that appends rows (or takes drafts back and appends others) calls.  Blocks
+    without rows are left as they are.  See pk_block_bounds."""
+    if n_new is not None and n_new < 0:
+        raise ValueError("n_new must not be negative")
+    if n_new is not None and bounds is None:
+        raise ValueError("n_new updates the bounds of a cache: they have to be given")
+    return L.native().block_bounds(keys, lengths, int(block), -1 if n_new is None else int(n_new), bounds)
+
+
+def select_blocks(queries, bounds, lengths, n_select, block=64, sink_blocks=1, local_blocks=1, blocks=None):
+    """The n_select blocks with the largest scores for every token and KV head, and always the first sink_blocks and the last
+    local_blocks that the token sees: queries bf16 [bs,T,Hq,128], the last T tokens of the sequences, bounds as block_bounds
+    makes them -> i32 [bs,T,H,n_select], ascending, -1 behind the last.  A block's score is an upper bound of the sum of its
+    best products with the group's query heads.  See pk_select_blocks."""
+    return L.native().select_blocks(queries, bounds, lengths, int(n_select), int(block), int(sink_blocks), int(local_blocks), blocks)
+
+
+def block_attention(queries, keys, values, blocks, lengths, block=64, scale=None, out=None, lse=None):
+    """Attention of the last T tokens of the sequences over the listed blocks of the cache, each token up to its own position:
+    queries bf16 [bs,T,Hq,128], keys / values bf16 [bs,H,cap,128], blocks i32 [bs,T,H,n] (select_blocks; entries below zero are
+    skipped), lengths i32 [bs] -> bf16 [bs,T,Hq,128].  See pk_block_attention."""
+    return L.native().block_attention(queries, keys, values, blocks, lengths, int(block),
+                                      queries.shape[-1] ** -0.5 if scale is None else float(scale), out, lse)
+
+
+def gemv_w4(weight, scales, x, offsets=None, gated=False):
+    """x [T, I] @ W^T -> bf16 [T, O] for up to 16 tokens and W of 4-bit codes: weight u8 [O, I/2] (low nibble: even column), scales
+    bf16 [O, I/group], group 32, 64 or 128.  W = (code - 8) * scale, with offsets (bf16 like scales) code * scale + offset.  gated:
+    weight = [gate; up] stacked, result [T, O/2] = silu(gate x) * (up x).  See pk_gemv_w4."""
+    return L.native().gemv_w4(weight, scales, offsets, x, gated)

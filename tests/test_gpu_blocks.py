@@ -1,0 +1,208 @@
+"""Block bounds, selection of blocks and attention over them against the definitions."""
+import pytest
+import torch
+
+import many_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def rnd(seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return lambda *s: torch.randn(*s, generator=g, device=DEV).to(torch.bfloat16)
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("bs,H,cap,lengths", [(1, 1, 1, [1]), (2, 3, 200, [200, 0]), (3, 2, 1000, [999, 64, 65]), (2, 1, 4097, [4097, -3]),
+                                              (1, 8, 20000, [30000]), (20, 1, 70, list(range(20)))])
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+def test_bounds(bs, H, cap, lengths, block):
+    from pariskv_b200 import ops
+    keys = rnd(cap + block)(bs, H, cap, 128)
+    old = torch.full((bs, H, (cap + block - 1) // block, 2, 128), 9.0, dtype=torch.bfloat16, device=DEV)
+    for n_new in (None, 0, 1, 3, block, 2 * block + 1, cap + 5):
+        got = old.clone()
+        assert ops.block_bounds(keys, i32(lengths), block=block, n_new=n_new, bounds=got) is got
+        assert torch.equal(got, R.bounds(keys, lengths, block, old, n_new)), n_new
+    want = R.bounds(keys, [cap] * bs, block, old)
+    assert torch.equal(ops.block_bounds(keys, block=block), want)
+
+
+def test_bounds_of_strided_keys_with_nan_and_infinities():
+    from pariskv_b200 import ops
+    store = rnd(1)(2, 3, 150, 2, 128)
+    keys = store[:, :, :, 1]
+    keys[0, 0, 5, 7], keys[0, 1, 70, 3], keys[1, 2, 149, 0], keys[1, 0, :, 9] = float("nan"), float("inf"), float("-inf"), -0.0
+    big = torch.zeros(2, 3, 5, 2, 128, dtype=torch.bfloat16, device=DEV)
+    got = ops.block_bounds(keys, i32([150, 140]), block=32, bounds=big)
+    want = R.bounds(keys, [150, 140], 32, torch.zeros_like(big))
+    assert torch.equal(got.nan_to_num(77.0, 1e30, -1e30), want.nan_to_num(77.0, 1e30, -1e30))
+    assert got[0, 0, 0, :, 7].isnan().all()
+
+
+SELECT = [(1, 1, 1, 1, 16, [1], 1, 16, 0, 1), (1, 1, 2, 4, 700, [700], 5, 16, 1, 1), (2, 3, 2, 3, 1000, [1000, 2], 6, 32, 1, 2), (1, 2, 1, 8, 5000, [4999], 33, 16, 2, 3),
+          (3, 1, 2, 5, 300, [300, 64, 0], 4, 64, 0, 1), (2, 16, 1, 4, 900, [900, 10], 7, 128, 1, 1), (1, 1, 8, 4, 40000, [39990], 32, 64, 1, 2),
+          (1, 1, 1, 2, 200000, [199999], 100, 16, 1, 1), (1, 1, 2, 16, 2100, [2100], 40, 64, 3, 4), (2, 40, 1, 1, 260, [260, 39], 3, 16, 0, 2)]
+
+
+@pytest.mark.parametrize("bs,T,H,G,cap,lengths,n,block,sink,local", SELECT)
+def test_selection(bs, T, H, G, cap, lengths, n, block, sink, local):
+    from pariskv_b200 import ops
+    r = rnd(cap + n)
+    keys, q = r(bs, H, cap, 128), r(bs, T, H * G, 128)
+    bnd = ops.block_bounds(keys, i32(lengths), block=block, bounds=torch.full((bs, H, (cap + block - 1) // block, 2, 128), float("nan"), dtype=torch.bfloat16, device=DEV))
+    got = ops.select_blocks(q, bnd, i32(lengths), n, block=block, sink_blocks=sink, local_blocks=local)
+    want = R.select(q.cpu(), bnd.cpu(), lengths, n, block, sink, local)
+    assert torch.equal(got.cpu(), want)
+
+
+def test_ties_go_to_the_lower_block():
+    from pariskv_b200 import ops
+    r = rnd(2)
+    bnd = r(1, 1, 1, 2, 128).sort(3).values.expand(1, 1, 300, 2, 128).contiguous()
+    bnd[:, :, 250] += 8      # one block above the others
+    q = r(1, 1, 2, 128).abs()
+    got = ops.select_blocks(q, bnd, i32([300 * 16]), 20, block=16, sink_blocks=2, local_blocks=3)
+    assert got.flatten().tolist() == list(range(16)) + [250, 297, 298, 299]
+
+
+def test_scores_that_are_not_numbers():
+    """NaN above all others, -inf and zeros of both signs below; sink and local blocks all the same."""
+    from pariskv_b200 import ops
+    bnd = torch.zeros(1, 1, 64, 2, 128, dtype=torch.bfloat16, device=DEV)
+    bnd[:, :, :, 1] = 0.0
+    bnd[:, :, 5:9] = float("nan")
+    bnd[:, :, 20, :] = float("-inf")
+    bnd[:, :, 30, :] = float("inf")
+    bnd[:, :, 33, :, 0] = -0.0
+    q = torch.ones(1, 1, 1, 128, dtype=torch.bfloat16, device=DEV)
+    pick = lambda n: ops.select_blocks(q, bnd, i32([64 * 16]), n, block=16, sink_blocks=1, local_blocks=1).flatten().tolist()
+    assert pick(2) == [0, 63]
+    assert pick(5) == [0, 5, 6, 7, 63]
+    assert pick(7) == [0, 5, 6, 7, 8, 30, 63]
+    assert pick(9) == [0, 1, 2, 5, 6, 7, 8, 30, 63]
+    assert pick(63) == [j for j in range(64) if j != 20]
+    assert pick(70) == list(range(64)) + [-1] * 6
+
+
+@pytest.mark.parametrize("bs,T,H,G,cap,lengths,n,block,sink,local", SELECT)
+def test_attention_over_selected_blocks(bs, T, H, G, cap, lengths, n, block, sink, local):
+    from pariskv_b200 import ops
+    r = rnd(cap + n + 1)
+    keys, values, q = r(bs, H, cap, 128), r(bs, H, cap, 128), r(bs, T, H * G, 128)
+    for b, m in enumerate(lengths):
+        keys[b, :, m:], values[b, :, m:] = float("nan"), float("nan")
+    bnd = ops.block_bounds(keys, i32(lengths), block=block)
+    ids = ops.select_blocks(q, bnd, i32(lengths), n, block=block, sink_blocks=sink, local_blocks=local)
+    lse = torch.full(q.shape[:3], 7.0, device=DEV)
+    out = ops.block_attention(q, keys, values, ids, i32(lengths), block=block, lse=lse)
+    want, tol, wl, ltol = R.block_attention(q, keys, values, ids, lengths, block)
+    R.close(out, want, tol, "out")
+    R.close(lse, wl, ltol, "lse")
+
+
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+def test_lists_in_any_order_with_gaps_and_repeats(block):
+    from pariskv_b200 import ops
+    r = rnd(block)
+    bs, T, H, G, cap, lengths = 2, 3, 2, 4, 900, [900, 333]
+    keys, values, q = r(bs, H, cap, 128), r(bs, H, cap, 128), r(bs, T, H * G, 128) * 2
+    nb = (cap + block - 1) // block
+    ids = torch.randint(-2, nb + 3, (bs, T, H, 9), generator=torch.Generator().manual_seed(block)).to(torch.int32)
+    ids[0, 0, 0] = -1
+    ids[0, 1, 1, 2:5] = 1
+    ids[0, 2, 0, 3] = 2 ** 31 - 1
+    ids = ids.to(DEV)
+    out = ops.block_attention(q, keys, values, ids, i32(lengths), block=block)
+    want, tol, _, _ = R.block_attention(q, keys, values, ids.clamp(max=nb + 3), lengths, block)
+    R.close(out, want, tol)
+    assert (out[0, 0, :G] == 0).all()
+
+
+def test_strided_cache_and_queries():
+    from pariskv_b200 import ops
+    r = rnd(4)
+    store = r(2, 2, 500, 2, 128)
+    keys, values = store[:, :, :, 0], store[:, :, :, 1]
+    q = r(2, 5, 12, 128)[:, 1:4, 2:10]
+    bnd = ops.block_bounds(keys, i32([500, 77]), block=16)
+    ids = ops.select_blocks(q, bnd, i32([500, 77]), 6, block=16)
+    assert torch.equal(ids.cpu(), R.select(q.cpu(), bnd.cpu(), [500, 77], 6, 16, 1, 1))
+    out = ops.block_attention(q, keys, values, ids, i32([500, 77]), block=16, scale=0.3)
+    want, tol, _, _ = R.block_attention(q, keys, values, ids, [500, 77], 16, 0.3)
+    R.close(out, want, tol)
+
+
+def test_head_groups_of_every_size():
+    from pariskv_b200 import ops
+    for G in (1, 2, 7, 9, 16, 17, 32, 128):
+        r = rnd(G)
+        keys, values, q = r(1, 1, 300, 128), r(1, 1, 300, 128), r(1, 2, G, 128)
+        ids = i32([[[[0, 2, 4]], [[1, 2, 4]]]])
+        out = ops.block_attention(q, keys, values, ids, i32([290]), block=64)
+        want, tol, _, _ = R.block_attention(q, keys, values, ids, [290], 64)
+        R.close(out, want, tol, f"G={G}")
+
+
+def test_captured_step_while_the_sequences_grow():
+    """Append a row, update the bounds, select, attend: one captured graph, positions on the device."""
+    from pariskv_b200 import ops
+    r = rnd(5)
+    bs, H, G, cap, block = 2, 2, 4, 600, 32
+    keys, values = torch.zeros(bs, H, cap, 128, dtype=torch.bfloat16, device=DEV), torch.zeros(bs, H, cap, 128, dtype=torch.bfloat16, device=DEV)
+    start = [500, 95]
+    for b in range(bs):
+        keys[b, :, :start[b]], values[b, :, :start[b]] = r(H, start[b], 128), r(H, start[b], 128)
+    lengths = i32(start)
+    bnd = ops.block_bounds(keys, lengths, block=block, bounds=torch.zeros(bs, H, 19, 2, 128, dtype=torch.bfloat16, device=DEV))
+    q, k_new, v_new = r(bs, 1, H * G, 128), r(bs, H, 1, 128), r(bs, H, 1, 128)
+
+    def step():
+        at = lengths.long()[:, None, None, None].expand(-1, H, 1, 128)
+        keys.scatter_(2, at, k_new)
+        values.scatter_(2, at, v_new)
+        lengths.add_(1)
+        ops.block_bounds(keys, lengths, block=block, n_new=1, bounds=bnd)
+        ids = ops.select_blocks(q, bnd, lengths, 5, block=block, sink_blocks=1, local_blocks=2)
+        return ids, ops.block_attention(q, keys, values, ids, lengths, block=block)
+
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ids, out = step()
+    for i in range(70):
+        q.copy_(r(bs, 1, H * G, 128)), k_new.copy_(r(bs, H, 1, 128)), v_new.copy_(r(bs, H, 1, 128))
+        g.replay()
+        if i % 23 == 0 or i == 69:
+            n = [s + 2 + i for s in start]
+            want = R.bounds(keys, n, block, torch.zeros_like(bnd))
+            assert torch.equal(bnd, want)
+            assert torch.equal(ids.cpu(), R.select(q.cpu(), want.cpu(), n, 5, block, 1, 2))
+            o, tol, _, _ = R.block_attention(q, keys, values, ids, n, block)
+            R.close(out, o, tol)
+
+
+def test_refusals():
+    from pariskv_b200 import ops
+    r = rnd(6)
+    keys, values, q, lengths = r(2, 2, 64, 128), r(2, 2, 64, 128), r(2, 1, 4, 128), i32([64, 3])
+    bnd = ops.block_bounds(keys, lengths, block=16)
+    ids = ops.select_blocks(q, bnd, lengths, 2, block=16)
+    bad = (RuntimeError, TypeError, ValueError)
+    for call in (lambda: ops.block_bounds(keys, lengths, block=24), lambda: ops.block_bounds(keys, lengths, block=0), lambda: ops.block_bounds(keys.float(), lengths),
+                 lambda: ops.block_bounds(keys, lengths, n_new=1), lambda: ops.block_bounds(keys, lengths, n_new=-1, bounds=bnd),
+                 lambda: ops.block_bounds(keys, lengths, block=32, bounds=bnd), lambda: ops.block_bounds(keys, lengths[:1]), lambda: ops.block_bounds(keys[..., :64], lengths),
+                 lambda: ops.block_bounds(keys.cpu(), lengths),
+                 lambda: ops.select_blocks(q, bnd, lengths, 2, block=16, sink_blocks=2), lambda: ops.select_blocks(q, bnd, lengths, 2, block=16, local_blocks=0),
+                 lambda: ops.select_blocks(q, bnd, lengths, 0, block=16), lambda: ops.select_blocks(q[:, :, :3], bnd, lengths, 2, block=16),
+                 lambda: ops.select_blocks(q, bnd[:, :, :, :1], lengths, 2, block=16), lambda: ops.select_blocks(q, bnd, lengths.long(), 2, block=16),
+                 lambda: ops.block_attention(q, keys, values, ids.long(), lengths, block=16), lambda: ops.block_attention(q, keys, values, ids[:, :, :1], lengths, block=16),
+                 lambda: ops.block_attention(q, keys, values, ids, lengths, block=48), lambda: ops.block_attention(q, keys, values[:, :1], ids, lengths, block=16),
+                 lambda: ops.block_attention(q, keys, values, ids, None, block=16), lambda: ops.block_attention(q[..., ::2], keys, values, ids, lengths, block=16)):
+        with pytest.raises(bad):
+            call()
