@@ -1,0 +1,20 @@
+// Attention over listed blocks of the cache.
+#include "attend.cuh"
+
+using namespace pk;
+
+extern "C" int64_t pk_block_attention_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) { return 256; }
+
+extern "C" int pk_block_attention(const pk_tensor* queries, const pk_tensor* keys, const pk_tensor* values, const pk_tensor* blocks,
+                                  const pk_tensor* lengths, int64_t block, float scale, const pk_tensor* out, const pk_tensor* lse,
+                                  void*, int64_t, void* stream) {
+  AttendParams p = {};
+  if (const int rc = fill_attend(&p, queries, keys, values, lengths, scale, out, lse)) return rc;
+  PK_CHECK_TENSOR(blocks, PK_I32, 4);
+  const int64_t bs = queries->shape[0];
+  PK_REQUIRE(block == 16 || block == 32 || block == 64 || block == 128, "block must be 16, 32, 64 or 128");
+  PK_REQUIRE(blocks->shape[0] == bs && blocks->shape[1] == p.T && blocks->shape[2] == p.H && is_contig(blocks), "blocks must be contiguous i32 [bs,T,H,n]");
+  PK_REQUIRE(blocks->shape[3] * block <= (1 << 24), "too many blocks");
+  p.blocks = (const int32_t*)blocks->data, p.n = (int)blocks->shape[3], p.block = (int)block;
+  return launch_attend_rows(p, bs, "block_attention", (cudaStream_t)stream);
+}

@@ -4,7 +4,7 @@
 //               block;  with P_d = sum_g max(q_gd, 0) and N_d = sum_g min(q_gd, 0) it is sum_d P_d hi_jd + N_d lo_jd: one pass over the
 //               bounds whatever the number of query heads.
 // Sums in 64 bits, rounded once to 32: the choice does not depend on their order.
-#include "common.cuh"
+#include "attend.cuh"
 
 namespace pk {
 namespace {
@@ -139,13 +139,6 @@ __global__ void __launch_bounds__(256) block_pick_kernel(SelectParams p) {
   }
 }
 
-inline bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
-bool row_tensor(const pk_tensor* x) {
-  if (x->stride[x->ndim - 1] != 1 || !aligned16(x->data)) return false;
-  for (int i = 0; i + 1 < x->ndim; i++)
-    if (x->shape[i] > 1 && (x->stride[i] % 8 || x->stride[i] < 0)) return false;
-  return true;
-}
 int check_bounds(const pk_tensor* bounds) {
   PK_CHECK_TENSOR(bounds, PK_BF16, 5);
   PK_REQUIRE(bounds->shape[3] == 2 && bounds->shape[4] == 128, "bounds must be bf16 [bs,H,blocks,2,128]");

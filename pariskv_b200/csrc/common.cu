@@ -7,6 +7,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "tma.cuh"
 
 namespace pk {
 static thread_local char g_err[512] = "";
@@ -102,6 +103,17 @@ int sm_count() {
     cached[dev] = n;
   }
   return cached[dev];
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> found{nullptr};
+  if (const auto fn = found.load(std::memory_order_relaxed)) return fn;
+  void* f = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+    return cudaGetLastError(), nullptr;
+  found.store((PFN_cuTensorMapEncodeTiled_v12000)f, std::memory_order_relaxed);
+  return (PFN_cuTensorMapEncodeTiled_v12000)f;
 }
 }  // namespace pk
 

@@ -1,129 +1,590 @@
-// Attention of the drafted tokens of a sequence - a tree, given by a mask - over the cache and over the drafts themselves, and
-// attention over listed blocks of the cache.  o = sum_j p_j v_j / sum_j p_j, p_j = 2^(s_j - max s), s_j = scale * log2(e) * q.k_j,
-// over the rows that the query sees; a query that sees none gets zeros.
-#include "common.cuh"
+// Attention of the drafted tokens of a sequence - a tree, given by a mask - over the cache and over the drafts themselves.
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(s_j - max s),  s_j = scale * log2(e) * q.k_j
+// over the rows j that the query sees; a query that sees none gets zeros.
+//
+// The T tokens and G query heads of a KV head are the T * G rows of one product with the same keys, so that the cache is read once
+// for all of them.  Tiles of 128 keys: S = Q K^T and O += P V run on tcgen05 with 128 query rows each, S, P and O in tensor memory,
+// K and V by TMA into a ring of 32 KB stages.  A block is two streams of four softmax warps (a thread per query row):
+//   NT = 2   (more than 128 rows)  a stream per 128 query rows, both over every tile: K and V are read once for 256 rows
+//   NT = 1   both streams have the same rows, one takes the even tiles and the other the odd ones
+// so that while one stream's scores become probabilities the tensor cores work for the other.
+// The tiles of all (sample, KV head, row group) items, laid end to end, are cut into equal ranges, one per SM; the lengths come from
+// device memory, every block finds its range by itself.  Items that are cut leave partial (m, l, O) records, which tree_merge_kernel joins
+// in a fixed order.
+#include "attend.cuh"
+#include "tma.cuh"
 
 namespace pk {
 namespace {
 
-struct AttendParams {
-  const uint16_t* q;
-  int64_t q_b, q_t, q_h;
-  const uint16_t *k, *v;
-  int64_t k_b, k_h, k_l, v_b, v_h, v_l, cap;
-  const uint16_t *dk, *dv;       // drafts
-  int64_t dk_b, dk_t, dk_h, dv_b, dv_t, dv_h;
-  const uint8_t* mask;
-  int64_t m_b, m_t, m_j;
-  const int32_t* blocks;         // [bs][T][H][n], or null: the tree's form
-  int n, block;
-  const int32_t* lengths;
-  int T, H, G;
-  float scale_log2;
-  uint16_t* out;
-  float* lse;
+constexpr int TA_TILE = 128;                   // keys of a tile
+constexpr int TA_THREADS = 320;                // two softmax groups of four warps, a warp for the copies, a warp for the products
+constexpr int TA_STAGE = 32768;                // a tile of K or V: two halves of 64 channels, 128 rows of 128 bytes
+constexpr int TA_WAIT_LIMIT = 4000000;
+constexpr float TA_LAZY = 8.0f;                // log2: the maximum that O is scaled to may lie this far below the true one
+
+template <int NT> struct TaRing { static constexpr int stages = NT == 2 ? 5 : 6; };
+
+struct TreeParams {
+  AttendParams a;
+  int bs;
+  int tile_tokens;     // tokens of 128 query rows: 128 / G
+  int row_groups;      // groups of NT * tile_tokens tokens
+  int draft_tiles;
+  float* records;      // [2 * blocks][rows * 130]: O rows of 128, then m, then l
 };
 
-// A warp per query row; lane L holds dims 4L .. 4L + 3.
-__global__ void __launch_bounds__(128) attend_kernel(AttendParams p, int64_t rows) {
+// Tiles of an item of sample b, and where the items of a sample begin in the sequence of all tiles.
+struct TilePlan {
+  int64_t total;       // tiles of the launch
+  int64_t before;      // tiles of the samples before `sample`
+  int sample;
+};
+__device__ __forceinline__ int tree_len(const TreeParams& p, int b) { return (int)min((int64_t)max(p.a.lengths[b], 0), p.a.cap); }
+__device__ __forceinline__ int tree_tiles(const TreeParams& p, int len) { return (len + TA_TILE - 1) / TA_TILE + p.draft_tiles; }
+// By one warp: the total, and the sample that holds tile `at(total)`.
+template <typename At>
+__device__ __forceinline__ TilePlan tile_plan(const TreeParams& p, At at) {
+  const int lane = threadIdx.x & 31;
+  const int64_t items = (int64_t)p.a.H * p.row_groups;
+  int64_t total = 0;
+  for (int b0 = 0; b0 < p.bs; b0 += 32) {
+    int n = b0 + lane < p.bs ? tree_tiles(p, tree_len(p, b0 + lane)) : 0;
+    total += items * __reduce_add_sync(0xffffffffu, n);
+  }
+  const int64_t t = at(total);
+  TilePlan r = {total, 0, 0};
+  for (int b0 = 0; b0 < p.bs; b0 += 32) {
+    const int64_t mine = b0 + lane < p.bs ? items * tree_tiles(p, tree_len(p, b0 + lane)) : 0;
+    int64_t end = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, end, off);
+      if (lane >= off) end += o;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, b0 + lane < p.bs && r.before + end > t);
+    if (past) {
+      const int i = __ffs(past) - 1;
+      r.sample = b0 + i;
+      r.before += __shfl_sync(0xffffffffu, end - mine, i);
+      return r;
+    }
+    r.before += __shfl_sync(0xffffffffu, end, 31);
+  }
+  return r;
+}
+
+// A block's way through its range: segments of consecutive tiles of one item.
+struct Cursor {
+  int b, h, group, len, n, tile;   // n tiles in the item, `tile` the next
+  int64_t left;                    // tiles of the range that are left
+  __device__ __forceinline__ int count() const { return (int)min((int64_t)(n - tile), left); }
+  __device__ __forceinline__ void next(const TreeParams& p) {
+    left -= count();
+    tile = 0;
+    if (++group == p.row_groups) {
+      group = 0;
+      if (++h == p.a.H) {
+        h = 0;
+        if (++b < p.bs) len = tree_len(p, b), n = tree_tiles(p, len);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ float ex2(float x) {   // 2^x, results below 2^-126 are zero
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// (a + c) f, (b + c) f: two fp32 operations in one instruction
+__device__ __forceinline__ void add_mul2(float& a, float& b, float c, float f) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 y, {%3, %3};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(f));
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {   // the values are there behind it, and no use of them moves before it
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ bool not_finite(uint32_t bf16) { return (bf16 & 0x7f80u) == 0x7f80u; }
+
+template <int NT>
+__global__ void __launch_bounds__(TA_THREADS, 1)
+    tree_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dk,
+                     const __grid_constant__ CUtensorMap map_dv, const __grid_constant__ TreeParams p) {
+  constexpr int NS = TaRing<NT>::stages;
+  extern __shared__ unsigned char dyn[];
+  __shared__ __align__(8) unsigned long long bars[2 * NS + 8];
+  __shared__ unsigned s_tmem, s_bad[8];
+  __shared__ volatile int s_dead;
+  __shared__ TilePlan s_plan;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const unsigned base = (smem_addr(dyn) + 1023) & ~1023u, q_smem = base, ring = base + NT * TA_STAGE;
+  const unsigned full = smem_addr(bars), empty = full + 8 * NS, s_full = empty + 8 * NS, p_full = s_full + 16, o_done = p_full + 16, q_full = o_done + 16, ending = q_full + 8;
+  if (tid == 0) {
+    for (int i = 0; i < NS; i++) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
+    for (int i = 0; i < 2; i++) mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, 128), mbar_init(o_done + 8 * i, 1);
+    mbar_init(q_full, 256), mbar_init(ending, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_dead = 0;
+  }
+  if (tid < 8) s_bad[tid] = 0;
+  if (warp == 8) tmem_alloc(smem_addr(&s_tmem), 512);
+  if (warp == 9 && lane < 4) tma_prefetch_map(lane == 0 ? &map_k : lane == 1 ? &map_v : lane == 2 ? &map_dk : &map_dv);
+  pdl_wait();
+  pdl_trigger();
+  const int blocks = (int)gridDim.x;
+  if (warp == 0) {
+    const TilePlan plan = tile_plan(p, [&](int64_t total) { return total * blockIdx.x / min((int64_t)blocks, total); });
+    if (lane == 0) s_plan = plan;
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const unsigned tmem = s_tmem;
+  const TilePlan plan = s_plan;
+  const int64_t shares = min((int64_t)blocks, plan.total);
+  Cursor cur;
+  {
+    const int64_t first = blockIdx.x < shares ? plan.total * blockIdx.x / shares : plan.total, end = blockIdx.x < shares ? plan.total * (blockIdx.x + 1) / shares : first;
+    cur.left = end - first, cur.b = plan.sample, cur.len = tree_len(p, plan.sample), cur.n = tree_tiles(p, cur.len);
+    const int64_t at = first - plan.before;
+    const int item = (int)(at / cur.n);
+    cur.tile = (int)(at % cur.n), cur.h = item / p.row_groups, cur.group = item % p.row_groups;
+  }
+  // Every wait has a limit.  Where one runs out the block stops waiting altogether, its copies land, its tensor memory is freed and its
+  // rows come out as NaN.
+  bool dead = false;
+  auto wait = [&](unsigned mb, unsigned parity) {
+    for (int it = 0; !dead; it++) {
+      if (mbar_try(mb, parity)) break;
+      if (it >= TA_WAIT_LIMIT || ((it & 1023) == 1023 && s_dead)) dead = true, s_dead = 1;
+    }
+  };
+
+  if (warp == 8) {
+    // ---- copies: K and V of every tile in turn ----
+    if (lane == 0) {
+      unsigned q = 0;
+      for (; cur.left > 0 && !dead; cur.next(p)) {
+        const int n = cur.count(), cache_tiles = cur.n - p.draft_tiles;
+        for (int j = 0; j < n && !dead; j++) {
+          const int t = cur.tile + j;
+          const bool draft = t >= cache_tiles;
+          const int row = (draft ? t - cache_tiles : t) * TA_TILE;
+          for (int v = 0; v < 2; v++, q++) {
+            const unsigned st = q % NS;
+            if (q >= NS) wait(empty + 8 * st, (q / NS - 1) & 1);
+            if (dead) break;
+            const CUtensorMap* map = draft ? (v ? &map_dv : &map_dk) : (v ? &map_v : &map_k);
+            mbar_expect(full + 8 * st, TA_STAGE);
+            tma_load4(ring + st * TA_STAGE, map, 0, row, cur.h, cur.b, full + 8 * st);
+            tma_load4(ring + st * TA_STAGE + TA_STAGE / 2, map, 64, row, cur.h, cur.b, full + 8 * st);
+          }
+        }
+      }
+      if (dead || s_dead)   // what is under way has to land before the block ends
+        for (unsigned i = q < NS ? 0 : q - NS; i < q; i++)
+          for (int it = 0; it < TA_WAIT_LIMIT && !mbar_try(full + 8 * (i % NS), (i / NS) & 1); it++) {}
+    }
+  } else if (warp == 9) {
+    // ---- products ----
+    if (lane == 0) {
+      constexpr unsigned ID_S = umma_idesc(128, 128, false), ID_O = umma_idesc(128, 128, true);
+      auto scores = [&](int s, unsigned kq) {   // S_s = Q K^T, K in stage kq
+        const unsigned a = q_smem + (NT == 2 ? s * TA_STAGE : 0), b = ring + kq * TA_STAGE;
+        if (dead) return;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const unsigned off = (k >> 2) * (TA_STAGE / 2) + (k & 3) * 32;
+          tc_mma_ss(tmem + 128 * s, umma_desc(a + off, 16), umma_desc(b + off, 16), ID_S, k > 0);
+        }
+        tc_commit(s_full + 8 * s);
+      };
+      auto values = [&](int s, unsigned vq, bool add) {   // O_s (+)= P_s V
+        const unsigned b = ring + vq * TA_STAGE;
+        if (dead) return;
+#pragma unroll
+        for (int k = 0; k < 8; k++) tc_mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + 8 * k, umma_desc(b + k * 2048, TA_STAGE / 2), ID_O, add || k > 0);
+      };
+      auto free_stage = [&](unsigned st) { if (!dead) tc_commit(empty + 8 * st); };
+      auto arrived = [&](unsigned q) {
+        wait(full + 8 * (q % NS), (q / NS) & 1);
+        tc_after();
+      };
+      unsigned q0 = 0, seg = 0, n_p[2] = {0, 0};   // q0: number of the segment's first copy
+      auto probabilities = [&](int s) {
+        wait(p_full + 8 * s, n_p[s]++ & 1);
+        tc_after();
+      };
+      for (; cur.left > 0; cur.next(p), seg++) {
+        const int n = cur.count();
+        wait(q_full, seg & 1);
+        tc_after();
+        arrived(q0);
+        scores(0, q0 % NS);
+        if (NT == 2) {
+          scores(1, q0 % NS);
+          free_stage(q0 % NS);
+        } else {
+          free_stage(q0 % NS);
+          if (n > 1) {
+            arrived(q0 + 2);
+            scores(1, (q0 + 2) % NS);
+            free_stage((q0 + 2) % NS);
+          }
+        }
+        for (int j = 0; j < n; j++) {
+          const unsigned v = q0 + 2 * j + 1, k_next = q0 + 2 * (j + (NT == 2 ? 1 : 2));
+          const bool more = j + (NT == 2 ? 1 : 2) < n;
+          arrived(v);
+#pragma unroll
+          for (int i = 0; i < NT; i++) {
+            const int s = NT == 2 ? i : j & 1;
+            probabilities(s);
+            values(s, v % NS, NT == 2 ? j > 0 : j > 1);
+            if (i == NT - 1) free_stage(v % NS);
+            if (more) {
+              if (i == 0) arrived(k_next);
+              scores(s, k_next % NS);
+              if (i == NT - 1) free_stage(k_next % NS);
+            } else if (!dead) {
+              tc_commit(o_done + 8 * s);
+            }
+          }
+        }
+        q0 += 2 * n;
+      }
+    }
+  } else {
+    // ---- softmax: stream `s`, a thread per query row ----
+    const int s = warp >> 2, r = tid & 127;
+    const unsigned lanes = tmem + ((unsigned)(warp & 3) << 21), s_cols = lanes + 128 * s, o_cols = lanes + 256;
+    const int Hq = p.a.H * p.a.G, tl = r / p.a.G, g = r % p.a.G;
+    const float scale = p.a.scale_log2;
+    unsigned q0 = 0, n_s = 0, n_o[2] = {0, 0};
+    for (; cur.left > 0; cur.next(p)) {
+      const int n = cur.count(), cache_tiles = cur.n - p.draft_tiles;
+      const int token0 = (NT == 2 ? 2 * cur.group + s : cur.group) * p.tile_tokens, t = token0 + tl;
+      const bool row_ok = tl < p.tile_tokens && t < p.a.T;
+      const bool warp_ok = __any_sync(0xffffffffu, row_ok);
+      {  // this thread's row of Q (NT = 1: this stream's half of it), swizzled as the copies of K are
+        const uint16_t* src = p.a.q + cur.b * p.a.q_b + (int64_t)t * p.a.q_t + (int64_t)(cur.h * p.a.G + g) * p.a.q_h;
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          if (NT == 1 && half != s) continue;
+          const unsigned dst = q_smem + (NT == 2 ? s * TA_STAGE : 0) + half * (TA_STAGE / 2) + r * 128;
+          uint4 x[8];
+#pragma unroll
+          for (int c = 0; c < 8; c++) x[c] = row_ok ? *reinterpret_cast<const uint4*>(src + half * 64 + 8 * c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int c = 0; c < 8; c++)
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + ((c ^ (r & 7)) << 4)), "r"(x[c].x), "r"(x[c].y), "r"(x[c].z), "r"(x[c].w) : "memory");
+        }
+        fence_async();
+        mbar_arrive1(q_full);
+      }
+      float m = -INFINITY, l = 0.0f;   // m: raw scores
+      for (int j = NT == 2 ? 0 : s; j < n; j += NT == 2 ? 1 : 2) {
+        const int tile = cur.tile + j, dt = tile - cache_tiles;
+        const int live = dt >= 0 ? TA_TILE : cur.len - tile * TA_TILE;
+        uint32_t w[4] = {~0u, ~0u, ~0u, ~0u};
+        if (dt >= 0) {
+          const int t_first = token0 + (32 * (warp & 3)) / p.a.G, t_last = min(token0 + (32 * (warp & 3) + 31) / p.a.G, p.a.T - 1);
+          const uint8_t* mask = p.a.mask + cur.b * p.a.m_b;
+          w[0] = w[1] = w[2] = w[3] = 0;
+          for (int tt = t_first; tt <= t_last; tt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const int d = dt * TA_TILE + 32 * i + lane;
+              const unsigned bits = __ballot_sync(0xffffffffu, d < p.a.T && mask[tt * p.a.m_t + d * p.a.m_j] != 0);
+              if (tt == t) w[i] = bits;
+            }
+        } else if (live < TA_TILE) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) w[i] = live >= 32 * i + 32 ? ~0u : live <= 32 * i ? 0u : (1u << (live - 32 * i)) - 1;
+        }
+        const bool masked = dt >= 0 || live < TA_TILE;
+        wait(s_full + 8 * s, n_s & 1);
+        n_s++;
+        __syncwarp();
+        tc_after();
+        if (warp_ok) {
+          uint32_t x[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; c++) tmem_ld32(x[c], s_cols + 32 * c);
+#pragma unroll
+          for (int c = 0; c < 4; c++) wait_ld(x[c]);
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+              for (int i = 0; i < 32; i++) x[c][i] = w[c] >> i & 1 ? x[c][i] : 0xff800000u;
+          }
+          float mx[4] = {m, m, m, m};
+#pragma unroll
+          for (int i = 0; i < 32; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) mx[c] = fmaxf(mx[c], __uint_as_float(x[c][i]));
+          const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          if (j < 2 - (NT == 2)) {   // the stream's first tile: nothing to scale
+            m = m_new;
+          } else {
+            const bool grow = (m_new - m) * scale > TA_LAZY;
+            if (__any_sync(0xffffffffu, grow)) {
+              const float f = grow ? ex2((m - m_new) * scale) : 1.0f;
+              if (grow) m = m_new;
+              l *= f;
+              // the products of the tile before have ended: their commit came before that of these scores
+#pragma unroll
+              for (int c = 0; c < 4; c++) {
+                uint32_t o[32];
+                tmem_ld32(o, o_cols + 128 * s + 32 * c);
+                wait_ld(o);
+#pragma unroll
+                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st32(o_cols + 128 * s + 32 * c, o);
+              }
+            }
+          }
+          const float least = m == -INFINITY ? 0.0f : -m;   // (x - m) scale, not x scale - m scale: the difference of close scores is exact
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            uint32_t pr[32];
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+              const int at = 64 * half + 2 * i;
+              float a = __uint_as_float(x[at >> 5][at & 31]), b = __uint_as_float(x[at >> 5][(at & 31) + 1]);
+              add_mul2(a, b, least, scale);
+              a = ex2(a), b = ex2(b);
+              sum[i & 1] += a, sum[2 + (i & 1)] += b;
+              pr[i] = pack2(a, b);   // 8 bits of each weight: a tcgen05 product of bf16 values takes bf16 weights; the sum has them all
+            }
+            tmem_st32(s_cols + 32 * half, pr);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_wait_st();
+        }
+        if (masked) {
+          // rows of V that no query sees must be zero, what is not a number in a draft's row must not reach the queries that do not see
+          // it: a weight of zero would not keep it out of the product.  Thread r: row r.
+          const unsigned vq = q0 + 2 * j + 1, row = ring + (vq % NS) * TA_STAGE + r * 128;
+          wait(full + 8 * (vq % NS), (vq / NS) & 1);
+          if (dt < 0) {
+            if (r >= live)
+#pragma unroll
+              for (int c = 0; c < 16; c++)
+                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(row + (c >> 3) * (TA_STAGE / 2) + (c & 7) * 16), "r"(0) : "memory");
+          } else {
+            bool bad = false;
+#pragma unroll 4
+            for (int c = 0; c < 16; c++) {
+              const unsigned at = row + (c >> 3) * (TA_STAGE / 2) + (c & 7) * 16;
+              uint32_t v[4];
+              asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+              bool here = false;
+#pragma unroll
+              for (int i = 0; i < 4; i++) here |= not_finite(v[i]) | not_finite(v[i] >> 16);
+              if (here) {
+                if (!bad) atomicOr(&s_bad[4 * dt + (r >> 5)], 1u << (r & 31)), __threadfence_block();
+                bad = true;
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] = (not_finite(v[i]) ? 0 : v[i] & 0xffffu) | (not_finite(v[i] >> 16) ? 0 : v[i] & 0xffff0000u);
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+              }
+            }
+          }
+          fence_async();
+        }
+        tc_before();
+        mbar_arrive1(p_full + 8 * s);
+      }
+      // ---- the segment's result ----
+      const bool whole = cur.tile == 0 && n == cur.n;
+      const int64_t out_row = ((int64_t)cur.b * p.a.T + t) * Hq + cur.h * p.a.G + g;
+      float* rec = nullptr;
+      constexpr int ROWS = NT * 128;
+      const int rec_row = NT == 2 ? s * 128 + r : r;
+      if (!whole) rec = p.records + (2 * (int64_t)blockIdx.x + (cur.tile == 0)) * (ROWS * 130);
+      const bool two = NT == 1 && n > 1;   // both streams have tiles of this segment
+      float f[2] = {1.0f, 1.0f}, M = m == -INFINITY ? -INFINITY : m * scale, L = l;
+      wait(o_done + 8 * (NT == 2 ? s : 0), n_o[0]++ & 1);
+      if (two) wait(o_done + 8, n_o[1]++ & 1);
+      __syncwarp();
+      tc_after();
+      if (NT == 1) {   // both streams' maxima and sums, through the room of Q
+        const unsigned at = q_smem + r * 8;
+        asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at + s * 1024), "f"(M), "f"(L) : "memory");
+        named_barrier(1, 256);
+        float m2[2], l2[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=f"(m2[i]), "=f"(l2[i]) : "r"(at + i * 1024) : "memory");
+        M = fmaxf(m2[0], m2[1]);
+#pragma unroll
+        for (int i = 0; i < 2; i++) f[i] = m2[i] == -INFINITY ? 0.0f : ex2(m2[i] - M);
+        L = l2[0] * f[0] + l2[1] * f[1];   // (of a stream without tiles: m = -inf, l = 0)
+      }
+      if (dead) L = NAN;
+      if (warp_ok) {
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          if (NT == 1 && (c >> 1) != s) continue;   // a half of the channels each
+          uint32_t o[32];
+          tmem_ld32(o, o_cols + (NT == 2 ? 128 * s : 0) + 32 * c);
+          wait_ld(o);
+          if (two) {
+            uint32_t o1[32];
+            tmem_ld32(o1, o_cols + 128 + 32 * c);
+            wait_ld(o1);
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f[0] + __uint_as_float(o1[i]) * f[1]);
+          }
+          // what was taken out of the drafts' rows, back to the queries that see it
+          if (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3] | s_bad[4] | s_bad[5] | s_bad[6] | s_bad[7]) {
+            const int d_first = max(cur.tile - cache_tiles, 0) * TA_TILE, d_end = min(p.a.T, (cur.tile + n - cache_tiles) * TA_TILE);
+            const uint8_t* mask = p.a.mask + cur.b * p.a.m_b + (int64_t)(row_ok ? t : 0) * p.a.m_t;
+            for (int d = d_first; d < d_end; d++)
+              if (row_ok && mask[d * p.a.m_j]) {
+                const uint16_t* v = p.a.dv + cur.b * p.a.dv_b + (int64_t)d * p.a.dv_t + cur.h * p.a.dv_h + 32 * c;
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+                  if (not_finite(v[i])) o[i] = __float_as_uint(__uint_as_float(o[i]) + bf2f(v[i]));
+              }
+          }
+          if (row_ok) {
+            if (whole) {
+              uint4* dst = reinterpret_cast<uint4*>(p.a.out + out_row * 128 + 32 * c);
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                uint32_t y[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = pack2(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+                dst[i] = make_uint4(y[0], y[1], y[2], y[3]);
+              }
+            } else {
+              uint4* dst = reinterpret_cast<uint4*>(rec + (int64_t)rec_row * 128 + 32 * c);
+#pragma unroll
+              for (int i = 0; i < 8; i++) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
+          }
+        }
+        if (row_ok && (NT == 2 || s == 0)) {
+          if (whole) {
+            if (p.a.lse) p.a.lse[out_row] = L == 0.0f ? -INFINITY : M + log2f(L);
+          } else {
+            rec[ROWS * 128 + rec_row] = M, rec[ROWS * 129 + rec_row] = L;
+          }
+        }
+      }
+      tc_before();
+      named_barrier(2, 256);   // both streams have read: the room of Q, O and the marks may be written
+      if (tid < 8) s_bad[tid] = 0;
+      q0 += 2 * n;
+    }
+  }
+  __syncwarp();
+  tc_before();
+  __syncthreads();
+  tc_after();
+  if (warp == 9 && lane == 0 && s_dead) {   // products under way end before the tensor memory goes
+    tc_commit(ending);
+    for (int it = 0; it < TA_WAIT_LIMIT && !mbar_try(ending, 0); it++) {}
+  }
+  __syncthreads();
+  if (warp == 8) tmem_free(tmem, 512);
+}
+
+// A warp per query row: the records of the blocks that share its item, in the order of the tiles.
+template <int NT>
+__global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__ TreeParams p, int blocks, int64_t rows) {
   pdl_wait();
   pdl_trigger();
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= rows) return;
-  const int lane = threadIdx.x & 31, Hq = p.H * p.G;
-  const int hq = (int)(row % Hq), t = (int)(row / Hq % p.T), h = hq / p.G;
-  const int64_t b = row / Hq / p.T;
-  auto four = [&](const uint16_t* x, float* f) {
-    const uint2 r = *reinterpret_cast<const uint2*>(x + 4 * lane);
-    f[0] = __uint_as_float(r.x << 16), f[1] = __uint_as_float(r.x & 0xffff0000u), f[2] = __uint_as_float(r.y << 16), f[3] = __uint_as_float(r.y & 0xffff0000u);
-  };
-  float q[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
-  four(p.q + b * p.q_b + t * p.q_t + hq * p.q_h, q);
-  auto see = [&](const uint16_t* k, const uint16_t* v) {
-    float kf[4], vf[4];
-    four(k, kf), four(v, vf);
-    float s = q[0] * kf[0] + q[1] * kf[1] + q[2] * kf[2] + q[3] * kf[3];
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    s *= p.scale_log2;
-    const float M = fmaxf(m, s), f = m == -INFINITY ? 0.0f : exp2f(m - M), w = M == -INFINITY ? 0.0f : exp2f(s - M);
-    l = l * f + w, m = M;
-#pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = o[i] * f + w * vf[i];
-  };
-  const int64_t len = min((int64_t)max(p.lengths[b], 0), p.cap);
-  const uint16_t *kb = p.k + b * p.k_b + h * p.k_h, *vb = p.v + b * p.v_b + h * p.v_h;
-  if (p.blocks) {
-    const int64_t end = len - p.T + t + 1;
-    const int32_t* ids = p.blocks + ((b * p.T + t) * p.H + h) * p.n;
-    for (int i = 0; i < p.n; i++) {
-      if (ids[i] < 0) continue;
-      const int64_t first = (int64_t)ids[i] * p.block, stop = min(first + p.block, end);
-      for (int64_t j = first; j < stop; j++) see(kb + j * p.k_l, vb + j * p.v_l);
-    }
-  } else {
-    for (int64_t j = 0; j < len; j++) see(kb + j * p.k_l, vb + j * p.v_l);
-    for (int j = 0; j < p.T; j++)
-      if (p.mask[b * p.m_b + t * p.m_t + j * p.m_j])
-        see(p.dk + b * p.dk_b + j * p.dk_t + h * p.dk_h, p.dv + b * p.dv_b + j * p.dv_t + h * p.dv_h);
+  const int lane = threadIdx.x & 31, Hq = p.a.H * p.a.G, hq = (int)(row % Hq), h = hq / p.a.G, g = hq % p.a.G;
+  const int b = (int)(row / Hq / p.a.T), t = (int)(row / Hq % p.a.T), mt = t / p.tile_tokens, group = mt / NT;
+  const int r = (mt % NT) * 128 + (t - mt * p.tile_tokens) * p.a.G + g;
+  const int64_t items = (int64_t)p.a.H * p.row_groups;
+  int64_t total = 0, before = 0;
+  for (int b0 = 0; b0 < p.bs; b0 += 32) {
+    const int n = b0 + lane < p.bs ? tree_tiles(p, tree_len(p, b0 + lane)) : 0;
+    total += items * __reduce_add_sync(0xffffffffu, n), before += items * __reduce_add_sync(0xffffffffu, b0 + lane < b ? n : 0);
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint2 w;
-  w.x = f2bf(o[0] * inv) | (uint32_t)f2bf(o[1] * inv) << 16;
-  w.y = f2bf(o[2] * inv) | (uint32_t)f2bf(o[3] * inv) << 16;
-  *reinterpret_cast<uint2*>(p.out + row * 128 + 4 * lane) = w;
-  if (p.lse && lane == 0) p.lse[row] = l == 0.0f ? -INFINITY : m + log2f(l);
-}
-
-inline bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
-// rows of 128 bf16 that 16-byte copies can read: unit inner stride, the other strides a multiple of 8
-bool row_tensor(const pk_tensor* x) {
-  if (x->stride[x->ndim - 1] != 1 || !aligned16(x->data)) return false;
-  for (int i = 0; i + 1 < x->ndim; i++)
-    if (x->shape[i] > 1 && (x->stride[i] % 8 || x->stride[i] < 0)) return false;
-  return true;
-}
-
-// What both entry points share: queries, cache, lengths, output.
-int fill_attend(AttendParams* p, const pk_tensor* queries, const pk_tensor* keys, const pk_tensor* values, const pk_tensor* lengths,
-                float scale, const pk_tensor* out, const pk_tensor* lse) {
-  PK_CHECK_TENSOR(queries, PK_BF16, 4);
-  PK_CHECK_TENSOR(keys, PK_BF16, 4);
-  PK_CHECK_TENSOR(values, PK_BF16, 4);
-  PK_CHECK_TENSOR(lengths, PK_I32, 1);
-  PK_CHECK_TENSOR(out, PK_BF16, 4);
-  const int64_t bs = queries->shape[0], T = queries->shape[1], Hq = queries->shape[2], H = keys->shape[1];
-  PK_REQUIRE(queries->shape[3] == 128, "queries must be bf16 [bs,T,Hq,128]");
-  PK_REQUIRE(keys->shape[0] == bs && keys->shape[3] == 128 && keys->shape[2] < (1LL << 31), "keys must be bf16 [bs,H,cap,128]");
-  for (int i = 0; i < 4; i++) PK_REQUIRE(values->shape[i] == keys->shape[i], "values must have the shape of keys");
-  PK_REQUIRE(H >= 1 && Hq % H == 0 && Hq >= H && Hq / H <= 128, "the query heads must be a multiple of the KV heads, at most 128 of them each");
-  PK_REQUIRE(row_tensor(queries) && row_tensor(keys) && row_tensor(values),
-             "queries, keys and values need a unit inner stride, other strides that are multiples of 8, and 16-byte alignment");
-  PK_REQUIRE(lengths->shape[0] == bs && is_contig(lengths), "lengths must be contiguous i32 [bs]");
-  for (int i = 0; i < 4; i++) PK_REQUIRE(out->shape[i] == queries->shape[i], "out must have the shape of queries");
-  PK_REQUIRE(is_contig(out) && aligned16(out->data), "out must be contiguous and 16-byte aligned");
-  if (lse) {
-    PK_CHECK_TENSOR(lse, PK_F32, 3);
-    PK_REQUIRE(is_contig(lse) && lse->shape[0] == bs && lse->shape[1] == T && lse->shape[2] == Hq, "lse must be contiguous f32 [bs,T,Hq]");
-    p->lse = (float*)lse->data;
+  const int n = tree_tiles(p, tree_len(p, b));
+  const int64_t first = before + ((int64_t)h * p.row_groups + group) * n, last = first + n - 1, shares = min((int64_t)blocks, total);
+  auto owner = [&](int64_t x) { return (int)(((x + 1) * shares - 1) / total); };
+  const int c0 = owner(first), c1 = owner(last);
+  if (c0 == c1) return;   // written by its block
+  constexpr int ROWS = NT * 128;
+  auto record = [&](int c) { return p.records + (2 * (int64_t)c + (c == c0)) * (ROWS * 130); };
+  float M = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, record(c)[ROWS * 128 + r]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  float L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int c = c0; c <= c1; c++) {
+    const float* rec = record(c);
+    const float mc = rec[ROWS * 128 + r], f = mc == -INFINITY ? 0.0f : exp2f(mc - M);
+    const float4 v = *reinterpret_cast<const float4*>(rec + (int64_t)r * 128 + 4 * lane);
+    L += rec[ROWS * 129 + r] * f;
+    o[0] += v.x * f, o[1] += v.y * f, o[2] += v.z * f, o[3] += v.w * f;
   }
-  PK_REQUIRE(bs < 65536 && bs * T * Hq < (1LL << 31), "sizes out of range");
-  p->q = (const uint16_t*)queries->data, p->q_b = queries->stride[0], p->q_t = queries->stride[1], p->q_h = queries->stride[2];
-  p->k = (const uint16_t*)keys->data, p->k_b = keys->stride[0], p->k_h = keys->stride[1], p->k_l = keys->stride[2];
-  p->v = (const uint16_t*)values->data, p->v_b = values->stride[0], p->v_h = values->stride[1], p->v_l = values->stride[2];
-  p->cap = keys->shape[2], p->lengths = (const int32_t*)lengths->data;
-  p->T = (int)T, p->H = (int)H, p->G = (int)(Hq / H);
-  p->scale_log2 = scale * 1.4426950408889634f;
-  p->out = (uint16_t*)out->data;
-  return PK_OK;
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  *reinterpret_cast<uint2*>(p.a.out + row * 128 + 4 * lane) = make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
+  if (p.a.lse && lane == 0) p.a.lse[row] = L == 0.0f ? -INFINITY : M + log2f(L);
 }
 
-int launch_attend(const AttendParams& p, int64_t bs, const char* what, cudaStream_t st) {
-  const int64_t rows = bs * p.T * p.H * p.G;
-  if (rows == 0) return PK_OK;
+// Rows of 128 bf16 in three dimensions, boxes of 64 channels x `box` rows; false where a tensor map cannot have these strides.
+bool rows_map(CUtensorMap* m, const void* base, int64_t d1, int64_t s1, int64_t d2, int64_t s2, int64_t d3, int64_t s3, int box) {
+  const auto encode = tensor_map_encoder();
+  const int64_t d[3] = {d1, d2, d3};
+  int64_t s[3] = {s1, s2, s3};
+  for (int i = 0; i < 3; i++) {
+    if (d[i] == 1) s[i] = 128;
+    if (s[i] <= 0 || s[i] >= (1ll << 38) || d[i] >= (1ll << 31)) return false;
+  }
+  if (!encode) return false;
+  const cuuint64_t dims[4] = {128, (cuuint64_t)d1, (cuuint64_t)d2, (cuuint64_t)d3}, strides[3] = {(cuuint64_t)s[0] * 2, (cuuint64_t)s[1] * 2, (cuuint64_t)s[2] * 2};
+  const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1}, steps[4] = {1, 1, 1, 1};
+  return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int NT>
+int launch_tree(const AttendParams& a, int64_t bs, void* workspace, cudaStream_t st) {
+  CUtensorMap mk, mv, mdk, mdv;
+  if (!rows_map(&mk, a.k, a.cap, a.k_l, a.H, a.k_h, bs, a.k_b, TA_TILE) || !rows_map(&mv, a.v, a.cap, a.v_l, a.H, a.v_h, bs, a.v_b, TA_TILE) ||
+      !rows_map(&mdk, a.dk, a.T, a.dk_t, a.H, a.dk_h, bs, a.dk_b, TA_TILE) || !rows_map(&mdv, a.dv, a.T, a.dv_t, a.H, a.dv_h, bs, a.dv_b, TA_TILE))
+    return launch_attend_rows(a, bs, "tree_attention", st);
+  TreeParams p = {};
+  p.a = a, p.bs = (int)bs, p.tile_tokens = 128 / a.G, p.row_groups = (a.T + NT * p.tile_tokens - 1) / (NT * p.tile_tokens);
+  p.draft_tiles = (a.T + TA_TILE - 1) / TA_TILE, p.records = (float*)workspace;
+  const int64_t most = bs * a.H * p.row_groups * ((a.cap + TA_TILE - 1) / TA_TILE + p.draft_tiles);
+  const int blocks = (int)(most < sm_count() ? most : sm_count());
+  static PerDevice opted;
+  constexpr int SMEM = 1024 + (NT + TaRing<NT>::stages) * TA_STAGE;
+  if (const unsigned long long bit = first_on_device(opted)) {
+    if (cudaFuncSetAttribute(tree_tile_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess)
+      return fail(PK_ERR_CUDA, "tree_attention: %s", cudaGetErrorString(cudaGetLastError()));
+    mark_on_device(opted, bit);
+  }
   StageTimer timer(ST_ATTENTION, st);
-  launch_chain(attend_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p, rows);
-  return check_launch(what);
+  launch_chain(tree_tile_kernel<NT>, dim3((unsigned)blocks), dim3(TA_THREADS), SMEM, st, mk, mv, mdk, mdv, p);
+  const int64_t rows = bs * a.T * a.H * a.G;
+  launch_chain(tree_merge_kernel<NT>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p, blocks, rows);
+  return check_launch("tree_attention", 2);
 }
 
 }  // namespace
@@ -131,11 +592,14 @@ int launch_attend(const AttendParams& p, int64_t bs, const char* what, cudaStrea
 
 using namespace pk;
 
-extern "C" int64_t pk_tree_attention_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t) { return 256; }
+extern "C" int64_t pk_tree_attention_workspace_bytes(int64_t, int64_t T, int64_t Hq, int64_t H, int64_t) {
+  const int64_t rows = H > 0 && T * (Hq / H) > 128 ? 256 : 128;
+  return 2 * (int64_t)sm_count() * rows * 130 * 4;
+}
 
 extern "C" int pk_tree_attention(const pk_tensor* queries, const pk_tensor* keys, const pk_tensor* values, const pk_tensor* draft_keys,
                                  const pk_tensor* draft_values, const pk_tensor* tree_mask, const pk_tensor* lengths, float scale,
-                                 const pk_tensor* out, const pk_tensor* lse, void*, int64_t, void* stream) {
+                                 const pk_tensor* out, const pk_tensor* lse, void* workspace, int64_t workspace_bytes, void* stream) {
   AttendParams p = {};
   if (const int rc = fill_attend(&p, queries, keys, values, lengths, scale, out, lse)) return rc;
   PK_CHECK_TENSOR(draft_keys, PK_BF16, 4);
@@ -152,21 +616,8 @@ extern "C" int pk_tree_attention(const pk_tensor* queries, const pk_tensor* keys
   p.dk = (const uint16_t*)draft_keys->data, p.dk_b = draft_keys->stride[0], p.dk_t = draft_keys->stride[1], p.dk_h = draft_keys->stride[2];
   p.dv = (const uint16_t*)draft_values->data, p.dv_b = draft_values->stride[0], p.dv_t = draft_values->stride[1], p.dv_h = draft_values->stride[2];
   p.mask = (const uint8_t*)tree_mask->data, p.m_b = tree_mask->shape[0] == 1 ? 0 : tree_mask->stride[0], p.m_t = tree_mask->stride[1], p.m_j = tree_mask->stride[2];
-  return launch_attend(p, bs, "tree_attention", (cudaStream_t)stream);
-}
-
-extern "C" int64_t pk_block_attention_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) { return 256; }
-
-extern "C" int pk_block_attention(const pk_tensor* queries, const pk_tensor* keys, const pk_tensor* values, const pk_tensor* blocks,
-                                  const pk_tensor* lengths, int64_t block, float scale, const pk_tensor* out, const pk_tensor* lse,
-                                  void*, int64_t, void* stream) {
-  AttendParams p = {};
-  if (const int rc = fill_attend(&p, queries, keys, values, lengths, scale, out, lse)) return rc;
-  PK_CHECK_TENSOR(blocks, PK_I32, 4);
-  const int64_t bs = queries->shape[0];
-  PK_REQUIRE(block == 16 || block == 32 || block == 64 || block == 128, "block must be 16, 32, 64 or 128");
-  PK_REQUIRE(blocks->shape[0] == bs && blocks->shape[1] == p.T && blocks->shape[2] == p.H && is_contig(blocks), "blocks must be contiguous i32 [bs,T,H,n]");
-  PK_REQUIRE(blocks->shape[3] * block <= (1 << 24), "too many blocks");
-  p.blocks = (const int32_t*)blocks->data, p.n = (int)blocks->shape[3], p.block = (int)block;
-  return launch_attend(p, bs, "block_attention", (cudaStream_t)stream);
+  if (bs == 0 || p.T == 0) return PK_OK;
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < pk_tree_attention_workspace_bytes(bs, p.T, queries->shape[2], p.H, p.cap))
+    return fail(PK_ERR_WORKSPACE, "tree_attention: workspace missing, misaligned or too small");
+  return p.T * p.G > 128 ? launch_tree<2>(p, bs, workspace, (cudaStream_t)stream) : launch_tree<1>(p, bs, workspace, (cudaStream_t)stream);
 }
