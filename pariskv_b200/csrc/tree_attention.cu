@@ -103,6 +103,11 @@ __device__ __forceinline__ void add_mul2(float& a, float& b, float c, float f) {
       : "+f"(a), "+f"(b)
       : "f"(c), "f"(f));
 }
+__device__ __forceinline__ void add2(float& a, float& b, float c, float d) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d));
+}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -293,22 +298,32 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         fence_async();
         mbar_arrive1(q_full);
       }
+      // which drafts of draft tile dt this row sees: a token's bytes by 32 lanes at a time
+      auto drafts_seen = [&](int dt, uint32_t (&w)[4]) {
+        const int t_first = token0 + (32 * (warp & 3)) / p.a.G, t_last = min(token0 + (32 * (warp & 3) + 31) / p.a.G, p.a.T - 1);
+        const uint8_t* mask = p.a.mask + cur.b * p.a.m_b;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int d = dt * TA_TILE + 32 * i + lane;
+          w[i] = 0;
+          if (dt * TA_TILE + 32 * i < p.a.T)
+#pragma unroll 4
+            for (int tt = t_first; tt <= t_last; tt++) {
+              const unsigned bits = __ballot_sync(0xffffffffu, d < p.a.T && mask[tt * p.a.m_t + d * p.a.m_j] != 0);
+              if (tt == t) w[i] = bits;
+            }
+        }
+      };
+      uint32_t drafts[4] = {};
+      if (cur.tile + n > cache_tiles && cur.tile <= cache_tiles) drafts_seen(0, drafts);
       float m = -INFINITY, l = 0.0f;   // m: raw scores
       for (int j = NT == 2 ? 0 : s; j < n; j += NT == 2 ? 1 : 2) {
         const int tile = cur.tile + j, dt = tile - cache_tiles;
         const int live = dt >= 0 ? TA_TILE : cur.len - tile * TA_TILE;
         uint32_t w[4] = {~0u, ~0u, ~0u, ~0u};
         if (dt >= 0) {
-          const int t_first = token0 + (32 * (warp & 3)) / p.a.G, t_last = min(token0 + (32 * (warp & 3) + 31) / p.a.G, p.a.T - 1);
-          const uint8_t* mask = p.a.mask + cur.b * p.a.m_b;
-          w[0] = w[1] = w[2] = w[3] = 0;
-          for (int tt = t_first; tt <= t_last; tt++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const int d = dt * TA_TILE + 32 * i + lane;
-              const unsigned bits = __ballot_sync(0xffffffffu, d < p.a.T && mask[tt * p.a.m_t + d * p.a.m_j] != 0);
-              if (tt == t) w[i] = bits;
-            }
+          if (dt == 0) w[0] = drafts[0], w[1] = drafts[1], w[2] = drafts[2], w[3] = drafts[3];
+          else drafts_seen(dt, w);
         } else if (live < TA_TILE) {
 #pragma unroll
           for (int i = 0; i < 4; i++) w[i] = live >= 32 * i + 32 ? ~0u : live <= 32 * i ? 0u : (1u << (live - 32 * i)) - 1;
@@ -319,22 +334,29 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         __syncwarp();
         tc_after();
         if (warp_ok) {
-          uint32_t x[4][32];
+          // The scores are read twice, 64 at a time, for the maximum and for the weights: all 128 in registers spill.
+          auto scores = [&](int half, uint32_t (&x)[2][32]) {
+            tmem_ld32(x[0], s_cols + 64 * half);
+            tmem_ld32(x[1], s_cols + 64 * half + 32);
+            wait_ld(x[0]);
+            wait_ld(x[1]);
+            if (masked) {
 #pragma unroll
-          for (int c = 0; c < 4; c++) tmem_ld32(x[c], s_cols + 32 * c);
+              for (int c = 0; c < 2; c++)
 #pragma unroll
-          for (int c = 0; c < 4; c++) wait_ld(x[c]);
-          if (masked) {
-#pragma unroll
-            for (int c = 0; c < 4; c++)
-#pragma unroll
-              for (int i = 0; i < 32; i++) x[c][i] = w[c] >> i & 1 ? x[c][i] : 0xff800000u;
-          }
+                for (int i = 0; i < 32; i++) x[c][i] = w[2 * half + c] >> i & 1 ? x[c][i] : 0xff800000u;
+            }
+          };
           float mx[4] = {m, m, m, m};
 #pragma unroll
-          for (int i = 0; i < 32; i++)
+          for (int half = 0; half < 2; half++) {
+            uint32_t x[2][32];
+            scores(half, x);
 #pragma unroll
-            for (int c = 0; c < 4; c++) mx[c] = fmaxf(mx[c], __uint_as_float(x[c][i]));
+            for (int i = 0; i < 32; i += 2)
+#pragma unroll
+              for (int c = 0; c < 4; c++) mx[c] = fmaxf(mx[c], __uint_as_float(x[c >> 1][i + (c & 1)]));
+          }
           const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           if (j < 2 - (NT == 2)) {   // the stream's first tile: nothing to scale
             m = m_new;
@@ -357,17 +379,17 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             }
           }
           const float least = m == -INFINITY ? 0.0f : -m;   // (x - m) scale, not x scale - m scale: the difference of close scores is exact
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // two pairs
 #pragma unroll
           for (int half = 0; half < 2; half++) {
-            uint32_t pr[32];
+            uint32_t x[2][32], pr[32];
+            scores(half, x);
 #pragma unroll
             for (int i = 0; i < 32; i++) {
-              const int at = 64 * half + 2 * i;
-              float a = __uint_as_float(x[at >> 5][at & 31]), b = __uint_as_float(x[at >> 5][(at & 31) + 1]);
+              float a = __uint_as_float(x[i >> 4][2 * i & 31]), b = __uint_as_float(x[i >> 4][(2 * i & 31) + 1]);
               add_mul2(a, b, least, scale);
               a = ex2(a), b = ex2(b);
-              sum[i & 1] += a, sum[2 + (i & 1)] += b;
+              add2(sum[2 * (i & 1)], sum[2 * (i & 1) + 1], a, b);
               pr[i] = pack2(a, b);   // 8 bits of each weight: a tcgen05 product of bf16 values takes bf16 weights; the sum has them all
             }
             tmem_st32(s_cols + 32 * half, pr);
