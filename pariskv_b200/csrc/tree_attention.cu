@@ -108,6 +108,11 @@ __device__ __forceinline__ void add2(float& a, float& b, float c, float d) {
       : "+f"(a), "+f"(b)
       : "f"(c), "f"(d));
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -353,9 +358,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             uint32_t x[2][32];
             scores(half, x);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2)
+            for (int i = 0; i < 32; i += 4)
 #pragma unroll
-              for (int c = 0; c < 4; c++) mx[c] = fmaxf(mx[c], __uint_as_float(x[c >> 1][i + (c & 1)]));
+              for (int c = 0; c < 4; c++) mx[c] = max3(mx[c], __uint_as_float(x[c >> 1][i + 2 * (c & 1)]), __uint_as_float(x[c >> 1][i + 2 * (c & 1) + 1]));
           }
           const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           if (j < 2 - (NT == 2)) {   // the stream's first tile: nothing to scale
@@ -384,13 +389,21 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           for (int half = 0; half < 2; half++) {
             uint32_t x[2][32], pr[32];
             scores(half, x);
+            // sixteen at a time, step by step, so that no step waits for the one before
 #pragma unroll
-            for (int i = 0; i < 32; i++) {
-              float a = __uint_as_float(x[i >> 4][2 * i & 31]), b = __uint_as_float(x[i >> 4][(2 * i & 31) + 1]);
-              add_mul2(a, b, least, scale);
-              a = ex2(a), b = ex2(b);
-              add2(sum[2 * (i & 1)], sum[2 * (i & 1) + 1], a, b);
-              pr[i] = pack2(a, b);   // 8 bits of each weight: a tcgen05 product of bf16 values takes bf16 weights; the sum has them all
+            for (int i0 = 0; i0 < 64; i0 += 16) {
+              float y[16];
+#pragma unroll
+              for (int i = 0; i < 16; i++) y[i] = __uint_as_float(x[i0 >> 5][(i0 & 31) + i]);
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) add_mul2(y[i], y[i + 1], least, scale);
+#pragma unroll
+              for (int i = 0; i < 16; i++) y[i] = ex2(y[i]);
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                add2(sum[i & 2], sum[(i & 2) + 1], y[i], y[i + 1]);
+                pr[(i0 + i) / 2] = pack2(y[i], y[i + 1]);   // 8 bits of each weight: a tcgen05 product of bf16 values takes bf16 weights; the sum has them all
+              }
             }
             tmem_st32(s_cols + 32 * half, pr);
           }
