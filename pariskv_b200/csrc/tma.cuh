@@ -20,9 +20,9 @@ __device__ __forceinline__ void mbar_init(unsigned mb, unsigned count) {
 __device__ __forceinline__ bool mbar_try(unsigned mb, unsigned parity) {
   unsigned done;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(done)
-      : "r"(mb), "r"(parity)
+      : "r"(mb), "r"(parity), "r"(10000)
       : "memory");
   return done != 0;
 }

@@ -11,8 +11,7 @@
 // The tiles of all (sample, KV head, row group) items, laid end to end, are cut into equal ranges, one per SM; the lengths come from
 // device memory, every block finds its range by itself.  Items that are cut leave partial (m, l, O) records, which tree_merge_kernel joins
 // in a fixed order.
-#include "attend.cuh"
-#include "tma.cuh"
+#include "tiles.cuh"
 
 namespace pk {
 namespace {
@@ -21,6 +20,7 @@ constexpr int TA_TILE = 128;                   // keys of a tile
 constexpr int TA_THREADS = 320;                // two softmax groups of four warps, a warp for the copies, a warp for the products
 constexpr int TA_STAGE = 32768;                // a tile of K or V: two halves of 64 channels, 128 rows of 128 bytes
 constexpr int TA_WAIT_LIMIT = 4000000;
+constexpr int TA_FEW = 32;                       // up to so many query rows attend_few.cu has the call
 constexpr float TA_LAZY = 8.0f;                // log2: the maximum that O is scaled to may lie this far below the true one
 
 template <int NT> struct TaRing { static constexpr int stages = NT == 2 ? 5 : 6; };
@@ -91,41 +91,6 @@ struct Cursor {
     }
   }
 };
-
-__device__ __forceinline__ float ex2(float x) {   // 2^x, results below 2^-126 are zero
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// (a + c) f, (b + c) f: two fp32 operations in one instruction
-__device__ __forceinline__ void add_mul2(float& a, float& b, float c, float f) {
-  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 y, {%3, %3};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "+f"(a), "+f"(b)
-      : "f"(c), "f"(f));
-}
-__device__ __forceinline__ void add2(float& a, float& b, float c, float d) {
-  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "+f"(a), "+f"(b)
-      : "f"(c), "f"(d));
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {   // the values are there behind it, and no use of them moves before it
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
-                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
-                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
-}
-__device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-__device__ __forceinline__ bool not_finite(uint32_t bf16) { return (bf16 & 0x7f80u) == 0x7f80u; }
 
 template <int NT>
 __global__ void __launch_bounds__(TA_THREADS, 1)
@@ -581,22 +546,6 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
   if (p.a.lse && lane == 0) p.a.lse[row] = L == 0.0f ? -INFINITY : M + log2f(L);
 }
 
-// Rows of 128 bf16 in three dimensions, boxes of 64 channels x `box` rows; false where a tensor map cannot have these strides.
-bool rows_map(CUtensorMap* m, const void* base, int64_t d1, int64_t s1, int64_t d2, int64_t s2, int64_t d3, int64_t s3, int box) {
-  const auto encode = tensor_map_encoder();
-  const int64_t d[3] = {d1, d2, d3};
-  int64_t s[3] = {s1, s2, s3};
-  for (int i = 0; i < 3; i++) {
-    if (d[i] == 1) s[i] = 128;
-    if (s[i] <= 0 || s[i] >= (1ll << 38) || d[i] >= (1ll << 31)) return false;
-  }
-  if (!encode) return false;
-  const cuuint64_t dims[4] = {128, (cuuint64_t)d1, (cuuint64_t)d2, (cuuint64_t)d3}, strides[3] = {(cuuint64_t)s[0] * 2, (cuuint64_t)s[1] * 2, (cuuint64_t)s[2] * 2};
-  const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1}, steps[4] = {1, 1, 1, 1};
-  return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int NT>
 int launch_tree(const AttendParams& a, int64_t bs, void* workspace, cudaStream_t st) {
   CUtensorMap mk, mv, mdk, mdv;
@@ -629,6 +578,7 @@ using namespace pk;
 
 extern "C" int64_t pk_tree_attention_workspace_bytes(int64_t, int64_t T, int64_t Hq, int64_t H, int64_t) {
   const int64_t rows = H > 0 && T * (Hq / H) > 128 ? 256 : 128;
+  if (H > 0 && T * (Hq / H) <= TA_FEW) return attend_few_workspace();
   return 2 * (int64_t)sm_count() * rows * 130 * 4;
 }
 
@@ -654,5 +604,6 @@ extern "C" int pk_tree_attention(const pk_tensor* queries, const pk_tensor* keys
   if (bs == 0 || p.T == 0) return PK_OK;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < pk_tree_attention_workspace_bytes(bs, p.T, queries->shape[2], p.H, p.cap))
     return fail(PK_ERR_WORKSPACE, "tree_attention: workspace missing, misaligned or too small");
+  if (p.T * p.G <= TA_FEW) return launch_attend_few(p, bs, workspace, "tree_attention", (cudaStream_t)stream);
   return p.T * p.G > 128 ? launch_tree<2>(p, bs, workspace, (cudaStream_t)stream) : launch_tree<1>(p, bs, workspace, (cudaStream_t)stream);
 }
