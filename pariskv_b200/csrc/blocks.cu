@@ -51,91 +51,204 @@ struct SelectParams {
   int32_t* ids;        // [rows][n]
 };
 
+// Keys order as the scores do.  NaN is above all numbers, what is always taken above that; 0: a block that is not seen.
 constexpr uint32_t FORCED = 0xffffffffu, NOT_A_NUMBER = 0xfffffffeu;
 
 // Blocks that row (b, t) sees.
-__device__ __forceinline__ int64_t visible_blocks(const SelectParams& p, int64_t b, int t) {
+__device__ __forceinline__ int visible_blocks(const SelectParams& p, int64_t b, int t) {
   const int64_t pos = min((int64_t)p.lengths[b], p.nb * p.block) - p.T + t;
-  return pos < 0 ? 0 : pos / p.block + 1;
+  return pos < 0 ? 0 : (int)(pos / p.block) + 1;
 }
 
-// A warp per (row, block of keys).
+// Sums of eight values over the lanes of a warp; lane L gets that of value L / 4.
+__device__ __forceinline__ double warp_sums8(double (&v)[8], int lane) {
+#pragma unroll
+  for (int n = 4, off = 16; n >= 1; n /= 2, off /= 2) {
+    const bool up = lane & off;
+#pragma unroll
+    for (int i = 0; i < n; i++) {
+      const double keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+    }
+  }
+  v[0] += __shfl_xor_sync(0xffffffffu, v[0], 2);
+  v[0] += __shfl_xor_sync(0xffffffffu, v[0], 1);
+  return v[0];
+}
+
+// A warp takes eight blocks of keys at a time, 4 KB that are in flight at once, for TT tokens: lanes 0 .. 15 hold eight channels of lo and N each, the
+// others of hi and P.  Bounded by the bounds' bytes where there are many (the conversions to 64 bits, 16 a clock and SM, take about three quarters
+// of that time), otherwise by latency.
+template <int TT>
 __global__ void __launch_bounds__(128) block_score_kernel(SelectParams p) {
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const int64_t row = blockIdx.y, h = row % p.H, t = row / p.H % p.T, b = row / p.H / p.T;
-  const int64_t seen = visible_blocks(p, b, (int)t), j = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (j >= seen) return;
-  double s = 0.0;
-  const uint16_t* bd = p.bounds + b * p.o_b + h * p.o_h + j * p.o_j;
+  const int lane = threadIdx.x & 31, h = blockIdx.y % p.H, t0 = blockIdx.y / p.H * TT;
+  const int64_t b = blockIdx.z;
+  const bool upper = lane >= 16;
+  int seen[TT], most = 0;
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    double up = 0.0, down = 0.0;
-    for (int g = 0; g < p.G; g++) {
-      const double x = bf2f(p.q[b * p.q_b + t * p.q_t + (h * p.G + g) * p.q_h + 4 * lane + i]);
-      if (x < 0) down += x;
-      else up += x;
-    }
-    // (no products of a zero with an infinite bound)
-    s += !(up == 0) ? up * bf2f(bd[128 + 4 * lane + i]) : 0.0;
-    s += !(down == 0) ? down * bf2f(bd[4 * lane + i]) : 0.0;
+  for (int i = 0; i < TT; i++) seen[i] = t0 + i < p.T ? visible_blocks(p, b, t0 + i) : 0, most = max(most, seen[i]);
+  const uint16_t* bounds = p.bounds + b * p.o_b + h * p.o_h + 8 * lane;
+  const int groups = (most + 7) / 8, stride = (int)gridDim.x * 4;
+  int group = (int)blockIdx.x * 4 + (threadIdx.x >> 5);
+  uint4 x[8];
+  auto load = [&](int at) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = 8 * at + i < most ? *reinterpret_cast<const uint4*>(bounds + (int64_t)(8 * at + i) * p.o_j) : make_uint4(0, 0, 0, 0);
+  };
+  if (group >= groups) return;
+  load(group);
+  double c[TT][8];   // P or N of this lane's channels
+#pragma unroll
+  for (int i = 0; i < TT; i++) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) c[i][e] = 0.0;
+    if (t0 + i < p.T)
+      for (int g = 0; g < p.G; g++) {
+        const uint4 q = *reinterpret_cast<const uint4*>(p.q + b * p.q_b + (int64_t)(t0 + i) * p.q_t + (int64_t)(h * p.G + g) * p.q_h + 8 * (lane & 15));
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float v = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+          if (upper ? !(v < 0.0f) : v < 0.0f) c[i][e] += (double)v;
+        }
+      }
   }
+  for (; group < groups; group += stride) {
+    double sum[TT][8];
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-  if (lane == 0) {
-    const float f = (float)s + 0.0f;   // (one zero)
-    p.keys[row * p.nb + j] = j < p.sink || j >= seen - p.local ? FORCED : f != f ? NOT_A_NUMBER : ord_key(f);
+    for (int i = 0; i < 8; i++) {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      bool odd = false;
+#pragma unroll
+      for (int e = 0; e < 4; e++) odd |= (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
+      double v[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = (double)__uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+      if (__any_sync(0xffffffffu, odd)) {   // an infinite bound (or NaN): nothing comes of it where the query has a zero
+#pragma unroll
+        for (int k = 0; k < TT; k++) {
+          double s = 0.0;
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            if (!(c[k][e] == 0.0)) s = fma(c[k][e], v[e], s);
+          sum[k][i] = s;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < TT; k++) {
+          double s = c[k][0] * v[0], r = c[k][1] * v[1];
+#pragma unroll
+          for (int e = 2; e < 8; e += 2) s = fma(c[k][e], v[e], s), r = fma(c[k][e + 1], v[e + 1], r);
+          sum[k][i] = s + r;
+        }
+      }
+    }
+    const int at = group;
+    if (group + stride < groups) load(group + stride);
+#pragma unroll
+    for (int k = 0; k < TT; k++) {
+      const float f = (float)warp_sums8(sum[k], lane) + 0.0f;   // (one zero)
+      const int j = 8 * at + (lane >> 2);
+      if ((lane & 3) == 0 && j < seen[k])
+        p.keys[((b * p.T + t0 + k) * p.H + h) * p.nb + j] = j < p.sink || j >= seen[k] - p.local ? FORCED : f != f ? NOT_A_NUMBER : ord_key(f);
+    }
   }
 }
 
-// A block per row: the n-th largest key bit by bit, then the chosen ones in order.
-__global__ void __launch_bounds__(256) block_pick_kernel(SelectParams p) {
+// A block per row.  The keys between the lowest and the highest are counted in 1024 bins of equal width, the bin of the n-th largest is cut again until it
+// is taken whole or holds one value (of which the lowest positions are taken); usually two rounds.  Then the chosen blocks in order, every warp
+// those of its part of the row.  Latency: keys in shared memory where they fit.
+constexpr int PICK_THREADS = 512, PICK_WARPS = PICK_THREADS / 32, PICK_BINS = 1024, PICK_KEPT = 16384;
+__global__ void __launch_bounds__(PICK_THREADS) block_pick_kernel(SelectParams p, bool kept) {
+  extern __shared__ uint32_t s_keys[];
+  __shared__ unsigned s_bins[PICK_BINS], s_a[PICK_WARPS], s_b[PICK_WARPS], s_c[PICK_WARPS], s_found[3];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t row = blockIdx.x, t = row / p.H % p.T, b = row / p.H / p.T;
   pdl_wait();
   pdl_trigger();
-  const int64_t row = blockIdx.x, t = row / p.H % p.T, b = row / p.H / p.T;
-  const int64_t seen = visible_blocks(p, b, (int)t);
-  const uint32_t* keys = p.keys + row * p.nb;
+  const int seen = visible_blocks(p, b, (int)t);
+  const uint32_t* in = p.keys + row * p.nb;
   int32_t* ids = p.ids + row * p.n;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  __shared__ int s_count[8], s_ties[8];
-  const int n = (int)min((int64_t)p.n, seen);
-  for (int i = n + tid; i < p.n; i += 256) ids[i] = -1;
-  uint32_t cut = 0;
-  int above = 0;
-  auto count = [&](uint32_t least) {   // keys >= least
-    int c = 0;
-    for (int64_t j = tid; j < seen; j += 256) c += keys[j] >= least;
-    c = __reduce_add_sync(0xffffffffu, c);
+  for (int i = min(p.n, seen) + tid; i < p.n; i += PICK_THREADS) ids[i] = -1;
+  if (seen <= p.n) {   // all of them
+    for (int i = tid; i < seen; i += PICK_THREADS) ids[i] = i;
+    return;
+  }
+  auto key = [&](int j) { return kept ? s_keys[j] : in[j]; };
+  uint32_t lo = 0xffffffffu, hi = 0;   // extremes of the keys that are not FORCED
+  unsigned forced = 0;
+  for (int j0 = tid; j0 < seen; j0 += 8 * PICK_THREADS) {
+    uint32_t k[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) k[i] = in[min(j0 + i * PICK_THREADS, seen - 1)];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (j0 + i * PICK_THREADS < seen) {
+        if (kept) s_keys[j0 + i * PICK_THREADS] = k[i];
+        if (k[i] == FORCED) forced++;
+        else lo = min(lo, k[i]), hi = max(hi, k[i]);
+      }
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi), forced = __reduce_add_sync(0xffffffffu, forced);
+  if (lane == 0) s_a[warp] = lo, s_b[warp] = hi, s_c[warp] = forced;
+  __syncthreads();
+  {
+    const unsigned x = s_a[lane % PICK_WARPS], y = s_b[lane % PICK_WARPS], z = lane < PICK_WARPS ? s_c[lane] : 0;
+    lo = __reduce_min_sync(0xffffffffu, x), hi = __reduce_max_sync(0xffffffffu, y), forced = __reduce_add_sync(0xffffffffu, z);
+  }
+  // (more blocks than are taken are seen, and the forced ones are at most n: there are others)
+  unsigned want = (unsigned)p.n - forced;   // of the keys in [lo, hi]; those above hi are taken
+  unsigned in_range = 0xffffffffu;
+  while (want > 0 && want != in_range && lo != hi) {
+    const int shift = max(0, 22 - __clz(hi - lo));   // (hi - lo) >> shift < 1024
     __syncthreads();
-    if (lane == 0) s_count[warp] = c;
+    for (int i = tid; i < PICK_BINS; i += PICK_THREADS) s_bins[i] = 0;
     __syncthreads();
-    int total = 0;
-    for (int w = 0; w < 8; w++) total += s_count[w];
-    return total;
-  };
-  for (int bit = 31; bit >= 0; bit--)
-    if (count(cut | 1u << bit) >= n) cut |= 1u << bit;
-  above = cut == 0xffffffffu ? 0 : count(cut + 1);
-  int placed = 0, ties_seen = 0;
-  for (int64_t j0 = 0; j0 < seen; j0 += 256) {
-    const int64_t j = j0 + tid;
-    const uint32_t k = j < seen ? keys[j] : 0;
-    const bool tie = j < seen && k == cut;
-    const unsigned tie_bits = __ballot_sync(0xffffffffu, tie);
+    for (int j = tid; j < seen; j += PICK_THREADS) {
+      const uint32_t k = key(j);
+      if (k >= lo && k <= hi && k != FORCED) atomicAdd(&s_bins[(k - lo) >> shift], 1u);
+    }
     __syncthreads();
-    if (lane == 0) s_ties[warp] = __popc(tie_bits);
+    // thread i: bins 1023 - 2 i and 1022 - 2 i, from the highest down
+    const unsigned c0 = s_bins[PICK_BINS - 1 - 2 * tid], c1 = s_bins[PICK_BINS - 2 - 2 * tid];
+    unsigned sum = c0 + c1;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const unsigned o = __shfl_up_sync(0xffffffffu, sum, off);
+      if (lane >= off) sum += o;
+    }
+    if (lane == 31) s_a[warp] = sum;
     __syncthreads();
-    int before = ties_seen, all = 0;
-    for (int w = 0; w < 8; w++) before += w < warp ? s_ties[w] : 0, all += s_ties[w];
-    const bool take = j < seen && (k > cut || (tie && before + __popc(tie_bits & ((1u << lane) - 1)) < n - above));
-    ties_seen += all;
-    const unsigned bits = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) s_count[warp] = __popc(bits);
+    const unsigned before = __reduce_add_sync(0xffffffffu, lane < warp ? s_a[lane & (PICK_WARPS - 1)] : 0u) + sum - c0 - c1;
+    if (before < want && before + c0 >= want) s_found[0] = PICK_BINS - 1 - 2 * tid, s_found[1] = before, s_found[2] = c0;
+    else if (before + c0 < want && before + c0 + c1 >= want) s_found[0] = PICK_BINS - 2 - 2 * tid, s_found[1] = before + c0, s_found[2] = c1;
     __syncthreads();
-    int at = placed;
-    for (int w = 0; w < 8; w++) at += w < warp ? s_count[w] : 0, placed += s_count[w];
-    if (take) ids[at + __popc(bits & ((1u << lane) - 1))] = (int32_t)j;
+    lo += s_found[0] << shift;
+    hi = min(hi, lo + ((1u << shift) - 1));
+    want -= s_found[1], in_range = s_found[2];
+  }
+  // above hi: taken; in [lo, hi]: the first `want` (all of them, or equal ones)
+  const int per = ((seen + PICK_WARPS - 1) / PICK_WARPS + 31) / 32 * 32, j0 = min(seen, warp * per), j1 = min(seen, j0 + per);
+  unsigned above = 0, inside = 0;
+  for (int j = j0 + lane; j < j1; j += 32) {
+    const uint32_t k = key(j);
+    if (k > hi) above++;
+    else if (k >= lo && want > 0) inside++;
+  }
+  above = __reduce_add_sync(0xffffffffu, above), inside = __reduce_add_sync(0xffffffffu, inside);
+  __syncthreads();
+  if (lane == 0) s_a[warp] = above, s_b[warp] = inside;
+  __syncthreads();
+  unsigned n_above = __reduce_add_sync(0xffffffffu, lane < warp ? s_a[lane & (PICK_WARPS - 1)] : 0u), n_inside = __reduce_add_sync(0xffffffffu, lane < warp ? s_b[lane & (PICK_WARPS - 1)] : 0u);
+  for (int j = j0; j < j1; j += 32) {
+    const uint32_t k = j + lane < j1 ? key(j + lane) : 0;
+    const bool a = j + lane < j1 && k > hi, i = j + lane < j1 && want > 0 && k >= lo && k <= hi;
+    const unsigned ab = __ballot_sync(0xffffffffu, a), ib = __ballot_sync(0xffffffffu, i), below = (1u << lane) - 1;
+    const unsigned i_at = n_inside + __popc(ib & below), at = n_above + __popc(ab & below) + min(i_at, want);
+    if (a || (i && i_at < want)) ids[at] = j + lane;
+    n_above += __popc(ab), n_inside += __popc(ib);
   }
 }
 
@@ -193,7 +306,7 @@ extern "C" int pk_select_blocks(const pk_tensor* queries, const pk_tensor* bound
   PK_REQUIRE(lengths->shape[0] == bs && is_contig(lengths), "lengths must be contiguous i32 [bs]");
   PK_REQUIRE(blocks->shape[0] == bs && blocks->shape[1] == T && blocks->shape[2] == H && is_contig(blocks), "blocks must be contiguous i32 [bs,T,H,n]");
   PK_REQUIRE(sink_blocks >= 0 && local_blocks >= 1 && sink_blocks + local_blocks <= n, "at least one local block, and no more sink and local blocks than are selected");
-  PK_REQUIRE(nb * block < (1LL << 31) && n < (1LL << 24) && bs * T * H < 65536LL * 32768, "sizes out of range");
+  PK_REQUIRE(nb * block < (1LL << 31) && n < (1LL << 24), "sizes out of range");
   if (bs * T * H == 0) return PK_OK;
   if (!workspace || workspace_bytes < pk_select_blocks_workspace_bytes(bs, T, H, nb)) return fail(PK_ERR_WORKSPACE, "select_blocks: workspace missing or too small");
   SelectParams p = {};
@@ -202,9 +315,28 @@ extern "C" int pk_select_blocks(const pk_tensor* queries, const pk_tensor* bound
   p.lengths = (const int32_t*)lengths->data, p.T = (int)T, p.H = (int)H, p.G = (int)(Hq / H), p.n = (int)n, p.block = (int)block;
   p.sink = (int)sink_blocks, p.local = (int)local_blocks, p.keys = (uint32_t*)workspace, p.ids = (int32_t*)blocks->data;
   const int64_t rows = bs * T * H;
-  PK_REQUIRE(rows < 65536, "at most 65535 rows (batch x tokens x KV heads)");
+  PK_REQUIRE(rows < (1LL << 31) && bs < 65536, "sizes out of range");
   StageTimer timer(ST_RANK, (cudaStream_t)stream);
-  if (nb > 0) launch_chain(block_score_kernel, dim3((unsigned)((nb + 3) / 4), (unsigned)rows), dim3(128), 0, (cudaStream_t)stream, p);
-  launch_chain(block_pick_kernel, dim3((unsigned)rows), dim3(256), 0, (cudaStream_t)stream, p);
+  if (nb > 0) {
+    // tokens share what is read, four at a time; warps up to four blocks of 128 threads per SM, eight keys' blocks a step
+    const int tt = T >= 3 ? 4 : (int)T;
+    const int64_t per_head = (nb + 31) / 32, heads = H * ((T + tt - 1) / tt);
+    const int64_t room = 4LL * sm_count() / (heads * bs) + 1;
+    PK_REQUIRE(heads < 65536, "at most 65535 KV heads x token groups");
+    const dim3 grid((unsigned)(per_head < room ? per_head : room), (unsigned)heads, (unsigned)bs);
+    if (tt == 1) launch_chain(block_score_kernel<1>, grid, dim3(128), 0, (cudaStream_t)stream, p);
+    else if (tt == 2) launch_chain(block_score_kernel<2>, grid, dim3(128), 0, (cudaStream_t)stream, p);
+    else launch_chain(block_score_kernel<4>, grid, dim3(128), 0, (cudaStream_t)stream, p);
+  }
+  const bool kept = nb <= PICK_KEPT;
+  if (kept && nb * 4 > 40 * 1024) {
+    static PerDevice opted;
+    if (const unsigned long long bit = first_on_device(opted)) {
+      if (cudaFuncSetAttribute(block_pick_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PICK_KEPT * 4) != cudaSuccess)
+        return fail(PK_ERR_CUDA, "select_blocks: %s", cudaGetErrorString(cudaGetLastError()));
+      mark_on_device(opted, bit);
+    }
+  }
+  launch_chain(block_pick_kernel, dim3((unsigned)rows), dim3(PICK_THREADS), kept ? (size_t)nb * 4 : 0, (cudaStream_t)stream, p, kept);
   return check_launch("select_blocks", nb > 0 ? 2 : 1);
 }
