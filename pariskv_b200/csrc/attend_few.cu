@@ -422,13 +422,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
       for (int it = 0; it < FEW_WAIT_LIMIT && !mbar_try(full + 8 * (i % FEW_BUFS), (unsigned)(i / FEW_BUFS & 1)); it++) {}
 }
 
-// A warp per query row: the records of the blocks that share its item, in the order of the tiles.
+// A block per query row: the records of the blocks that share its item, in the order of the tiles.
 template <bool TREE, int ROWS>
-__global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ FewParams p, int blocks, int64_t rows) {
+__global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ FewParams p, int blocks) {
   pdl_wait();
   pdl_trigger();
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= rows) return;
+  __shared__ MergeShared shared;
+  const int64_t row = blockIdx.x;
   const int lane = threadIdx.x & 31, Hq = p.a.H * p.a.G, hq = (int)(row % Hq), h = hq / p.a.G, g = hq % p.a.G;
   const int64_t bt = row / Hq;
   const int t = (int)(bt % p.a.T), b = (int)(bt / p.a.T), r = TREE ? t * p.a.G + g : g % ROWS;
@@ -450,23 +450,7 @@ __global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ 
   auto owner = [&](int64_t x) { return (int)(((x + 1) * shares - 1) / total); };
   const int c0 = owner(first), c1 = owner(first + n - 1);
   if (c0 == c1) return;   // written by its block
-  auto record = [&](int c) { return p.records + (2 * (int64_t)c + (c == c0)) * (ROWS * 130); };
-  float M = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, record(c)[ROWS * 128 + r]);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-  float L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-  for (int c = c0; c <= c1; c++) {
-    const float* rec = record(c);
-    const float mc = rec[ROWS * 128 + r], f = mc == -INFINITY ? 0.0f : exp2f(mc - M);
-    const float4 v = *reinterpret_cast<const float4*>(rec + (int64_t)r * 128 + 4 * lane);
-    L += rec[ROWS * 129 + r] * f;
-    o[0] += v.x * f, o[1] += v.y * f, o[2] += v.z * f, o[3] += v.w * f;
-  }
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  *reinterpret_cast<uint2*>(p.a.out + row * 128 + 4 * lane) = make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
-  if (p.a.lse && lane == 0) p.a.lse[row] = L == 0.0f ? -INFINITY : M + log2f(L);
+  merge_row(shared, c1 - c0 + 1, ROWS, r, [&](int i) { return p.records + (2 * (int64_t)(c0 + i) + (i == 0)) * (ROWS * 130); }, p.a.out + row * 128, p.a.lse ? p.a.lse + row : nullptr);
 }
 
 template <bool TREE, int ROWS>
@@ -482,7 +466,7 @@ int launch(const FewParams& p, const CUtensorMap (&maps)[4], int64_t most, const
   StageTimer timer(ST_ATTENTION, st);
   launch_chain(attend_few_kernel<TREE, ROWS>, dim3((unsigned)blocks), dim3(FEW_THREADS), FEW_SMEM, st, maps[0], maps[1], maps[2], maps[3], p);
   const int64_t rows = (int64_t)p.bs * p.a.T * p.a.H * p.a.G;
-  launch_chain(few_merge_kernel<TREE, ROWS>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p, blocks, rows);
+  launch_chain(few_merge_kernel<TREE, ROWS>, dim3((unsigned)rows), dim3(128), 0, st, p, blocks);
   return check_launch(what, 2);
 }
 

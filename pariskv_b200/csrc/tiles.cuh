@@ -40,6 +40,52 @@ __device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {   // the values are
 __device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ bool not_finite(uint32_t bf16) { return (bf16 & 0x7f80u) == 0x7f80u; }
 
+// Joins n partial results of a query row, record(i) = O rows of 128, then `rows` values m (log2), then `rows` sums l, in the order of i: a block of 128
+// threads.  A warp takes every fourth record, four channels a lane, eight loads in flight; latency is what bounds it.
+struct MergeShared {
+  float o[4][128], l[4];
+};
+template <class Record>
+__device__ __forceinline__ void merge_row(MergeShared& s, int n, int rows, int r, Record record, uint16_t* out, float* lse) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, record(i)[rows * 128 + r]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  float L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int mine = (n - warp + 3) / 4;   // records of this warp
+  for (int i0 = 0; i0 < mine; i0 += 32) {
+    float f = 0.0f;
+    if (i0 + lane < mine) {
+      const float* rec = record(4 * (i0 + lane) + warp);
+      const float m = rec[rows * 128 + r];
+      f = m == -INFINITY ? 0.0f : exp2f(m - M);
+      L += rec[rows * 129 + r] * f;
+    }
+    const int cnt = min(32, mine - i0);
+    for (int k0 = 0; k0 < cnt; k0 += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        v[k] = k0 + k < cnt ? *reinterpret_cast<const float4*>(record(4 * (i0 + k0 + k) + warp) + (int64_t)r * 128 + 4 * lane) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const float fk = __shfl_sync(0xffffffffu, f, k0 + k);
+        if (k0 + k < cnt && fk != 0.0f) o[0] += v[k].x * fk, o[1] += v[k].y * fk, o[2] += v[k].z * fk, o[3] += v[k].w * fk;   // (NaN != 0)
+      }
+    }
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+  *reinterpret_cast<float4*>(&s.o[warp][4 * lane]) = make_float4(o[0], o[1], o[2], o[3]);
+  if (lane == 0) s.l[warp] = L;
+  __syncthreads();
+  L = (s.l[0] + s.l[1]) + (s.l[2] + s.l[3]);
+  const float O = (s.o[0][tid] + s.o[1][tid]) + (s.o[2][tid] + s.o[3][tid]);
+  out[tid] = f2bf(L == 0.0f ? 0.0f : O / L);
+  if (lse && tid == 0) *lse = L == 0.0f ? -INFINITY : M + log2f(L);
+}
+
 // Rows of 128 bf16 in three dimensions, boxes of 64 channels x `box` rows; false where a tensor map cannot have these strides.
 inline bool rows_map(CUtensorMap* m, const void* base, int64_t d1, int64_t s1, int64_t d2, int64_t s2, int64_t d3, int64_t s3, int box) {
   const auto encode = tensor_map_encoder();

@@ -505,13 +505,13 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
   if (warp == 8) tmem_free(tmem, 512);
 }
 
-// A warp per query row: the records of the blocks that share its item, in the order of the tiles.
+// A block per query row: the records of the blocks that share its item, in the order of the tiles.
 template <int NT>
-__global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__ TreeParams p, int blocks, int64_t rows) {
+__global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__ TreeParams p, int blocks) {
   pdl_wait();
   pdl_trigger();
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= rows) return;
+  __shared__ MergeShared shared;
+  const int64_t row = blockIdx.x;
   const int lane = threadIdx.x & 31, Hq = p.a.H * p.a.G, hq = (int)(row % Hq), h = hq / p.a.G, g = hq % p.a.G;
   const int b = (int)(row / Hq / p.a.T), t = (int)(row / Hq % p.a.T), mt = t / p.tile_tokens, group = mt / NT;
   const int r = (mt % NT) * 128 + (t - mt * p.tile_tokens) * p.a.G + g;
@@ -527,23 +527,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
   const int c0 = owner(first), c1 = owner(last);
   if (c0 == c1) return;   // written by its block
   constexpr int ROWS = NT * 128;
-  auto record = [&](int c) { return p.records + (2 * (int64_t)c + (c == c0)) * (ROWS * 130); };
-  float M = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, record(c)[ROWS * 128 + r]);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-  float L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int c = c0; c <= c1; c++) {
-    const float* rec = record(c);
-    const float mc = rec[ROWS * 128 + r], f = mc == -INFINITY ? 0.0f : exp2f(mc - M);
-    const float4 v = *reinterpret_cast<const float4*>(rec + (int64_t)r * 128 + 4 * lane);
-    L += rec[ROWS * 129 + r] * f;
-    o[0] += v.x * f, o[1] += v.y * f, o[2] += v.z * f, o[3] += v.w * f;
-  }
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  *reinterpret_cast<uint2*>(p.a.out + row * 128 + 4 * lane) = make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
-  if (p.a.lse && lane == 0) p.a.lse[row] = L == 0.0f ? -INFINITY : M + log2f(L);
+  merge_row(shared, c1 - c0 + 1, ROWS, r, [&](int i) { return p.records + (2 * (int64_t)(c0 + i) + (i == 0)) * (ROWS * 130); }, p.a.out + row * 128, p.a.lse ? p.a.lse + row : nullptr);
 }
 
 template <int NT>
@@ -567,7 +551,7 @@ int launch_tree(const AttendParams& a, int64_t bs, void* workspace, cudaStream_t
   StageTimer timer(ST_ATTENTION, st);
   launch_chain(tree_tile_kernel<NT>, dim3((unsigned)blocks), dim3(TA_THREADS), SMEM, st, mk, mv, mdk, mdv, p);
   const int64_t rows = bs * a.T * a.H * a.G;
-  launch_chain(tree_merge_kernel<NT>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p, blocks, rows);
+  launch_chain(tree_merge_kernel<NT>, dim3((unsigned)rows), dim3(128), 0, st, p, blocks);
   return check_launch("tree_attention", 2);
 }
 
