@@ -3,7 +3,7 @@
 //   score_j   = sum_d sum_g max(q_gd lo_jd, q_gd hi_jd), no less than the sum over the group's query heads g of q_g.k for any key k of the
 //               block;  with P_d = sum_g max(q_gd, 0) and N_d = sum_g min(q_gd, 0) it is sum_d P_d hi_jd + N_d lo_jd: one pass over the
 //               bounds whatever the number of query heads.
-// Sums in 64 bits, rounded once to 32: the choice does not depend on their order.
+// The choice is that of sums in 64 bits, rounded once to 32: it does not depend on their order.
 #include "attend.cuh"
 
 namespace pk {
@@ -48,6 +48,7 @@ struct SelectParams {
   const int32_t* lengths;
   int T, H, G, n, block, sink, local;
   uint32_t* keys;      // [rows][nb] ordered keys of the scores
+  float* limits;       // [rows][warps of the score kernel on a row]
   int32_t* ids;        // [rows][n]
 };
 
@@ -61,13 +62,13 @@ __device__ __forceinline__ int visible_blocks(const SelectParams& p, int64_t b, 
 }
 
 // Sums of eight values over the lanes of a warp; lane L gets that of value L / 4.
-__device__ __forceinline__ double warp_sums8(double (&v)[8], int lane) {
+__device__ __forceinline__ float warp_sums8(float (&v)[8], int lane) {
 #pragma unroll
   for (int n = 4, off = 16; n >= 1; n /= 2, off /= 2) {
     const bool up = lane & off;
 #pragma unroll
     for (int i = 0; i < n; i++) {
-      const double keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
+      const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
       v[i] = keep + __shfl_xor_sync(0xffffffffu, give, off);
     }
   }
@@ -75,114 +76,153 @@ __device__ __forceinline__ double warp_sums8(double (&v)[8], int lane) {
   v[0] += __shfl_xor_sync(0xffffffffu, v[0], 1);
   return v[0];
 }
-
-// A warp takes eight blocks of keys at a time, 4 KB that are in flight at once, for TT tokens: lanes 0 .. 15 hold eight channels of lo and N each, the
-// others of hi and P.  Bounded by the bounds' bytes where there are many (the conversions to 64 bits, 16 a clock and SM, take about three quarters
-// of that time), otherwise by latency.
-template <int TT>
-__global__ void __launch_bounds__(128) block_score_kernel(SelectParams p) {
-  pdl_wait();
-  pdl_trigger();
-  const int lane = threadIdx.x & 31, h = blockIdx.y % p.H, t0 = blockIdx.y / p.H * TT;
-  const int64_t b = blockIdx.z;
-  const bool upper = lane >= 16;
-  int seen[TT], most = 0;
+// P (lanes 16 .. 31) or N (0 .. 15) of eight channels of token t: sums over the group's heads, four loads in flight.
+template <class F>
+__device__ __forceinline__ void query_sums(const SelectParams& p, int64_t b, int t, int h, int lane, F (&c)[8]) {
+  const uint16_t* q = p.q + b * p.q_b + (int64_t)t * p.q_t + (int64_t)h * p.G * p.q_h + 8 * (lane & 15);
 #pragma unroll
-  for (int i = 0; i < TT; i++) seen[i] = t0 + i < p.T ? visible_blocks(p, b, t0 + i) : 0, most = max(most, seen[i]);
-  const uint16_t* bounds = p.bounds + b * p.o_b + h * p.o_h + 8 * lane;
-  const int groups = (most + 7) / 8, stride = (int)gridDim.x * 4;
-  int group = (int)blockIdx.x * 4 + (threadIdx.x >> 5);
-  uint4 x[8];
-  auto load = [&](int at) {
+  for (int e = 0; e < 8; e++) c[e] = 0;
+  for (int g0 = 0; g0 < p.G; g0 += 4) {
+    uint4 x[4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = 8 * at + i < most ? *reinterpret_cast<const uint4*>(bounds + (int64_t)(8 * at + i) * p.o_j) : make_uint4(0, 0, 0, 0);
-  };
-  if (group >= groups) return;
-  load(group);
-  double c[TT][8];   // P or N of this lane's channels
+    for (int g = 0; g < 4; g++) x[g] = g0 + g < p.G ? *reinterpret_cast<const uint4*>(q + (g0 + g) * p.q_h) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-  for (int i = 0; i < TT; i++) {
+    for (int g = 0; g < 4; g++) {
+      const uint32_t w[4] = {x[g].x, x[g].y, x[g].z, x[g].w};
 #pragma unroll
-    for (int e = 0; e < 8; e++) c[i][e] = 0.0;
-    if (t0 + i < p.T)
-      for (int g = 0; g < p.G; g++) {
-        const uint4 q = *reinterpret_cast<const uint4*>(p.q + b * p.q_b + (int64_t)(t0 + i) * p.q_t + (int64_t)(h * p.G + g) * p.q_h + 8 * (lane & 15));
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float v = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
-          if (upper ? !(v < 0.0f) : v < 0.0f) c[i][e] += (double)v;
-        }
+      for (int e = 0; e < 8; e++) {
+        const float v = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+        if (lane >= 16 ? !(v < 0.0f) : v < 0.0f) c[e] += (F)v;
       }
-  }
-  for (; group < groups; group += stride) {
-    double sum[TT][8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      bool odd = false;
-#pragma unroll
-      for (int e = 0; e < 4; e++) odd |= (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
-      double v[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[e] = (double)__uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
-      if (__any_sync(0xffffffffu, odd)) {   // an infinite bound (or NaN): nothing comes of it where the query has a zero
-#pragma unroll
-        for (int k = 0; k < TT; k++) {
-          double s = 0.0;
-#pragma unroll
-          for (int e = 0; e < 8; e++)
-            if (!(c[k][e] == 0.0)) s = fma(c[k][e], v[e], s);
-          sum[k][i] = s;
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < TT; k++) {
-          double s = c[k][0] * v[0], r = c[k][1] * v[1];
-#pragma unroll
-          for (int e = 2; e < 8; e += 2) s = fma(c[k][e], v[e], s), r = fma(c[k][e + 1], v[e + 1], r);
-          sum[k][i] = s + r;
-        }
-      }
-    }
-    const int at = group;
-    if (group + stride < groups) load(group + stride);
-#pragma unroll
-    for (int k = 0; k < TT; k++) {
-      const float f = (float)warp_sums8(sum[k], lane) + 0.0f;   // (one zero)
-      const int j = 8 * at + (lane >> 2);
-      if ((lane & 3) == 0 && j < seen[k])
-        p.keys[((b * p.T + t0 + k) * p.H + h) * p.nb + j] = j < p.sink || j >= seen[k] - p.local ? FORCED : f != f ? NOT_A_NUMBER : ord_key(f);
     }
   }
 }
 
+// Scores in 32 bits, and a bound A of every sum of absolute values: A = sum_d P_d max |hi_d| + |N_d| max |lo_d| over the warp's blocks.  A score is off
+// by at most G + 13 roundings of 2^-24 A (P or N, eight products in a row, five additions of the lanes' sums): where the choice hangs on less
+// than that, block_pick_kernel takes the 64-bit scores.
+// A warp takes eight blocks of keys at a time, 4 KB that are in flight at once, for TT tokens: lanes 0 .. 15 hold eight channels of lo and N each, the
+// others of hi and P.  Bounded by the bounds' bytes where there are many, otherwise by latency.  (64-bit sums throughout: 8192 blocks of 8
+// heads for four tokens 46 us, of 128 heads x 770 blocks for one 26 us; the conversions to 64 bits alone, 8 a clock and SM, take longer than the bytes.)
+constexpr int SCORE_CTAS = 3;   // blocks per SM
+template <int TT>
+__global__ void __launch_bounds__(128, SCORE_CTAS) block_score_kernel(SelectParams p) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, h = blockIdx.y % p.H, t0 = blockIdx.y / p.H * TT;
+  const int64_t b = blockIdx.z;
+  int seen[TT], most = 0;
+#pragma unroll
+  for (int i = 0; i < TT; i++) seen[i] = t0 + i < p.T ? visible_blocks(p, b, t0 + i) : 0, most = max(most, seen[i]);
+  const uint16_t* bounds = p.bounds + b * p.o_b + h * p.o_h + 8 * lane;
+  const int groups = (most + 7) / 8, warps = (int)gridDim.x * 4, self = (int)blockIdx.x * 4 + (threadIdx.x >> 5);
+  struct Group {
+    uint4 x[8];
+  } now, next;
+  auto load = [&](Group& to, int at) {
+    const uint16_t* from = bounds + (int64_t)(8 * at) * p.o_j;
+#pragma unroll
+    for (int i = 0; i < 8; i++) to.x[i] = 8 * at + i < most ? *reinterpret_cast<const uint4*>(from + i * p.o_j) : make_uint4(0, 0, 0, 0);
+  };
+  load(now, self);
+  load(next, self + warps);
+  float c[TT][8];   // P or N of this lane's channels
+#pragma unroll
+  for (int i = 0; i < TT; i++) query_sums(p, b, min(t0 + i, p.T - 1), h, lane, c[i]);
+  __nv_bfloat162 top[4];   // largest magnitudes of this lane's channels
+#pragma unroll
+  for (int e = 0; e < 4; e++) top[e] = __nv_bfloat162(__ushort_as_bfloat16(0), __ushort_as_bfloat16(0));
+  auto take = [&](Group& of, int group) {   // and asks for the one after the next in its place
+    float sum[TT][8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const uint32_t w[4] = {of.x[i].x, of.x[i].y, of.x[i].z, of.x[i].w};
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        v[2 * e] = __uint_as_float(w[e] << 16), v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+        top[e] = __hmax2_nan(top[e], __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[e])));
+      }
+#pragma unroll
+      for (int k = 0; k < TT; k++) {
+        float s = c[k][0] * v[0];
+#pragma unroll
+        for (int e = 1; e < 8; e++) s = fmaf(c[k][e], v[e], s);
+        sum[k][i] = s;
+      }
+    }
+    load(of, group + 2 * warps);
+#pragma unroll
+    for (int k = 0; k < TT; k++) {
+      const float f = warp_sums8(sum[k], lane) + 0.0f;   // (one zero)
+      const int j = 8 * group + (lane >> 2);
+      if ((lane & 3) == 0 && j < seen[k])
+        p.keys[((b * p.T + t0 + k) * p.H + h) * p.nb + j] = j < p.sink || j >= seen[k] - p.local ? FORCED : f != f ? NOT_A_NUMBER : ord_key(f);
+    }
+  };
+  for (int group = self; group < groups; group += 2 * warps) {
+    take(now, group);
+    if (group + warps < groups) take(next, group + warps);
+  }
+#pragma unroll
+  for (int k = 0; k < TT; k++) {
+    float A = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) A += fabsf(c[k][e]) * (e & 1 ? __high2float(top[e >> 1]) : __low2float(top[e >> 1]));   // (infinite bounds: inf or NaN)
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) A += __shfl_xor_sync(0xffffffffu, A, off);
+    if (lane == 0 && t0 + k < p.T) p.limits[((b * p.T + t0 + k) * p.H + h) * warps + self] = A;
+  }
+}
+
 // A block per row.  The keys between the lowest and the highest are counted in 1024 bins of equal width, the bin of the n-th largest is cut again until it
-// is taken whole or holds one value (of which the lowest positions are taken); usually two rounds.  Then the chosen blocks in order, every warp
-// those of its part of the row.  Latency: keys in shared memory where they fit.
+// is taken whole or holds one value (of which the lowest positions are taken); usually two rounds.  Where the lowest score taken and the highest
+// one left lie closer than the rounding of the scores, those in question are summed again in 64 bits and chosen from once more.  Then the
+// chosen blocks in order, every warp those of its part of the row.  Latency: keys in shared memory where they fit.
 constexpr int PICK_THREADS = 512, PICK_WARPS = PICK_THREADS / 32, PICK_BINS = 1024, PICK_KEPT = 16384;
-__global__ void __launch_bounds__(PICK_THREADS) block_pick_kernel(SelectParams p, bool kept) {
+__global__ void __launch_bounds__(PICK_THREADS) block_pick_kernel(SelectParams p, bool kept, int warps) {
   extern __shared__ uint32_t s_keys[];
   __shared__ unsigned s_bins[PICK_BINS], s_a[PICK_WARPS], s_b[PICK_WARPS], s_c[PICK_WARPS], s_found[3];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.x, t = row / p.H % p.T, b = row / p.H / p.T;
+  const int h = (int)(row % p.H);
   pdl_wait();
   pdl_trigger();
   const int seen = visible_blocks(p, b, (int)t);
-  const uint32_t* in = p.keys + row * p.nb;
+  uint32_t* stored = p.keys + row * p.nb;
   int32_t* ids = p.ids + row * p.n;
   for (int i = min(p.n, seen) + tid; i < p.n; i += PICK_THREADS) ids[i] = -1;
   if (seen <= p.n) {   // all of them
     for (int i = tid; i < seen; i += PICK_THREADS) ids[i] = i;
     return;
   }
-  auto key = [&](int j) { return kept ? s_keys[j] : in[j]; };
+  auto key = [&](int j) { return kept ? s_keys[j] : stored[j]; };
+  auto put = [&](int j, uint32_t k) {
+    if (kept) s_keys[j] = k;
+    else stored[j] = k;
+  };
+  auto value = [](uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k); };
+  // lowest, highest and sum over the block, to every thread
+  auto range = [&](uint32_t& lo, uint32_t& hi, unsigned& n) {
+    lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi), n = __reduce_add_sync(0xffffffffu, n);
+    __syncthreads();
+    if (lane == 0) s_a[warp] = lo, s_b[warp] = hi, s_c[warp] = n;
+    __syncthreads();
+    lo = __reduce_min_sync(0xffffffffu, s_a[lane % PICK_WARPS]), hi = __reduce_max_sync(0xffffffffu, s_b[lane % PICK_WARPS]);
+    n = __reduce_add_sync(0xffffffffu, lane < PICK_WARPS ? s_c[lane] : 0u);
+  };
+  float A = 0.0f;
+  for (int i = tid; i < warps; i += PICK_THREADS) {
+    const float a = p.limits[row * warps + i];
+    A = a <= 3.0e38f ? fmaxf(A, a) : INFINITY;
+    if (!(A < INFINITY)) break;
+  }
   uint32_t lo = 0xffffffffu, hi = 0;   // extremes of the keys that are not FORCED
   unsigned forced = 0;
   for (int j0 = tid; j0 < seen; j0 += 8 * PICK_THREADS) {
     uint32_t k[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) k[i] = in[min(j0 + i * PICK_THREADS, seen - 1)];
+    for (int i = 0; i < 8; i++) k[i] = stored[min(j0 + i * PICK_THREADS, seen - 1)];
 #pragma unroll
     for (int i = 0; i < 8; i++)
       if (j0 + i * PICK_THREADS < seen) {
@@ -191,50 +231,106 @@ __global__ void __launch_bounds__(PICK_THREADS) block_pick_kernel(SelectParams p
         else lo = min(lo, k[i]), hi = max(hi, k[i]);
       }
   }
-  lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi), forced = __reduce_add_sync(0xffffffffu, forced);
-  if (lane == 0) s_a[warp] = lo, s_b[warp] = hi, s_c[warp] = forced;
-  __syncthreads();
+  range(lo, hi, forced);
   {
-    const unsigned x = s_a[lane % PICK_WARPS], y = s_b[lane % PICK_WARPS], z = lane < PICK_WARPS ? s_c[lane] : 0;
-    lo = __reduce_min_sync(0xffffffffu, x), hi = __reduce_max_sync(0xffffffffu, y), forced = __reduce_add_sync(0xffffffffu, z);
+    uint32_t a0 = 0, a1 = __float_as_uint(A);
+    unsigned none = 0;
+    range(a0, a1, none);
+    A = __uint_as_float(a1);
   }
-  // (more blocks than are taken are seen, and the forced ones are at most n: there are others)
-  unsigned want = (unsigned)p.n - forced;   // of the keys in [lo, hi]; those above hi are taken
-  unsigned in_range = 0xffffffffu;
-  while (want > 0 && want != in_range && lo != hi) {
-    const int shift = max(0, 22 - __clz(hi - lo));   // (hi - lo) >> shift < 1024
-    __syncthreads();
-    for (int i = tid; i < PICK_BINS; i += PICK_THREADS) s_bins[i] = 0;
-    __syncthreads();
+  unsigned want;
+  for (bool exact = false;; exact = true) {
+    // (more blocks than are taken are seen, and the forced ones are at most n: there are others)
+    want = (unsigned)p.n - forced;   // of the keys in [lo, hi]; those above hi are taken
+    unsigned in_range = 0xffffffffu;
+    while (want > 0 && want != in_range && lo != hi) {
+      const int shift = max(0, 22 - __clz(hi - lo));   // (hi - lo) >> shift < 1024
+      __syncthreads();
+      for (int i = tid; i < PICK_BINS; i += PICK_THREADS) s_bins[i] = 0;
+      __syncthreads();
+      for (int j = tid; j < seen; j += PICK_THREADS) {
+        const uint32_t k = key(j);
+        if (k >= lo && k <= hi && k != FORCED) atomicAdd(&s_bins[(k - lo) >> shift], 1u);
+      }
+      __syncthreads();
+      // thread i: bins 1023 - 2 i and 1022 - 2 i, from the highest down
+      const unsigned c0 = s_bins[PICK_BINS - 1 - 2 * tid], c1 = s_bins[PICK_BINS - 2 - 2 * tid];
+      unsigned sum = c0 + c1;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const unsigned o = __shfl_up_sync(0xffffffffu, sum, off);
+        if (lane >= off) sum += o;
+      }
+      if (lane == 31) s_a[warp] = sum;
+      __syncthreads();
+      const unsigned before = __reduce_add_sync(0xffffffffu, lane < warp ? s_a[lane & (PICK_WARPS - 1)] : 0u) + sum - c0 - c1;
+      if (before < want && before + c0 >= want) s_found[0] = PICK_BINS - 1 - 2 * tid, s_found[1] = before, s_found[2] = c0;
+      else if (before + c0 < want && before + c0 + c1 >= want) s_found[0] = PICK_BINS - 2 - 2 * tid, s_found[1] = before + c0, s_found[2] = c1;
+      __syncthreads();
+      lo += s_found[0] << shift;
+      hi = min(hi, lo + ((1u << shift) - 1));
+      want -= s_found[1], in_range = s_found[2];
+    }
+    if (exact || want + forced == 0 || forced == (unsigned)p.n) break;
+    // the lowest key taken and the highest one left ([lo, hi] is taken whole, or holds one key and is taken in part)
+    const bool part = lo == hi && want != in_range;
+    uint32_t low = 0xffffffffu, high = 0;
+    unsigned none = 0;
     for (int j = tid; j < seen; j += PICK_THREADS) {
       const uint32_t k = key(j);
-      if (k >= lo && k <= hi && k != FORCED) atomicAdd(&s_bins[(k - lo) >> shift], 1u);
+      if (k == FORCED) continue;
+      if (k >= lo) low = min(low, k);
+      if (k < lo || part) high = max(high, k <= hi ? k : 0u);
     }
+    range(low, high, none);
+    const float margin = 2.5f * (float)(p.G + 14) * 0x1p-24f * A;   // of each of two scores G + 13 roundings and one more to 32 bits, with room
+    const bool odd = !(A < 3.0e38f);
+    if (!odd && !part && value(low) - value(high) > margin) break;
+    if (!odd && part && 0.0f == A) break;   // zeros all
+    const float upper = value(high) + margin, lower = value(low) - margin;
+    // those in question, a warp each; the others are settled
+    double c[8];
+    query_sums(p, b, (int)t, h, lane, c);
+    const uint16_t* bounds = p.bounds + b * p.o_b + h * p.o_h + 8 * lane;
+    lo = 0xffffffffu, hi = 0, forced = 0;
     __syncthreads();
-    // thread i: bins 1023 - 2 i and 1022 - 2 i, from the highest down
-    const unsigned c0 = s_bins[PICK_BINS - 1 - 2 * tid], c1 = s_bins[PICK_BINS - 2 - 2 * tid];
-    unsigned sum = c0 + c1;
+    for (int j0 = 32 * warp; j0 < seen; j0 += PICK_THREADS) {
+      uint32_t k = j0 + lane < seen ? key(j0 + lane) : 0u;
+      bool open = false;
+      if (k != FORCED && k != 0) {
+        const float s = value(k);
+        open = odd || (s <= upper && s >= lower);
+        if (!open) k = s > upper ? FORCED : 0u;
+      }
+      for (unsigned left = __ballot_sync(0xffffffffu, open); left; left &= left - 1) {
+        const int i = __ffs(left) - 1;
+        const uint4 x = *reinterpret_cast<const uint4*>(bounds + (int64_t)(j0 + i) * p.o_j);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        double s = 0.0;
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const unsigned o = __shfl_up_sync(0xffffffffu, sum, off);
-      if (lane >= off) sum += o;
+        for (int e = 0; e < 8; e++)   // (no products of a zero with an infinite bound)
+          if (!(c[e] == 0.0)) s = fma(c[e], (double)__uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16), s);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        const float f = (float)s + 0.0f;
+        if (lane == i) k = f != f ? NOT_A_NUMBER : ord_key(f);
+      }
+      if (j0 + lane < seen) {
+        put(j0 + lane, k);
+        if (k == FORCED) forced++;
+        else lo = min(lo, k), hi = max(hi, k);
+      }
     }
-    if (lane == 31) s_a[warp] = sum;
+    range(lo, hi, forced);
     __syncthreads();
-    const unsigned before = __reduce_add_sync(0xffffffffu, lane < warp ? s_a[lane & (PICK_WARPS - 1)] : 0u) + sum - c0 - c1;
-    if (before < want && before + c0 >= want) s_found[0] = PICK_BINS - 1 - 2 * tid, s_found[1] = before, s_found[2] = c0;
-    else if (before + c0 < want && before + c0 + c1 >= want) s_found[0] = PICK_BINS - 2 - 2 * tid, s_found[1] = before + c0, s_found[2] = c1;
-    __syncthreads();
-    lo += s_found[0] << shift;
-    hi = min(hi, lo + ((1u << shift) - 1));
-    want -= s_found[1], in_range = s_found[2];
   }
   // above hi: taken; in [lo, hi]: the first `want` (all of them, or equal ones)
   const int per = ((seen + PICK_WARPS - 1) / PICK_WARPS + 31) / 32 * 32, j0 = min(seen, warp * per), j1 = min(seen, j0 + per);
+  auto is_above = [&](uint32_t k) { return k == FORCED || (want > 0 ? k > hi : false); };
   unsigned above = 0, inside = 0;
   for (int j = j0 + lane; j < j1; j += 32) {
     const uint32_t k = key(j);
-    if (k > hi) above++;
+    if (is_above(k)) above++;
     else if (k >= lo && want > 0) inside++;
   }
   above = __reduce_add_sync(0xffffffffu, above), inside = __reduce_add_sync(0xffffffffu, inside);
@@ -244,7 +340,7 @@ __global__ void __launch_bounds__(PICK_THREADS) block_pick_kernel(SelectParams p
   unsigned n_above = __reduce_add_sync(0xffffffffu, lane < warp ? s_a[lane & (PICK_WARPS - 1)] : 0u), n_inside = __reduce_add_sync(0xffffffffu, lane < warp ? s_b[lane & (PICK_WARPS - 1)] : 0u);
   for (int j = j0; j < j1; j += 32) {
     const uint32_t k = j + lane < j1 ? key(j + lane) : 0;
-    const bool a = j + lane < j1 && k > hi, i = j + lane < j1 && want > 0 && k >= lo && k <= hi;
+    const bool a = j + lane < j1 && is_above(k), i = j + lane < j1 && !a && want > 0 && k >= lo;
     const unsigned ab = __ballot_sync(0xffffffffu, a), ib = __ballot_sync(0xffffffffu, i), below = (1u << lane) - 1;
     const unsigned i_at = n_inside + __popc(ib & below), at = n_above + __popc(ab & below) + min(i_at, want);
     if (a || (i && i_at < want)) ids[at] = j + lane;
@@ -291,7 +387,9 @@ extern "C" int pk_block_bounds(const pk_tensor* keys, const pk_tensor* lengths, 
   return check_launch("block_bounds");
 }
 
-extern "C" int64_t pk_select_blocks_workspace_bytes(int64_t bs, int64_t T, int64_t H, int64_t n_blocks) { return bs * T * H * n_blocks * 4 + 256; }
+extern "C" int64_t pk_select_blocks_workspace_bytes(int64_t bs, int64_t T, int64_t H, int64_t n_blocks) {
+  return bs * T * H * (n_blocks + 4 * ((n_blocks + 31) / 32)) * 4 + 256;   // keys, and a limit for every warp
+}
 
 extern "C" int pk_select_blocks(const pk_tensor* queries, const pk_tensor* bounds, const pk_tensor* lengths, int64_t block, int64_t sink_blocks,
                                 int64_t local_blocks, const pk_tensor* blocks, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -308,6 +406,7 @@ extern "C" int pk_select_blocks(const pk_tensor* queries, const pk_tensor* bound
   PK_REQUIRE(sink_blocks >= 0 && local_blocks >= 1 && sink_blocks + local_blocks <= n, "at least one local block, and no more sink and local blocks than are selected");
   PK_REQUIRE(nb * block < (1LL << 31) && n < (1LL << 24), "sizes out of range");
   if (bs * T * H == 0) return PK_OK;
+  PK_REQUIRE(nb > 0, "bounds of no block");
   if (!workspace || workspace_bytes < pk_select_blocks_workspace_bytes(bs, T, H, nb)) return fail(PK_ERR_WORKSPACE, "select_blocks: workspace missing or too small");
   SelectParams p = {};
   p.q = (const uint16_t*)queries->data, p.q_b = queries->stride[0], p.q_t = queries->stride[1], p.q_h = queries->stride[2];
@@ -317,17 +416,15 @@ extern "C" int pk_select_blocks(const pk_tensor* queries, const pk_tensor* bound
   const int64_t rows = bs * T * H;
   PK_REQUIRE(rows < (1LL << 31) && bs < 65536, "sizes out of range");
   StageTimer timer(ST_RANK, (cudaStream_t)stream);
-  if (nb > 0) {
-    // tokens share what is read, four at a time; warps up to four blocks of 128 threads per SM, eight keys' blocks a step
-    const int tt = T >= 3 ? 4 : (int)T;
-    const int64_t per_head = (nb + 31) / 32, heads = H * ((T + tt - 1) / tt);
-    const int64_t room = 4LL * sm_count() / (heads * bs) + 1;
-    PK_REQUIRE(heads < 65536, "at most 65535 KV heads x token groups");
-    const dim3 grid((unsigned)(per_head < room ? per_head : room), (unsigned)heads, (unsigned)bs);
-    if (tt == 1) launch_chain(block_score_kernel<1>, grid, dim3(128), 0, (cudaStream_t)stream, p);
-    else if (tt == 2) launch_chain(block_score_kernel<2>, grid, dim3(128), 0, (cudaStream_t)stream, p);
-    else launch_chain(block_score_kernel<4>, grid, dim3(128), 0, (cudaStream_t)stream, p);
-  }
+  // tokens share what is read, four at a time; one wave where that is possible, a warp eight blocks of keys a step
+  const int tt = T >= 3 ? 4 : (int)T;
+  const int64_t per_head = (nb + 31) / 32, heads = H * ((T + tt - 1) / tt), slots = (int64_t)SCORE_CTAS * sm_count() / (heads * bs), room = slots < 1 ? 1 : slots;
+  PK_REQUIRE(heads < 65536, "at most 65535 KV heads x token groups");
+  const dim3 grid((unsigned)(per_head < room ? per_head : room), (unsigned)heads, (unsigned)bs);
+  p.limits = (float*)(p.keys + rows * nb);
+  if (tt == 1) launch_chain(block_score_kernel<1>, grid, dim3(128), 0, (cudaStream_t)stream, p);
+  else if (tt == 2) launch_chain(block_score_kernel<2>, grid, dim3(128), 0, (cudaStream_t)stream, p);
+  else launch_chain(block_score_kernel<4>, grid, dim3(128), 0, (cudaStream_t)stream, p);
   const bool kept = nb <= PICK_KEPT;
   if (kept && nb * 4 > 40 * 1024) {
     static PerDevice opted;
@@ -337,6 +434,6 @@ extern "C" int pk_select_blocks(const pk_tensor* queries, const pk_tensor* bound
       mark_on_device(opted, bit);
     }
   }
-  launch_chain(block_pick_kernel, dim3((unsigned)rows), dim3(PICK_THREADS), kept ? (size_t)nb * 4 : 0, (cudaStream_t)stream, p, kept);
-  return check_launch("select_blocks", nb > 0 ? 2 : 1);
+  launch_chain(block_pick_kernel, dim3((unsigned)rows), dim3(PICK_THREADS), kept ? (size_t)nb * 4 : 0, (cudaStream_t)stream, p, kept, (int)grid.x * 4);
+  return check_launch("select_blocks", 2);
 }

@@ -70,6 +70,24 @@ def test_ties_go_to_the_lower_block():
     assert got.flatten().tolist() == list(range(16)) + [250, 297, 298, 299]
 
 
+@pytest.mark.parametrize("nb,T,n", [(300, 1, 20), (5000, 3, 33), (20000, 1, 7)])
+def test_scores_that_32_bit_sums_confuse(nb, T, n):
+    """Blocks whose channels are permutations of each other: equal scores, which sums in 32 bits tell apart by their order; and a few that
+    are above the others by less than such a sum is off."""
+    from pariskv_b200 import ops
+    g = torch.Generator().manual_seed(nb)
+    base = (torch.randn(128, generator=g) * 1000).to(torch.bfloat16)
+    hi = torch.stack([base[torch.randperm(128, generator=g)] for _ in range(nb)])
+    better = torch.randperm(nb - 20, generator=g)[:n // 2] + 10
+    for i, j in enumerate(better.tolist()):   # the smallest magnitude a little larger: by less than one part in 10^7 of the sum of magnitudes
+        at = hi[j].abs().argmin()
+        hi[j, at] = hi[j, at].abs() + 2.0 ** -6 * (1 + i % 3)
+    bnd = torch.stack((torch.full_like(hi, -3.0), hi), 1).view(1, 1, nb, 2, 128).to(DEV)
+    q = torch.ones(1, T, 2, 128, dtype=torch.bfloat16, device=DEV)
+    got = ops.select_blocks(q, bnd, i32([nb * 16]), n, block=16, sink_blocks=1, local_blocks=1)
+    assert torch.equal(got.cpu(), R.select(q.cpu(), bnd.cpu(), [nb * 16], n, 16, 1, 1))
+
+
 def test_scores_that_are_not_numbers():
     """NaN above all others, -inf and zeros of both signs below; sink and local blocks all the same."""
     from pariskv_b200 import ops
