@@ -11,12 +11,14 @@
 namespace pk {
 namespace {
 
-constexpr int FEW_TILE = 64, FEW_BUFS = 3, FEW_THREADS = 128;
+constexpr int FEW_TILE = 64, FEW_BUFS = 3, FEW_THREADS = 160;   // four warps that share the keys, one that makes the copies
 constexpr int FEW_STAGE = 32768;                    // K 64 x 128, V 64 x 128: halves of 64 channels, rows of 128 bytes
 constexpr int FEW_OS = 136;                         // floats between two rows of a warp's partial: its stores fall into all banks
 constexpr int FEW_SMEM = 1024 + FEW_BUFS * FEW_STAGE;
 static_assert(4 * 8 * FEW_OS * 4 <= FEW_STAGE, "the warps' partials of eight rows take the place of a tile");
 constexpr int FEW_WAIT_LIMIT = 400000;              // (a try waits up to 10 us by itself)
+
+__host__ __device__ constexpr int few_ctas(int rows) { return rows > 16 ? 1 : 2; }   // blocks per SM: by the registers
 
 struct FewParams {
   AttendParams a;
@@ -115,23 +117,23 @@ __device__ __forceinline__ void ldmatrix4t(uint32_t (&r)[4], unsigned addr) {
 // ROWS 8: the eight rows are the upper half of the A operands; in P V the lower half carries what the rounding of P to bf16 left, and the two halves
 // of O are added: 17 bits of each weight for no further product.  ROWS 16, 32: one or two full operands, weights of 8 bits; the sums have them all.
 template <bool TREE, int ROWS>
-__global__ void __launch_bounds__(FEW_THREADS, 2)
+__global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
     attend_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dk,
                       const __grid_constant__ CUtensorMap map_dv, const __grid_constant__ FewParams p) {
   constexpr int MT = ROWS == 32 ? 2 : 1;          // operands of 16 rows
   constexpr bool PAIR = ROWS == 8;
   constexpr int RPT = PAIR ? 1 : 2;               // rows of an operand that a lane's fragments belong to
   extern __shared__ unsigned char dyn[];
-  __shared__ __align__(8) unsigned long long bars[FEW_BUFS];
+  __shared__ __align__(8) unsigned long long bars[2 * FEW_BUFS];
   __shared__ float s_m[4][ROWS], s_l[4][ROWS];
   __shared__ unsigned char s_live[FEW_BUFS][4];   // keys of each warp's sixteen that are seen (tree: by all tokens)
   __shared__ uint32_t s_mask[32], s_bad;
-  __shared__ int s_dead;
+  __shared__ volatile int s_dead;
   __shared__ Place s_place;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-  const unsigned base = (smem_addr(dyn) + 1023) & ~1023u, full = smem_addr(bars);
+  const unsigned base = (smem_addr(dyn) + 1023) & ~1023u, full = smem_addr(bars), empty = full + 8 * FEW_BUFS;
   if (tid == 0) {
-    for (int i = 0; i < FEW_BUFS; i++) mbar_init(full + 8 * i, 1);
+    for (int i = 0; i < FEW_BUFS; i++) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 4);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_dead = 0, s_bad = 0;
   }
@@ -153,59 +155,72 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
   if (blockIdx.x >= shares) return;
   const int64_t first = place.total * blockIdx.x / shares;
   const int count = (int)(place.total * (blockIdx.x + 1) / shares - first);
-  FewCursor<TREE> cur, ahead;
+  FewCursor<TREE> cur;
   cur.start(p, place, first);
-  ahead = cur;
 
-  // ---- copies, by warp 0: a lane per box of keys; `ahead` is the tile to come ----
-  int issued = 0;
-  auto issue = [&]() {
-    const int buf = issued % FEW_BUFS;
-    const unsigned dst = base + buf * FEW_STAGE, mb = full + 8 * buf;
-    int row = 0, live = 0, rows = p.box;   // this lane's box: first row, rows that are seen
-    bool draft = false, mine = false;
-    if (TREE) {
-      draft = ahead.tile == ahead.n - 1;
-      mine = lane == 0;
-      row = draft ? 0 : ahead.tile * FEW_TILE;
-      rows = FEW_TILE;
-      live = draft ? p.a.T : min(FEW_TILE, ahead.len - row);
-    } else {
-      const int per = FEW_TILE / p.box;
-      if (lane < per) {
-        const int64_t at = (int64_t)ahead.tile * FEW_TILE + lane * p.box;   // in the item's list of rows
-        const int i = (int)(at / p.a.block);
-        const int id = i < p.a.n ? p.a.blocks[(((int64_t)ahead.b * p.a.T + ahead.t) * p.a.H + ahead.h) * p.a.n + i] : -1;
-        const int64_t r = (int64_t)id * p.a.block + at % p.a.block;
-        live = id < 0 ? 0 : (int)max((int64_t)0, min((int64_t)p.box, ahead.len - r));
-        row = (int)(live > 0 ? r : 0), mine = live > 0;
-      }
+  bool dead = false;   // a wait has run out: no more waiting, the rows come out as NaN
+  auto wait = [&](unsigned mb, unsigned parity) {
+    for (int it = 0; !dead; it++) {
+      if (mbar_try(mb, parity)) break;
+      if (it >= FEW_WAIT_LIMIT || s_dead) dead = true, s_dead = 1;
     }
-    // a warp's sixteen keys lie in one box
-    const int box_of = TREE ? 0 : lane * 16 / p.box, off = TREE ? lane * 16 : lane * 16 % p.box;
-    const int l = __shfl_sync(0xffffffffu, live, box_of & 31);
-    if (lane < 4) s_live[buf][lane] = (unsigned char)max(0, min(16, l - off));
-    const unsigned boxes = __popc(__ballot_sync(0xffffffffu, mine));
-    const unsigned keys = TREE && draft ? 32 : rows;
     __syncwarp();
-    if (lane == 0) mbar_expect(mb, boxes * keys * 512);
-    __syncwarp();
-    if (mine) {
-      const CUtensorMap *mk = TREE && draft ? &map_dk : &map_k, *mv = TREE && draft ? &map_dv : &map_v;
-#pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const unsigned to = dst + half * (FEW_STAGE / 4) + lane * p.box * 128;
-        tma_load4(to, mk, 64 * half, row, ahead.h, ahead.b, mb);
-        tma_load4(to + FEW_STAGE / 2, mv, 64 * half, row, ahead.h, ahead.b, mb);
-      }
-    }
-    issued++;
-    ahead.step(p);
   };
-  if (warp == 0)
-    for (int i = 0; i < FEW_BUFS && i < count; i++) issue();
 
-  bool dead = false;
+  if (warp == 4) {
+    // ---- copies: a lane per box of keys ----
+    const int per = TREE ? 1 : FEW_TILE / p.box;   // boxes of a tile
+    int issued = 0;
+    // the block of this lane's box of the tile that `cur` is at
+    auto listed = [&]() -> int {
+      const int i = TREE ? 0 : (cur.tile * FEW_TILE + lane * p.box) / p.a.block;
+      return !TREE && lane < per && i < p.a.n ? p.a.blocks[(((int64_t)cur.b * p.a.T + cur.t) * p.a.H + cur.h) * p.a.n + i] : -1;
+    };
+    int id = listed();
+    for (; issued < count; issued++) {
+      const int buf = issued % FEW_BUFS;
+      const unsigned dst = base + buf * FEW_STAGE, mb = full + 8 * buf;
+      if (issued >= FEW_BUFS) wait(empty + 8 * buf, (unsigned)(issued / FEW_BUFS - 1) & 1);
+      if (__any_sync(0xffffffffu, dead)) break;
+      int row = 0, live = 0;   // this lane's box: first row, rows that are seen
+      const bool draft = TREE && cur.tile == cur.n - 1;
+      if (TREE) {
+        row = draft ? 0 : cur.tile * FEW_TILE;
+        live = lane > 0 ? 0 : draft ? p.a.T : min(FEW_TILE, cur.len - row);
+      } else if (id >= 0) {
+        const int64_t r = (int64_t)id * p.a.block + (cur.tile * FEW_TILE + lane * p.box) % p.a.block;
+        live = (int)max((int64_t)0, min((int64_t)p.box, cur.len - r));
+        row = (int)(live > 0 ? r : 0);
+      }
+      // a warp's sixteen keys lie in one box
+      const int box_of = TREE ? 0 : lane * 16 / p.box, off = TREE ? lane * 16 : lane * 16 % p.box;
+      const int l = __shfl_sync(0xffffffffu, live, box_of & 31);
+      if (lane < 4) s_live[buf][lane] = (unsigned char)max(0, min(16, l - off));
+      const unsigned boxes = __popc(__ballot_sync(0xffffffffu, live > 0));
+      const unsigned keys = draft ? 32 : TREE ? FEW_TILE : p.box;
+      __syncwarp();
+      if (lane == 0) mbar_expect(mb, boxes * keys * 512);
+      __syncwarp();
+      if (live > 0) {
+        const CUtensorMap *mk = draft ? &map_dk : &map_k, *mv = draft ? &map_dv : &map_v;
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          const unsigned to = dst + half * (FEW_STAGE / 4) + lane * p.box * 128;
+          tma_load4(to, mk, 64 * half, row, cur.h, cur.b, mb);
+          tma_load4(to + FEW_STAGE / 2, mv, 64 * half, row, cur.h, cur.b, mb);
+        }
+      }
+      if (issued + 1 < count) {
+        cur.step(p);
+        id = listed();
+      }
+    }
+    if (s_dead)   // what is under way has to land before the block ends
+      for (int i = issued < FEW_BUFS ? 0 : issued - FEW_BUFS; i < issued; i++)
+        for (int it = 0; it < FEW_WAIT_LIMIT && !mbar_try(full + 8 * (i % FEW_BUFS), (unsigned)(i / FEW_BUFS & 1)); it++) {}
+    return;
+  }
+
   constexpr int OUT_ROWS = PAIR ? 8 : ROWS;
   const int Hq = p.a.H * p.a.G;
   const float scale = p.a.scale_log2;
@@ -237,7 +252,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
         const unsigned bits = __ballot_sync(0xffffffffu, lane < p.a.T && p.a.mask[cur.b * p.a.m_b + t * p.a.m_t + lane * p.a.m_j] != 0);
         if (lane == 0) s_mask[t] = bits;
       }
-      __syncthreads();
+      named_barrier(1, 128);
     }
     float o[MT][16][4], m[MT][RPT], l[MT][RPT];
 #pragma unroll
@@ -249,9 +264,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
     }
     for (int j = 0; j < seg; j++, k++) {
       const int buf = k % FEW_BUFS;
-      for (int it = 0; !dead && !mbar_try(full + 8 * buf, (unsigned)(k / FEW_BUFS & 1)); it++)
-        if (it >= FEW_WAIT_LIMIT) dead = true, s_dead = 1;
-      __syncwarp();
+      wait(full + 8 * buf, (unsigned)(k / FEW_BUFS & 1));
       const int live = s_live[buf][warp];
       const bool draft = has_drafts && j == seg - 1;
       if (live > 0) {   // warp-uniform
@@ -349,8 +362,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
           }
         }
       }
-      __syncthreads();   // the stage may be filled again; that of the segment's last tile first serves the warps' partials
-      if (j < seg - 1 && warp == 0 && issued < count && !s_dead) issue();
+      __syncwarp();
+      if (j < seg - 1 && lane == 0) mbar_arrive1(empty + 8 * buf);   // (the stage of the segment's last tile first serves the warps' partials)
     }
     // ---- the four warps' shares of the segment ----
     float* s_o = reinterpret_cast<float*>(dyn + (base - smem_addr(dyn)) + (k - 1) % FEW_BUFS * FEW_STAGE);   // [4][8][FEW_OS]
@@ -362,7 +375,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
         l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 2);
         if (t4 == 0) s_m[warp][16 * mt + 8 * e + g] = m[mt][e] * scale, s_l[warp][16 * mt + 8 * e + g] = l[mt][e];
       }
-    __syncthreads();
+    named_barrier(1, 128);
     const uint32_t bad = has_drafts ? s_bad : 0;
     float* rec = whole ? nullptr : p.records + (2 * (int64_t)blockIdx.x + (seg_first == 0)) * (OUT_ROWS * 130);
 #pragma unroll
@@ -379,7 +392,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
           if (PAIR) v.x += o[mt][n][2], v.y += o[mt][n][3];
           *reinterpret_cast<float2*>(to + 8 * n) = make_float2(v.x * f, v.y * f);
         }
-        __syncthreads();
+        named_barrier(1, 128);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           const int row = 8 * round + i;
@@ -408,18 +421,16 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
             }
           }
         }
-        __syncthreads();
+        named_barrier(1, 128);
       }
     }
     if (has_drafts && tid == 0) s_bad = 0;
     fence_async();
-    __syncthreads();
-    if (warp == 0 && issued < count && !s_dead) issue();
+    __syncwarp();
+    if (lane == 0) mbar_arrive1(empty + 8 * ((k - 1) % FEW_BUFS));
+    if (TREE) named_barrier(1, 128);   // the marks are clear
     for (int j = 0; j < seg; j++) cur.step(p);
   }
-  if (s_dead && tid == 0)   // what is under way has to land before the block ends
-    for (int i = issued < FEW_BUFS ? 0 : issued - FEW_BUFS; i < issued; i++)
-      for (int it = 0; it < FEW_WAIT_LIMIT && !mbar_try(full + 8 * (i % FEW_BUFS), (unsigned)(i / FEW_BUFS & 1)); it++) {}
 }
 
 // A block per query row: the records of the blocks that share its item, in the order of the tiles.
@@ -455,7 +466,7 @@ __global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ 
 
 template <bool TREE, int ROWS>
 int launch(const FewParams& p, const CUtensorMap (&maps)[4], int64_t most, const char* what, cudaStream_t st) {
-  const int64_t slots = 2 * (int64_t)sm_count();
+  const int64_t slots = (int64_t)few_ctas(ROWS) * sm_count();
   const int blocks = (int)(most < slots ? most : slots);
   static PerDevice opted;
   if (const unsigned long long bit = first_on_device(opted)) {
