@@ -568,8 +568,9 @@ int64_t pk_block_attention_workspace_bytes(int64_t bs, int64_t T, int64_t Hq, in
 int pk_block_attention(const pk_tensor* queries, const pk_tensor* keys, const pk_tensor* values, const pk_tensor* blocks,
                        const pk_tensor* lengths, int64_t block, float scale, const pk_tensor* out, const pk_tensor* lse,
                        void* workspace, int64_t workspace_bytes, void* stream);
+int64_t pk_gemv_w4_workspace_bytes(int64_t T, int64_t O, int64_t I, int64_t group, int gated);   /* 0: none */
 int pk_gemv_w4(const pk_tensor* weight, const pk_tensor* scales, const pk_tensor* offsets, const pk_tensor* x,
-               const pk_tensor* out, int gated, void* stream);
+               const pk_tensor* out, int gated, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

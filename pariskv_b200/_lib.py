@@ -108,7 +108,8 @@ SIGNATURES = {
     "pk_select_blocks": (_INT, [TP, TP, TP, _I64, _I64, _I64, TP, _VP, _I64, _VP]),
     "pk_block_attention_workspace_bytes": (_I64, [_I64] * 6),
     "pk_block_attention": (_INT, [TP] * 5 + [_I64, _F32, TP, TP, _VP, _I64, _VP]),
-    "pk_gemv_w4": (_INT, [TP] * 5 + [_INT, _VP]),
+    "pk_gemv_w4_workspace_bytes": (_I64, [_I64] * 4 + [_INT]),
+    "pk_gemv_w4": (_INT, [TP] * 5 + [_INT, _VP, _I64, _VP]),
 }
 
 _lib = None

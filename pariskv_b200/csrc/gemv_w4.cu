@@ -1,47 +1,329 @@
 // y = x W^T for a few tokens, W of 4-bit codes c with a scale s (and an offset m) per row and group of columns:
-// W = (c - 8) s, or c s + m.  Products of a group are summed before they are scaled: y = sum over groups s (sum c x) + m (sum x).
-#include "common.cuh"
+//   W = (c - 8) s, or c s + m;   y = sum over groups q of  s_q (sum c x - 8 sum x), or s_q sum c x + m_q sum x
+// The codes become bf16 by their bits alone, 0x4300 | c = 128 + c, and sum (128 + c) x over a group runs on the tensor cores (mma.sync
+// m16n8k16: 16 rows of W, 8 tokens) with fp32 sums; what the 128 and the 8 add is 128 or 136 times the group's sum of x, which is taken off
+// with the group's scale:  y = sum_q s_q D_q + u_q X_q,  D_q = sum (128 + c) x, X_q = sum x, u_q = -136 s_q, or m_q - 128 s_q.  (D_q and u_q X_q cancel
+// to about a sixteenth: four of the 24 bits.)
+//
+// Bounded by the bytes of W.  Sixteen rows are a unit; a box is 256 of its columns, 2 KB that TMA brings with the 128-byte swizzle, a warp's share of
+// a stage of sixteen boxes.  A lane reads a word of 8 codes of rows g and g + 8 and 8 values of x per 32 columns for two products; x lies in
+// shared memory in the order of the codes' bits.  Where rows are long sixteen warps share a unit, where they are short as many units share a
+// stage; the warps' sums meet in shared memory once per unit.  Gated: eight rows of the gate and the eight of the up product they meet are a unit.
+#include <type_traits>
+
+#include "attend.cuh"
+#include "tma.cuh"
 
 namespace pk {
 namespace {
 
-// A warp per (output, token).
-__global__ void __launch_bounds__(128) gemv_w4_kernel(const uint8_t* w, const uint16_t* scales, const uint16_t* offsets, const uint16_t* x,
-                                                      int64_t x_t, uint16_t* out, int n_out, int I, int group, int gated) {
-  pdl_wait();
-  pdl_trigger();
-  const int lane = threadIdx.x & 31, o = blockIdx.x * 4 + (threadIdx.x >> 5), t = blockIdx.y;
-  if (o >= n_out) return;
-  const uint16_t* xt = x + t * x_t;
-  float y[2] = {0.0f, 0.0f};
-  for (int u = 0; u <= gated; u++) {
-    const int64_t row = o + (int64_t)u * n_out;
-    for (int i = 8 * lane; i < I; i += 256) {
-      const uint32_t c = *reinterpret_cast<const uint32_t*>(w + row * (I / 2) + i / 2);
-      float dot = 0.0f, sum = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float v = bf2f(xt[i + j]), code = (float)((c >> 4 * j) & 15);
-        dot += (offsets ? code : code - 8.0f) * v, sum += v;
-      }
-      const int64_t g = row * (I / group) + i / group;
-      y[u] += bf2f(scales[g]) * dot + (offsets ? bf2f(offsets[g]) * sum : 0.0f);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) y[u] += __shfl_xor_sync(0xffffffffu, y[u], off);
-  }
-  if (lane == 0) out[(int64_t)t * n_out + o] = f2bf(gated ? y[0] / (1.0f + __expf(-y[0])) * y[1] : y[0]);
+constexpr int W4_WARPS = 16, W4_THREADS = 32 * W4_WARPS + 32;   // the warps of the products, and one that makes the copies
+constexpr int W4_BOX = 2048, W4_STAGE = W4_WARPS * W4_BOX, W4_STAGES = 3;
+constexpr int W4_WAIT_LIMIT = 400000;
+constexpr int W4_SMEM = 227 * 1024 - 512;   // of a block; 512 bytes of barriers
+
+struct W4Params {
+  const uint8_t* w;
+  const uint16_t *scales, *offsets, *x;
+  int64_t x_t;
+  uint16_t* out;
+  int n_out, I, T, group_log, gated;
+  int units, boxes, kw_log;      // boxes of a unit and slice; 1 << kw_log warps on a unit
+  int slices;                    // parts of the columns, where x does not fit at once
+  int pitch;                     // bytes from one token's x to the next
+  int groups_smem;               // groups of a slice
+  float* partial;                // [units][32][4 NT]: sums of the slices before
+  bool early;
+};
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void tma_load2(unsigned dst, const CUtensorMap* map, int c0, int c1, unsigned mb) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(c0),
+               "r"(c1), "r"(mb)
+               : "memory");
+}
+// codes i and i + 4 of a word as bf16 128 + c
+template <int I>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+  return ((w >> (4 * I)) & 0x000f000fu) | 0x43004300u;
 }
 
-inline bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
+// NT: tokens in eights
+template <int NT>
+__global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ W4Params p) {
+  extern __shared__ unsigned char dyn[];
+  __shared__ __align__(8) unsigned long long bars[2 * W4_STAGES];
+  __shared__ volatile int s_dead;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+  const unsigned base = (smem_addr(dyn) + 1023) & ~1023u, full = smem_addr(bars), empty = full + 8 * W4_STAGES;
+  unsigned char* at_base = dyn + (base - smem_addr(dyn));
+  float* s_red = reinterpret_cast<float*>(at_base + W4_STAGES * W4_STAGE);          // [2][16 warps][32 lanes][4 NT]
+  float* s_sum = s_red + 2 * W4_WARPS * 32 * 4 * NT;                                // [groups][8 NT]: X
+  unsigned char* s_x = reinterpret_cast<unsigned char*>(s_sum + p.groups_smem * 8 * NT);   // [T][pitch]
+  const int kw = 1 << p.kw_log, per_stage = W4_WARPS >> p.kw_log;                   // warps on a unit, units of a stage
+  const int steps = (p.boxes + kw - 1) >> p.kw_log;                                 // stages of a unit
+  const int sets = (p.units + per_stage - 1) / per_stage, mine = ((int)gridDim.x - 1 - (int)blockIdx.x + sets) / (int)gridDim.x;   // sets of units that share stages
+  if (tid == 0) {
+    for (int i = 0; i < W4_STAGES; i++) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, W4_WARPS);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_dead = 0;
+  }
+  if (tid == 32 * W4_WARPS) tma_prefetch_map(&map);
+  __syncthreads();
+  bool dead = false;   // a wait has run out: no more waiting, the outputs come out as NaN
+  auto wait = [&](unsigned mb, unsigned parity) {
+    for (int it = 0; !dead; it++) {
+      if (mbar_try(mb, parity)) break;
+      if (it >= W4_WAIT_LIMIT || s_dead) dead = true, s_dead = 1;
+    }
+    __syncwarp();
+  };
+  const int F = p.n_out;
+  // first row of a unit: of the weights, or of the gate's
+  const int unit_rows = p.gated ? 8 : 16;
+
+  if (warp == W4_WARPS) {
+    // ---- copies: a lane per box, gated two lanes ----
+    if (!p.early) {
+      if (mine > 0 && lane < W4_WARPS) {   // the first rows on their way to L2 while the block waits (a hint: no value is taken before the wait)
+        const int row = (int)blockIdx.x * per_stage * unit_rows + lane;
+        if (row < F) {
+          const unsigned size = (unsigned)min(p.I / 2, W4_STAGE / 16) & ~15u;
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.w + (int64_t)row * (p.I / 2)), "r"(size) : "memory");
+        }
+      }
+      pdl_wait();
+      pdl_trigger();
+    }
+    bool waited = !p.early;
+    const int box = p.gated ? lane & 15 : lane, half = p.gated ? lane >> 4 : 0;
+    int q = 0;
+    for (int slice = 0; slice < p.slices; slice++)
+      for (int i = 0; i < mine; i++) {
+        const int set = (int)blockIdx.x + i * (int)gridDim.x;
+        const int unit = set * per_stage + (box >> p.kw_log);
+        for (int step = 0; step < steps; step++, q++) {
+          const int st = q % W4_STAGES;
+          if (!waited && q == W4_STAGES) pdl_wait(), pdl_trigger(), waited = true;
+          if (q >= W4_STAGES) wait(empty + 8 * st, (unsigned)(q / W4_STAGES - 1) & 1);
+          if (__any_sync(0xffffffffu, dead)) goto done;
+          const int kb = step * kw + (box & (kw - 1)), col = (slice * p.boxes + kb) * 128;   // bytes
+          const bool on = box < W4_WARPS && unit < p.units && kb < p.boxes && col < p.I / 2;
+          const unsigned n = __popc(__ballot_sync(0xffffffffu, on));
+          const unsigned mb = full + 8 * st;
+          if (lane == 0) mbar_expect(mb, n * (p.gated ? W4_BOX / 2 : W4_BOX));
+          __syncwarp();
+          if (on) tma_load2(base + st * W4_STAGE + box * W4_BOX + half * (W4_BOX / 2), &map, col, unit * unit_rows + half * F, mb);
+        }
+      }
+  done:
+    if (s_dead)   // what is under way has to land before the block ends
+      for (int i = q < W4_STAGES ? 0 : q - W4_STAGES; i < q; i++)
+        for (int it = 0; it < W4_WAIT_LIMIT && !mbar_try(full + 8 * (i % W4_STAGES), (unsigned)(i / W4_STAGES & 1)); it++) {}
+    if (!waited) pdl_wait(), pdl_trigger();
+    return;
+  }
+
+  // ---- products ----
+  const int group = 1 << p.group_log, per_box = 256 >> p.group_log, n_groups = p.I >> p.group_log;   // groups of a box, of a row
+  const float zero_code = p.offsets ? 128.0f : 136.0f;
+  struct Scales {
+    float s[2][2], u[2][2];   // [row g, g + 8][group t4, t4 + 4 of the box]
+  };
+  // of this warp's box of a step; read a step ahead
+  auto load_scales = [&](Scales& to, int slice, int i, int step) {
+    const int unit = ((int)blockIdx.x + i * (int)gridDim.x) * per_stage + (warp >> p.kw_log), kb = step * kw + (warp & (kw - 1));
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+      const int row = p.gated ? unit * 8 + g + r * F : unit * 16 + g + 8 * r;
+      const bool row_ok = unit < p.units && i < mine && kb < p.boxes && (p.gated ? unit * 8 + g < F : row < F);
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int in_box = t4 + 4 * e, at = (slice * p.boxes + kb) * per_box + in_box;
+        const bool ok = row_ok && in_box < per_box && at < n_groups;
+        const int64_t idx = (int64_t)row * n_groups + at;
+        to.s[r][e] = ok ? bf2f(p.scales[idx]) : 0.0f;
+        to.u[r][e] = ok && p.offsets ? bf2f(p.offsets[idx]) : 0.0f;
+      }
+    }
+  };
+  if (!p.early) pdl_wait();   // (scales are weights too)
+  Scales next;
+  load_scales(next, 0, 0, 0);
+  if (p.early) pdl_wait();
+  pdl_trigger();
+  int q = 0, n_red = 0;
+  const unsigned x_lane = smem_addr(s_x) + 16 * t4;
+  for (int slice = 0; slice < p.slices; slice++) {
+    // x of the slice into shared memory, eight values of a token at a time: (0, 4), (1, 5), (2, 6), (3, 7); zeros behind the last column
+    const int first_col = slice * p.boxes * 256, eights = p.boxes * 32;
+    if (slice > 0) asm volatile("bar.sync 1, 512;" ::: "memory");   // the last products with the x before
+    for (int i = tid; i < p.T * eights; i += 32 * W4_WARPS) {
+      const int t = i / eights, e = i - t * eights, col = first_col + 8 * e;
+      const uint4 v = col < p.I ? *reinterpret_cast<const uint4*>(p.x + (int64_t)t * p.x_t + col) : make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(s_x + t * p.pitch + 16 * e) =
+          make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+    }
+    asm volatile("bar.sync 1, 512;" ::: "memory");
+    for (int i = tid; i < p.groups_smem * 8 * NT; i += 32 * W4_WARPS) {
+      const int t = i & (8 * NT - 1), q = i / (8 * NT);
+      float sum = 0.0f;
+      if (t < p.T)
+        for (int e = 0; e < group / 8; e++) {
+          const uint4 v = *reinterpret_cast<const uint4*>(s_x + t * p.pitch + (q * group + 8 * e) * 2);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          float s8 = 0.0f;
+#pragma unroll
+          for (int k = 0; k < 4; k++) s8 += __uint_as_float(w[k] << 16) + __uint_as_float(w[k] & 0xffff0000u);
+          sum += s8;
+        }
+      s_sum[i] = sum;
+    }
+    asm volatile("bar.sync 1, 512;" ::: "memory");
+    for (int i = 0; i < mine; i++) {
+      const int unit = ((int)blockIdx.x + i * (int)gridDim.x) * per_stage + (warp >> p.kw_log);
+      float total[NT][4] = {};
+      for (int step = 0; step < steps; step++, q++) {
+        const Scales now = next;
+        const int kb = step * kw + (warp & (kw - 1)), st = q % W4_STAGES;
+        if (step + 1 < steps) load_scales(next, slice, i, step + 1);
+        else if (i + 1 < mine) load_scales(next, slice, i + 1, 0);
+        else load_scales(next, slice + 1, 0, 0);
+        wait(full + 8 * st, (unsigned)(q / W4_STAGES) & 1);
+        if (kb < p.boxes && (slice * p.boxes + kb) * 256 < p.I && unit < p.units) {   // warp-uniform
+          const unsigned w_at = base + st * W4_STAGE + warp * W4_BOX + g * 128 + 4 * t4, x_at = x_lane + kb * 512;
+          auto boxes = [&](auto log) {
+            constexpr int CH = 1 << (decltype(log)::value - 5);   // steps of 32 columns in a group
+#pragma unroll
+            for (int c0 = 0; c0 < 8; c0 += CH) {
+              float d[NT][4] = {};
+#pragma unroll
+              for (int c = c0; c < c0 + CH; c++) {
+                uint32_t w0, w1, b[NT][4];
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w0) : "r"(w_at + ((c ^ g) << 4)) : "memory");
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w1) : "r"(w_at + 1024 + ((c ^ g) << 4)) : "memory");
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                  b[n][0] = b[n][1] = b[n][2] = b[n][3] = 0;
+                  if (g + 8 * n < p.T)
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(b[n][0]), "=r"(b[n][1]), "=r"(b[n][2]), "=r"(b[n][3])
+                                 : "r"(x_at + (g + 8 * n) * p.pitch + 64 * c)
+                                 : "memory");
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                  mma_bf16(d[n], code_pair<0>(w0), code_pair<0>(w1), code_pair<1>(w0), code_pair<1>(w1), b[n][0], b[n][1]);
+                  mma_bf16(d[n], code_pair<2>(w0), code_pair<2>(w1), code_pair<3>(w0), code_pair<3>(w1), b[n][2], b[n][3]);
+                }
+              }
+              const int in_box = c0 / CH, from = (lane & 28) | (in_box & 3);
+              float s[2], u[2];
+#pragma unroll
+              for (int r = 0; r < 2; r++) {
+                s[r] = __shfl_sync(0xffffffffu, now.s[r][in_box >> 2], from);
+                u[r] = p.offsets ? __shfl_sync(0xffffffffu, now.u[r][in_box >> 2], from) : 0.0f;
+                u[r] = fmaf(-zero_code, s[r], u[r]);
+              }
+              const float* X = s_sum + (kb * per_box + in_box) * 8 * NT + 2 * t4;
+#pragma unroll
+              for (int n = 0; n < NT; n++) {
+                const float2 sums = *reinterpret_cast<const float2*>(X + 8 * n);
+#pragma unroll
+                for (int e = 0; e < 4; e++) total[n][e] = fmaf(s[e >> 1], d[n][e], fmaf(u[e >> 1], e & 1 ? sums.y : sums.x, total[n][e]));
+              }
+            }
+          };
+          if (p.group_log == 7) boxes(std::integral_constant<int, 7>());
+          else if (p.group_log == 6) boxes(std::integral_constant<int, 6>());
+          else boxes(std::integral_constant<int, 5>());
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(empty + 8 * st);
+      }
+      // ---- the sums of the unit's warps; one of them finishes it while the others go on ----
+      float* red = s_red + (n_red & 1) * (W4_WARPS * 32 * 4 * NT);
+#pragma unroll
+      for (int n = 0; n < NT; n++) *reinterpret_cast<float4*>(red + ((n * W4_WARPS + warp) * 32 + lane) * 4) = make_float4(total[n][0], total[n][1], total[n][2], total[n][3]);
+      asm volatile("bar.sync 1, 512;" ::: "memory");
+      if ((warp & (kw - 1)) == (n_red & (kw - 1)) && unit < p.units) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int w = 0; w < kw; w++) {
+            const float4 v = *reinterpret_cast<const float4*>(red + ((n * W4_WARPS + (warp & ~(kw - 1)) + w) * 32 + lane) * 4);
+            y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
+          }
+          float4* part = reinterpret_cast<float4*>(p.partial) + ((int64_t)unit * 32 + lane) * NT + n;
+          if (slice > 0) {
+            const float4 v = *part;
+            y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
+          }
+          if (slice + 1 < p.slices) {
+            *part = y;
+          } else {
+            if (s_dead) y.x = y.y = y.z = y.w = NAN;
+            const int t = 8 * n + 2 * t4;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              if (t + e >= p.T) continue;
+              const float lo = e ? y.y : y.x, hi = e ? y.w : y.z;
+              uint16_t* o = p.out + (int64_t)(t + e) * F;
+              if (p.gated) {
+                if (unit * 8 + g < F) o[unit * 8 + g] = f2bf(lo / (1.0f + __expf(-lo)) * hi);
+              } else {
+                if (unit * 16 + g < F) o[unit * 16 + g] = f2bf(lo);
+                if (unit * 16 + g + 8 < F) o[unit * 16 + g + 8] = f2bf(hi);
+              }
+            }
+          }
+        }
+      }
+      n_red++;
+    }
+  }
+}
+
+// How x and the rows are laid out for a product.
+struct W4Plan {
+  int units, boxes, kw_log, slices, pitch, groups_smem, smem;
+};
+W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated) {
+  W4Plan r = {};
+  const int NT = T > 8 ? 2 : 1;
+  r.units = (int)(gated ? (n_out + 7) / 8 : (n_out + 15) / 16);
+  const int all = (int)((I + 255) / 256), fixed = 1024 + W4_STAGES * W4_STAGE + 2 * W4_WARPS * 32 * 16 * NT;
+  for (r.slices = 1;; r.slices++) {
+    r.boxes = (all + r.slices - 1) / r.slices;
+    if (r.boxes > W4_WARPS) r.boxes = (r.boxes + W4_WARPS - 1) / W4_WARPS * W4_WARPS;   // whole stages, but for the last
+    if (r.slices == 1) r.boxes = all;
+    r.pitch = r.boxes * 512 + 64;   // (two tokens fill the banks)
+    r.groups_smem = r.boxes * (256 >> group_log);
+    r.smem = fixed + r.groups_smem * 8 * NT * 4 + (int)T * r.pitch;
+    if (r.smem <= W4_SMEM || r.boxes == 1) break;
+  }
+  r.slices = (all + r.boxes - 1) / r.boxes;
+  while ((1 << r.kw_log) < r.boxes && (1 << r.kw_log) < W4_WARPS) r.kw_log++;
+  return r;
+}
 
 }  // namespace
 }  // namespace pk
 
 using namespace pk;
 
+extern "C" int64_t pk_gemv_w4_workspace_bytes(int64_t T, int64_t O, int64_t I, int64_t group, int gated) {
+  if (T < 1 || O < 1 || I < 32 || (group != 32 && group != 64 && group != 128)) return 0;
+  const W4Plan plan = w4_plan(gated ? O / 2 : O, I, T, group == 128 ? 7 : group == 64 ? 6 : 5, gated != 0);
+  return plan.slices > 1 ? (int64_t)plan.units * 32 * 16 * (T > 8 ? 2 : 1) : 0;
+}
+
 extern "C" int pk_gemv_w4(const pk_tensor* weight, const pk_tensor* scales, const pk_tensor* offsets, const pk_tensor* x, const pk_tensor* out,
-                          int gated, void* stream) {
+                          int gated, void* workspace, int64_t workspace_bytes, void* stream) {
   PK_CHECK_TENSOR(weight, PK_U8, 2);
   PK_CHECK_TENSOR(scales, PK_BF16, 2);
   PK_CHECK_TENSOR(x, PK_BF16, 2);
@@ -62,10 +344,34 @@ extern "C" int pk_gemv_w4(const pk_tensor* weight, const pk_tensor* scales, cons
   PK_REQUIRE(is_contig(out) && out->shape[0] == T && out->shape[1] == (gated ? O / 2 : O), "out must be contiguous bf16 [T,O] (O/2 when gated)");
   PK_REQUIRE(aligned16(weight->data) && aligned16(x->data), "weight and x must be 16-byte aligned");
   if (T == 0) return PK_OK;
-  const int n_out = (int)(gated ? O / 2 : O);
+  const int n_out = (int)(gated ? O / 2 : O), group_log = group == 128 ? 7 : group == 64 ? 6 : 5;
+  const W4Plan plan = w4_plan(n_out, I, T, group_log, gated != 0);
+  if (plan.slices > 1 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < pk_gemv_w4_workspace_bytes(T, O, I, group, gated)))
+    return fail(PK_ERR_WORKSPACE, "gemv_w4: workspace missing, misaligned or too small");
+  CUtensorMap map;
+  const auto encode = tensor_map_encoder();
+  const cuuint64_t dims[2] = {(cuuint64_t)(I / 2), (cuuint64_t)O}, strides[1] = {(cuuint64_t)(I / 2)};
+  const cuuint32_t box[2] = {128, gated ? 8u : 16u}, ones[2] = {1, 1};
+  if (!encode || encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, weight->data, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return fail(PK_ERR_CUDA, "gemv_w4: the driver made no tensor map of the weights");
+  W4Params p = {};
+  p.w = (const uint8_t*)weight->data, p.scales = (const uint16_t*)scales->data, p.offsets = offsets ? (const uint16_t*)offsets->data : nullptr;
+  p.x = (const uint16_t*)x->data, p.x_t = x->stride[0], p.out = (uint16_t*)out->data;
+  p.n_out = n_out, p.I = (int)I, p.T = (int)T, p.group_log = group_log, p.gated = gated != 0;
+  p.units = plan.units, p.boxes = plan.boxes, p.kw_log = plan.kw_log, p.slices = plan.slices, p.pitch = plan.pitch, p.groups_smem = plan.groups_smem;
+  p.partial = (float*)workspace, p.early = pdl_early();
+  const int sets = (plan.units + (W4_WARPS >> plan.kw_log) - 1) / (W4_WARPS >> plan.kw_log);
+  const unsigned grid = (unsigned)(sets < sm_count() ? sets : sm_count());
+  static PerDevice opted;
+  if (const unsigned long long bit = first_on_device(opted)) {
+    if (cudaFuncSetAttribute(gemv_w4_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(gemv_w4_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM) != cudaSuccess)
+      return fail(PK_ERR_CUDA, "gemv_w4: %s", cudaGetErrorString(cudaGetLastError()));
+    mark_on_device(opted, bit);
+  }
   StageTimer timer(ST_GEMV, (cudaStream_t)stream);
-  launch_chain(gemv_w4_kernel, dim3((unsigned)((n_out + 3) / 4), (unsigned)T), dim3(128), 0, (cudaStream_t)stream, (const uint8_t*)weight->data,
-               (const uint16_t*)scales->data, offsets ? (const uint16_t*)offsets->data : (const uint16_t*)nullptr, (const uint16_t*)x->data, x->stride[0],
-               (uint16_t*)out->data, n_out, (int)I, (int)group, gated ? 1 : 0);
+  if (T > 8) launch_chain(gemv_w4_kernel<2>, dim3(grid), dim3(W4_THREADS), (size_t)plan.smem, (cudaStream_t)stream, map, p);
+  else launch_chain(gemv_w4_kernel<1>, dim3(grid), dim3(W4_THREADS), (size_t)plan.smem, (cudaStream_t)stream, map, p);
   return check_launch("gemv_w4");
 }

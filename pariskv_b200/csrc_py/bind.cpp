@@ -737,7 +737,12 @@ PyObject* py_gemv_w4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!output(Py_None, &o, &own, *x.t, {x.d.shape[0], gated ? O / 2 : O}, at::kBFloat16) || !same_device({&w, &s, &m}, *x.t)) return nullptr;
   if (own.numel() == 0) return THPVariable_Wrap(own);
   void* st = stream_of(*x.t);
-  const int rc = without_gil([&] { return pk_gemv_w4(w.p(), s.p(), m.p(), x.p(), o.p(), gated != 0, st); });
+  const int64_t groups = s.d.ndim == 2 && s.d.shape[1] > 0 ? s.d.shape[1] : 1;
+  const int64_t bytes = pk_gemv_w4_workspace_bytes(x.d.shape[0], O, 2 * w.d.shape[1], 2 * w.d.shape[1] / groups, gated != 0);
+  at::Tensor ws;
+  if (bytes > 0) ws = empty_on(*x.t, {bytes}, at::kByte);
+  void* scratch = bytes > 0 ? ws.data_ptr() : nullptr;
+  const int rc = without_gil([&] { return pk_gemv_w4(w.p(), s.p(), m.p(), x.p(), o.p(), gated != 0, scratch, bytes, st); });
   if (rc) return raise(rc);
   return THPVariable_Wrap(own);
   PK_PY_END

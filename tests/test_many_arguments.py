@@ -78,7 +78,7 @@ def test_block_attention(change, match):
     refused("pk_block_attention", list({**ATTEND, **change}.values()), match)
 
 
-W4 = dict(w=z(6, 64, dtype=U8), scales=z(6, 2), offsets=None, x=z(3, 128), out=z(3, 6), gated=0, stream=None)
+W4 = dict(w=z(6, 64, dtype=U8), scales=z(6, 2), offsets=None, x=z(3, 128), out=z(3, 6), gated=0, ws=None, ws_bytes=0, stream=None)
 
 
 @pytest.mark.parametrize("change,match", [
