@@ -46,10 +46,11 @@ __device__ __forceinline__ void tma_load2(unsigned dst, const CUtensorMap* map, 
                "r"(c1), "r"(mb)
                : "memory");
 }
-// codes i and i + 4 of a word as bf16 128 + c
-template <int I>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
-  return ((w >> (4 * I)) & 0x000f000fu) | 0x43004300u;
+// codes 0 and 4 of a word as bf16 128 + c
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t mask, uint32_t magic) {   // one instruction: both constants in registers
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
+  return r;
 }
 
 // NT: tokens in eights
@@ -63,7 +64,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
   unsigned char* at_base = dyn + (base - smem_addr(dyn));
   float* s_red = reinterpret_cast<float*>(at_base + W4_STAGES * W4_STAGE);          // [2][16 warps][32 lanes][4 NT]
   float* s_sum = s_red + 2 * W4_WARPS * 32 * 4 * NT;                                // [groups][8 NT]: X
-  unsigned char* s_x = reinterpret_cast<unsigned char*>(s_sum + p.groups_smem * 8 * NT);   // [T][pitch]
+  unsigned char* s_x = reinterpret_cast<unsigned char*>(s_sum + p.groups_smem * 8 * NT);   // [T, and one of zeros][pitch]
   const int kw = 1 << p.kw_log, per_stage = W4_WARPS >> p.kw_log;                   // warps on a unit, units of a stage
   const int steps = (p.boxes + kw - 1) >> p.kw_log;                                 // stages of a unit
   const int sets = (p.units + per_stage - 1) / per_stage, mine = ((int)gridDim.x - 1 - (int)blockIdx.x + sets) / (int)gridDim.x;   // sets of units that share stages
@@ -83,8 +84,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
     __syncwarp();
   };
   const int F = p.n_out;
-  // first row of a unit: of the weights, or of the gate's
-  const int unit_rows = p.gated ? 8 : 16;
+  const int unit_rows = p.gated ? 8 : 16;   // of the weights, or of the gate's
 
   if (warp == W4_WARPS) {
     // ---- copies: a lane per box, gated two lanes ----
@@ -131,40 +131,49 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
   // ---- products ----
   const int group = 1 << p.group_log, per_box = 256 >> p.group_log, n_groups = p.I >> p.group_log;   // groups of a box, of a row
   const float zero_code = p.offsets ? 128.0f : 136.0f;
+  // Scales and offsets of this warp's box, read two boxes ahead: group t4 (and, of eight groups, t4 + 4) of rows g and g + 8.  Behind the last row or group
+  // the last one is read again: the outputs are dropped, x and the codes are zero there.
   struct Scales {
-    float s[2][2], u[2][2];   // [row g, g + 8][group t4, t4 + 4 of the box]
+    uint16_t s[2][2], u[2][2];
   };
-  // of this warp's box of a step; read a step ahead
-  auto load_scales = [&](Scales& to, int slice, int i, int step) {
-    const int unit = ((int)blockIdx.x + i * (int)gridDim.x) * per_stage + (warp >> p.kw_log), kb = step * kw + (warp & (kw - 1));
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-      const int row = p.gated ? unit * 8 + g + r * F : unit * 16 + g + 8 * r;
-      const bool row_ok = unit < p.units && i < mine && kb < p.boxes && (p.gated ? unit * 8 + g < F : row < F);
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const int in_box = t4 + 4 * e, at = (slice * p.boxes + kb) * per_box + in_box;
-        const bool ok = row_ok && in_box < per_box && at < n_groups;
-        const int64_t idx = (int64_t)row * n_groups + at;
-        to.s[r][e] = ok ? bf2f(p.scales[idx]) : 0.0f;
-        to.u[r][e] = ok && p.offsets ? bf2f(p.offsets[idx]) : 0.0f;
-      }
+  int f_slice = 0, f_set = 0, f_step = 0;
+  auto fetch = [&](Scales& to) {
+    if (f_slice == p.slices) return;
+    const int unit = ((int)blockIdx.x + f_set * (int)gridDim.x) * per_stage + (warp >> p.kw_log);
+    const int row0 = min(unit * unit_rows + g, F - 1), row1 = p.gated ? row0 + F : min(row0 + 8, F - 1);
+    const int at = (f_slice * p.boxes + f_step * kw + (warp & (kw - 1))) * per_box + t4;   // (numbers of scales fit 31 bits)
+    const int a0 = min(at, n_groups - 1);
+    to.s[0][0] = p.scales[row0 * n_groups + a0], to.s[1][0] = p.scales[row1 * n_groups + a0];
+    if (p.offsets) to.u[0][0] = p.offsets[row0 * n_groups + a0], to.u[1][0] = p.offsets[row1 * n_groups + a0];
+    if (per_box > 4) {
+      const int a1 = min(at + 4, n_groups - 1);
+      to.s[0][1] = p.scales[row0 * n_groups + a1], to.s[1][1] = p.scales[row1 * n_groups + a1];
+      if (p.offsets) to.u[0][1] = p.offsets[row0 * n_groups + a1], to.u[1][1] = p.offsets[row1 * n_groups + a1];
+    }
+    if (++f_step == steps) {
+      f_step = 0;
+      if (++f_set == mine) f_set = 0, f_slice++;
     }
   };
   if (!p.early) pdl_wait();   // (scales are weights too)
-  Scales next;
-  load_scales(next, 0, 0, 0);
+  Scales next = {}, after = {};
+  fetch(next);
+  fetch(after);
   if (p.early) pdl_wait();
   pdl_trigger();
+  uint32_t mask, magic;
+  asm volatile("mov.b32 %0, 0x000f000f;\n\tmov.b32 %1, 0x43004300;" : "=r"(mask), "=r"(magic));
   int q = 0, n_red = 0;
-  const unsigned x_lane = smem_addr(s_x) + 16 * t4;
+  unsigned x_lane[NT];   // this lane's token; of those that there are not a row of zeros
+#pragma unroll
+  for (int n = 0; n < NT; n++) x_lane[n] = smem_addr(s_x) + min(g + 8 * n, p.T) * p.pitch + 16 * t4;
   for (int slice = 0; slice < p.slices; slice++) {
     // x of the slice into shared memory, eight values of a token at a time: (0, 4), (1, 5), (2, 6), (3, 7); zeros behind the last column
     const int first_col = slice * p.boxes * 256, eights = p.boxes * 32;
     if (slice > 0) asm volatile("bar.sync 1, 512;" ::: "memory");   // the last products with the x before
-    for (int i = tid; i < p.T * eights; i += 32 * W4_WARPS) {
+    for (int i = tid; i < (p.T + (p.T < 8 * NT)) * eights; i += 32 * W4_WARPS) {
       const int t = i / eights, e = i - t * eights, col = first_col + 8 * e;
-      const uint4 v = col < p.I ? *reinterpret_cast<const uint4*>(p.x + (int64_t)t * p.x_t + col) : make_uint4(0, 0, 0, 0);
+      const uint4 v = col < p.I && t < p.T ? *reinterpret_cast<const uint4*>(p.x + (int64_t)t * p.x_t + col) : make_uint4(0, 0, 0, 0);
       *reinterpret_cast<uint4*>(s_x + t * p.pitch + 16 * e) =
           make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
     }
@@ -190,12 +199,11 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
       for (int step = 0; step < steps; step++, q++) {
         const Scales now = next;
         const int kb = step * kw + (warp & (kw - 1)), st = q % W4_STAGES;
-        if (step + 1 < steps) load_scales(next, slice, i, step + 1);
-        else if (i + 1 < mine) load_scales(next, slice, i + 1, 0);
-        else load_scales(next, slice + 1, 0, 0);
+        next = after;
+        fetch(after);
         wait(full + 8 * st, (unsigned)(q / W4_STAGES) & 1);
         if (kb < p.boxes && (slice * p.boxes + kb) * 256 < p.I && unit < p.units) {   // warp-uniform
-          const unsigned w_at = base + st * W4_STAGE + warp * W4_BOX + g * 128 + 4 * t4, x_at = x_lane + kb * 512;
+          const unsigned w_at = base + st * W4_STAGE + warp * W4_BOX + g * 128 + 4 * t4 + 16 * g, x_at = kb * 512;   // chunk 0 of row g, swizzled
           auto boxes = [&](auto log) {
             constexpr int CH = 1 << (decltype(log)::value - 5);   // steps of 32 columns in a group
 #pragma unroll
@@ -204,30 +212,31 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
 #pragma unroll
               for (int c = c0; c < c0 + CH; c++) {
                 uint32_t w0, w1, b[NT][4];
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w0) : "r"(w_at + ((c ^ g) << 4)) : "memory");
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w1) : "r"(w_at + 1024 + ((c ^ g) << 4)) : "memory");
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w0) : "r"(w_at ^ (c << 4)) : "memory");
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w1) : "r"((w_at ^ (c << 4)) + 1024) : "memory");
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                  b[n][0] = b[n][1] = b[n][2] = b[n][3] = 0;
-                  if (g + 8 * n < p.T)
-                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                                 : "=r"(b[n][0]), "=r"(b[n][1]), "=r"(b[n][2]), "=r"(b[n][3])
-                                 : "r"(x_at + (g + 8 * n) * p.pitch + 64 * c)
-                                 : "memory");
+                  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                               : "=r"(b[n][0]), "=r"(b[n][1]), "=r"(b[n][2]), "=r"(b[n][3])
+                               : "r"(x_lane[n] + x_at + 64 * c)
+                               : "memory");
                 }
+                const uint32_t a0 = code_pair(w0, mask, magic), a1 = code_pair(w1, mask, magic), a2 = code_pair(w0 >> 4, mask, magic), a3 = code_pair(w1 >> 4, mask, magic);
+                const uint32_t a4 = code_pair(w0 >> 8, mask, magic), a5 = code_pair(w1 >> 8, mask, magic), a6 = code_pair(w0 >> 12, mask, magic), a7 = code_pair(w1 >> 12, mask, magic);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                  mma_bf16(d[n], code_pair<0>(w0), code_pair<0>(w1), code_pair<1>(w0), code_pair<1>(w1), b[n][0], b[n][1]);
-                  mma_bf16(d[n], code_pair<2>(w0), code_pair<2>(w1), code_pair<3>(w0), code_pair<3>(w1), b[n][2], b[n][3]);
+                  mma_bf16(d[n], a0, a1, a2, a3, b[n][0], b[n][1]);
+                  mma_bf16(d[n], a4, a5, a6, a7, b[n][2], b[n][3]);
                 }
               }
               const int in_box = c0 / CH, from = (lane & 28) | (in_box & 3);
               float s[2], u[2];
 #pragma unroll
               for (int r = 0; r < 2; r++) {
-                s[r] = __shfl_sync(0xffffffffu, now.s[r][in_box >> 2], from);
-                u[r] = p.offsets ? __shfl_sync(0xffffffffu, now.u[r][in_box >> 2], from) : 0.0f;
-                u[r] = fmaf(-zero_code, s[r], u[r]);
+                // scale and offset of a row in one word
+                const uint32_t both = __shfl_sync(0xffffffffu, (uint32_t)now.s[r][in_box >> 2] << 16 | now.u[r][in_box >> 2], from);
+                s[r] = __uint_as_float(both & 0xffff0000u);
+                u[r] = fmaf(-zero_code, s[r], __uint_as_float(both << 16));
               }
               const float* X = s_sum + (kb * per_box + in_box) * 8 * NT + 2 * t4;
 #pragma unroll
@@ -303,7 +312,7 @@ W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated) {
     if (r.slices == 1) r.boxes = all;
     r.pitch = r.boxes * 512 + 64;   // (two tokens fill the banks)
     r.groups_smem = r.boxes * (256 >> group_log);
-    r.smem = fixed + r.groups_smem * 8 * NT * 4 + (int)T * r.pitch;
+    r.smem = fixed + r.groups_smem * 8 * NT * 4 + (int)(T + (T < 8 * NT)) * r.pitch;
     if (r.smem <= W4_SMEM || r.boxes == 1) break;
   }
   r.slices = (all + r.boxes - 1) / r.boxes;
@@ -340,6 +349,7 @@ extern "C" int pk_gemv_w4(const pk_tensor* weight, const pk_tensor* scales, cons
   PK_REQUIRE(x->shape[1] == I && x->stride[1] == 1 && (T <= 1 || (x->stride[0] >= 0 && x->stride[0] % 8 == 0)), "x must be bf16 [T,I] with a unit inner stride and a row stride that is a multiple of 8");
   PK_REQUIRE(T <= 16, "at most 16 tokens");
   PK_REQUIRE(I <= 32768 && O >= 1 && O < (1LL << 30), "at most 32768 columns");
+  PK_REQUIRE(O * groups < (1LL << 31), "sizes out of range");
   PK_REQUIRE(!gated || O % 2 == 0, "a gated product takes an even number of rows");
   PK_REQUIRE(is_contig(out) && out->shape[0] == T && out->shape[1] == (gated ? O / 2 : O), "out must be contiguous bf16 [T,O] (O/2 when gated)");
   PK_REQUIRE(aligned16(weight->data) && aligned16(x->data), "weight and x must be 16-byte aligned");
