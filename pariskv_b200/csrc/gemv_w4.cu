@@ -1,9 +1,9 @@
 // y = x W^T for a few tokens, W of 4-bit codes c with a scale s (and an offset m) per row and group of columns:
 //   W = (c - 8) s, or c s + m;   y = sum over groups q of  s_q (sum c x - 8 sum x), or s_q sum c x + m_q sum x
 // The codes become bf16 by their bits alone, 0x4300 | c = 128 + c, and sum (128 + c) x over a group runs on the tensor cores (mma.sync
-// m16n8k16: 16 rows of W, 8 tokens) with fp32 sums; what the 128 and the 8 add is 128 or 136 times the group's sum of x, which is taken off
-// with the group's scale:  y = sum_q s_q D_q + u_q X_q,  D_q = sum (128 + c) x, X_q = sum x, u_q = -136 s_q, or m_q - 128 s_q.  (D_q and u_q X_q cancel
-// to about a sixteenth: four of the 24 bits.)
+// m16n8k16: 16 rows of W, 8 tokens) with fp32 sums; what the 128 and the 8 add is 128 or 136 times the group's sum of x, so the sum starts from
+// that, negative:  y = sum_q s_q (sum (128 + c) x - 136 X_q), or s_q (sum (128 + c) x - 128 X_q) + m_q X_q,  X_q = sum x.  (The two cancel to about a
+// sixteenth: four of the 24 bits.)
 //
 // Bounded by the bytes of W.  Sixteen rows are a unit; a box is 256 of its columns, 2 KB that TMA brings with the 128-byte swizzle, a warp's share of
 // a stage of sixteen boxes.  A lane reads a word of 8 codes of rows g and g + 8 and 8 values of x per 32 columns for two products; x lies in
@@ -18,7 +18,9 @@ namespace pk {
 namespace {
 
 constexpr int W4_WARPS = 16, W4_THREADS = 32 * W4_WARPS + 32;   // the warps of the products, and one that makes the copies
-constexpr int W4_BOX = 2048, W4_STAGE = W4_WARPS * W4_BOX, W4_STAGES = 3;
+constexpr int W4_PIECE = 2048;                  // 256 columns of 16 rows
+__host__ __device__ constexpr int w4_stages(int sub) { return sub == 1 ? 3 : 2; }
+constexpr int W4_LONG = 8;                       // stages of 64 KB per SM from which on boxes are of 512 columns
 constexpr int W4_WAIT_LIMIT = 400000;
 constexpr int W4_SMEM = 227 * 1024 - 512;   // of a block; 512 bytes of barriers
 
@@ -53,9 +55,10 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t mask, uint32_
   return r;
 }
 
-// NT: tokens in eights
-template <int NT>
+// NT: tokens in eights; SUB: pieces of 256 columns in a box
+template <int NT, int SUB>
 __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ W4Params p) {
+  constexpr int W4_BOX = SUB * W4_PIECE, W4_STAGE = W4_WARPS * W4_BOX, W4_STAGES = w4_stages(SUB), E = 2 * SUB;   // E: scales of a row that a lane holds
   extern __shared__ unsigned char dyn[];
   __shared__ __align__(8) unsigned long long bars[2 * W4_STAGES];
   __shared__ volatile int s_dead;
@@ -63,7 +66,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
   const unsigned base = (smem_addr(dyn) + 1023) & ~1023u, full = smem_addr(bars), empty = full + 8 * W4_STAGES;
   unsigned char* at_base = dyn + (base - smem_addr(dyn));
   float* s_red = reinterpret_cast<float*>(at_base + W4_STAGES * W4_STAGE);          // [2][16 warps][32 lanes][4 NT]
-  float* s_sum = s_red + 2 * W4_WARPS * 32 * 4 * NT;                                // [groups][8 NT]: X
+  float* s_sum = s_red + 2 * W4_WARPS * 32 * 4 * NT;                                // [groups][8 NT]: -136 X, or -128 X
   unsigned char* s_x = reinterpret_cast<unsigned char*>(s_sum + p.groups_smem * 8 * NT);   // [T, and one of zeros][pitch]
   const int kw = 1 << p.kw_log, per_stage = W4_WARPS >> p.kw_log;                   // warps on a unit, units of a stage
   const int steps = (p.boxes + kw - 1) >> p.kw_log;                                 // stages of a unit
@@ -92,7 +95,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
       if (mine > 0 && lane < W4_WARPS) {   // the first rows on their way to L2 while the block waits (a hint: no value is taken before the wait)
         const int row = (int)blockIdx.x * per_stage * unit_rows + lane;
         if (row < F) {
-          const unsigned size = (unsigned)min(p.I / 2, W4_STAGE / 16) & ~15u;
+          const unsigned size = (unsigned)min(p.I / 2, 2048) & ~15u;
           asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.w + (int64_t)row * (p.I / 2)), "r"(size) : "memory");
         }
       }
@@ -111,13 +114,17 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
           if (!waited && q == W4_STAGES) pdl_wait(), pdl_trigger(), waited = true;
           if (q >= W4_STAGES) wait(empty + 8 * st, (unsigned)(q / W4_STAGES - 1) & 1);
           if (__any_sync(0xffffffffu, dead)) goto done;
-          const int kb = step * kw + (box & (kw - 1)), col = (slice * p.boxes + kb) * 128;   // bytes
+          const int kb = step * kw + (box & (kw - 1)), col = (slice * p.boxes + kb) * (128 * SUB);   // bytes
           const bool on = box < W4_WARPS && unit < p.units && kb < p.boxes && col < p.I / 2;
-          const unsigned n = __popc(__ballot_sync(0xffffffffu, on));
+          const int pieces = !on ? 0 : SUB == 1 || col + 128 >= p.I / 2 ? 1 : 2;
+          const unsigned n = __reduce_add_sync(0xffffffffu, (unsigned)pieces);
           const unsigned mb = full + 8 * st;
-          if (lane == 0) mbar_expect(mb, n * (p.gated ? W4_BOX / 2 : W4_BOX));
+          if (lane == 0) mbar_expect(mb, n * (p.gated ? W4_PIECE / 2 : W4_PIECE));
           __syncwarp();
-          if (on) tma_load2(base + st * W4_STAGE + box * W4_BOX + half * (W4_BOX / 2), &map, col, unit * unit_rows + half * F, mb);
+#pragma unroll
+          for (int sb = 0; sb < SUB; sb++)
+            if (sb < pieces)
+              tma_load2(base + st * W4_STAGE + box * W4_BOX + sb * W4_PIECE + half * (W4_PIECE / 2), &map, col + 128 * sb, unit * unit_rows + half * F, mb);
         }
       }
   done:
@@ -129,31 +136,37 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
   }
 
   // ---- products ----
-  const int group = 1 << p.group_log, per_box = 256 >> p.group_log, n_groups = p.I >> p.group_log;   // groups of a box, of a row
-  const float zero_code = p.offsets ? 128.0f : 136.0f;
-  // Scales and offsets of this warp's box, read two boxes ahead: group t4 (and, of eight groups, t4 + 4) of rows g and g + 8.  Behind the last row or group
+  const int group = 1 << p.group_log, per_box = (256 * SUB) >> p.group_log, n_groups = p.I >> p.group_log;   // groups of a box, of a row
+  // Scales and offsets of this warp's box, read two boxes ahead: groups t4, t4 + 4 .. of rows g and g + 8.  Behind the last row or group
   // the last one is read again: the outputs are dropped, x and the codes are zero there.
   struct Scales {
-    uint16_t s[2][2], u[2][2];
+    uint16_t s[2][E], u[2][E];
   };
-  int f_slice = 0, f_set = 0, f_step = 0;
+  const bool with_offsets = p.offsets != nullptr;
+  int f_slice = 0, f_set = 0, f_step = 0, f_at = (warp & (kw - 1)) * per_box + t4, f_i0 = 0, f_i1 = 0;   // (numbers of scales fit 31 bits)
   auto fetch = [&](Scales& to) {
     if (f_slice == p.slices) return;
-    const int unit = ((int)blockIdx.x + f_set * (int)gridDim.x) * per_stage + (warp >> p.kw_log);
-    const int row0 = min(unit * unit_rows + g, F - 1), row1 = p.gated ? row0 + F : min(row0 + 8, F - 1);
-    const int at = (f_slice * p.boxes + f_step * kw + (warp & (kw - 1))) * per_box + t4;   // (numbers of scales fit 31 bits)
-    const int a0 = min(at, n_groups - 1);
-    to.s[0][0] = p.scales[row0 * n_groups + a0], to.s[1][0] = p.scales[row1 * n_groups + a0];
-    if (p.offsets) to.u[0][0] = p.offsets[row0 * n_groups + a0], to.u[1][0] = p.offsets[row1 * n_groups + a0];
-    if (per_box > 4) {
-      const int a1 = min(at + 4, n_groups - 1);
-      to.s[0][1] = p.scales[row0 * n_groups + a1], to.s[1][1] = p.scales[row1 * n_groups + a1];
-      if (p.offsets) to.u[0][1] = p.offsets[row0 * n_groups + a1], to.u[1][1] = p.offsets[row1 * n_groups + a1];
+    if (f_step == 0) {
+      const int unit = ((int)blockIdx.x + f_set * (int)gridDim.x) * per_stage + (warp >> p.kw_log);
+      const int row0 = min(unit * unit_rows + g, F - 1), row1 = p.gated ? row0 + F : min(row0 + 8, F - 1);
+      f_i0 = row0 * n_groups, f_i1 = row1 * n_groups;
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      if (e == 0 || 4 * e < per_box) {
+        const int a = min(f_at + 4 * e, n_groups - 1);
+        to.s[0][e] = p.scales[f_i0 + a], to.s[1][e] = p.scales[f_i1 + a];
+        if (with_offsets) to.u[0][e] = p.offsets[f_i0 + a], to.u[1][e] = p.offsets[f_i1 + a];
+      }
+    if (steps == 1 && p.slices == 1) {
+      if (++f_set == mine) f_slice++;
+      return;
     }
     if (++f_step == steps) {
       f_step = 0;
       if (++f_set == mine) f_set = 0, f_slice++;
     }
+    f_at = (f_slice * p.boxes + f_step * kw + (warp & (kw - 1))) * per_box + t4;
   };
   if (!p.early) pdl_wait();   // (scales are weights too)
   Scales next = {}, after = {};
@@ -169,7 +182,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
   for (int n = 0; n < NT; n++) x_lane[n] = smem_addr(s_x) + min(g + 8 * n, p.T) * p.pitch + 16 * t4;
   for (int slice = 0; slice < p.slices; slice++) {
     // x of the slice into shared memory, eight values of a token at a time: (0, 4), (1, 5), (2, 6), (3, 7); zeros behind the last column
-    const int first_col = slice * p.boxes * 256, eights = p.boxes * 32;
+    const int first_col = slice * p.boxes * (256 * SUB), eights = p.boxes * (32 * SUB);
     if (slice > 0) asm volatile("bar.sync 1, 512;" ::: "memory");   // the last products with the x before
     for (int i = tid; i < (p.T + (p.T < 8 * NT)) * eights; i += 32 * W4_WARPS) {
       const int t = i / eights, e = i - t * eights, col = first_col + 8 * e;
@@ -190,7 +203,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
           for (int k = 0; k < 4; k++) s8 += __uint_as_float(w[k] << 16) + __uint_as_float(w[k] & 0xffff0000u);
           sum += s8;
         }
-      s_sum[i] = sum;
+      s_sum[i] = sum * (with_offsets ? -128.0f : -136.0f);
     }
     asm volatile("bar.sync 1, 512;" ::: "memory");
     for (int i = 0; i < mine; i++) {
@@ -202,18 +215,24 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
         next = after;
         fetch(after);
         wait(full + 8 * st, (unsigned)(q / W4_STAGES) & 1);
-        if (kb < p.boxes && (slice * p.boxes + kb) * 256 < p.I && unit < p.units) {   // warp-uniform
-          const unsigned w_at = base + st * W4_STAGE + warp * W4_BOX + g * 128 + 4 * t4 + 16 * g, x_at = kb * 512;   // chunk 0 of row g, swizzled
+        if (kb < p.boxes && (slice * p.boxes + kb) * (256 * SUB) < p.I && unit < p.units) {   // warp-uniform
+          const unsigned w_at = base + st * W4_STAGE + warp * W4_BOX + g * 128 + 4 * t4 + 16 * g, x_at = kb * (512 * SUB);   // chunk 0 of row g, swizzled
           auto boxes = [&](auto log) {
             constexpr int CH = 1 << (decltype(log)::value - 5);   // steps of 32 columns in a group
 #pragma unroll
-            for (int c0 = 0; c0 < 8; c0 += CH) {
-              float d[NT][4] = {};
+            for (int c0 = 0; c0 < 8 * SUB; c0 += CH) {
+              const int in_box = c0 / CH, from = (lane & 28) | (in_box & 3);
+              float d[NT][4];   // the sum of c x: it starts from what the rest of the products will have added
+#pragma unroll
+              for (int n = 0; n < NT; n++) {
+                const float2 off = *reinterpret_cast<const float2*>(s_sum + (kb * per_box + in_box) * 8 * NT + 2 * t4 + 8 * n);
+                d[n][0] = d[n][2] = off.x, d[n][1] = d[n][3] = off.y;
+              }
 #pragma unroll
               for (int c = c0; c < c0 + CH; c++) {
                 uint32_t w0, w1, b[NT][4];
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w0) : "r"(w_at ^ (c << 4)) : "memory");
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w1) : "r"((w_at ^ (c << 4)) + 1024) : "memory");
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w0) : "r"((w_at ^ ((c & 7) << 4)) + (c >> 3) * W4_PIECE) : "memory");
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w1) : "r"((w_at ^ ((c & 7) << 4)) + (c >> 3) * W4_PIECE + 1024) : "memory");
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
@@ -229,21 +248,23 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
                   mma_bf16(d[n], a4, a5, a6, a7, b[n][2], b[n][3]);
                 }
               }
-              const int in_box = c0 / CH, from = (lane & 28) | (in_box & 3);
-              float s[2], u[2];
+              float sc[2];
 #pragma unroll
-              for (int r = 0; r < 2; r++) {
-                // scale and offset of a row in one word
-                const uint32_t both = __shfl_sync(0xffffffffu, (uint32_t)now.s[r][in_box >> 2] << 16 | now.u[r][in_box >> 2], from);
-                s[r] = __uint_as_float(both & 0xffff0000u);
-                u[r] = fmaf(-zero_code, s[r], __uint_as_float(both << 16));
-              }
-              const float* X = s_sum + (kb * per_box + in_box) * 8 * NT + 2 * t4;
+              for (int r = 0; r < 2; r++) sc[r] = __uint_as_float(__shfl_sync(0xffffffffu, (uint32_t)now.s[r][in_box >> 2], from) << 16);
 #pragma unroll
-              for (int n = 0; n < NT; n++) {
-                const float2 sums = *reinterpret_cast<const float2*>(X + 8 * n);
+              for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) total[n][e] = fmaf(s[e >> 1], d[n][e], fmaf(u[e >> 1], e & 1 ? sums.y : sums.x, total[n][e]));
+                for (int e = 0; e < 4; e++) total[n][e] = fmaf(sc[e >> 1], d[n][e], total[n][e]);
+              if (with_offsets) {
+                float u[2];
+#pragma unroll
+                for (int r = 0; r < 2; r++) u[r] = __uint_as_float(__shfl_sync(0xffffffffu, (uint32_t)now.u[r][in_box >> 2], from) << 16) * -0x1p-7f;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                  const float2 off = *reinterpret_cast<const float2*>(s_sum + (kb * per_box + in_box) * 8 * NT + 2 * t4 + 8 * n);
+#pragma unroll
+                  for (int e = 0; e < 4; e++) total[n][e] = fmaf(u[e >> 1], e & 1 ? off.y : off.x, total[n][e]);
+                }
               }
             }
           };
@@ -299,25 +320,31 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
 
 // How x and the rows are laid out for a product.
 struct W4Plan {
-  int units, boxes, kw_log, slices, pitch, groups_smem, smem;
+  int sub, units, boxes, kw_log, slices, pitch, groups_smem, smem, sets;
 };
-W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated) {
+W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated, int sub) {
   W4Plan r = {};
   const int NT = T > 8 ? 2 : 1;
+  r.sub = sub;
   r.units = (int)(gated ? (n_out + 7) / 8 : (n_out + 15) / 16);
-  const int all = (int)((I + 255) / 256), fixed = 1024 + W4_STAGES * W4_STAGE + 2 * W4_WARPS * 32 * 16 * NT;
+  const int all = (int)((I + 256 * sub - 1) / (256 * sub)), fixed = 1024 + w4_stages(sub) * W4_WARPS * sub * W4_PIECE + 2 * W4_WARPS * 32 * 16 * NT;
   for (r.slices = 1;; r.slices++) {
     r.boxes = (all + r.slices - 1) / r.slices;
-    if (r.boxes > W4_WARPS) r.boxes = (r.boxes + W4_WARPS - 1) / W4_WARPS * W4_WARPS;   // whole stages, but for the last
-    if (r.slices == 1) r.boxes = all;
-    r.pitch = r.boxes * 512 + 64;   // (two tokens fill the banks)
-    r.groups_smem = r.boxes * (256 >> group_log);
+    if (r.slices > 1 && r.boxes > W4_WARPS) r.boxes = (r.boxes + W4_WARPS - 1) / W4_WARPS * W4_WARPS;   // whole stages, but for the last
+    r.pitch = r.boxes * 512 * sub + 64;   // (two tokens fill the banks)
+    r.groups_smem = r.boxes * ((256 * sub) >> group_log);
     r.smem = fixed + r.groups_smem * 8 * NT * 4 + (int)(T + (T < 8 * NT)) * r.pitch;
     if (r.smem <= W4_SMEM || r.boxes == 1) break;
   }
   r.slices = (all + r.boxes - 1) / r.boxes;
   while ((1 << r.kw_log) < r.boxes && (1 << r.kw_log) < W4_WARPS) r.kw_log++;
+  r.sets = (r.units + (W4_WARPS >> r.kw_log) - 1) / (W4_WARPS >> r.kw_log);
   return r;
+}
+// Boxes of 512 columns, which spread what a box costs besides its products, where an SM has many stages of them all the same.
+W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated) {
+  const W4Plan two = w4_plan(n_out, I, T, group_log, gated, 2);
+  return (int64_t)two.sets * ((two.boxes + (1 << two.kw_log) - 1) >> two.kw_log) >= W4_LONG * (int64_t)sm_count() ? two : w4_plan(n_out, I, T, group_log, gated, 1);
 }
 
 }  // namespace
@@ -371,17 +398,21 @@ extern "C" int pk_gemv_w4(const pk_tensor* weight, const pk_tensor* scales, cons
   p.n_out = n_out, p.I = (int)I, p.T = (int)T, p.group_log = group_log, p.gated = gated != 0;
   p.units = plan.units, p.boxes = plan.boxes, p.kw_log = plan.kw_log, p.slices = plan.slices, p.pitch = plan.pitch, p.groups_smem = plan.groups_smem;
   p.partial = (float*)workspace, p.early = pdl_early();
-  const int sets = (plan.units + (W4_WARPS >> plan.kw_log) - 1) / (W4_WARPS >> plan.kw_log);
-  const unsigned grid = (unsigned)(sets < sm_count() ? sets : sm_count());
-  static PerDevice opted;
-  if (const unsigned long long bit = first_on_device(opted)) {
-    if (cudaFuncSetAttribute(gemv_w4_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(gemv_w4_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM) != cudaSuccess)
-      return fail(PK_ERR_CUDA, "gemv_w4: %s", cudaGetErrorString(cudaGetLastError()));
-    mark_on_device(opted, bit);
-  }
+  const unsigned grid = (unsigned)(plan.sets < sm_count() ? plan.sets : sm_count());
   StageTimer timer(ST_GEMV, (cudaStream_t)stream);
-  if (T > 8) launch_chain(gemv_w4_kernel<2>, dim3(grid), dim3(W4_THREADS), (size_t)plan.smem, (cudaStream_t)stream, map, p);
-  else launch_chain(gemv_w4_kernel<1>, dim3(grid), dim3(W4_THREADS), (size_t)plan.smem, (cudaStream_t)stream, map, p);
+  auto launch = [&](auto nt, auto sub) -> int {
+    constexpr int NT = decltype(nt)::value, SUB = decltype(sub)::value;
+    static PerDevice opted;
+    if (const unsigned long long bit = first_on_device(opted)) {
+      if (cudaFuncSetAttribute(gemv_w4_kernel<NT, SUB>, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM) != cudaSuccess)
+        return fail(PK_ERR_CUDA, "gemv_w4: %s", cudaGetErrorString(cudaGetLastError()));
+      mark_on_device(opted, bit);
+    }
+    launch_chain(gemv_w4_kernel<NT, SUB>, dim3(grid), dim3(W4_THREADS), (size_t)plan.smem, (cudaStream_t)stream, map, p);
+    return PK_OK;
+  };
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  if (const int rc = T > 8 ? (plan.sub == 2 ? launch(Two(), Two()) : launch(Two(), One())) : (plan.sub == 2 ? launch(One(), Two()) : launch(One(), One()))) return rc;
   return check_launch("gemv_w4");
 }
