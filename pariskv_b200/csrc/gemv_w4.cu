@@ -17,9 +17,10 @@
 namespace pk {
 namespace {
 
-constexpr int W4_WARPS = 16, W4_THREADS = 32 * W4_WARPS + 32;   // the warps of the products, and one that makes the copies
+constexpr int W4_WARPS = 16, W4_THREADS = 32 * W4_WARPS + 64;   // the warps of the products, one that makes the copies, one that adds the warps' sums
 constexpr int W4_PIECE = 2048;                  // 256 columns of 16 rows
 __host__ __device__ constexpr int w4_stages(int sub) { return sub == 1 ? 3 : 2; }
+__host__ __device__ constexpr int w4_sums(int nt) { return nt == 1 ? 4 : 2; }   // units whose warps' sums are kept
 constexpr int W4_LONG = 8;                       // stages of 64 KB per SM from which on boxes are of 512 columns
 constexpr int W4_WAIT_LIMIT = 400000;
 constexpr int W4_SMEM = 227 * 1024 - 512;   // of a block; 512 bytes of barriers
@@ -58,21 +59,22 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t mask, uint32_
 // NT: tokens in eights; SUB: pieces of 256 columns in a box
 template <int NT, int SUB>
 __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ W4Params p) {
-  constexpr int W4_BOX = SUB * W4_PIECE, W4_STAGE = W4_WARPS * W4_BOX, W4_STAGES = w4_stages(SUB), E = 2 * SUB;   // E: scales of a row that a lane holds
+  constexpr int W4_BOX = SUB * W4_PIECE, W4_STAGE = W4_WARPS * W4_BOX, W4_STAGES = w4_stages(SUB), SUMS = w4_sums(NT), E = 2 * SUB;   // E: scales of a row that a lane holds
   extern __shared__ unsigned char dyn[];
-  __shared__ __align__(8) unsigned long long bars[2 * W4_STAGES];
+  __shared__ __align__(8) unsigned long long bars[2 * W4_STAGES + 2 * SUMS];
   __shared__ volatile int s_dead;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-  const unsigned base = (smem_addr(dyn) + 1023) & ~1023u, full = smem_addr(bars), empty = full + 8 * W4_STAGES;
+  const unsigned base = (smem_addr(dyn) + 1023) & ~1023u, full = smem_addr(bars), empty = full + 8 * W4_STAGES, sums_full = empty + 8 * W4_STAGES, sums_empty = sums_full + 8 * SUMS;
   unsigned char* at_base = dyn + (base - smem_addr(dyn));
-  float* s_red = reinterpret_cast<float*>(at_base + W4_STAGES * W4_STAGE);          // [2][16 warps][32 lanes][4 NT]
-  float* s_sum = s_red + 2 * W4_WARPS * 32 * 4 * NT;                                // [groups][8 NT]: -136 X, or -128 X
+  float* s_red = reinterpret_cast<float*>(at_base + W4_STAGES * W4_STAGE);          // [SUMS][NT][16 warps][32 lanes][4]
+  float* s_sum = s_red + SUMS * W4_WARPS * 32 * 4 * NT;                                // [groups][8 NT]: -136 X, or -128 X
   unsigned char* s_x = reinterpret_cast<unsigned char*>(s_sum + p.groups_smem * 8 * NT);   // [T, and one of zeros][pitch]
   const int kw = 1 << p.kw_log, per_stage = W4_WARPS >> p.kw_log;                   // warps on a unit, units of a stage
   const int steps = (p.boxes + kw - 1) >> p.kw_log;                                 // stages of a unit
   const int sets = (p.units + per_stage - 1) / per_stage, mine = ((int)gridDim.x - 1 - (int)blockIdx.x + sets) / (int)gridDim.x;   // sets of units that share stages
   if (tid == 0) {
     for (int i = 0; i < W4_STAGES; i++) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, W4_WARPS);
+    for (int i = 0; i < SUMS; i++) mbar_init(sums_full + 8 * i, W4_WARPS), mbar_init(sums_empty + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_dead = 0;
   }
@@ -135,6 +137,58 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
     return;
   }
 
+  if (warp == W4_WARPS + 1) {
+    // ---- the sums of a unit's warps, and what becomes of them ----
+    pdl_wait();
+    pdl_trigger();
+    int n_units = 0;
+    for (int slice = 0; slice < p.slices; slice++)
+      for (int i = 0; i < mine; i++, n_units++) {
+        const int place = n_units % SUMS;
+        wait(sums_full + 8 * place, (unsigned)(n_units / SUMS) & 1);
+        const float* red = s_red + place * (W4_WARPS * 32 * 4 * NT);
+        for (int j = 0; j < per_stage; j++) {
+          const int unit = ((int)blockIdx.x + i * (int)gridDim.x) * per_stage + j;
+          if (unit >= p.units) break;
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+            for (int w = 0; w < kw; w++) {
+              const float4 v = *reinterpret_cast<const float4*>(red + ((n * W4_WARPS + j * kw + w) * 32 + lane) * 4);
+              y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
+            }
+            float4* part = reinterpret_cast<float4*>(p.partial) + ((int64_t)unit * 32 + lane) * NT + n;
+            if (slice > 0) {
+              const float4 v = *part;
+              y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
+            }
+            if (slice + 1 < p.slices) {
+              *part = y;
+              continue;
+            }
+            if (s_dead) y.x = y.y = y.z = y.w = NAN;
+            const int t = 8 * n + 2 * t4;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              if (t + e >= p.T) continue;
+              const float lo = e ? y.y : y.x, hi = e ? y.w : y.z;
+              uint16_t* o = p.out + (int64_t)(t + e) * F;
+              if (p.gated) {
+                if (unit * 8 + g < F) o[unit * 8 + g] = f2bf(lo / (1.0f + __expf(-lo)) * hi);
+              } else {
+                if (unit * 16 + g < F) o[unit * 16 + g] = f2bf(lo);
+                if (unit * 16 + g + 8 < F) o[unit * 16 + g + 8] = f2bf(hi);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(sums_empty + 8 * place);
+      }
+    return;
+  }
+
   // ---- products ----
   const int group = 1 << p.group_log, per_box = (256 * SUB) >> p.group_log, n_groups = p.I >> p.group_log;   // groups of a box, of a row
   // Scales and offsets of this warp's box, read two boxes ahead: groups t4, t4 + 4 .. of rows g and g + 8.  Behind the last row or group
@@ -176,7 +230,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
   pdl_trigger();
   uint32_t mask, magic;
   asm volatile("mov.b32 %0, 0x000f000f;\n\tmov.b32 %1, 0x43004300;" : "=r"(mask), "=r"(magic));
-  int q = 0, n_red = 0;
+  int q = 0, n_units = 0;
   unsigned x_lane[NT];   // this lane's token; of those that there are not a row of zeros
 #pragma unroll
   for (int n = 0; n < NT; n++) x_lane[n] = smem_addr(s_x) + min(g + 8 * n, p.T) * p.pitch + 16 * t4;
@@ -275,45 +329,15 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
         __syncwarp();
         if (lane == 0) mbar_arrive1(empty + 8 * st);
       }
-      // ---- the sums of the unit's warps; one of them finishes it while the others go on ----
-      float* red = s_red + (n_red & 1) * (W4_WARPS * 32 * 4 * NT);
+      // ---- this warp's sums of the unit ----
+      const int place = n_units % SUMS;
+      if (n_units >= SUMS) wait(sums_empty + 8 * place, (unsigned)(n_units / SUMS - 1) & 1);
+      float* red = s_red + place * (W4_WARPS * 32 * 4 * NT);
 #pragma unroll
       for (int n = 0; n < NT; n++) *reinterpret_cast<float4*>(red + ((n * W4_WARPS + warp) * 32 + lane) * 4) = make_float4(total[n][0], total[n][1], total[n][2], total[n][3]);
-      asm volatile("bar.sync 1, 512;" ::: "memory");
-      if ((warp & (kw - 1)) == (n_red & (kw - 1)) && unit < p.units) {
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          for (int w = 0; w < kw; w++) {
-            const float4 v = *reinterpret_cast<const float4*>(red + ((n * W4_WARPS + (warp & ~(kw - 1)) + w) * 32 + lane) * 4);
-            y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
-          }
-          float4* part = reinterpret_cast<float4*>(p.partial) + ((int64_t)unit * 32 + lane) * NT + n;
-          if (slice > 0) {
-            const float4 v = *part;
-            y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
-          }
-          if (slice + 1 < p.slices) {
-            *part = y;
-          } else {
-            if (s_dead) y.x = y.y = y.z = y.w = NAN;
-            const int t = 8 * n + 2 * t4;
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              if (t + e >= p.T) continue;
-              const float lo = e ? y.y : y.x, hi = e ? y.w : y.z;
-              uint16_t* o = p.out + (int64_t)(t + e) * F;
-              if (p.gated) {
-                if (unit * 8 + g < F) o[unit * 8 + g] = f2bf(lo / (1.0f + __expf(-lo)) * hi);
-              } else {
-                if (unit * 16 + g < F) o[unit * 16 + g] = f2bf(lo);
-                if (unit * 16 + g + 8 < F) o[unit * 16 + g + 8] = f2bf(hi);
-              }
-            }
-          }
-        }
-      }
-      n_red++;
+      __syncwarp();
+      if (lane == 0) mbar_arrive1(sums_full + 8 * place);
+      n_units++;
     }
   }
 }
@@ -327,7 +351,7 @@ W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated, i
   const int NT = T > 8 ? 2 : 1;
   r.sub = sub;
   r.units = (int)(gated ? (n_out + 7) / 8 : (n_out + 15) / 16);
-  const int all = (int)((I + 256 * sub - 1) / (256 * sub)), fixed = 1024 + w4_stages(sub) * W4_WARPS * sub * W4_PIECE + 2 * W4_WARPS * 32 * 16 * NT;
+  const int all = (int)((I + 256 * sub - 1) / (256 * sub)), fixed = 1024 + w4_stages(sub) * W4_WARPS * sub * W4_PIECE + w4_sums(NT) * W4_WARPS * 32 * 16 * NT;
   for (r.slices = 1;; r.slices++) {
     r.boxes = (all + r.slices - 1) / r.slices;
     if (r.slices > 1 && r.boxes > W4_WARPS) r.boxes = (r.boxes + W4_WARPS - 1) / W4_WARPS * W4_WARPS;   // whole stages, but for the last
