@@ -1,14 +1,20 @@
 // y = x W^T for a few tokens, W of 4-bit codes c with a scale s (and an offset m) per row and group of columns:
 //   W = (c - 8) s, or c s + m;   y = sum over groups q of  s_q (sum c x - 8 sum x), or s_q sum c x + m_q sum x
-// The codes become bf16 by their bits alone, 0x4300 | c = 128 + c, and sum (128 + c) x over a group runs on the tensor cores (mma.sync
-// m16n8k16: 16 rows of W, 8 tokens) with fp32 sums; what the 128 and the 8 add is 128 or 136 times the group's sum of x, so the sum starts from
-// that, negative:  y = sum_q s_q (sum (128 + c) x - 136 X_q), or s_q (sum (128 + c) x - 128 X_q) + m_q X_q,  X_q = sum x.  (The two cancel to about a
-// sixteenth: four of the 24 bits.)
+// The products run on the tensor cores (mma.sync), 16 rows of W by 8 columns, in one of two forms:
+//   whole numbers, for one or two tokens.  x = e (d0 + d1 / 2^7 + d2 / 2^14) per token and group, e a power of two, the digits of 8 bits, off by at most 2^-21
+//     of the group's largest value (not at all for values within 2^-13 of it): three columns a token, exact sums.  A word of eight codes costs
+//     three instructions of the integer unit.  The sums start from 2^23 + 2^22 - 8 sum d in the bits of a float, so that their bits are that
+//     float's: e and s follow in fp32.
+//   bf16, a column a token.  A code becomes one by its bits alone, 0x4300 | c = 128 + c, seven instructions a word; what the 128 and the 8 add is
+//     128 or 136 times the group's sum of x, so the fp32 sum starts from that, negative (the two cancel to about a sixteenth: four of 24 bits).
+// The integer unit, not the tensor cores, is what both spend most on.  B200, us, whole numbers | bf16: one token, 151936 x 4096 70 | 88, 6144 x 4096
+// 8.3 | 7.9; six tokens, gate and up of 12288 x 4096 in groups of 64 46 | 28.
 //
-// Bounded by the bytes of W.  Sixteen rows are a unit; a box is 256 of its columns, 2 KB that TMA brings with the 128-byte swizzle, a warp's share of
-// a stage of sixteen boxes.  A lane reads a word of 8 codes of rows g and g + 8 and 8 values of x per 32 columns for two products; x lies in
-// shared memory in the order of the codes' bits.  Where rows are long sixteen warps share a unit, where they are short as many units share a
-// stage; the warps' sums meet in shared memory once per unit.  Gated: eight rows of the gate and the eight of the up product they meet are a unit.
+// Bounded by the bytes of W.  Sixteen rows are a unit; a box is 256 (or 512) of its columns, 2 KB pieces that TMA brings with the 128-byte swizzle, a warp's
+// share of a stage of sixteen boxes.  A lane reads a word of 8 codes of rows g and g + 8 and 8 digits per 32 columns and product; the digits
+// lie in shared memory in the order of the codes' bits.  Where rows are long sixteen warps share a unit, where they are short as many units
+// share a stage; the warps' sums meet in shared memory once per unit.  Gated: eight rows of the gate and the eight of the up product they
+// meet are a unit.
 #include <type_traits>
 
 #include "attend.cuh"
@@ -19,8 +25,10 @@ namespace {
 
 constexpr int W4_WARPS = 16, W4_THREADS = 32 * W4_WARPS + 64;   // the warps of the products, one that makes the copies, one that adds the warps' sums
 constexpr int W4_PIECE = 2048;                  // 256 columns of 16 rows
-__host__ __device__ constexpr int w4_stages(int sub) { return sub == 1 ? 3 : 2; }
-__host__ __device__ constexpr int w4_sums(int nt) { return nt == 1 ? 4 : 2; }   // units whose warps' sums are kept
+// Stages at most; units whose warps' sums are kept, with NT times eight columns.
+constexpr int W4_STAGES_MAX = 6;
+__host__ __device__ constexpr int w4_sums(int nt) { return nt == 1 ? 4 : 2; }
+constexpr uint32_t W4_BIAS = 0x4b400000u;       // the float 2^23 + 2^22: adding a whole number below 2^22 to its bits adds it to the float
 constexpr int W4_LONG = 8;                       // stages of 64 KB per SM from which on boxes are of 512 columns
 constexpr int W4_WAIT_LIMIT = 400000;
 constexpr int W4_SMEM = 227 * 1024 - 512;   // of a block; 512 bytes of barriers
@@ -32,22 +40,28 @@ struct W4Params {
   uint16_t* out;
   int n_out, I, T, group_log, gated;
   int units, boxes, kw_log;      // boxes of a unit and slice; 1 << kw_log warps on a unit
+  int stages;
   int slices;                    // parts of the columns, where x does not fit at once
-  int pitch;                     // bytes from one token's x to the next
+  int pitch;                     // bytes from one column of digits to the next
   int groups_smem;               // groups of a slice
   float* partial;                // [units][32][4 NT]: sums of the slices before
   bool early;
 };
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+__device__ __forceinline__ void mma_codes(uint32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void tma_load2(unsigned dst, const CUtensorMap* map, int c0, int c1, unsigned mb) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(c0),
                "r"(c1), "r"(mb)
                : "memory");
+}
+__device__ __forceinline__ void mma_bf16(uint32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // codes 0 and 4 of a word as bf16 128 + c
 __device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t mask, uint32_t magic) {   // one instruction: both constants in registers
@@ -56,24 +70,33 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t mask, uint32_
   return r;
 }
 
-// NT: tokens in eights; SUB: pieces of 256 columns in a box
-template <int NT, int SUB>
+// What a group's sum of a column starts from and is scaled by.
+struct W4Column {
+  uint32_t start;   // whole numbers: W4_BIAS - 8 sum d, or W4_BIAS; bf16: -136 X, or -128 X
+  float e;          // whole numbers: e / 2^(7 digit)
+};
+
+// WHOLE: the form; NT: its columns in eights; SUB: pieces of 256 columns in a box
+template <bool WHOLE, int NT, int SUB>
 __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ W4Params p) {
-  constexpr int W4_BOX = SUB * W4_PIECE, W4_STAGE = W4_WARPS * W4_BOX, W4_STAGES = w4_stages(SUB), SUMS = w4_sums(NT), E = 2 * SUB;   // E: scales of a row that a lane holds
+  constexpr int W4_BOX = SUB * W4_PIECE, W4_STAGE = W4_WARPS * W4_BOX, SUMS = w4_sums(NT), E = 2 * SUB, PER = WHOLE ? 3 : 1;   // PER: columns of a token
+  constexpr int BYTES = WHOLE ? 1 : 2;   // of a value of x in shared memory   // E: scales of a row that a lane holds
   extern __shared__ unsigned char dyn[];
-  __shared__ __align__(8) unsigned long long bars[2 * W4_STAGES + 2 * SUMS];
+  __shared__ __align__(8) unsigned long long bars[2 * W4_STAGES_MAX + 2 * SUMS];
   __shared__ volatile int s_dead;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-  const unsigned base = (smem_addr(dyn) + 1023) & ~1023u, full = smem_addr(bars), empty = full + 8 * W4_STAGES, sums_full = empty + 8 * W4_STAGES, sums_empty = sums_full + 8 * SUMS;
+  const unsigned base = (smem_addr(dyn) + 1023) & ~1023u, full = smem_addr(bars), empty = full + 8 * W4_STAGES_MAX, sums_full = empty + 8 * W4_STAGES_MAX, sums_empty = sums_full + 8 * SUMS;
   unsigned char* at_base = dyn + (base - smem_addr(dyn));
-  float* s_red = reinterpret_cast<float*>(at_base + W4_STAGES * W4_STAGE);          // [SUMS][NT][16 warps][32 lanes][4]
-  float* s_sum = s_red + SUMS * W4_WARPS * 32 * 4 * NT;                                // [groups][8 NT]: -136 X, or -128 X
-  unsigned char* s_x = reinterpret_cast<unsigned char*>(s_sum + p.groups_smem * 8 * NT);   // [T, and one of zeros][pitch]
+  float* s_red = reinterpret_cast<float*>(at_base + p.stages * W4_STAGE);          // [SUMS][NT][16 warps][32 lanes][4]
+  float* s_out = s_red + SUMS * W4_WARPS * 32 * 4 * NT;                             // [NT][32 lanes][4]: of one unit
+  W4Column* s_col = reinterpret_cast<W4Column*>(s_out + 128 * NT);                  // [groups][8 NT]
+  float* s_x = reinterpret_cast<float*>(s_col + p.groups_smem * 8 * NT);            // [groups][8 NT]: sum of x, the column's part (with offsets)
+  unsigned char* s_dig = reinterpret_cast<unsigned char*>(s_x + (p.offsets ? p.groups_smem * 8 * NT : 0));   // x: [columns, and one of zeros][pitch]
   const int kw = 1 << p.kw_log, per_stage = W4_WARPS >> p.kw_log;                   // warps on a unit, units of a stage
   const int steps = (p.boxes + kw - 1) >> p.kw_log;                                 // stages of a unit
   const int sets = (p.units + per_stage - 1) / per_stage, mine = ((int)gridDim.x - 1 - (int)blockIdx.x + sets) / (int)gridDim.x;   // sets of units that share stages
   if (tid == 0) {
-    for (int i = 0; i < W4_STAGES; i++) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, W4_WARPS);
+    for (int i = 0; i < p.stages; i++) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, W4_WARPS);
     for (int i = 0; i < SUMS; i++) mbar_init(sums_full + 8 * i, W4_WARPS), mbar_init(sums_empty + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_dead = 0;
@@ -106,15 +129,15 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
     }
     bool waited = !p.early;
     const int box = p.gated ? lane & 15 : lane, half = p.gated ? lane >> 4 : 0;
-    int q = 0;
+    int q = 0, st = 0;
+    unsigned phase = 0;   // of the copies
     for (int slice = 0; slice < p.slices; slice++)
       for (int i = 0; i < mine; i++) {
         const int set = (int)blockIdx.x + i * (int)gridDim.x;
         const int unit = set * per_stage + (box >> p.kw_log);
         for (int step = 0; step < steps; step++, q++) {
-          const int st = q % W4_STAGES;
-          if (!waited && q == W4_STAGES) pdl_wait(), pdl_trigger(), waited = true;
-          if (q >= W4_STAGES) wait(empty + 8 * st, (unsigned)(q / W4_STAGES - 1) & 1);
+          if (!waited && q == p.stages) pdl_wait(), pdl_trigger(), waited = true;
+          if (q >= p.stages) wait(empty + 8 * st, phase ^ 1);
           if (__any_sync(0xffffffffu, dead)) goto done;
           const int kb = step * kw + (box & (kw - 1)), col = (slice * p.boxes + kb) * (128 * SUB);   // bytes
           const bool on = box < W4_WARPS && unit < p.units && kb < p.boxes && col < p.I / 2;
@@ -127,12 +150,13 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
           for (int sb = 0; sb < SUB; sb++)
             if (sb < pieces)
               tma_load2(base + st * W4_STAGE + box * W4_BOX + sb * W4_PIECE + half * (W4_PIECE / 2), &map, col + 128 * sb, unit * unit_rows + half * F, mb);
+          if (++st == p.stages) st = 0, phase ^= 1;
         }
       }
   done:
     if (s_dead)   // what is under way has to land before the block ends
-      for (int i = q < W4_STAGES ? 0 : q - W4_STAGES; i < q; i++)
-        for (int it = 0; it < W4_WAIT_LIMIT && !mbar_try(full + 8 * (i % W4_STAGES), (unsigned)(i / W4_STAGES & 1)); it++) {}
+      for (int i = q < p.stages ? 0 : q - p.stages; i < q; i++)
+        for (int it = 0; it < W4_WAIT_LIMIT && !mbar_try(full + 8 * (i % p.stages), (unsigned)(i / p.stages & 1)); it++) {}
     if (!waited) pdl_wait(), pdl_trigger();
     return;
   }
@@ -167,21 +191,23 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
               *part = y;
               continue;
             }
-            if (s_dead) y.x = y.y = y.z = y.w = NAN;
-            const int t = 8 * n + 2 * t4;
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              if (t + e >= p.T) continue;
-              const float lo = e ? y.y : y.x, hi = e ? y.w : y.z;
-              uint16_t* o = p.out + (int64_t)(t + e) * F;
-              if (p.gated) {
-                if (unit * 8 + g < F) o[unit * 8 + g] = f2bf(lo / (1.0f + __expf(-lo)) * hi);
-              } else {
-                if (unit * 16 + g < F) o[unit * 16 + g] = f2bf(lo);
-                if (unit * 16 + g + 8 < F) o[unit * 16 + g + 8] = f2bf(hi);
-              }
-            }
+            *reinterpret_cast<float4*>(s_out + (n * 32 + lane) * 4) = y;
           }
+          if (slice + 1 < p.slices) continue;
+          __syncwarp();
+          // row r, column c of the unit's sums
+          auto sum_at = [&](int r, int c) { return s_out[(((c >> 3) * 32 + (r & 7) * 4 + ((c & 7) >> 1)) * 4) + (r >> 3) * 2 + (c & 1)]; };
+          auto token = [&](int r, int t) { return WHOLE ? sum_at(r, 3 * t) + (sum_at(r, 3 * t + 1) + sum_at(r, 3 * t + 2)) : sum_at(r, t); };
+          const int per_token = p.gated ? 8 : 16;
+          for (int k = lane; k < per_token * p.T; k += 32) {
+            const int t = k / per_token, r = k % per_token, o = unit * unit_rows + r;
+            if (o >= F) continue;
+            float y = token(r, t);
+            if (p.gated) y = y / (1.0f + __expf(-y)) * token(r + 8, t);
+            if (s_dead) y = NAN;
+            p.out[(int64_t)t * F + o] = f2bf(y);
+          }
+          __syncwarp();
         }
         __syncwarp();
         if (lane == 0) mbar_arrive1(sums_empty + 8 * place);
@@ -228,96 +254,155 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
   fetch(after);
   if (p.early) pdl_wait();
   pdl_trigger();
+  int st = 0, n_units = 0;
+  unsigned phase = 0;
   uint32_t mask, magic;
   asm volatile("mov.b32 %0, 0x000f000f;\n\tmov.b32 %1, 0x43004300;" : "=r"(mask), "=r"(magic));
-  int q = 0, n_units = 0;
-  unsigned x_lane[NT];   // this lane's token; of those that there are not a row of zeros
+  unsigned d_lane[NT];   // this lane's column of x; of those that there are not a row of zeros
 #pragma unroll
-  for (int n = 0; n < NT; n++) x_lane[n] = smem_addr(s_x) + min(g + 8 * n, p.T) * p.pitch + 16 * t4;
+  for (int n = 0; n < NT; n++) d_lane[n] = smem_addr(s_dig) + min(g + 8 * n, PER * p.T) * p.pitch + 8 * BYTES * t4;
   for (int slice = 0; slice < p.slices; slice++) {
-    // x of the slice into shared memory, eight values of a token at a time: (0, 4), (1, 5), (2, 6), (3, 7); zeros behind the last column
-    const int first_col = slice * p.boxes * (256 * SUB), eights = p.boxes * (32 * SUB);
-    if (slice > 0) asm volatile("bar.sync 1, 512;" ::: "memory");   // the last products with the x before
-    for (int i = tid; i < (p.T + (p.T < 8 * NT)) * eights; i += 32 * W4_WARPS) {
-      const int t = i / eights, e = i - t * eights, col = first_col + 8 * e;
-      const uint4 v = col < p.I && t < p.T ? *reinterpret_cast<const uint4*>(p.x + (int64_t)t * p.x_t + col) : make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4*>(s_x + t * p.pitch + 16 * e) =
-          make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-    }
-    asm volatile("bar.sync 1, 512;" ::: "memory");
-    for (int i = tid; i < p.groups_smem * 8 * NT; i += 32 * W4_WARPS) {
-      const int t = i & (8 * NT - 1), q = i / (8 * NT);
-      float sum = 0.0f;
-      if (t < p.T)
-        for (int e = 0; e < group / 8; e++) {
-          const uint4 v = *reinterpret_cast<const uint4*>(s_x + t * p.pitch + (q * group + 8 * e) * 2);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          float s8 = 0.0f;
+    // x of the slice: a warp takes 256 columns of a token, a lane eight; zeros behind the last column.
+    const int first_col = slice * p.boxes * (256 * SUB), parts = p.boxes * SUB;
+    if (slice > 0) asm volatile("bar.sync 1, 512;" ::: "memory");   // the last products with the digits before
+    for (int i = warp; i < p.T * parts; i += W4_WARPS) {
+      const int t = i / parts, part = i - t * parts, col = first_col + 256 * part + 8 * lane;
+      const uint4 v = col < p.I ? *reinterpret_cast<const uint4*>(p.x + (int64_t)t * p.x_t + col) : make_uint4(0, 0, 0, 0);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      if constexpr (WHOLE) {
+        float x[8];
+        uint32_t top = 0;   // the largest magnitude's bits
 #pragma unroll
-          for (int k = 0; k < 4; k++) s8 += __uint_as_float(w[k] << 16) + __uint_as_float(w[k] & 0xffff0000u);
-          sum += s8;
+        for (int e = 0; e < 8; e++) {
+          x[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+          top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
         }
-      s_sum[i] = sum * (with_offsets ? -128.0f : -136.0f);
+        for (int off = group / 16; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const bool odd = top >= 0x7f800000u;                       // an infinity or NaN: the token comes out as NaN
+        const uint32_t k = max(top >> 23, 27u);                    // largest value: [1, 2) 2^(k - 127), or below 2^-99
+        const float up = odd ? 0.0f : __uint_as_float((127u + 6u + 127u - k) << 23);   // 2^(133 - k): magnitudes below 128
+        int sum[3] = {0, 0, 0};
+        uint32_t digits[3][2] = {};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          float r = odd ? 0.0f : x[e] * up;
+#pragma unroll
+          for (int d = 0; d < 3; d++) {
+            const float whole = fminf(rintf(r), 127.0f);
+            const int z = (int)whole;
+            r = (r - whole) * 128.0f;
+            sum[d] += z;
+            digits[d][e & 1] |= (uint32_t)(z & 255) << (8 * (e >> 1));   // even columns, odd columns
+          }
+        }
+        const float e0 = odd ? NAN : __uint_as_float((k - 6u) << 23);
+#pragma unroll
+        for (int d = 0; d < 3; d++) {
+          for (int off = group / 16; off > 0; off >>= 1) sum[d] += __shfl_xor_sync(0xffffffffu, sum[d], off);
+          *reinterpret_cast<uint2*>(s_dig + (3 * t + d) * p.pitch + 256 * part + 8 * lane) = make_uint2(digits[d][0], digits[d][1]);
+          if ((lane & (group / 8 - 1)) == 0) {
+            const int at = ((256 * part + 8 * lane) / group) * 8 * NT + 3 * t + d;
+            const float e = e0 * (d == 0 ? 1.0f : d == 1 ? 0x1p-7f : 0x1p-14f);
+            s_col[at] = {with_offsets ? W4_BIAS : W4_BIAS - 8u * (uint32_t)sum[d], e};
+            if (with_offsets) s_x[at] = (float)sum[d] * e;
+          }
+        }
+      } else {
+        // (0, 4), (1, 5), (2, 6), (3, 7): the order in which the codes' pairs come out of a word
+        *reinterpret_cast<uint4*>(s_dig + t * p.pitch + 512 * part + 16 * lane) =
+            make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+        float X = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) X += __uint_as_float(w[e] << 16) + __uint_as_float(w[e] & 0xffff0000u);
+        for (int off = group / 16; off > 0; off >>= 1) X += __shfl_xor_sync(0xffffffffu, X, off);
+        if ((lane & (group / 8 - 1)) == 0) {
+          const int at = ((256 * part + 8 * lane) / group) * 8 * NT + t;
+          s_col[at] = {__float_as_uint(X * (with_offsets ? -128.0f : -136.0f)), 1.0f};
+          if (with_offsets) s_x[at] = X;
+        }
+      }
+    }
+    for (int i = tid; i < p.pitch / 8; i += 32 * W4_WARPS) *reinterpret_cast<uint2*>(s_dig + PER * p.T * p.pitch + 8 * i) = make_uint2(0, 0);
+    for (int i = tid; i < p.groups_smem * (8 * NT - PER * p.T); i += 32 * W4_WARPS) {
+      const int at = i / (8 * NT - PER * p.T) * 8 * NT + PER * p.T + i % (8 * NT - PER * p.T);
+      s_col[at] = {WHOLE ? W4_BIAS : 0u, 0.0f};
+      if (with_offsets) s_x[at] = 0.0f;
     }
     asm volatile("bar.sync 1, 512;" ::: "memory");
     for (int i = 0; i < mine; i++) {
       const int unit = ((int)blockIdx.x + i * (int)gridDim.x) * per_stage + (warp >> p.kw_log);
       float total[NT][4] = {};
-      for (int step = 0; step < steps; step++, q++) {
+      for (int step = 0; step < steps; step++) {
         const Scales now = next;
-        const int kb = step * kw + (warp & (kw - 1)), st = q % W4_STAGES;
+        const int kb = step * kw + (warp & (kw - 1));
         next = after;
         fetch(after);
-        wait(full + 8 * st, (unsigned)(q / W4_STAGES) & 1);
+        wait(full + 8 * st, phase);
         if (kb < p.boxes && (slice * p.boxes + kb) * (256 * SUB) < p.I && unit < p.units) {   // warp-uniform
-          const unsigned w_at = base + st * W4_STAGE + warp * W4_BOX + g * 128 + 4 * t4 + 16 * g, x_at = kb * (512 * SUB);   // chunk 0 of row g, swizzled
+          const unsigned w_at = base + st * W4_STAGE + warp * W4_BOX + g * 128 + 4 * t4 + 16 * g, d_at = kb * (256 * SUB * BYTES);   // chunk 0 of row g, swizzled
           auto boxes = [&](auto log) {
             constexpr int CH = 1 << (decltype(log)::value - 5);   // steps of 32 columns in a group
 #pragma unroll
             for (int c0 = 0; c0 < 8 * SUB; c0 += CH) {
               const int in_box = c0 / CH, from = (lane & 28) | (in_box & 3);
-              float d[NT][4];   // the sum of c x: it starts from what the rest of the products will have added
+              uint32_t d[NT][4];
+              float4 column[NT];   // of this lane's two columns: start and e
 #pragma unroll
               for (int n = 0; n < NT; n++) {
-                const float2 off = *reinterpret_cast<const float2*>(s_sum + (kb * per_box + in_box) * 8 * NT + 2 * t4 + 8 * n);
-                d[n][0] = d[n][2] = off.x, d[n][1] = d[n][3] = off.y;
+                column[n] = *reinterpret_cast<const float4*>(s_col + (kb * per_box + in_box) * 8 * NT + 2 * t4 + 8 * n);
+                d[n][0] = d[n][2] = __float_as_uint(column[n].x), d[n][1] = d[n][3] = __float_as_uint(column[n].z);
               }
 #pragma unroll
               for (int c = c0; c < c0 + CH; c++) {
                 uint32_t w0, w1, b[NT][4];
                 asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w0) : "r"((w_at ^ ((c & 7) << 4)) + (c >> 3) * W4_PIECE) : "memory");
                 asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w1) : "r"((w_at ^ ((c & 7) << 4)) + (c >> 3) * W4_PIECE + 1024) : "memory");
+                if constexpr (WHOLE) {
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                               : "=r"(b[n][0]), "=r"(b[n][1]), "=r"(b[n][2]), "=r"(b[n][3])
-                               : "r"(x_lane[n] + x_at + 64 * c)
-                               : "memory");
-                }
-                const uint32_t a0 = code_pair(w0, mask, magic), a1 = code_pair(w1, mask, magic), a2 = code_pair(w0 >> 4, mask, magic), a3 = code_pair(w1 >> 4, mask, magic);
-                const uint32_t a4 = code_pair(w0 >> 8, mask, magic), a5 = code_pair(w1 >> 8, mask, magic), a6 = code_pair(w0 >> 12, mask, magic), a7 = code_pair(w1 >> 12, mask, magic);
+                  for (int n = 0; n < NT; n++)
+                    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(b[n][0]), "=r"(b[n][1]) : "r"(d_lane[n] + d_at + 32 * c) : "memory");
+                  const uint32_t a0 = w0 & 0x0f0f0f0fu, a1 = w1 & 0x0f0f0f0fu, a2 = w0 >> 4 & 0x0f0f0f0fu, a3 = w1 >> 4 & 0x0f0f0f0fu;
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                  mma_bf16(d[n], a0, a1, a2, a3, b[n][0], b[n][1]);
-                  mma_bf16(d[n], a4, a5, a6, a7, b[n][2], b[n][3]);
+                  for (int n = 0; n < NT; n++) mma_codes(d[n], a0, a1, a2, a3, b[n][0], b[n][1]);
+                } else {
+#pragma unroll
+                  for (int n = 0; n < NT; n++)
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(b[n][0]), "=r"(b[n][1]), "=r"(b[n][2]), "=r"(b[n][3])
+                                 : "r"(d_lane[n] + d_at + 64 * c)
+                                 : "memory");
+                  const uint32_t a0 = code_pair(w0, mask, magic), a1 = code_pair(w1, mask, magic), a2 = code_pair(w0 >> 4, mask, magic), a3 = code_pair(w1 >> 4, mask, magic);
+                  const uint32_t a4 = code_pair(w0 >> 8, mask, magic), a5 = code_pair(w1 >> 8, mask, magic), a6 = code_pair(w0 >> 12, mask, magic), a7 = code_pair(w1 >> 12, mask, magic);
+#pragma unroll
+                  for (int n = 0; n < NT; n++) {
+                    mma_bf16(d[n], a0, a1, a2, a3, b[n][0], b[n][1]);
+                    mma_bf16(d[n], a4, a5, a6, a7, b[n][2], b[n][3]);
+                  }
                 }
               }
               float sc[2];
 #pragma unroll
               for (int r = 0; r < 2; r++) sc[r] = __uint_as_float(__shfl_sync(0xffffffffu, (uint32_t)now.s[r][in_box >> 2], from) << 16);
 #pragma unroll
-              for (int n = 0; n < NT; n++)
+              for (int n = 0; n < NT; n++) {
+                if constexpr (WHOLE) {
+                  const float e0 = column[n].y, e1 = column[n].w, k0 = -12582912.0f * e0, k1 = -12582912.0f * e1;   // exact: e is a power of two
 #pragma unroll
-                for (int e = 0; e < 4; e++) total[n][e] = fmaf(sc[e >> 1], d[n][e], total[n][e]);
+                  for (int e = 0; e < 4; e++) total[n][e] = fmaf(sc[e >> 1], fmaf(__uint_as_float(d[n][e]), e & 1 ? e1 : e0, e & 1 ? k1 : k0), total[n][e]);
+                } else {
+#pragma unroll
+                  for (int e = 0; e < 4; e++) total[n][e] = fmaf(sc[e >> 1], __uint_as_float(d[n][e]), total[n][e]);
+                }
+              }
               if (with_offsets) {
                 float u[2];
 #pragma unroll
-                for (int r = 0; r < 2; r++) u[r] = __uint_as_float(__shfl_sync(0xffffffffu, (uint32_t)now.u[r][in_box >> 2], from) << 16) * -0x1p-7f;
+                for (int r = 0; r < 2; r++) u[r] = __uint_as_float(__shfl_sync(0xffffffffu, (uint32_t)now.u[r][in_box >> 2], from) << 16);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                  const float2 off = *reinterpret_cast<const float2*>(s_sum + (kb * per_box + in_box) * 8 * NT + 2 * t4 + 8 * n);
+                  const float2 sums = *reinterpret_cast<const float2*>(s_x + (kb * per_box + in_box) * 8 * NT + 2 * t4 + 8 * n);
 #pragma unroll
-                  for (int e = 0; e < 4; e++) total[n][e] = fmaf(u[e >> 1], e & 1 ? off.y : off.x, total[n][e]);
+                  for (int e = 0; e < 4; e++) total[n][e] = fmaf(u[e >> 1], e & 1 ? sums.y : sums.x, total[n][e]);
                 }
               }
             }
@@ -328,6 +413,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
         }
         __syncwarp();
         if (lane == 0) mbar_arrive1(empty + 8 * st);
+        if (++st == p.stages) st = 0, phase ^= 1;
       }
       // ---- this warp's sums of the unit ----
       const int place = n_units % SUMS;
@@ -343,32 +429,36 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
 }
 
 // How x and the rows are laid out for a product.
+// How x and the rows are laid out for a product.
 struct W4Plan {
-  int sub, units, boxes, kw_log, slices, pitch, groups_smem, smem, sets;
+  bool whole;
+  int tiles, sub, stages, units, boxes, kw_log, slices, pitch, groups_smem, smem, sets;
 };
-W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated, int sub) {
+W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated, bool offsets, bool whole, int sub) {
   W4Plan r = {};
-  const int NT = T > 8 ? 2 : 1;
-  r.sub = sub;
+  const int columns = (int)(whole ? 3 * T : T), NT = (columns + 7) / 8, bytes = whole ? 1 : 2;
+  r.whole = whole, r.tiles = NT, r.sub = sub;
   r.units = (int)(gated ? (n_out + 7) / 8 : (n_out + 15) / 16);
-  const int all = (int)((I + 256 * sub - 1) / (256 * sub)), fixed = 1024 + w4_stages(sub) * W4_WARPS * sub * W4_PIECE + w4_sums(NT) * W4_WARPS * 32 * 16 * NT;
+  const int all = (int)((I + 256 * sub - 1) / (256 * sub)), stage = W4_WARPS * sub * W4_PIECE, fixed = 1024 + 2 * stage + w4_sums(NT) * W4_WARPS * 32 * 16 * NT + 512 * NT;
   for (r.slices = 1;; r.slices++) {
     r.boxes = (all + r.slices - 1) / r.slices;
     if (r.slices > 1 && r.boxes > W4_WARPS) r.boxes = (r.boxes + W4_WARPS - 1) / W4_WARPS * W4_WARPS;   // whole stages, but for the last
-    r.pitch = r.boxes * 512 * sub + 64;   // (two tokens fill the banks)
+    r.pitch = r.boxes * 256 * sub * bytes + 32 * bytes;   // (four columns' 32 bytes, or two columns' 64, fill the banks)
     r.groups_smem = r.boxes * ((256 * sub) >> group_log);
-    r.smem = fixed + r.groups_smem * 8 * NT * 4 + (int)(T + (T < 8 * NT)) * r.pitch;
+    r.smem = fixed + r.groups_smem * 8 * NT * (offsets ? 12 : 8) + (columns + 1) * r.pitch;
     if (r.smem <= W4_SMEM || r.boxes == 1) break;
   }
   r.slices = (all + r.boxes - 1) / r.boxes;
+  for (r.stages = 2; r.stages < W4_STAGES_MAX && r.smem + stage <= W4_SMEM; r.stages++) r.smem += stage;
   while ((1 << r.kw_log) < r.boxes && (1 << r.kw_log) < W4_WARPS) r.kw_log++;
   r.sets = (r.units + (W4_WARPS >> r.kw_log) - 1) / (W4_WARPS >> r.kw_log);
   return r;
 }
-// Boxes of 512 columns, which spread what a box costs besides its products, where an SM has many stages of them all the same.
-W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated) {
-  const W4Plan two = w4_plan(n_out, I, T, group_log, gated, 2);
-  return (int64_t)two.sets * ((two.boxes + (1 << two.kw_log) - 1) >> two.kw_log) >= W4_LONG * (int64_t)sm_count() ? two : w4_plan(n_out, I, T, group_log, gated, 1);
+// Boxes of 512 columns, which spread what a box costs besides its products, where an SM has many stages of them all the same; for one or two tokens in
+// whole numbers, whose digits have to pay.
+W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated, bool offsets) {
+  const W4Plan two = w4_plan(n_out, I, T, group_log, gated, offsets, T <= 2, 2);
+  return (int64_t)two.sets * ((two.boxes + (1 << two.kw_log) - 1) >> two.kw_log) >= W4_LONG * (int64_t)sm_count() ? two : w4_plan(n_out, I, T, group_log, gated, offsets, false, 1);
 }
 
 }  // namespace
@@ -378,8 +468,13 @@ using namespace pk;
 
 extern "C" int64_t pk_gemv_w4_workspace_bytes(int64_t T, int64_t O, int64_t I, int64_t group, int gated) {
   if (T < 1 || O < 1 || I < 32 || (group != 32 && group != 64 && group != 128)) return 0;
-  const W4Plan plan = w4_plan(gated ? O / 2 : O, I, T, group == 128 ? 7 : group == 64 ? 6 : 5, gated != 0);
-  return plan.slices > 1 ? (int64_t)plan.units * 32 * 16 * (T > 8 ? 2 : 1) : 0;
+  // (the larger of what is needed with offsets and without)
+  int64_t most = 0;
+  for (const bool offsets : {false, true}) {
+    const W4Plan plan = w4_plan(gated ? O / 2 : O, I, T, group == 128 ? 7 : group == 64 ? 6 : 5, gated != 0, offsets);
+    if (plan.slices > 1) most = (int64_t)plan.units * 32 * 16 * plan.tiles;
+  }
+  return most;
 }
 
 extern "C" int pk_gemv_w4(const pk_tensor* weight, const pk_tensor* scales, const pk_tensor* offsets, const pk_tensor* x, const pk_tensor* out,
@@ -406,7 +501,7 @@ extern "C" int pk_gemv_w4(const pk_tensor* weight, const pk_tensor* scales, cons
   PK_REQUIRE(aligned16(weight->data) && aligned16(x->data), "weight and x must be 16-byte aligned");
   if (T == 0) return PK_OK;
   const int n_out = (int)(gated ? O / 2 : O), group_log = group == 128 ? 7 : group == 64 ? 6 : 5;
-  const W4Plan plan = w4_plan(n_out, I, T, group_log, gated != 0);
+  const W4Plan plan = w4_plan(n_out, I, T, group_log, gated != 0, offsets != nullptr);
   if (plan.slices > 1 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < pk_gemv_w4_workspace_bytes(T, O, I, group, gated)))
     return fail(PK_ERR_WORKSPACE, "gemv_w4: workspace missing, misaligned or too small");
   CUtensorMap map;
@@ -420,23 +515,27 @@ extern "C" int pk_gemv_w4(const pk_tensor* weight, const pk_tensor* scales, cons
   p.w = (const uint8_t*)weight->data, p.scales = (const uint16_t*)scales->data, p.offsets = offsets ? (const uint16_t*)offsets->data : nullptr;
   p.x = (const uint16_t*)x->data, p.x_t = x->stride[0], p.out = (uint16_t*)out->data;
   p.n_out = n_out, p.I = (int)I, p.T = (int)T, p.group_log = group_log, p.gated = gated != 0;
-  p.units = plan.units, p.boxes = plan.boxes, p.kw_log = plan.kw_log, p.slices = plan.slices, p.pitch = plan.pitch, p.groups_smem = plan.groups_smem;
+  p.units = plan.units, p.boxes = plan.boxes, p.kw_log = plan.kw_log, p.stages = plan.stages, p.slices = plan.slices, p.pitch = plan.pitch, p.groups_smem = plan.groups_smem;
   p.partial = (float*)workspace, p.early = pdl_early();
   const unsigned grid = (unsigned)(plan.sets < sm_count() ? plan.sets : sm_count());
   StageTimer timer(ST_GEMV, (cudaStream_t)stream);
-  auto launch = [&](auto nt, auto sub) -> int {
-    constexpr int NT = decltype(nt)::value, SUB = decltype(sub)::value;
+  auto launch = [&](auto whole, auto nt, auto sub) -> int {
+    constexpr auto kernel = gemv_w4_kernel<decltype(whole)::value, decltype(nt)::value, decltype(sub)::value>;
     static PerDevice opted;
     if (const unsigned long long bit = first_on_device(opted)) {
-      if (cudaFuncSetAttribute(gemv_w4_kernel<NT, SUB>, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM) != cudaSuccess)
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM) != cudaSuccess)
         return fail(PK_ERR_CUDA, "gemv_w4: %s", cudaGetErrorString(cudaGetLastError()));
       mark_on_device(opted, bit);
     }
-    launch_chain(gemv_w4_kernel<NT, SUB>, dim3(grid), dim3(W4_THREADS), (size_t)plan.smem, (cudaStream_t)stream, map, p);
+    launch_chain(kernel, dim3(grid), dim3(W4_THREADS), (size_t)plan.smem, (cudaStream_t)stream, map, p);
     return PK_OK;
   };
   using One = std::integral_constant<int, 1>;
   using Two = std::integral_constant<int, 2>;
-  if (const int rc = T > 8 ? (plan.sub == 2 ? launch(Two(), Two()) : launch(Two(), One())) : (plan.sub == 2 ? launch(One(), Two()) : launch(One(), One()))) return rc;
+  using Bf16 = std::false_type;
+  const int rc = plan.whole ? launch(std::true_type(), One(), Two())
+                 : plan.tiles == 1 ? (plan.sub == 1 ? launch(Bf16(), One(), One()) : launch(Bf16(), One(), Two()))
+                                   : (plan.sub == 1 ? launch(Bf16(), Two(), One()) : launch(Bf16(), Two(), Two()));
+  if (rc) return rc;
   return check_launch("gemv_w4");
 }

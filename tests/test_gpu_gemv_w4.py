@@ -46,6 +46,25 @@ def test_every_number_of_tokens(T):
     check(*make(T, T, 70, 1120, 32, True), False)
 
 
+@pytest.mark.parametrize("O,I,group,offsets,gated", [(38000, 4096, 128, False, False), (304200, 512, 64, True, False), (76001, 1568, 32, True, False),
+                                                     (75000, 2176, 128, True, True), (19001, 12288, 64, False, False)])
+def test_long_products_of_one_and_two_tokens(O, I, group, offsets, gated):
+    """What an SM has many stages of takes x in whole numbers: values of very different sizes, zeros, and a group of zeros."""
+    for T in (1, 2):
+        codes, scales, x, off = make(O + T, T, O, I, group, offsets)
+        x[0, ::7] *= 1000
+        x[0, 5::11] *= 2.0 ** -20
+        x[0, :group] = 0
+        x[-1, group:2 * group] *= 2.0 ** -110
+        check(codes, scales, x, off, gated)
+        if T == 2:
+            from pariskv_b200 import ops
+            clean = ops.gemv_w4(R.pack_w4(codes), scales, x, offsets=off, gated=gated)
+            x[0, 3], x[0, 200] = float("inf"), float("nan")
+            got = ops.gemv_w4(R.pack_w4(codes), scales, x, offsets=off, gated=gated)
+            assert torch.equal(got[1], clean[1]) and not got[0].isfinite().any()
+
+
 def test_every_code_and_column():
     """One token per column of a group, each code in turn: no two columns or codes are taken for each other."""
     from pariskv_b200 import ops
