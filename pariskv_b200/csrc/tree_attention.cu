@@ -4,7 +4,7 @@
 //
 // The T tokens and G query heads of a KV head are the T * G rows of one product with the same keys, so that the cache is read once
 // for all of them.  Tiles of 128 keys: S = Q K^T and O += P V run on tcgen05 with 128 query rows each, S, P and O in tensor memory,
-// K and V by TMA into a ring of 32 KB stages.  A block is two streams of four softmax warps (a thread per query row):
+// K and V by TMA into a ring of 32 KB stages.  A block is two streams of eight softmax warps (two threads per query row, half of a tile's keys each):
 //   NT = 2   (more than 128 rows)  a stream per 128 query rows, both over every tile: K and V are read once for 256 rows
 //   NT = 1   both streams have the same rows, one takes the even tiles and the other the odd ones
 // so that while one stream's scores become probabilities the tensor cores work for the other.
@@ -17,7 +17,7 @@ namespace pk {
 namespace {
 
 constexpr int TA_TILE = 128;                   // keys of a tile
-constexpr int TA_THREADS = 320;                // two softmax groups of four warps, a warp for the copies, a warp for the products
+constexpr int TA_THREADS = 576;                // two streams of eight softmax warps, a warp for the copies, a warp for the products
 constexpr int TA_STAGE = 32768;                // a tile of K or V: two halves of 64 channels, 128 rows of 128 bytes
 constexpr int TA_WAIT_LIMIT = 4000000;
 constexpr int TA_FEW = 32;                       // up to so many query rows attend_few.cu has the call
@@ -92,41 +92,49 @@ struct Cursor {
   }
 };
 
+template <int NS>
+struct TreeShared {
+  unsigned long long bars[2 * NS + 8];
+  float most[2][2][128];   // [stream][half of the keys][row]: maxima, on their way to the other half
+  TilePlan plan;
+  unsigned tmem, bad[8];   // bad: drafts whose rows of V hold what is not a number
+  int dead;
+};
+
 template <int NT>
 __global__ void __launch_bounds__(TA_THREADS, 1)
     tree_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dk,
                      const __grid_constant__ CUtensorMap map_dv, const __grid_constant__ TreeParams p) {
   constexpr int NS = TaRing<NT>::stages;
-  extern __shared__ unsigned char dyn[];
-  __shared__ __align__(8) unsigned long long bars[2 * NS + 8];
-  __shared__ unsigned s_tmem, s_bad[8];
-  __shared__ volatile int s_dead;
-  __shared__ TilePlan s_plan;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const unsigned base = (smem_addr(dyn) + 1023) & ~1023u, q_smem = base, ring = base + NT * TA_STAGE;
-  const unsigned full = smem_addr(bars), empty = full + 8 * NS, s_full = empty + 8 * NS, p_full = s_full + 16, o_done = p_full + 16, q_full = o_done + 16, ending = q_full + 8;
+  extern __shared__ __align__(1024) unsigned char dyn[];   // (the kernel has no other shared memory: it begins where the block's does, on such a boundary)
+  TreeShared<NS>& sh = *reinterpret_cast<TreeShared<NS>*>(dyn + (NT + NS) * TA_STAGE);
+  unsigned (&s_bad)[8] = sh.bad;
+  volatile int& s_dead = sh.dead;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const unsigned q_smem = smem_addr(dyn), ring = q_smem + NT * TA_STAGE;
+  const unsigned full = smem_addr(sh.bars), empty = full + 8 * NS, s_full = empty + 8 * NS, p_full = s_full + 16, o_done = p_full + 16, q_full = o_done + 16, ending = q_full + 8;
   if (tid == 0) {
     for (int i = 0; i < NS; i++) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
-    for (int i = 0; i < 2; i++) mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, 128), mbar_init(o_done + 8 * i, 1);
-    mbar_init(q_full, 256), mbar_init(ending, 1);
+    for (int i = 0; i < 2; i++) mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, 256), mbar_init(o_done + 8 * i, 1);
+    mbar_init(q_full, 512), mbar_init(ending, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_dead = 0;
   }
   if (tid < 8) s_bad[tid] = 0;
-  if (warp == 8) tmem_alloc(smem_addr(&s_tmem), 512);
-  if (warp == 9 && lane < 4) tma_prefetch_map(lane == 0 ? &map_k : lane == 1 ? &map_v : lane == 2 ? &map_dk : &map_dv);
+  if (warp == 16) tmem_alloc(smem_addr(&sh.tmem), 512);
+  if (warp == 17 && lane < 4) tma_prefetch_map(lane == 0 ? &map_k : lane == 1 ? &map_v : lane == 2 ? &map_dk : &map_dv);
   pdl_wait();
   pdl_trigger();
   const int blocks = (int)gridDim.x;
   if (warp == 0) {
     const TilePlan plan = tile_plan(p, [&](int64_t total) { return total * blockIdx.x / min((int64_t)blocks, total); });
-    if (lane == 0) s_plan = plan;
+    if (lane == 0) sh.plan = plan;
   }
   tc_before();
   __syncthreads();
   tc_after();
-  const unsigned tmem = s_tmem;
-  const TilePlan plan = s_plan;
+  const unsigned tmem = sh.tmem;
+  const TilePlan plan = sh.plan;
   const int64_t shares = min((int64_t)blocks, plan.total);
   Cursor cur;
   {
@@ -146,7 +154,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     }
   };
 
-  if (warp == 8) {
+  if (warp == 16) {
     // ---- copies: K and V of every tile in turn ----
     if (lane == 0) {
       unsigned q = 0;
@@ -171,79 +179,95 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         for (unsigned i = q < NS ? 0 : q - NS; i < q; i++)
           for (int it = 0; it < TA_WAIT_LIMIT && !mbar_try(full + 8 * (i % NS), (i / NS) & 1); it++) {}
     }
-  } else if (warp == 9) {
-    // ---- products ----
-    if (lane == 0) {
-      constexpr unsigned ID_S = umma_idesc(128, 128, false), ID_O = umma_idesc(128, 128, true);
-      auto scores = [&](int s, unsigned kq) {   // S_s = Q K^T, K in stage kq
-        const unsigned a = q_smem + (NT == 2 ? s * TA_STAGE : 0), b = ring + kq * TA_STAGE;
-        if (dead) return;
+  } else if (warp == 17) {
+    // ---- products: the whole warp goes the same way, one lane issues.  What an instruction needs besides is a constant added to a descriptor: computed
+    // anew for each, by a single thread, the descriptors took 100 clocks an instruction, which executes in 64. ----
+    constexpr unsigned ID_S = umma_idesc(128, 128, false), ID_O = umma_idesc(128, 128, true), STAGE = TA_STAGE >> 4;
+    const bool leader = elect_one();
+    const uint64_t q_desc = umma_desc(q_smem, 16), k_desc = umma_desc(ring, 16), v_desc = umma_desc(ring, TA_STAGE / 2);
+    struct Place {   // of a copy in the ring
+      unsigned st, phase;
+      __device__ __forceinline__ Place plus(unsigned n) const { return st + n < NS ? Place{st + n, phase} : Place{st + n - NS, phase ^ 1}; }
+    };
+    auto scores = [&](int s, Place k) {   // S_s = Q K^T
+      const uint64_t a = q_desc + (NT == 2 ? s * STAGE : 0u), b = k_desc + k.st * STAGE;
+      if (leader && !dead) {
+        tc_mma_ss<false>(tmem + 128 * s, a, b, ID_S);
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-          const unsigned off = (k >> 2) * (TA_STAGE / 2) + (k & 3) * 32;
-          tc_mma_ss(tmem + 128 * s, umma_desc(a + off, 16), umma_desc(b + off, 16), ID_S, k > 0);
+        for (int i = 1; i < 8; i++) {
+          const unsigned off = ((i >> 2) * (TA_STAGE / 2) + (i & 3) * 32) >> 4;
+          tc_mma_ss<true>(tmem + 128 * s, a + off, b + off, ID_S);
         }
         tc_commit(s_full + 8 * s);
-      };
-      auto values = [&](int s, unsigned vq, bool add) {   // O_s (+)= P_s V
-        const unsigned b = ring + vq * TA_STAGE;
-        if (dead) return;
+      }
+    };
+    auto values = [&](int s, Place v, bool add) {   // O_s (+)= P_s V
+      const uint64_t b = v_desc + v.st * STAGE;
+      if (leader && !dead) {
 #pragma unroll
-        for (int k = 0; k < 8; k++) tc_mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + 8 * k, umma_desc(b + k * 2048, TA_STAGE / 2), ID_O, add || k > 0);
-      };
-      auto free_stage = [&](unsigned st) { if (!dead) tc_commit(empty + 8 * st); };
-      auto arrived = [&](unsigned q) {
-        wait(full + 8 * (q % NS), (q / NS) & 1);
-        tc_after();
-      };
-      unsigned q0 = 0, seg = 0, n_p[2] = {0, 0};   // q0: number of the segment's first copy
-      auto probabilities = [&](int s) {
-        wait(p_full + 8 * s, n_p[s]++ & 1);
-        tc_after();
-      };
-      for (; cur.left > 0; cur.next(p), seg++) {
-        const int n = cur.count();
-        wait(q_full, seg & 1);
-        tc_after();
-        arrived(q0);
-        scores(0, q0 % NS);
-        if (NT == 2) {
-          scores(1, q0 % NS);
-          free_stage(q0 % NS);
-        } else {
-          free_stage(q0 % NS);
-          if (n > 1) {
-            arrived(q0 + 2);
-            scores(1, (q0 + 2) % NS);
-            free_stage((q0 + 2) % NS);
+        for (int i = 0; i < 8; i++) tc_mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + 64 * (i >> 2) + 8 * (i & 3), b + i * (2048 >> 4), ID_O, i > 0 ? 1u : (unsigned)add);
+      }
+    };
+    auto commit = [&](unsigned mb) {
+      if (leader && !dead) tc_commit(mb);
+    };
+    auto free_stage = [&](Place at) { commit(empty + 8 * at.st); };
+    auto arrived = [&](Place at) {
+      wait(full + 8 * at.st, at.phase);
+      __syncwarp();
+      tc_after();
+    };
+    unsigned n_p[2] = {0, 0}, seg = 0;
+    auto probabilities = [&](int s) {
+      wait(p_full + 8 * s, n_p[s] & 1);
+      n_p[s] ^= 1;
+      __syncwarp();
+      tc_after();
+    };
+    Place at = {0, 0};   // of the tile's K
+    for (; cur.left > 0; cur.next(p), seg ^= 1) {
+      const int n = cur.count();
+      wait(q_full, seg);
+      __syncwarp();
+      tc_after();
+      arrived(at);
+      scores(0, at);
+      if (NT == 2) scores(1, at);
+      free_stage(at);
+      if (NT == 1 && n > 1) {
+        arrived(at.plus(2));
+        scores(1, at.plus(2));
+        free_stage(at.plus(2));
+      }
+      for (int j = 0; j < n; j++, at = at.plus(2)) {
+        const Place v = at.plus(1), k_next = at.plus(NT == 2 ? 2 : 4);
+        const bool more = j + (NT == 2 ? 1 : 2) < n;
+        arrived(v);
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+          const int s = NT == 2 ? i : j & 1;
+          probabilities(s);
+          values(s, v, NT == 2 ? j > 0 : j > 1);
+          if (i == NT - 1) free_stage(v);
+          if (more) {
+            if (i == 0) arrived(k_next);
+            scores(s, k_next);
+            if (i == NT - 1) free_stage(k_next);
+          } else {
+            commit(o_done + 8 * s);
           }
         }
-        for (int j = 0; j < n; j++) {
-          const unsigned v = q0 + 2 * j + 1, k_next = q0 + 2 * (j + (NT == 2 ? 1 : 2));
-          const bool more = j + (NT == 2 ? 1 : 2) < n;
-          arrived(v);
-#pragma unroll
-          for (int i = 0; i < NT; i++) {
-            const int s = NT == 2 ? i : j & 1;
-            probabilities(s);
-            values(s, v % NS, NT == 2 ? j > 0 : j > 1);
-            if (i == NT - 1) free_stage(v % NS);
-            if (more) {
-              if (i == 0) arrived(k_next);
-              scores(s, k_next % NS);
-              if (i == NT - 1) free_stage(k_next % NS);
-            } else if (!dead) {
-              tc_commit(o_done + 8 * s);
-            }
-          }
-        }
-        q0 += 2 * n;
       }
     }
+    if (s_dead && leader) {   // products under way end before the tensor memory goes
+      tc_commit(ending);
+      for (int it = 0; it < TA_WAIT_LIMIT && !mbar_try(ending, 0); it++) {}
+    }
   } else {
-    // ---- softmax: stream `s`, a thread per query row ----
-    const int s = warp >> 2, r = tid & 127;
-    const unsigned lanes = tmem + ((unsigned)(warp & 3) << 21), s_cols = lanes + 128 * s, o_cols = lanes + 256;
+    // ---- softmax: stream `s`, two threads per query row: `part` is the half of a tile's keys, and of the channels of O ----
+    const int s = warp >> 3, part = warp >> 2 & 1, r = 32 * (warp & 3) + lane;
+    const unsigned lanes = tmem + ((unsigned)(warp & 3) << 21), s_cols = lanes + 128 * s + 64 * part, o_cols = lanes + 256;   // this half's scores, and its weights in their place
+    const int pair = 3 + 4 * s + (warp & 3);   // barrier of the two warps that share rows
     const int Hq = p.a.H * p.a.G, tl = r / p.a.G, g = r % p.a.G;
     const float scale = p.a.scale_log2;
     unsigned q0 = 0, n_s = 0, n_o[2] = {0, 0};
@@ -252,31 +276,29 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       const int token0 = (NT == 2 ? 2 * cur.group + s : cur.group) * p.tile_tokens, t = token0 + tl;
       const bool row_ok = tl < p.tile_tokens && t < p.a.T;
       const bool warp_ok = __any_sync(0xffffffffu, row_ok);
-      {  // this thread's row of Q (NT = 1: this stream's half of it), swizzled as the copies of K are
-        const uint16_t* src = p.a.q + cur.b * p.a.q_b + (int64_t)t * p.a.q_t + (int64_t)(cur.h * p.a.G + g) * p.a.q_h;
+      {  // this thread's share of its row of Q, swizzled as the copies of K are
+        constexpr int CHUNKS = NT == 2 ? 8 : 4;
+        const int half = NT == 2 ? part : s, c0 = NT == 2 ? 0 : 4 * part;
+        const uint16_t* src = p.a.q + cur.b * p.a.q_b + (int64_t)t * p.a.q_t + (int64_t)(cur.h * p.a.G + g) * p.a.q_h + half * 64 + 8 * c0;
+        const unsigned dst = q_smem + (NT == 2 ? s * TA_STAGE : 0) + half * (TA_STAGE / 2) + r * 128;
+        uint4 x[CHUNKS];
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-          if (NT == 1 && half != s) continue;
-          const unsigned dst = q_smem + (NT == 2 ? s * TA_STAGE : 0) + half * (TA_STAGE / 2) + r * 128;
-          uint4 x[8];
+        for (int c = 0; c < CHUNKS; c++) x[c] = row_ok ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-          for (int c = 0; c < 8; c++) x[c] = row_ok ? *reinterpret_cast<const uint4*>(src + half * 64 + 8 * c) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-          for (int c = 0; c < 8; c++)
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + ((c ^ (r & 7)) << 4)), "r"(x[c].x), "r"(x[c].y), "r"(x[c].z), "r"(x[c].w) : "memory");
-        }
+        for (int c = 0; c < CHUNKS; c++)
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (((c0 + c) ^ (r & 7)) << 4)), "r"(x[c].x), "r"(x[c].y), "r"(x[c].z), "r"(x[c].w) : "memory");
         fence_async();
         mbar_arrive1(q_full);
       }
       // which drafts of draft tile dt this row sees: a token's bytes by 32 lanes at a time
-      auto drafts_seen = [&](int dt, uint32_t (&w)[4]) {
+      auto drafts_seen = [&](int dt, uint32_t (&w)[2]) {
         const int t_first = token0 + (32 * (warp & 3)) / p.a.G, t_last = min(token0 + (32 * (warp & 3) + 31) / p.a.G, p.a.T - 1);
         const uint8_t* mask = p.a.mask + cur.b * p.a.m_b;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int d = dt * TA_TILE + 32 * i + lane;
+        for (int i = 0; i < 2; i++) {
+          const int d = dt * TA_TILE + 64 * part + 32 * i + lane;
           w[i] = 0;
-          if (dt * TA_TILE + 32 * i < p.a.T)
+          if (d - lane < p.a.T)
 #pragma unroll 4
             for (int tt = t_first; tt <= t_last; tt++) {
               const unsigned bits = __ballot_sync(0xffffffffu, d < p.a.T && mask[tt * p.a.m_t + d * p.a.m_j] != 0);
@@ -284,19 +306,23 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             }
         }
       };
-      uint32_t drafts[4] = {};
+      uint32_t drafts[2] = {};
       if (cur.tile + n > cache_tiles && cur.tile <= cache_tiles) drafts_seen(0, drafts);
       float m = -INFINITY, l = 0.0f;   // m: raw scores
       for (int j = NT == 2 ? 0 : s; j < n; j += NT == 2 ? 1 : 2) {
         const int tile = cur.tile + j, dt = tile - cache_tiles;
         const int live = dt >= 0 ? TA_TILE : cur.len - tile * TA_TILE;
-        uint32_t w[4] = {~0u, ~0u, ~0u, ~0u};
-        if (dt >= 0) {
-          if (dt == 0) w[0] = drafts[0], w[1] = drafts[1], w[2] = drafts[2], w[3] = drafts[3];
-          else drafts_seen(dt, w);
+        uint32_t w[2] = {~0u, ~0u};
+        if (dt == 0) {
+          w[0] = drafts[0], w[1] = drafts[1];
+        } else if (dt > 0) {
+          drafts_seen(dt, w);
         } else if (live < TA_TILE) {
 #pragma unroll
-          for (int i = 0; i < 4; i++) w[i] = live >= 32 * i + 32 ? ~0u : live <= 32 * i ? 0u : (1u << (live - 32 * i)) - 1;
+          for (int i = 0; i < 2; i++) {
+            const int n_live = live - 64 * part - 32 * i;
+            w[i] = n_live >= 32 ? ~0u : n_live <= 0 ? 0u : (1u << n_live) - 1;
+          }
         }
         const bool masked = dt >= 0 || live < TA_TILE;
         wait(s_full + 8 * s, n_s & 1);
@@ -304,30 +330,32 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         __syncwarp();
         tc_after();
         if (warp_ok) {
-          // The scores are read twice, 64 at a time, for the maximum and for the weights: all 128 in registers spill.
-          auto scores = [&](int half, uint32_t (&x)[2][32]) {
-            tmem_ld32(x[0], s_cols + 64 * half);
-            tmem_ld32(x[1], s_cols + 64 * half + 32);
-            wait_ld(x[0]);
-            wait_ld(x[1]);
+          // The scores are read twice, for the maximum and for the weights.
+          auto masked_scores = [&](int c, uint32_t (&x)[32]) {
+            wait_ld(x);
             if (masked) {
 #pragma unroll
-              for (int c = 0; c < 2; c++)
-#pragma unroll
-                for (int i = 0; i < 32; i++) x[c][i] = w[2 * half + c] >> i & 1 ? x[c][i] : 0xff800000u;
+              for (int i = 0; i < 32; i++) x[i] = w[c] >> i & 1 ? x[i] : 0xff800000u;
             }
           };
           float mx[4] = {m, m, m, m};
-#pragma unroll
-          for (int half = 0; half < 2; half++) {
+          {
             uint32_t x[2][32];
-            scores(half, x);
+            tmem_ld32(x[0], s_cols);
+            tmem_ld32(x[1], s_cols + 32);
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
+            for (int c = 0; c < 2; c++) {
+              masked_scores(c, x[c]);
 #pragma unroll
-              for (int c = 0; c < 4; c++) mx[c] = max3(mx[c], __uint_as_float(x[c >> 1][i + 2 * (c & 1)]), __uint_as_float(x[c >> 1][i + 2 * (c & 1) + 1]));
+              for (int i = 0; i < 32; i += 8)
+#pragma unroll
+                for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], __uint_as_float(x[c][i + 2 * e]), __uint_as_float(x[c][i + 2 * e + 1]));
+            }
           }
-          const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          sh.most[s][part][r] = mine;
+          named_barrier(pair, 64);
+          const float m_new = fmaxf(mine, sh.most[s][part ^ 1][r]);
           if (j < 2 - (NT == 2)) {   // the stream's first tile: nothing to scale
             m = m_new;
           } else {
@@ -338,7 +366,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
               l *= f;
               // the products of the tile before have ended: their commit came before that of these scores
 #pragma unroll
-              for (int c = 0; c < 4; c++) {
+              for (int c = 2 * part; c < 2 * part + 2; c++) {
                 uint32_t o[32];
                 tmem_ld32(o, o_cols + 128 * s + 32 * c);
                 wait_ld(o);
@@ -351,15 +379,16 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           const float least = m == -INFINITY ? 0.0f : -m;   // (x - m) scale, not x scale - m scale: the difference of close scores is exact
           float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // two pairs
 #pragma unroll
-          for (int half = 0; half < 2; half++) {
-            uint32_t x[2][32], pr[32];
-            scores(half, x);
+          for (int c = 0; c < 2; c++) {
+            uint32_t x[32], pr[16];
+            tmem_ld32(x, s_cols + 32 * c);
+            masked_scores(c, x);
             // sixteen at a time, step by step, so that no step waits for the one before
 #pragma unroll
-            for (int i0 = 0; i0 < 64; i0 += 16) {
+            for (int i0 = 0; i0 < 32; i0 += 16) {
               float y[16];
 #pragma unroll
-              for (int i = 0; i < 16; i++) y[i] = __uint_as_float(x[i0 >> 5][(i0 & 31) + i]);
+              for (int i = 0; i < 16; i++) y[i] = __uint_as_float(x[i0 + i]);
 #pragma unroll
               for (int i = 0; i < 16; i += 2) add_mul2(y[i], y[i + 1], least, scale);
 #pragma unroll
@@ -370,26 +399,25 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
                 pr[(i0 + i) / 2] = pack2(y[i], y[i + 1]);   // 8 bits of each weight: a tcgen05 product of bf16 values takes bf16 weights; the sum has them all
               }
             }
-            tmem_st32(s_cols + 32 * half, pr);
+            tmem_st16(s_cols + 16 * c, pr);
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tmem_wait_st();
         }
         if (masked) {
           // rows of V that no query sees must be zero, what is not a number in a draft's row must not reach the queries that do not see
-          // it: a weight of zero would not keep it out of the product.  Thread r: row r.
-          const unsigned vq = q0 + 2 * j + 1, row = ring + (vq % NS) * TA_STAGE + r * 128;
+          // it: a weight of zero would not keep it out of the product.  Half a row a thread.
+          const unsigned vq = q0 + 2 * j + 1, row = ring + (vq % NS) * TA_STAGE + part * (TA_STAGE / 2) + r * 128;
           wait(full + 8 * (vq % NS), (vq / NS) & 1);
           if (dt < 0) {
             if (r >= live)
 #pragma unroll
-              for (int c = 0; c < 16; c++)
-                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(row + (c >> 3) * (TA_STAGE / 2) + (c & 7) * 16), "r"(0) : "memory");
+              for (int c = 0; c < 8; c++) asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(row + c * 16), "r"(0) : "memory");
           } else {
             bool bad = false;
 #pragma unroll 4
-            for (int c = 0; c < 16; c++) {
-              const unsigned at = row + (c >> 3) * (TA_STAGE / 2) + (c & 7) * 16;
+            for (int c = 0; c < 8; c++) {
+              const unsigned at = row + c * 16;
               uint32_t v[4];
               asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
               bool here = false;
@@ -422,24 +450,31 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       if (two) wait(o_done + 8, n_o[1]++ & 1);
       __syncwarp();
       tc_after();
-      if (NT == 1) {   // both streams' maxima and sums, through the room of Q
-        const unsigned at = q_smem + r * 8;
-        asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at + s * 1024), "f"(M), "f"(L) : "memory");
-        named_barrier(1, 256);
-        float m2[2], l2[2];
+      {  // maxima and sums of both halves of the keys (NT = 1: and of both streams), through the room of Q
+        const unsigned at = q_smem + (NT == 2 ? s * TA_STAGE : 0) + r * 8;
+        asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(at + ((NT == 2 ? 0 : 2 * s) + part) * 1024), "f"(M), "f"(L) : "memory");
+        named_barrier(NT == 2 ? pair : 1, NT == 2 ? 64 : 512);
+        float m2[2 / NT], l2[2 / NT];
 #pragma unroll
-        for (int i = 0; i < 2; i++) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=f"(m2[i]), "=f"(l2[i]) : "r"(at + i * 1024) : "memory");
-        M = fmaxf(m2[0], m2[1]);
+        for (int i = 0; i < 2 / NT; i++) {
+          float again, more;
+          asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=f"(m2[i]), "=f"(l2[i]) : "r"(at + 2 * i * 1024) : "memory");
+          asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=f"(again), "=f"(more) : "r"(at + (2 * i + 1) * 1024) : "memory");
+          l2[i] += more;
+        }
+        M = NT == 2 ? m2[0] : fmaxf(m2[0], m2[2 / NT - 1]), L = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2; i++) f[i] = m2[i] == -INFINITY ? 0.0f : ex2(m2[i] - M);
-        L = l2[0] * f[0] + l2[1] * f[1];   // (of a stream without tiles: m = -inf, l = 0)
+        for (int i = 0; i < 2 / NT; i++) {
+          f[i] = m2[i] == -INFINITY ? 0.0f : NT == 2 ? 1.0f : ex2(m2[i] - M);
+          L += l2[i] * f[i];   // (of a stream without tiles: m = -inf, l = 0)
+        }
       }
       if (dead) L = NAN;
       if (warp_ok) {
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-          if (NT == 1 && (c >> 1) != s) continue;   // a half of the channels each
+          if (NT == 2 ? (c >> 1) != part : c != 2 * s + part) continue;   // this thread's channels
           uint32_t o[32];
           tmem_ld32(o, o_cols + (NT == 2 ? 128 * s : 0) + 32 * c);
           wait_ld(o);
@@ -479,7 +514,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             }
           }
         }
-        if (row_ok && (NT == 2 || s == 0)) {
+        if (row_ok && part == 0 && (NT == 2 || s == 0)) {
           if (whole) {
             if (p.a.lse) p.a.lse[out_row] = L == 0.0f ? -INFINITY : M + log2f(L);
           } else {
@@ -488,7 +523,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         }
       }
       tc_before();
-      named_barrier(2, 256);   // both streams have read: the room of Q, O and the marks may be written
+      named_barrier(2, 512);   // both streams have read: the room of Q, O and the marks may be written
       if (tid < 8) s_bad[tid] = 0;
       q0 += 2 * n;
     }
@@ -497,12 +532,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
   tc_before();
   __syncthreads();
   tc_after();
-  if (warp == 9 && lane == 0 && s_dead) {   // products under way end before the tensor memory goes
-    tc_commit(ending);
-    for (int it = 0; it < TA_WAIT_LIMIT && !mbar_try(ending, 0); it++) {}
-  }
-  __syncthreads();
-  if (warp == 8) tmem_free(tmem, 512);
+  if (warp == 16) tmem_free(tmem, 512);
 }
 
 // A block per query row: the records of the blocks that share its item, in the order of the tiles.
@@ -542,7 +572,8 @@ int launch_tree(const AttendParams& a, int64_t bs, void* workspace, cudaStream_t
   const int64_t most = bs * a.H * p.row_groups * ((a.cap + TA_TILE - 1) / TA_TILE + p.draft_tiles);
   const int blocks = (int)(most < sm_count() ? most : sm_count());
   static PerDevice opted;
-  constexpr int SMEM = 1024 + (NT + TaRing<NT>::stages) * TA_STAGE;
+  constexpr int SMEM = (NT + TaRing<NT>::stages) * TA_STAGE + (int)sizeof(TreeShared<TaRing<NT>::stages>);
+  static_assert(SMEM <= 227 * 1024, "shared memory of a block");
   if (const unsigned long long bit = first_on_device(opted)) {
     if (cudaFuncSetAttribute(tree_tile_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess)
       return fail(PK_ERR_CUDA, "tree_attention: %s", cudaGetErrorString(cudaGetLastError()));
