@@ -16,7 +16,7 @@ constexpr int FEW_STAGE = 32768;                    // K 64 x 128, V 64 x 128: h
 constexpr int FEW_OS = 136;                         // floats between two rows of a warp's partial: its stores fall into all banks
 constexpr int FEW_SMEM = 1024 + FEW_BUFS * FEW_STAGE;
 static_assert(4 * 8 * FEW_OS * 4 <= FEW_STAGE, "the warps' partials of eight rows take the place of a tile");
-constexpr int FEW_WAIT_LIMIT = 400000;              // (a try waits up to 10 us by itself)
+constexpr int FEW_WAIT_LIMIT = 100000;              // (a try waits up to 10 us by itself)
 
 __host__ __device__ constexpr int few_ctas(int rows) { return rows > 16 ? 1 : 2; }   // blocks per SM: by the registers
 

@@ -30,7 +30,7 @@ constexpr int W4_STAGES_MAX = 6;
 __host__ __device__ constexpr int w4_sums(int nt) { return nt == 1 ? 4 : 2; }
 constexpr uint32_t W4_BIAS = 0x4b400000u;       // the float 2^23 + 2^22: adding a whole number below 2^22 to its bits adds it to the float
 constexpr int W4_LONG = 8;                       // stages of 64 KB per SM from which on boxes are of 512 columns
-constexpr int W4_WAIT_LIMIT = 400000;
+constexpr int W4_WAIT_LIMIT = 100000;
 constexpr int W4_SMEM = 227 * 1024 - 512;   // of a block; 512 bytes of barriers
 
 struct W4Params {

@@ -19,7 +19,7 @@ namespace {
 constexpr int TA_TILE = 128;                   // keys of a tile
 constexpr int TA_THREADS = 576;                // two streams of eight softmax warps, a warp for the copies, a warp for the products
 constexpr int TA_STAGE = 32768;                // a tile of K or V: two halves of 64 channels, 128 rows of 128 bytes
-constexpr int TA_WAIT_LIMIT = 4000000;
+constexpr int TA_WAIT_LIMIT = 100000;          // tries; one waits up to 10 us by itself
 constexpr int TA_FEW = 32;                       // up to so many query rows attend_few.cu has the call
 constexpr float TA_LAZY = 8.0f;                // log2: the maximum that O is scaled to may lie this far below the true one
 
@@ -508,9 +508,12 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
                 dst[i] = make_uint4(y[0], y[1], y[2], y[3]);
               }
             } else {
-              uint4* dst = reinterpret_cast<uint4*>(rec + (int64_t)rec_row * 128 + 32 * c);
+              float* dst = rec + (int64_t)rec_row * 128 + 32 * c;
 #pragma unroll
-              for (int i = 0; i < 8; i++) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+              for (int i = 0; i < 32; i += 8)   // whole sectors
+                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + i), "r"(o[i]), "r"(o[i + 1]), "r"(o[i + 2]), "r"(o[i + 3]), "r"(o[i + 4]),
+                             "r"(o[i + 5]), "r"(o[i + 6]), "r"(o[i + 7])
+                             : "memory");
             }
           }
         }
