@@ -4,6 +4,8 @@
 //               block;  with P_d = sum_g max(q_gd, 0) and N_d = sum_g min(q_gd, 0) it is sum_d P_d hi_jd + N_d lo_jd: one pass over the
 //               bounds whatever the number of query heads.
 // The choice is that of sums in 64 bits, rounded once to 32: it does not depend on their order.
+#include <type_traits>
+
 #include "attend.cuh"
 
 namespace pk {
@@ -126,9 +128,37 @@ __global__ void __launch_bounds__(128, SCORE_CTAS) block_score_kernel(SelectPara
   };
   load(now, self);
   load(next, self + warps);
+  // P and N of the block's tokens, a thread per channel
+  __shared__ __align__(16) float s_sums[TT][2][128];
+  {
+    const int d = threadIdx.x;
+    float up[TT], down[TT];
+#pragma unroll
+    for (int i = 0; i < TT; i++) up[i] = down[i] = 0.0f;
+    const uint16_t* q = p.q + b * p.q_b + (int64_t)h * p.G * p.q_h + d;
+    for (int g0 = 0; g0 < p.G; g0 += 4) {
+      float v[TT][4];
+#pragma unroll
+      for (int i = 0; i < TT; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) v[i][g] = g0 + g < p.G ? bf2f(q[(int64_t)min(t0 + i, p.T - 1) * p.q_t + (g0 + g) * p.q_h]) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < TT; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          if (v[i][g] < 0.0f) down[i] += v[i][g];
+          else up[i] += v[i][g];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TT; i++) s_sums[i][0][d] = down[i], s_sums[i][1][d] = up[i];
+  }
+  __syncthreads();
   float c[TT][8];   // P or N of this lane's channels
 #pragma unroll
-  for (int i = 0; i < TT; i++) query_sums(p, b, min(t0 + i, p.T - 1), h, lane, c[i]);
+  for (int i = 0; i < TT; i++)
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) *reinterpret_cast<float4*>(&c[i][e]) = *reinterpret_cast<const float4*>(&s_sums[i][lane >> 4][8 * (lane & 15) + e]);
   __nv_bfloat162 top[4];   // largest magnitudes of this lane's channels
 #pragma unroll
   for (int e = 0; e < 4; e++) top[e] = __nv_bfloat162(__ushort_as_bfloat16(0), __ushort_as_bfloat16(0));
@@ -175,17 +205,22 @@ __global__ void __launch_bounds__(128, SCORE_CTAS) block_score_kernel(SelectPara
   }
 }
 
-// A block per row.  The keys between the lowest and the highest are counted in 1024 bins of equal width, the bin of the n-th largest is cut again until it
-// is taken whole or holds one value (of which the lowest positions are taken); usually two rounds.  Where the lowest score taken and the highest
-// one left lie closer than the rounding of the scores, those in question are summed again in 64 bits and chosen from once more.  Then the
-// chosen blocks in order, every warp those of its part of the row.  Latency: keys in shared memory where they fit.
-constexpr int PICK_THREADS = 512, PICK_WARPS = PICK_THREADS / 32, PICK_BINS = 1024, PICK_KEPT = 16384;
-__global__ void __launch_bounds__(PICK_THREADS) block_pick_kernel(SelectParams p, bool kept, int warps) {
-  extern __shared__ uint32_t s_keys[];
-  __shared__ unsigned s_bins[PICK_BINS], s_a[PICK_WARPS], s_b[PICK_WARPS], s_c[PICK_WARPS], s_found[3];
+// A block per row, a thread holds KPT of its keys.  The keys between the lowest and the highest are counted in 1024 bins of equal width, the bin of the n-th
+// largest is cut again until it is taken whole or holds one value (of which the lowest positions are taken); usually one or two rounds.
+// What is taken is listed and ranked by position.  Where the lowest score taken and the highest one left lie closer than the rounding of the
+// scores, those in question are summed again in 64 bits and chosen from once more; then, and where a value is taken in part or more than
+// PICK_LIST are, the chosen ones come out in order, every warp those of its part of the row.  Latency: a barrier and a pass over registers a
+// step.  (Keys in shared memory, 512 threads, every row written in order: 32 rows of 8192 keys 10 us, of which 3.5 for the order.)
+constexpr int PICK_THREADS = 1024, PICK_WARPS = PICK_THREADS / 32, PICK_BINS = 1024, PICK_LIST = 1024;
+template <int KPT>
+__global__ void __launch_bounds__(PICK_THREADS) block_pick_kernel(SelectParams p, int warps) {
+  __shared__ unsigned s_bins[2][PICK_BINS], s_a[PICK_WARPS], s_b[PICK_WARPS], s_c[PICK_WARPS], s_d[PICK_WARPS], s_found[3], s_n;
+  __shared__ int s_list[PICK_LIST];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.x, t = row / p.H % p.T, b = row / p.H / p.T;
   const int h = (int)(row % p.H);
+  s_bins[0][tid] = 0, s_bins[1][tid] = 0;
+  if (tid == 0) s_n = 0;
   pdl_wait();
   pdl_trigger();
   const int seen = visible_blocks(p, b, (int)t);
@@ -196,66 +231,58 @@ __global__ void __launch_bounds__(PICK_THREADS) block_pick_kernel(SelectParams p
     for (int i = tid; i < seen; i += PICK_THREADS) ids[i] = i;
     return;
   }
-  auto key = [&](int j) { return kept ? s_keys[j] : stored[j]; };
-  auto put = [&](int j, uint32_t k) {
-    if (kept) s_keys[j] = k;
-    else stored[j] = k;
+  // KPT = 0: more keys than fit, read from global memory in every pass
+  uint32_t kept[KPT > 0 ? KPT : 1];
+  if (KPT > 0)
+#pragma unroll
+    for (int i = 0; i < KPT; i++) kept[i] = i * PICK_THREADS + tid < seen ? stored[i * PICK_THREADS + tid] : 0u;
+  // f(position, key) for this thread's keys; 0 is the key of what is not chosen from
+  auto each = [&](auto&& f) {
+    if (KPT > 0) {
+#pragma unroll
+      for (int i = 0; i < KPT; i++)
+        if (i * PICK_THREADS + tid < seen) f(i * PICK_THREADS + tid, kept[i]);
+    } else {
+      for (int j = tid; j < seen; j += PICK_THREADS) f(j, stored[j]);
+    }
   };
   auto value = [](uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k); };
-  // lowest, highest and sum over the block, to every thread
-  auto range = [&](uint32_t& lo, uint32_t& hi, unsigned& n) {
-    lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi), n = __reduce_add_sync(0xffffffffu, n);
+  // lowest, two highest and a sum over the block, to every thread
+  auto range = [&](uint32_t& lo, uint32_t& hi, uint32_t& hi2, unsigned& n) {
+    lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi), hi2 = __reduce_max_sync(0xffffffffu, hi2), n = __reduce_add_sync(0xffffffffu, n);
     __syncthreads();
-    if (lane == 0) s_a[warp] = lo, s_b[warp] = hi, s_c[warp] = n;
+    if (lane == 0) s_a[warp] = lo, s_b[warp] = hi, s_c[warp] = n, s_d[warp] = hi2;
     __syncthreads();
-    lo = __reduce_min_sync(0xffffffffu, s_a[lane % PICK_WARPS]), hi = __reduce_max_sync(0xffffffffu, s_b[lane % PICK_WARPS]);
-    n = __reduce_add_sync(0xffffffffu, lane < PICK_WARPS ? s_c[lane] : 0u);
+    lo = __reduce_min_sync(0xffffffffu, s_a[lane]), hi = __reduce_max_sync(0xffffffffu, s_b[lane]);
+    n = __reduce_add_sync(0xffffffffu, s_c[lane]), hi2 = __reduce_max_sync(0xffffffffu, s_d[lane]);
   };
-  float A = 0.0f;
+  uint32_t lo = 0xffffffffu, hi = 0, limit = 0;   // extremes of the keys that are not FORCED; the largest limit's bits
+  unsigned forced = 0;
   for (int i = tid; i < warps; i += PICK_THREADS) {
     const float a = p.limits[row * warps + i];
-    A = a <= 3.0e38f ? fmaxf(A, a) : INFINITY;
-    if (!(A < INFINITY)) break;
+    limit = max(limit, a <= 3.0e38f ? __float_as_uint(a) : 0x7f800000u);
   }
-  uint32_t lo = 0xffffffffu, hi = 0;   // extremes of the keys that are not FORCED
-  unsigned forced = 0;
-  for (int j0 = tid; j0 < seen; j0 += 8 * PICK_THREADS) {
-    uint32_t k[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) k[i] = stored[min(j0 + i * PICK_THREADS, seen - 1)];
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (j0 + i * PICK_THREADS < seen) {
-        if (kept) s_keys[j0 + i * PICK_THREADS] = k[i];
-        if (k[i] == FORCED) forced++;
-        else lo = min(lo, k[i]), hi = max(hi, k[i]);
-      }
-  }
-  range(lo, hi, forced);
-  {
-    uint32_t a0 = 0, a1 = __float_as_uint(A);
-    unsigned none = 0;
-    range(a0, a1, none);
-    A = __uint_as_float(a1);
-  }
-  unsigned want;
-  for (bool exact = false;; exact = true) {
-    // (more blocks than are taken are seen, and the forced ones are at most n: there are others)
-    want = (unsigned)p.n - forced;   // of the keys in [lo, hi]; those above hi are taken
+  each([&](int, uint32_t k) {
+    if (k == FORCED) forced++;
+    else lo = min(lo, k), hi = max(hi, k);
+  });
+  range(lo, hi, limit, forced);
+  const float A = __uint_as_float(limit);
+  unsigned want = 0;
+  int round = 0;
+  // Narrows [lo, hi] to keys of which `want` are taken (all of them, or equal ones), those above hi being taken as well.
+  auto narrow = [&]() {
+    want = (unsigned)p.n - forced;   // (more blocks than are taken are seen, and the forced ones are at most n: there are others)
     unsigned in_range = 0xffffffffu;
-    while (want > 0 && want != in_range && lo != hi) {
+    for (; want > 0 && want != in_range && lo != hi; round++) {
+      unsigned* bins = s_bins[round & 1];
       const int shift = max(0, 22 - __clz(hi - lo));   // (hi - lo) >> shift < 1024
+      each([&](int, uint32_t k) {
+        if (k >= lo && k <= hi && k != FORCED) atomicAdd(&bins[(k - lo) >> shift], 1u);
+      });
       __syncthreads();
-      for (int i = tid; i < PICK_BINS; i += PICK_THREADS) s_bins[i] = 0;
-      __syncthreads();
-      for (int j = tid; j < seen; j += PICK_THREADS) {
-        const uint32_t k = key(j);
-        if (k >= lo && k <= hi && k != FORCED) atomicAdd(&s_bins[(k - lo) >> shift], 1u);
-      }
-      __syncthreads();
-      // thread i: bins 1023 - 2 i and 1022 - 2 i, from the highest down
-      const unsigned c0 = s_bins[PICK_BINS - 1 - 2 * tid], c1 = s_bins[PICK_BINS - 2 - 2 * tid];
-      unsigned sum = c0 + c1;
+      const unsigned c = bins[PICK_BINS - 1 - tid];   // from the highest down
+      unsigned sum = c;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
         const unsigned o = __shfl_up_sync(0xffffffffu, sum, off);
@@ -263,83 +290,113 @@ __global__ void __launch_bounds__(PICK_THREADS) block_pick_kernel(SelectParams p
       }
       if (lane == 31) s_a[warp] = sum;
       __syncthreads();
-      const unsigned before = __reduce_add_sync(0xffffffffu, lane < warp ? s_a[lane & (PICK_WARPS - 1)] : 0u) + sum - c0 - c1;
-      if (before < want && before + c0 >= want) s_found[0] = PICK_BINS - 1 - 2 * tid, s_found[1] = before, s_found[2] = c0;
-      else if (before + c0 < want && before + c0 + c1 >= want) s_found[0] = PICK_BINS - 2 - 2 * tid, s_found[1] = before + c0, s_found[2] = c1;
+      bins[PICK_BINS - 1 - tid] = 0;   // for the round after the next
+      const unsigned before = __reduce_add_sync(0xffffffffu, lane < warp ? s_a[lane] : 0u) + sum - c;
+      if (before < want && before + c >= want) s_found[0] = PICK_BINS - 1 - tid, s_found[1] = before, s_found[2] = c;
       __syncthreads();
       lo += s_found[0] << shift;
       hi = min(hi, lo + ((1u << shift) - 1));
       want -= s_found[1], in_range = s_found[2];
     }
-    if (exact || want + forced == 0 || forced == (unsigned)p.n) break;
-    // the lowest key taken and the highest one left ([lo, hi] is taken whole, or holds one key and is taken in part)
-    const bool part = lo == hi && want != in_range;
-    uint32_t low = 0xffffffffu, high = 0;
+    return lo == hi && want != in_range;   // taken in part
+  };
+  bool part = narrow(), listed = p.n <= PICK_LIST;
+  {
+    // the lowest key taken and the highest one left, and the list of what is taken
+    uint32_t low = 0xffffffffu, high = 0, high2 = 0;
     unsigned none = 0;
-    for (int j = tid; j < seen; j += PICK_THREADS) {
-      const uint32_t k = key(j);
-      if (k == FORCED) continue;
-      if (k >= lo) low = min(low, k);
-      if (k < lo || part) high = max(high, k <= hi ? k : 0u);
-    }
-    range(low, high, none);
+    const bool only_forced = forced == (unsigned)p.n;
+    each([&](int j, uint32_t k) {
+      const bool taken = k == FORCED || (!only_forced && k >= lo);
+      if (k != FORCED) {
+        if (taken) low = min(low, k);
+        if (!taken || part) high = max(high, k <= hi || only_forced ? k : 0u);
+      }
+      if (taken && listed && !part) {
+        const unsigned at = atomicAdd(&s_n, 1u);
+        if (at < PICK_LIST) s_list[at] = j;
+      }
+    });
+    range(low, high, high2, none);
     const float margin = 2.5f * (float)(p.G + 14) * 0x1p-24f * A;   // of each of two scores G + 13 roundings and one more to 32 bits, with room
     const bool odd = !(A < 3.0e38f);
-    if (!odd && !part && value(low) - value(high) > margin) break;
-    if (!odd && part && 0.0f == A) break;   // zeros all
-    const float upper = value(high) + margin, lower = value(low) - margin;
-    // those in question, a warp each; the others are settled
-    double c[8];
-    query_sums(p, b, (int)t, h, lane, c);
-    const uint16_t* bounds = p.bounds + b * p.o_b + h * p.o_h + 8 * lane;
-    lo = 0xffffffffu, hi = 0, forced = 0;
-    __syncthreads();
-    for (int j0 = 32 * warp; j0 < seen; j0 += PICK_THREADS) {
-      uint32_t k = j0 + lane < seen ? key(j0 + lane) : 0u;
-      bool open = false;
-      if (k != FORCED && k != 0) {
-        const float s = value(k);
-        open = odd || (s <= upper && s >= lower);
-        if (!open) k = s > upper ? FORCED : 0u;
+    const bool settled = only_forced || (!odd && (part ? A == 0.0f : value(low) - value(high) > margin));
+    if (settled && listed && !part) {
+      for (int i = tid; i < p.n; i += PICK_THREADS) {
+        const int j = s_list[i];
+        int rank = 0;
+        for (int o = 0; o < p.n; o++) rank += s_list[o] < j;
+        ids[rank] = j;
       }
-      for (unsigned left = __ballot_sync(0xffffffffu, open); left; left &= left - 1) {
-        const int i = __ffs(left) - 1;
-        const uint4 x = *reinterpret_cast<const uint4*>(bounds + (int64_t)(j0 + i) * p.o_j);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-        double s = 0.0;
-#pragma unroll
-        for (int e = 0; e < 8; e++)   // (no products of a zero with an infinite bound)
-          if (!(c[e] == 0.0)) s = fma(c[e], (double)__uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16), s);
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        const float f = (float)s + 0.0f;
-        if (lane == i) k = f != f ? NOT_A_NUMBER : ord_key(f);
-      }
-      if (j0 + lane < seen) {
-        put(j0 + lane, k);
-        if (k == FORCED) forced++;
-        else lo = min(lo, k), hi = max(hi, k);
-      }
+      return;
     }
-    range(lo, hi, forced);
-    __syncthreads();
+    if (!settled) {
+      const float upper = value(high) + margin, lower = value(low) - margin;
+      // those in question, a warp each; the others are settled
+      double c[8];
+      query_sums(p, b, (int)t, h, lane, c);
+      const uint16_t* bounds = p.bounds + b * p.o_b + h * p.o_h + 8 * lane;
+      lo = 0xffffffffu, hi = 0, forced = 0;
+      auto again = [&](int j, uint32_t k) -> uint32_t {   // by a whole warp: j of its lanes
+        bool open = false;
+        if (j < seen && k != FORCED && k != 0) {
+          const float s = value(k);
+          open = odd || (s <= upper && s >= lower);
+          if (!open) k = s > upper ? FORCED : 0u;
+        }
+        for (unsigned left = __ballot_sync(0xffffffffu, open); left; left &= left - 1) {
+          const int i = __ffs(left) - 1;
+          const uint4 x = *reinterpret_cast<const uint4*>(bounds + (int64_t)(j - lane + i) * p.o_j);
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          double s = 0.0;
+#pragma unroll
+          for (int e = 0; e < 8; e++)   // (no products of a zero with an infinite bound)
+            if (!(c[e] == 0.0)) s = fma(c[e], (double)__uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16), s);
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+          const float f = (float)s + 0.0f;
+          if (lane == i) k = f != f ? NOT_A_NUMBER : ord_key(f);
+        }
+        if (j < seen) {
+          if (k == FORCED) forced++;
+          else lo = min(lo, k), hi = max(hi, k);
+        }
+        return k;
+      };
+      if (KPT > 0) {
+#pragma unroll
+        for (int i = 0; i < KPT; i++) kept[i] = again(i * PICK_THREADS + tid, kept[i]);
+      } else {
+        for (int j0 = 32 * warp; j0 < seen; j0 += PICK_THREADS) {
+          const uint32_t k = again(j0 + lane, j0 + lane < seen ? stored[j0 + lane] : 0u);
+          if (j0 + lane < seen) stored[j0 + lane] = k;
+        }
+      }
+      uint32_t none2 = 0;
+      range(lo, hi, none2, forced);
+      narrow();
+    }
   }
-  // above hi: taken; in [lo, hi]: the first `want` (all of them, or equal ones)
+  // In order: above hi, or FORCED: taken; in [lo, hi]: the first `want`.
+  auto is_above = [&](uint32_t k) { return k == FORCED || (want > 0 && k > hi); };
+  if (KPT > 0)
+#pragma unroll
+    for (int i = 0; i < KPT; i++)
+      if (i * PICK_THREADS + tid < seen) stored[i * PICK_THREADS + tid] = kept[i];
+  __syncthreads();
   const int per = ((seen + PICK_WARPS - 1) / PICK_WARPS + 31) / 32 * 32, j0 = min(seen, warp * per), j1 = min(seen, j0 + per);
-  auto is_above = [&](uint32_t k) { return k == FORCED || (want > 0 ? k > hi : false); };
   unsigned above = 0, inside = 0;
   for (int j = j0 + lane; j < j1; j += 32) {
-    const uint32_t k = key(j);
+    const uint32_t k = stored[j];
     if (is_above(k)) above++;
     else if (k >= lo && want > 0) inside++;
   }
   above = __reduce_add_sync(0xffffffffu, above), inside = __reduce_add_sync(0xffffffffu, inside);
-  __syncthreads();
   if (lane == 0) s_a[warp] = above, s_b[warp] = inside;
   __syncthreads();
-  unsigned n_above = __reduce_add_sync(0xffffffffu, lane < warp ? s_a[lane & (PICK_WARPS - 1)] : 0u), n_inside = __reduce_add_sync(0xffffffffu, lane < warp ? s_b[lane & (PICK_WARPS - 1)] : 0u);
+  unsigned n_above = __reduce_add_sync(0xffffffffu, lane < warp ? s_a[lane] : 0u), n_inside = __reduce_add_sync(0xffffffffu, lane < warp ? s_b[lane] : 0u);
   for (int j = j0; j < j1; j += 32) {
-    const uint32_t k = j + lane < j1 ? key(j + lane) : 0;
+    const uint32_t k = j + lane < j1 ? stored[j + lane] : 0;
     const bool a = j + lane < j1 && is_above(k), i = j + lane < j1 && !a && want > 0 && k >= lo;
     const unsigned ab = __ballot_sync(0xffffffffu, a), ib = __ballot_sync(0xffffffffu, i), below = (1u << lane) - 1;
     const unsigned i_at = n_inside + __popc(ib & below), at = n_above + __popc(ab & below) + min(i_at, want);
@@ -425,15 +482,12 @@ extern "C" int pk_select_blocks(const pk_tensor* queries, const pk_tensor* bound
   if (tt == 1) launch_chain(block_score_kernel<1>, grid, dim3(128), 0, (cudaStream_t)stream, p);
   else if (tt == 2) launch_chain(block_score_kernel<2>, grid, dim3(128), 0, (cudaStream_t)stream, p);
   else launch_chain(block_score_kernel<4>, grid, dim3(128), 0, (cudaStream_t)stream, p);
-  const bool kept = nb <= PICK_KEPT;
-  if (kept && nb * 4 > 40 * 1024) {
-    static PerDevice opted;
-    if (const unsigned long long bit = first_on_device(opted)) {
-      if (cudaFuncSetAttribute(block_pick_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PICK_KEPT * 4) != cudaSuccess)
-        return fail(PK_ERR_CUDA, "select_blocks: %s", cudaGetErrorString(cudaGetLastError()));
-      mark_on_device(opted, bit);
-    }
-  }
-  launch_chain(block_pick_kernel, dim3((unsigned)rows), dim3(PICK_THREADS), kept ? (size_t)nb * 4 : 0, (cudaStream_t)stream, p, kept, (int)grid.x * 4);
+  auto pick = [&](auto kpt) {
+    launch_chain(block_pick_kernel<decltype(kpt)::value>, dim3((unsigned)rows), dim3(PICK_THREADS), 0, (cudaStream_t)stream, p, (int)grid.x * 4);
+  };
+  if (nb <= PICK_THREADS) pick(std::integral_constant<int, 1>());
+  else if (nb <= 4 * PICK_THREADS) pick(std::integral_constant<int, 4>());
+  else if (nb <= 16 * PICK_THREADS) pick(std::integral_constant<int, 16>());
+  else pick(std::integral_constant<int, 0>());
   return check_launch("select_blocks", 2);
 }
