@@ -106,9 +106,9 @@ __device__ __forceinline__ void query_sums(const SelectParams& p, int64_t b, int
 // A warp takes eight blocks of keys at a time, 4 KB that are in flight at once, for TT tokens: lanes 0 .. 15 hold eight channels of lo and N each, the
 // others of hi and P.  Bounded by the bounds' bytes where there are many, otherwise by latency.  (64-bit sums throughout: 8192 blocks of 8
 // heads for four tokens 46 us, of 128 heads x 770 blocks for one 26 us; the conversions to 64 bits alone, 8 a clock and SM, take longer than the bytes.)
-constexpr int SCORE_CTAS = 3;   // blocks per SM
+__host__ __device__ constexpr int score_ctas(int tt) { return tt <= 2 ? 3 : 2; }   // blocks per SM, by the registers
 template <int TT>
-__global__ void __launch_bounds__(128, SCORE_CTAS) block_score_kernel(SelectParams p) {
+__global__ void __launch_bounds__(128, score_ctas(TT)) block_score_kernel(SelectParams p) {
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, h = blockIdx.y % p.H, t0 = blockIdx.y / p.H * TT;
@@ -475,7 +475,7 @@ extern "C" int pk_select_blocks(const pk_tensor* queries, const pk_tensor* bound
   StageTimer timer(ST_RANK, (cudaStream_t)stream);
   // tokens share what is read, four at a time; one wave where that is possible, a warp eight blocks of keys a step
   const int tt = T >= 3 ? 4 : (int)T;
-  const int64_t per_head = (nb + 31) / 32, heads = H * ((T + tt - 1) / tt), slots = (int64_t)SCORE_CTAS * sm_count() / (heads * bs), room = slots < 1 ? 1 : slots;
+  const int64_t per_head = (nb + 31) / 32, heads = H * ((T + tt - 1) / tt), slots = (int64_t)score_ctas(tt) * sm_count() / (heads * bs), room = slots < 1 ? 1 : slots;
   PK_REQUIRE(heads < 65536, "at most 65535 KV heads x token groups");
   const dim3 grid((unsigned)(per_head < room ? per_head : room), (unsigned)heads, (unsigned)bs);
   p.limits = (float*)(p.keys + rows * nb);
