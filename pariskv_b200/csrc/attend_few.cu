@@ -29,32 +29,34 @@ struct FewParams {
   float* records;     // [2 * blocks][rows * 130]
 };
 
-__device__ __forceinline__ int few_len(const FewParams& p, int b) { return (int)min((int64_t)max(p.a.lengths[b], 0), p.a.cap); }
-
-// Where the tiles of an item lie: tree: samples of different lengths; blocks: all items alike.
-struct Place {
-  int64_t total;
-  int64_t before;   // tiles of the samples before `sample` (tree)
+struct TilePlan {
+  int64_t total;    // tiles of the launch
+  int64_t before;   // tiles of the samples before `sample`
   int sample;
 };
-template <bool TREE, typename At>
-__device__ __forceinline__ Place few_place(const FewParams& p, At at) {   // by a whole warp
-  if (!TREE) return {(int64_t)p.bs * p.a.T * p.a.H * p.row_groups * p.tiles, 0, 0};
+// By a whole warp: the total, and the sample that holds tile share_begin(total, block, min(blocks, total)); tiles_of(b): tiles of sample b, 0 behind the last.
+template <class TilesOf>
+__device__ __forceinline__ TilePlan tile_plan(int bs, unsigned block, unsigned blocks, TilesOf tiles_of) {
   const int lane = threadIdx.x & 31;
-  auto tiles_of = [&](int b) { return b < p.bs ? p.a.H * ((few_len(p, b) + FEW_TILE - 1) / FEW_TILE + 1) : 0; };
-  int64_t total = 0;
-  for (int b0 = 0; b0 < p.bs; b0 += 32) total += __reduce_add_sync(0xffffffffu, tiles_of(b0 + lane));
-  const int64_t t = at(total);
-  Place r = {total, 0, 0};
-  for (int b0 = 0; b0 < p.bs; b0 += 32) {
-    const int64_t mine = tiles_of(b0 + lane);
+  const int64_t first = tiles_of(lane);
+  TilePlan r = {0, 0, 0};
+  auto sum = [](int64_t v) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    return v;
+  };
+  r.total = sum(first);
+  for (int b0 = 32; b0 < bs; b0 += 32) r.total += sum(tiles_of(b0 + lane));
+  const int64_t t = share_begin(r.total, block, (unsigned)min((int64_t)blocks, r.total));
+  for (int b0 = 0; b0 < bs; b0 += 32) {
+    const int64_t mine = b0 == 0 ? first : tiles_of(b0 + lane);
     int64_t end = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const int64_t o = __shfl_up_sync(0xffffffffu, end, off);
       if (lane >= off) end += o;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, b0 + lane < p.bs && r.before + end > t);
+    const unsigned past = __ballot_sync(0xffffffffu, b0 + lane < bs && r.before + end > t);
     if (past) {
       const int i = __ffs(past) - 1;
       r.sample = b0 + i, r.before += __shfl_sync(0xffffffffu, end - mine, i);
@@ -65,16 +67,22 @@ __device__ __forceinline__ Place few_place(const FewParams& p, At at) {   // by 
   return r;
 }
 
+__device__ __forceinline__ int few_len(const FewParams& p, int b) { return (int)min((int64_t)max(p.a.lengths[b], 0), p.a.cap); }
+
+__device__ __forceinline__ int few_tiles(const FewParams& p, int b) {   // of a tree's item
+  return (few_len(p, b) + FEW_TILE - 1) / FEW_TILE + 1;
+}
+
 // A way through consecutive tiles.
 template <bool TREE>
 struct FewCursor {
   int b, t, h, group, len, n, tile;   // len: rows of the cache (tree), rows up to the token's position (blocks)
   __device__ __forceinline__ void sample(const FewParams& p) {
     const int rows = few_len(p, b);
-    if (TREE) len = rows, n = (rows + FEW_TILE - 1) / FEW_TILE + 1;
+    if (TREE) len = rows, n = few_tiles(p, b);
     else len = max(rows - p.a.T + t + 1, 0), n = p.tiles;
   }
-  __device__ __forceinline__ void start(const FewParams& p, const Place& w, int64_t first) {
+  __device__ __forceinline__ void start(const FewParams& p, const TilePlan& w, int64_t first) {
     if (TREE) {
       b = w.sample, t = 0, group = 0;
       sample(p);
@@ -129,7 +137,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
   __shared__ unsigned char s_live[FEW_BUFS][4];   // keys of each warp's sixteen that are seen (tree: by all tokens)
   __shared__ uint32_t s_mask[32], s_bad;
   __shared__ volatile int s_dead;
-  __shared__ Place s_place;
+  __shared__ TilePlan s_place;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const unsigned base = (smem_addr(dyn) + 1023) & ~1023u, full = smem_addr(bars), empty = full + 8 * FEW_BUFS;
   if (tid == 0) {
@@ -143,18 +151,16 @@ __global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
   const int blocks = (int)gridDim.x;
   if (TREE) {
     if (warp == 0) {
-      const Place w = few_place<TREE>(p, [&](int64_t total) { return total * blockIdx.x / min((int64_t)blocks, total); });
+      const TilePlan w = tile_plan(p.bs, blockIdx.x, (unsigned)blocks, [&](int b) -> int64_t { return b < p.bs ? (int64_t)p.a.H * few_tiles(p, b) : 0; });
       if (lane == 0) s_place = w;
     }
-  } else if (tid == 0) {
-    s_place = few_place<TREE>(p, [](int64_t) { return (int64_t)0; });
+    __syncthreads();
   }
-  __syncthreads();
-  const Place place = s_place;
-  const int64_t shares = min((int64_t)blocks, place.total);
+  const TilePlan place = TREE ? s_place : TilePlan{(int64_t)p.bs * p.a.T * p.a.H * p.row_groups * p.tiles, 0, 0};
+  const unsigned shares = (unsigned)min((int64_t)blocks, place.total);
   if (blockIdx.x >= shares) return;
-  const int64_t first = place.total * blockIdx.x / shares;
-  const int count = (int)(place.total * (blockIdx.x + 1) / shares - first);
+  const int64_t first = share_begin(place.total, blockIdx.x, shares);
+  const int count = (int)(share_begin(place.total, blockIdx.x + 1, shares) - first);
   FewCursor<TREE> cur;
   cur.start(p, place, first);
 
@@ -448,18 +454,17 @@ __global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ 
   if (TREE) {
     int64_t before = 0;
     for (int b0 = 0; b0 < p.bs; b0 += 32) {
-      const int tiles = b0 + lane < p.bs ? (few_len(p, b0 + lane) + FEW_TILE - 1) / FEW_TILE + 1 : 0;
+      const int tiles = b0 + lane < p.bs ? few_tiles(p, b0 + lane) : 0;
       total += (int64_t)p.a.H * __reduce_add_sync(0xffffffffu, tiles), before += (int64_t)p.a.H * __reduce_add_sync(0xffffffffu, b0 + lane < b ? tiles : 0);
     }
-    n = (few_len(p, b) + FEW_TILE - 1) / FEW_TILE + 1;
+    n = few_tiles(p, b);
     first = before + (int64_t)h * n;
   } else {
     n = p.tiles, total = (int64_t)p.bs * p.a.T * p.a.H * p.row_groups * n;
     first = ((bt * p.a.H + h) * p.row_groups + g / ROWS) * n;
   }
-  const int64_t shares = min((int64_t)blocks, total);
-  auto owner = [&](int64_t x) { return (int)(((x + 1) * shares - 1) / total); };
-  const int c0 = owner(first), c1 = owner(first + n - 1);
+  const unsigned shares = (unsigned)min((int64_t)blocks, total);
+  const int c0 = share_owner(first, total, shares), c1 = share_owner(first + n - 1, total, shares);
   if (c0 == c1) return;   // written by its block
   merge_row(shared, c1 - c0 + 1, ROWS, r, [&](int i) { return p.records + (2 * (int64_t)(c0 + i) + (i == 0)) * (ROWS * 130); }, p.a.out + row * 128, p.a.lse ? p.a.lse + row : nullptr);
 }

@@ -40,6 +40,14 @@ __device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {   // the values are
 __device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ bool not_finite(uint32_t bf16) { return (bf16 & 0x7f80u) == 0x7f80u; }
 
+// ---- equal ranges of the tiles of all items, laid end to end; the lengths come from device memory ----
+// Where the range of block i of `shares` begins, and which block has tile x.
+__device__ __forceinline__ int64_t share_begin(int64_t total, unsigned i, unsigned shares) {
+  return total < 1 << 22 ? (unsigned)total * i / shares : total * i / shares;   // (a division of 64 bits takes a hundred clocks)
+}
+__device__ __forceinline__ int share_owner(int64_t x, int64_t total, unsigned shares) {
+  return total < 1 << 22 ? (int)(((unsigned)(x + 1) * shares - 1) / (unsigned)total) : (int)(((x + 1) * shares - 1) / total);
+}
 // Joins n partial results of a query row, record(i) = O rows of 128, then `rows` values m (log2), then `rows` sums l, in the order of i: a block of 128
 // threads.  A warp takes every fourth record, four channels a lane, eight loads in flight; latency is what bounds it.
 struct MergeShared {

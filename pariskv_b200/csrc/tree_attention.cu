@@ -35,7 +35,7 @@ struct TreeParams {
 };
 
 // Tiles of an item of sample b, and where the items of a sample begin in the sequence of all tiles.
-struct TilePlan {
+struct TreePlan {
   int64_t total;       // tiles of the launch
   int64_t before;      // tiles of the samples before `sample`
   int sample;
@@ -44,7 +44,7 @@ __device__ __forceinline__ int tree_len(const TreeParams& p, int b) { return (in
 __device__ __forceinline__ int tree_tiles(const TreeParams& p, int len) { return (len + TA_TILE - 1) / TA_TILE + p.draft_tiles; }
 // By one warp: the total, and the sample that holds tile `at(total)`.
 template <typename At>
-__device__ __forceinline__ TilePlan tile_plan(const TreeParams& p, At at) {
+__device__ __forceinline__ TreePlan tree_plan(const TreeParams& p, At at) {
   const int lane = threadIdx.x & 31;
   const int64_t items = (int64_t)p.a.H * p.row_groups;
   int64_t total = 0;
@@ -53,7 +53,7 @@ __device__ __forceinline__ TilePlan tile_plan(const TreeParams& p, At at) {
     total += items * __reduce_add_sync(0xffffffffu, n);
   }
   const int64_t t = at(total);
-  TilePlan r = {total, 0, 0};
+  TreePlan r = {total, 0, 0};
   for (int b0 = 0; b0 < p.bs; b0 += 32) {
     const int64_t mine = b0 + lane < p.bs ? items * tree_tiles(p, tree_len(p, b0 + lane)) : 0;
     int64_t end = mine;
@@ -96,7 +96,7 @@ template <int NS>
 struct TreeShared {
   unsigned long long bars[2 * NS + 8];
   float most[2][2][128];   // [stream][half of the keys][row]: maxima, on their way to the other half
-  TilePlan plan;
+  TreePlan plan;
   unsigned tmem, bad[8];   // bad: drafts whose rows of V hold what is not a number
   int dead;
 };
@@ -127,14 +127,14 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
   pdl_trigger();
   const int blocks = (int)gridDim.x;
   if (warp == 0) {
-    const TilePlan plan = tile_plan(p, [&](int64_t total) { return total * blockIdx.x / min((int64_t)blocks, total); });
+    const TreePlan plan = tree_plan(p, [&](int64_t total) { return total * blockIdx.x / min((int64_t)blocks, total); });
     if (lane == 0) sh.plan = plan;
   }
   tc_before();
   __syncthreads();
   tc_after();
   const unsigned tmem = sh.tmem;
-  const TilePlan plan = sh.plan;
+  const TreePlan plan = sh.plan;
   const int64_t shares = min((int64_t)blocks, plan.total);
   Cursor cur;
   {
@@ -555,9 +555,9 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
     total += items * __reduce_add_sync(0xffffffffu, n), before += items * __reduce_add_sync(0xffffffffu, b0 + lane < b ? n : 0);
   }
   const int n = tree_tiles(p, tree_len(p, b));
-  const int64_t first = before + ((int64_t)h * p.row_groups + group) * n, last = first + n - 1, shares = min((int64_t)blocks, total);
-  auto owner = [&](int64_t x) { return (int)(((x + 1) * shares - 1) / total); };
-  const int c0 = owner(first), c1 = owner(last);
+  const int64_t first = before + ((int64_t)h * p.row_groups + group) * n, last = first + n - 1;
+  const unsigned shares = (unsigned)min((int64_t)blocks, total);
+  const int c0 = share_owner(first, total, shares), c1 = share_owner(last, total, shares);
   if (c0 == c1) return;   // written by its block
   constexpr int ROWS = NT * 128;
   merge_row(shared, c1 - c0 + 1, ROWS, r, [&](int i) { return p.records + (2 * (int64_t)(c0 + i) + (i == 0)) * (ROWS * 130); }, p.a.out + row * 128, p.a.lse ? p.a.lse + row : nullptr);
