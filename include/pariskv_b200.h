@@ -533,7 +533,7 @@ int pk_gemv(const pk_tensor* weight, const pk_tensor* x, const pk_tensor* out, i
  * so that a captured step stays valid while the sequences grow.  Rows of 128 bf16 with a unit inner stride, the other strides
  * multiples of 8 elements, 16-byte aligned.  A query that sees no row gets zeros, and lse = -inf.  What a query does not see
  * does not reach it, whatever is stored there (NaN and infinities included).  lse (f32 [bs,T,Hq] or NULL) is the log2 of the
- * softmax denominator, as in pk_sparse_attention.  workspace: device, 256-byte aligned, pk_*_workspace_bytes; nothing in it
+ * softmax denominator, as in pk_sparse_attention; scale has to be positive.  workspace: device, 256-byte aligned, pk_*_workspace_bytes; nothing in it
  * has to be cleared and nothing carries over between calls.  No counterpart in the reference.
  *
  * pk_tree_attention: T drafted tokens per sequence (at most 256) attend to rows [0, lengths[b]) of the cache and to the drafts that
@@ -553,7 +553,8 @@ int pk_gemv(const pk_tensor* weight, const pk_tensor* x, const pk_tensor* out, i
  *   and blocks behind the position are skipped; the order is free; a block listed twice counts twice.
  * pk_gemv_w4: out[T,O] = x[T,I] W^T for up to 16 tokens, fp32 sums.  weight u8 [O,I/2], the low nibble of a byte the even column;
  *   scales bf16 [O,I/group], group 32, 64 or 128; W = (code - 8) * scale, or code * scale + offset with offsets bf16 like scales.
- *   gated: weight is [gate; up] stacked, out[T,O/2] = silu(gate x) * (up x), rounded once.  I at most 32768. */
+ *   gated: weight is [gate; up] stacked, out[T,O/2] = silu(gate x) * (up x), rounded once.  I at most 32768.  A token with an infinity
+ *   or NaN comes out as NaN, the others do not notice. */
 int64_t pk_tree_attention_workspace_bytes(int64_t bs, int64_t T, int64_t Hq, int64_t H, int64_t cap);
 int pk_tree_attention(const pk_tensor* queries, const pk_tensor* keys, const pk_tensor* values, const pk_tensor* draft_keys,
                       const pk_tensor* draft_values, const pk_tensor* tree_mask, const pk_tensor* lengths, float scale,

@@ -498,7 +498,6 @@ int launch_attend_few(const AttendParams& a, int64_t bs, void* workspace, const 
   p.row_groups = tree ? 1 : (a.G + per - 1) / per;
   p.box = tree ? FEW_TILE : a.block < FEW_TILE ? a.block : FEW_TILE;
   p.tiles = tree ? 0 : (int)(((int64_t)a.n * a.block + FEW_TILE - 1) / FEW_TILE);
-  if (!tree && p.tiles == 0) return launch_attend_rows(a, bs, what, st);
   CUtensorMap maps[4];
   bool ok = rows_map(&maps[0], a.k, a.cap, a.k_l, a.H, a.k_h, bs, a.k_b, p.box) && rows_map(&maps[1], a.v, a.cap, a.v_l, a.H, a.v_h, bs, a.v_b, p.box);
   if (tree) ok = ok && rows_map(&maps[2], a.dk, a.T, a.dk_t, a.H, a.dk_h, bs, a.dk_b, 32) && rows_map(&maps[3], a.dv, a.T, a.dv_t, a.H, a.dv_h, bs, a.dv_b, 32);

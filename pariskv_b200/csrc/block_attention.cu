@@ -14,7 +14,7 @@ extern "C" int pk_block_attention(const pk_tensor* queries, const pk_tensor* key
   const int64_t bs = queries->shape[0];
   PK_REQUIRE(block == 16 || block == 32 || block == 64 || block == 128, "block must be 16, 32, 64 or 128");
   PK_REQUIRE(blocks->shape[0] == bs && blocks->shape[1] == p.T && blocks->shape[2] == p.H && is_contig(blocks), "blocks must be contiguous i32 [bs,T,H,n]");
-  PK_REQUIRE(blocks->shape[3] * block <= (1 << 24), "too many blocks");
+  PK_REQUIRE(blocks->shape[3] >= 1 && blocks->shape[3] * block <= (1 << 24), "between one block and 2^24 keys a list");
   p.blocks = (const int32_t*)blocks->data, p.n = (int)blocks->shape[3], p.block = (int)block;
   if (bs == 0 || p.T == 0) return PK_OK;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < attend_few_workspace())

@@ -464,7 +464,7 @@ extern "C" int pk_select_blocks(const pk_tensor* queries, const pk_tensor* bound
   PK_REQUIRE(nb * block < (1LL << 31) && n < (1LL << 24), "sizes out of range");
   if (bs * T * H == 0) return PK_OK;
   PK_REQUIRE(nb > 0, "bounds of no block");
-  if (!workspace || workspace_bytes < pk_select_blocks_workspace_bytes(bs, T, H, nb)) return fail(PK_ERR_WORKSPACE, "select_blocks: workspace missing or too small");
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < pk_select_blocks_workspace_bytes(bs, T, H, nb)) return fail(PK_ERR_WORKSPACE, "select_blocks: workspace missing, misaligned or too small");
   SelectParams p = {};
   p.q = (const uint16_t*)queries->data, p.q_b = queries->stride[0], p.q_t = queries->stride[1], p.q_h = queries->stride[2];
   p.bounds = (const uint16_t*)bounds->data, p.o_b = bounds->stride[0], p.o_h = bounds->stride[1], p.o_j = bounds->stride[2], p.nb = nb;

@@ -511,7 +511,8 @@ def tree_attention(queries, keys, values, draft_keys, draft_values, tree_mask, l
     queries bf16 [bs,T,Hq,128]; keys / values bf16 [bs,H,cap,128], of which sample b holds lengths[b] rows (i32 [bs], read on the
     device); draft_keys / draft_values bf16 [bs,T,H,128]; tree_mask bool or uint8 [1 or bs,T,T]: token t sees draft j (itself
     included only if the mask says so).  Returns bf16 [bs,T,Hq,128]; lse, if given (f32 [bs,T,Hq]), receives log2 of the softmax
-    denominators.  The verification of a tree needs one call per layer; see pk_tree_attention."""
+    denominators.  scale: positive, 1 / sqrt(128) by default.  The verification of a tree needs one call per layer; see
+    pk_tree_attention."""
     return L.native().tree_attention(queries, keys, values, draft_keys, draft_values, tree_mask, lengths,
                                      queries.shape[-1] ** -0.5 if scale is None else float(scale), out, lse)
 

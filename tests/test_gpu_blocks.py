@@ -155,6 +155,19 @@ def test_strided_cache_and_queries():
     R.close(out, want, tol)
 
 
+def test_one_head_of_keys_for_all():
+    """Strides of zero: keys, values and bounds expanded over the KV heads."""
+    from pariskv_b200 import ops
+    r = rnd(8)
+    keys, values, q = r(2, 1, 700, 128).expand(2, 3, 700, 128), r(2, 1, 700, 128).expand(2, 3, 700, 128), r(2, 2, 6, 128)
+    bnd = ops.block_bounds(keys[:, :1], i32([700, 65]), block=32).expand(2, 3, 22, 2, 128)
+    ids = ops.select_blocks(q, bnd, i32([700, 65]), 5, block=32)
+    assert torch.equal(ids.cpu(), R.select(q.cpu(), bnd.cpu(), [700, 65], 5, 32, 1, 1))
+    out = ops.block_attention(q, keys, values, ids, i32([700, 65]), block=32)
+    want, tol, _, _ = R.block_attention(q, keys, values, ids, [700, 65], 32)
+    R.close(out, want, tol)
+
+
 def test_head_groups_of_every_size():
     from pariskv_b200 import ops
     for G in (1, 2, 7, 9, 16, 17, 32, 128):

@@ -111,10 +111,11 @@ def test_no_tokens_and_refusals():
             call()
 
 
-def test_a_layer_of_a_step_with_drafts_captured():
+@pytest.mark.parametrize("launches", ["dependent", "early loads", "plain"])
+def test_a_layer_of_a_step_with_drafts_captured(launches):
     """4-bit projection, tree over the cache, then the accepted rows appended, bounds, selection, attention, 4-bit projection back:
     captured once and replayed, against the same definitions step by step."""
-    from pariskv_b200 import ops
+    from pariskv_b200 import _lib, ops
     g = torch.Generator(device=DEV).manual_seed(9)
     r = lambda *s: torch.randn(*s, generator=g, device=DEV).to(torch.bfloat16)
     bs, T, H, G, cap, hidden, block = 2, 4, 2, 4, 500, 512, 16
@@ -143,8 +144,15 @@ def test_a_layer_of_a_step_with_drafts_captured():
     step()
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        rows, tree, ids, sparse, y = step()
+    try:
+        if launches == "early loads":
+            _lib.set_pdl(True)
+        elif launches == "plain":
+            _lib.set_dependent_launch(False)
+        with torch.cuda.graph(graph):
+            rows, tree, ids, sparse, y = step()
+    finally:
+        _lib.set_pdl(False)
     for lens in ([400, 37], [404, 0], [496, 41]):
         x.copy_(r(bs * T, hidden))
         lengths.copy_(i32(lens))

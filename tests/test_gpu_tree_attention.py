@@ -140,6 +140,16 @@ def test_strides(layout):
     check(d)
 
 
+@pytest.mark.parametrize("T", [3, 20])
+def test_one_head_of_keys_for_all(T):
+    """Strides of zero, which no tensor map takes: a cache, and drafts, expanded over the KV heads."""
+    d = make(15, 2, T, 1, 8, 150, [150, 33])
+    for names, heads_at in ((("keys", "values"), 1), (("draft_keys", "draft_values"), 2)):
+        for name in names:
+            d[name] = d[name].expand(*[4 if i == heads_at else n for i, n in enumerate(d[name].shape)])
+    check(d)
+
+
 def test_one_mask_for_the_batch():
     d = make(10, 3, 11, 1, 4, 150, [150, 20, 0], shared_mask=True)
     check(d)
@@ -218,7 +228,7 @@ def test_refusals():
     for change in (dict(keys=d["keys"].float()), dict(keys=odd), dict(values=shifted), dict(lengths=d["lengths"][:1]),
                    dict(lengths=d["lengths"].long()), dict(tree_mask=d["tree_mask"][:, :3]), dict(tree_mask=d["tree_mask"].float()),
                    dict(queries=d["queries"][:, :, :3]), dict(draft_keys=d["draft_keys"][:, :3]), dict(values=d["values"][:, :, :60]),
-                   dict(queries=d["queries"][..., :64]), dict(keys=d["keys"].cpu()), dict(out=torch.empty(2, 4, 4, 64, dtype=torch.bfloat16, device=DEV)),
+                   dict(queries=d["queries"][..., :64]), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(keys=d["keys"].cpu()), dict(out=torch.empty(2, 4, 4, 64, dtype=torch.bfloat16, device=DEV)),
                    dict(lse=torch.empty(2, 4, 2, device=DEV))):
         with pytest.raises((RuntimeError, TypeError, ValueError)):
             ops.tree_attention(**{**d, **change})
