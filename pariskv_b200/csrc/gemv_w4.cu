@@ -29,7 +29,7 @@ constexpr int W4_PIECE = 2048;                  // 256 columns of 16 rows
 constexpr int W4_STAGES_MAX = 6;
 __host__ __device__ constexpr int w4_sums(int nt) { return nt == 1 ? 4 : 2; }
 constexpr uint32_t W4_BIAS = 0x4b400000u;       // the float 2^23 + 2^22: adding a whole number below 2^22 to its bits adds it to the float
-constexpr int W4_LONG = 8;                       // stages of 64 KB per SM from which on boxes are of 512 columns
+constexpr int W4_LONG = 4, W4_LONG_BF16 = 8;     // stages of 64 KB per SM from which on boxes are of 512 columns
 constexpr int W4_WAIT_LIMIT = 100000;
 constexpr int W4_SMEM = 227 * 1024 - 512;   // of a block; 512 bytes of barriers
 
@@ -455,10 +455,13 @@ W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated, b
   return r;
 }
 // Boxes of 512 columns, which spread what a box costs besides its products, where an SM has many stages of them all the same; for one or two tokens in
-// whole numbers, whose digits have to pay.
+// whole numbers, whose digits have to pay.  Boxes of 256 and bf16 | of 512 and in whole numbers: one token, 24576 x 4096 (5 stages per SM) 22.9 | 20.9,
+// 151936 x 4096 (32) 105 | 70, 6144 x 4096 (1) 7.9 | 8.3;  of 256 | of 512, both bf16: six tokens, 24576 x 4096 (5) 25.5 | 27.3.
 W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated, bool offsets) {
-  const W4Plan two = w4_plan(n_out, I, T, group_log, gated, offsets, T <= 2, 2);
-  return (int64_t)two.sets * ((two.boxes + (1 << two.kw_log) - 1) >> two.kw_log) >= W4_LONG * (int64_t)sm_count() ? two : w4_plan(n_out, I, T, group_log, gated, offsets, false, 1);
+  const bool whole = T <= 2;
+  const W4Plan two = w4_plan(n_out, I, T, group_log, gated, offsets, whole, 2);
+  const int64_t stages = (int64_t)two.sets * ((two.boxes + (1 << two.kw_log) - 1) >> two.kw_log);
+  return stages >= (whole ? W4_LONG : W4_LONG_BF16) * (int64_t)sm_count() ? two : w4_plan(n_out, I, T, group_log, gated, offsets, false, 1);
 }
 
 }  // namespace
