@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(PICK_THREADS) block_pick_kernel(SelectParams p
       if (before < want && before + c >= want) s_found[0] = PICK_BINS - 1 - tid, s_found[1] = before, s_found[2] = c;
       __syncthreads();
       lo += s_found[0] << shift;
-      hi = min(hi, lo + ((1u << shift) - 1));
+      hi = lo + min(hi - lo, (1u << shift) - 1);   // (NaN's bin ends behind the last 32-bit number)
       want -= s_found[1], in_range = s_found[2];
     }
     return lo == hi && want != in_range;   // taken in part

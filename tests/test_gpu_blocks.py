@@ -107,6 +107,21 @@ def test_scores_that_are_not_numbers():
     assert pick(70) == list(range(64)) + [-1] * 6
 
 
+@pytest.mark.parametrize("first", [-50.0, 0.001, 10.0, 300.0])
+@pytest.mark.parametrize("nb,T", [(60, 1), (3000, 2), (17000, 1)])
+def test_more_scores_that_are_not_numbers_than_are_taken(first, nb, T):
+    """Twenty NaN among scores of every size: the lowest of them are taken."""
+    from pariskv_b200 import ops
+    bnd = torch.zeros(1, 1, nb, 2, 128, dtype=torch.bfloat16, device=DEV)
+    bnd[0, 0, :, :, 0] = (first + torch.arange(nb, device=DEV) % 40)[:, None].to(torch.bfloat16)
+    bnd[:, :, 30:50] = float("nan")
+    q = torch.zeros(1, T, 1, 128, dtype=torch.bfloat16, device=DEV)
+    q[..., 0] = 1
+    got = ops.select_blocks(q, bnd, i32([nb * 16]), 9, block=16, sink_blocks=1, local_blocks=1)
+    assert got[0, -1, 0].tolist() == [0, *range(30, 37), nb - 1]
+    assert got[0, 0, 0].tolist() == [0, *range(30, 37), nb - 1]
+
+
 @pytest.mark.parametrize("bs,T,H,G,cap,lengths,n,block,sink,local", SELECT)
 def test_attention_over_selected_blocks(bs, T, H, G, cap, lengths, n, block, sink, local):
     from pariskv_b200 import ops
