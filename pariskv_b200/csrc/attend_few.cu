@@ -149,13 +149,11 @@ __global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
   pdl_wait();
   pdl_trigger();
   const int blocks = (int)gridDim.x;
-  if (TREE) {
-    if (warp == 0) {
-      const TilePlan w = tile_plan(p.bs, blockIdx.x, (unsigned)blocks, [&](int b) -> int64_t { return b < p.bs ? (int64_t)p.a.H * few_tiles(p, b) : 0; });
-      if (lane == 0) s_place = w;
-    }
-    __syncthreads();
+  if (TREE && warp == 0) {
+    const TilePlan w = tile_plan(p.bs, blockIdx.x, (unsigned)blocks, [&](int b) -> int64_t { return b < p.bs ? (int64_t)p.a.H * few_tiles(p, b) : 0; });
+    if (lane == 0) s_place = w;
   }
+  __syncthreads();   // the barriers are there, and the place
   const TilePlan place = TREE ? s_place : TilePlan{(int64_t)p.bs * p.a.T * p.a.H * p.row_groups * p.tiles, 0, 0};
   const unsigned shares = (unsigned)min((int64_t)blocks, place.total);
   if (blockIdx.x >= shares) return;
