@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
             float L = 0.0f, O = 0.0f;
 #pragma unroll
             for (int w = 0; w < 4; w++) {
-              L += s_m[w][row] == -INFINITY ? 0.0f : s_l[w][row] * ex2(s_m[w][row] - Mi);
+              L += s_l[w][row] * (s_m[w][row] == -INFINITY ? 0.0f : ex2(s_m[w][row] - Mi));   // (a NaN stays: all scores that a warp saw were NaN)
               O += s_o[(w * 8 + i) * FEW_OS + tid];
             }
             if (s_dead) L = NAN;

@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(128) attend_kernel(AttendParams p, int64_t row
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
     s *= p.scale_log2;
-    const float M = fmaxf(m, s), f = m == -INFINITY ? 0.0f : exp2f(m - M), w = M == -INFINITY ? 0.0f : exp2f(s - M);
+    const float M = fmaxf(m, s), f = m == -INFINITY ? 0.0f : exp2f(m - M), w = exp2f(s - (M == -INFINITY ? 0.0f : M));   // (NaN stays)
     l = l * f + w, m = M;
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] = o[i] * f + w * vf[i];

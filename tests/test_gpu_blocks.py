@@ -156,6 +156,21 @@ def test_lists_in_any_order_with_gaps_and_repeats(block):
     assert (out[0, 0, :G] == 0).all()
 
 
+@pytest.mark.parametrize("G,n", [(1, 1), (4, 9), (16, 40), (20, 300)])
+def test_a_query_that_is_not_a_number(G, n):
+    from pariskv_b200 import ops
+    r = rnd(G)
+    keys, values, q = r(1, 2, 6000, 128), r(1, 2, 6000, 128), r(1, 2, 2 * G, 128)
+    q[0, 1, G] = float("nan")
+    ids = torch.arange(n, dtype=torch.int32, device=DEV).expand(1, 2, 2, n).contiguous()
+    lse = torch.zeros(1, 2, 2 * G, device=DEV)
+    out = ops.block_attention(q, keys, values, ids, i32([6000]), block=16, lse=lse)
+    assert out[0, 1, G].isnan().all() and lse[0, 1, G].isnan()
+    want, tol, _, _ = R.block_attention(q, keys, values, ids, [6000], 16)
+    R.close(out, want, tol)
+    assert int(out.isnan().sum()) == 128
+
+
 def test_strided_cache_and_queries():
     from pariskv_b200 import ops
     r = rnd(4)

@@ -94,6 +94,25 @@ def test_what_is_masked_does_not_reach_a_token(T, G):
         R.close(out[:, t][..., rest], want[:, t][..., rest], tol[:, t][..., rest])
 
 
+@pytest.mark.parametrize("T,G,n", [(1, 1, 1), (2, 4, 0), (2, 4, 3000), (3, 8, 40), (40, 4, 300), (70, 4, 3000)])
+@pytest.mark.parametrize("shared_head", [False, True])
+def test_a_query_that_is_not_a_number(T, G, n, shared_head):
+    """It comes out as NaN, lse too, where it sees a row; the other queries do not notice."""
+    d = make(9, 2, T, 2, G, 3000, [n, 3000], empty=0.0)
+    if shared_head:
+        for k in ("keys", "values"):
+            d[k] = d[k][:, :1].expand(2, 2, 3000, 128)
+    d["tree_mask"][:] = torch.eye(T, dtype=torch.bool, device=DEV)
+    d["queries"][:, T - 1, G] = float("nan")
+    from pariskv_b200 import ops
+    lse = torch.zeros(2, T, 2 * G, device=DEV)
+    out = ops.tree_attention(**d, lse=lse)
+    assert out[:, T - 1, G].isnan().all() and lse[:, T - 1, G].isnan().all()
+    want, tol, _, _ = R.tree(*[d[k] for k in ("queries", "keys", "values", "draft_keys", "draft_values", "tree_mask")], [n, 3000])
+    R.close(out, want, tol)
+    assert int(out.isnan().sum()) == 2 * 128
+
+
 def test_a_row_of_lowest_scores_is_a_row():
     """Every score at the type's lowest values: the weights are equal, not lost."""
     d = make(8, 1, 2, 1, 1, 64, [64], empty=0.0)
