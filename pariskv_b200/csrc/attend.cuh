@@ -42,7 +42,7 @@ inline int fill_attend(AttendParams* p, const pk_tensor* queries, const pk_tenso
   PK_CHECK_TENSOR(out, PK_BF16, 4);
   const int64_t bs = queries->shape[0], T = queries->shape[1], Hq = queries->shape[2], H = keys->shape[1];
   PK_REQUIRE(queries->shape[3] == 128, "queries must be bf16 [bs,T,Hq,128]");
-  PK_REQUIRE(keys->shape[0] == bs && keys->shape[3] == 128 && keys->shape[2] < (1LL << 31), "keys must be bf16 [bs,H,cap,128]");
+  PK_REQUIRE(keys->shape[0] == bs && keys->shape[3] == 128 && keys->shape[2] <= (1LL << 31) - 128, "keys must be bf16 [bs,H,cap,128]");
   for (int i = 0; i < 4; i++) PK_REQUIRE(values->shape[i] == keys->shape[i], "values must have the shape of keys");
   PK_REQUIRE(H >= 1 && Hq % H == 0 && Hq >= H && Hq / H <= 128, "the query heads must be a multiple of the KV heads, at most 128 of them each");
   PK_REQUIRE(row_tensor(queries) && row_tensor(keys) && row_tensor(values),

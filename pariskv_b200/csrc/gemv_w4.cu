@@ -79,8 +79,8 @@ struct W4Column {
 // WHOLE: the form; NT: its columns in eights; SUB: pieces of 256 columns in a box
 template <bool WHOLE, int NT, int SUB>
 __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ W4Params p) {
-  constexpr int W4_BOX = SUB * W4_PIECE, W4_STAGE = W4_WARPS * W4_BOX, SUMS = w4_sums(NT), E = 2 * SUB, PER = WHOLE ? 3 : 1;   // PER: columns of a token
-  constexpr int BYTES = WHOLE ? 1 : 2;   // of a value of x in shared memory   // E: scales of a row that a lane holds
+  constexpr int W4_BOX = SUB * W4_PIECE, W4_STAGE = W4_WARPS * W4_BOX, SUMS = w4_sums(NT), E = 2 * SUB, PER = WHOLE ? 3 : 1;   // E: scales of a row that a lane holds; PER: columns of a token
+  constexpr int BYTES = WHOLE ? 1 : 2;   // of a value of x in shared memory
   extern __shared__ unsigned char dyn[];
   __shared__ __align__(8) unsigned long long bars[2 * W4_STAGES_MAX + 2 * SUMS];
   __shared__ volatile int s_dead;
@@ -429,7 +429,6 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
 }
 
 // How x and the rows are laid out for a product.
-// How x and the rows are laid out for a product.
 struct W4Plan {
   bool whole;
   int tiles, sub, stages, units, boxes, kw_log, slices, pitch, groups_smem, smem, sets;
@@ -470,7 +469,7 @@ W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated, b
 using namespace pk;
 
 extern "C" int64_t pk_gemv_w4_workspace_bytes(int64_t T, int64_t O, int64_t I, int64_t group, int gated) {
-  if (T < 1 || O < 1 || I < 32 || (group != 32 && group != 64 && group != 128)) return 0;
+  if (T < 1 || T > 16 || O < 1 || O >= (1LL << 30) || I < 32 || I > 32768 || (group != 32 && group != 64 && group != 128)) return 0;
   // (the larger of what is needed with offsets and without)
   int64_t most = 0;
   for (const bool offsets : {false, true}) {

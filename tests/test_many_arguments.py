@@ -106,3 +106,13 @@ def test_workspace_sizes():
     for rc in (lib.pk_tree_attention_workspace_bytes(8, 61, 32, 8, 131072), lib.pk_block_attention_workspace_bytes(8, 4, 32, 8, 32, 64),
                lib.pk_select_blocks_workspace_bytes(8, 4, 8, 2048)):
         assert 0 < rc < 1 << 32
+
+
+def test_sizes_that_no_call_takes():
+    """Workspace sizes of what would be refused are zero, and a cache ends where 128 rows more still have 31-bit numbers."""
+    lib = L.load()
+    for T, O, I in ((1, 64, 1 << 41), (1, 64, 32768 + 128), (17, 64, 128), (1, 1 << 40, 128), (0, 64, 128)):
+        assert lib.pk_gemv_w4_workspace_bytes(T, O, I, 128, 0) == 0
+    long = z(1, 1, 1, 128).expand(2, 2, 2 ** 31 - 100, 128)
+    refused("pk_tree_attention", list({**TREE, "k": long, "v": long}.values()), "keys must be")
+    refused("pk_block_attention", list({**ATTEND, "k": long, "v": long}.values()), "keys must be")
