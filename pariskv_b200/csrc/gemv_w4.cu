@@ -8,7 +8,7 @@
 //   bf16, a column a token.  A code becomes one by its bits alone, 0x4300 | c = 128 + c, seven instructions a word; what the 128 and the 8 add is
 //     128 or 136 times the group's sum of x, so the fp32 sum starts from that, negative (the two cancel to about a sixteenth: four of 24 bits).
 // The integer unit, not the tensor cores, is what both spend most on.  B200, us, whole numbers | bf16: one token, 151936 x 4096 70 | 88, 6144 x 4096
-// 8.3 | 7.9; six tokens, gate and up of 12288 x 4096 in groups of 64 46 | 28.
+// 8.3 | 7.9; six tokens, gate and up of 12288 x 4096 in groups of 64 46 | 27.
 //
 // Bounded by the bytes of W.  Sixteen rows are a unit; a box is 256 (or 512) of its columns, 2 KB pieces that TMA brings with the 128-byte swizzle, a warp's
 // share of a stage of sixteen boxes.  A lane reads a word of 8 codes of rows g and g + 8 and 8 digits per 32 columns and product; the digits
@@ -265,9 +265,15 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
     // x of the slice: a warp takes 256 columns of a token, a lane eight; zeros behind the last column.
     const int first_col = slice * p.boxes * (256 * SUB), parts = p.boxes * SUB;
     if (slice > 0) asm volatile("bar.sync 1, 512;" ::: "memory");   // the last products with the digits before
-    for (int i = warp; i < p.T * parts; i += W4_WARPS) {
-      const int t = i / parts, part = i - t * parts, col = first_col + 256 * part + 8 * lane;
-      const uint4 v = col < p.I ? *reinterpret_cast<const uint4*>(p.x + (int64_t)t * p.x_t + col) : make_uint4(0, 0, 0, 0);
+    auto load_x = [&](int t, int part) -> uint4 {
+      const int col = first_col + 256 * part + 8 * lane;
+      return t < p.T && col < p.I ? *reinterpret_cast<const uint4*>(p.x + (int64_t)t * p.x_t + col) : make_uint4(0, 0, 0, 0);
+    };
+    int t = warp / parts, part = warp - t * parts, t_next, part_next;
+    uint4 v = load_x(t, part), v_next;   // one turn ahead
+    for (; t < p.T; t = t_next, part = part_next, v = v_next) {
+      for (t_next = t, part_next = part + W4_WARPS; part_next >= parts; t_next++) part_next -= parts;
+      v_next = load_x(t_next, part_next);
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
       if constexpr (WHOLE) {
         float x[8];
