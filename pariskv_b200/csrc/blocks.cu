@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "attend.cuh"
+#include "tma.cuh"
 
 namespace pk {
 namespace {
@@ -103,31 +104,61 @@ __device__ __forceinline__ void query_sums(const SelectParams& p, int64_t b, int
 // Scores in 32 bits, and a bound A of every sum of absolute values: A = sum_d P_d max |hi_d| + |N_d| max |lo_d| over the warp's blocks.  A score is off
 // by at most G + 13 roundings of 2^-24 A (P or N, eight products in a row, five additions of the lanes' sums): where the choice hangs on less
 // than that, block_pick_kernel takes the 64-bit scores.
-// A warp takes eight blocks of keys at a time, 4 KB that are in flight at once, for TT tokens: lanes 0 .. 15 hold eight channels of lo and N each, the
-// others of hi and P.  Bounded by the bounds' bytes where there are many, otherwise by latency.  (64-bit sums throughout: 8192 blocks of 8
-// heads for four tokens 46 us, of 128 heads x 770 blocks for one 26 us; the conversions to 64 bits alone, 8 a clock and SM, take longer than the bytes.)
-__host__ __device__ constexpr int score_ctas(int tt) { return tt <= 2 ? 3 : 2; }   // blocks per SM, by the registers
+// A warp of its own brings 32 blocks of keys at a time, 16 KB, into a ring of four stages; each of four warps takes eight of them for TT tokens: lanes
+// 0 .. 15 hold eight channels of lo and N each, the others of hi and P.  Bounded by the bounds' bytes where there are many, otherwise by
+// latency.  With the choice, us, by loads to registers two groups ahead | by the ring: 8192 blocks of 8 heads for four tokens 29 | 28, for one 21 | 18,
+// 512 blocks 8.3 | 7.7.  Copies of one block each, which bounds with gaps need, cost more the more of them there are: 128 heads x 400 blocks
+// 14.5, in copies of 512 bytes 16.5.  (64-bit sums throughout: four tokens 46 us for the scores alone; the conversions to 64 bits, 8 a
+// clock and SM, take longer than the bytes.)
+constexpr int SCORE_BLOCKS = 32, SCORE_STAGE = 512 * SCORE_BLOCKS, SCORE_STAGES = 4, SCORE_THREADS = 160, SCORE_CTAS = 3;   // blocks per SM, by the registers
+constexpr int SCORE_WAIT_LIMIT = 100000;   // tries; one waits up to 10 us by itself
 template <int TT>
-__global__ void __launch_bounds__(128, score_ctas(TT)) block_score_kernel(SelectParams p) {
+__global__ void __launch_bounds__(SCORE_THREADS, SCORE_CTAS) block_score_kernel(SelectParams p) {
+  extern __shared__ __align__(128) unsigned char ring[];
+  __shared__ __align__(8) unsigned long long bars[2 * SCORE_STAGES];
+  __shared__ volatile int s_dead;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.y % p.H, t0 = blockIdx.y / p.H * TT;
+  const unsigned full = smem_addr(bars), empty = full + 8 * SCORE_STAGES;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SCORE_STAGES; i++) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 4);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_dead = 0;
+  }
+  __syncthreads();
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31, h = blockIdx.y % p.H, t0 = blockIdx.y / p.H * TT;
   const int64_t b = blockIdx.z;
   int seen[TT], most = 0;
 #pragma unroll
   for (int i = 0; i < TT; i++) seen[i] = t0 + i < p.T ? visible_blocks(p, b, t0 + i) : 0, most = max(most, seen[i]);
-  const uint16_t* bounds = p.bounds + b * p.o_b + h * p.o_h + 8 * lane;
-  const int groups = (most + 7) / 8, warps = (int)gridDim.x * 4, self = (int)blockIdx.x * 4 + (threadIdx.x >> 5);
-  struct Group {
-    uint4 x[8];
-  } now, next;
-  auto load = [&](Group& to, int at) {
-    const uint16_t* from = bounds + (int64_t)(8 * at) * p.o_j;
-#pragma unroll
-    for (int i = 0; i < 8; i++) to.x[i] = 8 * at + i < most ? *reinterpret_cast<const uint4*>(from + i * p.o_j) : make_uint4(0, 0, 0, 0);
+  const int steps = (most + SCORE_BLOCKS - 1) / SCORE_BLOCKS;
+  bool dead = false;   // a wait has run out: no more waiting; the limits become NaN, and the choice is made of 64-bit sums
+  auto wait = [&](unsigned mb, unsigned parity) {
+    for (int it = 0; !dead; it++) {
+      if (mbar_try(mb, parity)) break;
+      if (it >= SCORE_WAIT_LIMIT || s_dead) dead = true, s_dead = 1;
+    }
+    __syncwarp();
   };
-  load(now, self);
-  load(next, self + warps);
+  if (warp == 4) {
+    const uint16_t* bounds = p.bounds + b * p.o_b + h * p.o_h;
+    int q = 0;
+    for (int step = blockIdx.x; step < steps; step += gridDim.x, q++) {
+      const int st = q % SCORE_STAGES, n = min(SCORE_BLOCKS, most - SCORE_BLOCKS * step);
+      if (q >= SCORE_STAGES) wait(empty + 8 * st, (unsigned)(q / SCORE_STAGES - 1) & 1);
+      if (__any_sync(0xffffffffu, dead)) break;
+      if (lane == 0) mbar_expect(full + 8 * st, 512 * n);
+      __syncwarp();
+      const int per = p.o_j == 256 ? 8 : 1, first = per * lane;   // blocks of a copy
+      if (first < n)
+        bulk_load(smem_addr(ring) + st * SCORE_STAGE + 512 * first, bounds + (int64_t)(SCORE_BLOCKS * step + first) * p.o_j, 512 * min(per, n - first), full + 8 * st);
+    }
+    if (s_dead)   // what is under way has to land before the block ends
+      for (int i = q < SCORE_STAGES ? 0 : q - SCORE_STAGES; i < q; i++)
+        for (int it = 0; it < SCORE_WAIT_LIMIT && !mbar_try(full + 8 * (i % SCORE_STAGES), (unsigned)(i / SCORE_STAGES & 1)); it++) {}
+    return;
+  }
+  const int warps = (int)gridDim.x * 4, self = (int)blockIdx.x * 4 + warp;
   // P and N of the block's tokens, a thread per channel
   __shared__ __align__(16) float s_sums[TT][2][128];
   {
@@ -153,7 +184,7 @@ __global__ void __launch_bounds__(128, score_ctas(TT)) block_score_kernel(Select
 #pragma unroll
     for (int i = 0; i < TT; i++) s_sums[i][0][d] = down[i], s_sums[i][1][d] = up[i];
   }
-  __syncthreads();
+  asm volatile("bar.sync 1, 128;" ::: "memory");
   float c[TT][8];   // P or N of this lane's channels
 #pragma unroll
   for (int i = 0; i < TT; i++)
@@ -162,11 +193,16 @@ __global__ void __launch_bounds__(128, score_ctas(TT)) block_score_kernel(Select
   __nv_bfloat162 top[4];   // largest magnitudes of this lane's channels
 #pragma unroll
   for (int e = 0; e < 4; e++) top[e] = __nv_bfloat162(__ushort_as_bfloat16(0), __ushort_as_bfloat16(0));
-  auto take = [&](Group& of, int group) {   // and asks for the one after the next in its place
+  int q = 0;
+  for (int step = blockIdx.x; step < steps; step += gridDim.x, q++) {
+    const int st = q % SCORE_STAGES, first = SCORE_BLOCKS * step + 8 * warp;
+    wait(full + 8 * st, (unsigned)(q / SCORE_STAGES) & 1);
+    const uint4* from = reinterpret_cast<const uint4*>(ring + st * SCORE_STAGE + 4096 * warp) + lane;
     float sum[TT][8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const uint32_t w[4] = {of.x[i].x, of.x[i].y, of.x[i].z, of.x[i].w};
+      const uint4 x = first + i < most ? from[32 * i] : make_uint4(0, 0, 0, 0);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
       float v[8];
 #pragma unroll
       for (int e = 0; e < 4; e++) {
@@ -181,18 +217,15 @@ __global__ void __launch_bounds__(128, score_ctas(TT)) block_score_kernel(Select
         sum[k][i] = s;
       }
     }
-    load(of, group + 2 * warps);
+    __syncwarp();
+    if (lane == 0) mbar_arrive1(empty + 8 * st);
 #pragma unroll
     for (int k = 0; k < TT; k++) {
       const float f = warp_sums8(sum[k], lane) + 0.0f;   // (one zero)
-      const int j = 8 * group + (lane >> 2);
+      const int j = first + (lane >> 2);
       if ((lane & 3) == 0 && j < seen[k])
         p.keys[((b * p.T + t0 + k) * p.H + h) * p.nb + j] = j < p.sink || j >= seen[k] - p.local ? FORCED : f != f ? NOT_A_NUMBER : ord_key(f);
     }
-  };
-  for (int group = self; group < groups; group += 2 * warps) {
-    take(now, group);
-    if (group + warps < groups) take(next, group + warps);
   }
 #pragma unroll
   for (int k = 0; k < TT; k++) {
@@ -201,7 +234,7 @@ __global__ void __launch_bounds__(128, score_ctas(TT)) block_score_kernel(Select
     for (int e = 0; e < 8; e++) A += fabsf(c[k][e]) * (e & 1 ? __high2float(top[e >> 1]) : __low2float(top[e >> 1]));   // (infinite bounds: inf or NaN)
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) A += __shfl_xor_sync(0xffffffffu, A, off);
-    if (lane == 0 && t0 + k < p.T) p.limits[((b * p.T + t0 + k) * p.H + h) * warps + self] = A;
+    if (lane == 0 && t0 + k < p.T) p.limits[((b * p.T + t0 + k) * p.H + h) * warps + self] = dead ? NAN : A;
   }
 }
 
@@ -475,13 +508,22 @@ extern "C" int pk_select_blocks(const pk_tensor* queries, const pk_tensor* bound
   StageTimer timer(ST_RANK, (cudaStream_t)stream);
   // tokens share what is read, four at a time; one wave where that is possible, a warp eight blocks of keys a step
   const int tt = T >= 3 ? 4 : (int)T;
-  const int64_t per_head = (nb + 31) / 32, heads = H * ((T + tt - 1) / tt), slots = (int64_t)score_ctas(tt) * sm_count() / (heads * bs), room = slots < 1 ? 1 : slots;
+  const int64_t per_head = (nb + 31) / 32, heads = H * ((T + tt - 1) / tt), slots = (int64_t)SCORE_CTAS * sm_count() / (heads * bs), room = slots < 1 ? 1 : slots;
   PK_REQUIRE(heads < 65536, "at most 65535 KV heads x token groups");
   const dim3 grid((unsigned)(per_head < room ? per_head : room), (unsigned)heads, (unsigned)bs);
   p.limits = (float*)(p.keys + rows * nb);
-  if (tt == 1) launch_chain(block_score_kernel<1>, grid, dim3(128), 0, (cudaStream_t)stream, p);
-  else if (tt == 2) launch_chain(block_score_kernel<2>, grid, dim3(128), 0, (cudaStream_t)stream, p);
-  else launch_chain(block_score_kernel<4>, grid, dim3(128), 0, (cudaStream_t)stream, p);
+  auto score = [&](auto tokens) -> int {
+    constexpr auto kernel = block_score_kernel<decltype(tokens)::value>;
+    static PerDevice opted;
+    if (const unsigned long long bit = first_on_device(opted)) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SCORE_STAGES * SCORE_STAGE) != cudaSuccess)
+        return fail(PK_ERR_CUDA, "select_blocks: %s", cudaGetErrorString(cudaGetLastError()));
+      mark_on_device(opted, bit);
+    }
+    launch_chain(kernel, grid, dim3(SCORE_THREADS), SCORE_STAGES * SCORE_STAGE, (cudaStream_t)stream, p);
+    return PK_OK;
+  };
+  if (const int rc = tt == 1 ? score(std::integral_constant<int, 1>()) : tt == 2 ? score(std::integral_constant<int, 2>()) : score(std::integral_constant<int, 4>())) return rc;
   auto pick = [&](auto kpt) {
     launch_chain(block_pick_kernel<decltype(kpt)::value>, dim3((unsigned)rows), dim3(PICK_THREADS), 0, (cudaStream_t)stream, p, (int)grid.x * 4);
   };

@@ -36,6 +36,10 @@ __device__ __forceinline__ void tma_load4(unsigned dst, const CUtensorMap* map, 
                "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(mb)
                : "memory");
 }
+// bytes in a row: both addresses and the size multiples of 16
+__device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes, unsigned mb) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(mb) : "memory");
+}
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

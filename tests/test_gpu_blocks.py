@@ -60,6 +60,33 @@ def test_selection(bs, T, H, G, cap, lengths, n, block, sink, local):
     assert torch.equal(got.cpu(), want)
 
 
+@pytest.mark.parametrize("bs,T,H,nb,n", [(4, 1, 16, 3000, 20), (3, 4, 8, 2100, 17), (1, 2, 300, 70, 9), (2, 1, 1, 33, 4)])
+@pytest.mark.parametrize("gaps", [False, True])
+def test_selection_of_long_rows(bs, T, H, nb, n, gaps):
+    """Many steps for every block of the launch; bounds that lie next to each other and bounds with gaps, which hold NaN."""
+    from pariskv_b200 import ops
+    r = rnd(nb)
+    store = torch.full((bs, H, nb + 2, 3, 128), float("nan"), dtype=torch.bfloat16, device=DEV)
+    bnd = store[:, :, 1:nb + 1, :2]
+    bnd.copy_(r(bs, H, nb, 2, 128).sort(3).values)
+    if not gaps:
+        bnd = bnd.contiguous()
+    lengths = [nb * 32 - 700 * b for b in range(bs)]
+    lengths[-1] = nb * 32
+    q = r(bs, T, 2 * H, 128)
+    got = ops.select_blocks(q, bnd, i32(lengths), n, block=32, sink_blocks=1, local_blocks=2)
+    qs, lo, hi = q.double().view(bs, T, H, 2, 128), bnd[..., 0, :].double(), bnd[..., 1, :].double()
+    P, N = qs.clamp(min=0).sum(3), qs.clamp(max=0).sum(3)
+    score = (torch.einsum("bthd,bhjd->bthj", P, hi) + torch.einsum("bthd,bhjd->bthj", N, lo)).float()
+    for b in range(bs):
+        for t in range(T):
+            seen = (lengths[b] - T + t) // 32 + 1
+            s = score[b, t, :, :seen].clone()
+            s[:, 0] = s[:, seen - 2:] = float("inf")
+            want = s.sort(dim=1, descending=True, stable=True).indices[:, :n].sort(dim=1).values
+            assert torch.equal(got[b, t].long(), want), (b, t)
+
+
 def test_ties_go_to_the_lower_block():
     from pariskv_b200 import ops
     r = rnd(2)
