@@ -554,7 +554,9 @@ int pk_gemv(const pk_tensor* weight, const pk_tensor* x, const pk_tensor* out, i
  * pk_gemv_w4: out[T,O] = x[T,I] W^T for up to 16 tokens, fp32 sums.  weight u8 [O,I/2], the low nibble of a byte the even column;
  *   scales bf16 [O,I/group], group 32, 64 or 128; W = (code - 8) * scale, or code * scale + offset with offsets bf16 like scales.
  *   gated: weight is [gate; up] stacked, out[T,O/2] = silu(gate x) * (up x), rounded once.  I at most 32768.  A token with an infinity
- *   or NaN comes out as NaN, the others do not notice; so may one with magnitudes of 2^100 and more, whose sums pass 32 bits. */
+ *   or NaN comes out as NaN, the others do not notice; so may one with magnitudes of 2^100 and more, whose sums pass 32 bits.  One token by a
+ *   long matrix goes as fixed-point numbers: a value below 2^-48 of the largest of its group of columns, or below 2^-119, may lose bits, one
+ *   below 2^-55 of it, or below 2^-126, counts as zero. */
 int64_t pk_tree_attention_workspace_bytes(int64_t bs, int64_t T, int64_t Hq, int64_t H, int64_t cap);
 int pk_tree_attention(const pk_tensor* queries, const pk_tensor* keys, const pk_tensor* values, const pk_tensor* draft_keys,
                       const pk_tensor* draft_values, const pk_tensor* tree_mask, const pk_tensor* lengths, float scale,

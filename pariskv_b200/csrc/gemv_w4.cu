@@ -1,14 +1,13 @@
 // y = x W^T for a few tokens, W of 4-bit codes c with a scale s (and an offset m) per row and group of columns:
 //   W = (c - 8) s, or c s + m;   y = sum over groups q of  s_q (sum c x - 8 sum x), or s_q sum c x + m_q sum x
 // The products run on the tensor cores (mma.sync), 16 rows of W by 8 columns, in one of two forms:
-//   whole numbers, for one or two tokens.  x = e (d0 + d1 / 2^7 + d2 / 2^14) per token and group, e a power of two, the digits of 8 bits, off by at most 2^-21
-//     of the group's largest value (not at all for values within 2^-13 of it): three columns a token, exact sums.  A word of eight codes costs
-//     three instructions of the integer unit.  The sums start from 2^23 + 2^22 - 8 sum d in the bits of a float, so that their bits are that
-//     float's: e and s follow in fp32.
-//   bf16, a column a token.  A code becomes one by its bits alone, 0x4300 | c = 128 + c, seven instructions a word; what the 128 and the 8 add is
-//     128 or 136 times the group's sum of x, so the fp32 sum starts from that, negative (the two cancel to about a sixteenth: four of 24 bits).
-// The integer unit, not the tensor cores, is what both spend most on.  B200, us, whole numbers | bf16: one token, 151936 x 4096 70 | 88, 6144 x 4096
-// 8.3 | 7.9; six tokens, gate and up of 12288 x 4096 in groups of 64 46 | 27.
+//   whole numbers, for one token.  x = e (d0 + d1 / 2^7 + .. + d7 / 2^49) per group, e a power of two, the digits of 8 bits: the eight columns of a
+//     product, exact sums.  A value that is 2^-48 of its group's largest still has all of its bits, one below 2^-55 of it counts as zero; no smaller
+//     unit than 2^-126 is used.  A word of eight codes costs three instructions of the integer unit.  The sums start from 2^23 + 2^22 - 8 sum d
+//     in the bits of a float, so that their bits are that float's: e and s follow in fp32.
+//   bf16, a column a token.  A code becomes one by its bits, 0x4300 | c = 128 + c, less 136 (128 with offsets), which is exact: seven instructions of
+//     the integer unit and four subtractions a word, and a weight of zero adds nothing whatever it meets.
+// The integer unit, not the tensor cores, is what both spend most on; what each takes stands at w4_plan().
 //
 // Bounded by the bytes of W.  Sixteen rows are a unit; a box is 256 (or 512) of its columns, 2 KB pieces that TMA brings with the 128-byte swizzle, a warp's
 // share of a stage of sixteen boxes.  A lane reads a word of 8 codes of rows g and g + 8 and 8 digits per 32 columns and product; the digits
@@ -28,8 +27,9 @@ constexpr int W4_PIECE = 2048;                  // 256 columns of 16 rows
 // Stages at most; units whose warps' sums are kept, with NT times eight columns.
 constexpr int W4_STAGES_MAX = 6;
 __host__ __device__ constexpr int w4_sums(int nt) { return nt == 1 ? 4 : 2; }
+constexpr int W4_DIGITS = 8;                    // of a value in whole numbers
 constexpr uint32_t W4_BIAS = 0x4b400000u;       // the float 2^23 + 2^22: adding a whole number below 2^22 to its bits adds it to the float
-constexpr int W4_LONG = 4, W4_LONG_BF16 = 8;     // stages of 64 KB per SM from which on boxes are of 512 columns
+constexpr int W4_LONG = 8;                       // stages of 64 KB per SM from which on boxes are of 512 columns
 constexpr int W4_WAIT_LIMIT = 100000;
 constexpr int W4_SMEM = 227 * 1024 - 512;   // of a block; 512 bytes of barriers
 
@@ -70,16 +70,23 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t mask, uint32_
   return r;
 }
 
-// What a group's sum of a column starts from and is scaled by.
+// two bf16 less another: whole numbers below 256, exact
+__device__ __forceinline__ uint32_t less2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Whole numbers: what a group's sum of a column starts from and is scaled by.
 struct W4Column {
-  uint32_t start;   // whole numbers: W4_BIAS - 8 sum d, or W4_BIAS; bf16: -136 X, or -128 X
-  float e;          // whole numbers: e / 2^(7 digit)
+  uint32_t start;   // W4_BIAS - 8 sum d, or W4_BIAS
+  float e;          // e / 2^(7 digit)
 };
 
 // WHOLE: the form; NT: its columns in eights; SUB: pieces of 256 columns in a box
 template <bool WHOLE, int NT, int SUB>
 __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ W4Params p) {
-  constexpr int W4_BOX = SUB * W4_PIECE, W4_STAGE = W4_WARPS * W4_BOX, SUMS = w4_sums(NT), E = 2 * SUB, PER = WHOLE ? 3 : 1;   // E: scales of a row that a lane holds; PER: columns of a token
+  constexpr int W4_BOX = SUB * W4_PIECE, W4_STAGE = W4_WARPS * W4_BOX, SUMS = w4_sums(NT), E = 2 * SUB, PER = WHOLE ? W4_DIGITS : 1;   // E: scales of a row that a lane holds; PER: columns of a token
   constexpr int BYTES = WHOLE ? 1 : 2;   // of a value of x in shared memory
   extern __shared__ unsigned char dyn[];
   __shared__ __align__(8) unsigned long long bars[2 * W4_STAGES_MAX + 2 * SUMS];
@@ -89,9 +96,9 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
   unsigned char* at_base = dyn + (base - smem_addr(dyn));
   float* s_red = reinterpret_cast<float*>(at_base + p.stages * W4_STAGE);          // [SUMS][NT][16 warps][32 lanes][4]
   float* s_out = s_red + SUMS * W4_WARPS * 32 * 4 * NT;                             // [NT][32 lanes][4]: of one unit
-  W4Column* s_col = reinterpret_cast<W4Column*>(s_out + 128 * NT);                  // [groups][8 NT]
-  float* s_x = reinterpret_cast<float*>(s_col + p.groups_smem * 8 * NT);            // [groups][8 NT]: sum of x, the column's part (with offsets)
-  unsigned char* s_dig = reinterpret_cast<unsigned char*>(s_x + (p.offsets ? p.groups_smem * 8 * NT : 0));   // x: [columns, and one of zeros][pitch]
+  W4Column* s_col = reinterpret_cast<W4Column*>(s_out + 128 * NT);                  // [groups][8 NT] (whole numbers)
+  float* s_x = reinterpret_cast<float*>(s_col + (WHOLE ? p.groups_smem * 8 * NT : 0));   // [groups][8 NT]: sum of x, the column's part (with offsets)
+  unsigned char* s_dig = reinterpret_cast<unsigned char*>(s_x + (p.offsets ? p.groups_smem * 8 * NT : 0));   // x: [columns, and one of zeros if there are no eights of them][pitch]
   const int kw = 1 << p.kw_log, per_stage = W4_WARPS >> p.kw_log;                   // warps on a unit, units of a stage
   const int steps = (p.boxes + kw - 1) >> p.kw_log;                                 // stages of a unit
   const int sets = (p.units + per_stage - 1) / per_stage, mine = ((int)gridDim.x - 1 - (int)blockIdx.x + sets) / (int)gridDim.x;   // sets of units that share stages
@@ -197,7 +204,13 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
           __syncwarp();
           // row r, column c of the unit's sums
           auto sum_at = [&](int r, int c) { return s_out[(((c >> 3) * 32 + (r & 7) * 4 + ((c & 7) >> 1)) * 4) + (r >> 3) * 2 + (c & 1)]; };
-          auto token = [&](int r, int t) { return WHOLE ? sum_at(r, 3 * t) + (sum_at(r, 3 * t + 1) + sum_at(r, 3 * t + 2)) : sum_at(r, t); };
+          auto token = [&](int r, int t) {
+            if (!WHOLE) return sum_at(r, t);
+            float y = 0.0f;
+#pragma unroll
+            for (int d = W4_DIGITS - 1; d >= 0; d--) y += sum_at(r, d);   // the smallest first
+            return y;
+          };
           const int per_token = p.gated ? 8 : 16;
           for (int k = lane; k < per_token * p.T; k += 32) {
             const int t = k / per_token, r = k % per_token, o = unit * unit_rows + r;
@@ -258,6 +271,7 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
   unsigned phase = 0;
   uint32_t mask, magic;
   asm volatile("mov.b32 %0, 0x000f000f;\n\tmov.b32 %1, 0x43004300;" : "=r"(mask), "=r"(magic));
+  const uint32_t bias = with_offsets ? 0x43004300u : 0x43084308u;   // 128, or 136
   unsigned d_lane[NT];   // this lane's column of x; of those that there are not a row of zeros
 #pragma unroll
   for (int n = 0; n < NT; n++) d_lane[n] = smem_addr(s_dig) + min(g + 8 * n, PER * p.T) * p.pitch + 8 * BYTES * t4;
@@ -276,63 +290,75 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
       v_next = load_x(t_next, part_next);
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
       if constexpr (WHOLE) {
-        float x[8];
         uint32_t top = 0;   // the largest magnitude's bits
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          x[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
-          top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-        }
+        for (int i = 0; i < 4; i++) top = max(top, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
         for (int off = group / 16; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
-        const bool odd = top >= 0x7f800000u;                       // an infinity or NaN: the token comes out as NaN
-        const uint32_t k = max(top >> 23, 27u);                    // largest value: [1, 2) 2^(k - 127), or below 2^-99
-        const float up = odd ? 0.0f : __uint_as_float((127u + 6u + 127u - k) << 23);   // 2^(133 - k): magnitudes below 128
-        int sum[3] = {0, 0, 0};
-        uint32_t digits[3][2] = {};
+        const bool odd = top >= 0x7f80u;                           // an infinity or NaN: the token comes out as NaN
+        const int k = max((int)(top >> 7), 7 * W4_DIGITS);         // largest value: [1, 2) 2^(k - 127), or less; the last digit's unit is 2^-126 at least
+        float e = odd ? NAN : __uint_as_float((uint32_t)(k - 6) << 23);
+        // A value is m 2^bit of the last digit's unit, m of 8 bits: two digits that follow one another, in their places of eight bytes.
+        uint32_t lo[8], hi[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          float r = odd ? 0.0f : x[e] * up;
-#pragma unroll
-          for (int d = 0; d < 3; d++) {
-            const float whole = fminf(rintf(r), 127.0f);
-            const int z = (int)whole;
-            r = (r - whole) * 128.0f;
-            sum[d] += z;
-            digits[d][e & 1] |= (uint32_t)(z & 255) << (8 * (e >> 1));   // even columns, odd columns
-          }
+        for (int i = 0; i < 8; i++) {
+          const uint32_t v = i & 1 ? w[i >> 1] >> 16 : w[i >> 1];
+          const int exponent = (int)(v >> 7 & 255);
+          uint32_t m = odd ? 0u : (v & 127) | (exponent ? 128u : 0u);
+          int bit = max(exponent, 1) - k + 7 * W4_DIGITS - 8;
+          m >>= min(max(-bit, 0), 31), bit = max(bit, 0);
+          const int digit = bit * 37 >> 8;   // bit / 7, up to 48
+          m <<= bit - 7 * digit;
+          const int sign = v & 0x8000u ? -1 : 1;
+          const uint32_t both = ((uint32_t)((int)(m & 127) * sign) & 255u) | ((uint32_t)((int)(m >> 7) * sign) & 255u) << 8;
+          const uint64_t at = (uint64_t)both << (8 * digit);
+          lo[i] = (uint32_t)at, hi[i] = (uint32_t)(at >> 32);
         }
-        const float e0 = odd ? NAN : __uint_as_float((k - 6u) << 23);
 #pragma unroll
-        for (int d = 0; d < 3; d++) {
-          for (int off = group / 16; off > 0; off >>= 1) sum[d] += __shfl_xor_sync(0xffffffffu, sum[d], off);
-          *reinterpret_cast<uint2*>(s_dig + (3 * t + d) * p.pitch + 256 * part + 8 * lane) = make_uint2(digits[d][0], digits[d][1]);
-          if ((lane & (group / 8 - 1)) == 0) {
-            const int at = ((256 * part + 8 * lane) / group) * 8 * NT + 3 * t + d;
-            const float e = e0 * (d == 0 ? 1.0f : d == 1 ? 0x1p-7f : 0x1p-14f);
-            s_col[at] = {with_offsets ? W4_BIAS : W4_BIAS - 8u * (uint32_t)sum[d], e};
-            if (with_offsets) s_x[at] = (float)sum[d] * e;
+        for (int half = 0; half < 2; half++) {   // the larger digits first
+          const uint32_t(&x)[8] = half ? lo : hi;
+          uint32_t even[4], uneven[4];           // [digit]: its bytes of the even columns, and of the others
+          auto turn = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t(&r)[4]) {
+            const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362), cd0 = __byte_perm(c, d, 0x5140), cd1 = __byte_perm(c, d, 0x7362);
+            r[3] = __byte_perm(ab0, cd0, 0x5410), r[2] = __byte_perm(ab0, cd0, 0x7632), r[1] = __byte_perm(ab1, cd1, 0x5410), r[0] = __byte_perm(ab1, cd1, 0x7632);
+          };
+          turn(x[0], x[2], x[4], x[6], even), turn(x[1], x[3], x[5], x[7], uneven);
+#pragma unroll
+          for (int j = 0; j < 4; j += 2) {   // two sums of 16 bits (at most 128 digits of 127) in a word
+            uint32_t sums = 0;
+#pragma unroll
+            for (int i = 1; i >= 0; i--) sums = (sums << 16) + (uint32_t)__dp4a((int)even[j + i], 0x01010101, __dp4a((int)uneven[j + i], 0x01010101, 0));
+            for (int off = group / 16; off > 0; off >>= 1) sums += __shfl_xor_sync(0xffffffffu, sums, off);
+            const int sum0 = (int16_t)sums, sum1 = (int)(sums - (uint32_t)sum0) >> 16;
+#pragma unroll
+            for (int i = 0; i < 2; i++, e *= 0x1p-7f) {
+              const int d = 4 * half + j + i, sum = i ? sum1 : sum0;
+              *reinterpret_cast<uint2*>(s_dig + (PER * t + d) * p.pitch + 256 * part + 8 * lane) = make_uint2(even[j + i], uneven[j + i]);
+              if ((lane & (group / 8 - 1)) == 0) {
+                const int at = ((256 * part + 8 * lane) / group) * 8 * NT + PER * t + d;
+                s_col[at] = {with_offsets ? W4_BIAS : W4_BIAS - 8u * (uint32_t)sum, e};
+                if (with_offsets) s_x[at] = (float)sum * e;
+              }
+            }
           }
         }
       } else {
         // (0, 4), (1, 5), (2, 6), (3, 7): the order in which the codes' pairs come out of a word
         *reinterpret_cast<uint4*>(s_dig + t * p.pitch + 512 * part + 16 * lane) =
             make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-        float X = 0.0f;
+        if (with_offsets) {
+          float X = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) X += __uint_as_float(w[e] << 16) + __uint_as_float(w[e] & 0xffff0000u);
-        for (int off = group / 16; off > 0; off >>= 1) X += __shfl_xor_sync(0xffffffffu, X, off);
-        if ((lane & (group / 8 - 1)) == 0) {
-          const int at = ((256 * part + 8 * lane) / group) * 8 * NT + t;
-          s_col[at] = {__float_as_uint(X * (with_offsets ? -128.0f : -136.0f)), 1.0f};
-          if (with_offsets) s_x[at] = X;
+          for (int e = 0; e < 4; e++) X += __uint_as_float(w[e] << 16) + __uint_as_float(w[e] & 0xffff0000u);
+          for (int off = group / 16; off > 0; off >>= 1) X += __shfl_xor_sync(0xffffffffu, X, off);
+          if ((lane & (group / 8 - 1)) == 0) s_x[((256 * part + 8 * lane) / group) * 8 * NT + t] = X;
         }
       }
     }
-    for (int i = tid; i < p.pitch / 8; i += 32 * W4_WARPS) *reinterpret_cast<uint2*>(s_dig + PER * p.T * p.pitch + 8 * i) = make_uint2(0, 0);
-    for (int i = tid; i < p.groups_smem * (8 * NT - PER * p.T); i += 32 * W4_WARPS) {
-      const int at = i / (8 * NT - PER * p.T) * 8 * NT + PER * p.T + i % (8 * NT - PER * p.T);
-      s_col[at] = {WHOLE ? W4_BIAS : 0u, 0.0f};
-      if (with_offsets) s_x[at] = 0.0f;
+    if (PER * p.T < 8 * NT) {   // columns that there are not
+      for (int i = tid; i < p.pitch / 8; i += 32 * W4_WARPS) *reinterpret_cast<uint2*>(s_dig + PER * p.T * p.pitch + 8 * i) = make_uint2(0, 0);
+      if (with_offsets)
+        for (int i = tid; i < p.groups_smem * (8 * NT - PER * p.T); i += 32 * W4_WARPS)
+          s_x[i / (8 * NT - PER * p.T) * 8 * NT + PER * p.T + i % (8 * NT - PER * p.T)] = 0.0f;
     }
     asm volatile("bar.sync 1, 512;" ::: "memory");
     for (int i = 0; i < mine; i++) {
@@ -352,11 +378,15 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
             for (int c0 = 0; c0 < 8 * SUB; c0 += CH) {
               const int in_box = c0 / CH, from = (lane & 28) | (in_box & 3);
               uint32_t d[NT][4];
-              float4 column[NT];   // of this lane's two columns: start and e
+              float4 column[NT];   // whole numbers: of this lane's two columns, start and e
 #pragma unroll
               for (int n = 0; n < NT; n++) {
-                column[n] = *reinterpret_cast<const float4*>(s_col + (kb * per_box + in_box) * 8 * NT + 2 * t4 + 8 * n);
-                d[n][0] = d[n][2] = __float_as_uint(column[n].x), d[n][1] = d[n][3] = __float_as_uint(column[n].z);
+                if constexpr (WHOLE) {
+                  column[n] = *reinterpret_cast<const float4*>(s_col + (kb * per_box + in_box) * 8 * NT + 2 * t4 + 8 * n);
+                  d[n][0] = d[n][2] = __float_as_uint(column[n].x), d[n][1] = d[n][3] = __float_as_uint(column[n].z);
+                } else {
+                  d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0;
+                }
               }
 #pragma unroll
               for (int c = c0; c < c0 + CH; c++) {
@@ -377,8 +407,8 @@ __global__ void __launch_bounds__(W4_THREADS, 1) gemv_w4_kernel(const __grid_con
                                  : "=r"(b[n][0]), "=r"(b[n][1]), "=r"(b[n][2]), "=r"(b[n][3])
                                  : "r"(d_lane[n] + d_at + 64 * c)
                                  : "memory");
-                  const uint32_t a0 = code_pair(w0, mask, magic), a1 = code_pair(w1, mask, magic), a2 = code_pair(w0 >> 4, mask, magic), a3 = code_pair(w1 >> 4, mask, magic);
-                  const uint32_t a4 = code_pair(w0 >> 8, mask, magic), a5 = code_pair(w1 >> 8, mask, magic), a6 = code_pair(w0 >> 12, mask, magic), a7 = code_pair(w1 >> 12, mask, magic);
+                  auto pair = [&](uint32_t w) { return less2(code_pair(w, mask, magic), bias); };
+                  const uint32_t a0 = pair(w0), a1 = pair(w1), a2 = pair(w0 >> 4), a3 = pair(w1 >> 4), a4 = pair(w0 >> 8), a5 = pair(w1 >> 8), a6 = pair(w0 >> 12), a7 = pair(w1 >> 12);
 #pragma unroll
                   for (int n = 0; n < NT; n++) {
                     mma_bf16(d[n], a0, a1, a2, a3, b[n][0], b[n][1]);
@@ -441,7 +471,7 @@ struct W4Plan {
 };
 W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated, bool offsets, bool whole, int sub) {
   W4Plan r = {};
-  const int columns = (int)(whole ? 3 * T : T), NT = (columns + 7) / 8, bytes = whole ? 1 : 2;
+  const int columns = (int)(whole ? W4_DIGITS * T : T), NT = (columns + 7) / 8, bytes = whole ? 1 : 2;
   r.whole = whole, r.tiles = NT, r.sub = sub;
   r.units = (int)(gated ? (n_out + 7) / 8 : (n_out + 15) / 16);
   const int all = (int)((I + 256 * sub - 1) / (256 * sub)), stage = W4_WARPS * sub * W4_PIECE, fixed = 1024 + 2 * stage + w4_sums(NT) * W4_WARPS * 32 * 16 * NT + 512 * NT;
@@ -450,7 +480,7 @@ W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated, b
     if (r.slices > 1 && r.boxes > W4_WARPS) r.boxes = (r.boxes + W4_WARPS - 1) / W4_WARPS * W4_WARPS;   // whole stages, but for the last
     r.pitch = r.boxes * 256 * sub * bytes + 32 * bytes;   // (four columns' 32 bytes, or two columns' 64, fill the banks)
     r.groups_smem = r.boxes * ((256 * sub) >> group_log);
-    r.smem = fixed + r.groups_smem * 8 * NT * (offsets ? 12 : 8) + (columns + 1) * r.pitch;
+    r.smem = fixed + r.groups_smem * 8 * NT * ((whole ? 8 : 0) + (offsets ? 4 : 0)) + (columns + (columns % 8 != 0)) * r.pitch;
     if (r.smem <= W4_SMEM || r.boxes == 1) break;
   }
   r.slices = (all + r.boxes - 1) / r.boxes;
@@ -459,14 +489,18 @@ W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated, b
   r.sets = (r.units + (W4_WARPS >> r.kw_log) - 1) / (W4_WARPS >> r.kw_log);
   return r;
 }
-// Boxes of 512 columns, which spread what a box costs besides its products, where an SM has many stages of them all the same; for one or two tokens in
-// whole numbers, whose digits have to pay.  Boxes of 256 and bf16 | of 512 and in whole numbers: one token, 24576 x 4096 (5 stages per SM) 22.9 | 20.9,
-// 151936 x 4096 (32) 105 | 70, 6144 x 4096 (1) 7.9 | 8.3;  of 256 | of 512, both bf16: six tokens, 24576 x 4096 (5) 25.5 | 27.3.
+// Boxes of 512 columns, which spread what a box costs besides its products, from eight stages per SM on; for one token in whole numbers, where all of its
+// digits fit at once.  B200, us, caches cold, events around a call, groups of 128 | of 64 with offsets.  One token, whole numbers, bf16 in boxes of 512,
+// of 256:  24576 x 4096 (5 stages per SM) 25.6, 25.6, 26.7 | gated 32.7, 30.8, 30.7;  36000 x 4096 (8) 30.8, 31.7, 34.8 | 38.9, 38.9, 39.9;  151936 x 4096 (32)
+// 80.8, 97.2, 112 | 109, 119, 128;  19000 x 12288 in two pieces 56.4, 51.3, 49.1.  Bf16 in boxes of 512, of 256:  six tokens, 24576 x 4096 gated 37.0, 34.9,
+// 36000 x 4096 42.9, 43.1, 64000 x 4096 gated 65.5, 67.6;  eight tokens, 151936 x 4096 104, 119.
 W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated, bool offsets) {
-  const bool whole = T <= 2;
-  const W4Plan two = w4_plan(n_out, I, T, group_log, gated, offsets, whole, 2);
-  const int64_t stages = (int64_t)two.sets * ((two.boxes + (1 << two.kw_log) - 1) >> two.kw_log);
-  return stages >= (whole ? W4_LONG : W4_LONG_BF16) * (int64_t)sm_count() ? two : w4_plan(n_out, I, T, group_log, gated, offsets, false, 1);
+  for (const bool whole : {T == 1, false}) {
+    const W4Plan two = w4_plan(n_out, I, T, group_log, gated, offsets, whole, 2);
+    const int64_t stages = (int64_t)two.sets * ((two.boxes + (1 << two.kw_log) - 1) >> two.kw_log);
+    if (stages >= W4_LONG * (int64_t)sm_count() && !(whole && two.slices > 1)) return two;
+  }
+  return w4_plan(n_out, I, T, group_log, gated, offsets, false, 1);
 }
 
 }  // namespace
