@@ -490,12 +490,14 @@ W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated, b
   return r;
 }
 // Boxes of 512 columns, which spread what a box costs besides its products, from eight stages per SM on; for one token in whole numbers, where all of its
-// digits fit at once.  B200, us, caches cold, events around a call, groups of 128 | of 64 with offsets.  One token, whole numbers, bf16 in boxes of 512,
+// digits fit at once.  Nine tokens and more, whose sums take two columns of eight and whose x then fits in fewer pieces, have boxes of 256.  B200, us, caches cold, events around a call, groups of 128 | of 64 with offsets.  One token, whole numbers, bf16 in boxes of 512,
 // of 256:  24576 x 4096 (5 stages per SM) 25.6, 25.6, 26.7 | gated 32.7, 30.8, 30.7;  36000 x 4096 (8) 30.8, 31.7, 34.8 | 38.9, 38.9, 39.9;  151936 x 4096 (32)
 // 80.8, 97.2, 112 | 109, 119, 128;  19000 x 12288 in two pieces 56.4, 51.3, 49.1.  Bf16 in boxes of 512, of 256:  six tokens, 24576 x 4096 gated 37.0, 34.9,
-// 36000 x 4096 42.9, 43.1, 64000 x 4096 gated 65.5, 67.6;  eight tokens, 151936 x 4096 104, 119.
+// 36000 x 4096 42.9, 43.1, 64000 x 4096 gated 65.5, 67.6;  eight tokens, 151936 x 4096 104, 119, 19000 x 12288 64, 72, 19000 x 16384 82, 78;  nine, 151936 x 4096 233, 154;  sixteen, the same 339, 236, 24576 x 4096 78, 55,
+// twelve, 152000 x 768 111, 113.
 W4Plan w4_plan(int64_t n_out, int64_t I, int64_t T, int group_log, bool gated, bool offsets) {
   for (const bool whole : {T == 1, false}) {
+    if (T > 8) break;
     const W4Plan two = w4_plan(n_out, I, T, group_log, gated, offsets, whole, 2);
     const int64_t stages = (int64_t)two.sets * ((two.boxes + (1 << two.kw_log) - 1) >> two.kw_log);
     if (stages >= W4_LONG * (int64_t)sm_count() && !(whole && two.slices > 1)) return two;
@@ -576,8 +578,9 @@ extern "C" int pk_gemv_w4(const pk_tensor* weight, const pk_tensor* scales, cons
   using Two = std::integral_constant<int, 2>;
   using Bf16 = std::false_type;
   const int rc = plan.whole ? launch(std::true_type(), One(), Two())
-                 : plan.tiles == 1 ? (plan.sub == 1 ? launch(Bf16(), One(), One()) : launch(Bf16(), One(), Two()))
-                                   : (plan.sub == 1 ? launch(Bf16(), Two(), One()) : launch(Bf16(), Two(), Two()));
+                 : plan.tiles == 2 ? launch(Bf16(), Two(), One())
+                 : plan.sub == 2   ? launch(Bf16(), One(), Two())
+                                   : launch(Bf16(), One(), One());
   if (rc) return rc;
   return check_launch("gemv_w4");
 }
