@@ -122,8 +122,10 @@ __device__ __forceinline__ void ldmatrix4t(uint32_t (&r)[4], unsigned addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
 // ROWS 8: the eight rows are the upper half of the A operands; in P V the lower half carries what the rounding of P to bf16 left, and the two halves
-// of O are added: 17 bits of each weight for no further product.  ROWS 16, 32: one or two full operands, weights of 8 bits; the sums have them all.
+// of O are added, where that one is finite: 17 bits of each weight for no further product.  ROWS 16, 32: one or two full operands, weights of 8 bits; the sums have them all.
 template <bool TREE, int ROWS>
 __global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
     attend_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dk,
@@ -393,7 +395,8 @@ __global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
 #pragma unroll
         for (int n = 0; n < 16; n++) {
           float2 v = make_float2(o[mt][n][2 * e], o[mt][n][2 * e + 1]);
-          if (PAIR) v.x += o[mt][n][2], v.y += o[mt][n][3];
+          // an infinite value times what a rounding left is an infinity of any sign, or NaN where nothing was left: the other half has it
+          if (PAIR) v.x += finite(o[mt][n][2]) ? o[mt][n][2] : 0.0f, v.y += finite(o[mt][n][3]) ? o[mt][n][3] : 0.0f;
           *reinterpret_cast<float2*>(to + 8 * n) = make_float2(v.x * f, v.y * f);
         }
         named_barrier(1, 128);
