@@ -103,7 +103,8 @@ __device__ __forceinline__ void query_sums(const SelectParams& p, int64_t b, int
 
 // Scores in 32 bits, and a bound A of every sum of absolute values: A = sum_d P_d max |hi_d| + |N_d| max |lo_d| over the warp's blocks.  A score is off
 // by at most G + 13 roundings of 2^-24 A (P or N, eight products in a row, five additions of the lanes' sums): where the choice hangs on less
-// than that, block_pick_kernel takes the 64-bit scores.
+// than that, block_pick_kernel takes the 64-bit scores.  Products below 2^-100 count as that much in A, which leaves room for what 32 bits lose where they hold
+// numbers by fewer digits: A is zero only where every product is.
 // A warp of its own brings 32 blocks of keys at a time, 16 KB, into a ring of four stages; each of four warps takes eight of them for TT tokens: lanes
 // 0 .. 15 hold eight channels of lo and N each, the others of hi and P.  Bounded by the bounds' bytes where there are many, otherwise by
 // latency.  With the choice, us, by loads to registers two groups ahead | by the ring: 8192 blocks of 8 heads for four tokens 29 | 28, for one 21 | 18,
@@ -231,7 +232,10 @@ __global__ void __launch_bounds__(SCORE_THREADS, SCORE_CTAS) block_score_kernel(
   for (int k = 0; k < TT; k++) {
     float A = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; e++) A += fabsf(c[k][e]) * (e & 1 ? __high2float(top[e >> 1]) : __low2float(top[e >> 1]));   // (infinite bounds: inf or NaN)
+    for (int e = 0; e < 8; e++) {   // (infinite bounds: inf or NaN)
+      const float x = fabsf(c[k][e]), y = e & 1 ? __high2float(top[e >> 1]) : __low2float(top[e >> 1]), a = x * y;
+      A += a < 0x1p-100f && x != 0.0f && y != 0.0f ? 0x1p-100f : a;
+    }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) A += __shfl_xor_sync(0xffffffffu, A, off);
     if (lane == 0 && t0 + k < p.T) p.limits[((b * p.T + t0 + k) * p.H + h) * warps + self] = dead ? NAN : A;
