@@ -529,8 +529,8 @@ int pk_gemv(const pk_tensor* weight, const pk_tensor* x, const pk_tensor* out, i
 
 /* ---- several tokens a step: a tree of drafts, blocks of the cache, 4-bit weights ------------------------- */
 
-/* Positions follow the device: lengths i32 [bs] holds the rows of the cache per sample (values outside [0, cap] are clamped),
- * so that a captured step stays valid while the sequences grow.  Rows of 128 bf16 with a unit inner stride, the other strides
+/* Positions follow the device: lengths i32 [bs] holds the rows of the cache per sample (values outside [0, cap] are clamped; by
+ * pk_select_blocks, which does not know cap, to its whole blocks), so that a captured step stays valid while the sequences grow.  Rows of 128 bf16 with a unit inner stride, the other strides
  * multiples of 8 elements, 16-byte aligned.  A query that sees no row gets zeros, and lse = -inf.  What a query does not see
  * does not reach it, whatever is stored there (NaN and infinities included).  lse (f32 [bs,T,Hq] or NULL) is the log2 of the
  * softmax denominator, as in pk_sparse_attention; scale has to be positive.  workspace: device, 256-byte aligned, pk_*_workspace_bytes; nothing in it
@@ -548,7 +548,8 @@ int pk_gemv(const pk_tensor* weight, const pk_tensor* x, const pk_tensor* out, i
  *   with the largest score are listed in blocks i32 [bs,T,H,n], ascending, -1 behind the last; the first sink_blocks and the
  *   last local_blocks (>= 1) are always among them.  score = sum over the group's query heads and the channels of
  *   max(q lo, q hi) (a zero of q adds nothing), summed in 64 bits and rounded once to 32; ties go to the lower block, a NaN score is
- *   above all others.
+ *   above all others.  pk_select_blocks_ex: the same with the rows of the cache, so that lengths above them are clamped as the attention
+ *   clamps them; ceil(cap/block) blocks, or cap -1 for pk_select_blocks.
  * pk_block_attention: query (b,t,h*G+g), at the same position, attends to the rows up to it of the listed blocks.  Entries below zero
  *   and blocks behind the position are skipped; the order is free; a block listed twice counts twice.
  * pk_gemv_w4: out[T,O] = x[T,I] W^T for up to 16 tokens, fp32 sums.  weight u8 [O,I/2], the low nibble of a byte the even column;
@@ -567,6 +568,9 @@ int64_t pk_select_blocks_workspace_bytes(int64_t bs, int64_t T, int64_t H, int64
 int pk_select_blocks(const pk_tensor* queries, const pk_tensor* bounds, const pk_tensor* lengths, int64_t block,
                      int64_t sink_blocks, int64_t local_blocks, const pk_tensor* blocks, void* workspace,
                      int64_t workspace_bytes, void* stream);
+int pk_select_blocks_ex(const pk_tensor* queries, const pk_tensor* bounds, const pk_tensor* lengths, int64_t block, int64_t cap,
+                        int64_t sink_blocks, int64_t local_blocks, const pk_tensor* blocks, void* workspace,
+                        int64_t workspace_bytes, void* stream);
 int64_t pk_block_attention_workspace_bytes(int64_t bs, int64_t T, int64_t Hq, int64_t H, int64_t n, int64_t block);
 int pk_block_attention(const pk_tensor* queries, const pk_tensor* keys, const pk_tensor* values, const pk_tensor* blocks,
                        const pk_tensor* lengths, int64_t block, float scale, const pk_tensor* out, const pk_tensor* lse,

@@ -106,6 +106,7 @@ SIGNATURES = {
     "pk_block_bounds": (_INT, [TP, TP, _I64, _I64, TP, _VP]),
     "pk_select_blocks_workspace_bytes": (_I64, [_I64] * 4),
     "pk_select_blocks": (_INT, [TP, TP, TP, _I64, _I64, _I64, TP, _VP, _I64, _VP]),
+    "pk_select_blocks_ex": (_INT, [TP, TP, TP, _I64, _I64, _I64, _I64, TP, _VP, _I64, _VP]),
     "pk_block_attention_workspace_bytes": (_I64, [_I64] * 6),
     "pk_block_attention": (_INT, [TP] * 5 + [_I64, _F32, TP, TP, _VP, _I64, _VP]),
     "pk_gemv_w4_workspace_bytes": (_I64, [_I64] * 4 + [_INT]),

@@ -47,7 +47,7 @@ struct SelectParams {
   const uint16_t* q;
   int64_t q_b, q_t, q_h;
   const uint16_t* bounds;
-  int64_t o_b, o_h, o_j, nb;
+  int64_t o_b, o_h, o_j, nb, cap;   // cap: rows of the cache, in nb blocks
   const int32_t* lengths;
   int T, H, G, n, block, sink, local;
   uint32_t* keys;      // [rows][nb] ordered keys of the scores
@@ -60,7 +60,7 @@ constexpr uint32_t FORCED = 0xffffffffu, NOT_A_NUMBER = 0xfffffffeu;
 
 // Blocks that row (b, t) sees.
 __device__ __forceinline__ int visible_blocks(const SelectParams& p, int64_t b, int t) {
-  const int64_t pos = min((int64_t)p.lengths[b], p.nb * p.block) - p.T + t;
+  const int64_t pos = min((int64_t)p.lengths[b], p.cap) - p.T + t;
   return pos < 0 ? 0 : (int)(pos / p.block) + 1;
 }
 
@@ -487,6 +487,12 @@ extern "C" int64_t pk_select_blocks_workspace_bytes(int64_t bs, int64_t T, int64
 
 extern "C" int pk_select_blocks(const pk_tensor* queries, const pk_tensor* bounds, const pk_tensor* lengths, int64_t block, int64_t sink_blocks,
                                 int64_t local_blocks, const pk_tensor* blocks, void* workspace, int64_t workspace_bytes, void* stream) {
+  return pk_select_blocks_ex(queries, bounds, lengths, block, -1, sink_blocks, local_blocks, blocks, workspace, workspace_bytes, stream);
+}
+
+extern "C" int pk_select_blocks_ex(const pk_tensor* queries, const pk_tensor* bounds, const pk_tensor* lengths, int64_t block, int64_t cap,
+                                   int64_t sink_blocks, int64_t local_blocks, const pk_tensor* blocks, void* workspace,
+                                   int64_t workspace_bytes, void* stream) {
   PK_CHECK_TENSOR(queries, PK_BF16, 4);
   if (const int rc = check_bounds(bounds)) return rc;
   PK_CHECK_TENSOR(lengths, PK_I32, 1);
@@ -499,12 +505,14 @@ extern "C" int pk_select_blocks(const pk_tensor* queries, const pk_tensor* bound
   PK_REQUIRE(blocks->shape[0] == bs && blocks->shape[1] == T && blocks->shape[2] == H && is_contig(blocks), "blocks must be contiguous i32 [bs,T,H,n]");
   PK_REQUIRE(sink_blocks >= 0 && local_blocks >= 1 && sink_blocks + local_blocks <= n, "at least one local block, and no more sink and local blocks than are selected");
   PK_REQUIRE(nb * block < (1LL << 31) && n < (1LL << 24), "sizes out of range");
+  PK_REQUIRE(cap == -1 || (cap >= 0 && (cap + block - 1) / block == nb), "cap must be the rows of the cache that the bounds are of, or -1");
   if (bs * T * H == 0) return PK_OK;
   PK_REQUIRE(nb > 0, "bounds of no block");
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < pk_select_blocks_workspace_bytes(bs, T, H, nb)) return fail(PK_ERR_WORKSPACE, "select_blocks: workspace missing, misaligned or too small");
   SelectParams p = {};
   p.q = (const uint16_t*)queries->data, p.q_b = queries->stride[0], p.q_t = queries->stride[1], p.q_h = queries->stride[2];
   p.bounds = (const uint16_t*)bounds->data, p.o_b = bounds->stride[0], p.o_h = bounds->stride[1], p.o_j = bounds->stride[2], p.nb = nb;
+  p.cap = cap < 0 ? nb * block : cap;
   p.lengths = (const int32_t*)lengths->data, p.T = (int)T, p.H = (int)H, p.G = (int)(Hq / H), p.n = (int)n, p.block = (int)block;
   p.sink = (int)sink_blocks, p.local = (int)local_blocks, p.keys = (uint32_t*)workspace, p.ids = (int32_t*)blocks->data;
   const int64_t rows = bs * T * H;

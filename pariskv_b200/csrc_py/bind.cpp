@@ -673,15 +673,15 @@ PyObject* py_block_bounds(PyObject*, PyObject* const* a, Py_ssize_t n) {
   PK_PY_END
 }
 
-// (queries, bounds, lengths, n_select, block, sink_blocks, local_blocks, blocks or None) -> blocks
+// (queries, bounds, lengths, n_select, block, sink_blocks, local_blocks, blocks or None, cap or -1) -> blocks
 PyObject* py_select_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!arity(n, 8, "select_blocks")) return nullptr;
+  if (!arity(n, 9, "select_blocks")) return nullptr;
   PK_PY_BEGIN
   Arg q, bd, len, out;
   at::Tensor own;
-  int64_t k, block, sink, local;
+  int64_t k, block, sink, local, cap;
   if (!need(a[0], &q, CUDA) || !need(a[1], &bd, CUDA) || !need(a[2], &len, CUDA) || !to_i64(a[3], &k) || !to_i64(a[4], &block) ||
-      !to_i64(a[5], &sink) || !to_i64(a[6], &local) || !dims(q, 4, "queries") || !dims(bd, 5, "bounds"))
+      !to_i64(a[5], &sink) || !to_i64(a[6], &local) || !to_i64(a[8], &cap) || !dims(q, 4, "queries") || !dims(bd, 5, "bounds"))
     return nullptr;
   if (k < 1) return PyErr_SetString(PyExc_RuntimeError, "pariskv_b200: n_select must be at least 1"), nullptr;
   const c10::cuda::CUDAGuard guard(q.t->device());
@@ -690,7 +690,7 @@ PyObject* py_select_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t bytes = pk_select_blocks_workspace_bytes(q.d.shape[0], q.d.shape[1], bd.d.shape[1], bd.d.shape[2]);
   const at::Tensor ws = empty_on(*q.t, {bytes}, at::kByte);
   void* st = stream_of(*q.t);
-  const int rc = without_gil([&] { return pk_select_blocks(q.p(), bd.p(), len.p(), block, sink, local, out.p(), ws.data_ptr(), bytes, st); });
+  const int rc = without_gil([&] { return pk_select_blocks_ex(q.p(), bd.p(), len.p(), block, cap, sink, local, out.p(), ws.data_ptr(), bytes, st); });
   if (rc) return raise(rc);
   return give(a[7], out);
   PK_PY_END

@@ -529,12 +529,16 @@ def block_bounds(keys, lengths=None, block=64, n_new=None, bounds=None):
     return L.native().block_bounds(keys, lengths, int(block), -1 if n_new is None else int(n_new), bounds)
 
 
-def select_blocks(queries, bounds, lengths, n_select, block=64, sink_blocks=1, local_blocks=1, blocks=None):
+def select_blocks(queries, bounds, lengths, n_select, block=64, sink_blocks=1, local_blocks=1, blocks=None, cap=None):
     """The n_select blocks with the largest scores for every token and KV head, and always the first sink_blocks and the last
     local_blocks that the token sees: queries bf16 [bs,T,Hq,128], the last T tokens of the sequences, bounds as block_bounds
     makes them -> i32 [bs,T,H,n_select], ascending, -1 behind the last.  A block's score is an upper bound of the sum of its
-    best products with the group's query heads.  See pk_select_blocks."""
-    return L.native().select_blocks(queries, bounds, lengths, int(n_select), int(block), int(sink_blocks), int(local_blocks), blocks)
+    best products with the group's query heads.  cap: the rows of the cache; lengths above it are then clamped as block_attention clamps
+    them, without it to whole blocks.  See pk_select_blocks."""
+    if cap is not None and cap < 0:
+        raise ValueError("cap must not be negative")
+    return L.native().select_blocks(queries, bounds, lengths, int(n_select), int(block), int(sink_blocks), int(local_blocks), blocks,
+                                    -1 if cap is None else int(cap))
 
 
 def block_attention(queries, keys, values, blocks, lengths, block=64, scale=None, out=None, lse=None):
