@@ -533,7 +533,7 @@ int pk_gemv(const pk_tensor* weight, const pk_tensor* x, const pk_tensor* out, i
  * pk_select_blocks, which does not know cap, to its whole blocks), so that a captured step stays valid while the sequences grow.  Rows of 128 bf16 with a unit inner stride, the other strides
  * multiples of 8 elements, 16-byte aligned.  A query that sees no row gets zeros, and lse = -inf.  What a query does not see
  * does not reach it, whatever is stored there (NaN and infinities included).  lse (f32 [bs,T,Hq] or NULL) is the log2 of the
- * softmax denominator, as in pk_sparse_attention; scale has to be positive.  workspace: device, 256-byte aligned, pk_*_workspace_bytes; nothing in it
+ * softmax denominator, as in pk_sparse_attention; scale has to be positive, and scale * log2 e finite in 32 bits.  workspace: device, 256-byte aligned, pk_*_workspace_bytes; nothing in it
  * has to be cleared and nothing carries over between calls.  No counterpart in the reference.
  *
  * pk_tree_attention: T drafted tokens per sequence (at most 256) attend to rows [0, lengths[b]) of the cache and to the drafts that

@@ -63,7 +63,7 @@ inline int fill_attend(AttendParams* p, const pk_tensor* queries, const pk_tenso
   p->T = (int)T, p->H = (int)H, p->G = (int)(Hq / H);
   p->scale_log2 = scale * 1.4426950408889634f;
   p->out = (uint16_t*)out->data;
-  PK_REQUIRE(scale > 0.0f && scale <= 3.0e38f, "scale must be positive");
+  PK_REQUIRE(scale > 0.0f && p->scale_log2 <= 3.4e38f, "scale must be positive, and finite as a factor of log2 e");
   return PK_OK;
 }
 
