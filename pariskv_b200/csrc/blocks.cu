@@ -525,14 +525,14 @@ extern "C" int pk_select_blocks_ex(const pk_tensor* queries, const pk_tensor* bo
   const dim3 grid((unsigned)(per_head < room ? per_head : room), (unsigned)heads, (unsigned)bs);
   p.limits = (float*)(p.keys + rows * nb);
   auto score = [&](auto tokens) -> int {
-    constexpr auto kernel = block_score_kernel<decltype(tokens)::value>;
+    constexpr int TT = decltype(tokens)::value;
     static PerDevice opted;
     if (const unsigned long long bit = first_on_device(opted)) {
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SCORE_STAGES * SCORE_STAGE) != cudaSuccess)
+      if (cudaFuncSetAttribute(block_score_kernel<TT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SCORE_STAGES * SCORE_STAGE) != cudaSuccess)
         return fail(PK_ERR_CUDA, "select_blocks: %s", cudaGetErrorString(cudaGetLastError()));
       mark_on_device(opted, bit);
     }
-    launch_chain(kernel, grid, dim3(SCORE_THREADS), SCORE_STAGES * SCORE_STAGE, (cudaStream_t)stream, p);
+    launch_chain(block_score_kernel<TT>, grid, dim3(SCORE_THREADS), SCORE_STAGES * SCORE_STAGE, (cudaStream_t)stream, p);
     return PK_OK;
   };
   if (const int rc = tt == 1 ? score(std::integral_constant<int, 1>()) : tt == 2 ? score(std::integral_constant<int, 2>()) : score(std::integral_constant<int, 4>())) return rc;

@@ -564,14 +564,15 @@ extern "C" int pk_gemv_w4(const pk_tensor* weight, const pk_tensor* scales, cons
   const unsigned grid = (unsigned)(plan.sets < sm_count() ? plan.sets : sm_count());
   StageTimer timer(ST_GEMV, (cudaStream_t)stream);
   auto launch = [&](auto whole, auto nt, auto sub) -> int {
-    constexpr auto kernel = gemv_w4_kernel<decltype(whole)::value, decltype(nt)::value, decltype(sub)::value>;
+    constexpr bool WHOLE = decltype(whole)::value;
+    constexpr int NT = decltype(nt)::value, SUB = decltype(sub)::value;
     static PerDevice opted;
     if (const unsigned long long bit = first_on_device(opted)) {
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM) != cudaSuccess)
+      if (cudaFuncSetAttribute(gemv_w4_kernel<WHOLE, NT, SUB>, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM) != cudaSuccess)
         return fail(PK_ERR_CUDA, "gemv_w4: %s", cudaGetErrorString(cudaGetLastError()));
       mark_on_device(opted, bit);
     }
-    launch_chain(kernel, dim3(grid), dim3(W4_THREADS), (size_t)plan.smem, (cudaStream_t)stream, map, p);
+    launch_chain(gemv_w4_kernel<WHOLE, NT, SUB>, dim3(grid), dim3(W4_THREADS), (size_t)plan.smem, (cudaStream_t)stream, map, p);
     return PK_OK;
   };
   using One = std::integral_constant<int, 1>;
