@@ -1,9 +1,9 @@
 // Attention of a few query rows per KV head - a token over the blocks that it selected, a small tree of drafted tokens over the cache - with
 // the keys spread over the warps:  o = sum_j p_j v_j / sum_j p_j,  p_j = 2^((s_j - max s) scale log2 e),  s_j = q.k_j.
 //
-// 4 to 32 rows cannot fill the 128 rows of a tcgen05 product, and a softmax thread per row would leave most threads idle: here a warp takes
+// 1 to 32 rows cannot fill the 128 rows of a tcgen05 product, and a softmax thread per row would leave most threads idle: here a warp takes
 // 16 of a tile's 64 keys for all rows (mma.sync m16n8k16), its fragments of S are the operand of P V, and the four warps' (m, l, O) meet once per
-// segment.  K and V come by TMA, a box per block of keys and half of the channels, three tiles of 32 KB under way in each of two blocks per SM:
+// segment.  K and V come by TMA, a box per block of keys and half of the channels, three tiles of 32 KB under way in each of two blocks per SM (one for more than 16 rows):
 // the copies, not the products, are what bounds it.  As in tree_attention.cu the tiles of all items, laid end to end, are cut into equal
 // ranges, and few_merge_kernel joins the records of items that are cut.
 #include "tiles.cuh"
