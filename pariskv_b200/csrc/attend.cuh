@@ -69,7 +69,7 @@ inline int fill_attend(AttendParams* p, const pk_tensor* queries, const pk_tenso
 
 // One warp per query row, plain loads: for the strides that tensor maps do not take.
 int launch_attend_rows(const AttendParams& p, int64_t bs, const char* what, cudaStream_t st);
-// Up to 32 query rows per KV head (attend_few.cu); workspace: attend_few_workspace() bytes.
+// Drafted tokens of up to 16 query rows per KV head, listed blocks (attend_few.cu); workspace: attend_few_workspace() bytes.
 int launch_attend_few(const AttendParams& p, int64_t bs, void* workspace, const char* what, cudaStream_t st);
 int64_t attend_few_workspace();
 

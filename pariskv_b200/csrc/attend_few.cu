@@ -1,4 +1,4 @@
-// Attention of a few query rows per KV head - a token over the blocks that it selected, a small tree of drafted tokens over the cache - with
+// Attention of a few query rows per KV head - a token over the blocks that it selected, up to 16 rows of drafted tokens over the cache - with
 // the keys spread over the warps:  o = sum_j p_j v_j / sum_j p_j,  p_j = 2^((s_j - max s) scale log2 e),  s_j = q.k_j.
 //
 // 1 to 32 rows cannot fill the 128 rows of a tcgen05 product, and a softmax thread per row would leave most threads idle: here a warp takes
@@ -505,7 +505,7 @@ int launch_attend_few(const AttendParams& a, int64_t bs, void* workspace, const 
   else maps[2] = maps[0], maps[3] = maps[1];
   if (!ok) return launch_attend_rows(a, bs, what, st);
   const int64_t most = tree ? bs * a.H * ((a.cap + FEW_TILE - 1) / FEW_TILE + 1) : bs * a.T * a.H * p.row_groups * (int64_t)p.tiles;
-  if (tree) return per == 8 ? launch<true, 8>(p, maps, most, what, st) : per == 16 ? launch<true, 16>(p, maps, most, what, st) : launch<true, 32>(p, maps, most, what, st);
+  if (tree) return per == 8 ? launch<true, 8>(p, maps, most, what, st) : launch<true, 16>(p, maps, most, what, st);
   return per == 8 ? launch<false, 8>(p, maps, most, what, st) : per == 16 ? launch<false, 16>(p, maps, most, what, st) : launch<false, 32>(p, maps, most, what, st);
 }
 

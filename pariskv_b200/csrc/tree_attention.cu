@@ -20,7 +20,10 @@ constexpr int TA_TILE = 128;                   // keys of a tile
 constexpr int TA_THREADS = 576;                // two streams of eight softmax warps, a warp for the copies, a warp for the products
 constexpr int TA_STAGE = 32768;                // a tile of K or V: two halves of 64 channels, 128 rows of 128 bytes
 constexpr int TA_WAIT_LIMIT = 100000;          // tries; one waits up to 10 us by itself
-constexpr int TA_FEW = 32;                       // up to so many query rows attend_few.cu has the call
+// Up to so many query rows attend_few.cu has the call: two operands of 16 rows take its registers, one block per SM, and twice the time.  B200, us, replayed graphs, 8 KV
+// heads of 4 queries, attend_few.cu | here:  701 keys, 4 rows 8.7 | 11.3, 16 rows 11.4 | 11.7, 32 rows 23.1 | 12.5;  131072 keys, 4 rows 91.2 | 92.1, 8 rows
+// 92.8 | 92.3, 16 rows 95.6 | 94.3, 20 rows 175 | 94, 32 rows 202 | 97;  8 x 8192 keys, 8 rows 53.9 | 58, 16 rows 58.5 | 59, 32 rows 131 | 63.
+constexpr int TA_FEW = 16;
 constexpr float TA_LAZY = 8.0f;                // log2: the maximum that O is scaled to may lie this far below the true one
 
 template <int NT> struct TaRing { static constexpr int stages = NT == 2 ? 5 : 6; };
