@@ -3,7 +3,7 @@
 //
 // 1 to 32 rows cannot fill the 128 rows of a tcgen05 product, and a softmax thread per row would leave most threads idle: here a warp takes
 // 16 of a tile's 64 keys for all rows (mma.sync m16n8k16), its fragments of S are the operand of P V, and the four warps' (m, l, O) meet once per
-// segment.  K and V come by TMA, a box per block of keys and half of the channels, three tiles of 32 KB under way in each of two blocks per SM (one for more than 16 rows):
+// segment.  K and V come by TMA, a box per block of keys and half of the channels, three tiles of 32 KB under way in each of two blocks per SM:
 // the copies, not the products, are what bounds it.  As in tree_attention.cu the tiles of all items, laid end to end, are cut into equal
 // ranges, and few_merge_kernel joins the records of items that are cut.
 #include "tiles.cuh"
@@ -18,7 +18,7 @@ constexpr int FEW_SMEM = 1024 + FEW_BUFS * FEW_STAGE;
 static_assert(4 * 8 * FEW_OS * 4 <= FEW_STAGE, "the warps' partials of eight rows take the place of a tile");
 constexpr int FEW_WAIT_LIMIT = 100000;              // (a try waits up to 10 us by itself)
 
-__host__ __device__ constexpr int few_ctas(int rows) { return rows > 16 ? 1 : 2; }   // blocks per SM: by the registers
+constexpr int FEW_CTAS = 2;                         // blocks per SM: by the registers
 
 struct FewParams {
   AttendParams a;
@@ -125,12 +125,13 @@ __device__ __forceinline__ void ldmatrix4t(uint32_t (&r)[4], unsigned addr) {
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
 // ROWS 8: the eight rows are the upper half of the A operands; in P V the lower half carries what the rounding of P to bf16 left, and the two halves
-// of O are added, where that one is finite: 17 bits of each weight for no further product.  ROWS 16, 32: one or two full operands, weights of 8 bits; the sums have them all.
+// of O are added, where that one is finite: 17 bits of each weight for no further product.  ROWS 16: a full operand, weights of 8 bits; the sums have them
+// all.  More heads of a listed block are groups of 16: two operands at once took the registers of one of the two blocks per SM.  B200, us, groups of 16 | two
+// operands: 16 sequences x 8 x 20 heads over 32 blocks of 64 keys 47 | 55, 4 sequences x 128 heads over 64 blocks 21 | 29, one sequence x 8 x 32 12 | 15.
 template <bool TREE, int ROWS>
-__global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
+__global__ void __launch_bounds__(FEW_THREADS, FEW_CTAS)
     attend_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dk,
                       const __grid_constant__ CUtensorMap map_dv, const __grid_constant__ FewParams p) {
-  constexpr int MT = ROWS == 32 ? 2 : 1;          // operands of 16 rows
   constexpr bool PAIR = ROWS == 8;
   constexpr int RPT = PAIR ? 1 : 2;               // rows of an operand that a lane's fragments belong to
   extern __shared__ unsigned char dyn[];
@@ -227,7 +228,6 @@ __global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
     return;
   }
 
-  constexpr int OUT_ROWS = PAIR ? 8 : ROWS;
   const int Hq = p.a.H * p.a.G;
   const float scale = p.a.scale_log2;
   // row r of the item -> token and query head
@@ -239,20 +239,18 @@ __global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
     const int n_rows = TREE ? tree_rows : min(ROWS, p.a.G - cur.group * ROWS);
     const int seg_first = cur.tile, seg = min(cur.n - cur.tile, count - k);
     const bool whole = seg == cur.n, has_drafts = TREE && seg_first + seg == cur.n;
-    uint32_t qa[MT][8][2 * RPT];
+    uint32_t qa[8][2 * RPT];
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++)
+    for (int e = 0; e < RPT; e++) {
+      const int r = 8 * e + g;
+      const bool ok = r < n_rows;
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(p.a.q + cur.b * p.a.q_b + (ok ? (int64_t)row_token(r) * p.a.q_t + (int64_t)row_head(r) * p.a.q_h : 0));
 #pragma unroll
-      for (int e = 0; e < RPT; e++) {
-        const int r = 16 * mt + 8 * e + g;
-        const bool ok = r < n_rows;
-        const uint32_t* q = reinterpret_cast<const uint32_t*>(p.a.q + cur.b * p.a.q_b + (ok ? (int64_t)row_token(r) * p.a.q_t + (int64_t)row_head(r) * p.a.q_h : 0));
-#pragma unroll
-        for (int ks = 0; ks < 8; ks++) {
-          qa[mt][ks][e] = ok ? q[8 * ks + t4] : 0u;             // columns 2 t4 of the step
-          qa[mt][ks][RPT + e] = ok ? q[8 * ks + 4 + t4] : 0u;   // and eight further
-        }
+      for (int ks = 0; ks < 8; ks++) {
+        qa[ks][e] = ok ? q[8 * ks + t4] : 0u;             // columns 2 t4 of the step
+        qa[ks][RPT + e] = ok ? q[8 * ks + 4 + t4] : 0u;   // and eight further
       }
+    }
     if (has_drafts) {   // a bit per draft for every token
       for (int t = warp; t < p.a.T; t += 4) {
         const unsigned bits = __ballot_sync(0xffffffffu, lane < p.a.T && p.a.mask[cur.b * p.a.m_b + t * p.a.m_t + lane * p.a.m_j] != 0);
@@ -260,14 +258,9 @@ __global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
       }
       named_barrier(1, 128);
     }
-    float o[MT][16][4], m[MT][RPT], l[MT][RPT];
+    float o[16][4] = {}, m[RPT], l[RPT];
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-#pragma unroll
-      for (int n = 0; n < 16; n++) o[mt][n][0] = o[mt][n][1] = o[mt][n][2] = o[mt][n][3] = 0.0f;
-#pragma unroll
-      for (int e = 0; e < RPT; e++) m[mt][e] = -INFINITY, l[mt][e] = 0.0f;
-    }
+    for (int e = 0; e < RPT; e++) m[e] = -INFINITY, l[e] = 0.0f;
     for (int j = 0; j < seg; j++, k++) {
       const int buf = k % FEW_BUFS;
       wait(full + 8 * buf, (unsigned)(k / FEW_BUFS & 1));
@@ -300,60 +293,53 @@ __global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
           fence_async();   // before the copy that will fill the stage again
           __syncwarp();
         }
-        float sc[MT][2][4];
+        float sc[2][4];
 #pragma unroll
         for (int nt = 0; nt < 2; nt++) {
-          float acc[MT][2][4] = {};
+          float acc[2][4] = {};
           const int key = 16 * warp + 8 * nt + (lane & 7);
 #pragma unroll
           for (int q = 0; q < 4; q++) {   // 32 channels each
             uint32_t b[4];
             ldmatrix4(b, kt + (q >> 1) * (FEW_STAGE / 4) + key * 128 + ((((q & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4));
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-              for (int e = 0; e < 2; e++)
-                mma16816(acc[mt][e], qa[mt][2 * q + e][0], PAIR ? 0u : qa[mt][2 * q + e][RPT - 1], qa[mt][2 * q + e][RPT], PAIR ? 0u : qa[mt][2 * q + e][2 * RPT - 1], b[2 * e], b[2 * e + 1]);
+            for (int e = 0; e < 2; e++)
+              mma16816(acc[e], qa[2 * q + e][0], PAIR ? 0u : qa[2 * q + e][RPT - 1], qa[2 * q + e][RPT], PAIR ? 0u : qa[2 * q + e][2 * RPT - 1], b[2 * e], b[2 * e + 1]);
           }
 #pragma unroll
-          for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) sc[mt][nt][i] = acc[mt][0][i] + acc[mt][1][i];
+          for (int i = 0; i < 4; i++) sc[nt][i] = acc[0][i] + acc[1][i];
         }
-        uint32_t pa[MT][4];
+        uint32_t pa[4];
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
+        for (int e = 0; e < RPT; e++) {
+          const uint32_t bits = draft ? s_mask[min((8 * e + g) / p.a.G, p.a.T - 1)] : live >= 16 ? ~0u : ((1u << live) - 1) << (16 * (warp & 1));
+          float x[4], mx = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < RPT; e++) {
-            const uint32_t bits = draft ? s_mask[min((16 * mt + 8 * e + g) / p.a.G, p.a.T - 1)] : live >= 16 ? ~0u : ((1u << live) - 1) << (16 * (warp & 1));
-            float x[4], mx = -INFINITY;
+          for (int i = 0; i < 4; i++) {   // n-tile i / 2, column 2 t4 + i % 2
+            const int key = 16 * (warp & 1) + 8 * (i >> 1) + 2 * t4 + (i & 1);
+            x[i] = bits >> key & 1 && (!draft || warp < 2) ? sc[i >> 1][2 * e + (i & 1)] : -INFINITY;
+            mx = fmaxf(mx, x[i]);
+          }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float m_new = fmaxf(m[e], mx), least = m_new == -INFINITY ? 0.0f : m_new;
+          const float f = m_new > m[e] ? ex2((m[e] - m_new) * scale) : 1.0f;
+          float y[4], sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {   // n-tile i / 2, column 2 t4 + i % 2
-              const int key = 16 * (warp & 1) + 8 * (i >> 1) + 2 * t4 + (i & 1);
-              x[i] = bits >> key & 1 && (!draft || warp < 2) ? sc[mt][i >> 1][2 * e + (i & 1)] : -INFINITY;
-              mx = fmaxf(mx, x[i]);
+          for (int i = 0; i < 4; i++) y[i] = ex2((x[i] - least) * scale), sum += y[i];
+          l[e] = l[e] * f + sum, m[e] = m_new;
+          if (__any_sync(0xffffffffu, f != 1.0f)) {
+#pragma unroll
+            for (int n = 0; n < 16; n++) {
+              o[n][2 * e] *= f, o[n][2 * e + 1] *= f;
+              if (PAIR) o[n][2] *= f, o[n][3] *= f;
             }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float m_new = fmaxf(m[mt][e], mx), least = m_new == -INFINITY ? 0.0f : m_new;
-            const float f = m_new > m[mt][e] ? ex2((m[mt][e] - m_new) * scale) : 1.0f;
-            float y[4], sum = 0.0f;
+          }
 #pragma unroll
-            for (int i = 0; i < 4; i++) y[i] = ex2((x[i] - least) * scale), sum += y[i];
-            l[mt][e] = l[mt][e] * f + sum, m[mt][e] = m_new;
-            if (__any_sync(0xffffffffu, f != 1.0f)) {
-#pragma unroll
-              for (int n = 0; n < 16; n++) {
-                o[mt][n][2 * e] *= f, o[mt][n][2 * e + 1] *= f;
-                if (PAIR) o[mt][n][2] *= f, o[mt][n][3] *= f;
-              }
-            }
-#pragma unroll
-            for (int nt = 0; nt < 2; nt++) {
-              const uint32_t hi = pack2(y[2 * nt], y[2 * nt + 1]);
-              pa[mt][2 * nt + e] = hi;
-              if (PAIR) pa[mt][2 * nt + 1] = pack2(y[2 * nt] - __uint_as_float(hi << 16), y[2 * nt + 1] - __uint_as_float(hi & 0xffff0000u));
-            }
+          for (int nt = 0; nt < 2; nt++) {
+            const uint32_t hi = pack2(y[2 * nt], y[2 * nt + 1]);
+            pa[2 * nt + e] = hi;
+            if (PAIR) pa[2 * nt + 1] = pack2(y[2 * nt] - __uint_as_float(hi << 16), y[2 * nt + 1] - __uint_as_float(hi & 0xffff0000u));
           }
         }
         const int vkey = 16 * warp + (lane >> 3 & 1) * 8 + (lane & 7);
@@ -361,11 +347,8 @@ __global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
         for (int np = 0; np < 8; np++) {
           uint32_t b[4];
           ldmatrix4t(b, vt + (np >> 2) * (FEW_STAGE / 4) + vkey * 128 + ((((np & 3) * 2 + (lane >> 4)) ^ (lane & 7)) << 4));
-#pragma unroll
-          for (int mt = 0; mt < MT; mt++) {
-            mma16816(o[mt][2 * np], pa[mt][0], pa[mt][1], pa[mt][2], pa[mt][3], b[0], b[1]);
-            mma16816(o[mt][2 * np + 1], pa[mt][0], pa[mt][1], pa[mt][2], pa[mt][3], b[2], b[3]);
-          }
+          mma16816(o[2 * np], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
+          mma16816(o[2 * np + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
         }
       }
       __syncwarp();
@@ -374,29 +357,27 @@ __global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
     // ---- the four warps' shares of the segment ----
     float* s_o = reinterpret_cast<float*>(dyn + (base - smem_addr(dyn)) + (k - 1) % FEW_BUFS * FEW_STAGE);   // [4][8][FEW_OS]
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-      for (int e = 0; e < RPT; e++) {
-        l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 1);
-        l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 2);
-        if (t4 == 0) s_m[warp][16 * mt + 8 * e + g] = m[mt][e] * scale, s_l[warp][16 * mt + 8 * e + g] = l[mt][e];
-      }
+    for (int e = 0; e < RPT; e++) {
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+      if (t4 == 0) s_m[warp][8 * e + g] = m[e] * scale, s_l[warp][8 * e + g] = l[e];
+    }
     named_barrier(1, 128);
     const uint32_t bad = has_drafts ? s_bad : 0;
-    float* rec = whole ? nullptr : p.records + (2 * (int64_t)blockIdx.x + (seg_first == 0)) * (OUT_ROWS * 130);
+    float* rec = whole ? nullptr : p.records + (2 * (int64_t)blockIdx.x + (seg_first == 0)) * (ROWS * 130);
 #pragma unroll
-    for (int round = 0; round < OUT_ROWS / 8; round++) {
+    for (int round = 0; round < ROWS / 8; round++) {
       if (8 * round < n_rows) {
         const int r = 8 * round + g;
         const float M = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
         const float f = s_m[warp][r] == -INFINITY ? 0.0f : ex2(s_m[warp][r] - M);
-        const int mt = round / 2, e = PAIR ? 0 : round & 1;
+        const int e = PAIR ? 0 : round;
         float* to = s_o + (warp * 8 + g) * FEW_OS + 2 * t4;
 #pragma unroll
         for (int n = 0; n < 16; n++) {
-          float2 v = make_float2(o[mt][n][2 * e], o[mt][n][2 * e + 1]);
+          float2 v = make_float2(o[n][2 * e], o[n][2 * e + 1]);
           // an infinite value times what a rounding left is an infinity of any sign, or NaN where nothing was left: the other half has it
-          if (PAIR) v.x += finite(o[mt][n][2]) ? o[mt][n][2] : 0.0f, v.y += finite(o[mt][n][3]) ? o[mt][n][3] : 0.0f;
+          if (PAIR) v.x += finite(o[n][2]) ? o[n][2] : 0.0f, v.y += finite(o[n][3]) ? o[n][3] : 0.0f;
           *reinterpret_cast<float2*>(to + 8 * n) = make_float2(v.x * f, v.y * f);
         }
         named_barrier(1, 128);
@@ -424,7 +405,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_ctas(ROWS))
               if (p.a.lse && tid == 0) p.a.lse[out_row] = L == 0.0f ? -INFINITY : Mi + log2f(L);
             } else {
               rec[row * 128 + tid] = O;
-              if (tid == 0) rec[OUT_ROWS * 128 + row] = Mi, rec[OUT_ROWS * 129 + row] = L;
+              if (tid == 0) rec[ROWS * 128 + row] = Mi, rec[ROWS * 129 + row] = L;
             }
           }
         }
@@ -472,7 +453,7 @@ __global__ void __launch_bounds__(128) few_merge_kernel(const __grid_constant__ 
 
 template <bool TREE, int ROWS>
 int launch(const FewParams& p, const CUtensorMap (&maps)[4], int64_t most, const char* what, cudaStream_t st) {
-  const int64_t slots = (int64_t)few_ctas(ROWS) * sm_count();
+  const int64_t slots = (int64_t)FEW_CTAS * sm_count();
   const int blocks = (int)(most < slots ? most : slots);
   static PerDevice opted;
   if (const unsigned long long bit = first_on_device(opted)) {
@@ -489,13 +470,13 @@ int launch(const FewParams& p, const CUtensorMap (&maps)[4], int64_t most, const
 
 }  // namespace
 
-int64_t attend_few_workspace() { return 4 * (int64_t)sm_count() * 32 * 130 * 4; }
+int64_t attend_few_workspace() { return 2 * (int64_t)FEW_CTAS * sm_count() * 16 * 130 * 4; }
 
 int launch_attend_few(const AttendParams& a, int64_t bs, void* workspace, const char* what, cudaStream_t st) {
   const bool tree = a.blocks == nullptr;
   FewParams p = {};
   p.a = a, p.bs = (int)bs, p.records = (float*)workspace;
-  const int rows = tree ? a.T * a.G : a.G, per = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+  const int rows = tree ? a.T * a.G : a.G, per = rows <= 8 ? 8 : 16;
   p.row_groups = tree ? 1 : (a.G + per - 1) / per;
   p.box = tree ? FEW_TILE : a.block < FEW_TILE ? a.block : FEW_TILE;
   p.tiles = tree ? 0 : (int)(((int64_t)a.n * a.block + FEW_TILE - 1) / FEW_TILE);
@@ -506,7 +487,7 @@ int launch_attend_few(const AttendParams& a, int64_t bs, void* workspace, const 
   if (!ok) return launch_attend_rows(a, bs, what, st);
   const int64_t most = tree ? bs * a.H * ((a.cap + FEW_TILE - 1) / FEW_TILE + 1) : bs * a.T * a.H * p.row_groups * (int64_t)p.tiles;
   if (tree) return per == 8 ? launch<true, 8>(p, maps, most, what, st) : launch<true, 16>(p, maps, most, what, st);
-  return per == 8 ? launch<false, 8>(p, maps, most, what, st) : per == 16 ? launch<false, 16>(p, maps, most, what, st) : launch<false, 32>(p, maps, most, what, st);
+  return per == 8 ? launch<false, 8>(p, maps, most, what, st) : launch<false, 16>(p, maps, most, what, st);
 }
 
 }  // namespace pk
