@@ -462,6 +462,7 @@ extern "C" int pk_block_bounds(const pk_tensor* keys, const pk_tensor* lengths, 
   PK_REQUIRE(block_size_ok(block), "block must be 16, 32, 64 or 128");
   PK_REQUIRE(keys->shape[3] == 128 && cap < (1LL << 31) && row_tensor(keys), "keys must be bf16 [bs,H,cap,128] with a unit inner stride, other strides that are multiples of 8, and 16-byte alignment");
   PK_REQUIRE(bounds->shape[0] == bs && bounds->shape[1] == H && bounds->shape[2] == (cap + block - 1) / block, "bounds must be bf16 [bs,H,ceil(cap/block),2,128]");
+  for (int i = 0; i < 3; i++) PK_REQUIRE(bounds->shape[i] <= 1 || bounds->stride[i] > 0, "bounds are written: heads or blocks of them must not share memory");
   PK_REQUIRE(n_new >= -1 && n_new < (1LL << 31), "n_new must be a number of rows, or -1 for all blocks");
   BoundsParams p = {};
   if (lengths) {

@@ -521,7 +521,7 @@ def block_bounds(keys, lengths=None, block=64, n_new=None, bounds=None):
     """Smallest and largest value per channel of every block of `block` keys: keys bf16 [bs,H,cap,128], the first lengths[b] rows
     (i32 [bs]; None: all) -> bf16 [bs,H,ceil(cap/block),2,128].  With n_new only the blocks of the last n_new rows are made
     again, in the `bounds` given: what a step that appends rows (or takes drafts back and appends others) calls.  Blocks
-    without rows are left as they are.  See pk_block_bounds."""
+    without rows are left as they are (in a new tensor: not initialised).  See pk_block_bounds."""
     if n_new is not None and n_new < 0:
         raise ValueError("n_new must not be negative")
     if n_new is not None and bounds is None:
