@@ -534,7 +534,9 @@ int pk_gemv(const pk_tensor* weight, const pk_tensor* x, const pk_tensor* out, i
  * multiples of 8 elements, 16-byte aligned.  A query that sees no row gets zeros, and lse = -inf.  What a query does not see
  * does not reach it, whatever is stored there (NaN and infinities included).  lse (f32 [bs,T,Hq] or NULL) is the log2 of the
  * softmax denominator, as in pk_sparse_attention; scale has to be positive, and scale * log2 e finite in 32 bits.  workspace: device, 256-byte aligned, pk_*_workspace_bytes; nothing in it
- * has to be cleared and nothing carries over between calls.  No counterpart in the reference.
+ * has to be cleared and nothing carries over between calls.  The weights of a KV head with more than eight query rows (T * Hq / H of a tree, Hq / H of
+ * listed blocks) are rounded to bf16 before they meet the values, up to eight rows have 17 bits; scores, maxima and sums have 32.  A cache with a stride of
+ * zero goes by a kernel that reads it once per query row.  No counterpart in the reference.
  *
  * pk_tree_attention: T drafted tokens per sequence (at most 256) attend to rows [0, lengths[b]) of the cache and to the drafts that
  *   tree_mask[b][t] names.  queries bf16 [bs,T,Hq,128], query head h*G+g belonging to KV head h; keys / values bf16

@@ -107,10 +107,11 @@ __device__ __forceinline__ void query_sums(const SelectParams& p, int64_t b, int
 // numbers by fewer digits: A is zero only where every product is.
 // A warp of its own brings 32 blocks of keys at a time, 16 KB, into a ring of four stages; each of four warps takes eight of them for TT tokens: lanes
 // 0 .. 15 hold eight channels of lo and N each, the others of hi and P.  Bounded by the bounds' bytes where there are many, otherwise by
-// latency.  With the choice, us, by loads to registers two groups ahead | by the ring: 8192 blocks of 8 heads for four tokens 29 | 28, for one 21 | 18,
-// 512 blocks 8.3 | 7.7.  Copies of one block each, which bounds with gaps need, cost more the more of them there are: 128 heads x 400 blocks
-// 14.5, in copies of 512 bytes 16.5.  (64-bit sums throughout: four tokens 46 us for the scores alone; the conversions to 64 bits, 8 a
-// clock and SM, take longer than the bytes.)
+// latency.  With the choice, us a call in a replayed graph, bounds in HBM (in L2): 8192 blocks of 8 heads for four tokens 23.0 (21.0), for one 16.3 (14.2),
+// 512 blocks 5.9 (5.9), 128 heads x 400 blocks 11.5 (10.0).  Call after call, which adds the launches: by loads to registers two groups
+// ahead | by the ring 29 | 28, 21 | 18, 8.3 | 7.7;  copies of one block each, which bounds with gaps need, cost more the more of them there are: 128 heads x 400
+// blocks 14.5, in copies of 512 bytes 16.5.  (64-bit sums throughout: four tokens 46 us for the scores alone; the conversions to 64 bits, 8
+// a clock and SM, take longer than the bytes.)
 constexpr int SCORE_BLOCKS = 32, SCORE_STAGE = 512 * SCORE_BLOCKS, SCORE_STAGES = 4, SCORE_THREADS = 160, SCORE_CTAS = 3;   // blocks per SM, by the registers
 constexpr int SCORE_WAIT_LIMIT = 100000;   // tries; one waits up to 10 us by itself
 template <int TT>

@@ -51,3 +51,25 @@ def test_an_infinite_value_in_a_listed_block_comes_out(G, n):
     out = ops.block_attention(q, keys, values, ids, i32([6000]), block=16)
     want, tol, _, _ = R.block_attention(q, keys, values, ids, [6000], 16)
     _infinite_channels(out, want, tol, {5: 1, 9: -1})
+
+
+def test_results_over_two_sets_of_rows_are_joined_by_lse():
+    """A cache in two parts, the drafts with the second; one part is empty for one sample."""
+    from pariskv_b200 import dist, ops
+    r = rnd(1)
+    bs, T, H, G, n = 2, 5, 2, 4, 700
+    keys, values, q, dk, dv = r(bs, H, n, 128), r(bs, H, n, 128), r(bs, T, H * G, 128), r(bs, T, H, 128), r(bs, T, H, 128)
+    mask = torch.ones(1, T, T, dtype=torch.bool, device=DEV).tril()
+    cut = [300, 0]
+    first, second = i32(cut), i32([n - 300, n])
+    tail_k, tail_v = keys.clone(), values.clone()
+    tail_k[0, :, :n - 300], tail_v[0, :, :n - 300] = keys[0, :, 300:], values[0, :, 300:]
+    parts = []
+    for k, v, m, lengths in ((keys, values, torch.zeros_like(mask), first), (tail_k, tail_v, mask, second)):
+        lse = torch.empty(bs, T, H * G, device=DEV)
+        parts.append((ops.tree_attention(q, k, v, dk, dv, m, lengths, lse=lse), lse))
+    packed = torch.stack([torch.cat((o.float().flatten(0, 1), lse.flatten(0, 1)[..., None]), -1) for o, lse in parts])
+    out = dist.merge_gathered_partials(packed).view(bs, T, H * G, 128)
+    want, tol, _, _ = R.tree(q, keys, values, dk, dv, mask, [n, n])
+    # each part has been rounded to bf16 once
+    R.close(out, want, 2 * tol + R.U * sum(o.double().abs() for o, _ in parts))
