@@ -26,7 +26,7 @@ extern "C" {
 
 #define PK_MAX_DIMS 6
 
-enum pk_dtype { PK_U8 = 0, PK_I32 = 1, PK_I64 = 2, PK_F32 = 3, PK_BF16 = 4 };
+enum pk_dtype { PK_U8 = 0, PK_I32 = 1, PK_I64 = 2, PK_F32 = 3, PK_BF16 = 4, PK_I8 = 5, PK_E4M3 = 6 };
 
 enum pk_status {
   PK_OK = 0,
@@ -580,6 +580,48 @@ int pk_block_attention(const pk_tensor* queries, const pk_tensor* keys, const pk
 int64_t pk_gemv_w4_workspace_bytes(int64_t T, int64_t O, int64_t I, int64_t group, int gated);   /* 0: none */
 int pk_gemv_w4(const pk_tensor* weight, const pk_tensor* scales, const pk_tensor* offsets, const pk_tensor* x,
                const pk_tensor* out, int gated, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- a step in 8 bits: the cache and what reads it, the products and what feeds them ---------------------- */
+
+/* A cache in 8 bits.  codes i8 or e4m3 [bs,H,cap,2,128] (K and V of a row); scales f32 [bs,H,ceil(cap/block),2]: a value is code * scale; recent bf16
+ * [bs,H,R,2,128]: row r of a sequence at place r % R, R a multiple of block.  Block j is the rows j*block .. of one sequence and head, 16, 32, 64 or 128 of them.
+ * As soon as a sequence is (j + 1) * block rows long the rows of block j are those of the codes; the rows behind its last whole block are those of `recent`, in 16
+ * bits.  A block is coded once, from its rows in 16 bits, so that what a cache holds does not depend on how the rows were cut into calls:
+ *   amax = largest magnitude of the block's rows (K and V each for itself), scale = amax / 127 (e4m3: 448), code = x 127 / amax, to the nearest, ties to the even one
+ * as exact arithmetic has them.  A block of zeros has scale zero; one that holds an infinity or NaN has scale NaN and codes of zero: all of it reads as NaN.
+ * codes with a unit inner stride, the other strides multiples of 16; scales with any; recent as queries; 16-byte aligned.  Every operator is one call for all
+ * sequences; lengths i32 [bs] (device) holds their rows, as in the other operators for several tokens; a cache ends below 2^31 - 256 rows.
+ * Rows taken back (a smaller length) are as if they had never been, as long as what is left of a block that is no longer whole is still in `recent`: up to
+ * R - block rows may be taken back.
+ *
+ * pk_cache8_append: the last counts[b] (i32 [bs], or NULL: T) of lengths[b] rows are keys / values [b][0 ..], bf16 [bs,T,H,128].  Rows at positions below zero or from cap on are
+ *   left out.  codes, scales and recent must not overlap themselves.
+ * pk_cache8_read: out bf16 [bs,H,n,2,128] = row i, or row rows[b][h][i] (i64 [bs,H,n]), rounded to bf16.  Without rows, out's rows from the length on are left as they are (n <= cap);
+ *   with rows, an entry that is no row of the sequence gives zeros.
+ * pk_cache8_attention: token t of T (at most 256) is at position lengths[b] - T + t and sees the rows up to its own: queries, out, lse and scale as in pk_block_attention.  Scores, maxima and
+ *   sums have 32 bits; queries and codes meet exactly, the weights times the values' scales meet the codes as 11 bits (fp16).  An e4m3 code of NaN (which the append never writes)
+ *   counts as 480.
+ *
+ * pk_add_rmsnorm_i8: h_out = bf16(a + residual) (residual may be NULL), y = h_out * rstd(h_out) * weight in 32 bits, scales[b] = max |y| / 127, codes[b] = y / scale to the nearest;
+ *   a, residual, h_out bf16 [B,n], weight bf16 [n], codes i8 [B,n], scales f32 [B]; n a multiple of 8, at most 65536; the mean square is summed in 64 bits.  A token with an infinity or NaN has
+ *   scale NaN and codes of zero.  h_out may be a or residual.
+ * pk_quantize_rows_i8: the same codes and scales of x bf16 [B,n] itself; gated: of silu(x[:, :n]) * x[:, n:] in 32 bits, x bf16 [B,2n].
+ * pk_matmul_i8: out[T,O] = bf16( (sum over k of x[t,k] weight[o,k]) * x_scales[t] * weight_scales[o] ): i8 [T,I], i8 [O,I], f32 [T], f32 [O] -> bf16 [T,O], whole-number sums without
+ *   rounding; any T; I a multiple of 16, at most 65536; rows at strides that are multiples of 16. */
+typedef struct pk_cache8 {
+  const pk_tensor* codes;
+  const pk_tensor* scales;
+  const pk_tensor* recent;
+  int64_t block;
+} pk_cache8;
+int pk_cache8_append(const pk_cache8* cache, const pk_tensor* keys, const pk_tensor* values, const pk_tensor* lengths, const pk_tensor* counts, void* stream);
+int pk_cache8_read(const pk_cache8* cache, const pk_tensor* lengths, const pk_tensor* rows, const pk_tensor* out, void* stream);
+int64_t pk_cache8_attention_workspace_bytes(int64_t bs, int64_t T, int64_t Hq, int64_t H, int64_t cap);
+int pk_cache8_attention(const pk_tensor* queries, const pk_cache8* cache, const pk_tensor* lengths, float scale, const pk_tensor* out, const pk_tensor* lse, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+int pk_add_rmsnorm_i8(const pk_tensor* a, const pk_tensor* residual, const pk_tensor* weight, const pk_tensor* h_out, const pk_tensor* codes, const pk_tensor* scales, double eps, void* stream);
+int pk_quantize_rows_i8(const pk_tensor* x, int gated, const pk_tensor* codes, const pk_tensor* scales, void* stream);
+int pk_matmul_i8(const pk_tensor* x, const pk_tensor* x_scales, const pk_tensor* weight, const pk_tensor* weight_scales, const pk_tensor* out, void* stream);
 
 #ifdef __cplusplus
 }

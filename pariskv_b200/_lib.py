@@ -13,9 +13,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libpariskv_b200.so")
 
 PK_MAX_DIMS = 6
-PK_U8, PK_I32, PK_I64, PK_F32, PK_BF16 = range(5)
+PK_U8, PK_I32, PK_I64, PK_F32, PK_BF16, PK_I8, PK_E4M3 = range(7)
 _DTYPES = {torch.uint8: PK_U8, torch.int32: PK_I32, torch.int64: PK_I64, torch.float32: PK_F32,
-           torch.bfloat16: PK_BF16}
+           torch.bfloat16: PK_BF16, torch.int8: PK_I8, torch.float8_e4m3fn: PK_E4M3}
 
 
 class PkTensor(ctypes.Structure):
@@ -30,6 +30,13 @@ class PkZoneSchedule(ctypes.Structure):
 
 
 TP = ctypes.POINTER(PkTensor)
+
+
+class PkCache8(ctypes.Structure):
+    _fields_ = [("codes", TP), ("scales", TP), ("recent", TP), ("block", ctypes.c_int64)]
+
+
+C8P = ctypes.POINTER(PkCache8)
 
 
 class PkRetrieveArgs(ctypes.Structure):
@@ -111,6 +118,13 @@ SIGNATURES = {
     "pk_block_attention": (_INT, [TP] * 5 + [_I64, _F32, TP, TP, _VP, _I64, _VP]),
     "pk_gemv_w4_workspace_bytes": (_I64, [_I64] * 4 + [_INT]),
     "pk_gemv_w4": (_INT, [TP] * 5 + [_INT, _VP, _I64, _VP]),
+    "pk_cache8_append": (_INT, [C8P, TP, TP, TP, TP, _VP]),
+    "pk_cache8_read": (_INT, [C8P, TP, TP, TP, _VP]),
+    "pk_cache8_attention_workspace_bytes": (_I64, [_I64] * 5),
+    "pk_cache8_attention": (_INT, [TP, C8P, TP, _F32, TP, TP, _VP, _I64, _VP]),
+    "pk_add_rmsnorm_i8": (_INT, [TP] * 6 + [ctypes.c_double, _VP]),
+    "pk_quantize_rows_i8": (_INT, [TP, _INT, TP, TP, _VP]),
+    "pk_matmul_i8": (_INT, [TP] * 5 + [_VP]),
 }
 
 _lib = None

@@ -1,0 +1,209 @@
+// Rows into the cache in 8 bits and back.
+//   append  scale = max |x| / 127, code = x / scale to the nearest, over the rows of a block (K and V each for itself), once all of them are there
+//   read    code * scale, rounded to bf16
+// Both move each byte once; HBM bounds them where there are many rows, two dependent loads where there are few.
+#include "cache8.cuh"
+
+namespace pk {
+namespace {
+
+// A thread block per block of rows, a warp per row of K and V: 8 values a lane.  The values of a block that is now whole stay in registers between the
+// maximum and the codes.
+template <int BLOCK, bool E4M3>
+__global__ void __launch_bounds__(256)
+    cache8_append_kernel(const __grid_constant__ Cache8 c, const uint16_t* k, const uint16_t* v, int64_t k_b, int64_t k_t, int64_t k_h, int64_t v_b, int64_t v_t, int64_t v_h,
+                         const int32_t* lengths, const int32_t* counts, int T) {
+  constexpr int N = BLOCK / 8;   // rows of a warp
+  __shared__ uint32_t s_max[8][2];
+  pdl_wait();
+  pdl_trigger();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kv = lane >> 4, ch = (lane & 15) * 8;
+  const int64_t b = blockIdx.z, h = blockIdx.y;
+  const int n = counts ? min(max(counts[b], 0), T) : T;
+  const int64_t len = lengths[b], start = len - n, first = start > 0 ? start : 0, end = len < c.cap ? len : c.cap;
+  if (first >= end || n == 0) return;
+  const int64_t j0 = first >> c.shift, j = j0 + blockIdx.x, row0 = j << c.shift;
+  if (row0 >= end) return;
+  const uint16_t* from = kv ? v + b * v_b + h * v_h + ch : k + b * k_b + h * k_h + ch;
+  const int64_t from_t = kv ? v_t : k_t;
+  uint16_t* ring = c.recent + b * c.r_b + h * c.r_h + kv * c.r_kv + ch;
+  auto place = [&](int64_t r) { return ring + (r % c.R) * c.r_l; };
+  if (row0 + BLOCK <= end) {
+    uint4 x[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int64_t r = row0 + 8 * i + warp;
+      x[i] = *reinterpret_cast<const uint4*>(r >= first ? from + (r - start) * from_t : place(r));
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      m = __vmaxu2(m, x[i].x & 0x7fff7fffu);
+      m = __vmaxu2(m, x[i].y & 0x7fff7fffu);
+      m = __vmaxu2(m, x[i].z & 0x7fff7fffu);
+      m = __vmaxu2(m, x[i].w & 0x7fff7fffu);
+    }
+    m = max(m & 0xffffu, m >> 16);
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
+    if ((lane & 15) == 0) s_max[warp][kv] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = max(m, s_max[i][kv]);
+    const float amax = bf2f((uint16_t)m);
+    const bool fine = m < 0x7f80u;
+    const float unit = m == 0 ? 1.0f : __fmul_rn(amax, E4M3 ? 0.001953125f : 0.0078125f);
+    uint8_t* to = c.codes + b * c.c_b + h * c.c_h + kv * c.c_kv + ch;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      float q[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float f = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+        q[e] = E4M3 ? e4m3_quotient(f, unit) : i8_quotient(f, unit);
+      }
+      uint2 o;
+      if (E4M3) o = make_uint2(pack_e4m3(q[0], q[1], q[2], q[3]), pack_e4m3(q[4], q[5], q[6], q[7]));
+      else o = make_uint2(pack_i8(q[0], q[1], q[2], q[3]), pack_i8(q[4], q[5], q[6], q[7]));
+      if (!fine) o = make_uint2(0, 0);
+      *reinterpret_cast<uint2*>(to + (row0 + 8 * i + warp) * c.c_l) = o;
+    }
+    if (warp == 0 && (lane & 15) == 0) c.scales[b * c.s_b + h * c.s_h + j * c.s_j + kv * c.s_kv] = fine ? __fdiv_rn(amax, E4M3 ? 448.0f : 127.0f) : NAN;
+  }
+  // The last R rows stay in 16 bits.  Rows of the first block that were there before may lie where new ones go: the thread block that reads them also
+  // writes what replaces them.
+  const int blocks = c.R >> c.shift;
+  const bool old = first > j0 << c.shift;
+  const int64_t kept = max(first, end - c.R);   // the first new row that is kept
+  auto keep = [&](int64_t jj) {
+    for (int64_t r = max(jj << c.shift, kept) + warp; r < min((jj + 1) << c.shift, end); r += 8)
+      *reinterpret_cast<uint4*>(place(r)) = *reinterpret_cast<const uint4*>(from + (r - start) * from_t);
+  };
+  if (!old) return keep(j);
+  if (j == j0) {
+    __syncthreads();
+    int64_t jj = j0;
+    if ((kept >> c.shift) > j0) jj += ((kept >> c.shift) - j0 + blocks - 1) / blocks * blocks;
+    for (; jj << c.shift < end; jj += blocks) keep(jj);
+  } else if ((j - j0) % blocks != 0) {
+    keep(j);
+  }
+}
+
+// A warp per row, eight rows in flight.
+template <bool E4M3, bool LISTED>
+__global__ void __launch_bounds__(256) cache8_read_kernel(const __grid_constant__ Cache8 c, const int32_t* lengths, const int64_t* rows, uint16_t* out, int64_t o_b, int64_t o_h, int64_t o_l,
+                                                          int64_t o_kv, int64_t n) {
+  constexpr int N = 8;
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kv = lane >> 4, ch = (lane & 15) * 8;
+  const int64_t b = blockIdx.z, h = blockIdx.y, i0 = ((int64_t)blockIdx.x * 8 + warp) * N;
+  const int64_t len = min((int64_t)max(lengths[b], 0), c.cap), whole = len >> c.shift << c.shift;
+  if (i0 >= (LISTED ? n : min(n, len))) return;
+  const uint8_t* codes = c.codes + b * c.c_b + h * c.c_h + kv * c.c_kv + ch;
+  const float* scales = c.scales + b * c.s_b + h * c.s_h + kv * c.s_kv;
+  const uint16_t* ring = c.recent + b * c.r_b + h * c.r_h + kv * c.r_kv + ch;
+  uint16_t* to = out + b * o_b + h * o_h + kv * o_kv + ch;
+  int64_t r[N];
+  uint2 x[N];
+  float s[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) r[i] = LISTED ? (i0 + i < n ? rows[(b * c.H + h) * n + i0 + i] : -1) : i0 + i;
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const bool ok = r[i] >= 0 && r[i] < whole;
+    x[i] = ok ? *reinterpret_cast<const uint2*>(codes + r[i] * c.c_l) : make_uint2(0, 0);
+    s[i] = ok ? scales[(r[i] >> c.shift) * c.s_j] : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    uint4 o = make_uint4(0, 0, 0, 0);
+    if (r[i] >= whole && r[i] < len) {
+      o = *reinterpret_cast<const uint4*>(ring + (r[i] % c.R) * c.r_l);
+    } else if (r[i] >= 0 && r[i] < whole) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const uint32_t four = e < 2 ? x[i].x : x[i].y;
+        float2 f;
+        if (E4M3) f = e4m3_floats(four >> (16 * (e & 1)) & 0xffffu);
+        else f = make_float2(i8_float(four ^ 0x80808080u, 2 * (e & 1)), i8_float(four ^ 0x80808080u, 2 * (e & 1) + 1));
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[e]) : "f"(__fmul_rn(f.y, s[i])), "f"(__fmul_rn(f.x, s[i])));
+      }
+      o = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (LISTED ? i0 + i < n : r[i] < min(n, len)) *reinterpret_cast<uint4*>(to + (i0 + i) * o_l) = o;
+  }
+}
+
+int lengths_ok(const pk_tensor* lengths, int64_t bs) {
+  PK_CHECK_TENSOR(lengths, PK_I32, 1);
+  PK_REQUIRE(lengths->shape[0] == bs && is_contig(lengths), "lengths must be contiguous i32 [bs]");
+  return PK_OK;
+}
+
+}  // namespace
+}  // namespace pk
+
+using namespace pk;
+
+extern "C" int pk_cache8_append(const pk_cache8* cache, const pk_tensor* keys, const pk_tensor* values, const pk_tensor* lengths, const pk_tensor* counts, void* stream) {
+  Cache8 c = {};
+  if (const int rc = fill_cache8(&c, cache, true)) return rc;
+  const int64_t bs = cache->codes->shape[0];
+  PK_CHECK_TENSOR(keys, PK_BF16, 4);
+  PK_CHECK_TENSOR(values, PK_BF16, 4);
+  PK_REQUIRE(keys->shape[0] == bs && keys->shape[2] == c.H && keys->shape[3] == 128 && keys->shape[1] < (1LL << 31) - 256, "keys must be bf16 [bs,T,H,128]");
+  for (int i = 0; i < 4; i++) PK_REQUIRE(values->shape[i] == keys->shape[i], "values must have the shape of keys");
+  PK_REQUIRE(row_tensor(keys) && row_tensor(values), "keys and values need a unit inner stride, other strides that are multiples of 8, and 16-byte alignment");
+  if (const int rc = lengths_ok(lengths, bs)) return rc;
+  if (counts) {
+    PK_CHECK_TENSOR(counts, PK_I32, 1);
+    PK_REQUIRE(counts->shape[0] == bs && is_contig(counts), "counts must be contiguous i32 [bs]");
+  }
+  const int T = (int)keys->shape[1], block = 1 << c.shift;
+  if (bs == 0 || T == 0 || c.cap == 0) return PK_OK;
+  const int64_t touched = (T + block - 2) / block + 1;
+  const dim3 grid((unsigned)touched, (unsigned)c.H, (unsigned)bs);
+  const cudaStream_t st = (cudaStream_t)stream;
+  StageTimer timer(ST_APPEND, st);
+  const bool e4m3 = cache->codes->dtype == PK_E4M3;
+#define PK_LAUNCH(B, E)                                                                                                                                                     \
+  launch_chain(cache8_append_kernel<B, E>, grid, dim3(256), 0, st, c, (const uint16_t*)keys->data, (const uint16_t*)values->data, keys->stride[0], keys->stride[1], keys->stride[2], \
+               values->stride[0], values->stride[1], values->stride[2], (const int32_t*)lengths->data, (const int32_t*)(counts ? counts->data : nullptr), T)
+#define PK_BLOCK(B) e4m3 ? PK_LAUNCH(B, true) : PK_LAUNCH(B, false)
+  block == 16 ? (PK_BLOCK(16)) : block == 32 ? (PK_BLOCK(32)) : block == 64 ? (PK_BLOCK(64)) : (PK_BLOCK(128));
+#undef PK_BLOCK
+#undef PK_LAUNCH
+  return check_launch("cache8_append");
+}
+
+extern "C" int pk_cache8_read(const pk_cache8* cache, const pk_tensor* lengths, const pk_tensor* rows, const pk_tensor* out, void* stream) {
+  Cache8 c = {};
+  if (const int rc = fill_cache8(&c, cache, false)) return rc;
+  const int64_t bs = cache->codes->shape[0];
+  if (const int rc = lengths_ok(lengths, bs)) return rc;
+  PK_CHECK_TENSOR(out, PK_BF16, 5);
+  const int64_t n = out->shape[2];
+  PK_REQUIRE(out->shape[0] == bs && out->shape[1] == c.H && out->shape[3] == 2 && out->shape[4] == 128 && n < (1LL << 31) - 256, "out must be bf16 [bs,H,n,2,128]");
+  PK_REQUIRE(row_tensor(out) && apart(out), "out needs a unit inner stride, other strides that are multiples of 8, 16-byte alignment, and must not share memory within itself");
+  if (rows) {
+    PK_CHECK_TENSOR(rows, PK_I64, 3);
+    PK_REQUIRE(rows->shape[0] == bs && rows->shape[1] == c.H && rows->shape[2] == n && is_contig(rows), "rows must be contiguous i64 [bs,H,n], n as in out");
+  } else {
+    PK_REQUIRE(n <= c.cap, "out has more rows than the cache");
+  }
+  if (bs == 0 || n == 0) return PK_OK;
+  const dim3 grid((unsigned)((n + 63) / 64), (unsigned)c.H, (unsigned)bs);
+  const cudaStream_t st = (cudaStream_t)stream;
+  StageTimer timer(ST_GATHER, st);
+#define PK_LAUNCH(E, L)                                                                                                                                                           \
+  launch_chain(cache8_read_kernel<E, L>, grid, dim3(256), 0, st, c, (const int32_t*)lengths->data, (const int64_t*)(rows ? rows->data : nullptr), (uint16_t*)out->data, out->stride[0], \
+               out->stride[1], out->stride[2], out->stride[3], n)
+  if (cache->codes->dtype == PK_E4M3) rows ? PK_LAUNCH(true, true) : PK_LAUNCH(true, false);
+  else rows ? PK_LAUNCH(false, true) : PK_LAUNCH(false, false);
+#undef PK_LAUNCH
+  return check_launch("cache8_read");
+}

@@ -1,0 +1,90 @@
+// The cache in 8 bits as its kernels see it: codes of whole blocks with a scale per block, and the last rows in 16 bits.
+#pragma once
+#include "attend.cuh"
+
+namespace pk {
+
+struct Cache8 {
+  uint8_t* codes;
+  int64_t c_b, c_h, c_l, c_kv;   // strides in codes
+  float* scales;
+  int64_t s_b, s_h, s_j, s_kv;
+  uint16_t* recent;
+  int64_t r_b, r_h, r_l, r_kv;
+  int64_t cap;
+  int R, shift, H;               // places of `recent`; log2 of the block
+};
+
+// Whether no two elements share memory: a dimension's step reaches behind all that the smaller steps span.
+inline bool apart(const pk_tensor* t) {
+  bool used[PK_MAX_DIMS] = {};
+  int64_t span = 0;
+  for (int n = 0; n < t->ndim; n++) {
+    int k = -1;
+    for (int i = 0; i < t->ndim; i++)
+      if (!used[i] && (k < 0 || t->stride[i] < t->stride[k] || (t->stride[i] == t->stride[k] && t->shape[i] < t->shape[k]))) k = i;
+    used[k] = true;
+    if (t->shape[k] <= 1) continue;
+    if (t->stride[k] <= span) return false;
+    span += (t->shape[k] - 1) * t->stride[k];
+  }
+  return true;
+}
+
+inline int fill_cache8(Cache8* c, const pk_cache8* cache, bool write) {
+  PK_REQUIRE(cache != nullptr, "cache is null");
+  const pk_tensor *codes = cache->codes, *scales = cache->scales, *recent = cache->recent;
+  PK_REQUIRE(codes != nullptr && codes->data != nullptr, "codes is null");
+  PK_REQUIRE(codes->dtype == PK_I8 || codes->dtype == PK_E4M3, "codes has dtype tag %d, expected i8 or e4m3", codes->dtype);
+  PK_REQUIRE(codes->ndim == 5 && codes->shape[3] == 2 && codes->shape[4] == 128 && codes->shape[2] <= (1LL << 31) - 256, "codes must be [bs,H,cap,2,128]");
+  PK_CHECK_TENSOR(scales, PK_F32, 4);
+  PK_CHECK_TENSOR(recent, PK_BF16, 5);
+  const int64_t bs = codes->shape[0], H = codes->shape[1], cap = codes->shape[2], block = cache->block;
+  PK_REQUIRE(block == 16 || block == 32 || block == 64 || block == 128, "block must be 16, 32, 64 or 128");
+  PK_REQUIRE(bs < 65536 && H >= 1 && H < 65536, "sizes out of range");
+  PK_REQUIRE(codes->stride[4] == 1 && aligned16(codes->data), "codes needs a unit inner stride and 16-byte alignment");
+  for (int i = 0; i < 4; i++) PK_REQUIRE(codes->shape[i] <= 1 || (codes->stride[i] % 16 == 0 && codes->stride[i] >= 0), "the strides of codes must be multiples of 16");
+  PK_REQUIRE(scales->shape[0] == bs && scales->shape[1] == H && scales->shape[2] == (cap + block - 1) / block && scales->shape[3] == 2, "scales must be f32 [bs,H,ceil(cap/block),2]");
+  for (int i = 0; i < 4; i++) PK_REQUIRE(scales->shape[i] <= 1 || scales->stride[i] >= 0, "the strides of scales must not be negative");
+  PK_REQUIRE(recent->shape[0] == bs && recent->shape[1] == H && recent->shape[3] == 2 && recent->shape[4] == 128, "recent must be bf16 [bs,H,R,2,128]");
+  PK_REQUIRE(recent->shape[2] >= block && recent->shape[2] % block == 0 && recent->shape[2] < (1 << 24), "the places of recent must be a multiple of block, at least one block");
+  PK_REQUIRE(row_tensor(recent), "recent needs a unit inner stride, other strides that are multiples of 8, and 16-byte alignment");
+  if (write) PK_REQUIRE(apart(codes) && apart(scales) && apart(recent), "codes, scales and recent must not share memory within themselves");
+  c->codes = (uint8_t*)codes->data, c->c_b = codes->stride[0], c->c_h = codes->stride[1], c->c_l = codes->stride[2], c->c_kv = codes->stride[3];
+  c->scales = (float*)scales->data, c->s_b = scales->stride[0], c->s_h = scales->stride[1], c->s_j = scales->stride[2], c->s_kv = scales->stride[3];
+  c->recent = (uint16_t*)recent->data, c->r_b = recent->stride[0], c->r_h = recent->stride[1], c->r_l = recent->stride[2], c->r_kv = recent->stride[3];
+  c->cap = cap, c->R = (int)recent->shape[2], c->H = (int)H;
+  c->shift = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7;
+  return PK_OK;
+}
+
+#ifdef __CUDACC__
+// e4m3 x2 -> two floats, exactly
+__device__ __forceinline__ float2 e4m3_floats(uint32_t two) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
+  float2 f;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(f.x), "=f"(f.y) : "r"(h));
+  return f;
+}
+// byte i of four whole numbers as a float: 2^23 + (code + 128) is a float whose last bits are the biased code
+__device__ __forceinline__ float i8_float(uint32_t biased, int i) { return __uint_as_float(__byte_perm(biased, 0x4b000000u, 0x7540 + i)) - 8388736.0f; }
+// y 127 / amax (e4m3: 448) as the definition has it: `unit` is amax 2^-7 (2^-9), 1 for a block of zeros
+__device__ __forceinline__ float i8_quotient(float y, float unit) { return __fdiv_rn(__fmul_rn(y, 0.9921875f), unit); }
+__device__ __forceinline__ float e4m3_quotient(float y, float unit) { return __fdiv_rn(__fmul_rn(y, 0.875f), unit); }
+__device__ __forceinline__ uint32_t pack_i8(float a, float b, float c, float d) {   // to the nearest, ties to the even one
+  uint32_t r;
+  asm("{\n\t.reg .b32 t;\n\tcvt.pack.sat.s8.s32.b32 t, %4, %3, 0;\n\tcvt.pack.sat.s8.s32.b32 %0, %2, %1, t;\n\t}"
+      : "=r"(r)
+      : "r"(__float2int_rn(a)), "r"(__float2int_rn(b)), "r"(__float2int_rn(c)), "r"(__float2int_rn(d)));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  return (uint32_t)lo | (uint32_t)hi << 16;
+}
+#endif
+
+}  // namespace pk

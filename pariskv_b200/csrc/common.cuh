@@ -55,6 +55,8 @@ inline int elem_size(int dtype) {
     case PK_I64: return 8;
     case PK_F32: return 4;
     case PK_BF16: return 2;
+    case PK_I8: return 1;
+    case PK_E4M3: return 1;
   }
   return 0;
 }

@@ -1,0 +1,278 @@
+// Product of tokens and a matrix in 8-bit whole numbers:  out[t,o] = bf16( (sum_k x[t,k] w[o,k]) sx[t] so[o] ),  the sum in 32-bit whole numbers, exact.
+//
+// tcgen05.mma (kind::i8): 128 rows of the matrix are the 128 lanes of tensor memory, NT tokens its columns; 128 columns of both operands a stage, by TMA.
+// Few tokens: the matrix' bytes bound it.  A cluster of S blocks shares a tile's columns, so that all SMs copy; its partial sums meet through distributed shared memory.
+// Many tokens: the tensor cores bound it.  A block per SM goes from tile to tile, the sums of one leave tensor memory under the products of the next.
+#include "cache8.cuh"
+#include "tiles.cuh"
+
+namespace pk {
+namespace {
+
+constexpr int MM_THREADS = 192;        // a warp for the copies, one for the products, four that scale and store
+constexpr int MM_ROWS = 128, MM_K = 128;
+constexpr int MM_WAIT_LIMIT = 100000;  // tries; one waits up to 10 us by itself
+
+struct MmParams {
+  const float *sx, *so;
+  uint16_t* out;
+  int64_t out_t;      // stride of a token's row
+  int T, O, chunks;   // chunks of 128 columns
+  int t_tiles, tiles; // tiles of tokens; tiles in all, tokens first
+  int split;          // blocks of a cluster
+};
+
+template <int NT> struct MmRing { static constexpr int bytes = MM_ROWS * MM_K + NT * MM_K, stages = NT >= 256 ? 4 : NT >= 128 ? 6 : NT >= 64 ? 8 : 10; };
+template <int NT> constexpr int mm_smem() { return 1024 + MmRing<NT>::stages * MmRing<NT>::bytes; }
+
+__device__ __forceinline__ void tma_load2(unsigned dst, const CUtensorMap* map, int c0, int c1, unsigned mb) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(mb) : "memory");
+}
+// D[tmem] (+)= A[smem] B[smem]: 8-bit whole numbers, 32-bit sums
+__device__ __forceinline__ void tc_mma_i8(unsigned d, uint64_t a, uint64_t b, unsigned idesc, unsigned add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t (&r)[16], unsigned addr) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+                 "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint4 remote16(unsigned at, unsigned rank) {   // the same place in the shared memory of block `rank` of the cluster
+  uint4 r;
+  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.b32 {%0,%1,%2,%3}, [a];\n\t}" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at), "r"(rank) : "memory");
+  return r;
+}
+__device__ __forceinline__ unsigned remote4(unsigned at, unsigned rank) {
+  unsigned r;
+  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.u32 %0, [a];\n\t}" : "=r"(r) : "r"(at), "r"(rank) : "memory");
+  return r;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ MmParams p) {
+  constexpr int NS = MmRing<NT>::stages, STAGE = MmRing<NT>::bytes, COLS = NT < 32 ? 32 : NT;   // columns of a set of sums
+  constexpr unsigned IDESC = 2u << 4 | 1u << 7 | 1u << 10 | (unsigned)(NT >> 3) << 17 | (unsigned)(MM_ROWS >> 4) << 24;
+  extern __shared__ unsigned char dyn[];
+  __shared__ __align__(8) unsigned long long bars[2 * NS + 5];
+  __shared__ unsigned s_tmem;
+  __shared__ __align__(16) volatile int s_dead;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const unsigned ring = (smem_addr(dyn) + 1023) & ~1023u;
+  const unsigned full = smem_addr(bars), empty = full + 8 * NS, done = empty + 8 * NS, taken = done + 16, ending = taken + 16;
+  if (tid == 0) {
+    for (int i = 0; i < NS; i++) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
+    for (int i = 0; i < 2; i++) mbar_init(done + 8 * i, 1), mbar_init(taken + 8 * i, 128);
+    mbar_init(ending, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_dead = 0;
+  }
+  if (warp == 1) tmem_alloc(smem_addr(&s_tmem), 2 * COLS);
+  if (warp == 0 && lane < 2) tma_prefetch_map(lane ? &map_x : &map_w);
+  pdl_wait();
+  pdl_trigger();
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const unsigned tmem = s_tmem;
+  const int rank = (int)(blockIdx.x % p.split), cluster = (int)(blockIdx.x / p.split), clusters = (int)(gridDim.x / p.split);
+  const int k0 = (int)((int64_t)p.chunks * rank / p.split), k1 = (int)((int64_t)p.chunks * (rank + 1) / p.split);
+  bool dead = false;   // a wait has run out: no more waiting, the sums come out as NaN
+  auto wait = [&](unsigned mb, unsigned parity) {
+    for (int it = 0; !dead; it++) {
+      if (mbar_try(mb, parity)) break;
+      if (it >= MM_WAIT_LIMIT || ((it & 1023) == 1023 && s_dead)) dead = true, s_dead = 1;
+    }
+  };
+  if (warp == 0) {
+    if (lane == 0) {
+      int q = 0;
+      for (int tile = cluster; tile < p.tiles && !dead; tile += clusters) {
+        const int t0 = tile % p.t_tiles * NT, o0 = tile / p.t_tiles * MM_ROWS;
+        for (int k = k0; k < k1; k++, q++) {
+          const int st = q % NS;
+          if (q >= NS) wait(empty + 8 * st, (unsigned)(q / NS - 1) & 1);
+          if (dead) break;
+          mbar_expect(full + 8 * st, STAGE);
+          tma_load2(ring + st * STAGE, &map_w, k * MM_K, o0, full + 8 * st);
+          tma_load2(ring + st * STAGE + MM_ROWS * MM_K, &map_x, k * MM_K, t0, full + 8 * st);
+        }
+      }
+      if (dead || s_dead)   // what is under way has to land before the block ends
+        for (int i = q < NS ? 0 : q - NS; i < q; i++)
+          for (int it = 0; it < MM_WAIT_LIMIT && !mbar_try(full + 8 * (i % NS), (unsigned)(i / NS) & 1); it++) {}
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    const uint64_t w_desc = umma_desc(ring, 16), x_desc = umma_desc(ring + MM_ROWS * MM_K, 16);
+    int q = 0, n = 0;
+    for (int tile = cluster; tile < p.tiles; tile += clusters, n++) {
+      const int set = n & 1;
+      if (n >= 2) wait(taken + 8 * set, (unsigned)(n / 2 - 1) & 1);
+      __syncwarp();
+      tc_after();
+      for (int k = k0; k < k1; k++, q++) {
+        const int st = q % NS;
+        wait(full + 8 * st, (unsigned)(q / NS) & 1);
+        __syncwarp();
+        tc_after();
+        if (leader && !dead) {
+          const uint64_t a = w_desc + (uint64_t)st * (STAGE >> 4), b = x_desc + (uint64_t)st * (STAGE >> 4);
+#pragma unroll
+          for (int i = 0; i < 4; i++) tc_mma_i8(tmem + COLS * set, a + 2 * i, b + 2 * i, IDESC, k > k0 || i > 0);
+          tc_commit(empty + 8 * st);
+        }
+      }
+      if (leader && !dead) tc_commit(done + 8 * set);
+    }
+    if (s_dead && leader) {   // products under way end before the tensor memory goes
+      tc_commit(ending);
+      for (int it = 0; it < MM_WAIT_LIMIT && !mbar_try(ending, 0); it++) {}
+    }
+  } else {
+    const int quarter = warp & 3, o_lane = 32 * quarter + lane;
+    const unsigned lanes = tmem + ((unsigned)quarter << 21);
+    int n = 0;
+    for (int tile = cluster; tile < p.tiles; tile += clusters, n++) {
+      const int set = n & 1, t0 = tile % p.t_tiles * NT, o = tile / p.t_tiles * MM_ROWS + o_lane;
+      wait(done + 8 * set, (unsigned)(n / 2) & 1);
+      __syncwarp();
+      tc_after();
+      const float so = o < p.O ? p.so[o] : 0.0f;
+      if (p.split == 1) {
+#pragma unroll 1
+        for (int c = 0; c < NT; c += 16) {
+          uint32_t acc[16];
+          tmem_ld16(acc, lanes + COLS * set + c);
+          if (c + 16 == NT) {
+            tc_before();
+            mbar_arrive1(taken + 8 * set);
+          }
+          if (o < p.O) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const int t = t0 + c + i;
+              if (t < p.T) p.out[t * p.out_t + o] = f2bf(dead ? NAN : (float)(int)acc[i] * p.sx[t] * so);
+            }
+          }
+        }
+      } else {
+        // this block's partial sums, column by column, where the copies were (they have all been multiplied)
+#pragma unroll 1
+        for (int c = 0; c < NT; c += 16) {
+          uint32_t acc[16];
+          tmem_ld16(acc, lanes + COLS * set + c);
+#pragma unroll
+          for (int i = 0; i < 16; i++) asm volatile("st.shared.b32 [%0], %1;" ::"r"(ring + ((c + i) * MM_ROWS + o_lane) * 4), "r"(acc[i]) : "memory");
+        }
+      }
+    }
+  }
+  if (p.split > 1) {   // one tile a cluster.  Column t of the tile, four rows a thread: the block that has t mod split adds them
+    __syncwarp();
+    tc_before();
+    cluster_sync();
+    const int tile = cluster, t0 = tile % p.t_tiles * NT, o0 = tile / p.t_tiles * MM_ROWS;
+    bool lost = false;
+    for (int s = 0; s < p.split; s++) lost |= remote4(smem_addr((const void*)&s_dead), (unsigned)s) != 0;
+    for (int c = rank * (MM_THREADS / 32) + warp; c < NT; c += p.split * (MM_THREADS / 32)) {
+      const int t = t0 + c;
+      if (t >= p.T) continue;
+      uint4 sum = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+      for (int s = 0; s < p.split; s++) {
+        const uint4 v = remote16(ring + (c * MM_ROWS + 4 * lane) * 4, (unsigned)s);
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+      }
+      const uint32_t a[4] = {sum.x, sum.y, sum.z, sum.w};
+      const float sx = p.sx[t];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int o = o0 + 4 * lane + i;
+        if (o < p.O) p.out[t * p.out_t + o] = f2bf(lost ? NAN : (float)(int)a[i] * sx * p.so[o]);
+      }
+    }
+    cluster_sync();
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  if (warp == 1) tmem_free(tmem, 2 * COLS);
+}
+
+// Rows of 8-bit numbers in boxes of 128 columns; what is behind the last row or column comes as zeros.
+bool bytes_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t stride, int box) {
+  const auto encode = tensor_map_encoder();
+  if (!encode) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
+  const cuuint32_t boxes[2] = {MM_K, (cuuint32_t)box}, steps[2] = {1, 1};
+  return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int NT>
+int launch(const pk_tensor* x, const pk_tensor* w, MmParams p, cudaStream_t st) {
+  CUtensorMap mw, mx;
+  const int64_t I = x->shape[1];
+  if (!bytes_map(&mw, w->data, p.O, I, p.O > 1 ? w->stride[0] : (I + 15) / 16 * 16, MM_ROWS) || !bytes_map(&mx, x->data, p.T, I, p.T > 1 ? x->stride[0] : (I + 15) / 16 * 16, NT))
+    return fail(PK_ERR_CUDA, "matmul_i8: no tensor map for these rows");
+  static PerDevice opted;
+  if (const unsigned long long bit = first_on_device(opted)) {
+    if (cudaFuncSetAttribute(matmul_i8_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, mm_smem<NT>()) != cudaSuccess)
+      return fail(PK_ERR_CUDA, "matmul_i8: %s", cudaGetErrorString(cudaGetLastError()));
+    mark_on_device(opted, bit);
+  }
+  p.t_tiles = (p.T + NT - 1) / NT;
+  p.tiles = p.t_tiles * ((p.O + MM_ROWS - 1) / MM_ROWS);
+  const int sms = sm_count();
+  p.split = 1;
+  while (p.split < 8 && p.tiles * p.split * 2 <= sms && p.split * 2 <= p.chunks) p.split *= 2;
+  const int clusters = p.split > 1 ? p.tiles : p.tiles < sms ? p.tiles : sms;
+  StageTimer timer(ST_GEMV, st);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(clusters * p.split)), cfg.blockDim = dim3(MM_THREADS), cfg.dynamicSmemBytes = mm_smem<NT>(), cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (p.split > 1) attr[n].id = cudaLaunchAttributeClusterDimension, attr[n].val.clusterDim.x = (unsigned)p.split, attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1, n++;
+  if (pdl_enabled()) attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[n].val.programmaticStreamSerializationAllowed = 1, n++;
+  cfg.attrs = attr, cfg.numAttrs = n;
+  cudaLaunchKernelEx(&cfg, matmul_i8_kernel<NT>, mw, mx, p);
+  return check_launch("matmul_i8");
+}
+
+bool rows16(const pk_tensor* t) {
+  return (t->shape[1] <= 1 || t->stride[1] == 1) && aligned16(t->data) && (t->shape[0] <= 1 || (t->stride[0] % 16 == 0 && t->stride[0] > 0));
+}
+
+}  // namespace
+}  // namespace pk
+
+using namespace pk;
+
+extern "C" int pk_matmul_i8(const pk_tensor* x, const pk_tensor* x_scales, const pk_tensor* weight, const pk_tensor* weight_scales, const pk_tensor* out, void* stream) {
+  PK_CHECK_TENSOR(x, PK_I8, 2);
+  PK_CHECK_TENSOR(x_scales, PK_F32, 1);
+  PK_CHECK_TENSOR(weight, PK_I8, 2);
+  PK_CHECK_TENSOR(weight_scales, PK_F32, 1);
+  PK_CHECK_TENSOR(out, PK_BF16, 2);
+  const int64_t T = x->shape[0], I = x->shape[1], O = weight->shape[0];
+  PK_REQUIRE(I >= 16 && I % 16 == 0 && I <= 65536, "the width must be a multiple of 16, at most 65536");
+  PK_REQUIRE(weight->shape[1] == I, "weight must be i8 [O,I], as wide as x");
+  PK_REQUIRE(T < (1LL << 31) - 256 && O < (1LL << 31) - 256 && ((T + 15) / 16) * ((O + 127) / 128) < (1LL << 31), "sizes out of range");
+  PK_REQUIRE(rows16(x) && rows16(weight), "x and weight need a unit inner stride, rows at strides that are multiples of 16, and 16-byte alignment");
+  PK_REQUIRE(x_scales->shape[0] == T && is_contig(x_scales), "x_scales must be contiguous f32 [T]");
+  PK_REQUIRE(weight_scales->shape[0] == O && is_contig(weight_scales), "weight_scales must be contiguous f32 [O]");
+  PK_REQUIRE(out->shape[0] == T && out->shape[1] == O && (O <= 1 || out->stride[1] == 1) && (T <= 1 || out->stride[0] >= O), "out must be bf16 [T,O] with a unit inner stride, rows apart");
+  if (T == 0 || O == 0) return PK_OK;
+  MmParams p = {};
+  p.sx = (const float*)x_scales->data, p.so = (const float*)weight_scales->data, p.out = (uint16_t*)out->data, p.out_t = out->stride[0];
+  p.T = (int)T, p.O = (int)O, p.chunks = (int)((I + MM_K - 1) / MM_K);
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (T <= 16) return launch<16>(x, weight, p, st);
+  if (T <= 32) return launch<32>(x, weight, p, st);
+  if (T <= 64) return launch<64>(x, weight, p, st);
+  if (T <= 128) return launch<128>(x, weight, p, st);
+  return launch<256>(x, weight, p, st);
+}

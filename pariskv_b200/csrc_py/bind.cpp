@@ -34,6 +34,8 @@ int dtype_tag(at::ScalarType s) {
     case at::kLong: return PK_I64;
     case at::kFloat: return PK_F32;
     case at::kBFloat16: return PK_BF16;
+    case at::kChar: return PK_I8;
+    case at::kFloat8_e4m3fn: return PK_E4M3;
     default: return -1;
   }
 }
@@ -748,6 +750,135 @@ PyObject* py_gemv_w4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   PK_PY_END
 }
 
+// ---- a step in 8 bits ----
+struct Cache {
+  Arg codes, scales, recent;
+  pk_cache8 c = {};
+};
+bool take_cache(PyObject* const* a, Cache* c) {   // codes, scales, recent, block
+  if (!need(a[0], &c->codes, CUDA) || !need(a[1], &c->scales, CUDA) || !need(a[2], &c->recent, CUDA) || !to_i64(a[3], &c->c.block) || !dims(c->codes, 5, "codes")) return false;
+  c->c.codes = c->codes.p(), c->c.scales = c->scales.p(), c->c.recent = c->recent.p();
+  return same_device({&c->scales, &c->recent}, *c->codes.t);
+}
+
+// (codes, scales, recent, block, keys, values, lengths, counts or None)
+PyObject* py_cache8_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 8, "cache8_append")) return nullptr;
+  PK_PY_BEGIN
+  Cache c;
+  Arg k, v, len, cnt;
+  if (!take_cache(a, &c) || !need(a[4], &k, CUDA) || !need(a[5], &v, CUDA) || !need(a[6], &len, CUDA) || !take(a[7], &cnt, CUDA) || !dims(k, 4, "keys")) return nullptr;
+  const at::Tensor& like = *c.codes.t;
+  const c10::cuda::CUDAGuard guard(like.device());
+  if (!same_device({&k, &v, &len, &cnt}, like)) return nullptr;
+  if (k.t->numel() == 0 && k.d.shape[1] == 0) Py_RETURN_NONE;
+  void* st = stream_of(like);
+  const int rc = without_gil([&] { return pk_cache8_append(&c.c, k.p(), v.p(), len.p(), cnt.p(), st); });
+  if (rc) return raise(rc);
+  Py_RETURN_NONE;
+  PK_PY_END
+}
+
+// (codes, scales, recent, block, lengths, rows or None, out or None) -> out
+PyObject* py_cache8_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 7, "cache8_read")) return nullptr;
+  PK_PY_BEGIN
+  Cache c;
+  Arg len, rows, out;
+  at::Tensor own;
+  if (!take_cache(a, &c) || !need(a[4], &len, CUDA) || !take(a[5], &rows, CUDA)) return nullptr;
+  if (rows.t && !dims(rows, 3, "rows")) return nullptr;
+  const at::Tensor& like = *c.codes.t;
+  const c10::cuda::CUDAGuard guard(like.device());
+  if (!output(a[6], &out, &own, like, {c.codes.d.shape[0], c.codes.d.shape[1], rows.t ? rows.d.shape[2] : c.codes.d.shape[2], 2, 128}, at::kBFloat16) ||
+      !same_device({&len, &rows, &out}, like))
+    return nullptr;
+  if (out.t->numel() == 0) return give(a[6], out);
+  void* st = stream_of(like);
+  const int rc = without_gil([&] { return pk_cache8_read(&c.c, len.p(), rows.p(), out.p(), st); });
+  if (rc) return raise(rc);
+  return give(a[6], out);
+  PK_PY_END
+}
+
+// (queries, codes, scales, recent, block, lengths, scale, out, lse) -> out
+PyObject* py_cache8_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 9, "cache8_attention")) return nullptr;
+  PK_PY_BEGIN
+  Cache c;
+  Arg q, len, out, lse;
+  at::Tensor own;
+  double scale;
+  if (!need(a[0], &q, CUDA) || !take_cache(a + 1, &c) || !need(a[5], &len, CUDA) || !to_f64(a[6], &scale) || !take(a[8], &lse, CUDA) || !dims(q, 4, "queries")) return nullptr;
+  const c10::cuda::CUDAGuard guard(q.t->device());
+  if (!output(a[7], &out, &own, *q.t, q.t->sizes(), at::kBFloat16) || !same_device({&c.codes, &len, &out, &lse}, *q.t)) return nullptr;
+  if (q.t->numel() == 0) return give(a[7], out);
+  const int64_t bytes = pk_cache8_attention_workspace_bytes(q.d.shape[0], q.d.shape[1], q.d.shape[2], c.codes.d.shape[1], c.codes.d.shape[2]);
+  const at::Tensor ws = empty_on(*q.t, {bytes}, at::kByte);
+  void* st = stream_of(*q.t);
+  const int rc = without_gil([&] { return pk_cache8_attention(q.p(), &c.c, len.p(), (float)scale, out.p(), lse.p(), ws.data_ptr(), bytes, st); });
+  if (rc) return raise(rc);
+  return give(a[7], out);
+  PK_PY_END
+}
+
+// (a, residual or None, weight, eps) -> (h, codes, scales)
+PyObject* py_add_rmsnorm_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 4, "add_rmsnorm_i8")) return nullptr;
+  PK_PY_BEGIN
+  Arg x, r, w, h, q, s;
+  at::Tensor th, tq, ts;
+  double eps;
+  if (!need(a[0], &x, CUDA) || !take(a[1], &r, CUDA) || !need(a[2], &w, CUDA) || !to_f64(a[3], &eps) || !dims(x, 2, "a")) return nullptr;
+  const c10::cuda::CUDAGuard guard(x.t->device());
+  if (!same_device({&r, &w}, *x.t) || !output(Py_None, &h, &th, *x.t, x.t->sizes(), at::kBFloat16) || !output(Py_None, &q, &tq, *x.t, x.t->sizes(), at::kChar) ||
+      !output(Py_None, &s, &ts, *x.t, {x.d.shape[0]}, at::kFloat))
+    return nullptr;
+  if (x.d.shape[0] > 0) {
+    void* st = stream_of(*x.t);
+    const int rc = without_gil([&] { return pk_add_rmsnorm_i8(x.p(), r.p(), w.p(), h.p(), q.p(), s.p(), eps, st); });
+    if (rc) return raise(rc);
+  }
+  return Py_BuildValue("(NNN)", THPVariable_Wrap(th), THPVariable_Wrap(tq), THPVariable_Wrap(ts));
+  PK_PY_END
+}
+
+// (x, gated) -> (codes, scales)
+PyObject* py_quantize_rows_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 2, "quantize_rows_i8")) return nullptr;
+  PK_PY_BEGIN
+  Arg x, q, s;
+  at::Tensor tq, ts;
+  int64_t gated;
+  if (!need(a[0], &x, CUDA) || !to_i64(a[1], &gated) || !dims(x, 2, "x")) return nullptr;
+  const c10::cuda::CUDAGuard guard(x.t->device());
+  if (!output(Py_None, &q, &tq, *x.t, {x.d.shape[0], gated ? x.d.shape[1] / 2 : x.d.shape[1]}, at::kChar) || !output(Py_None, &s, &ts, *x.t, {x.d.shape[0]}, at::kFloat)) return nullptr;
+  if (x.d.shape[0] > 0) {
+    void* st = stream_of(*x.t);
+    const int rc = without_gil([&] { return pk_quantize_rows_i8(x.p(), gated != 0, q.p(), s.p(), st); });
+    if (rc) return raise(rc);
+  }
+  return Py_BuildValue("(NN)", THPVariable_Wrap(tq), THPVariable_Wrap(ts));
+  PK_PY_END
+}
+
+// (x, x_scales, weight, weight_scales, out or None) -> out
+PyObject* py_matmul_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 5, "matmul_i8")) return nullptr;
+  PK_PY_BEGIN
+  Arg x, sx, w, so, out;
+  at::Tensor own;
+  if (!need(a[0], &x, CUDA) || !need(a[1], &sx, CUDA) || !need(a[2], &w, CUDA) || !need(a[3], &so, CUDA) || !dims(x, 2, "x") || !dims(w, 2, "weight")) return nullptr;
+  const c10::cuda::CUDAGuard guard(x.t->device());
+  if (!output(a[4], &out, &own, *x.t, {x.d.shape[0], w.d.shape[0]}, at::kBFloat16) || !same_device({&sx, &w, &so, &out}, *x.t)) return nullptr;
+  if (out.t->numel() == 0) return give(a[4], out);
+  void* st = stream_of(*x.t);
+  const int rc = without_gil([&] { return pk_matmul_i8(x.p(), sx.p(), w.p(), so.p(), out.p(), st); });
+  if (rc) return raise(rc);
+  return give(a[4], out);
+  PK_PY_END
+}
+
 PyObject* py_attention_workspace_bytes(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arity(n, 3, "attention_workspace_bytes")) return nullptr;
   int64_t v[3];
@@ -791,6 +922,12 @@ PyMethodDef methods[] = {
     PK_METHOD("select_blocks", py_select_blocks),
     PK_METHOD("block_attention", py_block_attention),
     PK_METHOD("gemv_w4", py_gemv_w4),
+    PK_METHOD("cache8_append", py_cache8_append),
+    PK_METHOD("cache8_read", py_cache8_read),
+    PK_METHOD("cache8_attention", py_cache8_attention),
+    PK_METHOD("add_rmsnorm_i8", py_add_rmsnorm_i8),
+    PK_METHOD("quantize_rows_i8", py_quantize_rows_i8),
+    PK_METHOD("matmul_i8", py_matmul_i8),
     PK_METHOD("attention_workspace_bytes", py_attention_workspace_bytes),
     PK_METHOD("retrieve_workspace_bytes", py_retrieve_workspace_bytes),
     {nullptr, nullptr, 0, nullptr}};

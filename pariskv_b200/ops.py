@@ -554,3 +554,63 @@ def gemv_w4(weight, scales, x, offsets=None, gated=False):
     bf16 [O, I/group], group 32, 64 or 128.  W = (code - 8) * scale, with offsets (bf16 like scales) code * scale + offset.  gated:
     weight = [gate; up] stacked, result [T, O/2] = silu(gate x) * (up x).  See pk_gemv_w4."""
     return L.native().gemv_w4(weight, scales, offsets, x, gated)
+
+
+# --------------------------------------------------------------------------------------------------
+# a step in 8 bits: the cache and what reads it, the products and what feeds them
+# --------------------------------------------------------------------------------------------------
+class Cache8:
+    """A cache in 8 bits of one layer: codes int8 or float8_e4m3fn [bs,H,cap,2,128] (K and V of a row), scales f32 [bs,H,ceil(cap/block),2], recent bf16
+    [bs,H,R,2,128].  A value is code * scale; `block` (16, 32, 64 or 128) rows of a sequence and head share a scale.  The rows behind a sequence's last whole block are
+    those of `recent`, row r at place r % R, in 16 bits; a block is coded once, when it is whole.  Views of any layout (separate tensors for K and V:
+    permuted to these shapes); see pk_cache8 for what they need.  The lengths of the sequences stay with the caller, on the device."""
+    __slots__ = ("codes", "scales", "recent", "block")
+
+    def __init__(self, codes, scales, recent, block=64):
+        self.codes, self.scales, self.recent, self.block = codes, scales, recent, int(block)
+
+    @classmethod
+    def empty(cls, bs, heads, cap, block=64, dtype=torch.int8, recent=None, device="cuda"):
+        """A cache of `cap` rows per sequence, without any.  recent: the rows kept in 16 bits, a multiple of block (2 * block by default); up to
+        recent - block rows may be taken back."""
+        places = 2 * block if recent is None else int(recent)
+        return cls(torch.zeros(bs, heads, cap, 2, 128, dtype=torch.uint8, device=device).view(dtype),
+                   torch.zeros(bs, heads, -(-cap // block), 2, dtype=torch.float32, device=device),
+                   torch.zeros(bs, heads, places, 2, 128, dtype=torch.bfloat16, device=device), block)
+
+
+def cache8_append(cache, keys, values, lengths, counts=None):
+    """Rows into a Cache8, in place: keys / values bf16 [bs,T,H,128].  lengths (i32 [bs], read on the device): the rows of each sequence with the new ones; counts (i32 [bs]): how
+    many of the T are a sequence's, T by default (a padded prompt has fewer; what follows them is not read).  One launch; what the cache holds does not depend on how
+    rows are cut into calls.  See pk_cache8_append."""
+    L.native().cache8_append(cache.codes, cache.scales, cache.recent, cache.block, keys, values, lengths, counts)
+
+
+def cache8_read(cache, lengths, rows=None, out=None):
+    """Rows of a Cache8 back in bf16 [bs,H,n,2,128]: all of them (those from a sequence's length on are left as they are; in a new tensor: not initialised), or the listed ones, rows i64
+    [bs,H,n] (an entry that is no row of the sequence gives zeros).  See pk_cache8_read."""
+    return L.native().cache8_read(cache.codes, cache.scales, cache.recent, cache.block, lengths, rows, out)
+
+
+def cache8_attention(queries, cache, lengths, scale=None, out=None, lse=None):
+    """Attention of the last T tokens of the sequences over a Cache8, each token up to its own position: queries bf16 [bs,T,Hq,128] (T at most 256), lengths i32 [bs] with these tokens ->
+    bf16 [bs,T,Hq,128]; lse, if given (f32 [bs,T,Hq]), receives log2 of the softmax denominators.  See pk_cache8_attention."""
+    return L.native().cache8_attention(queries, cache.codes, cache.scales, cache.recent, cache.block, lengths,
+                                       queries.shape[-1] ** -0.5 if scale is None else float(scale), out, lse)
+
+
+def add_rmsnorm_i8(a, residual, weight, eps=1e-6):
+    """add_rmsnorm for a product in 8 bits: h = a + residual (residual may be None), y = RMS-norm(h) * weight as int8 codes with a scale per token.  Returns (h, codes, scales): bf16 [B,n], int8
+    [B,n], f32 [B].  See pk_add_rmsnorm_i8."""
+    return L.native().add_rmsnorm_i8(a, residual, weight, eps)
+
+
+def quantize_rows_i8(x, gated=False):
+    """Rows of bf16 [B,n] as int8 codes with a scale per row; gated: of silu(x[:, :n]) * x[:, n:], x [B,2n].  Returns (codes, scales): what matmul_i8 takes.  See pk_quantize_rows_i8."""
+    return L.native().quantize_rows_i8(x, gated)
+
+
+def matmul_i8(x, x_scales, weight, weight_scales, out=None):
+    """x [T,I] @ weight[O,I]^T -> bf16 [T,O] of int8 codes, x_scales f32 [T] per token, weight_scales f32 [O] per row of the matrix; the sums are whole numbers, exact.  Any number of tokens; I a
+    multiple of 16.  See pk_matmul_i8."""
+    return L.native().matmul_i8(x, x_scales, weight, weight_scales, out)
