@@ -15,14 +15,16 @@
 namespace pk {
 namespace {
 
-constexpr int A8_TILE = 128, A8_THREADS = 128, A8_STAGES = 2;
-constexpr int A8_ROWS = 16;                       // query rows of an item: those of one operand
+constexpr int A8_TILE = 128, A8_THREADS = 128;
 constexpr int A8_STAGE = 8192;                    // 32 rows of K and V in codes, 16 in bf16
 constexpr int A8_SLOT = A8_STAGE + 16;            // and the scales: K of the first and second 16 rows, V of them
-constexpr int A8_SMEM = 4 * A8_STAGES * A8_SLOT;
-constexpr int A8_CTAS = 3;
-constexpr int A8_OS = 136;                        // floats between two rows of a warp's partial
+constexpr int A8_OT = 36, A8_OS = 4 * A8_OT;      // a warp's partial: floats between two lanes' 32 channels, and two rows, so that its stores fall into all banks
 static_assert(8 * A8_OS * 4 <= A8_STAGE, "a warp's partial of eight rows takes the place of a stage");
+constexpr int A8_QS = 272;                        // bytes between two rows of the queries in bf16
+// ROWS: query rows of an item.
+template <int ROWS> struct A8 {
+  static constexpr int ctas = ROWS == 32 ? 2 : 3, q_bytes = ROWS * (256 + A8_QS), smem = 4 * 2 * A8_SLOT + q_bytes;
+};
 
 struct Attend8 {
   Cache8 c;
@@ -32,7 +34,7 @@ struct Attend8 {
   int bs, T, G, row_groups;
   float scale_log2;
   uint16_t* out;
-  float *lse, *records;   // records: [2 * blocks][16 * 130]
+  float *lse, *records;   // records: [2 * blocks][ROWS * 130]
 };
 
 __device__ __forceinline__ int len8(const Attend8& p, int b) { return (int)min((int64_t)max(p.lengths[b], 0), p.c.cap); }
@@ -41,24 +43,14 @@ __device__ __forceinline__ int tiles8(const Attend8& p, int len) {   // of an it
   return max(1, (whole + A8_TILE - 1) / A8_TILE + (whole < len));
 }
 
-// A warp's way through its steps: a tile of codes is one, a tile of 16-bit rows is two.
+// A block's way through its range: segments of consecutive tiles of one item.
 struct Way8 {
-  int b, h, group, len, whole, n, tile, sub;
-  int64_t left;   // tiles of the block's range that are left, this one included
+  int b, h, group, len, whole, n, tile;
+  int64_t left;   // tiles of the range that are left
   __device__ __forceinline__ void sample(const Attend8& p) { len = len8(p, b), whole = len >> p.c.shift << p.c.shift, n = tiles8(p, len); }
-  __device__ __forceinline__ bool recent() const { return tile * A8_TILE >= whole && len > whole; }
-  __device__ __forceinline__ int row0(int warp) const { return recent() ? whole + 32 * warp + 16 * sub : tile * A8_TILE + 32 * warp; }
-  __device__ __forceinline__ int live(int warp) const {   // rows of this warp's step that are there
-    return recent() ? max(0, min(16, len - row0(warp))) : max(0, min(32, whole - row0(warp)));
-  }
-  __device__ __forceinline__ bool last_of_item() const { return (recent() ? sub == 1 : true) && (tile == n - 1 || left == 1); }
-  __device__ __forceinline__ void step(const Attend8& p) {
-    if (recent() && sub == 0) {
-      sub = 1;
-      return;
-    }
-    sub = 0, left--;
-    if (++tile < n) return;
+  __device__ __forceinline__ int count() const { return (int)min((int64_t)(n - tile), left); }
+  __device__ __forceinline__ void next(const Attend8& p) {
+    left -= count();
     tile = 0;
     if (++group < p.row_groups) return;
     group = 0;
@@ -68,105 +60,89 @@ struct Way8 {
   }
 };
 
+__device__ __forceinline__ void cp16(unsigned dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void cp16(unsigned dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp4(unsigned dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ uint4 lds16(unsigned at) {
-  uint4 r;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
-  return r;
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+  __syncwarp();
 }
-__device__ __forceinline__ float lds4(unsigned at) {
-  float r;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(at) : "memory");
-  return r;
-}
+// Reads that the compiler may move between the barriers: plain loads of the block's shared memory, at an offset.
+extern __shared__ __align__(128) unsigned char dyn8[];
+__device__ __forceinline__ uint4 lds16(unsigned off) { return *reinterpret_cast<const uint4*>(dyn8 + off); }
+__device__ __forceinline__ uint2 lds8(unsigned off) { return *reinterpret_cast<const uint2*>(dyn8 + off); }
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Two codes (bytes lo, lo + 1 of w) as fp16 numbers.  Whole numbers come biased by 128.  e4m3: sign, exponent and significand in their places are 2^-8 of the value.
-template <bool E4M3, int LO>
-__device__ __forceinline__ uint32_t halves(uint32_t w) {
+// Two codes as fp16 numbers.  Whole numbers: bytes 0 and 2 of w (hi: 1 and 3) become the last bits of 1024 + (code + 128), and 1152 is taken off.  e4m3: bytes 0 and 1 (hi: 2 and 3).
+// The queries lie in the same order.
+template <bool E4M3>
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
   uint32_t r;
-  if (E4M3) {
-    const uint32_t x = __byte_perm(w, 0, LO ? 0x3424 : 0x1404);   // each code is the upper byte of its half
-    r = (x & 0x80008000u) | ((x & 0x7f007f00u) >> 1);
-  } else {
-    const uint32_t x = __byte_perm(w, 0x64646464u, LO ? 0x4342 : 0x4140);
-    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0xe480e480u));   // 1024 + 128 + code - 1152
-  }
+  if (E4M3) asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(r) : "r"(w));
+  else asm("{\n\t.reg .b32 x;\n\tlop3.b32 x, %1, 0x00ff00ff, 0x64806480, 0x6a;\n\tadd.rn.f16x2 %0, x, %2;\n\t}" : "=r"(r) : "r"(w), "r"(0xe480e480u));
   return r;
 }
 template <bool E4M3>
-__device__ __forceinline__ uint32_t biased(uint32_t w) { return E4M3 ? w : w ^ 0x80808080u; }
-
-// Running state of a lane's two rows (g and g + 8 of the item).
-struct RowState {
-  float m, l, u;        // largest score, sum of p (this lane's columns), largest p vs so far, all relative to m
-  float up, down;       // 2^-E and 2^E: O is kept as 2^-E of what it stands for
-};
-
-// The weights of a step's columns: x[e][i] scores of row e (masked ones -inf), vs[i] the value scale of column i.  Leaves p vs 2^-E in x and scales what there is of O.
-template <int N>
-__device__ __forceinline__ void weigh(RowState (&st)[2], float (&o)[16][4], float (&x)[2][N], const float (&vs)[N], const float (&factor)[2]) {
-  float f[2];
-#pragma unroll
-  for (int e = 0; e < 2; e++) {
-    RowState& s = st[e];
-    float mx = x[e][0];
-#pragma unroll
-    for (int i = 1; i < N; i++) mx = fmaxf(mx, x[e][i]);
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const float m = fmaxf(s.m, mx), least = m == -INFINITY ? 0.0f : m;
-    f[e] = s.m == -INFINITY ? 0.0f : m > s.m ? ex2((s.m - m) * factor[e]) : 1.0f;
-    float sum = 0.0f, top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-      const bool seen = x[e][i] != -INFINITY;   // (a NaN is seen)
-      const float y = seen ? ex2((x[e][i] - least) * factor[e]) : 0.0f;
-      sum += y;
-      x[e][i] = seen ? y * vs[i] : 0.0f;   // (the scale of a block that it does not see may be NaN)
-      top = fmaxf(top, x[e][i]);
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    s.m = m, s.l = s.l * f[e] + sum;
-    const float before = s.u * f[e];
-    s.u = fmaxf(before, top);
-    const float t = s.u * s.up;
-    if (s.u > 0.0f && !(t >= 0.0625f && t <= 256.0f)) {   // (the same for the four lanes of a row)
-      const unsigned ex = min(__float_as_uint(s.u) >> 23, 252u);
-      s.up = __uint_as_float((254u - ex) << 23);
-      f[e] = before == 0.0f ? 0.0f : f[e] * s.up * s.down;
-      s.down = ex == 0 ? __uint_as_float(1u << 22) : __uint_as_float(ex << 23);
-    }
-#pragma unroll
-    for (int i = 0; i < N; i++) x[e][i] *= s.up;
-  }
-  if (__any_sync(0xffffffffu, f[0] != 1.0f || f[1] != 1.0f)) {
-#pragma unroll
-    for (int n = 0; n < 16; n++) o[n][0] *= f[0], o[n][1] *= f[0], o[n][2] *= f[1], o[n][3] *= f[1];
-  }
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+  uint32_t r;
+  if (E4M3) asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, b;\n\t}" : "=r"(r) : "r"(w));
+  else r = codes_lo<false>(w >> 8);
+  return r;
+}
+// Words a, c of two rows -> words with the two rows' codes side by side as codes_lo / codes_hi take them: channels 0, 1 of the word, and 2, 3
+template <bool E4M3> __device__ __forceinline__ uint32_t pair01(uint32_t a, uint32_t c) { return __byte_perm(a, c, E4M3 ? 0x5140 : 0x5410); }
+template <bool E4M3> __device__ __forceinline__ uint32_t pair23(uint32_t a, uint32_t c) { return __byte_perm(a, c, E4M3 ? 0x7362 : 0x7632); }
+__device__ __forceinline__ float quad_max(float x) {
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
 }
 
-template <bool E4M3>
-__global__ void __launch_bounds__(A8_THREADS, A8_CTAS) attend8_kernel(const __grid_constant__ Attend8 p) {
-  extern __shared__ __align__(128) unsigned char dyn[];
-  __shared__ float s_m[4][16], s_l[4][16], s_u[4][16];
+// Running state of one of a lane's query rows.  m: the largest score so far, times log2 e / sqrt d; l: the sum of p over this lane's columns, relative to 2^m; u: the largest p vs; O is kept as
+// 2^-E of what it stands for, up = 2^-E, down = 2^E with E following u, so that the weights p vs 2^-E are fp16 numbers with all of their bits.
+struct RowState {
+  float m, l, u, up, down;
+};
+// To a new largest score and a new largest p vs (relative to it): what O has to be multiplied by.
+__device__ __forceinline__ float move(RowState& s, float m, float top) {
+  float f = s.m == -INFINITY ? 0.0f : m > s.m ? ex2(s.m - m) : 1.0f;
+  s.m = m, s.l *= f;
+  const float before = s.u * f;
+  s.u = fmaxf(before, top);
+  const float t = s.u * s.up;
+  if (s.u > 0.0f && !(t >= 0.0625f && t <= 256.0f)) {
+    const unsigned ex = min(__float_as_uint(s.u) >> 23, 252u);
+    s.up = __uint_as_float((254u - ex) << 23);
+    f = before == 0.0f ? 0.0f : f * s.up * s.down;
+    s.down = ex == 0 ? __uint_as_float(1u << 22) : __uint_as_float(ex << 23);
+  }
+  return f;
+}
+__device__ __forceinline__ void scale_rows(float (&o)[16][4], int e, float f) {
+#pragma unroll
+  for (int n = 0; n < 16; n++) o[n][2 * e] *= f, o[n][2 * e + 1] *= f;
+}
+
+template <bool E4M3, int ROWS>
+__global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(const __grid_constant__ Attend8 p) {
+  constexpr int MT = ROWS == 32 ? 2 : 1, RPT = ROWS == 8 ? 1 : 2, NR = MT * RPT;   // operands of 16 rows, rows of a lane in each, in all
+  __shared__ float s_m[4][ROWS], s_l[4][ROWS], s_factor[ROWS];
   __shared__ TilePlan s_plan;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   pdl_wait();
@@ -185,278 +161,392 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS) attend8_kernel(const __gr
   {
     const int64_t first = share_begin(plan.total, blockIdx.x, shares);
     way.left = share_begin(plan.total, blockIdx.x + 1, shares) - first;
-    way.b = plan.sample, way.sub = 0;
+    way.b = plan.sample;
     way.sample(p);
     const int64_t at = first - plan.before;
     const int64_t item = at / way.n;
     way.tile = (int)(at % way.n), way.h = (int)(item / p.row_groups), way.group = (int)(item % p.row_groups);
   }
-  const unsigned mine = smem_addr(dyn) + warp * A8_STAGES * A8_SLOT;
-  // One step's rows on their way.  A chunk of 16 bytes lies where its row's number moves it, so that the reads below fall into all banks.
-  auto load = [&](const Way8& w, int slot) {
-    const unsigned to = mine + slot * A8_SLOT;
-    const int live = w.live(warp), row0 = w.row0(warp);
-    if (live > 0) {
-      if (w.recent()) {
-        const uint16_t* src = p.c.recent + w.b * p.c.r_b + w.h * p.c.r_h + (lane >> 4) * p.c.r_kv + (lane & 15) * 8;
-#pragma unroll
-        for (int i = 0; i < 16; i++) cp16(to + (lane >> 4) * 4096 + i * 256 + (lane & 15) * 16, src + (int64_t)((i < live ? row0 + i : row0) % p.c.R) * p.c.r_l, i < live);
-      } else {
-        const int c = lane & 7, kv = lane >> 3 & 1, odd = lane >> 4;
-        const uint8_t* src = p.c.codes + w.b * p.c.c_b + w.h * p.c.c_h + kv * p.c.c_kv + (int64_t)row0 * p.c.c_l + c * 16;
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int r = 2 * i + odd;
-          cp16(to + kv * 4096 + r * 128 + ((c ^ (kv ? r & 6 : r & 1)) << 4), src + (r < live ? r : 0) * p.c.c_l, r < live);
-        }
-        if (lane < 4) {
-          const int j = min(row0 + 16 * (lane & 1), w.whole - 1) >> p.c.shift;
-          cp4(to + A8_STAGE + 4 * lane, p.c.scales + w.b * p.c.s_b + w.h * p.c.s_h + (int64_t)j * p.c.s_j + (lane >> 1) * p.c.s_kv);
-        }
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  Way8 ahead = way;
-  int slot = 0;
-#pragma unroll
-  for (int i = 0; i < A8_STAGES - 1; i++) {
-    if (ahead.left > 0) load(ahead, i), ahead.step(p);
-    else asm volatile("cp.async.commit_group;" ::: "memory");
-  }
+  const unsigned base = smem_addr(dyn8), mine = A8<ROWS>::q_bytes + warp * 2 * A8_SLOT, q_off = (ROWS == 8 ? 8 : 16) * lane;   // offsets in the block's shared memory
   const int n_rows_all = p.T * p.G, Hq = p.c.H * p.G;
-  while (way.left > 0) {
-    // ---- a segment: consecutive tiles of one item ----
-    const int b = way.b, h = way.h, group = way.group, seg_first = way.tile;
-    const bool whole_item = way.tile == 0 && way.left >= way.n;
-    const int n_rows = min(A8_ROWS, n_rows_all - group * A8_ROWS);
-    uint32_t qa[8][4];
-    float factor[2];   // of the scores of codes: what the query row was scaled by, and log2 e / sqrt d
-    int last[2];       // the last row that a query row sees
-    const uint16_t* q_row[2];
+  for (; way.left > 0; way.next(p)) {
+    // ---- a segment ----
+    const int b = way.b, h = way.h, group = way.group, whole = way.whole, count = way.count();
+    const bool whole_item = count == way.n;
+    const int coded = (whole + A8_TILE - 1) / A8_TILE;                          // tiles of codes of the item
+    const int n_coded = max(0, min(coded, way.tile + count) - way.tile);        // of the segment
+    const bool recent = way.len > whole && way.tile + count == way.n;
+    const int n_rows = min(ROWS, n_rows_all - group * ROWS);
+    int row0 = way.tile * A8_TILE + 32 * warp;
+    // A step's 32 rows on their way.  A chunk of 16 bytes lies where its row's number moves it, so that the reads below fall into all banks.
+    const int ck = lane & 7, ckv = lane >> 3 & 1, odd = lane >> 4;
+    const uint8_t* src = p.c.codes + b * p.c.c_b + h * p.c.c_h + ckv * p.c.c_kv + (int64_t)(row0 + odd) * p.c.c_l + ck * 16;
+    const float* scales = p.c.scales + b * p.c.s_b + h * p.c.s_h + (lane >> 1 & 1) * p.c.s_kv;
+    auto load = [&](int slot) {
+      const unsigned to = base + mine + slot * A8_SLOT, chunk = to + ckv * 4096 + odd * 128;
+      const int live = whole - row0;
+      if (live >= 32) {
+        const uint8_t* from = src;
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-      const int r = group * A8_ROWS + min(8 * e + g, n_rows - 1), t = r / p.G;
-      last[e] = p.lengths[b] > p.c.cap ? (int)p.c.cap - p.T + t : p.lengths[b] - p.T + t;
-      q_row[e] = p.q + b * p.q_b + (int64_t)t * p.q_t + (int64_t)(h * p.G + r % p.G) * p.q_h + 32 * t4;
-      uint4 x[4];
+        for (int i = 0; i < 16; i++, from += 2 * p.c.c_l) cp16(chunk + i * 256 + ((ck ^ (ckv ? (2 * i) & 6 : odd)) << 4), from);
+      } else if (live > 0) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) x[i] = *reinterpret_cast<const uint4*>(q_row[e] + 8 * i);
-      const uint32_t* xw = reinterpret_cast<const uint32_t*>(x);
+        for (int i = 0; i < 16; i++) cp16(chunk + i * 256 + ((ck ^ (ckv ? (2 * i) & 6 : odd)) << 4), 2 * i + odd < live ? src + 2 * i * p.c.c_l : src - odd * p.c.c_l, 2 * i + odd < live);
+      }
+      if (lane < 4 && live > 0) cp4(to + A8_STAGE + 4 * lane, scales + (int64_t)(min(row0 + 16 * (lane & 1), whole - 1) >> p.c.shift) * p.c.s_j);
+      cp_commit();
+      src += A8_TILE * p.c.c_l, row0 += A8_TILE;
+    };
+    if (n_coded > 0) load(0);
+    // queries: as they are, and as fp16 after a power of two per row in the order in which a lane needs them as operands; eight threads a row
+#pragma unroll 1
+    for (int r0 = 0; r0 < ROWS; r0 += 16) {
+      const int row = r0 + (tid >> 3), c = tid & 7;   // 16 channels from 16 c on
+      const int r = group * ROWS + min(row, n_rows - 1);
+      const uint4* from = reinterpret_cast<const uint4*>(p.q + b * p.q_b + (int64_t)(r / p.G) * p.q_t + (int64_t)(h * p.G + r % p.G) * p.q_h + 16 * c);
+      const uint4 x[2] = {from[0], from[1]};
+      const uint32_t xw[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
       uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < 16; i++) top = __vmaxu2(top, xw[i] & 0x7fff7fffu);
+      for (int i = 0; i < 8; i++) top = __vmaxu2(top, xw[i] & 0x7fff7fffu);
       top = max(top & 0xffffu, top >> 16);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+#pragma unroll
+      for (int off = 1; off < 8; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
       // the largest of the row becomes a number from 1 to 2; a row with an infinity or NaN becomes NaN
       const unsigned ex = max(min(top >> 7, 252u), 2u);
       const bool fine = top < 0x7f80u;
       const float up = fine ? __uint_as_float((254u - ex) << 23) : NAN;
+      if (row < ROWS) {
+        if (c == 0) s_factor[row] = fine ? __uint_as_float(ex << 23) * p.scale_log2 : NAN;
+        uint4* raw = reinterpret_cast<uint4*>(dyn8 + ROWS * 256 + row * A8_QS + 32 * c);
+        raw[0] = x[0], raw[1] = x[1];
 #pragma unroll
-      for (int i = 0; i < 16; i++)   // word i: channels 2 i, 2 i + 1 of this lane's 32
-        qa[i >> 1][2 * (i & 1) + e] = half2_of(__uint_as_float(xw[i] << 16) * up, __uint_as_float(xw[i] & 0xffff0000u) * up);
-      factor[e] = fine ? __uint_as_float(ex << 23) * p.scale_log2 : NAN;
-    }
-    if (E4M3) factor[0] *= 256.0f, factor[1] *= 256.0f;
-    float o[16][4] = {};
-    RowState st[2];
-#pragma unroll
-    for (int e = 0; e < 2; e++) st[e] = {-INFINITY, 0.0f, 0.0f, 1.0f, 1.0f};
-    bool end = false;
-    unsigned at;
-    do {
-      if (ahead.left > 0) load(ahead, (slot + A8_STAGES - 1) % A8_STAGES), ahead.step(p);
-      else asm volatile("cp.async.commit_group;" ::: "memory");
-      asm volatile("cp.async.wait_group %0;" ::"n"(A8_STAGES - 1) : "memory");
-      __syncwarp();
-      at = mine + slot * A8_SLOT;
-      const int live = way.live(warp), row0 = way.row0(warp);
-      if (live > 0 && !way.recent()) {
-        float ks[2], vs2[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) ks[i] = lds4(at + A8_STAGE + 4 * i), vs2[i] = lds4(at + A8_STAGE + 8 + 4 * i);
-        float x[2][8], vs[8];
-#pragma unroll
-        for (int nt = 0; nt < 4; nt++) {
-          const int key = 8 * nt + g;
-          const uint4 w0 = lds16(at + key * 128 + (((2 * t4) ^ (key & 1)) << 4)), w1 = lds16(at + key * 128 + (((2 * t4 + 1) ^ (key & 1)) << 4));
-          const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-          float acc[2][4] = {};
-#pragma unroll
-          for (int s = 0; s < 8; s++) {
-            const uint32_t c = biased<E4M3>(w[s]);
-            mma_f16(acc[s & 1], qa[s], halves<E4M3, 0>(c), halves<E4M3, 1>(c));
+        for (int k = 0; k < 4; k++) {
+          const float f[4] = {__uint_as_float(xw[2 * k] << 16) * up, __uint_as_float(xw[2 * k] & 0xffff0000u) * up, __uint_as_float(xw[2 * k + 1] << 16) * up,
+                              __uint_as_float(xw[2 * k + 1] & 0xffff0000u) * up};
+          const uint32_t lo = half2_of(f[0], f[E4M3 ? 1 : 2]), hi = half2_of(f[E4M3 ? 2 : 1], f[3]);
+          const int s = 4 * (c & 1) + k, of = 4 * (row & 7) + (c >> 1);   // the lane that it is for
+          if (ROWS == 8) {
+            *reinterpret_cast<uint2*>(dyn8 + s * 256 + of * 8) = make_uint2(lo, hi);
+          } else {   // a0, a1 rows g and g + 8 of the first pair of channels, a2, a3 of the second
+            uint32_t* to = reinterpret_cast<uint32_t*>(dyn8 + ((row >> 4) * 8 + s) * 512 + of * 16) + (row >> 3 & 1);
+            to[0] = lo, to[2] = hi;
           }
-#pragma unroll
-          for (int i = 0; i < 4; i++) x[i >> 1][2 * nt + (i & 1)] = (acc[0][i] + acc[1][i]) * ks[nt >> 1];
-          vs[2 * nt] = vs[2 * nt + 1] = vs2[nt >> 1];
         }
-        const int lim = min(last[0], last[1]);
-        if (__any_sync(0xffffffffu, live < 32 || row0 + 31 > lim)) {
+      }
+    }
+    __syncthreads();
+    float o[MT][16][4] = {};
+    RowState st[NR];
+    float factor[NR];   // log2 e / sqrt d, and what the row was scaled by
+    int last[NR];       // the last row that a query row sees
+    const int end = (p.lengths[b] > p.c.cap ? (int)p.c.cap : p.lengths[b]) - p.T;
 #pragma unroll
-          for (int e = 0; e < 2; e++)
+    for (int e = 0; e < NR; e++) {
+      st[e] = {-INFINITY, 0.0f, 0.0f, 1.0f, 1.0f};
+      factor[e] = s_factor[8 * e + g];
+      last[e] = end + (group * ROWS + min(8 * e + g, n_rows - 1)) / p.G;
+    }
+    const int lim = min(end + group * ROWS / p.G, whole - 1);   // rows up to here are seen by all
+    unsigned at = mine;
+    for (int j = 0; j < n_coded; j++) {
+      const int first = row0 - A8_TILE;   // of this step; `load` is a step ahead
+      at = mine + (j & 1) * A8_SLOT;
+      if (j + 1 < n_coded) {
+        load((j + 1) & 1);
+        cp_wait<1>();
+      } else {
+        row0 += A8_TILE;
+        cp_wait<0>();
+      }
+      if (first >= whole) continue;
+      float s[MT][4][4];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-              const int r = 8 * (i >> 1) + 2 * t4 + (i & 1);
-              if (r >= live || row0 + r > last[e]) x[e][i] = -INFINITY;
-            }
+      for (int half = 0; half < 2; half++) {   // 16 rows of K at a time
+        uint4 kw[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const unsigned from = at + (8 * (2 * half + i) + g) * 128;
+          kw[i][0] = lds16(from + (((2 * t4) ^ (g & 1)) << 4)), kw[i][1] = lds16(from + (((2 * t4 + 1) ^ (g & 1)) << 4));
         }
-        weigh<8>(st, o, x, vs, factor);
 #pragma unroll
-        for (int ks2 = 0; ks2 < 2; ks2++) {
-          uint32_t pa[4];
+        for (int mt = 0; mt < MT; mt++)
 #pragma unroll
           for (int i = 0; i < 2; i++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) pa[2 * i + e] = half2_of(x[e][4 * ks2 + 2 * i], x[e][4 * ks2 + 2 * i + 1]);
-          uint32_t v[4][4];
+            for (int c = 0; c < 4; c++) s[mt][2 * half + i][c] = 0.0f;
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int key = 16 * ks2 + 8 * (i >> 1) + 2 * t4 + (i & 1);
-            const uint4 w = lds16(at + 4096 + key * 128 + ((g ^ (key & 6)) << 4));
-            v[i][0] = w.x, v[i][1] = w.y, v[i][2] = w.z, v[i][3] = w.w;
-          }
+        for (int ks = 0; ks < 8; ks++) {
+          uint32_t q[MT][4];
 #pragma unroll
-          for (int wd = 0; wd < 4; wd++) {
-            uint32_t pr[2][2];   // [rows of the first or second eight][channels 0, 1 or 2, 3 of the word]: two rows' codes of a channel side by side
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-              const uint32_t a = biased<E4M3>(v[2 * i][wd]), c = biased<E4M3>(v[2 * i + 1][wd]);
-              pr[i][0] = __byte_perm(a, c, 0x5140), pr[i][1] = __byte_perm(a, c, 0x7362);
+          for (int mt = 0; mt < MT; mt++) {
+            if (ROWS == 8) {
+              const uint2 x = lds8(q_off + ks * 256);
+              q[mt][0] = x.x, q[mt][1] = 0, q[mt][2] = x.y, q[mt][3] = 0;
+            } else {
+              const uint4 x = lds16(q_off + (mt * 8 + ks) * 512);
+              q[mt][0] = x.x, q[mt][1] = x.y, q[mt][2] = x.z, q[mt][3] = x.w;
             }
-            mma_f16(o[4 * wd], pa, halves<E4M3, 0>(pr[0][0]), halves<E4M3, 0>(pr[1][0]));
-            mma_f16(o[4 * wd + 1], pa, halves<E4M3, 1>(pr[0][0]), halves<E4M3, 1>(pr[1][0]));
-            mma_f16(o[4 * wd + 2], pa, halves<E4M3, 0>(pr[0][1]), halves<E4M3, 0>(pr[1][1]));
-            mma_f16(o[4 * wd + 3], pa, halves<E4M3, 1>(pr[0][1]), halves<E4M3, 1>(pr[1][1]));
+          }
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const uint4 v = kw[i][ks >> 2];
+            const uint32_t w = (ks & 3) == 0 ? v.x : (ks & 3) == 1 ? v.y : (ks & 3) == 2 ? v.z : v.w;
+            const uint32_t b0 = codes_lo<E4M3>(w), b1 = codes_hi<E4M3>(w);
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) mma_f16(s[mt][2 * half + i], q[mt][0], q[mt][1], q[mt][2], q[mt][3], b0, b1);
           }
         }
-      } else if (live > 0) {
-        // ---- 16 rows in bf16 ----
-        float x[2][4];
-        const float raw[2] = {p.scale_log2 / factor[0], p.scale_log2 / factor[1]};   // scores in the units of the codes' ones
+      }
+      float4 sc;   // scales: K of the first and second 16 rows, V of them
+      {
+        const uint4 x = lds16(at + A8_STAGE);
+        sc = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
+      }
+      uint32_t pa[MT][2][4];   // weights as operands: [16 rows of V]
 #pragma unroll
-        for (int nt = 0; nt < 2; nt++) {
-          float acc[4] = {};
+      for (int e = 0; e < NR; e++) {
+        RowState& r = st[e];
+        float (&a)[4][4] = s[e / RPT];
+        const int c = 2 * (e % RPT);
+        const float kf[2] = {sc.x * factor[e], sc.y * factor[e]}, vs[2] = {sc.z, sc.w};
+        float w[4][2], f;
+        if (first + 31 <= lim) {
+          // the largest of 16 rows, which share a scale, is scaled once; so is the largest weight of them
+          const float t0 = quad_max(fmaxf(fmaxf(a[0][c], a[0][c + 1]), fmaxf(a[1][c], a[1][c + 1]))) * kf[0];
+          const float t1 = quad_max(fmaxf(fmaxf(a[2][c], a[2][c + 1]), fmaxf(a[3][c], a[3][c + 1]))) * kf[1];
+          const float m = fmaxf(r.m, fmaxf(t0, t1)), least = m == -INFINITY ? 0.0f : m;
+          f = move(r, m, fmaxf(ex2(t0 - least) * vs[0], ex2(t1 - least) * vs[1]));
+          float sum = 0.0f;
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const uint4 w = lds16(at + (8 * nt + g) * 256 + t4 * 64 + i * 16);
-            const uint4 a = *reinterpret_cast<const uint4*>(q_row[0] + 8 * i), c = *reinterpret_cast<const uint4*>(q_row[1] + 8 * i);
-            const uint32_t f0[4] = {a.x, c.x, a.y, c.y}, f1[4] = {a.z, c.z, a.w, c.w};
-            mma_bf16(acc, f0, w.x, w.y);
-            mma_bf16(acc, f1, w.z, w.w);
+            const float y0 = ex2(fmaf(a[i][c], kf[i >> 1], -least)), y1 = ex2(fmaf(a[i][c + 1], kf[i >> 1], -least)), v = vs[i >> 1] * r.up;
+            sum += y0 + y1;
+            w[i][0] = y0 * v, w[i][1] = y1 * v;
           }
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int r = 8 * nt + 2 * t4 + (i & 1), e = i >> 1;
-            x[e][2 * nt + (i & 1)] = r < live && row0 + r <= last[e] ? acc[i] * raw[e] : -INFINITY;
-          }
-        }
-        const float one = E4M3 ? 0.00390625f : 1.0f;   // O of e4m3 codes is kept as 2^-8 of what it stands for
-        const float vs[4] = {one, one, one, one};
-        weigh<4>(st, o, x, vs, factor);
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const float a = x[e][2 * i], c = x[e][2 * i + 1];
-            const uint32_t w = pack2(a, c);
-            hi[2 * i + e] = w;
-            lo[2 * i + e] = pack2(a - __uint_as_float(w << 16), c - __uint_as_float(w & 0xffff0000u));
-          }
-        uint32_t v[4][8];
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int key = 8 * (i >> 1) + 2 * t4 + (i & 1);
-          const uint4 w0 = lds16(at + 4096 + key * 256 + g * 32), w1 = lds16(at + 4096 + key * 256 + g * 32 + 16);
-          v[i][0] = w0.x, v[i][1] = w0.y, v[i][2] = w0.z, v[i][3] = w0.w, v[i][4] = w1.x, v[i][5] = w1.y, v[i][6] = w1.z, v[i][7] = w1.w;
-#pragma unroll
-          for (int k = 0; k < 8; k++) bad |= not_finite(v[i][k]) | not_finite(v[i][k] >> 16);
-        }
-        bad = __any_sync(0xffffffffu, bad);
-        if (bad) {   // a weight of zero does not keep what is not a number out of a product: it is taken out, and given to the query rows that see it
+          r.l += sum;
+        } else {
+          float x[4][2], m = r.m, top = 0.0f, sum = 0.0f;
+          bool seen[4][2];
 #pragma unroll
           for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[i][k] = (not_finite(v[i][k]) ? 0 : v[i][k] & 0xffffu) | (not_finite(v[i][k] >> 16) ? 0 : v[i][k] & 0xffff0000u);
+            for (int k = 0; k < 2; k++) {
+              const int row = first + 8 * i + 2 * t4 + k;
+              seen[i][k] = row < whole && row <= last[e];
+              x[i][k] = a[i][c + k] * kf[i >> 1];
+              if (seen[i][k]) m = fmaxf(m, x[i][k]);
+            }
+          m = quad_max(m);
+          const float least = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              x[i][k] = seen[i][k] ? ex2(x[i][k] - least) : 0.0f;
+              sum += x[i][k];
+              w[i][k] = seen[i][k] ? x[i][k] * vs[i >> 1] : 0.0f;   // (the scale of a block that it does not see may be NaN)
+              top = fmaxf(top, w[i][k]);
+            }
+          f = move(r, m, quad_max(top));
+          r.l += sum;
+#pragma unroll
+          for (int i = 0; i < 4; i++) w[i][0] *= r.up, w[i][1] *= r.up;
         }
+        if (__any_sync(0xffffffffu, f != 1.0f)) scale_rows(o[e / RPT], e % RPT, f);
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-          const uint32_t b0 = __byte_perm(v[0][k], v[1][k], 0x5410), b1 = __byte_perm(v[2][k], v[3][k], 0x5410), c0 = __byte_perm(v[0][k], v[1][k], 0x7632),
-                         c1 = __byte_perm(v[2][k], v[3][k], 0x7632);
-          mma_bf16(o[2 * k], hi, b0, b1);
-          mma_bf16(o[2 * k], lo, b0, b1);
-          mma_bf16(o[2 * k + 1], hi, c0, c1);
-          mma_bf16(o[2 * k + 1], lo, c0, c1);
-        }
-        if (bad) {
-          for (int r = 0; r < live; r++)
+        for (int i = 0; i < 4; i++) pa[e / RPT][i >> 1][2 * (i & 1) + e % RPT] = half2_of(w[i][0], w[i][1]);
+        if (RPT == 1) pa[0][0][1] = pa[0][0][3] = pa[0][1][1] = pa[0][1][3] = 0;
+      }
 #pragma unroll
-            for (int n = 0; n < 16; n++)
+      for (int half = 0; half < 2; half++) {
+        uint4 v[4];   // rows 2 t4, 2 t4 + 1, and eight further; channels 16 g ..
 #pragma unroll
-              for (int i = 0; i < 2; i++) {   // column n of the two n-tile columns 2 t4, 2 t4 + 1 of this lane: channel 32 t4 + 16 i + n
-                uint16_t w;
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(at + 4096 + r * 256 + 2 * (32 * t4 + 16 * i + n)) : "memory");
-                if (not_finite(w)) {
-                  if (row0 + r <= last[0]) o[n][i] += bf2f(w);
-                  if (row0 + r <= last[1]) o[n][2 + i] += bf2f(w);
-                }
-              }
+        for (int i = 0; i < 4; i++) v[i] = lds16(at + 4096 + (16 * half + 8 * (i >> 1) + 2 * t4 + (i & 1)) * 128 + ((g ^ (2 * t4)) << 4));
+#pragma unroll
+        for (int wd = 0; wd < 4; wd++) {
+          auto word = [&](int i) { return wd == 0 ? v[i].x : wd == 1 ? v[i].y : wd == 2 ? v[i].z : v[i].w; };
+          const uint32_t a0 = pair01<E4M3>(word(0), word(1)), a1 = pair01<E4M3>(word(2), word(3)), c0 = pair23<E4M3>(word(0), word(1)), c1 = pair23<E4M3>(word(2), word(3));
+          const uint32_t bs[4][2] = {{codes_lo<E4M3>(a0), codes_lo<E4M3>(a1)}, {codes_hi<E4M3>(a0), codes_hi<E4M3>(a1)}, {codes_lo<E4M3>(c0), codes_lo<E4M3>(c1)},
+                                     {codes_hi<E4M3>(c0), codes_hi<E4M3>(c1)}};
+#pragma unroll
+          for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) mma_f16(o[mt][4 * wd + i], pa[mt][half][0], pa[mt][half][1], pa[mt][half][2], pa[mt][half][3], bs[i][0], bs[i][1]);
         }
       }
       __syncwarp();
-      end = way.last_of_item();
-      way.step(p);
-      slot = (slot + 1) % A8_STAGES;
-    } while (!end);
+    }
+    if (recent) {
+      // ---- the rows behind the last whole block, 16 bf16 rows of this warp at a time.  Weights are two bf16 numbers each. ----
+      at = mine;
+#pragma unroll 1
+      for (int sub = 0; sub < 2; sub++) {
+        const int r0 = whole + 32 * warp + 16 * sub, live = min(16, way.len - r0);
+        if (live <= 0) break;
+        const int kv = lane >> 4;
+        const uint16_t* ring = p.c.recent + b * p.c.r_b + h * p.c.r_h + kv * p.c.r_kv + (lane & 15) * 8;
+#pragma unroll 4
+        for (int i = 0; i < 16; i++) cp16(base + at + kv * 4096 + i * 256 + (lane & 15) * 16, ring + (int64_t)((i < live ? r0 + i : r0) % p.c.R) * p.c.r_l, i < live);
+        cp_commit();
+        cp_wait<0>();
+        float x[NR][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+          for (int nt = 0; nt < 2; nt++) {
+            float acc[4] = {};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const unsigned q = ROWS * 256 + (16 * mt + g) * A8_QS + t4 * 64 + i * 16;
+              const uint4 w = lds16(at + (8 * nt + g) * 256 + t4 * 64 + i * 16), a = lds16(q), c = RPT == 2 ? lds16(q + 8 * A8_QS) : make_uint4(0, 0, 0, 0);
+              mma_bf16(acc, a.x, c.x, a.y, c.y, w.x, w.y);
+              mma_bf16(acc, a.z, c.z, a.w, c.w, w.z, w.w);
+            }
+#pragma unroll
+            for (int e = 0; e < RPT; e++) x[RPT * mt + e][2 * nt] = acc[2 * e], x[RPT * mt + e][2 * nt + 1] = acc[2 * e + 1];
+          }
+        uint32_t hi[MT][4] = {}, lo[MT][4] = {};
+#pragma unroll
+        for (int e = 0; e < NR; e++) {
+          RowState& r = st[e];
+          float m = r.m, top = 0.0f, sum = 0.0f;
+          bool seen[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int row = 8 * (i >> 1) + 2 * t4 + (i & 1);
+            seen[i] = row < live && r0 + row <= last[e];
+            x[e][i] *= factor[e] != factor[e] ? NAN : p.scale_log2;
+            if (seen[i]) m = fmaxf(m, x[e][i]);
+          }
+          m = quad_max(m);
+          const float least = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            x[e][i] = seen[i] ? ex2(x[e][i] - least) : 0.0f;
+            sum += x[e][i], top = fmaxf(top, x[e][i]);
+          }
+          const float f = move(r, m, quad_max(top));
+          r.l += sum;
+          if (__any_sync(0xffffffffu, f != 1.0f)) scale_rows(o[e / RPT], e % RPT, f);
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const float a = x[e][2 * i] * r.up, c = x[e][2 * i + 1] * r.up;
+            const uint32_t w = pack2(a, c);
+            hi[e / RPT][2 * i + e % RPT] = w;
+            lo[e / RPT][2 * i + e % RPT] = pack2(a - __uint_as_float(w << 16), c - __uint_as_float(w & 0xffff0000u));
+          }
+        }
+        // A weight of zero does not keep what is not a number out of a product: it is taken out, and given to the query rows that see it.
+        bool bad = false;
+#pragma unroll 1
+        for (int i = lane; i < 256; i += 32) {
+          const uint4 w = lds16(at + 4096 + i * 16);
+          uint32_t v[4] = {w.x, w.y, w.z, w.w};
+          bool mine_bad = false;
+#pragma unroll
+          for (int k = 0; k < 4; k++) mine_bad |= not_finite(v[k]) | not_finite(v[k] >> 16);
+          bad |= mine_bad;
+        }
+        bad = __any_sync(0xffffffffu, bad);
+        if (bad) {
+#pragma unroll 1
+          for (int row = 0; row < live; row++)
+#pragma unroll
+            for (int n = 0; n < 16; n++)
+#pragma unroll
+              for (int i = 0; i < 2; i++) {   // column n of the tile columns 2 t4, 2 t4 + 1 of this lane: channel 32 t4 + 16 i + n
+                uint16_t w;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(base + at + 4096 + row * 256 + 2 * (32 * t4 + 16 * i + n)) : "memory");
+                if (not_finite(w)) {
+#pragma unroll
+                  for (int e = 0; e < NR; e++)
+                    if (r0 + row <= last[e]) o[e / RPT][n][2 * (e % RPT) + i] += bf2f(w);
+                }
+              }
+          __syncwarp();
+#pragma unroll 1
+          for (int i = lane; i < 1024; i += 32) {
+            uint32_t v;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(base + at + 4096 + i * 4) : "memory");
+            v = (not_finite(v) ? 0 : v & 0xffffu) | (not_finite(v >> 16) ? 0 : v & 0xffff0000u);
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + at + 4096 + i * 4), "r"(v) : "memory");
+          }
+          __syncwarp();
+        }
+#pragma unroll
+        for (int part = 0; part < 2; part++) {
+          uint4 v[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) v[i] = lds16(at + 4096 + (8 * (i >> 1) + 2 * t4 + (i & 1)) * 256 + g * 32 + 16 * part);
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            auto word = [&](int i) { return k == 0 ? v[i].x : k == 1 ? v[i].y : k == 2 ? v[i].z : v[i].w; };
+            const uint32_t b0 = __byte_perm(word(0), word(1), 0x5410), b1 = __byte_perm(word(2), word(3), 0x5410), c0 = __byte_perm(word(0), word(1), 0x7632),
+                           c1 = __byte_perm(word(2), word(3), 0x7632);
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+              float (&x0)[4] = o[mt][8 * part + 2 * k], (&x1)[4] = o[mt][8 * part + 2 * k + 1];
+              mma_bf16(x0, hi[mt][0], hi[mt][1], hi[mt][2], hi[mt][3], b0, b1);
+              mma_bf16(x0, lo[mt][0], lo[mt][1], lo[mt][2], lo[mt][3], b0, b1);
+              mma_bf16(x1, hi[mt][0], hi[mt][1], hi[mt][2], hi[mt][3], c0, c1);
+              mma_bf16(x1, lo[mt][0], lo[mt][1], lo[mt][2], lo[mt][3], c0, c1);
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
     // ---- the four warps' shares of the segment ----
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
+    for (int e = 0; e < NR; e++) {
       st[e].l += __shfl_xor_sync(0xffffffffu, st[e].l, 1);
       st[e].l += __shfl_xor_sync(0xffffffffu, st[e].l, 2);
-      if (t4 == 0) s_m[warp][8 * e + g] = st[e].m == -INFINITY ? -INFINITY : st[e].m * factor[e], s_l[warp][8 * e + g] = st[e].l, s_u[warp][8 * e + g] = st[e].down * (E4M3 ? 256.0f : 1.0f);
+      if (t4 == 0) s_m[warp][8 * e + g] = st[e].m, s_l[warp][8 * e + g] = st[e].l;
     }
     __syncthreads();
-    float* rec = whole_item ? nullptr : p.records + (2 * (int64_t)blockIdx.x + (seg_first == 0)) * (A8_ROWS * 130);
-    const unsigned part = at - smem_addr(dyn);   // the stage of the segment's last step: the same of every warp
-    float* to = reinterpret_cast<float*>(dyn + part) + g * A8_OS + 32 * t4;
+    float* parts = reinterpret_cast<float*>(dyn8 + A8<ROWS>::q_bytes);   // a warp's first stage
+    float* to = parts + warp * 2 * A8_SLOT / 4 + g * A8_OS + A8_OT * t4;
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
+    for (int e = 0; e < NR; e++) {
       if (8 * e < n_rows) {
         const int r = 8 * e + g;
         const float M = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-        const float f = s_m[warp][r] == -INFINITY ? 0.0f : ex2(s_m[warp][r] - M);
+        const float f = st[e].m == -INFINITY ? 0.0f : ex2(st[e].m - M) * st[e].down;
+        const int c = 2 * (e % RPT);
+        float (&x)[16][4] = o[e / RPT];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-          for (int n = 0; n < 16; n += 4)
-            *reinterpret_cast<float4*>(to + 16 * i + n) = make_float4(o[n][2 * e + i] * f * s_u[warp][r], o[n + 1][2 * e + i] * f * s_u[warp][r], o[n + 2][2 * e + i] * f * s_u[warp][r],
-                                                                       o[n + 3][2 * e + i] * f * s_u[warp][r]);
+        for (int n = 0; n < 16; n += 4) {
+          *reinterpret_cast<float4*>(to + n) = make_float4(x[n][c] * f, x[n + 1][c] * f, x[n + 2][c] * f, x[n + 3][c] * f);
+          *reinterpret_cast<float4*>(to + 16 + n) = make_float4(x[n][c + 1] * f, x[n + 1][c + 1] * f, x[n + 2][c + 1] * f, x[n + 3][c + 1] * f);
+        }
       }
       __syncthreads();
-      if (8 * e < n_rows) {
+      const int row = 8 * e + (tid >> 4), c = 8 * (tid & 15);   // 16 threads a row
+      if (row < n_rows) {
+        const float M = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+        float L = 0.0f, O[8] = {};
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const int row = 8 * e + i;
-          if (row < n_rows) {
-            const float M = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
-            float L = 0.0f, O = 0.0f;
+        for (int w = 0; w < 4; w++) {
+          L += s_l[w][row] * (s_m[w][row] == -INFINITY ? (s_l[w][row] == 0.0f ? 0.0f : 1.0f) : ex2(s_m[w][row] - M));   // (all NaN: the sum is NaN and stays)
+          const float4* from = reinterpret_cast<const float4*>(parts + w * 2 * A8_SLOT / 4 + (tid >> 4) * A8_OS + (c >> 5) * A8_OT + (c & 31));
+          const float4 x = from[0], y = from[1];
+          O[0] += x.x, O[1] += x.y, O[2] += x.z, O[3] += x.w, O[4] += y.x, O[5] += y.y, O[6] += y.z, O[7] += y.w;
+        }
+        if (whole_item) {
+          const int rr = group * ROWS + row, t = rr / p.G, hq = h * p.G + rr % p.G;
+          const int64_t out_row = ((int64_t)b * p.T + t) * Hq + hq;
+          uint32_t w[4];
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
-              L += s_l[w][row] * (s_m[w][row] == -INFINITY ? (s_l[w][row] == 0.0f ? 0.0f : 1.0f) : ex2(s_m[w][row] - M));   // (all NaN: the sum is NaN and stays)
-              O += reinterpret_cast<const float*>(dyn + (part % (A8_STAGES * A8_SLOT)) + w * A8_STAGES * A8_SLOT)[i * A8_OS + tid];
-            }
-            const int rr = group * A8_ROWS + row, t = rr / p.G, hq = h * p.G + rr % p.G;
-            if (whole_item) {
-              const int64_t out_row = ((int64_t)b * p.T + t) * Hq + hq;
-              p.out[out_row * 128 + tid] = f2bf(L == 0.0f ? 0.0f : O / L);
-              if (p.lse && tid == 0) p.lse[out_row] = L == 0.0f ? -INFINITY : M + log2f(L);
-            } else {
-              rec[row * 128 + tid] = O;
-              if (tid == 0) rec[A8_ROWS * 128 + row] = M, rec[A8_ROWS * 129 + row] = L;
-            }
+          for (int i = 0; i < 4; i++) w[i] = pack2(L == 0.0f ? 0.0f : O[2 * i] / L, L == 0.0f ? 0.0f : O[2 * i + 1] / L);
+          *reinterpret_cast<uint4*>(p.out + out_row * 128 + c) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (p.lse && c == 0) p.lse[out_row] = L == 0.0f ? -INFINITY : M + log2f(L);
+        } else {
+          float4* rec = reinterpret_cast<float4*>(p.records + (2 * (int64_t)blockIdx.x + (way.tile == 0)) * (ROWS * 130) + row * 128 + c);
+          rec[0] = make_float4(O[0], O[1], O[2], O[3]), rec[1] = make_float4(O[4], O[5], O[6], O[7]);
+          if (c == 0) {
+            float* tail = p.records + (2 * (int64_t)blockIdx.x + (way.tile == 0)) * (ROWS * 130) + ROWS * 128 + row;
+            tail[0] = M, tail[ROWS] = L;
           }
         }
       }
@@ -466,6 +556,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS) attend8_kernel(const __gr
 }
 
 // A block per query row: the records of the blocks that share its item, in the order of the tiles.
+template <int ROWS>
 __global__ void __launch_bounds__(128) attend8_merge_kernel(const __grid_constant__ Attend8 p, int blocks) {
   pdl_wait();
   pdl_trigger();
@@ -481,27 +572,28 @@ __global__ void __launch_bounds__(128) attend8_merge_kernel(const __grid_constan
     total += items * __reduce_add_sync(0xffffffffu, tiles), before += items * __reduce_add_sync(0xffffffffu, b0 + lane < b ? tiles : 0);
   }
   const int n = tiles8(p, len8(p, b));
-  const int64_t first = before + ((int64_t)h * p.row_groups + r / A8_ROWS) * n;
+  const int64_t first = before + ((int64_t)h * p.row_groups + r / ROWS) * n;
   const unsigned shares = (unsigned)min((int64_t)blocks, total);
   const int c0 = share_owner(first, total, shares), c1 = share_owner(first + n - 1, total, shares);
   if (c0 == c1) return;   // written by its block
-  merge_row(shared, c1 - c0 + 1, A8_ROWS, r % A8_ROWS, [&](int i) { return p.records + (2 * (int64_t)(c0 + i) + (i == 0)) * (A8_ROWS * 130); }, p.out + row * 128,
+  merge_row(shared, c1 - c0 + 1, ROWS, r % ROWS, [&](int i) { return p.records + (2 * (int64_t)(c0 + i) + (i == 0)) * (ROWS * 130); }, p.out + row * 128,
             p.lse ? p.lse + row : nullptr);
 }
 
-template <bool E4M3>
-int launch(const Attend8& p, cudaStream_t st) {
-  const int64_t slots = (int64_t)A8_CTAS * sm_count(), most = (int64_t)p.bs * p.c.H * p.row_groups * ((p.c.cap + A8_TILE - 1) / A8_TILE + 1);
+template <bool E4M3, int ROWS>
+int launch(Attend8 p, cudaStream_t st) {
+  p.row_groups = (p.T * p.G + ROWS - 1) / ROWS;
+  const int64_t slots = (int64_t)A8<ROWS>::ctas * sm_count(), most = (int64_t)p.bs * p.c.H * p.row_groups * ((p.c.cap + A8_TILE - 1) / A8_TILE + 1);
   const int blocks = (int)(most < slots ? most : slots);
   static PerDevice opted;
   if (const unsigned long long bit = first_on_device(opted)) {
-    if (cudaFuncSetAttribute(attend8_kernel<E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, A8_SMEM) != cudaSuccess)
+    if (cudaFuncSetAttribute(attend8_kernel<E4M3, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, A8<ROWS>::smem) != cudaSuccess)
       return fail(PK_ERR_CUDA, "cache8_attention: %s", cudaGetErrorString(cudaGetLastError()));
     mark_on_device(opted, bit);
   }
   StageTimer timer(ST_ATTENTION, st);
-  launch_chain(attend8_kernel<E4M3>, dim3((unsigned)blocks), dim3(A8_THREADS), A8_SMEM, st, p);
-  launch_chain(attend8_merge_kernel, dim3((unsigned)((int64_t)p.bs * p.T * p.c.H * p.G)), dim3(128), 0, st, p, blocks);
+  launch_chain(attend8_kernel<E4M3, ROWS>, dim3((unsigned)blocks), dim3(A8_THREADS), A8<ROWS>::smem, st, p);
+  launch_chain(attend8_merge_kernel<ROWS>, dim3((unsigned)((int64_t)p.bs * p.T * p.c.H * p.G)), dim3(128), 0, st, p, blocks);
   return check_launch("cache8_attention", 2);
 }
 
@@ -512,7 +604,8 @@ using namespace pk;
 
 extern "C" int64_t pk_cache8_attention_workspace_bytes(int64_t bs, int64_t T, int64_t Hq, int64_t H, int64_t cap) {
   if (bs < 1 || T < 1 || T > 256 || H < 1 || Hq < H || cap < 0) return 0;
-  return 2 * (int64_t)A8_CTAS * sm_count() * A8_ROWS * 130 * 4;
+  const int rows = T * (Hq / H) <= 8 ? 8 : T * (Hq / H) <= 16 ? 16 : 32;
+  return 2 * (int64_t)(rows == 32 ? A8<32>::ctas : A8<8>::ctas) * sm_count() * rows * 130 * 4;
 }
 
 extern "C" int pk_cache8_attention(const pk_tensor* queries, const pk_cache8* cache, const pk_tensor* lengths, float scale, const pk_tensor* out, const pk_tensor* lse, void* workspace,
@@ -542,7 +635,10 @@ extern "C" int pk_cache8_attention(const pk_tensor* queries, const pk_cache8* ca
   PK_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "workspace must be 256-byte aligned device memory");
   if (workspace_bytes < pk_cache8_attention_workspace_bytes(bs, T, Hq, H, p.c.cap)) return fail(PK_ERR_WORKSPACE, "cache8_attention: workspace too small");
   p.q = (const uint16_t*)queries->data, p.q_b = queries->stride[0], p.q_t = queries->stride[1], p.q_h = queries->stride[2];
-  p.lengths = (const int32_t*)lengths->data, p.bs = (int)bs, p.T = (int)T, p.G = (int)(Hq / H), p.row_groups = (int)((T * p.G + A8_ROWS - 1) / A8_ROWS);
+  p.lengths = (const int32_t*)lengths->data, p.bs = (int)bs, p.T = (int)T, p.G = (int)(Hq / H);
   p.out = (uint16_t*)out->data, p.records = (float*)workspace;
-  return cache->codes->dtype == PK_E4M3 ? launch<true>(p, (cudaStream_t)stream) : launch<false>(p, (cudaStream_t)stream);
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int rows = p.T * p.G;
+  if (cache->codes->dtype == PK_E4M3) return rows <= 8 ? launch<true, 8>(p, st) : rows <= 16 ? launch<true, 16>(p, st) : launch<true, 32>(p, st);
+  return rows <= 8 ? launch<false, 8>(p, st) : rows <= 16 ? launch<false, 16>(p, st) : launch<false, 32>(p, st);
 }
