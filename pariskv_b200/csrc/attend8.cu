@@ -18,12 +18,15 @@ namespace {
 constexpr int A8_TILE = 128, A8_THREADS = 128;
 constexpr int A8_STAGE = 8192;                    // 32 rows of K and V in codes, 16 in bf16
 constexpr int A8_SLOT = A8_STAGE + 16;            // and the scales: K of the first and second 16 rows, V of them
-constexpr int A8_OT = 36, A8_OS = 4 * A8_OT;      // a warp's partial: floats between two lanes' 32 channels, and two rows, so that its stores fall into all banks
-static_assert(8 * A8_OS * 4 <= A8_STAGE, "a warp's partial of eight rows takes the place of a stage");
 constexpr int A8_QS = 272;                        // bytes between two rows of the queries in bf16
 // ROWS: query rows of an item.
 template <int ROWS> struct A8 {
+  static constexpr bool across = ROWS == 8;       // query rows are the columns of the products, rows of the cache and channels their rows: eight fill an operand
   static constexpr int ctas = ROWS == 32 ? 2 : 3, q_bytes = ROWS * (256 + A8_QS), smem = 4 * 2 * A8_SLOT + q_bytes;
+  // A warp's partial of eight rows, in floats: channels lie in runs of `run`, padded so that the stores fall into all banks.
+  static constexpr int run = across ? 16 : 32, step = across ? 164 : 144;
+  static __device__ __forceinline__ int place(int row, int channel) { return row * step + channel / run * (run + 4) + channel % run; }
+  static_assert(8 * step * 4 <= A8_STAGE, "the partial takes the place of a stage");
 };
 
 struct Attend8 {
@@ -80,12 +83,12 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -109,12 +112,14 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
 // Words a, c of two rows -> words with the two rows' codes side by side as codes_lo / codes_hi take them: channels 0, 1 of the word, and 2, 3
 template <bool E4M3> __device__ __forceinline__ uint32_t pair01(uint32_t a, uint32_t c) { return __byte_perm(a, c, E4M3 ? 0x5140 : 0x5410); }
 template <bool E4M3> __device__ __forceinline__ uint32_t pair23(uint32_t a, uint32_t c) { return __byte_perm(a, c, E4M3 ? 0x7362 : 0x7632); }
-__device__ __forceinline__ float quad_max(float x) {
-  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+// Rows and columns of 8 x 8 numbers of 16 bits change places.
+__device__ __forceinline__ uint32_t turn(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 
-// Running state of one of a lane's query rows.  m: the largest score so far, times log2 e / sqrt d; l: the sum of p over this lane's columns, relative to 2^m; u: the largest p vs; O is kept as
+// Running state of one of a lane's query rows.  m: the largest score when it was last looked for, times log2 e / sqrt d; l: the sum of p over this lane's scores, relative to 2^m; u: the largest p vs then; O is kept as
 // 2^-E of what it stands for, up = 2^-E, down = 2^E with E following u, so that the weights p vs 2^-E are fp16 numbers with all of their bits.
 struct RowState {
   float m, l, u, up, down;
@@ -126,7 +131,7 @@ __device__ __forceinline__ float move(RowState& s, float m, float top) {
   const float before = s.u * f;
   s.u = fmaxf(before, top);
   const float t = s.u * s.up;
-  if (s.u > 0.0f && !(t >= 0.0625f && t <= 256.0f)) {
+  if (s.u > 0.0f && !(t >= 0.0625f && t <= 64.0f)) {
     const unsigned ex = min(__float_as_uint(s.u) >> 23, 252u);
     s.up = __uint_as_float((254u - ex) << 23);
     f = before == 0.0f ? 0.0f : f * s.up * s.down;
@@ -134,14 +139,11 @@ __device__ __forceinline__ float move(RowState& s, float m, float top) {
   }
   return f;
 }
-__device__ __forceinline__ void scale_rows(float (&o)[16][4], int e, float f) {
-#pragma unroll
-  for (int n = 0; n < 16; n++) o[n][2 * e] *= f, o[n][2 * e + 1] *= f;
-}
-
-template <bool E4M3, int ROWS>
+template <bool E4M3, int ROWS, bool DENSE>
 __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(const __grid_constant__ Attend8 p) {
-  constexpr int MT = ROWS == 32 ? 2 : 1, RPT = ROWS == 8 ? 1 : 2, NR = MT * RPT;   // operands of 16 rows, rows of a lane in each, in all
+  constexpr bool ACROSS = A8<ROWS>::across;
+  constexpr int MT = ROWS == 32 ? 2 : 1, NR = 2 * MT;   // operands of 16 query rows; query rows that a lane's scores belong to: 8 e + g, across 2 t4 + e
+  constexpr int NV = ACROSS ? 4 : 8;                    // its scores of each in a step
   __shared__ float s_m[4][ROWS], s_l[4][ROWS], s_factor[ROWS];
   __shared__ TilePlan s_plan;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
@@ -163,9 +165,9 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
     way.left = share_begin(plan.total, blockIdx.x + 1, shares) - first;
     way.b = plan.sample;
     way.sample(p);
-    const int64_t at = first - plan.before;
-    const int64_t item = at / way.n;
-    way.tile = (int)(at % way.n), way.h = (int)(item / p.row_groups), way.group = (int)(item % p.row_groups);
+    const unsigned at = (unsigned)(first - plan.before);   // tiles of a sample are below 2^32: the launch sees to it
+    const unsigned item = at / (unsigned)way.n;
+    way.tile = (int)(at % (unsigned)way.n), way.h = (int)(item / (unsigned)p.row_groups), way.group = (int)(item % (unsigned)p.row_groups);
   }
   const unsigned base = smem_addr(dyn8), mine = A8<ROWS>::q_bytes + warp * 2 * A8_SLOT, q_off = (ROWS == 8 ? 8 : 16) * lane;   // offsets in the block's shared memory
   const int n_rows_all = p.T * p.G, Hq = p.c.H * p.G;
@@ -185,19 +187,32 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
     auto load = [&](int slot) {
       const unsigned to = base + mine + slot * A8_SLOT, chunk = to + ckv * 4096 + odd * 128;
       const int live = whole - row0;
+      const int64_t c_l = DENSE ? 256 : p.c.c_l;
       if (live >= 32) {
         const uint8_t* from = src;
 #pragma unroll
-        for (int i = 0; i < 16; i++, from += 2 * p.c.c_l) cp16(chunk + i * 256 + ((ck ^ (ckv ? (2 * i) & 6 : odd)) << 4), from);
+        for (int i = 0; i < 16; i++, from += 2 * c_l) cp16(chunk + i * 256 + ((ck ^ (ckv ? (2 * i) & 6 : odd)) << 4), from);
       } else if (live > 0) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) cp16(chunk + i * 256 + ((ck ^ (ckv ? (2 * i) & 6 : odd)) << 4), 2 * i + odd < live ? src + 2 * i * p.c.c_l : src - odd * p.c.c_l, 2 * i + odd < live);
+        for (int i = 0; i < 16; i++) cp16(chunk + i * 256 + ((ck ^ (ckv ? (2 * i) & 6 : odd)) << 4), 2 * i + odd < live ? src + 2 * i * c_l : src - odd * c_l, 2 * i + odd < live);
       }
       if (lane < 4 && live > 0) cp4(to + A8_STAGE + 4 * lane, scales + (int64_t)(min(row0 + 16 * (lane & 1), whole - 1) >> p.c.shift) * p.c.s_j);
       cp_commit();
-      src += A8_TILE * p.c.c_l, row0 += A8_TILE;
+      src += A8_TILE * c_l, row0 += A8_TILE;
+    };
+    auto load_recent = [&](int sub, int slot) {   // 16 rows in 16 bits
+      const int r0 = whole + 32 * warp + 16 * sub, live = min(16, way.len - r0), kv = lane >> 4;
+      const uint16_t* ring = p.c.recent + b * p.c.r_b + h * p.c.r_h + kv * p.c.r_kv + (lane & 15) * 8;
+      const unsigned to = base + mine + slot * A8_SLOT + kv * 4096 + (lane & 15) * 16;
+      if (live > 0) {
+        int place = r0 % p.c.R;
+#pragma unroll 4
+        for (int i = 0; i < 16; i++, place = place + 1 == p.c.R ? 0 : place + 1) cp16(to + i * 256, ring + (int64_t)(i < live ? place : r0 % p.c.R) * p.c.r_l, i < live);
+      }
+      cp_commit();
     };
     if (n_coded > 0) load(0);
+    else if (recent) load_recent(0, 0);
     // queries: as they are, and as fp16 after a power of two per row in the order in which a lane needs them as operands; eight threads a row
 #pragma unroll 1
     for (int r0 = 0; r0 < ROWS; r0 += 16) {
@@ -236,17 +251,36 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
       }
     }
     __syncthreads();
-    float o[MT][16][4] = {};
+    // O: operand rows g, g + 8 are query rows, the two columns channels 32 t4 + n and + 16; across: the two columns query rows, operand rows channels 16 g + 2 n, + 1
+    constexpr int ON = ACROSS ? 8 : 16;
+    float o[MT][ON][4] = {};
     RowState st[NR];
     float factor[NR];   // log2 e / sqrt d, and what the row was scaled by
     int last[NR];       // the last row that a query row sees
     const int end = (p.lengths[b] > p.c.cap ? (int)p.c.cap : p.lengths[b]) - p.T;
+    auto row_of = [&](int e) { return ACROSS ? 2 * t4 + e : 8 * e + g; };
 #pragma unroll
     for (int e = 0; e < NR; e++) {
       st[e] = {-INFINITY, 0.0f, 0.0f, 1.0f, 1.0f};
-      factor[e] = s_factor[8 * e + g];
-      last[e] = end + (group * ROWS + min(8 * e + g, n_rows - 1)) / p.G;
+      factor[e] = s_factor[row_of(e)];
+      last[e] = end + (group * ROWS + min(row_of(e), n_rows - 1)) / p.G;
     }
+    auto scale_row = [&](int e, float f) {
+#pragma unroll
+      for (int n = 0; n < ON; n++) {
+        if (ACROSS) o[0][n][e & 1] *= f, o[0][n][2 + (e & 1)] *= f;
+        else o[e >> 1][n][2 * (e & 1)] *= f, o[e >> 1][n][2 * (e & 1) + 1] *= f;
+      }
+    };
+    auto row_max = [&](float x) {   // over the lanes that have scores of the same query rows
+      if (ACROSS) {
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+      }
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+      return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+    };
     const int lim = min(end + group * ROWS / p.G, whole - 1);   // rows up to here are seen by all
     unsigned at = mine;
     for (int j = 0; j < n_coded; j++) {
@@ -257,12 +291,18 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
         cp_wait<1>();
       } else {
         row0 += A8_TILE;
-        cp_wait<0>();
+        if (recent) {
+          load_recent(0, (j + 1) & 1);
+          cp_wait<1>();
+        } else {
+          cp_wait<0>();
+        }
       }
       if (first >= whole) continue;
-      float s[MT][4][4];
+      // scores of a lane: s[half of the rows][..]: row 8 i + 2 t4 + k of the half (i = c / 4, k = c & 1) and query row g, 8 + g (c >> 1 & 1); across: row g, 8 + g (c >> 1) and query row c & 1
+      float s[MT][2][ACROSS ? 4 : 8];
 #pragma unroll
-      for (int half = 0; half < 2; half++) {   // 16 rows of K at a time
+      for (int half = 0; half < 2; half++) {
         uint4 kw[2][2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -272,29 +312,26 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
 #pragma unroll
         for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-          for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) s[mt][2 * half + i][c] = 0.0f;
+          for (int c = 0; c < (ACROSS ? 4 : 8); c++) s[mt][half][c] = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < 8; ks++) {
-          uint32_t q[MT][4];
-#pragma unroll
-          for (int mt = 0; mt < MT; mt++) {
-            if (ROWS == 8) {
-              const uint2 x = lds8(q_off + ks * 256);
-              q[mt][0] = x.x, q[mt][1] = 0, q[mt][2] = x.y, q[mt][3] = 0;
-            } else {
-              const uint4 x = lds16(q_off + (mt * 8 + ks) * 512);
-              q[mt][0] = x.x, q[mt][1] = x.y, q[mt][2] = x.z, q[mt][3] = x.w;
-            }
-          }
+          uint32_t b[2][2];
 #pragma unroll
           for (int i = 0; i < 2; i++) {
             const uint4 v = kw[i][ks >> 2];
             const uint32_t w = (ks & 3) == 0 ? v.x : (ks & 3) == 1 ? v.y : (ks & 3) == 2 ? v.z : v.w;
-            const uint32_t b0 = codes_lo<E4M3>(w), b1 = codes_hi<E4M3>(w);
+            b[i][0] = codes_lo<E4M3>(w), b[i][1] = codes_hi<E4M3>(w);
+          }
+          if (ACROSS) {
+            const uint2 q = lds8(q_off + ks * 256);
+            mma_f16(s[0][half], b[0][0], b[1][0], b[0][1], b[1][1], q.x, q.y);
+          } else {
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) mma_f16(s[mt][2 * half + i], q[mt][0], q[mt][1], q[mt][2], q[mt][3], b0, b1);
+            for (int mt = 0; mt < MT; mt++) {
+              const uint4 q = lds16(q_off + (mt * 8 + ks) * 512);
+              mma_f16(s[mt][half], q.x, q.y, q.z, q.w, b[0][0], b[0][1]);
+              mma_f16(s[mt][half] + (ACROSS ? 0 : 4), q.x, q.y, q.z, q.w, b[1][0], b[1][1]);
+            }
           }
         }
       }
@@ -303,60 +340,75 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
         const uint4 x = lds16(at + A8_STAGE);
         sc = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
       }
-      uint32_t pa[MT][2][4];   // weights as operands: [16 rows of V]
+      // score v of query row e: half v / (NV / 2), and its row in the step
+      auto score = [&](int e, int v) -> float& {
+        if (ACROSS) return s[0][v >> 1][2 * (v & 1) + (e & 1)];
+        return s[e >> 1][v >> 2][4 * (v >> 1 & 1) + 2 * (e & 1) + (v & 1)];
+      };
+      auto row_at = [&](int v) { return ACROSS ? 16 * (v >> 1) + 8 * (v & 1) + g : 16 * (v >> 2) + 8 * (v >> 1 & 1) + 2 * t4 + (v & 1); };
+      uint32_t pw[NR][NV / 2];   // weights as pairs of fp16 numbers: of the columns 2 t4, 2 t4 + 1; across: see below
+      float w[NR][NV];
+      const bool all = first + 31 <= lim;
+      bool far = !all;
 #pragma unroll
       for (int e = 0; e < NR; e++) {
-        RowState& r = st[e];
-        float (&a)[4][4] = s[e / RPT];
-        const int c = 2 * (e % RPT);
-        const float kf[2] = {sc.x * factor[e], sc.y * factor[e]}, vs[2] = {sc.z, sc.w};
-        float w[4][2], f;
-        if (first + 31 <= lim) {
-          // the largest of 16 rows, which share a scale, is scaled once; so is the largest weight of them
-          const float t0 = quad_max(fmaxf(fmaxf(a[0][c], a[0][c + 1]), fmaxf(a[1][c], a[1][c + 1]))) * kf[0];
-          const float t1 = quad_max(fmaxf(fmaxf(a[2][c], a[2][c + 1]), fmaxf(a[3][c], a[3][c + 1]))) * kf[1];
-          const float m = fmaxf(r.m, fmaxf(t0, t1)), least = m == -INFINITY ? 0.0f : m;
-          f = move(r, m, fmaxf(ex2(t0 - least) * vs[0], ex2(t1 - least) * vs[1]));
+        const float kf[2] = {sc.x * factor[e], sc.y * factor[e]};
+        float x[NV], top = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < NV; v++) x[v] = fmaf(score(e, v), kf[v / (NV / 2)], -st[e].m), top = fmaxf(top, x[v]);
+        // The running maximum may lie 2^8 below the true one, and p vs 2^-E may reach 2^15: then nothing has to be moved.
+        far |= top > 8.0f || fmaxf(sc.z, sc.w) * st[e].up > 128.0f;
+#pragma unroll
+        for (int v = 0; v < NV; v++) w[e][v] = x[v];
+      }
+      if (!__any_sync(0xffffffffu, far)) {
+#pragma unroll
+        for (int e = 0; e < NR; e++) {
+          const float vs[2] = {sc.z * st[e].up, sc.w * st[e].up};
           float sum = 0.0f;
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float y0 = ex2(fmaf(a[i][c], kf[i >> 1], -least)), y1 = ex2(fmaf(a[i][c + 1], kf[i >> 1], -least)), v = vs[i >> 1] * r.up;
-            sum += y0 + y1;
-            w[i][0] = y0 * v, w[i][1] = y1 * v;
+          for (int v = 0; v < NV; v++) {
+            const float y = ex2(w[e][v]);
+            sum += y, w[e][v] = y * vs[v / (NV / 2)];
           }
-          r.l += sum;
-        } else {
-          float x[4][2], m = r.m, top = 0.0f, sum = 0.0f;
-          bool seen[4][2];
+          st[e].l += sum;
+        }
+      } else {
 #pragma unroll
-          for (int i = 0; i < 4; i++)
+        for (int e = 0; e < NR; e++) {
+          const float kf[2] = {sc.x * factor[e], sc.y * factor[e]}, vs[2] = {sc.z, sc.w};
+          float m = st[e].m, top = 0.0f, sum = 0.0f;
+          bool seen[NV];
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-              const int row = first + 8 * i + 2 * t4 + k;
-              seen[i][k] = row < whole && row <= last[e];
-              x[i][k] = a[i][c + k] * kf[i >> 1];
-              if (seen[i][k]) m = fmaxf(m, x[i][k]);
-            }
-          m = quad_max(m);
+          for (int v = 0; v < NV; v++) {
+            seen[v] = all || (first + row_at(v) < whole && first + row_at(v) <= last[e]);
+            if (seen[v]) m = fmaxf(m, score(e, v) * kf[v / (NV / 2)]);
+          }
+          m = row_max(m);
           const float least = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-          for (int i = 0; i < 4; i++)
+          for (int v = 0; v < NV; v++) {
+            const float y = seen[v] ? ex2(fmaf(score(e, v), kf[v / (NV / 2)], -least)) : 0.0f;
+            sum += y;
+            w[e][v] = seen[v] ? y * vs[v / (NV / 2)] : 0.0f;   // (the scale of a block that it does not see may be NaN)
+            top = fmaxf(top, w[e][v]);
+          }
+          const float f = move(st[e], m, row_max(top));
+          st[e].l += sum;
+          if (__any_sync(0xffffffffu, f != 1.0f)) scale_row(e, f);
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-              x[i][k] = seen[i][k] ? ex2(x[i][k] - least) : 0.0f;
-              sum += x[i][k];
-              w[i][k] = seen[i][k] ? x[i][k] * vs[i >> 1] : 0.0f;   // (the scale of a block that it does not see may be NaN)
-              top = fmaxf(top, w[i][k]);
-            }
-          f = move(r, m, quad_max(top));
-          r.l += sum;
-#pragma unroll
-          for (int i = 0; i < 4; i++) w[i][0] *= r.up, w[i][1] *= r.up;
+          for (int v = 0; v < NV; v++) w[e][v] *= st[e].up;
         }
-        if (__any_sync(0xffffffffu, f != 1.0f)) scale_rows(o[e / RPT], e % RPT, f);
+      }
+      // across: pairs are two query rows of one row of the cache; an exchange of 8 x 8 numbers makes them two rows of one query row
+      if (ACROSS) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) pa[e / RPT][i >> 1][2 * (i & 1) + e % RPT] = half2_of(w[i][0], w[i][1]);
-        if (RPT == 1) pa[0][0][1] = pa[0][0][3] = pa[0][1][1] = pa[0][1][3] = 0;
+        for (int v = 0; v < 4; v++) pw[v >> 1][v & 1] = turn(half2_of(w[0][v], w[1][v]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < NR; e++)
+#pragma unroll
+          for (int v = 0; v < NV; v += 2) pw[e][v >> 1] = half2_of(w[e][v], w[e][v + 1]);
       }
 #pragma unroll
       for (int half = 0; half < 2; half++) {
@@ -369,84 +421,108 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
           const uint32_t a0 = pair01<E4M3>(word(0), word(1)), a1 = pair01<E4M3>(word(2), word(3)), c0 = pair23<E4M3>(word(0), word(1)), c1 = pair23<E4M3>(word(2), word(3));
           const uint32_t bs[4][2] = {{codes_lo<E4M3>(a0), codes_lo<E4M3>(a1)}, {codes_hi<E4M3>(a0), codes_hi<E4M3>(a1)}, {codes_lo<E4M3>(c0), codes_lo<E4M3>(c1)},
                                      {codes_hi<E4M3>(c0), codes_hi<E4M3>(c1)}};
+          if (ACROSS) {
+            mma_f16(o[0][2 * wd], bs[0][0], bs[1][0], bs[0][1], bs[1][1], pw[half][0], pw[half][1]);
+            mma_f16(o[0][2 * wd + 1], bs[2][0], bs[3][0], bs[2][1], bs[3][1], pw[half][0], pw[half][1]);
+          } else {
 #pragma unroll
-          for (int mt = 0; mt < MT; mt++)
+            for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) mma_f16(o[mt][4 * wd + i], pa[mt][half][0], pa[mt][half][1], pa[mt][half][2], pa[mt][half][3], bs[i][0], bs[i][1]);
+              for (int i = 0; i < 4; i++)
+                mma_f16(o[mt][(4 * wd + i) % ON], pw[2 * mt][2 * half % (NV / 2)], pw[2 * mt + 1][2 * half % (NV / 2)], pw[2 * mt][(2 * half + 1) % (NV / 2)], pw[2 * mt + 1][(2 * half + 1) % (NV / 2)], bs[i][0], bs[i][1]);
+          }
         }
       }
       __syncwarp();
     }
     if (recent) {
       // ---- the rows behind the last whole block, 16 bf16 rows of this warp at a time.  Weights are two bf16 numbers each. ----
-      at = mine;
+      load_recent(1, (n_coded + 1) & 1);
 #pragma unroll 1
       for (int sub = 0; sub < 2; sub++) {
         const int r0 = whole + 32 * warp + 16 * sub, live = min(16, way.len - r0);
-        if (live <= 0) break;
-        const int kv = lane >> 4;
-        const uint16_t* ring = p.c.recent + b * p.c.r_b + h * p.c.r_h + kv * p.c.r_kv + (lane & 15) * 8;
-#pragma unroll 4
-        for (int i = 0; i < 16; i++) cp16(base + at + kv * 4096 + i * 256 + (lane & 15) * 16, ring + (int64_t)((i < live ? r0 + i : r0) % p.c.R) * p.c.r_l, i < live);
-        cp_commit();
-        cp_wait<0>();
-        float x[NR][4];
+        at = mine + ((n_coded + sub) & 1) * A8_SLOT;
+        if (sub == 0) cp_wait<1>();
+        else cp_wait<0>();
+        if (live <= 0) continue;
+        float x[NR][4];   // score v: row 8 (v >> 1) + 2 t4 + (v & 1); across: row 8 v + g, v < 2
+        constexpr int NB = ACROSS ? 2 : 4;
+        if (ACROSS) {
+          float acc[4] = {};
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-          for (int nt = 0; nt < 2; nt++) {
-            float acc[4] = {};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const unsigned q = ROWS * 256 + (16 * mt + g) * A8_QS + t4 * 64 + i * 16;
-              const uint4 w = lds16(at + (8 * nt + g) * 256 + t4 * 64 + i * 16), a = lds16(q), c = RPT == 2 ? lds16(q + 8 * A8_QS) : make_uint4(0, 0, 0, 0);
-              mma_bf16(acc, a.x, c.x, a.y, c.y, w.x, w.y);
-              mma_bf16(acc, a.z, c.z, a.w, c.w, w.z, w.w);
-            }
-#pragma unroll
-            for (int e = 0; e < RPT; e++) x[RPT * mt + e][2 * nt] = acc[2 * e], x[RPT * mt + e][2 * nt + 1] = acc[2 * e + 1];
+          for (int i = 0; i < 4; i++) {
+            const uint4 q = lds16(ROWS * 256 + g * A8_QS + t4 * 64 + i * 16), a = lds16(at + g * 256 + t4 * 64 + i * 16), c = lds16(at + (8 + g) * 256 + t4 * 64 + i * 16);
+            mma_bf16(acc, a.x, c.x, a.y, c.y, q.x, q.y);
+            mma_bf16(acc, a.z, c.z, a.w, c.w, q.z, q.w);
           }
-        uint32_t hi[MT][4] = {}, lo[MT][4] = {};
+          x[0][0] = acc[0], x[0][1] = acc[2], x[1][0] = acc[1], x[1][1] = acc[3];
+        } else {
+#pragma unroll
+          for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int nt = 0; nt < 2; nt++) {
+              float acc[4] = {};
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const unsigned q = ROWS * 256 + (16 * mt + g) * A8_QS + t4 * 64 + i * 16;
+                const uint4 w = lds16(at + (8 * nt + g) * 256 + t4 * 64 + i * 16), a = lds16(q), c = lds16(q + 8 * A8_QS);
+                mma_bf16(acc, a.x, c.x, a.y, c.y, w.x, w.y);
+                mma_bf16(acc, a.z, c.z, a.w, c.w, w.z, w.w);
+              }
+#pragma unroll
+              for (int e = 0; e < 2; e++) x[2 * mt + e][2 * nt] = acc[2 * e], x[2 * mt + e][2 * nt + 1] = acc[2 * e + 1];
+            }
+        }
+        uint32_t hi[NR][2], lo[NR][2];   // pairs of weights, and what their rounding left; across as above
 #pragma unroll
         for (int e = 0; e < NR; e++) {
-          RowState& r = st[e];
-          float m = r.m, top = 0.0f, sum = 0.0f;
-          bool seen[4];
+          float m = st[e].m, top = 0.0f, sum = 0.0f;
+          bool seen[NB];
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int row = 8 * (i >> 1) + 2 * t4 + (i & 1);
-            seen[i] = row < live && r0 + row <= last[e];
-            x[e][i] *= factor[e] != factor[e] ? NAN : p.scale_log2;
-            if (seen[i]) m = fmaxf(m, x[e][i]);
+          for (int v = 0; v < NB; v++) {
+            const int row = ACROSS ? 8 * v + g : 8 * (v >> 1) + 2 * t4 + (v & 1);
+            seen[v] = row < live && r0 + row <= last[e];
+            x[e][v] *= factor[e] != factor[e] ? NAN : p.scale_log2;
+            if (seen[v]) m = fmaxf(m, x[e][v]);
           }
-          m = quad_max(m);
+          m = row_max(m);
           const float least = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            x[e][i] = seen[i] ? ex2(x[e][i] - least) : 0.0f;
-            sum += x[e][i], top = fmaxf(top, x[e][i]);
+          for (int v = 0; v < NB; v++) {
+            x[e][v] = seen[v] ? ex2(x[e][v] - least) : 0.0f;
+            sum += x[e][v], top = fmaxf(top, x[e][v]);
           }
-          const float f = move(r, m, quad_max(top));
-          r.l += sum;
-          if (__any_sync(0xffffffffu, f != 1.0f)) scale_rows(o[e / RPT], e % RPT, f);
+          const float f = move(st[e], m, row_max(top));
+          st[e].l += sum;
+          if (__any_sync(0xffffffffu, f != 1.0f)) scale_row(e, f);
+#pragma unroll
+          for (int v = 0; v < NB; v++) x[e][v] *= st[e].up;
+        }
+#pragma unroll
+        for (int e = 0; e < NR; e++)
 #pragma unroll
           for (int i = 0; i < 2; i++) {
-            const float a = x[e][2 * i] * r.up, c = x[e][2 * i + 1] * r.up;
-            const uint32_t w = pack2(a, c);
-            hi[e / RPT][2 * i + e % RPT] = w;
-            lo[e / RPT][2 * i + e % RPT] = pack2(a - __uint_as_float(w << 16), c - __uint_as_float(w & 0xffff0000u));
+            const float a = ACROSS ? x[0][(2 * e + i) % 2] : x[e][2 * i], c = ACROSS ? x[1][(2 * e + i) % 2] : x[e][(2 * i + 1) % 4];
+            hi[e][i] = pack2(a, c), lo[e][i] = pack2(a - __uint_as_float(hi[e][i] << 16), c - __uint_as_float(hi[e][i] & 0xffff0000u));
           }
+        if (ACROSS) {
+#pragma unroll
+          for (int i = 0; i < 2; i++) hi[0][i] = turn(hi[0][i]), lo[0][i] = turn(lo[0][i]);
         }
         // A weight of zero does not keep what is not a number out of a product: it is taken out, and given to the query rows that see it.
-        bool bad = false;
-#pragma unroll 1
-        for (int i = lane; i < 256; i += 32) {
-          const uint4 w = lds16(at + 4096 + i * 16);
-          uint32_t v[4] = {w.x, w.y, w.z, w.w};
-          bool mine_bad = false;
+        uint4 v[2][4];   // [half of the lane's channels]: rows 2 t4, 2 t4 + 1, and eight further; channels 16 g ..
+        auto load_v = [&]() {
 #pragma unroll
-          for (int k = 0; k < 4; k++) mine_bad |= not_finite(v[k]) | not_finite(v[k] >> 16);
-          bad |= mine_bad;
+          for (int part = 0; part < 2; part++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[part][i] = lds16(at + 4096 + (8 * (i >> 1) + 2 * t4 + (i & 1)) * 256 + g * 32 + 16 * part);
+        };
+        load_v();
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const uint4 w = v[i >> 2][i & 3];
+          bad |= not_finite(w.x) | not_finite(w.x >> 16) | not_finite(w.y) | not_finite(w.y >> 16) | not_finite(w.z) | not_finite(w.z >> 16) | not_finite(w.w) | not_finite(w.w >> 16);
         }
         bad = __any_sync(0xffffffffu, bad);
         if (bad) {
@@ -455,13 +531,16 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
 #pragma unroll
             for (int n = 0; n < 16; n++)
 #pragma unroll
-              for (int i = 0; i < 2; i++) {   // column n of the tile columns 2 t4, 2 t4 + 1 of this lane: channel 32 t4 + 16 i + n
+              for (int i = 0; i < (ACROSS ? 1 : 2); i++) {
                 uint16_t w;
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(base + at + 4096 + row * 256 + 2 * (32 * t4 + 16 * i + n)) : "memory");
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(base + at + 4096 + row * 256 + 2 * (ACROSS ? 16 * g + n : 32 * t4 + 16 * i + n)) : "memory");
                 if (not_finite(w)) {
 #pragma unroll
                   for (int e = 0; e < NR; e++)
-                    if (r0 + row <= last[e]) o[e / RPT][n][2 * (e % RPT) + i] += bf2f(w);
+                    if (r0 + row <= last[e]) {
+                      if (ACROSS) o[0][(n >> 1) % ON][2 * (n & 1) + (e & 1)] += bf2f(w);
+                      else o[e >> 1][n % ON][2 * (e & 1) + i] += bf2f(w);
+                    }
                 }
               }
           __syncwarp();
@@ -473,24 +552,27 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
             asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + at + 4096 + i * 4), "r"(v) : "memory");
           }
           __syncwarp();
+          load_v();
         }
 #pragma unroll
         for (int part = 0; part < 2; part++) {
-          uint4 v[4];
-#pragma unroll
-          for (int i = 0; i < 4; i++) v[i] = lds16(at + 4096 + (8 * (i >> 1) + 2 * t4 + (i & 1)) * 256 + g * 32 + 16 * part);
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            auto word = [&](int i) { return k == 0 ? v[i].x : k == 1 ? v[i].y : k == 2 ? v[i].z : v[i].w; };
+            auto word = [&](int i) { return k == 0 ? v[part][i].x : k == 1 ? v[part][i].y : k == 2 ? v[part][i].z : v[part][i].w; };
             const uint32_t b0 = __byte_perm(word(0), word(1), 0x5410), b1 = __byte_perm(word(2), word(3), 0x5410), c0 = __byte_perm(word(0), word(1), 0x7632),
                            c1 = __byte_perm(word(2), word(3), 0x7632);
+            if (ACROSS) {
+              mma_bf16(o[0][4 * part + k], b0, c0, b1, c1, hi[0][0], hi[0][1]);
+              mma_bf16(o[0][4 * part + k], b0, c0, b1, c1, lo[0][0], lo[0][1]);
+            } else {
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-              float (&x0)[4] = o[mt][8 * part + 2 * k], (&x1)[4] = o[mt][8 * part + 2 * k + 1];
-              mma_bf16(x0, hi[mt][0], hi[mt][1], hi[mt][2], hi[mt][3], b0, b1);
-              mma_bf16(x0, lo[mt][0], lo[mt][1], lo[mt][2], lo[mt][3], b0, b1);
-              mma_bf16(x1, hi[mt][0], hi[mt][1], hi[mt][2], hi[mt][3], c0, c1);
-              mma_bf16(x1, lo[mt][0], lo[mt][1], lo[mt][2], lo[mt][3], c0, c1);
+              for (int mt = 0; mt < MT; mt++) {
+                float (&x0)[4] = o[mt][(8 * part + 2 * k) % ON], (&x1)[4] = o[mt][(8 * part + 2 * k + 1) % ON];
+                mma_bf16(x0, hi[2 * mt][0], hi[2 * mt + 1][0], hi[2 * mt][1], hi[2 * mt + 1][1], b0, b1);
+                mma_bf16(x0, lo[2 * mt][0], lo[2 * mt + 1][0], lo[2 * mt][1], lo[2 * mt + 1][1], b0, b1);
+                mma_bf16(x1, hi[2 * mt][0], hi[2 * mt + 1][0], hi[2 * mt][1], hi[2 * mt + 1][1], c0, c1);
+                mma_bf16(x1, lo[2 * mt][0], lo[2 * mt + 1][0], lo[2 * mt][1], lo[2 * mt + 1][1], c0, c1);
+              }
             }
           }
         }
@@ -500,25 +582,36 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
     // ---- the four warps' shares of the segment ----
 #pragma unroll
     for (int e = 0; e < NR; e++) {
-      st[e].l += __shfl_xor_sync(0xffffffffu, st[e].l, 1);
-      st[e].l += __shfl_xor_sync(0xffffffffu, st[e].l, 2);
-      if (t4 == 0) s_m[warp][8 * e + g] = st[e].m, s_l[warp][8 * e + g] = st[e].l;
+#pragma unroll
+      for (int off = ACROSS ? 4 : 1; off < (ACROSS ? 32 : 4); off <<= 1) st[e].l += __shfl_xor_sync(0xffffffffu, st[e].l, off);
+      if (ACROSS ? g == 0 : t4 == 0) s_m[warp][row_of(e)] = st[e].m, s_l[warp][row_of(e)] = st[e].l;
     }
     __syncthreads();
     float* parts = reinterpret_cast<float*>(dyn8 + A8<ROWS>::q_bytes);   // a warp's first stage
-    float* to = parts + warp * 2 * A8_SLOT / 4 + g * A8_OS + A8_OT * t4;
+    float* to = parts + warp * 2 * A8_SLOT / 4;
+    auto share = [&](int e) {   // what this warp's O of a query row counts for
+      const int r = row_of(e);
+      const float M = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+      return st[e].m == -INFINITY ? 0.0f : ex2(st[e].m - M) * st[e].down;
+    };
 #pragma unroll
-    for (int e = 0; e < NR; e++) {
-      if (8 * e < n_rows) {
-        const int r = 8 * e + g;
-        const float M = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-        const float f = st[e].m == -INFINITY ? 0.0f : ex2(st[e].m - M) * st[e].down;
-        const int c = 2 * (e % RPT);
-        float (&x)[16][4] = o[e / RPT];
+    for (int e = 0; e < (ACROSS ? 1 : NR); e++) {   // eight query rows at a time
+      if (ACROSS) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const float f = share(k);
+#pragma unroll
+          for (int n = 0; n < 8; n += 2)
+            *reinterpret_cast<float4*>(to + A8<ROWS>::place(2 * t4 + k, 16 * g + 2 * n)) = make_float4(o[0][n][k] * f, o[0][n][2 + k] * f, o[0][n + 1][k] * f, o[0][n + 1][2 + k] * f);
+        }
+      } else if (8 * e < n_rows) {
+        const float f = share(e);
+        const int c = 2 * (e & 1);
 #pragma unroll
         for (int n = 0; n < 16; n += 4) {
-          *reinterpret_cast<float4*>(to + n) = make_float4(x[n][c] * f, x[n + 1][c] * f, x[n + 2][c] * f, x[n + 3][c] * f);
-          *reinterpret_cast<float4*>(to + 16 + n) = make_float4(x[n][c + 1] * f, x[n + 1][c + 1] * f, x[n + 2][c + 1] * f, x[n + 3][c + 1] * f);
+          float (&x0)[4] = o[e >> 1][n % ON], (&x1)[4] = o[e >> 1][(n + 1) % ON], (&x2)[4] = o[e >> 1][(n + 2) % ON], (&x3)[4] = o[e >> 1][(n + 3) % ON];
+          *reinterpret_cast<float4*>(to + A8<ROWS>::place(g, 32 * t4 + n)) = make_float4(x0[c] * f, x1[c] * f, x2[c] * f, x3[c] * f);
+          *reinterpret_cast<float4*>(to + A8<ROWS>::place(g, 32 * t4 + 16 + n)) = make_float4(x0[c + 1] * f, x1[c + 1] * f, x2[c + 1] * f, x3[c + 1] * f);
         }
       }
       __syncthreads();
@@ -529,7 +622,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
 #pragma unroll
         for (int w = 0; w < 4; w++) {
           L += s_l[w][row] * (s_m[w][row] == -INFINITY ? (s_l[w][row] == 0.0f ? 0.0f : 1.0f) : ex2(s_m[w][row] - M));   // (all NaN: the sum is NaN and stays)
-          const float4* from = reinterpret_cast<const float4*>(parts + w * 2 * A8_SLOT / 4 + (tid >> 4) * A8_OS + (c >> 5) * A8_OT + (c & 31));
+          const float4* from = reinterpret_cast<const float4*>(parts + w * 2 * A8_SLOT / 4 + A8<ROWS>::place(tid >> 4, c));
           const float4 x = from[0], y = from[1];
           O[0] += x.x, O[1] += x.y, O[2] += x.z, O[3] += x.w, O[4] += y.x, O[5] += y.y, O[6] += y.z, O[7] += y.w;
         }
@@ -558,8 +651,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
 // A block per query row: the records of the blocks that share its item, in the order of the tiles.
 template <int ROWS>
 __global__ void __launch_bounds__(128) attend8_merge_kernel(const __grid_constant__ Attend8 p, int blocks) {
-  pdl_wait();
-  pdl_trigger();
+  // The lengths are read before the wait: this kernel starts once every block of the one before has triggered, which it does behind its own wait, and that one does not write them.
   __shared__ MergeShared shared;
   const int64_t row = blockIdx.x;
   const int lane = threadIdx.x & 31, Hq = p.c.H * p.G, hq = (int)(row % Hq), h = hq / p.G;
@@ -575,26 +667,39 @@ __global__ void __launch_bounds__(128) attend8_merge_kernel(const __grid_constan
   const int64_t first = before + ((int64_t)h * p.row_groups + r / ROWS) * n;
   const unsigned shares = (unsigned)min((int64_t)blocks, total);
   const int c0 = share_owner(first, total, shares), c1 = share_owner(first + n - 1, total, shares);
+  pdl_wait();
+  pdl_trigger();
   if (c0 == c1) return;   // written by its block
   merge_row(shared, c1 - c0 + 1, ROWS, r % ROWS, [&](int i) { return p.records + (2 * (int64_t)(c0 + i) + (i == 0)) * (ROWS * 130); }, p.out + row * 128,
             p.lse ? p.lse + row : nullptr);
 }
 
-template <bool E4M3, int ROWS>
-int launch(Attend8 p, cudaStream_t st) {
+// Ranges per place on an SM.  SMs do not get the same share of HBM (with a range each the last ends a sixth after the average): of long ranges there are up to four, of which a fast one takes more.
+int64_t a8_waves(int64_t most, int64_t slots) {
+  const int64_t n = most / (slots * 24);
+  return n < 1 ? 1 : n > 4 ? 4 : n;
+}
+
+template <bool E4M3, int ROWS, bool DENSE>
+int launch_as(Attend8 p, cudaStream_t st) {
   p.row_groups = (p.T * p.G + ROWS - 1) / ROWS;
   const int64_t slots = (int64_t)A8<ROWS>::ctas * sm_count(), most = (int64_t)p.bs * p.c.H * p.row_groups * ((p.c.cap + A8_TILE - 1) / A8_TILE + 1);
-  const int blocks = (int)(most < slots ? most : slots);
+  const int blocks = (int)(most < slots ? most : slots * a8_waves(most, slots));
   static PerDevice opted;
   if (const unsigned long long bit = first_on_device(opted)) {
-    if (cudaFuncSetAttribute(attend8_kernel<E4M3, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, A8<ROWS>::smem) != cudaSuccess)
+    if (cudaFuncSetAttribute(attend8_kernel<E4M3, ROWS, DENSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, A8<ROWS>::smem) != cudaSuccess)
       return fail(PK_ERR_CUDA, "cache8_attention: %s", cudaGetErrorString(cudaGetLastError()));
     mark_on_device(opted, bit);
   }
   StageTimer timer(ST_ATTENTION, st);
-  launch_chain(attend8_kernel<E4M3, ROWS>, dim3((unsigned)blocks), dim3(A8_THREADS), A8<ROWS>::smem, st, p);
+  launch_chain(attend8_kernel<E4M3, ROWS, DENSE>, dim3((unsigned)blocks), dim3(A8_THREADS), A8<ROWS>::smem, st, p);
   launch_chain(attend8_merge_kernel<ROWS>, dim3((unsigned)((int64_t)p.bs * p.T * p.c.H * p.G)), dim3(128), 0, st, p, blocks);
   return check_launch("cache8_attention", 2);
+}
+
+template <bool E4M3, int ROWS>
+int launch(const Attend8& p, cudaStream_t st) {   // K and V of a row side by side, row after row: the copies' addresses are constants apart
+  return p.c.c_l == 256 ? launch_as<E4M3, ROWS, true>(p, st) : launch_as<E4M3, ROWS, false>(p, st);
 }
 
 }  // namespace
@@ -605,7 +710,8 @@ using namespace pk;
 extern "C" int64_t pk_cache8_attention_workspace_bytes(int64_t bs, int64_t T, int64_t Hq, int64_t H, int64_t cap) {
   if (bs < 1 || T < 1 || T > 256 || H < 1 || Hq < H || cap < 0) return 0;
   const int rows = T * (Hq / H) <= 8 ? 8 : T * (Hq / H) <= 16 ? 16 : 32;
-  return 2 * (int64_t)(rows == 32 ? A8<32>::ctas : A8<8>::ctas) * sm_count() * rows * 130 * 4;
+  const int64_t slots = (int64_t)(rows == 32 ? A8<32>::ctas : A8<8>::ctas) * sm_count(), most = bs * H * ((T * (Hq / H) + rows - 1) / rows) * ((cap + A8_TILE - 1) / A8_TILE + 1);
+  return 2 * (most < slots ? most : slots * a8_waves(most, slots)) * rows * 130 * 4;
 }
 
 extern "C" int pk_cache8_attention(const pk_tensor* queries, const pk_cache8* cache, const pk_tensor* lengths, float scale, const pk_tensor* out, const pk_tensor* lse, void* workspace,
@@ -628,7 +734,7 @@ extern "C" int pk_cache8_attention(const pk_tensor* queries, const pk_cache8* ca
     PK_REQUIRE(is_contig(lse) && lse->shape[0] == bs && lse->shape[1] == T && lse->shape[2] == Hq, "lse must be contiguous f32 [bs,T,Hq]");
     p.lse = (float*)lse->data;
   }
-  PK_REQUIRE(bs < 65536 && bs * T * Hq < (1LL << 31), "sizes out of range");
+  PK_REQUIRE(bs < 65536 && bs * T * Hq < (1LL << 31) && (p.c.cap / A8_TILE + 2) * H * ((T * (Hq / H) + 7) / 8) < (1LL << 31), "sizes out of range");
   p.scale_log2 = scale * 1.4426950408889634f;
   PK_REQUIRE(scale > 0.0f && p.scale_log2 <= 3.4e38f, "scale must be positive, and finite as a factor of log2 e");
   if (bs == 0 || T == 0) return PK_OK;
