@@ -52,24 +52,19 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < 8; i++) m = max(m, s_max[i][kv]);
     const float amax = bf2f((uint16_t)m);
     const bool fine = m < 0x7f80u;
-    const float unit = m == 0 ? 1.0f : __fmul_rn(amax, E4M3 ? 0.001953125f : 0.0078125f);
+    const Coder<E4M3> code(amax);
     uint8_t* to = c.codes + b * c.c_b + h * c.c_h + kv * c.c_kv + ch;
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      float q[8];
+      float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float f = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
-        q[e] = E4M3 ? e4m3_quotient(f, unit) : i8_quotient(f, unit);
-      }
-      uint2 o;
-      if (E4M3) o = make_uint2(pack_e4m3(q[0], q[1], q[2], q[3]), pack_e4m3(q[4], q[5], q[6], q[7]));
-      else o = make_uint2(pack_i8(q[0], q[1], q[2], q[3]), pack_i8(q[4], q[5], q[6], q[7]));
-      if (!fine) o = make_uint2(0, 0);
+      for (int e = 0; e < 8; e++) y[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+      uint2 o = make_uint2(0, 0);
+      if (fine) o = code(y);
       *reinterpret_cast<uint2*>(to + (row0 + 8 * i + warp) * c.c_l) = o;
     }
-    if (warp == 0 && (lane & 15) == 0) c.scales[b * c.s_b + h * c.s_h + j * c.s_j + kv * c.s_kv] = fine ? __fdiv_rn(amax, E4M3 ? 448.0f : 127.0f) : NAN;
+    if (warp == 0 && (lane & 15) == 0) c.scales[b * c.s_b + h * c.s_h + j * c.s_j + kv * c.s_kv] = fine ? __fdiv_rn(amax, Coder<E4M3>::MOST) : NAN;
   }
   // The last R rows stay in 16 bits.  Rows of the first block that were there before may lie where new ones go: the thread block that reads them also
   // writes what replaces them.

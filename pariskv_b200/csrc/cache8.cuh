@@ -69,22 +69,63 @@ __device__ __forceinline__ float2 e4m3_floats(uint32_t two) {
 }
 // byte i of four whole numbers as a float: 2^23 + (code + 128) is a float whose last bits are the biased code
 __device__ __forceinline__ float i8_float(uint32_t biased, int i) { return __uint_as_float(__byte_perm(biased, 0x4b000000u, 0x7540 + i)) - 8388736.0f; }
-// y 127 / amax (e4m3: 448) as the definition has it: `unit` is amax 2^-7 (2^-9), 1 for a block of zeros
-__device__ __forceinline__ float i8_quotient(float y, float unit) { return __fdiv_rn(__fmul_rn(y, 0.9921875f), unit); }
-__device__ __forceinline__ float e4m3_quotient(float y, float unit) { return __fdiv_rn(__fmul_rn(y, 0.875f), unit); }
-__device__ __forceinline__ uint32_t pack_i8(float a, float b, float c, float d) {   // to the nearest, ties to the even one
-  uint32_t r;
-  asm("{\n\t.reg .b32 t;\n\tcvt.pack.sat.s8.s32.b32 t, %4, %3, 0;\n\tcvt.pack.sat.s8.s32.b32 %0, %2, %1, t;\n\t}"
-      : "=r"(r)
-      : "r"(__float2int_rn(a)), "r"(__float2int_rn(b)), "r"(__float2int_rn(c)), "r"(__float2int_rn(d)));
-  return r;
-}
 __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
   uint16_t lo, hi;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
   return (uint32_t)lo | (uint32_t)hi << 16;
 }
+// Codes of values whose largest magnitude is amax:  y M / amax to the nearest, ties to the even one, M = 127 (e4m3: 448), as 32-bit arithmetic gives it from (y M / u) / (amax / u) with a power of two
+// u = 128 (512).  A division per value took two thirds of the kernels' instructions.  Instead each is multiplied by a factor that is surely above M / amax and by one that is surely below: where both round
+// to the same code that is the code, whatever the last bits.  Others, one group of eight values in some hundred, are divided.
+template <bool E4M3>
+struct Coder {
+  static constexpr float MOST = E4M3 ? 448.0f : 127.0f, U = E4M3 ? 512.0f : 128.0f;
+  float unit, above, below;
+  __device__ __forceinline__ explicit Coder(float amax) {
+    unit = amax == 0.0f ? 1.0f : __fmul_rn(amax, 1.0f / U);
+    const float f = __fdiv_rn(MOST, amax);
+    const bool plain = amax > 1e-30f;   // (else the factor might be infinite)
+    above = plain ? f * (1.0f + 0x1p-21f) : INFINITY, below = plain ? f * (1.0f - 0x1p-21f) : 0.0f;   // f is off by 2^-24 of itself, this product too; the quotient is off by 2^-23
+  }
+  __device__ __forceinline__ float quotient(float y) const { return __fdiv_rn(__fmul_rn(y, MOST / U), unit); }
+  __device__ __forceinline__ uint2 operator()(const float (&y)[8]) const {
+    uint32_t a[2], differ = 0;
+    if (E4M3) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        a[i] = pack_e4m3(y[4 * i] * above, y[4 * i + 1] * above, y[4 * i + 2] * above, y[4 * i + 3] * above);
+        differ |= a[i] ^ pack_e4m3(y[4 * i] * below, y[4 * i + 1] * below, y[4 * i + 2] * below, y[4 * i + 3] * below);
+      }
+    } else {
+      uint32_t n[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {   // the sum with 1.5 2^23 ends in the whole number
+        n[i] = __float_as_uint(__fmaf_rn(y[i], above, 12582912.0f));
+        differ |= n[i] ^ __float_as_uint(__fmaf_rn(y[i], below, 12582912.0f));
+      }
+#pragma unroll
+      for (int i = 0; i < 2; i++) a[i] = __byte_perm(__byte_perm(n[4 * i], n[4 * i + 1], 0x0040), __byte_perm(n[4 * i + 2], n[4 * i + 3], 0x0040), 0x5410);
+    }
+    if (differ) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        float q[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) q[e] = quotient(y[4 * i + e]);
+        if (E4M3) {
+          a[i] = pack_e4m3(q[0], q[1], q[2], q[3]);
+        } else {
+          uint32_t n[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) n[e] = (uint32_t)__float2int_rn(q[e]);
+          a[i] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+        }
+      }
+    }
+    return make_uint2(a[0], a[1]);
+  }
+};
 #endif
 
 }  // namespace pk

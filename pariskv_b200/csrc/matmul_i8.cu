@@ -202,6 +202,148 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_c
   if (warp == 1) tmem_free(tmem, 2 * COLS);
 }
 
+// ---- many tokens: two SMs on a tile of 256 rows and 256 tokens ----
+// Each block of a pair copies 128 rows of the matrix and 128 tokens, and has the sums of its rows; a product reads both blocks' operands (cta_group::2), so that a block copies 32 KB for the work that takes 48 KB alone.
+// The first block issues; copies of both arrive on its barriers, and its commits reach both.
+constexpr int MP_NT = 256, MP_STAGES = 6, MP_STAGE = 2 * 128 * MM_K, MP_SMEM = 1024 + MP_STAGES * MP_STAGE;
+
+__device__ __forceinline__ unsigned in_block0(unsigned at) {   // the same place in the pair's first block
+  unsigned r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ void tma_load2_pair(unsigned dst, const CUtensorMap* map, int c0, int c1, unsigned mb) {   // mb: in either block of the pair
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(mb)
+               : "memory");
+}
+__device__ __forceinline__ void tc_mma_i8_pair(unsigned d, uint64_t a, uint64_t b, unsigned idesc, unsigned add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+__device__ __forceinline__ void tc_commit_pair(unsigned mb) {   // to that place of both blocks
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(mb), "h"((uint16_t)3) : "memory");
+}
+
+__global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ MmParams p) {
+  constexpr int NS = MP_STAGES, STAGE = MP_STAGE, NT = MP_NT;
+  constexpr unsigned IDESC = 2u << 4 | 1u << 7 | 1u << 10 | (unsigned)(NT >> 3) << 17 | (unsigned)(256 >> 4) << 24;
+  extern __shared__ unsigned char dyn[];
+  __shared__ __align__(8) unsigned long long bars[2 * NS + 5];
+  __shared__ unsigned s_tmem;
+  __shared__ volatile int s_dead;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const unsigned ring = (smem_addr(dyn) + 1023) & ~1023u;
+  const unsigned full = smem_addr(bars), empty = full + 8 * NS, done = empty + 8 * NS, taken = done + 16, ending = taken + 16;
+  const int rank = (int)(blockIdx.x & 1), pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
+  if (tid == 0) {
+    for (int i = 0; i < NS; i++) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
+    for (int i = 0; i < 2; i++) mbar_init(done + 8 * i, 1), mbar_init(taken + 8 * i, 8);
+    mbar_init(ending, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_dead = 0;
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  if (warp == 0 && lane < 2) tma_prefetch_map(lane ? &map_x : &map_w);
+  pdl_wait();
+  pdl_trigger();
+  tc_before();
+  __syncthreads();
+  cluster_sync();   // the barriers of both are there
+  tc_after();
+  const unsigned tmem = s_tmem;
+  bool dead = false;   // a wait has run out: no more waiting, the sums come out as NaN
+  auto wait = [&](unsigned mb, unsigned parity) {
+    for (int it = 0; !dead; it++) {
+      if (mbar_try(mb, parity)) break;
+      if (it >= MM_WAIT_LIMIT || ((it & 1023) == 1023 && s_dead)) dead = true, s_dead = 1;
+    }
+  };
+  if (warp == 0) {
+    if (lane == 0) {
+      int q = 0;
+      const unsigned full0 = in_block0(full);
+      for (int tile = pair; tile < p.tiles && !dead; tile += pairs) {
+        const int t0 = tile % p.t_tiles * NT + 128 * rank, o0 = tile / p.t_tiles * 256 + 128 * rank;
+        for (int k = 0; k < p.chunks; k++, q++) {
+          const int st = q % NS;
+          if (q >= NS) wait(empty + 8 * st, (unsigned)(q / NS - 1) & 1);
+          if (dead) break;
+          if (rank == 0) mbar_expect(full + 8 * st, 2 * STAGE);
+          tma_load2_pair(ring + st * STAGE, &map_w, k * MM_K, o0, full0 + 8 * st);
+          tma_load2_pair(ring + st * STAGE + 128 * MM_K, &map_x, k * MM_K, t0, full0 + 8 * st);
+        }
+      }
+      if (rank == 0 && (dead || s_dead))   // what is under way has to land before the blocks end
+        for (int i = q < NS ? 0 : q - NS; i < q; i++)
+          for (int it = 0; it < MM_WAIT_LIMIT && !mbar_try(full + 8 * (i % NS), (unsigned)(i / NS) & 1); it++) {}
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const bool leader = elect_one();
+      const uint64_t w_desc = umma_desc(ring, 16), x_desc = umma_desc(ring + 128 * MM_K, 16);
+      int q = 0, n = 0;
+      for (int tile = pair; tile < p.tiles; tile += pairs, n++) {
+        const int set = n & 1;
+        if (n >= 2) wait(taken + 8 * set, (unsigned)(n / 2 - 1) & 1);
+        __syncwarp();
+        tc_after();
+        for (int k = 0; k < p.chunks; k++, q++) {
+          const int st = q % NS;
+          wait(full + 8 * st, (unsigned)(q / NS) & 1);
+          __syncwarp();
+          tc_after();
+          if (leader && !dead) {
+            const uint64_t a = w_desc + (uint64_t)st * (STAGE >> 4), b = x_desc + (uint64_t)st * (STAGE >> 4);
+#pragma unroll
+            for (int i = 0; i < 4; i++) tc_mma_i8_pair(tmem + NT * set, a + 2 * i, b + 2 * i, IDESC, k > 0 || i > 0);
+            tc_commit_pair(empty + 8 * st);
+          }
+        }
+        if (leader && !dead) tc_commit_pair(done + 8 * set);
+      }
+      if (s_dead && leader) {   // products under way end before the tensor memory goes
+        tc_commit_pair(ending);
+        for (int it = 0; it < MM_WAIT_LIMIT && !mbar_try(ending, 0); it++) {}
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    const unsigned lanes = tmem + ((unsigned)quarter << 21), taken0 = in_block0(taken);
+    int n = 0;
+    for (int tile = pair; tile < p.tiles; tile += pairs, n++) {
+      const int set = n & 1, t0 = tile % p.t_tiles * NT, o = tile / p.t_tiles * 256 + 128 * rank + 32 * quarter + lane;
+      wait(done + 8 * set, (unsigned)(n / 2) & 1);
+      __syncwarp();
+      tc_after();
+      const float so = o < p.O ? p.so[o] : 0.0f;
+#pragma unroll 1
+      for (int c = 0; c < NT; c += 16) {
+        uint32_t acc[16];
+        tmem_ld16(acc, lanes + NT * set + c);
+        if (c + 16 == NT) {
+          tc_before();
+          __syncwarp();
+          if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(taken0 + 8 * set) : "memory");
+        }
+        if (o < p.O) {
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const int t = t0 + c + i;
+            if (t < p.T) p.out[t * p.out_t + o] = f2bf(dead ? NAN : (float)(int)acc[i] * p.sx[t] * so);
+          }
+        }
+      }
+    }
+  }
+  tc_before();
+  __syncthreads();
+  cluster_sync();   // neither block ends while the other may reach into it
+  tc_after();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
 // Rows of 8-bit numbers in boxes of 128 columns; what is behind the last row or column comes as zeros.
 bool bytes_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t stride, int box) {
   const auto encode = tensor_map_encoder();
@@ -242,6 +384,32 @@ int launch(const pk_tensor* x, const pk_tensor* w, MmParams p, cudaStream_t st) 
   return check_launch("matmul_i8");
 }
 
+int launch_pair(const pk_tensor* x, const pk_tensor* w, MmParams p, cudaStream_t st) {
+  CUtensorMap mw, mx;
+  const int64_t I = x->shape[1];
+  if (!bytes_map(&mw, w->data, p.O, I, p.O > 1 ? w->stride[0] : I, 128) || !bytes_map(&mx, x->data, p.T, I, p.T > 1 ? x->stride[0] : I, 128))
+    return fail(PK_ERR_CUDA, "matmul_i8: no tensor map for these rows");
+  static PerDevice opted;
+  if (const unsigned long long bit = first_on_device(opted)) {
+    if (cudaFuncSetAttribute(matmul_i8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MP_SMEM) != cudaSuccess)
+      return fail(PK_ERR_CUDA, "matmul_i8: %s", cudaGetErrorString(cudaGetLastError()));
+    mark_on_device(opted, bit);
+  }
+  p.t_tiles = (p.T + MP_NT - 1) / MP_NT;
+  p.tiles = p.t_tiles * ((p.O + 255) / 256);
+  p.split = 1;
+  const int pairs = sm_count() / 2;
+  StageTimer timer(ST_GEMV, st);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * (p.tiles < pairs ? p.tiles : pairs))), cfg.blockDim = dim3(MM_THREADS), cfg.dynamicSmemBytes = MP_SMEM, cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension, attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, matmul_i8_pair_kernel, mw, mx, p);
+  return check_launch("matmul_i8");
+}
+
 bool rows16(const pk_tensor* t) {
   return (t->shape[1] <= 1 || t->stride[1] == 1) && aligned16(t->data) && (t->shape[0] <= 1 || (t->stride[0] % 16 == 0 && t->stride[0] > 0));
 }
@@ -274,5 +442,6 @@ extern "C" int pk_matmul_i8(const pk_tensor* x, const pk_tensor* x_scales, const
   if (T <= 32) return launch<32>(x, weight, p, st);
   if (T <= 64) return launch<64>(x, weight, p, st);
   if (T <= 128) return launch<128>(x, weight, p, st);
+  if ((T + 255) / 256 * ((O + 255) / 256) >= sm_count() / 2) return launch_pair(x, weight, p, st);
   return launch<256>(x, weight, p, st);
 }

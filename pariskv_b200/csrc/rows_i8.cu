@@ -7,7 +7,6 @@ namespace pk {
 namespace {
 
 enum { NORM, PLAIN, GATED };
-constexpr int THREADS = 512;
 
 struct RowParams {
   const uint16_t *a, *r, *w;
@@ -16,12 +15,21 @@ struct RowParams {
   uint8_t* codes;
   float* scales;
   int n;
-  double eps;
+  double eps, one_n;   // one_n: 1 / n
 };
 
 __device__ __forceinline__ float part(uint32_t w, int i) { return __uint_as_float(i ? w & 0xffff0000u : w << 16); }
 
-template <int MODE, int N>   // N groups of 8 values a thread
+// 1 / sqrt(x) to the last bits of 64, by Newton's iteration from 32 bits: every thread computes it, and a division and a root of 64 bits are some hundred instructions.
+__device__ __forceinline__ double inverse_root(double x) {
+  if (!(x > 1e-30 && x < 1e30)) return 1.0 / sqrt(x);
+  double r = rsqrtf((float)x);
+#pragma unroll
+  for (int i = 0; i < 2; i++) r = fma(0.5 * r, fma(-x * r, r, 1.0), r);
+  return r;
+}
+
+template <int MODE, int THREADS, int N>   // N groups of 8 values a thread
 __global__ void __launch_bounds__(THREADS) rows_i8_kernel(const __grid_constant__ RowParams p) {
   __shared__ double s_sum[THREADS / 32];
   __shared__ uint32_t s_max[THREADS / 32];
@@ -62,7 +70,7 @@ __global__ void __launch_bounds__(THREADS) rows_i8_kernel(const __grid_constant_
     ss = 0.0;
 #pragma unroll
     for (int i = 0; i < THREADS / 32; i++) ss += s_sum[i];
-    const float rstd = (float)(1.0 / sqrt(ss / (double)p.n + p.eps));
+    const float rstd = (float)inverse_root(fma(ss, p.one_n, p.eps));
 #pragma unroll
     for (int k = 0; k < N; k++) {
       const int i = (k * THREADS + tid) * 8;
@@ -104,32 +112,38 @@ __global__ void __launch_bounds__(THREADS) rows_i8_kernel(const __grid_constant_
 #pragma unroll
   for (int i = 0; i < THREADS / 32; i++) m = max(m, s_max[i]);
   const bool fine = m < 0x7f800000u;
-  const float amax = __uint_as_float(m), unit = m == 0 ? 1.0f : __fmul_rn(amax, 0.0078125f);
+  const float amax = __uint_as_float(m);
+  const Coder<false> code(amax);
 #pragma unroll
   for (int k = 0; k < N; k++) {
     const int i = (k * THREADS + tid) * 8;
     if (i < p.n) {
-      float q[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) q[e] = i8_quotient(y[k][e], unit);
-      uint2 o = make_uint2(pack_i8(q[0], q[1], q[2], q[3]), pack_i8(q[4], q[5], q[6], q[7]));
-      if (!fine) o = make_uint2(0, 0);
+      uint2 o = make_uint2(0, 0);
+      if (fine) o = code(y[k]);
       *reinterpret_cast<uint2*>(p.codes + row * p.c_s + i) = o;
     }
   }
   if (tid == 0) p.scales[row] = fine ? __fdiv_rn(amax, 127.0f) : NAN;
 }
 
+template <int MODE, int THREADS, int N>
+void launch_as(const RowParams& p, int64_t rows, cudaStream_t st) {
+  launch_chain(rows_i8_kernel<MODE, THREADS, N>, dim3((unsigned)rows), dim3(THREADS), 0, st, p);
+}
+// Few rows: 512 threads, a group of eight values each as far as that goes, for the shortest way through a row.  Many: four groups a thread, so that a block has few warps to wait for and an SM more blocks
+// at different places.
 template <int MODE>
 int launch(const RowParams& p, int64_t rows, const char* what, cudaStream_t st) {
   StageTimer timer(ST_GLUE, st);
-  const int per = THREADS * 8;
-  const dim3 grid((unsigned)rows), block(THREADS);
-  if (p.n <= per) launch_chain(rows_i8_kernel<MODE, 1>, grid, block, 0, st, p);
-  else if (p.n <= 2 * per) launch_chain(rows_i8_kernel<MODE, 2>, grid, block, 0, st, p);
-  else if (p.n <= 4 * per) launch_chain(rows_i8_kernel<MODE, 4>, grid, block, 0, st, p);
-  else if (p.n <= 8 * per) launch_chain(rows_i8_kernel<MODE, 8>, grid, block, 0, st, p);
-  else launch_chain(rows_i8_kernel<MODE, 16>, grid, block, 0, st, p);
+  const bool many = rows >= 2 * sm_count();
+  if (many && p.n <= 2048) launch_as<MODE, 64, 4>(p, rows, st);
+  else if (many && p.n <= 4096) launch_as<MODE, 128, 4>(p, rows, st);
+  else if (many && p.n <= 8192) launch_as<MODE, 256, 4>(p, rows, st);
+  else if (p.n <= 4096) launch_as<MODE, 512, 1>(p, rows, st);
+  else if (p.n <= 8192) launch_as<MODE, 512, 2>(p, rows, st);
+  else if (p.n <= 16384) launch_as<MODE, 512, 4>(p, rows, st);
+  else if (p.n <= 32768) launch_as<MODE, 512, 8>(p, rows, st);
+  else launch_as<MODE, 512, 16>(p, rows, st);
   return check_launch(what);
 }
 
@@ -174,7 +188,7 @@ extern "C" int pk_add_rmsnorm_i8(const pk_tensor* a, const pk_tensor* residual, 
   if (B == 0) return PK_OK;
   RowParams p = {};
   p.a = (const uint16_t*)a->data, p.r = residual ? (const uint16_t*)residual->data : nullptr, p.w = (const uint16_t*)weight->data, p.h = (uint16_t*)h_out->data;
-  p.codes = (uint8_t*)codes->data, p.scales = (float*)scales->data, p.n = (int)n, p.eps = eps;
+  p.codes = (uint8_t*)codes->data, p.scales = (float*)scales->data, p.n = (int)n, p.eps = eps, p.one_n = 1.0 / (double)n;
   p.a_s = a->stride[0], p.r_s = residual ? residual->stride[0] : 0, p.h_s = h_out->stride[0], p.c_s = codes->stride[0];
   return launch<NORM>(p, B, "add_rmsnorm_i8", (cudaStream_t)stream);
 }
