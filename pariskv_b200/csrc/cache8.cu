@@ -30,10 +30,16 @@ __global__ void __launch_bounds__(256)
   auto place = [&](int64_t r) { return ring + (r % c.R) * c.r_l; };
   if (row0 + BLOCK <= end) {
     uint4 x[N];
+    if (row0 >= first) {
+      const uint16_t* src = from + (row0 + warp - start) * from_t;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const int64_t r = row0 + 8 * i + warp;
-      x[i] = *reinterpret_cast<const uint4*>(r >= first ? from + (r - start) * from_t : place(r));
+      for (int i = 0; i < N; i++, src += 8 * from_t) x[i] = *reinterpret_cast<const uint4*>(src);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const int64_t r = row0 + 8 * i + warp;
+        x[i] = *reinterpret_cast<const uint4*>(r >= first ? from + (r - start) * from_t : place(r));
+      }
     }
     uint32_t m = 0;
 #pragma unroll
@@ -52,8 +58,8 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < 8; i++) m = max(m, s_max[i][kv]);
     const float amax = bf2f((uint16_t)m);
     const bool fine = m < 0x7f80u;
-    const Coder<E4M3> code(amax);
-    uint8_t* to = c.codes + b * c.c_b + h * c.c_h + kv * c.c_kv + ch;
+    const Coder<E4M3, true> code(amax);
+    uint8_t* to = c.codes + b * c.c_b + h * c.c_h + kv * c.c_kv + ch + (row0 + warp) * c.c_l;
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
@@ -62,9 +68,10 @@ __global__ void __launch_bounds__(256)
       for (int e = 0; e < 8; e++) y[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
       uint2 o = make_uint2(0, 0);
       if (fine) o = code(y);
-      *reinterpret_cast<uint2*>(to + (row0 + 8 * i + warp) * c.c_l) = o;
+      *reinterpret_cast<uint2*>(to) = o;
+      to += 8 * c.c_l;
     }
-    if (warp == 0 && (lane & 15) == 0) c.scales[b * c.s_b + h * c.s_h + j * c.s_j + kv * c.s_kv] = fine ? __fdiv_rn(amax, Coder<E4M3>::MOST) : NAN;
+    if (warp == 0 && (lane & 15) == 0) c.scales[b * c.s_b + h * c.s_h + j * c.s_j + kv * c.s_kv] = fine ? __fdiv_rn(amax, Coder<E4M3, true>::MOST) : NAN;
   }
   // The last R rows stay in 16 bits.  Rows of the first block that were there before may lie where new ones go: the thread block that reads them also
   // writes what replaces them.

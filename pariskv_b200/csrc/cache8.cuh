@@ -77,18 +77,21 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
 }
 // Codes of values whose largest magnitude is amax:  y M / amax to the nearest, ties to the even one, M = 127 (e4m3: 448), as 32-bit arithmetic gives it from (y M / u) / (amax / u) with a power of two
 // u = 128 (512).  A division per value took two thirds of the kernels' instructions.  Instead each is multiplied by a factor that is surely above M / amax and by one that is surely below: where both round
-// to the same code that is the code, whatever the last bits.  Others, one group of eight values in some hundred, are divided.
-template <bool E4M3>
+// to the same code that is the code, whatever the last bits.  EXACT (whole numbers of values of 16 bits): the others, which are ties or next to one, go by the sign of 2 y' - (n + n') unit, y' = y M / u,
+// n and n' the two codes: products of 16 bits, one rounding.  Ties are a matter of the block's largest value - 128, 192, 160 times a power of two have many - and a division took a quarter of such a block's time.
+template <bool E4M3, bool EXACT>
 struct Coder {
   static constexpr float MOST = E4M3 ? 448.0f : 127.0f, U = E4M3 ? 512.0f : 128.0f;
   float unit, above, below;
+  bool plain;
   __device__ __forceinline__ explicit Coder(float amax) {
     unit = amax == 0.0f ? 1.0f : __fmul_rn(amax, 1.0f / U);
     const float f = __fdiv_rn(MOST, amax);
-    const bool plain = amax > 1e-30f;   // (else the factor might be infinite)
+    plain = amax > 1e-30f;   // (else the factor might be infinite)
     above = plain ? f * (1.0f + 0x1p-21f) : INFINITY, below = plain ? f * (1.0f - 0x1p-21f) : 0.0f;   // f is off by 2^-24 of itself, this product too; the quotient is off by 2^-23
   }
   __device__ __forceinline__ float quotient(float y) const { return __fdiv_rn(__fmul_rn(y, MOST / U), unit); }
+  static __device__ __forceinline__ uint32_t bytes(const uint32_t* n) { return __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410); }
   __device__ __forceinline__ uint2 operator()(const float (&y)[8]) const {
     uint32_t a[2], differ = 0;
     if (E4M3) {
@@ -97,6 +100,10 @@ struct Coder {
         a[i] = pack_e4m3(y[4 * i] * above, y[4 * i + 1] * above, y[4 * i + 2] * above, y[4 * i + 3] * above);
         differ |= a[i] ^ pack_e4m3(y[4 * i] * below, y[4 * i + 1] * below, y[4 * i + 2] * below, y[4 * i + 3] * below);
       }
+      if (differ) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) a[i] = pack_e4m3(quotient(y[4 * i]), quotient(y[4 * i + 1]), quotient(y[4 * i + 2]), quotient(y[4 * i + 3]));
+      }
     } else {
       uint32_t n[8];
 #pragma unroll
@@ -104,24 +111,21 @@ struct Coder {
         n[i] = __float_as_uint(__fmaf_rn(y[i], above, 12582912.0f));
         differ |= n[i] ^ __float_as_uint(__fmaf_rn(y[i], below, 12582912.0f));
       }
+      if (differ) {
+        if (EXACT && plain) {
 #pragma unroll
-      for (int i = 0; i < 2; i++) a[i] = __byte_perm(__byte_perm(n[4 * i], n[4 * i + 1], 0x0040), __byte_perm(n[4 * i + 2], n[4 * i + 3], 0x0040), 0x5410);
-    }
-    if (differ) {
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        float q[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++) q[e] = quotient(y[4 * i + e]);
-        if (E4M3) {
-          a[i] = pack_e4m3(q[0], q[1], q[2], q[3]);
+          for (int i = 0; i < 8; i++) {
+            const uint32_t m = __float_as_uint(__fmaf_rn(y[i], below, 12582912.0f));
+            const float both = (__uint_as_float(n[i]) - 12582912.0f) + (__uint_as_float(m) - 12582912.0f);
+            const float d = __fmaf_rn(2.0f, __fmul_rn(y[i], MOST / U), -both * unit) * (y[i] < 0.0f ? -1.0f : 1.0f);   // above zero: n, which is the one of the larger magnitude
+            n[i] = d > 0.0f || (d == 0.0f && (n[i] & 1) == 0) ? n[i] : m;
+          }
         } else {
-          uint32_t n[4];
 #pragma unroll
-          for (int e = 0; e < 4; e++) n[e] = (uint32_t)__float2int_rn(q[e]);
-          a[i] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+          for (int i = 0; i < 8; i++) n[i] = (uint32_t)__float2int_rn(quotient(y[i]));
         }
       }
+      a[0] = bytes(n), a[1] = bytes(n + 4);
     }
     return make_uint2(a[0], a[1]);
   }

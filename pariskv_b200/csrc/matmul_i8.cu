@@ -39,6 +39,36 @@ __device__ __forceinline__ void tmem_ld16(uint32_t (&r)[16], unsigned addr) {
                : "r"(addr)
                : "memory");
 }
+// A lane's row of sums - matrix row o, `n` tokens from t0 on - out of tensor memory, scaled and stored; sx: the tokens' scales.  All of a step's reads come before its stores, which the compiler
+// must not reorder.
+template <class Free>
+__device__ __forceinline__ void mm_store(const MmParams& p, unsigned addr, int n, int t0, int o, const float* sx, bool dead, Free all_read) {
+  const float so = o < p.O ? p.so[o] : 0.0f;
+  uint16_t* to = p.out + t0 * p.out_t + o;
+  const bool inside = t0 + n <= p.T;
+#pragma unroll 1
+  for (int c = 0; c < n; c += 16) {
+    uint32_t acc[16];
+    tmem_ld16(acc, addr + c);
+    if (c + 16 == n) all_read();
+    uint16_t y[16];
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const float4 s = *reinterpret_cast<const float4*>(sx + c + i);
+      y[i] = f2bf((float)(int)acc[i] * s.x * so), y[i + 1] = f2bf((float)(int)acc[i + 1] * s.y * so);
+      y[i + 2] = f2bf((float)(int)acc[i + 2] * s.z * so), y[i + 3] = f2bf((float)(int)acc[i + 3] * s.w * so);
+    }
+    if (dead) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) y[i] = 0x7fff;
+    }
+    if (o < p.O) {
+#pragma unroll
+      for (int i = 0; i < 16; i++, to += p.out_t)
+        if (inside || t0 + c + i < p.T) *to = y[i];
+    }
+  }
+}
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint4 remote16(unsigned at, unsigned rank) {   // the same place in the shared memory of block `rank` of the cluster
   uint4 r;
@@ -58,6 +88,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_c
   extern __shared__ unsigned char dyn[];
   __shared__ __align__(8) unsigned long long bars[2 * NS + 5];
   __shared__ unsigned s_tmem;
+  __shared__ __align__(16) float s_sx[2][NT];
   __shared__ __align__(16) volatile int s_dead;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const unsigned ring = (smem_addr(dyn) + 1023) & ~1023u;
@@ -137,27 +168,18 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_c
     int n = 0;
     for (int tile = cluster; tile < p.tiles; tile += clusters, n++) {
       const int set = n & 1, t0 = tile % p.t_tiles * NT, o = tile / p.t_tiles * MM_ROWS + o_lane;
+      if (p.split == 1) {   // (the threads before the ones of this tile have passed the barrier of the tile before: two places do)
+        for (int i = tid - 64; i < NT; i += 128) s_sx[set][i] = t0 + i < p.T ? p.sx[t0 + i] : 0.0f;
+        named_barrier(1, 128);
+      }
       wait(done + 8 * set, (unsigned)(n / 2) & 1);
       __syncwarp();
       tc_after();
-      const float so = o < p.O ? p.so[o] : 0.0f;
       if (p.split == 1) {
-#pragma unroll 1
-        for (int c = 0; c < NT; c += 16) {
-          uint32_t acc[16];
-          tmem_ld16(acc, lanes + COLS * set + c);
-          if (c + 16 == NT) {
-            tc_before();
-            mbar_arrive1(taken + 8 * set);
-          }
-          if (o < p.O) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const int t = t0 + c + i;
-              if (t < p.T) p.out[t * p.out_t + o] = f2bf(dead ? NAN : (float)(int)acc[i] * p.sx[t] * so);
-            }
-          }
-        }
+        mm_store(p, lanes + COLS * set, NT, t0, o, s_sx[set], dead, [&] {
+          tc_before();
+          mbar_arrive1(taken + 8 * set);
+        });
       } else {
         // this block's partial sums, column by column, where the copies were (they have all been multiplied)
 #pragma unroll 1
@@ -229,6 +251,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_pair_kernel(const __g
   extern __shared__ unsigned char dyn[];
   __shared__ __align__(8) unsigned long long bars[2 * NS + 5];
   __shared__ unsigned s_tmem;
+  __shared__ __align__(16) float s_sx[2][NT];
   __shared__ volatile int s_dead;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const unsigned ring = (smem_addr(dyn) + 1023) & ~1023u;
@@ -314,27 +337,16 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_pair_kernel(const __g
     int n = 0;
     for (int tile = pair; tile < p.tiles; tile += pairs, n++) {
       const int set = n & 1, t0 = tile % p.t_tiles * NT, o = tile / p.t_tiles * 256 + 128 * rank + 32 * quarter + lane;
+      for (int i = tid - 64; i < NT; i += 128) s_sx[set][i] = t0 + i < p.T ? p.sx[t0 + i] : 0.0f;
+      named_barrier(1, 128);
       wait(done + 8 * set, (unsigned)(n / 2) & 1);
       __syncwarp();
       tc_after();
-      const float so = o < p.O ? p.so[o] : 0.0f;
-#pragma unroll 1
-      for (int c = 0; c < NT; c += 16) {
-        uint32_t acc[16];
-        tmem_ld16(acc, lanes + NT * set + c);
-        if (c + 16 == NT) {
-          tc_before();
-          __syncwarp();
-          if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(taken0 + 8 * set) : "memory");
-        }
-        if (o < p.O) {
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const int t = t0 + c + i;
-            if (t < p.T) p.out[t * p.out_t + o] = f2bf(dead ? NAN : (float)(int)acc[i] * p.sx[t] * so);
-          }
-        }
-      }
+      mm_store(p, lanes + NT * set, NT, t0, o, s_sx[set], dead, [&] {
+        tc_before();
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(taken0 + 8 * set) : "memory");
+      });
     }
   }
   tc_before();

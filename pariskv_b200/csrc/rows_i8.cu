@@ -39,27 +39,40 @@ __global__ void __launch_bounds__(THREADS) rows_i8_kernel(const __grid_constant_
   const int64_t row = blockIdx.x;
   float y[N][8];
   if (MODE == NORM) {
-    uint4 h[N];
+    constexpr int M = N < 4 ? N : 4;   // groups whose loads are all under way before the first is used
     double ss = 0.0;
 #pragma unroll
-    for (int k = 0; k < N; k++) {
-      const int i = (k * THREADS + tid) * 8;
-      h[k] = make_uint4(0, 0, 0, 0);
-      if (i < p.n) {
-        h[k] = *reinterpret_cast<const uint4*>(p.a + row * p.a_s + i);
-        uint32_t* hw = reinterpret_cast<uint32_t*>(&h[k]);
-        if (p.r) {
-          const uint4 rv = *reinterpret_cast<const uint4*>(p.r + row * p.r_s + i);
-          const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
+    for (int k0 = 0; k0 < N; k0 += M) {
+      uint4 h[M], rv[M];
 #pragma unroll
-          for (int e = 0; e < 4; e++) hw[e] = (uint32_t)f2bf(part(hw[e], 0) + part(rw[e], 0)) | (uint32_t)f2bf(part(hw[e], 1) + part(rw[e], 1)) << 16;
+      for (int k = 0; k < M; k++) {
+        const int i = ((k0 + k) * THREADS + tid) * 8;
+        h[k] = i < p.n ? *reinterpret_cast<const uint4*>(p.a + row * p.a_s + i) : make_uint4(0, 0, 0, 0);
+      }
+      if (p.r) {
+#pragma unroll
+        for (int k = 0; k < M; k++) {
+          const int i = ((k0 + k) * THREADS + tid) * 8;
+          rv[k] = i < p.n ? *reinterpret_cast<const uint4*>(p.r + row * p.r_s + i) : make_uint4(0, 0, 0, 0);
         }
-        *reinterpret_cast<uint4*>(p.h + row * p.h_s + i) = h[k];
+      }
+#pragma unroll
+      for (int k = 0; k < M; k++) {
+        const int i = ((k0 + k) * THREADS + tid) * 8;
+        uint32_t hw[4] = {h[k].x, h[k].y, h[k].z, h[k].w};
+        if (p.r) {
+          const uint32_t rw[4] = {rv[k].x, rv[k].y, rv[k].z, rv[k].w};
+#pragma unroll
+          for (int e = 0; e < 4; e++) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hw[e]) : "f"(part(hw[e], 1) + part(rw[e], 1)), "f"(part(hw[e], 0) + part(rw[e], 0)));
+        }
+        if (i < p.n) *reinterpret_cast<uint4*>(p.h + row * p.h_s + i) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const float f = part(hw[e >> 1], e & 1);
-          y[k][e] = f;
-          ss = fma((double)f, (double)f, ss);
+          y[k0 + k][e] = f;
+          // f as a double, by its bits (a conversion takes four times as long): what is below 2^-126 counts as at most that, what is not a number as 2^128 - the row's maximum tells
+          const double d = __hiloint2double((int)((__float_as_uint(f) & 0x7fffffffu) >> 3) + 0x38000000, 0);
+          ss = fma(d, d, ss);
         }
       }
     }
@@ -70,7 +83,7 @@ __global__ void __launch_bounds__(THREADS) rows_i8_kernel(const __grid_constant_
     ss = 0.0;
 #pragma unroll
     for (int i = 0; i < THREADS / 32; i++) ss += s_sum[i];
-    const float rstd = (float)inverse_root(fma(ss, p.one_n, p.eps));
+    const float rstd = (float)inverse_root(fma(ss < 1e-70 ? 0.0 : ss, p.one_n, p.eps));
 #pragma unroll
     for (int k = 0; k < N; k++) {
       const int i = (k * THREADS + tid) * 8;
@@ -87,11 +100,11 @@ __global__ void __launch_bounds__(THREADS) rows_i8_kernel(const __grid_constant_
       const int i = (k * THREADS + tid) * 8;
       if (i < p.n) {
         const uint4 xv = *reinterpret_cast<const uint4*>(p.a + row * p.a_s + i);
+        const uint4 uv = MODE == GATED ? *reinterpret_cast<const uint4*>(p.a + row * p.a_s + p.n + i) : make_uint4(0, 0, 0, 0);
         const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
 #pragma unroll
         for (int e = 0; e < 8; e++) y[k][e] = part(xw[e >> 1], e & 1);
         if (MODE == GATED) {
-          const uint4 uv = *reinterpret_cast<const uint4*>(p.a + row * p.a_s + p.n + i);
           const uint32_t uw[4] = {uv.x, uv.y, uv.z, uv.w};
 #pragma unroll
           for (int e = 0; e < 8; e++) y[k][e] = y[k][e] / (1.0f + expf(-y[k][e])) * part(uw[e >> 1], e & 1);
@@ -113,7 +126,7 @@ __global__ void __launch_bounds__(THREADS) rows_i8_kernel(const __grid_constant_
   for (int i = 0; i < THREADS / 32; i++) m = max(m, s_max[i]);
   const bool fine = m < 0x7f800000u;
   const float amax = __uint_as_float(m);
-  const Coder<false> code(amax);
+  const Coder<false, MODE == PLAIN> code(amax);
 #pragma unroll
   for (int k = 0; k < N; k++) {
     const int i = (k * THREADS + tid) * 8;
