@@ -44,10 +44,8 @@ __global__ void __launch_bounds__(256)
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      m = __vmaxu2(m, x[i].x & 0x7fff7fffu);
-      m = __vmaxu2(m, x[i].y & 0x7fff7fffu);
-      m = __vmaxu2(m, x[i].z & 0x7fff7fffu);
-      m = __vmaxu2(m, x[i].w & 0x7fff7fffu);
+      m = __vimax3_u16x2(m, x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu);
+      m = __vimax3_u16x2(m, x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu);
     }
     m = max(m & 0xffffu, m >> 16);
 #pragma unroll
@@ -58,20 +56,23 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < 8; i++) m = max(m, s_max[i][kv]);
     const float amax = bf2f((uint16_t)m);
     const bool fine = m < 0x7f80u;
-    const Coder<E4M3, true> code(amax);
+    const Coder16<E4M3> code(amax);
     uint8_t* to = c.codes + b * c.c_b + h * c.c_h + kv * c.c_kv + ch + (row0 + warp) * c.c_l;
+    auto store = [&](auto encode) {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      float y[8];
+      for (int i = 0; i < N; i++) {
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++) y[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
-      uint2 o = make_uint2(0, 0);
-      if (fine) o = code(y);
-      *reinterpret_cast<uint2*>(to) = o;
-      to += 8 * c.c_l;
-    }
-    if (warp == 0 && (lane & 15) == 0) c.scales[b * c.s_b + h * c.s_h + j * c.s_j + kv * c.s_kv] = fine ? __fdiv_rn(amax, Coder<E4M3, true>::MOST) : NAN;
+        for (int e = 0; e < 8; e++) y[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+        *reinterpret_cast<uint2*>(to) = encode(y);
+        to += 8 * c.c_l;
+      }
+    };
+    if (!fine) store([](const float (&)[8]) { return make_uint2(0, 0); });
+    else if (!code.plain) store([&](const float (&y)[8]) { return code.divided(y); });
+    else store(code);
+    if (warp == 0 && (lane & 15) == 0) c.scales[b * c.s_b + h * c.s_h + j * c.s_j + kv * c.s_kv] = fine ? __fdiv_rn(amax, CodeScale<E4M3>::MOST) : NAN;
   }
   // The last R rows stay in 16 bits.  Rows of the first block that were there before may lie where new ones go: the thread block that reads them also
   // writes what replaces them.

@@ -76,58 +76,66 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
   return (uint32_t)lo | (uint32_t)hi << 16;
 }
 // Codes of values whose largest magnitude is amax:  y M / amax to the nearest, ties to the even one, M = 127 (e4m3: 448), as 32-bit arithmetic gives it from (y M / u) / (amax / u) with a power of two
-// u = 128 (512).  A division per value took two thirds of the kernels' instructions.  Instead each is multiplied by a factor that is surely above M / amax and by one that is surely below: where both round
-// to the same code that is the code, whatever the last bits.  EXACT (whole numbers of values of 16 bits): the others, which are ties or next to one, go by the sign of 2 y' - (n + n') unit, y' = y M / u,
-// n and n' the two codes: products of 16 bits, one rounding.  Ties are a matter of the block's largest value - 128, 192, 160 times a power of two have many - and a division took a quarter of such a block's time.
-template <bool E4M3, bool EXACT>
-struct Coder {
+// u = 128 (512), which keeps the product from overflowing.  A division per value took two thirds of the kernels' instructions.
+constexpr float CODE_MAGIC = 12582912.0f;   // 1.5 2^23: a sum with it ends in the whole number that the other is rounded to
+__device__ __forceinline__ uint32_t code_bytes(const uint32_t* n) { return __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410); }
+template <bool E4M3>
+__device__ __forceinline__ uint32_t code_pack(const float* q) {
+  if (E4M3) return pack_e4m3(q[0], q[1], q[2], q[3]);
+  uint32_t n[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) n[e] = __float_as_uint(q[e] + CODE_MAGIC);
+  return code_bytes(n);
+}
+template <bool E4M3>
+struct CodeScale {
   static constexpr float MOST = E4M3 ? 448.0f : 127.0f, U = E4M3 ? 512.0f : 128.0f;
-  float unit, above, below;
-  bool plain;
-  __device__ __forceinline__ explicit Coder(float amax) {
-    unit = amax == 0.0f ? 1.0f : __fmul_rn(amax, 1.0f / U);
-    const float f = __fdiv_rn(MOST, amax);
-    plain = amax > 1e-30f;   // (else the factor might be infinite)
+  float unit;
+  bool plain;   // factors are finite
+  __device__ __forceinline__ explicit CodeScale(float amax) : unit(amax == 0.0f ? 1.0f : amax * (1.0f / U)), plain(amax > 1e-30f) {}
+  __device__ __forceinline__ float quotient(float y) const { return (y * (MOST / U)) / unit; }
+  __device__ __forceinline__ uint2 divided(const float (&y)[8]) const {
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) q[i] = quotient(y[i]);
+    return make_uint2(code_pack<E4M3>(q), code_pack<E4M3>(q + 4));
+  }
+};
+// Of values and a maximum of 16 bits: one Newton step.  y' = y M / u is exact, q1 = y' r with r near 1 / unit, rem = y' - q1 unit is exact (8 bits), and q1 + rem r is within 2^-44 of the quotient before
+// its rounding: a tie, which is a number of nine bits, comes out as it is, and no other quotient is nearer to one than 2^-17 of itself.  Ties are a matter of the maximum: 128, 192, 160 times a power
+// of two have many, so that a form with an exception for them took it for a third of all groups.
+template <bool E4M3>
+struct Coder16 : CodeScale<E4M3> {
+  float r;
+  __device__ __forceinline__ explicit Coder16(float amax) : CodeScale<E4M3>(amax) { asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(this->unit)); }
+  __device__ __forceinline__ uint2 operator()(const float (&y)[8]) const {
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {   // two values an instruction
+      asm("{\n\t.reg .b64 y, q, e, r, u, m;\n\tmov.b64 y, {%2, %3};\n\tmov.b64 r, {%4, %4};\n\tmov.b64 u, {%5, %5};\n\tmov.b64 m, {%6, %6};\n\t"
+          "mul.rn.f32x2 y, y, m;\n\tmul.rn.f32x2 q, y, r;\n\tfma.rn.f32x2 e, q, u, y;\n\tfma.rn.f32x2 q, e, r, q;\n\tmov.b64 {%0, %1}, q;\n\t}"
+          : "=f"(q[i]), "=f"(q[i + 1])
+          : "f"(y[i]), "f"(y[i + 1]), "f"(r), "f"(-this->unit), "f"(CodeScale<E4M3>::MOST / CodeScale<E4M3>::U));
+    }
+    return make_uint2(code_pack<E4M3>(q), code_pack<E4M3>(q + 4));
+  }
+};
+// Whole numbers of values of 32 bits: each is multiplied by a factor that is surely above M / amax and by one that is surely below: where both round to the same code that is the code, whatever the last
+// bits.  Others, one group of eight values in some hundred, are divided.
+struct Coder32 : CodeScale<false> {
+  float above, below;
+  __device__ __forceinline__ explicit Coder32(float amax) : CodeScale<false>(amax) {
+    const float f = MOST / amax;
     above = plain ? f * (1.0f + 0x1p-21f) : INFINITY, below = plain ? f * (1.0f - 0x1p-21f) : 0.0f;   // f is off by 2^-24 of itself, this product too; the quotient is off by 2^-23
   }
-  __device__ __forceinline__ float quotient(float y) const { return __fdiv_rn(__fmul_rn(y, MOST / U), unit); }
-  static __device__ __forceinline__ uint32_t bytes(const uint32_t* n) { return __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410); }
   __device__ __forceinline__ uint2 operator()(const float (&y)[8]) const {
-    uint32_t a[2], differ = 0;
-    if (E4M3) {
+    uint32_t n[8], differ = 0;
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        a[i] = pack_e4m3(y[4 * i] * above, y[4 * i + 1] * above, y[4 * i + 2] * above, y[4 * i + 3] * above);
-        differ |= a[i] ^ pack_e4m3(y[4 * i] * below, y[4 * i + 1] * below, y[4 * i + 2] * below, y[4 * i + 3] * below);
-      }
-      if (differ) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) a[i] = pack_e4m3(quotient(y[4 * i]), quotient(y[4 * i + 1]), quotient(y[4 * i + 2]), quotient(y[4 * i + 3]));
-      }
-    } else {
-      uint32_t n[8];
-#pragma unroll
-      for (int i = 0; i < 8; i++) {   // the sum with 1.5 2^23 ends in the whole number
-        n[i] = __float_as_uint(__fmaf_rn(y[i], above, 12582912.0f));
-        differ |= n[i] ^ __float_as_uint(__fmaf_rn(y[i], below, 12582912.0f));
-      }
-      if (differ) {
-        if (EXACT && plain) {
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const uint32_t m = __float_as_uint(__fmaf_rn(y[i], below, 12582912.0f));
-            const float both = (__uint_as_float(n[i]) - 12582912.0f) + (__uint_as_float(m) - 12582912.0f);
-            const float d = __fmaf_rn(2.0f, __fmul_rn(y[i], MOST / U), -both * unit) * (y[i] < 0.0f ? -1.0f : 1.0f);   // above zero: n, which is the one of the larger magnitude
-            n[i] = d > 0.0f || (d == 0.0f && (n[i] & 1) == 0) ? n[i] : m;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; i++) n[i] = (uint32_t)__float2int_rn(quotient(y[i]));
-        }
-      }
-      a[0] = bytes(n), a[1] = bytes(n + 4);
+    for (int i = 0; i < 8; i++) {
+      n[i] = __float_as_uint(__fmaf_rn(y[i], above, CODE_MAGIC));
+      differ |= n[i] ^ __float_as_uint(__fmaf_rn(y[i], below, CODE_MAGIC));
     }
-    return make_uint2(a[0], a[1]);
+    return differ ? divided(y) : make_uint2(code_bytes(n), code_bytes(n + 4));
   }
 };
 #endif

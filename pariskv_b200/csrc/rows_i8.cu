@@ -1,6 +1,8 @@
 // Rows of 16-bit values as 8-bit whole numbers with a scale per row: of a residual stream through its norm, of a gated activation, or of the rows themselves.
 //   y = bf16(a + r) rstd w  |  silu(g) u  |  x,      scale = max |y| / 127,   code = y 127 / max |y| to the nearest
 // A block per row; the row stays in registers through both reductions.
+#include <type_traits>
+
 #include "cache8.cuh"
 
 namespace pk {
@@ -126,13 +128,13 @@ __global__ void __launch_bounds__(THREADS) rows_i8_kernel(const __grid_constant_
   for (int i = 0; i < THREADS / 32; i++) m = max(m, s_max[i]);
   const bool fine = m < 0x7f800000u;
   const float amax = __uint_as_float(m);
-  const Coder<false, MODE == PLAIN> code(amax);
+  const std::conditional_t<MODE == PLAIN, Coder16<false>, Coder32> code(amax);
 #pragma unroll
   for (int k = 0; k < N; k++) {
     const int i = (k * THREADS + tid) * 8;
     if (i < p.n) {
       uint2 o = make_uint2(0, 0);
-      if (fine) o = code(y[k]);
+      if (fine) o = MODE == PLAIN && !code.plain ? code.divided(y[k]) : code(y[k]);
       *reinterpret_cast<uint2*>(p.codes + row * p.c_s + i) = o;
     }
   }
