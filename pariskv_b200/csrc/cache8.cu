@@ -94,11 +94,11 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// A warp per row, eight rows in flight.
+// A warp per row, eight rows in flight; four where they are listed, which are fewer.
 template <bool E4M3, bool LISTED>
 __global__ void __launch_bounds__(256) cache8_read_kernel(const __grid_constant__ Cache8 c, const int32_t* lengths, const int64_t* rows, uint16_t* out, int64_t o_b, int64_t o_h, int64_t o_l,
                                                           int64_t o_kv, int64_t n) {
-  constexpr int N = 8;
+  constexpr int N = LISTED ? 4 : 8;
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kv = lane >> 4, ch = (lane & 15) * 8;
@@ -199,7 +199,8 @@ extern "C" int pk_cache8_read(const pk_cache8* cache, const pk_tensor* lengths, 
     PK_REQUIRE(n <= c.cap, "out has more rows than the cache");
   }
   if (bs == 0 || n == 0) return PK_OK;
-  const dim3 grid((unsigned)((n + 63) / 64), (unsigned)c.H, (unsigned)bs);
+  const int per = rows ? 32 : 64;
+  const dim3 grid((unsigned)((n + per - 1) / per), (unsigned)c.H, (unsigned)bs);
   const cudaStream_t st = (cudaStream_t)stream;
   StageTimer timer(ST_GATHER, st);
 #define PK_LAUNCH(E, L)                                                                                                                                                           \

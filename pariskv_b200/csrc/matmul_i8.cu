@@ -22,7 +22,10 @@ struct MmParams {
   int split;          // blocks of a cluster
 };
 
-template <int NT> struct MmRing { static constexpr int bytes = MM_ROWS * MM_K + NT * MM_K, stages = NT >= 256 ? 4 : NT >= 128 ? 6 : NT >= 64 ? 8 : 10; };
+// Two blocks per SM: the start and the end of one lie under the copies of the other.
+template <int NT> struct MmRing {
+  static constexpr int bytes = MM_ROWS * MM_K + NT * MM_K, ctas = 2, stages = NT >= 128 ? 3 : NT >= 64 ? 4 : 5;
+};
 template <int NT> constexpr int mm_smem() { return 1024 + MmRing<NT>::stages * MmRing<NT>::bytes; }
 
 __device__ __forceinline__ void tma_load2(unsigned dst, const CUtensorMap* map, int c0, int c1, unsigned mb) {
@@ -82,7 +85,7 @@ __device__ __forceinline__ unsigned remote4(unsigned at, unsigned rank) {
 }
 
 template <int NT>
-__global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ MmParams p) {
+__global__ void __launch_bounds__(MM_THREADS, MmRing<NT>::ctas) matmul_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ MmParams p) {
   constexpr int NS = MmRing<NT>::stages, STAGE = MmRing<NT>::bytes, COLS = NT < 32 ? 32 : NT;   // columns of a set of sums
   constexpr unsigned IDESC = 2u << 4 | 1u << 7 | 1u << 10 | (unsigned)(NT >> 3) << 17 | (unsigned)(MM_ROWS >> 4) << 24;
   extern __shared__ unsigned char dyn[];
@@ -356,6 +359,108 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_pair_kernel(const __g
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
+// ---- up to four tokens: no tensor cores ----
+// Rows of the matrix straight into registers, 512 columns a warp and load, eight loads under way; four products an instruction (dp4a), a warp's sum in one (redux).  A block per SM has an even share of the
+// rows; `cw` warps share a row's columns, with the tokens' values for them in registers, and add up in shared memory: whole numbers, so that the order does not matter.
+constexpr int MV_THREADS = 512, MV_ROWS = 1024;   // rows between two stores
+struct MvParams {
+  const int8_t *w, *x;
+  int64_t w_o, x_t;
+  const float *sx, *so;
+  uint16_t* out;
+  int64_t out_t;
+  int O, I, cw;
+};
+template <int T, int CH, int U>   // CH: loads of a row by a warp; U: rows at a time, and as many under way
+__global__ void __launch_bounds__(MV_THREADS, 1) matvec_i8_kernel(const __grid_constant__ MvParams p) {
+  __shared__ int s_sum[MV_ROWS * T];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int r0 = (int)((int64_t)p.O * blockIdx.x / gridDim.x), r1 = (int)((int64_t)p.O * (blockIdx.x + 1) / gridDim.x);
+  const int groups = MV_THREADS / 32 / p.cw, group = warp / p.cw, col = (warp % p.cw) * 512 + lane * 16;
+  if (lane == 0 && group < groups) {   // the first rows on their way to L2 while the kernel before ends
+    for (int u = 0; u < U; u++)
+      if (r0 + group * U + u < r1 && (warp % p.cw) * 512 < p.I)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.w + (int64_t)(r0 + group * U + u) * p.w_o + (warp % p.cw) * 512), "r"(min(512, p.I - (warp % p.cw) * 512)) : "memory");
+  }
+  pdl_wait();
+  pdl_trigger();
+  for (int i = tid; i < MV_ROWS * T; i += MV_THREADS) s_sum[i] = 0;
+  int4 x[T][CH];
+#pragma unroll
+  for (int t = 0; t < T; t++)
+#pragma unroll
+    for (int c = 0; c < CH; c++)
+      x[t][c] = col + c * p.cw * 512 < p.I ? *reinterpret_cast<const int4*>(p.x + t * p.x_t + col + c * p.cw * 512) : make_int4(0, 0, 0, 0);
+  for (int base = r0; base < r1; base += MV_ROWS) {
+    const int n = min(MV_ROWS, r1 - base);
+    __syncthreads();
+    if (group < groups) {
+      int4 w[2][U][CH];
+      auto load = [&](int4 (&to)[U][CH], int r) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int c = 0; c < CH; c++)
+            to[u][c] = r + u < n && col + c * p.cw * 512 < p.I ? *reinterpret_cast<const int4*>(p.w + (int64_t)(base + r + u) * p.w_o + col + c * p.cw * 512) : make_int4(0, 0, 0, 0);
+      };
+      auto multiply = [&](const int4 (&w)[U][CH], int r) {
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+          int mine = 0;
+#pragma unroll
+          for (int u = 0; u < U; u++) {
+            int a = 0;
+#pragma unroll
+            for (int c = 0; c < CH; c++)
+              a = __dp4a(w[u][c].x, x[t][c].x, a), a = __dp4a(w[u][c].y, x[t][c].y, a), a = __dp4a(w[u][c].z, x[t][c].z, a), a = __dp4a(w[u][c].w, x[t][c].w, a);
+            a = __reduce_add_sync(0xffffffffu, a);
+            if (lane == u) mine = a;
+          }
+          if (lane < U && r + lane < n) atomicAdd(&s_sum[t * MV_ROWS + r + lane], mine);
+        }
+      };
+      int r = group * U;
+      load(w[0], r);
+      for (; r < n; r += 2 * groups * U) {   // the next rows are under way
+        load(w[1], r + groups * U);
+        multiply(w[0], r);
+        if (r + groups * U >= n) break;
+        load(w[0], r + 2 * groups * U);
+        multiply(w[1], r + groups * U);
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += MV_THREADS) {
+      const float so = p.so[base + i];
+#pragma unroll
+      for (int t = 0; t < T; t++) {
+        p.out[t * p.out_t + base + i] = f2bf((float)s_sum[t * MV_ROWS + i] * p.sx[t] * so);
+        s_sum[t * MV_ROWS + i] = 0;
+      }
+    }
+  }
+}
+
+template <int T, int CH, int U>
+int launch_vec_as(const MvParams& p, int blocks, cudaStream_t st) {
+  StageTimer timer(ST_GEMV, st);
+  launch_chain(matvec_i8_kernel<T, CH, U>, dim3((unsigned)blocks), dim3(MV_THREADS), 0, st, p);
+  return check_launch("matmul_i8");
+}
+// Rows at a time: four of 512 columns where a warp has few (B200, us, one token, four | eight at a time: 1024 x 1024 1.9 | 2.7, 6144 x 4096 4.3 | 5.3), eight where it has many (12288 x 4096 11.2 | 10.3,
+// 24576 x 4096 18.9 | 17.5, 151936 x 4096 95 | 91).
+template <int T>
+int launch_vec(MvParams p, cudaStream_t st) {
+  const int loads = (p.I + 511) / 512;
+  p.cw = loads < 8 ? loads : 8;
+  const int per = (loads + p.cw - 1) / p.cw, groups = MV_THREADS / 32 / p.cw, sms = sm_count(), most = (p.O + groups - 1) / groups, blocks = most < sms ? most : sms;
+  const bool many = p.O / (blocks * groups) >= 32;
+  if (per == 1) return many ? launch_vec_as<T, 1, 8>(p, blocks, st) : launch_vec_as<T, 1, 4>(p, blocks, st);
+  if (per == 2) return many ? launch_vec_as<T, 2, 4>(p, blocks, st) : launch_vec_as<T, 2, 2>(p, blocks, st);
+  return per == 3 ? launch_vec_as<T, 3, 2>(p, blocks, st) : launch_vec_as<T, 4, 2>(p, blocks, st);
+}
+constexpr int MV_MOST = 4 * 8 * 512;   // columns
+
 // Rows of 8-bit numbers in boxes of 128 columns; what is behind the last row or column comes as zeros.
 bool bytes_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t stride, int box) {
   const auto encode = tensor_map_encoder();
@@ -364,6 +469,15 @@ bool bytes_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int
   const cuuint32_t boxes[2] = {MM_K, (cuuint32_t)box}, steps[2] = {1, 1};
   return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Blocks that share a tile's columns: as many as there are SMs for, each with so many steps that the sums' way through shared memory is worth it.  B200, us, 4096 columns, by 1 | 2 | 3 | 4 | 6 | 8 blocks:
+// 16 tokens, 1024 rows 9.6 | 7.6 | 6.3 | 5.5 | 5.6 | 5.2, 6144 rows 10.4 | 8.3 | 7.6 | 7.6 | 12.0 | 11.6, 24576 rows 18.9 | 26 | 30 | 28 | 39 | 42;  128 tokens, 6144 rows 13.4 | 15.5 | 14.2 | 12.8 | 21 | 20.
+int mm_split(int64_t tiles, int chunks, int nt) {
+  const int least = nt / 8;
+  int s = 1;
+  while (s < 8 && tiles * (s + 1) <= sm_count() && chunks >= (s + 1) * least) s++;
+  return s;
 }
 
 template <int NT>
@@ -380,10 +494,9 @@ int launch(const pk_tensor* x, const pk_tensor* w, MmParams p, cudaStream_t st) 
   }
   p.t_tiles = (p.T + NT - 1) / NT;
   p.tiles = p.t_tiles * ((p.O + MM_ROWS - 1) / MM_ROWS);
-  const int sms = sm_count();
-  p.split = 1;
-  while (p.split < 8 && p.tiles * p.split * 2 <= sms && p.split * 2 <= p.chunks) p.split *= 2;
-  const int clusters = p.split > 1 ? p.tiles : p.tiles < sms ? p.tiles : sms;
+  const int slots = MmRing<NT>::ctas * sm_count();
+  p.split = mm_split(p.tiles, p.chunks, NT);
+  const int clusters = p.split > 1 ? p.tiles : p.tiles < slots ? p.tiles : slots;
   StageTimer timer(ST_GEMV, st);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(clusters * p.split)), cfg.blockDim = dim3(MM_THREADS), cfg.dynamicSmemBytes = mm_smem<NT>(), cfg.stream = st;
@@ -450,10 +563,16 @@ extern "C" int pk_matmul_i8(const pk_tensor* x, const pk_tensor* x_scales, const
   p.sx = (const float*)x_scales->data, p.so = (const float*)weight_scales->data, p.out = (uint16_t*)out->data, p.out_t = out->stride[0];
   p.T = (int)T, p.O = (int)O, p.chunks = (int)((I + MM_K - 1) / MM_K);
   const cudaStream_t st = (cudaStream_t)stream;
+  // Which kernel, B200, us, without | with tensor cores: 6144 x 4096, one token 4.3 | 8.2, four 7.0 | 8.2; 24576 x 4096, two tokens 18.5 | 19.6, four 20.8 | 19.6.
+  if (I <= MV_MOST && (T <= 2 || (T <= 4 && O * I <= 48 << 20))) {
+    const MvParams v = {(const int8_t*)weight->data, (const int8_t*)x->data, O > 1 ? weight->stride[0] : I, T > 1 ? x->stride[0] : I, p.sx, p.so, p.out, p.out_t, (int)O, (int)I, 0};
+    return T == 1 ? launch_vec<1>(v, st) : T == 2 ? launch_vec<2>(v, st) : T == 3 ? launch_vec<3>(v, st) : launch_vec<4>(v, st);
+  }
   if (T <= 16) return launch<16>(x, weight, p, st);
   if (T <= 32) return launch<32>(x, weight, p, st);
   if (T <= 64) return launch<64>(x, weight, p, st);
+  // Tiles of 128 rows and 64 tokens, two blocks an SM, or of 256 x 256 on pairs: 256 x 6144 x 4096 13.7 | 16.2, 512 x 4096 x 12288 32 | 34, 512 x 6144 x 4096 (384 tiles) 21.8 | 17.6, 2048 x 4096 x 12288 109 | 65.
+  if ((T + 63) / 64 * ((O + 127) / 128) <= 2 * sm_count()) return launch<64>(x, weight, p, st);
   if (T <= 128) return launch<128>(x, weight, p, st);
-  if ((T + 255) / 256 * ((O + 255) / 256) >= sm_count() / 2) return launch_pair(x, weight, p, st);
-  return launch<256>(x, weight, p, st);
+  return launch_pair(x, weight, p, st);
 }
