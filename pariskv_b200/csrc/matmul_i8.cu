@@ -9,7 +9,7 @@
 namespace pk {
 namespace {
 
-constexpr int MM_THREADS = 192;        // a warp for the copies, one for the products, four that scale and store
+constexpr int MM_THREADS = 320;        // a warp for the copies, one for the products, eight that scale and store: two for every quarter of the rows, each with half of the tokens
 constexpr int MM_ROWS = 128, MM_K = 128;
 constexpr int MM_WAIT_LIMIT = 100000;  // tries; one waits up to 10 us by itself
 
@@ -36,24 +36,34 @@ __device__ __forceinline__ void tc_mma_i8(unsigned d, uint64_t a, uint64_t b, un
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
 }
 __device__ __forceinline__ void tmem_ld16(uint32_t (&r)[16], unsigned addr) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
                  "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                : "r"(addr)
                : "memory");
 }
-// A lane's row of sums - matrix row o, `n` tokens from t0 on - out of tensor memory, scaled and stored; sx: the tokens' scales.  All of a step's reads come before its stores, which the compiler
-// must not reorder.
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {   // the values are there behind it, and no use of them moves before it
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                 "+r"(r[14]), "+r"(r[15])::"memory");
+}
+// A lane's row of sums - matrix row o, the tile's tokens c0 .. c1, t0 the first of the tile - out of tensor memory, scaled and stored; sx: the tokens' scales.  The next sixteen are under way while sixteen
+// are stored; all of a step's reads come before its stores, which the compiler must not reorder.
 template <class Free>
-__device__ __forceinline__ void mm_store(const MmParams& p, unsigned addr, int n, int t0, int o, const float* sx, bool dead, Free all_read) {
+__device__ __forceinline__ void mm_store(const MmParams& p, unsigned addr, int c0, int c1, int t0, int o, const float* sx, bool dead, Free all_read) {
   const float so = o < p.O ? p.so[o] : 0.0f;
-  uint16_t* to = p.out + t0 * p.out_t + o;
-  const bool inside = t0 + n <= p.T;
+  uint16_t* to = p.out + (t0 + c0) * p.out_t + o;
+  const bool inside = t0 + c1 <= p.T;
+  uint32_t next[16];
+  if (c0 < c1) tmem_ld16(next, addr + c0);
 #pragma unroll 1
-  for (int c = 0; c < n; c += 16) {
+  for (int c = c0; c < c1; c += 16) {
     uint32_t acc[16];
-    tmem_ld16(acc, addr + c);
-    if (c + 16 == n) all_read();
+    tmem_wait16(next);
+#pragma unroll
+    for (int i = 0; i < 16; i++) acc[i] = next[i];
+    if (c + 16 < c1) tmem_ld16(next, addr + c + 16);
+    else all_read();
     uint16_t y[16];
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
@@ -71,6 +81,7 @@ __device__ __forceinline__ void mm_store(const MmParams& p, unsigned addr, int n
         if (inside || t0 + c + i < p.T) *to = y[i];
     }
   }
+  if (c0 >= c1) all_read();
 }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint4 remote16(unsigned at, unsigned rank) {   // the same place in the shared memory of block `rank` of the cluster
@@ -98,7 +109,7 @@ __global__ void __launch_bounds__(MM_THREADS, MmRing<NT>::ctas) matmul_i8_kernel
   const unsigned full = smem_addr(bars), empty = full + 8 * NS, done = empty + 8 * NS, taken = done + 16, ending = taken + 16;
   if (tid == 0) {
     for (int i = 0; i < NS; i++) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
-    for (int i = 0; i < 2; i++) mbar_init(done + 8 * i, 1), mbar_init(taken + 8 * i, 128);
+    for (int i = 0; i < 2; i++) mbar_init(done + 8 * i, 1), mbar_init(taken + 8 * i, 256);
     mbar_init(ending, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_dead = 0;
@@ -166,29 +177,30 @@ __global__ void __launch_bounds__(MM_THREADS, MmRing<NT>::ctas) matmul_i8_kernel
       for (int it = 0; it < MM_WAIT_LIMIT && !mbar_try(ending, 0); it++) {}
     }
   } else {
-    const int quarter = warp & 3, o_lane = 32 * quarter + lane;
+    const int quarter = warp & 3, o_lane = 32 * quarter + lane, part = (warp - 2) >> 2, c0 = NT >= 32 ? part * (NT / 2) : part * NT, c1 = NT >= 32 ? c0 + NT / 2 : NT;
     const unsigned lanes = tmem + ((unsigned)quarter << 21);
     int n = 0;
     for (int tile = cluster; tile < p.tiles; tile += clusters, n++) {
       const int set = n & 1, t0 = tile % p.t_tiles * NT, o = tile / p.t_tiles * MM_ROWS + o_lane;
       if (p.split == 1) {   // (the threads before the ones of this tile have passed the barrier of the tile before: two places do)
-        for (int i = tid - 64; i < NT; i += 128) s_sx[set][i] = t0 + i < p.T ? p.sx[t0 + i] : 0.0f;
-        named_barrier(1, 128);
+        for (int i = tid - 64; i < NT; i += 256) s_sx[set][i] = t0 + i < p.T ? p.sx[t0 + i] : 0.0f;
+        named_barrier(1, 256);
       }
       wait(done + 8 * set, (unsigned)(n / 2) & 1);
       __syncwarp();
       tc_after();
       if (p.split == 1) {
-        mm_store(p, lanes + COLS * set, NT, t0, o, s_sx[set], dead, [&] {
+        mm_store(p, lanes + COLS * set, c0, c1, t0, o, s_sx[set], dead, [&] {
           tc_before();
           mbar_arrive1(taken + 8 * set);
         });
       } else {
         // this block's partial sums, column by column, where the copies were (they have all been multiplied)
 #pragma unroll 1
-        for (int c = 0; c < NT; c += 16) {
+        for (int c = c0; c < c1; c += 16) {
           uint32_t acc[16];
           tmem_ld16(acc, lanes + COLS * set + c);
+          tmem_wait16(acc);
 #pragma unroll
           for (int i = 0; i < 16; i++) asm volatile("st.shared.b32 [%0], %1;" ::"r"(ring + ((c + i) * MM_ROWS + o_lane) * 4), "r"(acc[i]) : "memory");
         }
@@ -262,7 +274,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_pair_kernel(const __g
   const int rank = (int)(blockIdx.x & 1), pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
   if (tid == 0) {
     for (int i = 0; i < NS; i++) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
-    for (int i = 0; i < 2; i++) mbar_init(done + 8 * i, 1), mbar_init(taken + 8 * i, 8);
+    for (int i = 0; i < 2; i++) mbar_init(done + 8 * i, 1), mbar_init(taken + 8 * i, 16);
     mbar_init(ending, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_dead = 0;
@@ -335,17 +347,17 @@ __global__ void __launch_bounds__(MM_THREADS, 1) matmul_i8_pair_kernel(const __g
       }
     }
   } else {
-    const int quarter = warp & 3;
+    const int quarter = warp & 3, c0 = (warp - 2) / 4 * (NT / 2);
     const unsigned lanes = tmem + ((unsigned)quarter << 21), taken0 = in_block0(taken);
     int n = 0;
     for (int tile = pair; tile < p.tiles; tile += pairs, n++) {
       const int set = n & 1, t0 = tile % p.t_tiles * NT, o = tile / p.t_tiles * 256 + 128 * rank + 32 * quarter + lane;
-      for (int i = tid - 64; i < NT; i += 128) s_sx[set][i] = t0 + i < p.T ? p.sx[t0 + i] : 0.0f;
-      named_barrier(1, 128);
+      for (int i = tid - 64; i < NT; i += 256) s_sx[set][i] = t0 + i < p.T ? p.sx[t0 + i] : 0.0f;
+      named_barrier(1, 256);
       wait(done + 8 * set, (unsigned)(n / 2) & 1);
       __syncwarp();
       tc_after();
-      mm_store(p, lanes + NT * set, NT, t0, o, s_sx[set], dead, [&] {
+      mm_store(p, lanes + NT * set, c0, c0 + NT / 2, t0, o, s_sx[set], dead, [&] {
         tc_before();
         __syncwarp();
         if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(taken0 + 8 * set) : "memory");
