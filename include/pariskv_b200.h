@@ -616,7 +616,7 @@ typedef struct pk_cache8 {
 } pk_cache8;
 int pk_cache8_append(const pk_cache8* cache, const pk_tensor* keys, const pk_tensor* values, const pk_tensor* lengths, const pk_tensor* counts, void* stream);
 int pk_cache8_read(const pk_cache8* cache, const pk_tensor* lengths, const pk_tensor* rows, const pk_tensor* out, void* stream);
-int64_t pk_cache8_attention_workspace_bytes(int64_t bs, int64_t T, int64_t Hq, int64_t H, int64_t cap);
+int64_t pk_cache8_attention_workspace_bytes(int64_t bs, int64_t T, int64_t Hq, int64_t H, int64_t cap);   /* 0: none */
 int pk_cache8_attention(const pk_tensor* queries, const pk_cache8* cache, const pk_tensor* lengths, float scale, const pk_tensor* out, const pk_tensor* lse, void* workspace,
                         int64_t workspace_bytes, void* stream);
 int pk_add_rmsnorm_i8(const pk_tensor* a, const pk_tensor* residual, const pk_tensor* weight, const pk_tensor* h_out, const pk_tensor* codes, const pk_tensor* scales, double eps, void* stream);

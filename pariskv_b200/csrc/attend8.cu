@@ -34,7 +34,7 @@ struct Attend8 {
   const uint16_t* q;
   int64_t q_b, q_t, q_h;
   const int32_t* lengths;
-  int bs, T, G, row_groups;
+  int bs, T, G, row_groups, cluster;   // cluster: blocks that share an item, 0 where the ranges do not follow the items
   float scale_log2;
   uint16_t* out;
   float *lse, *records;   // records: [2 * blocks][ROWS * 130]
@@ -139,33 +139,47 @@ __device__ __forceinline__ float move(RowState& s, float m, float top) {
   }
   return f;
 }
+// The same place in the shared memory of block `rank` of the cluster.
+__device__ __forceinline__ float remote(const void* at, int rank) {
+  float r;
+  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(r) : "r"(smem_addr(at)), "r"(rank) : "memory");
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 template <bool E4M3, int ROWS, bool DENSE>
 __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(const __grid_constant__ Attend8 p) {
   constexpr bool ACROSS = A8<ROWS>::across;
   constexpr int MT = ROWS == 32 ? 2 : 1, NR = 2 * MT;   // operands of 16 query rows; query rows that a lane's scores belong to: 8 e + g, across 2 t4 + e
   constexpr int NV = ACROSS ? 4 : 8;                    // its scores of each in a step
-  __shared__ float s_m[4][ROWS], s_l[4][ROWS], s_factor[ROWS];
+  __shared__ float s_m[4][ROWS], s_l[4][ROWS], s_factor[ROWS], s_M[ROWS], s_L[ROWS];   // of the warps; of the block, for its cluster
   __shared__ TilePlan s_plan;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   pdl_wait();
   pdl_trigger();
   const int blocks = (int)gridDim.x;
   const int64_t items = (int64_t)p.c.H * p.row_groups;
-  if (warp == 0) {
-    const TilePlan w = tile_plan(p.bs, blockIdx.x, (unsigned)blocks, [&](int b) -> int64_t { return b < p.bs ? items * tiles8(p, len8(p, b)) : 0; });
-    if (lane == 0) s_plan = w;
-  }
-  __syncthreads();
-  const TilePlan plan = s_plan;
-  const unsigned shares = (unsigned)min((int64_t)blocks, plan.total);
-  if (blockIdx.x >= shares) return;
   Way8 way;
-  {
+  if (p.cluster) {
+    const int item = (int)blockIdx.x / p.cluster, rank = (int)blockIdx.x % p.cluster;
+    way.b = item / (int)items, way.h = item % (int)items / p.row_groups, way.group = item % p.row_groups;
+    way.sample(p);
+    way.tile = way.n * rank / p.cluster, way.left = way.n * (rank + 1) / p.cluster - way.tile;
+    if (tid < ROWS) s_M[tid] = -INFINITY, s_L[tid] = 0.0f;
+  } else {
+    if (warp == 0) {
+      const TilePlan w = tile_plan(p.bs, blockIdx.x, (unsigned)blocks, [&](int b) -> int64_t { return b < p.bs ? items * tiles8(p, len8(p, b)) : 0; });
+      if (lane == 0) s_plan = w;
+    }
+    __syncthreads();
+    const TilePlan plan = s_plan;
+    const unsigned shares = (unsigned)min((int64_t)blocks, plan.total);
+    if (blockIdx.x >= shares) return;
     const int64_t first = share_begin(plan.total, blockIdx.x, shares);
     way.left = share_begin(plan.total, blockIdx.x + 1, shares) - first;
     way.b = plan.sample;
     way.sample(p);
-    const unsigned at = (unsigned)(first - plan.before);   // tiles of a sample are below 2^32: the launch sees to it
+    const unsigned at = (unsigned)(first - plan.before);   // tiles of a sample are below 2^31: the launch sees to it
     const unsigned item = at / (unsigned)way.n;
     way.tile = (int)(at % (unsigned)way.n), way.h = (int)(item / (unsigned)p.row_groups), way.group = (int)(item % (unsigned)p.row_groups);
   }
@@ -174,7 +188,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
   for (; way.left > 0; way.next(p)) {
     // ---- a segment ----
     const int b = way.b, h = way.h, group = way.group, whole = way.whole, count = way.count();
-    const bool whole_item = count == way.n;
+    const bool whole_item = count == way.n && p.cluster <= 1;
     const int coded = (whole + A8_TILE - 1) / A8_TILE;                          // tiles of codes of the item
     const int n_coded = max(0, min(coded, way.tile + count) - way.tile);        // of the segment
     const bool recent = way.len > whole && way.tile + count == way.n;
@@ -634,6 +648,10 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
           for (int i = 0; i < 4; i++) w[i] = pack2(L == 0.0f ? 0.0f : O[2 * i] / L, L == 0.0f ? 0.0f : O[2 * i + 1] / L);
           *reinterpret_cast<uint4*>(p.out + out_row * 128 + c) = make_uint4(w[0], w[1], w[2], w[3]);
           if (p.lse && c == 0) p.lse[out_row] = L == 0.0f ? -INFINITY : M + log2f(L);
+        } else if (p.cluster) {
+          float4* rec = reinterpret_cast<float4*>(dyn8 + A8<ROWS>::q_bytes + e * 2 * A8_SLOT + A8_SLOT) + (tid >> 4) * 32 + (c >> 2);   // the second stage of warp e
+          rec[0] = make_float4(O[0], O[1], O[2], O[3]), rec[1] = make_float4(O[4], O[5], O[6], O[7]);
+          if (c == 0) s_M[row] = M, s_L[row] = L;
         } else {
           float4* rec = reinterpret_cast<float4*>(p.records + (2 * (int64_t)blockIdx.x + (way.tile == 0)) * (ROWS * 130) + row * 128 + c);
           rec[0] = make_float4(O[0], O[1], O[2], O[3]), rec[1] = make_float4(O[4], O[5], O[6], O[7]);
@@ -645,6 +663,33 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
       }
       __syncthreads();
     }
+  }
+  if (p.cluster > 1) {   // the blocks of an item: each joins the rows that are its turn
+    cluster_sync();
+    const int item = (int)blockIdx.x / p.cluster, item_b = item / (int)items, item_h = item % (int)items / p.row_groups, item_group = item % p.row_groups;
+    const int n_rows = min(ROWS, n_rows_all - item_group * ROWS);
+    for (int row = (int)blockIdx.x % p.cluster; row < n_rows; row += p.cluster) {
+      const float* o = reinterpret_cast<const float*>(dyn8 + A8<ROWS>::q_bytes + (row >> 3) * 2 * A8_SLOT + A8_SLOT) + (row & 7) * 128 + tid;
+      float m[8], l[8], x[8], M = -INFINITY, L = 0.0f, O = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int r = min(i, p.cluster - 1);
+        m[i] = remote(&s_M[row], r), l[i] = remote(&s_L[row], r), x[i] = remote(o, r);
+        M = fmaxf(M, m[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (i < p.cluster) {
+          const float f = m[i] == -INFINITY ? 0.0f : ex2(m[i] - M);
+          L += l[i] * f;
+          if (f != 0.0f) O += x[i] * f;   // (a block without rows of this item has not written any; NaN != 0)
+        }
+      const int rr = item_group * ROWS + row, t = rr / p.G, hq = item_h * p.G + rr % p.G;
+      const int64_t out_row = ((int64_t)item_b * p.T + t) * Hq + hq;
+      p.out[out_row * 128 + tid] = f2bf(L == 0.0f ? 0.0f : O / L);
+      if (p.lse && tid == 0) p.lse[out_row] = L == 0.0f ? -INFINITY : M + log2f(L);
+    }
+    cluster_sync();   // no block ends while others read from it
   }
 }
 
@@ -680,6 +725,15 @@ int64_t a8_waves(int64_t most, int64_t slots) {
   return n < 1 ? 1 : n > 4 ? 4 : n;
 }
 
+// Blocks of a cluster that share an item, so that one launch does and needs no scratch: where that leaves each at most three tiles.  0: ranges and a second launch.  B200, us, 701 keys of 8 KV heads of
+// four queries 6.4, by two launches 8.5.
+int a8_cluster(int64_t items, int64_t tiles, int64_t slots) {
+  int64_t n = slots / items;
+  n = n > 8 ? 8 : n < 1 ? 1 : n;
+  n = n < tiles ? n : tiles;
+  return (tiles + n - 1) / n <= 3 ? (int)n : 0;
+}
+
 template <bool E4M3, int ROWS, bool DENSE>
 int launch_as(Attend8 p, cudaStream_t st) {
   p.row_groups = (p.T * p.G + ROWS - 1) / ROWS;
@@ -692,6 +746,18 @@ int launch_as(Attend8 p, cudaStream_t st) {
     mark_on_device(opted, bit);
   }
   StageTimer timer(ST_ATTENTION, st);
+  const int64_t items = (int64_t)p.bs * p.c.H * p.row_groups;
+  p.cluster = a8_cluster(items, most / items, slots);
+  if (p.cluster) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(items * p.cluster)), cfg.blockDim = dim3(A8_THREADS), cfg.dynamicSmemBytes = A8<ROWS>::smem, cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension, attr[0].val.clusterDim.x = (unsigned)p.cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, attend8_kernel<E4M3, ROWS, DENSE>, p);
+    return check_launch("cache8_attention");
+  }
   launch_chain(attend8_kernel<E4M3, ROWS, DENSE>, dim3((unsigned)blocks), dim3(A8_THREADS), A8<ROWS>::smem, st, p);
   launch_chain(attend8_merge_kernel<ROWS>, dim3((unsigned)((int64_t)p.bs * p.T * p.c.H * p.G)), dim3(128), 0, st, p, blocks);
   return check_launch("cache8_attention", 2);
@@ -711,6 +777,8 @@ extern "C" int64_t pk_cache8_attention_workspace_bytes(int64_t bs, int64_t T, in
   if (bs < 1 || T < 1 || T > 256 || H < 1 || Hq < H || cap < 0) return 0;
   const int rows = T * (Hq / H) <= 8 ? 8 : T * (Hq / H) <= 16 ? 16 : 32;
   const int64_t slots = (int64_t)(rows == 32 ? A8<32>::ctas : A8<8>::ctas) * sm_count(), most = bs * H * ((T * (Hq / H) + rows - 1) / rows) * ((cap + A8_TILE - 1) / A8_TILE + 1);
+  const int64_t items = bs * H * ((T * (Hq / H) + rows - 1) / rows);
+  if (a8_cluster(items, most / items, slots)) return 0;
   return 2 * (most < slots ? most : slots * a8_waves(most, slots)) * rows * 130 * 4;
 }
 
@@ -738,8 +806,9 @@ extern "C" int pk_cache8_attention(const pk_tensor* queries, const pk_cache8* ca
   p.scale_log2 = scale * 1.4426950408889634f;
   PK_REQUIRE(scale > 0.0f && p.scale_log2 <= 3.4e38f, "scale must be positive, and finite as a factor of log2 e");
   if (bs == 0 || T == 0) return PK_OK;
-  PK_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "workspace must be 256-byte aligned device memory");
-  if (workspace_bytes < pk_cache8_attention_workspace_bytes(bs, T, Hq, H, p.c.cap)) return fail(PK_ERR_WORKSPACE, "cache8_attention: workspace too small");
+  const int64_t bytes = pk_cache8_attention_workspace_bytes(bs, T, Hq, H, p.c.cap);
+  PK_REQUIRE(bytes == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0), "workspace must be 256-byte aligned device memory");
+  if (workspace_bytes < bytes) return fail(PK_ERR_WORKSPACE, "cache8_attention: workspace too small");
   p.q = (const uint16_t*)queries->data, p.q_b = queries->stride[0], p.q_t = queries->stride[1], p.q_h = queries->stride[2];
   p.lengths = (const int32_t*)lengths->data, p.bs = (int)bs, p.T = (int)T, p.G = (int)(Hq / H);
   p.out = (uint16_t*)out->data, p.records = (float*)workspace;

@@ -814,9 +814,11 @@ PyObject* py_cache8_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!output(a[7], &out, &own, *q.t, q.t->sizes(), at::kBFloat16) || !same_device({&c.codes, &len, &out, &lse}, *q.t)) return nullptr;
   if (q.t->numel() == 0) return give(a[7], out);
   const int64_t bytes = pk_cache8_attention_workspace_bytes(q.d.shape[0], q.d.shape[1], q.d.shape[2], c.codes.d.shape[1], c.codes.d.shape[2]);
-  const at::Tensor ws = empty_on(*q.t, {bytes}, at::kByte);
+  at::Tensor ws;
+  if (bytes > 0) ws = empty_on(*q.t, {bytes}, at::kByte);
+  void* scratch = bytes > 0 ? ws.data_ptr() : nullptr;
   void* st = stream_of(*q.t);
-  const int rc = without_gil([&] { return pk_cache8_attention(q.p(), &c.c, len.p(), (float)scale, out.p(), lse.p(), ws.data_ptr(), bytes, st); });
+  const int rc = without_gil([&] { return pk_cache8_attention(q.p(), &c.c, len.p(), (float)scale, out.p(), lse.p(), scratch, bytes, st); });
   if (rc) return raise(rc);
   return give(a[7], out);
   PK_PY_END

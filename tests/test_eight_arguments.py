@@ -37,6 +37,7 @@ CACHE = dict(codes=z(2, 2, 40, 2, 128, dtype=I8), scales=z(2, 2, 3, 2, dtype=F32
 APPEND = dict(cache=CACHE, keys=z(2, 3, 2, 128), values=z(2, 3, 2, 128), lengths=z(2, dtype=I32), counts=None, stream=None)
 READ = dict(cache=CACHE, lengths=z(2, dtype=I32), rows=None, out=z(2, 2, 40, 2, 128), stream=None)
 ATTEND = dict(queries=z(2, 1, 4, 128), cache=CACHE, lengths=z(2, dtype=I32), scale=0.1, out=z(2, 1, 4, 128), lse=None, ws=None, ws_bytes=0, stream=None)
+LONG = {**CACHE, "codes": z(1, 1, 1, 2, 128, dtype=I8).expand(2, 2, 20000, 2, 128), "scales": z(1, 1, 1, 2, dtype=F32).expand(2, 2, 1250, 2)}   # a short cache needs no scratch
 NORM = dict(a=z(3, 64), residual=z(3, 64), weight=z(64), h=z(3, 64), codes=z(3, 64, dtype=I8), scales=z(3, dtype=F32), eps=1e-6, stream=None)
 ROWS = dict(x=z(3, 64), gated=0, codes=z(3, 64, dtype=I8), scales=z(3, dtype=F32), stream=None)
 MM = dict(x=z(3, 64, dtype=I8), sx=z(3, dtype=F32), w=z(5, 64, dtype=I8), so=z(5, dtype=F32), out=z(3, 5), stream=None)
@@ -82,8 +83,8 @@ def test_read(change, match):
     (dict(queries=z(2, 1, 3, 128), out=z(2, 1, 3, 128)), "multiple of the KV heads", 1), (dict(queries=z(2, 1, 4, 64)), "queries must be", 1), (dict(queries=odd(ATTEND["queries"])), "queries must be", 1),
     (dict(queries=z(1, 1, 4, 128), out=z(1, 1, 4, 128)), "codes must be", 1), (dict(out=z(2, 1, 4, 256)[..., ::2]), "out must be", 1), (dict(out=z(2, 1, 2, 128)), "shape of queries", 1),
     (dict(lse=z(2, 1, 2, dtype=F32)), "lse must be", 1), (dict(scale=0.0), "scale must be", 1), (dict(scale=float("nan")), "scale must be", 1), (dict(scale=float("inf")), "scale must be", 1),
-    (dict(queries=z(2, 257, 4, 128), out=z(2, 257, 4, 128)), "at most 256", 1), (dict(queries=z(2, 1, 260, 128), out=z(2, 1, 260, 128)), "at most 128", 1), (dict(ws=None), "workspace must be", 1),
-    (dict(ws=4096, ws_bytes=8), "too small", 4), (dict(lengths=z(4, dtype=I32)[::2]), "lengths must be", 1)])
+    (dict(queries=z(2, 257, 4, 128), out=z(2, 257, 4, 128)), "at most 256", 1), (dict(queries=z(2, 1, 260, 128), out=z(2, 1, 260, 128)), "at most 128", 1), (dict(cache=LONG), "workspace must be", 1), (dict(cache=LONG, ws=4100, ws_bytes=1 << 30), "workspace must be", 1),
+    (dict(cache=LONG, ws=4096, ws_bytes=8), "too small", 4), (dict(lengths=z(4, dtype=I32)[::2]), "lengths must be", 1)])
 def test_attention(change, match, code):
     refused("pk_cache8_attention", list({**ATTEND, **change}.values()), match, code)
 
@@ -127,3 +128,4 @@ def test_workspace_sizes():
     lib = L.load()
     assert 0 < lib.pk_cache8_attention_workspace_bytes(8, 4, 32, 8, 131072) < 1 << 30
     assert lib.pk_cache8_attention_workspace_bytes(8, 300, 32, 8, 131072) == 0
+    assert lib.pk_cache8_attention_workspace_bytes(1, 1, 32, 8, 256) == 0
