@@ -78,14 +78,28 @@ __global__ void __launch_bounds__(THREADS) rows_i8_kernel(const __grid_constant_
         }
       }
     }
+    auto row_sum = [&](double v) {
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-    if (lane == 0) s_sum[warp] = ss;
-    __syncthreads();
-    ss = 0.0;
+      for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+      if (lane == 0) s_sum[warp] = v;
+      __syncthreads();
+      v = 0.0;
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; i++) ss += s_sum[i];
-    const float rstd = (float)inverse_root(fma(ss < 1e-70 ? 0.0 : ss, p.one_n, p.eps));
+      for (int i = 0; i < THREADS / 32; i++) v += s_sum[i];
+      return v;
+    };
+    ss = row_sum(ss);
+    if (ss < 1e-60 && p.eps < 1e-50) {   // a row of next to nothing, without an eps to speak of: by conversions after all
+      ss = 0.0;
+#pragma unroll 1
+      for (int i = tid; i < p.n; i += THREADS) {
+        const double d = bf2f(p.h[row * p.h_s + i]);
+        ss = fma(d, d, ss);
+      }
+      __syncthreads();
+      ss = row_sum(ss);
+    }
+    const float rstd = (float)inverse_root(fma(ss, p.one_n, p.eps));
 #pragma unroll
     for (int k = 0; k < N; k++) {
       const int i = (k * THREADS + tid) * 8;
