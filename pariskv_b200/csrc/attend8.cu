@@ -46,6 +46,19 @@ __device__ __forceinline__ int tiles8(const Attend8& p, int len) {   // of an it
   return max(1, (whole + A8_TILE - 1) / A8_TILE + (whole < len));
 }
 
+// Where every item has eight blocks' tiles or more, the ranges end where the items do: the blocks whose range would begin in an item share it evenly.  A range over the end of an item costs its block
+// another set of queries and another sum over its warps, 4 us that the whole launch waits for.  first8: the first of an item's blocks, `at` its first tile.
+__device__ __forceinline__ bool apart8(int64_t total, int fewest, unsigned shares) { return (int64_t)fewest * shares >= 8 * total; }
+__device__ __forceinline__ unsigned first8(int64_t at, int64_t total, unsigned shares) {
+  return total < 1 << 22 ? ((unsigned)at * shares + (unsigned)total - 1) / (unsigned)total : (unsigned)((at * shares + total - 1) / total);
+}
+// The fewest tiles of an item, by a warp.
+__device__ __forceinline__ int fewest8(const Attend8& p) {
+  int n = 0x7fffffff;
+  for (int b = threadIdx.x & 31; b < p.bs; b += 32) n = min(n, tiles8(p, len8(p, b)));
+  return __reduce_min_sync(0xffffffffu, n);
+}
+
 // A block's way through its range: segments of consecutive tiles of one item.
 struct Way8 {
   int b, h, group, len, whole, n, tile;
@@ -112,6 +125,19 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
 // Words a, c of two rows -> words with the two rows' codes side by side as codes_lo / codes_hi take them: channels 0, 1 of the word, and 2, 3
 template <bool E4M3> __device__ __forceinline__ uint32_t pair01(uint32_t a, uint32_t c) { return __byte_perm(a, c, E4M3 ? 0x5140 : 0x5410); }
 template <bool E4M3> __device__ __forceinline__ uint32_t pair23(uint32_t a, uint32_t c) { return __byte_perm(a, c, E4M3 ? 0x7362 : 0x7632); }
+// (a, b) (c, d) + (e, f), and (a, b) (c, d): two fp32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float a, float b, float c, float d, float e, float f) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a), "f"(b), "f"(c), "f"(d), "f"(e), "f"(f));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float a, float b, float c, float d) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
+}
 // Rows and columns of 8 x 8 numbers of 16 bits change places.
 __device__ __forceinline__ uint32_t turn(uint32_t x) {
   uint32_t r;
@@ -154,6 +180,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
   constexpr int NV = ACROSS ? 4 : 8;                    // its scores of each in a step
   __shared__ float s_m[4][ROWS], s_l[4][ROWS], s_factor[ROWS], s_M[ROWS], s_L[ROWS];   // of the warps; of the block, for its cluster
   __shared__ TilePlan s_plan;
+  __shared__ int s_fewest;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   pdl_wait();
   pdl_trigger();
@@ -169,19 +196,26 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
   } else {
     if (warp == 0) {
       const TilePlan w = tile_plan(p.bs, blockIdx.x, (unsigned)blocks, [&](int b) -> int64_t { return b < p.bs ? items * tiles8(p, len8(p, b)) : 0; });
-      if (lane == 0) s_plan = w;
+      const int fewest = fewest8(p);
+      if (lane == 0) s_plan = w, s_fewest = fewest;
     }
     __syncthreads();
     const TilePlan plan = s_plan;
     const unsigned shares = (unsigned)min((int64_t)blocks, plan.total);
     if (blockIdx.x >= shares) return;
     const int64_t first = share_begin(plan.total, blockIdx.x, shares);
-    way.left = share_begin(plan.total, blockIdx.x + 1, shares) - first;
     way.b = plan.sample;
     way.sample(p);
     const unsigned at = (unsigned)(first - plan.before);   // tiles of a sample are below 2^31: the launch sees to it
     const unsigned item = at / (unsigned)way.n;
-    way.tile = (int)(at % (unsigned)way.n), way.h = (int)(item / (unsigned)p.row_groups), way.group = (int)(item % (unsigned)p.row_groups);
+    way.h = (int)(item / (unsigned)p.row_groups), way.group = (int)(item % (unsigned)p.row_groups);
+    if (apart8(plan.total, s_fewest, shares)) {
+      const int64_t from = plan.before + (int64_t)item * way.n;
+      const unsigned c0 = first8(from, plan.total, shares), n = first8(from + way.n, plan.total, shares) - c0, rank = blockIdx.x - c0;
+      way.tile = (int)share_begin(way.n, rank, n), way.left = (int)share_begin(way.n, rank + 1, n) - way.tile;
+    } else {
+      way.tile = (int)(at % (unsigned)way.n), way.left = share_begin(plan.total, blockIdx.x + 1, shares) - first;
+    }
   }
   const unsigned base = smem_addr(dyn8), mine = A8<ROWS>::q_bytes + warp * 2 * A8_SLOT, q_off = (ROWS == 8 ? 8 : 16) * lane;   // offsets in the block's shared memory
   const int n_rows_all = p.T * p.G, Hq = p.c.H * p.G;
@@ -364,28 +398,42 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
       float w[NR][NV];
       const bool all = first + 31 <= lim;
       bool far = !all;
+      // Two scores at a time: neighbours of a query row; across, the two query rows of a row of the cache.
 #pragma unroll
-      for (int e = 0; e < NR; e++) {
-        const float kf[2] = {sc.x * factor[e], sc.y * factor[e]};
-        float x[NV], top = -INFINITY;
+      for (int e = 0; e < NR; e += ACROSS ? 2 : 1) {
+        const float k0[2] = {sc.x * factor[e], sc.y * factor[e]}, k1[2] = {ACROSS ? sc.x * factor[e + ACROSS] : k0[0], ACROSS ? sc.y * factor[e + ACROSS] : k0[1]};
+        const float m0 = -st[e].m, m1 = ACROSS ? -st[e + ACROSS].m : m0;
+        float top = -INFINITY;
 #pragma unroll
-        for (int v = 0; v < NV; v++) x[v] = fmaf(score(e, v), kf[v / (NV / 2)], -st[e].m), top = fmaxf(top, x[v]);
+        for (int v = 0; v < NV; v += ACROSS ? 1 : 2) {
+          const int h2 = v / (NV / 2);
+          const float2 x = ACROSS ? fma2(score(e, v), score(e + ACROSS, v), k0[h2], k1[h2], m0, m1) : fma2(score(e, v), score(e, v + 1), k0[h2], k0[h2], m0, m0);
+          top = max3(top, x.x, x.y);
+          w[e][v] = x.x;
+          if (ACROSS) w[e + ACROSS][v] = x.y;
+          else w[e][v + 1] = x.y;
+        }
         // The running maximum may lie 2^8 below the true one, and p vs 2^-E may reach 2^15: then nothing has to be moved.
-        far |= top > 8.0f || fmaxf(sc.z, sc.w) * st[e].up > 128.0f;
-#pragma unroll
-        for (int v = 0; v < NV; v++) w[e][v] = x[v];
+        far |= top > 8.0f || fmaxf(sc.z, sc.w) * (ACROSS ? fmaxf(st[e].up, st[e + ACROSS].up) : st[e].up) > 128.0f;
       }
       if (!__any_sync(0xffffffffu, far)) {
 #pragma unroll
-        for (int e = 0; e < NR; e++) {
-          const float vs[2] = {sc.z * st[e].up, sc.w * st[e].up};
-          float sum = 0.0f;
+        for (int e = 0; e < NR; e += ACROSS ? 2 : 1) {
+          const float u0 = st[e].up, u1 = ACROSS ? st[e + ACROSS].up : u0;
+          const float2 vs[2] = {mul2(sc.z, sc.z, u0, u1), mul2(sc.w, sc.w, u0, u1)};
+          float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-          for (int v = 0; v < NV; v++) {
-            const float y = ex2(w[e][v]);
-            sum += y, w[e][v] = y * vs[v / (NV / 2)];
+          for (int v = 0; v < NV; v += ACROSS ? 1 : 2) {
+            const float2 z = vs[v / (NV / 2)];
+            float& a = w[e][v];
+            float& c = ACROSS ? w[e + ACROSS][v] : w[e][(v + 1) % NV];
+            a = ex2(a), c = ex2(c);
+            add2(sum0, sum1, a, c);
+            const float2 x = mul2(a, c, z.x, z.y);
+            a = x.x, c = x.y;
           }
-          st[e].l += sum;
+          if (ACROSS) st[e].l += sum0, st[e + ACROSS].l += sum1;
+          else st[e].l += sum0 + sum1;
         }
       } else {
 #pragma unroll
@@ -711,7 +759,8 @@ __global__ void __launch_bounds__(128) attend8_merge_kernel(const __grid_constan
   const int n = tiles8(p, len8(p, b));
   const int64_t first = before + ((int64_t)h * p.row_groups + r / ROWS) * n;
   const unsigned shares = (unsigned)min((int64_t)blocks, total);
-  const int c0 = share_owner(first, total, shares), c1 = share_owner(first + n - 1, total, shares);
+  const bool apart = apart8(total, fewest8(p), shares);
+  const int c0 = apart ? (int)first8(first, total, shares) : share_owner(first, total, shares), c1 = apart ? (int)first8(first + n, total, shares) - 1 : share_owner(first + n - 1, total, shares);
   pdl_wait();
   pdl_trigger();
   if (c0 == c1) return;   // written by its block
@@ -719,10 +768,10 @@ __global__ void __launch_bounds__(128) attend8_merge_kernel(const __grid_constan
             p.lse ? p.lse + row : nullptr);
 }
 
-// Ranges per place on an SM.  SMs do not get the same share of HBM (with a range each the last ends a sixth after the average): of long ranges there are up to four, of which a fast one takes more.
+// Ranges per place on an SM.  SMs do not get the same share of HBM (with a range each the last ends a sixth after the average): of long ranges there are two, so that a fast place may take another.  (Below 1024
+// blocks the shares are computed in 32 bits.)
 int64_t a8_waves(int64_t most, int64_t slots) {
-  const int64_t n = most / (slots * 24);
-  return n < 1 ? 1 : n > 4 ? 4 : n;
+  return most / slots >= 48 ? 2 : 1;
 }
 
 // Blocks of a cluster that share an item, so that one launch does and needs no scratch: where that leaves each at most three tiles.  0: ranges and a second launch.  B200, us, 701 keys of 8 KV heads of
