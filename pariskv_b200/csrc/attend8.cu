@@ -774,8 +774,15 @@ int64_t a8_waves(int64_t most, int64_t slots) {
   return most / slots >= 48 ? 2 : 1;
 }
 
+// Query rows of an item.  Few tiles in all: eight, which has the shortest way through its code (B200, us, five tokens of five heads over 43 keys 8.7 | 15.7 with 32 rows, eight tokens of four heads over 1000
+// keys 11.0 | 14.9); then as many as the KV head has, up to 32, because each item reads the cache again.
+int a8_rows(int64_t heads, int64_t rows, int64_t tiles, int sms) {
+  for (int n = 8; n < 32; n *= 2)
+    if (rows <= n || heads * ((rows + n - 1) / n) * tiles <= 6 * sms) return n;
+  return 32;
+}
 // Blocks of a cluster that share an item, so that one launch does and needs no scratch: where that leaves each at most three tiles.  0: ranges and a second launch.  B200, us, 701 keys of 8 KV heads of
-// four queries 6.4, by two launches 8.5.
+// four queries 7.1, by two launches 8.5.
 int a8_cluster(int64_t items, int64_t tiles, int64_t slots) {
   int64_t n = slots / items;
   n = n > 8 ? 8 : n < 1 ? 1 : n;
@@ -824,8 +831,9 @@ using namespace pk;
 
 extern "C" int64_t pk_cache8_attention_workspace_bytes(int64_t bs, int64_t T, int64_t Hq, int64_t H, int64_t cap) {
   if (bs < 1 || T < 1 || T > 256 || H < 1 || Hq < H || cap < 0) return 0;
-  const int rows = T * (Hq / H) <= 8 ? 8 : T * (Hq / H) <= 16 ? 16 : 32;
-  const int64_t slots = (int64_t)(rows == 32 ? A8<32>::ctas : A8<8>::ctas) * sm_count(), most = bs * H * ((T * (Hq / H) + rows - 1) / rows) * ((cap + A8_TILE - 1) / A8_TILE + 1);
+  const int64_t tiles = (cap + A8_TILE - 1) / A8_TILE + 1;
+  const int rows = a8_rows(bs * H, T * (Hq / H), tiles, sm_count());
+  const int64_t slots = (int64_t)(rows == 32 ? A8<32>::ctas : A8<8>::ctas) * sm_count(), most = bs * H * ((T * (Hq / H) + rows - 1) / rows) * tiles;
   const int64_t items = bs * H * ((T * (Hq / H) + rows - 1) / rows);
   if (a8_cluster(items, most / items, slots)) return 0;
   return 2 * (most < slots ? most : slots * a8_waves(most, slots)) * rows * 130 * 4;
@@ -862,7 +870,7 @@ extern "C" int pk_cache8_attention(const pk_tensor* queries, const pk_cache8* ca
   p.lengths = (const int32_t*)lengths->data, p.bs = (int)bs, p.T = (int)T, p.G = (int)(Hq / H);
   p.out = (uint16_t*)out->data, p.records = (float*)workspace;
   const cudaStream_t st = (cudaStream_t)stream;
-  const int rows = p.T * p.G;
-  if (cache->codes->dtype == PK_E4M3) return rows <= 8 ? launch<true, 8>(p, st) : rows <= 16 ? launch<true, 16>(p, st) : launch<true, 32>(p, st);
-  return rows <= 8 ? launch<false, 8>(p, st) : rows <= 16 ? launch<false, 16>(p, st) : launch<false, 32>(p, st);
+  const int rows = a8_rows(bs * H, p.T * p.G, (p.c.cap + A8_TILE - 1) / A8_TILE + 1, sm_count());
+  if (cache->codes->dtype == PK_E4M3) return rows == 8 ? launch<true, 8>(p, st) : rows == 16 ? launch<true, 16>(p, st) : launch<true, 32>(p, st);
+  return rows == 8 ? launch<false, 8>(p, st) : rows == 16 ? launch<false, 16>(p, st) : launch<false, 32>(p, st);
 }

@@ -583,8 +583,11 @@ extern "C" int pk_matmul_i8(const pk_tensor* x, const pk_tensor* x_scales, const
   if (T <= 16) return launch<16>(x, weight, p, st);
   if (T <= 32) return launch<32>(x, weight, p, st);
   if (T <= 64) return launch<64>(x, weight, p, st);
-  // Tiles of 128 rows and 64 tokens, two blocks an SM, or of 256 x 256 on pairs: 256 x 6144 x 4096 13.7 | 16.2, 512 x 4096 x 12288 32 | 34, 512 x 6144 x 4096 (384 tiles) 21.8 | 17.6, 2048 x 4096 x 12288 109 | 65.
-  if ((T + 63) / 64 * ((O + 127) / 128) <= 2 * sm_count()) return launch<64>(x, weight, p, st);
+  // Tiles of 128 rows and 64 tokens, two blocks an SM, or of 256 x 256 on pairs, by what a round of each takes: 0.33 or 0.4 us for 128 columns, at least 0.6 or 2.3 us for its sums' way out.
+  // 256 x 6144 x 4096 13.5 | 16.2, 512 x 4096 x 12288 32 | 34, 512 x 6144 x 4096 21.8 | 17.4, 2048 x 4096 x 12288 109 | 65, 533 x 17888 x 96 11.5 | 14.1.
+  const int64_t small = (T + 63) / 64 * ((O + 127) / 128), large = (T + 255) / 256 * ((O + 255) / 256), small_places = 2 * sm_count(), pairs = sm_count() / 2;
+  const int64_t small_round = 33 * p.chunks > 60 ? 33 * p.chunks : 60, large_round = 40 * p.chunks > 230 ? 40 * p.chunks : 230;
+  if (small <= small_places || (T > 128 && (small + small_places - 1) / small_places * small_round < (large + pairs - 1) / pairs * large_round)) return launch<64>(x, weight, p, st);
   if (T <= 128) return launch<128>(x, weight, p, st);
   return launch_pair(x, weight, p, st);
 }
