@@ -2,13 +2,20 @@
 //   s_j = ks (q . kc_j),  p_j v_j = (p_j vs) vc_j    with codes kc, vc of a row and the scales ks, vs of its block.
 //
 // HBM bounds a step: 256 bytes a row.  The products run on mma.sync with fp16 operands: a code is an fp16 number exactly (whole numbers: the byte becomes the last bits
-// of 1024 + 128 + code, and 1152 is taken off), so is a query's value once its row has been scaled by a power of two; weights times value scales are rounded to 11 bits, scaled row by
-// row by a power of two that follows the largest of them.
+// of 1024 + 128 + code, and 1152 is taken off), so is a query's value once its row has been scaled by a power of two (below 2^-14 of the row's largest it keeps whole multiples of 2^-24 of that); weights times
+// value scales are rounded to 11 bits, scaled row by row by a power of two that follows the largest of them.  tcgen05 would want the codes as bf16 or fp16 in shared memory first, and up to 32 query rows fill a
+// quarter of its operand.
 // The rows behind the last whole block come from `recent` as bf16, their weights as two bf16 numbers each.
 //
-// Every warp is by itself: 32 rows a step from global memory into its own stages of shared memory by cp.async, one step ahead.  The order of channels in Q K^T and of rows in P V is free, and
+// Every warp is by itself: 32 rows a step from global memory into its own stages of shared memory by cp.async, one step ahead, at any strides.  The order of channels in Q K^T and of rows in P V is free, and
 // chosen so that a lane's fragments of K are 32 consecutive codes of a row, and those of V 16 consecutive codes of four rows.
-// Tiles of 128 rows, four warps of a block side by side, laid end to end over all (sample, KV head, row group) items, cut into equal ranges as in attend_few.cu.
+// Tiles of 128 rows, four warps of a block side by side.  Short caches: a cluster of blocks per item (sample, KV head, group of query rows), one launch.  Others: the tiles of all items, laid end to end, are cut
+// into equal ranges as in attend_few.cu, and attend8_merge_kernel joins the records of items that are cut.
+//
+// B200, us, replayed graphs.  128K keys of 8 heads, a token of four queries each (269 MB) 54, of which the copies with nothing between them take 43, the products 5, the joining launch 3; 16 sequences of 16 - 32K (e4m3)
+// 135, 6.1 TB/s; 32 query rows a KV head over 8 x 58K keys 47 (copies 29, products 12): eight warps an SM by their registers, which wait for one another's turn on the tensor cores 36 % of the time.
+// Kept: loops by segment with one scaling for the 16 rows that share a scale, 100 -> 60; less code around the loops (run once, it costs its fetching) 97 -> 60 for 32 rows; query rows across and a lazy maximum
+// 56 -> 55, 60 -> 52; ranges that end where the items do 50 -> 47.  No better: three stages, two blocks an SM (52 - 54), four ranges a place (67; of long ones two are), two scores an instruction.
 #include "cache8.cuh"
 #include "tiles.cuh"
 
