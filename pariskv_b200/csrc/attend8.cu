@@ -178,6 +178,11 @@ __device__ __forceinline__ float remote(const void* at, int rank) {
   asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(r) : "r"(smem_addr(at)), "r"(rank) : "memory");
   return r;
 }
+__device__ __forceinline__ float4 remote4(const void* at, int rank) {
+  float4 r;
+  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [a];\n\t}" : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "r"(smem_addr(at)), "r"(rank) : "memory");
+  return r;
+}
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 template <bool E4M3, int ROWS, bool DENSE>
@@ -193,10 +198,19 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
   pdl_trigger();
   const int blocks = (int)gridDim.x;
   const int64_t items = (int64_t)p.c.H * p.row_groups;
+  const int n_rows_all = p.T * p.G, Hq = p.c.H * p.G;
+  // 16 channels of query row `row` of an item for this thread, eight of them a row
+  auto query = [&](int b, int h, int group, int row, uint4 (&x)[2]) {
+    const int r = group * ROWS + min(row, min(ROWS, n_rows_all - group * ROWS) - 1);
+    const uint4* from = reinterpret_cast<const uint4*>(p.q + b * p.q_b + (int64_t)(r / p.G) * p.q_t + (int64_t)(h * p.G + r % p.G) * p.q_h + 16 * (tid & 7));
+    x[0] = from[0], x[1] = from[1];
+  };
   Way8 way;
+  uint4 q_first[2];   // a cluster knows its item before it knows the lengths: its queries come together with them
   if (p.cluster) {
     const int item = (int)blockIdx.x / p.cluster, rank = (int)blockIdx.x % p.cluster;
     way.b = item / (int)items, way.h = item % (int)items / p.row_groups, way.group = item % p.row_groups;
+    if (ROWS <= 16) query(way.b, way.h, way.group, tid >> 3, q_first);
     way.sample(p);
     way.tile = way.n * rank / p.cluster, way.left = way.n * (rank + 1) / p.cluster - way.tile;
     if (tid < ROWS) s_M[tid] = -INFINITY, s_L[tid] = 0.0f;
@@ -225,7 +239,6 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
     }
   }
   const unsigned base = smem_addr(dyn8), mine = A8<ROWS>::q_bytes + warp * 2 * A8_SLOT, q_off = (ROWS == 8 ? 8 : 16) * lane;   // offsets in the block's shared memory
-  const int n_rows_all = p.T * p.G, Hq = p.c.H * p.G;
   for (; way.left > 0; way.next(p)) {
     // ---- a segment ----
     const int b = way.b, h = way.h, group = way.group, whole = way.whole, count = way.count();
@@ -255,8 +268,8 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
       cp_commit();
       src += A8_TILE * c_l, row0 += A8_TILE;
     };
-    auto load_recent = [&](int sub, int slot) {   // 16 rows in 16 bits
-      const int r0 = whole + 32 * warp + 16 * sub, live = min(16, way.len - r0), kv = lane >> 4;
+    auto load_recent = [&](int sub, int slot) {   // 16 rows in 16 bits: those of the four warps follow one another, so that blocks of up to 64 rows need one turn
+      const int r0 = whole + 64 * sub + 16 * warp, live = min(16, way.len - r0), kv = lane >> 4;
       const uint16_t* ring = p.c.recent + b * p.c.r_b + h * p.c.r_h + kv * p.c.r_kv + (lane & 15) * 8;
       const unsigned to = base + mine + slot * A8_SLOT + kv * 4096 + (lane & 15) * 16;
       if (live > 0) {
@@ -272,9 +285,9 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
 #pragma unroll 1
     for (int r0 = 0; r0 < ROWS; r0 += 16) {
       const int row = r0 + (tid >> 3), c = tid & 7;   // 16 channels from 16 c on
-      const int r = group * ROWS + min(row, n_rows - 1);
-      const uint4* from = reinterpret_cast<const uint4*>(p.q + b * p.q_b + (int64_t)(r / p.G) * p.q_t + (int64_t)(h * p.G + r % p.G) * p.q_h + 16 * c);
-      const uint4 x[2] = {from[0], from[1]};
+      uint4 x[2];
+      if (ROWS <= 16 && p.cluster) x[0] = q_first[0], x[1] = q_first[1];
+      else query(b, h, group, row, x);
       const uint32_t xw[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
       uint32_t top = 0;
 #pragma unroll
@@ -509,7 +522,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
       load_recent(1, (n_coded + 1) & 1);
 #pragma unroll 1
       for (int sub = 0; sub < 2; sub++) {
-        const int r0 = whole + 32 * warp + 16 * sub, live = min(16, way.len - r0);
+        const int r0 = whole + 64 * sub + 16 * warp, live = min(16, way.len - r0);
         at = mine + ((n_coded + sub) & 1) * A8_SLOT;
         if (sub == 0) cp_wait<1>();
         else cp_wait<0>();
@@ -723,26 +736,30 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
     cluster_sync();
     const int item = (int)blockIdx.x / p.cluster, item_b = item / (int)items, item_h = item % (int)items / p.row_groups, item_group = item % p.row_groups;
     const int n_rows = min(ROWS, n_rows_all - item_group * ROWS);
-    for (int row = (int)blockIdx.x % p.cluster; row < n_rows; row += p.cluster) {
-      const float* o = reinterpret_cast<const float*>(dyn8 + A8<ROWS>::q_bytes + (row >> 3) * 2 * A8_SLOT + A8_SLOT) + (row & 7) * 128 + tid;
-      float m[8], l[8], x[8], M = -INFINITY, L = 0.0f, O = 0.0f;
+    for (int row = (int)blockIdx.x % p.cluster + warp * p.cluster; row < n_rows; row += 4 * p.cluster) {   // a warp a row, four channels a lane
+      const float* o = reinterpret_cast<const float*>(dyn8 + A8<ROWS>::q_bytes + (row >> 3) * 2 * A8_SLOT + A8_SLOT) + (row & 7) * 128 + 4 * lane;
+      float m[8], l[8], M = -INFINITY, L = 0.0f;
+      float4 x[8], O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        const int r = min(i, p.cluster - 1);
-        m[i] = remote(&s_M[row], r), l[i] = remote(&s_L[row], r), x[i] = remote(o, r);
-        M = fmaxf(M, m[i]);
+        if (i >= p.cluster) break;
+        m[i] = remote(&s_M[row], i), l[i] = remote(&s_L[row], i), x[i] = remote4(o, i);
       }
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (i < p.cluster) M = fmaxf(M, m[i]);
 #pragma unroll
       for (int i = 0; i < 8; i++)
         if (i < p.cluster) {
           const float f = m[i] == -INFINITY ? 0.0f : ex2(m[i] - M);
           L += l[i] * f;
-          if (f != 0.0f) O += x[i] * f;   // (a block without rows of this item has not written any; NaN != 0)
+          if (f != 0.0f) O.x += x[i].x * f, O.y += x[i].y * f, O.z += x[i].z * f, O.w += x[i].w * f;   // (a block without rows of this item has not written any; NaN != 0)
         }
       const int rr = item_group * ROWS + row, t = rr / p.G, hq = item_h * p.G + rr % p.G;
       const int64_t out_row = ((int64_t)item_b * p.T + t) * Hq + hq;
-      p.out[out_row * 128 + tid] = f2bf(L == 0.0f ? 0.0f : O / L);
-      if (p.lse && tid == 0) p.lse[out_row] = L == 0.0f ? -INFINITY : M + log2f(L);
+      const bool none = L == 0.0f;
+      *reinterpret_cast<uint2*>(p.out + out_row * 128 + 4 * lane) = make_uint2(pack2(none ? 0.0f : O.x / L, none ? 0.0f : O.y / L), pack2(none ? 0.0f : O.z / L, none ? 0.0f : O.w / L));
+      if (p.lse && lane == 0) p.lse[out_row] = none ? -INFINITY : M + log2f(L);
     }
     cluster_sync();   // no block ends while others read from it
   }
