@@ -65,6 +65,40 @@ __device__ __forceinline__ int fewest8(const Attend8& p) {
   for (int b = threadIdx.x & 31; b < p.bs; b += 32) n = min(n, tiles8(p, len8(p, b)));
   return __reduce_min_sync(0xffffffffu, n);
 }
+// By a warp: the tiles of all items (below 2^31: the launch sees to it), the fewest of one, and the sample with the tile that the block's range begins with.
+struct Plan8 {
+  unsigned total, before;   // before: tiles of the samples before `sample`
+  int sample, fewest;
+};
+__device__ __forceinline__ Plan8 plan8(const Attend8& p, unsigned items, unsigned block, unsigned blocks) {
+  const int lane = threadIdx.x & 31;
+  Plan8 r = {0, 0, 0, 0x7fffffff};
+  unsigned first = 0;
+  for (int b0 = 0; b0 < p.bs; b0 += 32) {
+    const int n = b0 + lane < p.bs ? tiles8(p, len8(p, b0 + lane)) : 0;
+    if (b0 == 0) first = n * items;
+    r.total += __reduce_add_sync(0xffffffffu, n * items), r.fewest = min(r.fewest, n == 0 ? 0x7fffffff : n);
+  }
+  r.fewest = __reduce_min_sync(0xffffffffu, r.fewest);
+  const unsigned at = (unsigned)share_begin(r.total, block, min(blocks, r.total));
+  for (int b0 = 0; b0 < p.bs; b0 += 32) {
+    const unsigned mine = b0 == 0 ? first : b0 + lane < p.bs ? items * tiles8(p, len8(p, b0 + lane)) : 0;
+    unsigned end = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const unsigned o = __shfl_up_sync(0xffffffffu, end, off);
+      if (lane >= off) end += o;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, b0 + lane < p.bs && r.before + end > at);
+    if (past) {
+      const int i = __ffs(past) - 1;
+      r.sample = b0 + i, r.before += __shfl_sync(0xffffffffu, end - mine, i);
+      return r;
+    }
+    r.before += __shfl_sync(0xffffffffu, end, 31);
+  }
+  return r;
+}
 
 // A block's way through its range: segments of consecutive tiles of one item.
 struct Way8 {
@@ -191,8 +225,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
   constexpr int MT = ROWS == 32 ? 2 : 1, NR = 2 * MT;   // operands of 16 query rows; query rows that a lane's scores belong to: 8 e + g, across 2 t4 + e
   constexpr int NV = ACROSS ? 4 : 8;                    // its scores of each in a step
   __shared__ float s_m[4][ROWS], s_l[4][ROWS], s_factor[ROWS], s_M[ROWS], s_L[ROWS];   // of the warps; of the block, for its cluster
-  __shared__ TilePlan s_plan;
-  __shared__ int s_fewest;
+  __shared__ Plan8 s_plan;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   pdl_wait();
   pdl_trigger();
@@ -216,13 +249,12 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
     if (tid < ROWS) s_M[tid] = -INFINITY, s_L[tid] = 0.0f;
   } else {
     if (warp == 0) {
-      const TilePlan w = tile_plan(p.bs, blockIdx.x, (unsigned)blocks, [&](int b) -> int64_t { return b < p.bs ? items * tiles8(p, len8(p, b)) : 0; });
-      const int fewest = fewest8(p);
-      if (lane == 0) s_plan = w, s_fewest = fewest;
+      const Plan8 w = plan8(p, (unsigned)items, blockIdx.x, (unsigned)blocks);
+      if (lane == 0) s_plan = w;
     }
     __syncthreads();
-    const TilePlan plan = s_plan;
-    const unsigned shares = (unsigned)min((int64_t)blocks, plan.total);
+    const Plan8 plan = s_plan;
+    const unsigned shares = min((unsigned)blocks, plan.total);
     if (blockIdx.x >= shares) return;
     const int64_t first = share_begin(plan.total, blockIdx.x, shares);
     way.b = plan.sample;
@@ -230,7 +262,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
     const unsigned at = (unsigned)(first - plan.before);   // tiles of a sample are below 2^31: the launch sees to it
     const unsigned item = at / (unsigned)way.n;
     way.h = (int)(item / (unsigned)p.row_groups), way.group = (int)(item % (unsigned)p.row_groups);
-    if (apart8(plan.total, s_fewest, shares)) {
+    if (apart8(plan.total, plan.fewest, shares)) {
       const int64_t from = plan.before + (int64_t)item * way.n;
       const unsigned c0 = first8(from, plan.total, shares), n = first8(from + way.n, plan.total, shares) - c0, rank = blockIdx.x - c0;
       way.tile = (int)share_begin(way.n, rank, n), way.left = (int)share_begin(way.n, rank + 1, n) - way.tile;
@@ -279,15 +311,26 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
       }
       cp_commit();
     };
-    if (n_coded > 0) load(0);
-    else if (recent) load_recent(0, 0);
+    // Steps of the segment: its tiles of codes, then two of rows in 16 bits.  A group of copies for each, without any where there is none.
+    auto load_step = [&](int j) {
+      if (j < n_coded) load(j & 1);
+      else if (recent && j < n_coded + 2) load_recent(j - n_coded, j & 1);
+      else cp_commit();
+    };
+    // The queries are asked for before the rows, which all blocks ask for at once: behind them they came 2 us later.
+    uint4 q_rows[ROWS / 16 + (ROWS == 8)][2];
+#pragma unroll
+    for (int i = 0; i < (ROWS + 15) / 16; i++) {
+      if (ROWS <= 16 && p.cluster) q_rows[i][0] = q_first[0], q_rows[i][1] = q_first[1];
+      else query(b, h, group, 16 * i + (tid >> 3), q_rows[i]);
+    }
+    load_step(0);
+    load_step(1);
     // queries: as they are, and as fp16 after a power of two per row in the order in which a lane needs them as operands; eight threads a row
-#pragma unroll 1
-    for (int r0 = 0; r0 < ROWS; r0 += 16) {
-      const int row = r0 + (tid >> 3), c = tid & 7;   // 16 channels from 16 c on
-      uint4 x[2];
-      if (ROWS <= 16 && p.cluster) x[0] = q_first[0], x[1] = q_first[1];
-      else query(b, h, group, row, x);
+#pragma unroll
+    for (int i16 = 0; i16 < (ROWS + 15) / 16; i16++) {
+      const int row = 16 * i16 + (tid >> 3), c = tid & 7;   // 16 channels from 16 c on
+      const uint4 (&x)[2] = q_rows[i16];
       const uint32_t xw[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
       uint32_t top = 0;
 #pragma unroll
@@ -352,21 +395,13 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
     const int lim = min(end + group * ROWS / p.G, whole - 1);   // rows up to here are seen by all
     unsigned at = mine;
     for (int j = 0; j < n_coded; j++) {
-      const int first = row0 - A8_TILE;   // of this step; `load` is a step ahead
+      const int first = (way.tile + j) * A8_TILE + 32 * warp;
       at = mine + (j & 1) * A8_SLOT;
-      if (j + 1 < n_coded) {
-        load((j + 1) & 1);
-        cp_wait<1>();
-      } else {
-        row0 += A8_TILE;
-        if (recent) {
-          load_recent(0, (j + 1) & 1);
-          cp_wait<1>();
-        } else {
-          cp_wait<0>();
-        }
+      cp_wait<1>();
+      if (first >= whole) {
+        load_step(j + 2);
+        continue;
       }
-      if (first >= whole) continue;
       // scores of a lane: s[half of the rows][..]: row 8 i + 2 t4 + k of the half (i = c / 4, k = c & 1) and query row g, 8 + g (c >> 1 & 1); across: row g, 8 + g (c >> 1) and query row c & 1
       float s[MT][2][ACROSS ? 4 : 8];
 #pragma unroll
@@ -516,17 +551,19 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
         }
       }
       __syncwarp();
+      load_step(j + 2);
     }
     if (recent) {
       // ---- the rows behind the last whole block, 16 bf16 rows of this warp at a time.  Weights are two bf16 numbers each. ----
-      load_recent(1, (n_coded + 1) & 1);
 #pragma unroll 1
       for (int sub = 0; sub < 2; sub++) {
         const int r0 = whole + 64 * sub + 16 * warp, live = min(16, way.len - r0);
         at = mine + ((n_coded + sub) & 1) * A8_SLOT;
-        if (sub == 0) cp_wait<1>();
-        else cp_wait<0>();
-        if (live <= 0) continue;
+        cp_wait<1>();
+        if (live <= 0) {
+          cp_commit();
+          continue;
+        }
         float x[NR][4];   // score v: row 8 (v >> 1) + 2 t4 + (v & 1); across: row 8 v + g, v < 2
         constexpr int NB = ACROSS ? 2 : 4;
         if (ACROSS) {
@@ -659,6 +696,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
           }
         }
         __syncwarp();
+        cp_commit();
       }
     }
     // ---- the four warps' shares of the segment ----
@@ -788,8 +826,38 @@ __global__ void __launch_bounds__(128) attend8_merge_kernel(const __grid_constan
   pdl_wait();
   pdl_trigger();
   if (c0 == c1) return;   // written by its block
-  merge_row(shared, c1 - c0 + 1, ROWS, r % ROWS, [&](int i) { return p.records + (2 * (int64_t)(c0 + i) + (i == 0)) * (ROWS * 130); }, p.out + row * 128,
-            p.lse ? p.lse + row : nullptr);
+  const int cnt = c1 - c0 + 1, warp = threadIdx.x >> 5, q = r % ROWS;
+  auto record = [&](int i) -> const float* { return p.records + (2 * (int64_t)(c0 + i) + (i == 0)) * (ROWS * 130); };
+  if (cnt > 64) return merge_row(shared, cnt, ROWS, q, record, p.out + row * 128, p.lse ? p.lse + row : nullptr);
+  // Up to 64 records: all of them under way at once, a warp has every fourth, four channels a lane.
+  float4 v[16], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float m[2], l[2], f[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    m[i] = lane + 32 * i < cnt ? record(lane + 32 * i)[ROWS * 128 + q] : -INFINITY;
+    l[i] = lane + 32 * i < cnt ? record(lane + 32 * i)[ROWS * 129 + q] : 0.0f;
+  }
+#pragma unroll
+  for (int k = 0; k < 16; k++) v[k] = 4 * k + warp < cnt ? *reinterpret_cast<const float4*>(record(4 * k + warp) + (int64_t)q * 128 + 4 * lane) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float M = fmaxf(m[0], m[1]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+#pragma unroll
+  for (int i = 0; i < 2; i++) f[i] = m[i] == -INFINITY ? 0.0f : ex2(m[i] - M);
+  float L = l[0] * f[0] + l[1] * f[1];   // (NaN stays, whatever it counts for)
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+#pragma unroll
+  for (int k = 0; k < 16; k++) {
+    const float w = __shfl_sync(0xffffffffu, f[k >> 3], (4 * k + warp) & 31);
+    if (w != 0.0f) o.x += v[k].x * w, o.y += v[k].y * w, o.z += v[k].z * w, o.w += v[k].w * w;   // (NaN != 0)
+  }
+  *reinterpret_cast<float4*>(&shared.o[warp][4 * lane]) = o;
+  __syncthreads();
+  const int c = threadIdx.x;
+  const float O = (shared.o[0][c] + shared.o[1][c]) + (shared.o[2][c] + shared.o[3][c]);
+  p.out[row * 128 + c] = f2bf(L == 0.0f ? 0.0f : O / L);
+  if (p.lse && c == 0) p.lse[row] = L == 0.0f ? -INFINITY : M + log2f(L);
 }
 
 // Ranges per place on an SM.  SMs do not get the same share of HBM (with a range each the last ends a sixth after the average): of long ranges there are two, so that a fast place may take another.  (Below 1024
@@ -883,7 +951,7 @@ extern "C" int pk_cache8_attention(const pk_tensor* queries, const pk_cache8* ca
     PK_REQUIRE(is_contig(lse) && lse->shape[0] == bs && lse->shape[1] == T && lse->shape[2] == Hq, "lse must be contiguous f32 [bs,T,Hq]");
     p.lse = (float*)lse->data;
   }
-  PK_REQUIRE(bs < 65536 && bs * T * Hq < (1LL << 31) && (p.c.cap / A8_TILE + 2) * H * ((T * (Hq / H) + 7) / 8) < (1LL << 31), "sizes out of range");
+  PK_REQUIRE(bs < 65536 && bs * T * Hq < (1LL << 31) && bs * H * ((T * (Hq / H) + 7) / 8) < (1LL << 31) / (p.c.cap / A8_TILE + 2), "sizes out of range");
   p.scale_log2 = scale * 1.4426950408889634f;
   PK_REQUIRE(scale > 0.0f && p.scale_log2 <= 3.4e38f, "scale must be positive, and finite as a factor of log2 e");
   if (bs == 0 || T == 0) return PK_OK;
