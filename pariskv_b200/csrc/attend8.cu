@@ -67,12 +67,12 @@ __device__ __forceinline__ int fewest8(const Attend8& p) {
 }
 // By a warp: the tiles of all items (below 2^31: the launch sees to it), the fewest of one, and the sample with the tile that the block's range begins with.
 struct Plan8 {
-  unsigned total, before;   // before: tiles of the samples before `sample`
+  unsigned total, before, begin;   // before: tiles of the samples before `sample`; begin: of the range
   int sample, fewest;
 };
 __device__ __forceinline__ Plan8 plan8(const Attend8& p, unsigned items, unsigned block, unsigned blocks) {
   const int lane = threadIdx.x & 31;
-  Plan8 r = {0, 0, 0, 0x7fffffff};
+  Plan8 r = {0, 0, 0, 0, 0x7fffffff};
   unsigned first = 0;
   for (int b0 = 0; b0 < p.bs; b0 += 32) {
     const int n = b0 + lane < p.bs ? tiles8(p, len8(p, b0 + lane)) : 0;
@@ -80,7 +80,7 @@ __device__ __forceinline__ Plan8 plan8(const Attend8& p, unsigned items, unsigne
     r.total += __reduce_add_sync(0xffffffffu, n * items), r.fewest = min(r.fewest, n == 0 ? 0x7fffffff : n);
   }
   r.fewest = __reduce_min_sync(0xffffffffu, r.fewest);
-  const unsigned at = (unsigned)share_begin(r.total, block, min(blocks, r.total));
+  const unsigned at = r.begin = (unsigned)share_begin(r.total, block, min(blocks, r.total));
   for (int b0 = 0; b0 < p.bs; b0 += 32) {
     const unsigned mine = b0 == 0 ? first : b0 + lane < p.bs ? items * tiles8(p, len8(p, b0 + lane)) : 0;
     unsigned end = mine;
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
   constexpr int MT = ROWS == 32 ? 2 : 1, NR = 2 * MT;   // operands of 16 query rows; query rows that a lane's scores belong to: 8 e + g, across 2 t4 + e
   constexpr int NV = ACROSS ? 4 : 8;                    // its scores of each in a step
   __shared__ float s_m[4][ROWS], s_l[4][ROWS], s_factor[ROWS], s_M[ROWS], s_L[ROWS];   // of the warps; of the block, for its cluster
-  __shared__ Plan8 s_plan;
+  __shared__ Way8 s_way;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   pdl_wait();
   pdl_trigger();
@@ -248,27 +248,29 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
     way.tile = way.n * rank / p.cluster, way.left = way.n * (rank + 1) / p.cluster - way.tile;
     if (tid < ROWS) s_M[tid] = -INFINITY, s_L[tid] = 0.0f;
   } else {
-    if (warp == 0) {
-      const Plan8 w = plan8(p, (unsigned)items, blockIdx.x, (unsigned)blocks);
-      if (lane == 0) s_plan = w;
+    if (warp == 0) {   // (a division of whole numbers is some forty instructions: two lanes do two of a kind at once)
+      const Plan8 plan = plan8(p, (unsigned)items, blockIdx.x, (unsigned)blocks);
+      const unsigned shares = min((unsigned)blocks, plan.total);
+      Way8 w = {};
+      w.b = plan.sample;
+      if (blockIdx.x < shares) {
+        w.sample(p);
+        const unsigned n = (unsigned)w.n, at = plan.begin - plan.before, item = at / n;
+        w.h = (int)item, w.group = 0;
+        if (p.row_groups > 1) w.h = (int)(item / (unsigned)p.row_groups), w.group = (int)(item % (unsigned)p.row_groups);
+        if (apart8(plan.total, plan.fewest, shares)) {
+          const unsigned c = first8(plan.before + (item + (lane & 1)) * n, plan.total, shares), c0 = __shfl_sync(0xffffffffu, c, 0), cnt = __shfl_sync(0xffffffffu, c, 1) - c0;
+          const unsigned t = (unsigned)share_begin(n, blockIdx.x - c0 + (lane & 1), cnt);
+          w.tile = (int)__shfl_sync(0xffffffffu, t, 0), w.left = __shfl_sync(0xffffffffu, t, 1) - (unsigned)w.tile;
+        } else {
+          w.tile = (int)(at - item * n), w.left = share_begin(plan.total, blockIdx.x + 1, shares) - plan.begin;
+        }
+      }
+      if (lane == 0) s_way = w;
     }
     __syncthreads();
-    const Plan8 plan = s_plan;
-    const unsigned shares = min((unsigned)blocks, plan.total);
-    if (blockIdx.x >= shares) return;
-    const int64_t first = share_begin(plan.total, blockIdx.x, shares);
-    way.b = plan.sample;
-    way.sample(p);
-    const unsigned at = (unsigned)(first - plan.before);   // tiles of a sample are below 2^31: the launch sees to it
-    const unsigned item = at / (unsigned)way.n;
-    way.h = (int)(item / (unsigned)p.row_groups), way.group = (int)(item % (unsigned)p.row_groups);
-    if (apart8(plan.total, plan.fewest, shares)) {
-      const int64_t from = plan.before + (int64_t)item * way.n;
-      const unsigned c0 = first8(from, plan.total, shares), n = first8(from + way.n, plan.total, shares) - c0, rank = blockIdx.x - c0;
-      way.tile = (int)share_begin(way.n, rank, n), way.left = (int)share_begin(way.n, rank + 1, n) - way.tile;
-    } else {
-      way.tile = (int)(at % (unsigned)way.n), way.left = share_begin(plan.total, blockIdx.x + 1, shares) - first;
-    }
+    way = s_way;
+    if (way.left == 0) return;
   }
   const unsigned base = smem_addr(dyn8), mine = A8<ROWS>::q_bytes + warp * 2 * A8_SLOT, q_off = (ROWS == 8 ? 8 : 16) * lane;   // offsets in the block's shared memory
   for (; way.left > 0; way.next(p)) {
