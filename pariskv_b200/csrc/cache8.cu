@@ -23,13 +23,16 @@ __global__ void __launch_bounds__(32 * Append8<BLOCK>::warps, BLOCK == 128 ? 2 :
   pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kv = lane >> 4, ch = (lane & 15) * 8;
   const int64_t b = blockIdx.z, h = blockIdx.y;
+  const uint16_t* from = kv ? v + b * v_b + h * v_h + ch : k + b * k_b + h * k_h + ch;
+  const int64_t from_t = kv ? v_t : k_t;
+  const bool few = T <= WARPS;   // a step: a warp per new row, which is asked for together with the lengths
+  uint4 fresh = make_uint4(0, 0, 0, 0);
+  if (few && blockIdx.x == 0 && warp < T) fresh = *reinterpret_cast<const uint4*>(from + warp * from_t);
   const int n = counts ? min(max(counts[b], 0), T) : T;
   const int64_t len = lengths[b], start = len - n, first = start > 0 ? start : 0, end = len < c.cap ? len : c.cap;
   if (first >= end || n == 0) return;
   const int64_t j0 = first >> c.shift, j = j0 + (int64_t)blockIdx.x * NB, row0 = j << c.shift;   // the first block of this thread block
   if (row0 >= end) return;
-  const uint16_t* from = kv ? v + b * v_b + h * v_h + ch : k + b * k_b + h * k_h + ch;
-  const int64_t from_t = kv ? v_t : k_t;
   uint16_t* ring = c.recent + b * c.r_b + h * c.r_h + kv * c.r_kv + ch;
   auto place = [&](int64_t r) { return ring + (r % c.R) * c.r_l; };
   const int whole = (int)min((int64_t)NB, (end >> c.shift) - j);   // blocks that are whole now
@@ -93,6 +96,12 @@ __global__ void __launch_bounds__(32 * Append8<BLOCK>::warps, BLOCK == 128 ? 2 :
     for (int64_t r = max(jj << c.shift, kept) + warp; r < min((jj + 1) << c.shift, end); r += WARPS)
       *reinterpret_cast<uint4*>(place(r)) = *reinterpret_cast<const uint4*>(from + (r - start) * from_t);
   };
+  if (few) {   // the first thread block, which alone reads rows that were there, writes all that are new
+    if (blockIdx.x != 0) return;
+    if (old) __syncthreads();
+    if (warp < n && start + warp >= kept && start + warp < end) *reinterpret_cast<uint4*>(place(start + warp)) = fresh;
+    return;
+  }
   if (row0 + Append8<BLOCK>::rows <= kept && !(old && j == j0)) return;
   if (old && j == j0) __syncthreads();
 #pragma unroll 1
