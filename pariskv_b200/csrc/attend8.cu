@@ -12,10 +12,12 @@
 // Tiles of 128 rows, four warps of a block side by side.  Short caches: a cluster of blocks per item (sample, KV head, group of query rows), one launch.  Others: the tiles of all items, laid end to end, are cut
 // into equal ranges as in attend_few.cu, and attend8_merge_kernel joins the records of items that are cut.
 //
-// B200, us, replayed graphs.  128K keys of 8 heads, a token of four queries each (269 MB) 54, of which the copies with nothing between them take 43, the products 5, the joining launch 3; 16 sequences of 16 - 32K (e4m3)
-// 135, 6.1 TB/s; 32 query rows a KV head over 8 x 58K keys 47 (copies 29, products 12): eight warps an SM by their registers, which wait for one another's turn on the tensor cores 36 % of the time.
+// B200, us, replayed graphs.  128K keys of 8 heads, a token of four queries each (269 MB) 53: blocks begin their rows 2 us after the start and end after 33 to 49, as fast as their SMs get them (with the products left
+// out the whole takes 46), the joining launch takes 2; 16 sequences of 16 - 32K (e4m3) 135, 6.1 TB/s; 32 query rows a KV head over 8 x 58K keys 44: eight warps an SM by their registers, which wait for one
+// another's turn on the tensor cores 36 % of the time.
 // Kept: loops by segment with one scaling for the 16 rows that share a scale, 100 -> 60; less code around the loops (run once, it costs its fetching) 97 -> 60 for 32 rows; query rows across and a lazy maximum
-// 56 -> 55, 60 -> 52; ranges that end where the items do 50 -> 47.  No better: three stages, two blocks an SM (52 - 54), four ranges a place (67; of long ones two are), two scores an instruction.
+// 56 -> 55, 60 -> 52; ranges that end where the items do 50 -> 47; queries asked for before the rows, two steps of copies at once, all records under way 47.6 -> 44.5.  No better: three stages, two blocks an SM
+// (52 - 54), two ranges a place (58; of long ranges they are kept), two scores an instruction.
 #include "cache8.cuh"
 #include "tiles.cuh"
 

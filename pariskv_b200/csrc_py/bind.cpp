@@ -8,12 +8,15 @@
 // The C ABI stays free of torch types; this module is one of its callers.
 #include <Python.h>
 
+#include <array>
+
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/core/ScalarTypeToTypeMeta.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/pariskv_b200.h"
@@ -824,6 +827,36 @@ PyObject* py_cache8_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   PK_PY_END
 }
 
+// Fresh outputs of one call.  An allocation, its tensor and its end are a microsecond of the host, as much as a quarter of a call on one token: small outputs are parts of one.
+struct Part {
+  at::Tensor* t;
+  std::array<int64_t, 2> shape;
+  int dims;
+  at::ScalarType dt;
+  int64_t bytes() const { return shape[0] * (dims == 2 ? shape[1] : 1) * (int64_t)c10::elementSize(dt); }
+};
+void fresh(const at::Tensor& like, std::initializer_list<Part> parts) {
+  constexpr int64_t MOST = 1 << 17;
+  int64_t total = 0;
+  for (const Part& p : parts) total += (p.bytes() + 255) / 256 * 256;
+  if (total > MOST || total == 0) {
+    for (const Part& p : parts) *p.t = empty_on(like, at::IntArrayRef(p.shape.data(), p.dims), p.dt);
+    return;
+  }
+  const at::Tensor all = empty_on(like, {total}, at::kByte);
+  int64_t at_byte = 0;
+  for (const Part& p : parts) {
+    *p.t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(p.dt));
+    p.t->unsafeGetTensorImpl()->set_sizes_contiguous(at::IntArrayRef(p.shape.data(), p.dims));
+    p.t->unsafeGetTensorImpl()->set_storage_offset(at_byte / (int64_t)c10::elementSize(p.dt));
+    at_byte += (p.bytes() + 255) / 256 * 256;
+  }
+}
+bool describe_fresh(const at::Tensor& t, Arg* a) {
+  a->t = &t;
+  return describe(t, &a->d);
+}
+
 // (a, residual or None, weight, eps) -> (h, codes, scales)
 PyObject* py_add_rmsnorm_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arity(n, 4, "add_rmsnorm_i8")) return nullptr;
@@ -833,9 +866,10 @@ PyObject* py_add_rmsnorm_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   double eps;
   if (!need(a[0], &x, CUDA) || !take(a[1], &r, CUDA) || !need(a[2], &w, CUDA) || !to_f64(a[3], &eps) || !dims(x, 2, "a")) return nullptr;
   const c10::cuda::CUDAGuard guard(x.t->device());
-  if (!same_device({&r, &w}, *x.t) || !output(Py_None, &h, &th, *x.t, x.t->sizes(), at::kBFloat16) || !output(Py_None, &q, &tq, *x.t, x.t->sizes(), at::kChar) ||
-      !output(Py_None, &s, &ts, *x.t, {x.d.shape[0]}, at::kFloat))
-    return nullptr;
+  if (!same_device({&r, &w}, *x.t)) return nullptr;
+  const int64_t B = x.d.shape[0], width = x.d.shape[1];
+  fresh(*x.t, {{&th, {B, width}, 2, at::kBFloat16}, {&tq, {B, width}, 2, at::kChar}, {&ts, {B, 0}, 1, at::kFloat}});
+  if (!describe_fresh(th, &h) || !describe_fresh(tq, &q) || !describe_fresh(ts, &s)) return nullptr;
   if (x.d.shape[0] > 0) {
     void* st = stream_of(*x.t);
     const int rc = without_gil([&] { return pk_add_rmsnorm_i8(x.p(), r.p(), w.p(), h.p(), q.p(), s.p(), eps, st); });
@@ -854,7 +888,8 @@ PyObject* py_quantize_rows_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int64_t gated;
   if (!need(a[0], &x, CUDA) || !to_i64(a[1], &gated) || !dims(x, 2, "x")) return nullptr;
   const c10::cuda::CUDAGuard guard(x.t->device());
-  if (!output(Py_None, &q, &tq, *x.t, {x.d.shape[0], gated ? x.d.shape[1] / 2 : x.d.shape[1]}, at::kChar) || !output(Py_None, &s, &ts, *x.t, {x.d.shape[0]}, at::kFloat)) return nullptr;
+  fresh(*x.t, {{&tq, {x.d.shape[0], gated ? x.d.shape[1] / 2 : x.d.shape[1]}, 2, at::kChar}, {&ts, {x.d.shape[0], 0}, 1, at::kFloat}});
+  if (!describe_fresh(tq, &q) || !describe_fresh(ts, &s)) return nullptr;
   if (x.d.shape[0] > 0) {
     void* st = stream_of(*x.t);
     const int rc = without_gil([&] { return pk_quantize_rows_i8(x.p(), gated != 0, q.p(), s.p(), st); });

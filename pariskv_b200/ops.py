@@ -601,7 +601,7 @@ def cache8_attention(queries, cache, lengths, scale=None, out=None, lse=None):
 
 def add_rmsnorm_i8(a, residual, weight, eps=1e-6):
     """add_rmsnorm for a product in 8 bits: h = a + residual (residual may be None), y = RMS-norm(h) * weight as int8 codes with a scale per token.  Returns (h, codes, scales): bf16 [B,n], int8
-    [B,n], f32 [B].  See pk_add_rmsnorm_i8."""
+    [B,n], f32 [B]; small ones are parts of one allocation.  See pk_add_rmsnorm_i8."""
     return L.native().add_rmsnorm_i8(a, residual, weight, eps)
 
 
