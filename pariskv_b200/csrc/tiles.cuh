@@ -48,44 +48,6 @@ __device__ __forceinline__ int64_t share_begin(int64_t total, unsigned i, unsign
 __device__ __forceinline__ int share_owner(int64_t x, int64_t total, unsigned shares) {
   return total < 1 << 22 ? (int)(((unsigned)(x + 1) * shares - 1) / (unsigned)total) : (int)(((x + 1) * shares - 1) / total);
 }
-struct TilePlan {
-  int64_t total;    // tiles of the launch
-  int64_t before;   // tiles of the samples before `sample`
-  int sample;
-};
-// By a whole warp: the total, and the sample that holds tile share_begin(total, block, min(blocks, total)); tiles_of(b): tiles of sample b, 0 behind the last.
-template <class TilesOf>
-__device__ __forceinline__ TilePlan tile_plan(int bs, unsigned block, unsigned blocks, TilesOf tiles_of) {
-  const int lane = threadIdx.x & 31;
-  const int64_t first = tiles_of(lane);
-  TilePlan r = {0, 0, 0};
-  auto sum = [](int64_t v) {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-    return v;
-  };
-  r.total = sum(first);
-  for (int b0 = 32; b0 < bs; b0 += 32) r.total += sum(tiles_of(b0 + lane));
-  const int64_t t = share_begin(r.total, block, (unsigned)min((int64_t)blocks, r.total));
-  for (int b0 = 0; b0 < bs; b0 += 32) {
-    const int64_t mine = b0 == 0 ? first : tiles_of(b0 + lane);
-    int64_t end = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int64_t o = __shfl_up_sync(0xffffffffu, end, off);
-      if (lane >= off) end += o;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, b0 + lane < bs && r.before + end > t);
-    if (past) {
-      const int i = __ffs(past) - 1;
-      r.sample = b0 + i, r.before += __shfl_sync(0xffffffffu, end - mine, i);
-      return r;
-    }
-    r.before += __shfl_sync(0xffffffffu, end, 31);
-  }
-  return r;
-}
-
 // Joins n partial results of a query row, record(i) = O rows of 128, then `rows` values m (log2), then `rows` sums l, in the order of i: a block of 128
 // threads.  A warp takes every fourth record, four channels a lane, eight loads in flight; latency is what bounds it.
 struct MergeShared {

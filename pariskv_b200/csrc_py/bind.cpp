@@ -774,7 +774,7 @@ PyObject* py_cache8_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor& like = *c.codes.t;
   const c10::cuda::CUDAGuard guard(like.device());
   if (!same_device({&k, &v, &len, &cnt}, like)) return nullptr;
-  if (k.t->numel() == 0 && k.d.shape[1] == 0) Py_RETURN_NONE;
+  if (k.t->numel() == 0) Py_RETURN_NONE;
   void* st = stream_of(like);
   const int rc = without_gil([&] { return pk_cache8_append(&c.c, k.p(), v.p(), len.p(), cnt.p(), st); });
   if (rc) return raise(rc);
