@@ -3,9 +3,26 @@ import pytest
 import torch
 
 from eight_ref import RefCache, attention, kv_rows
-from test_gpu_cache8 import DEV, TYPES, check_attention, filled, i32, ops, queries, samples
+from test_gpu_cache8 import DEV, TYPES, check_attention, check_cache, filled, i32, ops, queries, samples
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("block,recent", [(128, 128), (128, 384), (16, 16), (32, 96)])
+@pytest.mark.parametrize("step", [1, 7, 8, 9, 16, 17, 140])
+def test_append_of_steps_of_every_size(dtype, block, recent, step):
+    """A warp per row, and rows by blocks; a sequence that ends behind the cache, one that begins before it."""
+    n, cap = 420, 400
+    rows = samples((n,), H=1, seed=step)
+    cache = ops().Cache8.empty(2, 1, cap, block=block, dtype=dtype, recent=recent, device=DEV)
+    x = rows[0].transpose(0, 1)[None].expand(2, -1, -1, -1, -1)
+    for at in range(0, n, step):
+        part = x[:, at:at + step]
+        upto = min(n, at + step)
+        ops().cache8_append(cache, part[:, :, :, 0], part[:, :, :, 1], i32(upto, upto - 13))
+    for b, want in ((0, rows[0][:, :cap]), (1, rows[0][:, 13:413][:, :400])):
+        check_cache(ops().Cache8(cache.codes[b:b + 1], cache.scales[b:b + 1], cache.recent[b:b + 1], block), [want], block, dtype)
 
 
 @pytest.mark.parametrize("lengths", [[(i * 37) % 150 for i in range(70)], [(i * 53) % 700 for i in range(40)]])
