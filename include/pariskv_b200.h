@@ -599,7 +599,7 @@ int pk_gemv_w4(const pk_tensor* weight, const pk_tensor* scales, const pk_tensor
  * pk_cache8_read: out bf16 [bs,H,n,2,128] = row i, or row rows[b][h][i] (i64 [bs,H,n]), rounded to bf16.  Without rows, out's rows from the length on are left as they are (n <= cap);
  *   with rows, an entry that is no row of the sequence gives zeros.
  * pk_cache8_attention: token t of T (at most 256) is at position lengths[b] - T + t and sees the rows up to its own: queries, out, lse and scale as in pk_block_attention.  Scores, maxima and
- *   sums have 32 bits; queries and codes meet exactly (values below 2^-14 of the largest of their query as whole multiples of 2^-24 of it), the weights times the values' scales meet the codes as 11 bits (fp16), rows in 16 bits as 17.  Codes of NaN, which
+ *   sums have 32 bits; queries and codes meet exactly, the weights (times the values' scales) meet the codes and the rows in 16 bits as 17 bits, whatever their size.  Codes of NaN, which
  *   the append never writes, and scales below zero are not provided for.
  *
  * pk_add_rmsnorm_i8: h_out = bf16(a + residual) (residual may be NULL), y = h_out * rstd(h_out) * weight in 32 bits, scales[b] = max |y| / 127, codes[b] = y / scale to the nearest;

@@ -1,11 +1,11 @@
 // Attention of the last tokens of the sequences over the cache in 8 bits:  o = sum_j p_j v_j / sum_j p_j,  p_j = 2^((s_j - max s) scale log2 e),
 //   s_j = ks (q . kc_j),  p_j v_j = (p_j vs) vc_j    with codes kc, vc of a row and the scales ks, vs of its block.
 //
-// HBM bounds a step: 256 bytes a row.  The products run on mma.sync with fp16 operands: a code is an fp16 number exactly (whole numbers: the byte becomes the last bits
-// of 1024 + 128 + code, and 1152 is taken off), so is a query's value once its row has been scaled by a power of two (below 2^-14 of the row's largest it keeps whole multiples of 2^-24 of that); weights times
-// value scales are rounded to 11 bits, scaled row by row by a power of two that follows the largest of them.  tcgen05 would want the codes as bf16 or fp16 in shared memory first, and up to 32 query rows fill a
-// quarter of its operand.
-// The rows behind the last whole block come from `recent` as bf16, their weights as two bf16 numbers each.
+// HBM bounds a step: 256 bytes a row.  The products run on mma.sync with bf16 operands, which have the range of 32 bits: a code is a bf16 number exactly, a query's value is one (its row is scaled by a power of two, so
+// that no score overflows before it is scaled back), and a weight times the scale of the values is taken as two of them, 17 bits whatever its size.  One fp16 number for it, under a power of two per query row that
+// follows the largest, has 11 bits down to 2^-14 of the largest and none below 2^-25: a long tail behind one key of most of the weight and a value near zero was lost (B200, us, one fp16 | two bf16: 128K keys
+// 53.5 | 54.5, 16 sequences of 16 - 32K 137 | 140, 32 query rows over 8 x 58K 44.5 | 52).  tcgen05, with rows of the cache as the 128 rows of an operand, would want the codes in 16 bits in shared memory first.
+// The rows behind the last whole block come from `recent` as bf16, their weights as two bf16 numbers each too.
 //
 // Every warp is by itself: 32 rows a step from global memory into its own stages of shared memory by cp.async, one step ahead, at any strides.  The order of channels in Q K^T and of rows in P V is free, and
 // chosen so that a lane's fragments of K are 32 consecutive codes of a row, and those of V 16 consecutive codes of four rows.
@@ -134,40 +134,41 @@ __device__ __forceinline__ void cp_wait() {
 extern __shared__ __align__(128) unsigned char dyn8[];
 __device__ __forceinline__ uint4 lds16(unsigned off) { return *reinterpret_cast<const uint4*>(dyn8 + off); }
 __device__ __forceinline__ uint2 lds8(unsigned off) { return *reinterpret_cast<const uint2*>(dyn8 + off); }
-__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Two codes as fp16 numbers.  Whole numbers: bytes 0 and 2 of w (hi: 1 and 3) become the last bits of 1024 + (code + 128), and 1152 is taken off.  e4m3: bytes 0 and 1 (hi: 2 and 3).
-// The queries lie in the same order.
-template <bool E4M3>
-__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
+// Two codes as bf16 numbers.  Whole numbers, the last bytes of the halves of w: 128 + the last seven bits, and 128, or 256 where the code is below zero, is taken off.  (As lop3 by hand: the compiler's own form of the two
+// masks, with constants on both sides, takes twice the instructions, 128K keys 65 us for 54.)
+__device__ __forceinline__ uint32_t i8_pair(uint32_t w) {
   uint32_t r;
-  if (E4M3) asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(r) : "r"(w));
-  else asm("{\n\t.reg .b32 x;\n\tlop3.b32 x, %1, 0x00ff00ff, 0x64806480, 0x6a;\n\tadd.rn.f16x2 %0, x, %2;\n\t}" : "=r"(r) : "r"(w), "r"(0xe480e480u));
+  asm("{\n\t.reg .b32 x, y;\n\tlop3.b32 x, %1, 0x007f007f, 0x43004300, 0xea;\n\tlop3.b32 y, %1, 0x00800080, 0x43004300, 0xea;\n\tsub.rn.bf16x2 %0, x, y;\n\t}" : "=r"(r) : "r"(w));
   return r;
 }
-template <bool E4M3>
-__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+// e4m3, each continued by its sign to 16 bits: its seven bits as the last of the exponent and the first of the fraction, 2^-120 of the number (below 2^-126: a bf16 number without a leading one, exactly)
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) { return w << 4 & 0x87f087f0u; }
+template <int SELECT>
+__device__ __forceinline__ uint32_t bytes_of(uint32_t a, uint32_t b) {   // with the sign's form of a selector
   uint32_t r;
-  if (E4M3) asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, b;\n\t}" : "=r"(r) : "r"(w));
-  else r = codes_lo<false>(w >> 8);
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "n"(SELECT));
   return r;
 }
-// Words a, c of two rows -> words with the two rows' codes side by side as codes_lo / codes_hi take them: channels 0, 1 of the word, and 2, 3
-template <bool E4M3> __device__ __forceinline__ uint32_t pair01(uint32_t a, uint32_t c) { return __byte_perm(a, c, E4M3 ? 0x5140 : 0x5410); }
-template <bool E4M3> __device__ __forceinline__ uint32_t pair23(uint32_t a, uint32_t c) { return __byte_perm(a, c, E4M3 ? 0x7362 : 0x7632); }
+// K: codes 0 and 2 of w (hi: 1 and 3), of e4m3 2^-120 of them: the queries, which lie in the same order, are multiplied by 2^120
+template <bool E4M3> __device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return E4M3 ? e4m3_pair(bytes_of<0xa280>(w, w)) : i8_pair(w); }
+template <bool E4M3> __device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return E4M3 ? e4m3_pair(bytes_of<0xb391>(w, w)) : i8_pair(w >> 8); }
+// V: code I of words a and c, which are of two rows
+template <bool E4M3, int I>
+__device__ __forceinline__ uint32_t codes_of(uint32_t a, uint32_t c) {
+  if (!E4M3) return i8_pair(bytes_of<(4 + I) << 8 | I>(a, c));
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(e4m3_pair(bytes_of<(12 + I) << 12 | (4 + I) << 8 | (8 + I) << 4 | I>(a, c))), "r"(0x7b807b80u));
+  return r;
+}
+// Weights as two bf16 numbers each, 17 bits: pairs of them, and of what their rounding leaves
+__device__ __forceinline__ void two_of(float a, float c, uint32_t& hi, uint32_t& lo) {
+  hi = pack2(a, c), lo = pack2(a - __uint_as_float(hi << 16), c - __uint_as_float(hi & 0xffff0000u));
+}
 // (a, b) (c, d) + (e, f), and (a, b) (c, d): two fp32 operations in one instruction
 __device__ __forceinline__ float2 fma2(float a, float b, float c, float d, float e, float f) {
   float2 r;
@@ -188,24 +189,14 @@ __device__ __forceinline__ uint32_t turn(uint32_t x) {
   return r;
 }
 
-// Running state of one of a lane's query rows.  m: the largest score when it was last looked for, times log2 e / sqrt d; l: the sum of p over this lane's scores, relative to 2^m; u: the largest p vs then; O is kept as
-// 2^-E of what it stands for, up = 2^-E, down = 2^E with E following u, so that the weights p vs 2^-E are fp16 numbers with all of their bits.
+// Running state of one of a lane's query rows.  m: the largest score when it was last looked for, times log2 e / sqrt d; l: the sum of p over this lane's scores, relative to 2^m, as O is.
 struct RowState {
-  float m, l, u, up, down;
+  float m, l;
 };
-// To a new largest score and a new largest p vs (relative to it): what O has to be multiplied by.
-__device__ __forceinline__ float move(RowState& s, float m, float top) {
-  float f = s.m == -INFINITY ? 0.0f : m > s.m ? ex2(s.m - m) : 1.0f;
+// To a new largest score: what O has to be multiplied by.
+__device__ __forceinline__ float move(RowState& s, float m) {
+  const float f = s.m == -INFINITY ? 0.0f : m > s.m ? ex2(s.m - m) : 1.0f;
   s.m = m, s.l *= f;
-  const float before = s.u * f;
-  s.u = fmaxf(before, top);
-  const float t = s.u * s.up;
-  if (s.u > 0.0f && !(t >= 0.0625f && t <= 64.0f)) {
-    const unsigned ex = min(__float_as_uint(s.u) >> 23, 252u);
-    s.up = __uint_as_float((254u - ex) << 23);
-    f = before == 0.0f ? 0.0f : f * s.up * s.down;
-    s.down = ex == 0 ? __uint_as_float(1u << 22) : __uint_as_float(ex << 23);
-  }
   return f;
 }
 // The same place in the shared memory of block `rank` of the cluster.
@@ -330,7 +321,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
     }
     load_step(0);
     load_step(1);
-    // queries: as they are, and as fp16 after a power of two per row in the order in which a lane needs them as operands; eight threads a row
+    // queries: as they are, and after a power of two per row, so that no score overflows before it is scaled back, in the order in which a lane needs them as operands; eight threads a row
 #pragma unroll
     for (int i16 = 0; i16 < (ROWS + 15) / 16; i16++) {
       const int row = 16 * i16 + (tid >> 3), c = tid & 7;   // 16 channels from 16 c on
@@ -352,9 +343,13 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
         raw[0] = x[0], raw[1] = x[1];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          const float f[4] = {__uint_as_float(xw[2 * k] << 16) * up, __uint_as_float(xw[2 * k] & 0xffff0000u) * up, __uint_as_float(xw[2 * k + 1] << 16) * up,
-                              __uint_as_float(xw[2 * k + 1] & 0xffff0000u) * up};
-          const uint32_t lo = half2_of(f[0], f[E4M3 ? 1 : 2]), hi = half2_of(f[E4M3 ? 2 : 1], f[3]);
+          float f[4] = {__uint_as_float(xw[2 * k] << 16) * up, __uint_as_float(xw[2 * k] & 0xffff0000u) * up, __uint_as_float(xw[2 * k + 1] << 16) * up,
+                        __uint_as_float(xw[2 * k + 1] & 0xffff0000u) * up};
+          if (E4M3) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) f[i] *= 0x1p120f;
+          }
+          const uint32_t lo = pack2(f[0], f[2]), hi = pack2(f[1], f[3]);
           const int s = 4 * (c & 1) + k, of = 4 * (row & 7) + (c >> 1);   // the lane that it is for
           if (ROWS == 8) {
             *reinterpret_cast<uint2*>(dyn8 + s * 256 + of * 8) = make_uint2(lo, hi);
@@ -376,7 +371,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
     auto row_of = [&](int e) { return ACROSS ? 2 * t4 + e : 8 * e + g; };
 #pragma unroll
     for (int e = 0; e < NR; e++) {
-      st[e] = {-INFINITY, 0.0f, 0.0f, 1.0f, 1.0f};
+      st[e] = {-INFINITY, 0.0f};
       factor[e] = s_factor[row_of(e)];
       last[e] = end + (group * ROWS + min(row_of(e), n_rows - 1)) / p.G;
     }
@@ -431,13 +426,13 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
           }
           if (ACROSS) {
             const uint2 q = lds8(q_off + ks * 256);
-            mma_f16(s[0][half], b[0][0], b[1][0], b[0][1], b[1][1], q.x, q.y);
+            mma_bf16(s[0][half], b[0][0], b[1][0], b[0][1], b[1][1], q.x, q.y);
           } else {
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) {
               const uint4 q = lds16(q_off + (mt * 8 + ks) * 512);
-              mma_f16(s[mt][half], q.x, q.y, q.z, q.w, b[0][0], b[0][1]);
-              mma_f16(s[mt][half] + (ACROSS ? 0 : 4), q.x, q.y, q.z, q.w, b[1][0], b[1][1]);
+              mma_bf16(s[mt][half], q.x, q.y, q.z, q.w, b[0][0], b[0][1]);
+              mma_bf16(s[mt][half] + (ACROSS ? 0 : 4), q.x, q.y, q.z, q.w, b[1][0], b[1][1]);
             }
           }
         }
@@ -453,7 +448,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
         return s[e >> 1][v >> 2][4 * (v >> 1 & 1) + 2 * (e & 1) + (v & 1)];
       };
       auto row_at = [&](int v) { return ACROSS ? 16 * (v >> 1) + 8 * (v & 1) + g : 16 * (v >> 2) + 8 * (v >> 1 & 1) + 2 * t4 + (v & 1); };
-      uint32_t pw[NR][NV / 2];   // weights as pairs of fp16 numbers: of the columns 2 t4, 2 t4 + 1; across: see below
+      uint32_t pw[NR][NV / 2], pl[NR][NV / 2];   // weights as pairs of bf16 numbers, of the columns 2 t4, 2 t4 + 1, and what their rounding left; across: see below
       float w[NR][NV];
       const bool all = first + 31 <= lim;
       bool far = !all;
@@ -472,23 +467,20 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
           if (ACROSS) w[e + ACROSS][v] = x.y;
           else w[e][v + 1] = x.y;
         }
-        // The running maximum may lie 2^8 below the true one, and p vs 2^-E may reach 2^15: then nothing has to be moved.
-        far |= top > 8.0f || fmaxf(sc.z, sc.w) * (ACROSS ? fmaxf(st[e].up, st[e + ACROSS].up) : st[e].up) > 128.0f;
+        far |= top > 8.0f;   // the running maximum may lie 2^8 below the true one: then nothing has to be moved
       }
       if (!__any_sync(0xffffffffu, far)) {
 #pragma unroll
         for (int e = 0; e < NR; e += ACROSS ? 2 : 1) {
-          const float u0 = st[e].up, u1 = ACROSS ? st[e + ACROSS].up : u0;
-          const float2 vs[2] = {mul2(sc.z, sc.z, u0, u1), mul2(sc.w, sc.w, u0, u1)};
           float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
           for (int v = 0; v < NV; v += ACROSS ? 1 : 2) {
-            const float2 z = vs[v / (NV / 2)];
+            const float z = v / (NV / 2) ? sc.w : sc.z;
             float& a = w[e][v];
             float& c = ACROSS ? w[e + ACROSS][v] : w[e][(v + 1) % NV];
             a = ex2(a), c = ex2(c);
             add2(sum0, sum1, a, c);
-            const float2 x = mul2(a, c, z.x, z.y);
+            const float2 x = mul2(a, c, z, z);
             a = x.x, c = x.y;
           }
           if (ACROSS) st[e].l += sum0, st[e + ACROSS].l += sum1;
@@ -498,7 +490,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
 #pragma unroll
         for (int e = 0; e < NR; e++) {
           const float kf[2] = {sc.x * factor[e], sc.y * factor[e]}, vs[2] = {sc.z, sc.w};
-          float m = st[e].m, top = 0.0f, sum = 0.0f;
+          float m = st[e].m, sum = 0.0f;
           bool seen[NV];
 #pragma unroll
           for (int v = 0; v < NV; v++) {
@@ -512,24 +504,25 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
             const float y = seen[v] ? ex2(fmaf(score(e, v), kf[v / (NV / 2)], -least)) : 0.0f;
             sum += y;
             w[e][v] = seen[v] ? y * vs[v / (NV / 2)] : 0.0f;   // (the scale of a block that it does not see may be NaN)
-            top = fmaxf(top, w[e][v]);
           }
-          const float f = move(st[e], m, row_max(top));
+          const float f = move(st[e], m);
           st[e].l += sum;
           if (__any_sync(0xffffffffu, f != 1.0f)) scale_row(e, f);
-#pragma unroll
-          for (int v = 0; v < NV; v++) w[e][v] *= st[e].up;
         }
       }
       // across: pairs are two query rows of one row of the cache; an exchange of 8 x 8 numbers makes them two rows of one query row
       if (ACROSS) {
 #pragma unroll
-        for (int v = 0; v < 4; v++) pw[v >> 1][v & 1] = turn(half2_of(w[0][v], w[1][v]));
+        for (int v = 0; v < 4; v++) {
+          uint32_t hi, lo;
+          two_of(w[0][v], w[1][v], hi, lo);
+          pw[v >> 1][v & 1] = turn(hi), pl[v >> 1][v & 1] = turn(lo);
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < NR; e++)
 #pragma unroll
-          for (int v = 0; v < NV; v += 2) pw[e][v >> 1] = half2_of(w[e][v], w[e][v + 1]);
+          for (int v = 0; v < NV; v += 2) two_of(w[e][v], w[e][v + 1], pw[e][v >> 1], pl[e][v >> 1]);
       }
 #pragma unroll
       for (int half = 0; half < 2; half++) {
@@ -539,18 +532,23 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
 #pragma unroll
         for (int wd = 0; wd < 4; wd++) {
           auto word = [&](int i) { return wd == 0 ? v[i].x : wd == 1 ? v[i].y : wd == 2 ? v[i].z : v[i].w; };
-          const uint32_t a0 = pair01<E4M3>(word(0), word(1)), a1 = pair01<E4M3>(word(2), word(3)), c0 = pair23<E4M3>(word(0), word(1)), c1 = pair23<E4M3>(word(2), word(3));
-          const uint32_t bs[4][2] = {{codes_lo<E4M3>(a0), codes_lo<E4M3>(a1)}, {codes_hi<E4M3>(a0), codes_hi<E4M3>(a1)}, {codes_lo<E4M3>(c0), codes_lo<E4M3>(c1)},
-                                     {codes_hi<E4M3>(c0), codes_hi<E4M3>(c1)}};
+          const uint32_t bs[4][2] = {{codes_of<E4M3, 0>(word(0), word(1)), codes_of<E4M3, 0>(word(2), word(3))}, {codes_of<E4M3, 1>(word(0), word(1)), codes_of<E4M3, 1>(word(2), word(3))},
+                                     {codes_of<E4M3, 2>(word(0), word(1)), codes_of<E4M3, 2>(word(2), word(3))}, {codes_of<E4M3, 3>(word(0), word(1)), codes_of<E4M3, 3>(word(2), word(3))}};
           if (ACROSS) {
-            mma_f16(o[0][2 * wd], bs[0][0], bs[1][0], bs[0][1], bs[1][1], pw[half][0], pw[half][1]);
-            mma_f16(o[0][2 * wd + 1], bs[2][0], bs[3][0], bs[2][1], bs[3][1], pw[half][0], pw[half][1]);
+#pragma unroll
+            for (int i = 0; i < 2; i++) mma_bf16(o[0][2 * wd + i], bs[2 * i][0], bs[2 * i + 1][0], bs[2 * i][1], bs[2 * i + 1][1], pw[half][0], pw[half][1]);
+#pragma unroll
+            for (int i = 0; i < 2; i++) mma_bf16(o[0][2 * wd + i], bs[2 * i][0], bs[2 * i + 1][0], bs[2 * i][1], bs[2 * i + 1][1], pl[half][0], pl[half][1]);
           } else {
+            const int c = 2 * half % (NV / 2), d = (2 * half + 1) % (NV / 2);
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-              for (int i = 0; i < 4; i++)
-                mma_f16(o[mt][(4 * wd + i) % ON], pw[2 * mt][2 * half % (NV / 2)], pw[2 * mt + 1][2 * half % (NV / 2)], pw[2 * mt][(2 * half + 1) % (NV / 2)], pw[2 * mt + 1][(2 * half + 1) % (NV / 2)], bs[i][0], bs[i][1]);
+              for (int i = 0; i < 4; i++) mma_bf16(o[mt][(4 * wd + i) % ON], pw[2 * mt][c], pw[2 * mt + 1][c], pw[2 * mt][d], pw[2 * mt + 1][d], bs[i][0], bs[i][1]);
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) mma_bf16(o[mt][(4 * wd + i) % ON], pl[2 * mt][c], pl[2 * mt + 1][c], pl[2 * mt][d], pl[2 * mt + 1][d], bs[i][0], bs[i][1]);
           }
         }
       }
@@ -599,7 +597,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
         uint32_t hi[NR][2], lo[NR][2];   // pairs of weights, and what their rounding left; across as above
 #pragma unroll
         for (int e = 0; e < NR; e++) {
-          float m = st[e].m, top = 0.0f, sum = 0.0f;
+          float m = st[e].m, sum = 0.0f;
           bool seen[NB];
 #pragma unroll
           for (int v = 0; v < NB; v++) {
@@ -613,20 +611,18 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
 #pragma unroll
           for (int v = 0; v < NB; v++) {
             x[e][v] = seen[v] ? ex2(x[e][v] - least) : 0.0f;
-            sum += x[e][v], top = fmaxf(top, x[e][v]);
+            sum += x[e][v];
           }
-          const float f = move(st[e], m, row_max(top));
+          const float f = move(st[e], m);
           st[e].l += sum;
           if (__any_sync(0xffffffffu, f != 1.0f)) scale_row(e, f);
-#pragma unroll
-          for (int v = 0; v < NB; v++) x[e][v] *= st[e].up;
         }
 #pragma unroll
         for (int e = 0; e < NR; e++)
 #pragma unroll
           for (int i = 0; i < 2; i++) {
             const float a = ACROSS ? x[0][(2 * e + i) % 2] : x[e][2 * i], c = ACROSS ? x[1][(2 * e + i) % 2] : x[e][(2 * i + 1) % 4];
-            hi[e][i] = pack2(a, c), lo[e][i] = pack2(a - __uint_as_float(hi[e][i] << 16), c - __uint_as_float(hi[e][i] & 0xffff0000u));
+            two_of(a, c, hi[e][i], lo[e][i]);
           }
         if (ACROSS) {
 #pragma unroll
@@ -716,7 +712,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
     auto share = [&](int e) {   // what this warp's O of a query row counts for
       const int r = row_of(e);
       const float M = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-      return st[e].m == -INFINITY ? 0.0f : ex2(st[e].m - M) * st[e].down;
+      return st[e].m == -INFINITY ? 0.0f : ex2(st[e].m - M);
     };
 #pragma unroll
     for (int e = 0; e < (ACROSS ? 1 : NR); e++) {   // eight query rows at a time
