@@ -791,7 +791,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
         if (i < p.cluster) {
           const float f = m[i] == -INFINITY ? 0.0f : ex2(m[i] - M);
           L += l[i] * f;
-          if (f != 0.0f) O.x += x[i].x * f, O.y += x[i].y * f, O.z += x[i].z * f, O.w += x[i].w * f;   // (a block without rows of this item has not written any; NaN != 0)
+          if (m[i] != -INFINITY) O.x += x[i].x * f, O.y += x[i].y * f, O.z += x[i].z * f, O.w += x[i].w * f;   // (a block without rows of this item has not written any)
         }
       const int rr = item_group * ROWS + row, t = rr / p.G, hq = item_h * p.G + rr % p.G;
       const int64_t out_row = ((int64_t)item_b * p.T + t) * Hq + hq;
@@ -828,7 +828,7 @@ __global__ void __launch_bounds__(128) attend8_merge_kernel(const __grid_constan
   if (c0 == c1) return;   // written by its block
   const int cnt = c1 - c0 + 1, warp = threadIdx.x >> 5, q = r % ROWS;
   auto record = [&](int i) -> const float* { return p.records + (2 * (int64_t)(c0 + i) + (i == 0)) * (ROWS * 130); };
-  if (cnt > 64) return merge_row(shared, cnt, ROWS, q, record, p.out + row * 128, p.lse ? p.lse + row : nullptr);
+  if (cnt > 64) return merge_row<true>(shared, cnt, ROWS, q, record, p.out + row * 128, p.lse ? p.lse + row : nullptr);
   // Up to 64 records: all of them under way at once, a warp has every fourth, four channels a lane.
   float4 v[16], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float m[2], l[2], f[2];
@@ -850,7 +850,7 @@ __global__ void __launch_bounds__(128) attend8_merge_kernel(const __grid_constan
 #pragma unroll
   for (int k = 0; k < 16; k++) {
     const float w = __shfl_sync(0xffffffffu, f[k >> 3], (4 * k + warp) & 31);
-    if (w != 0.0f) o.x += v[k].x * w, o.y += v[k].y * w, o.z += v[k].z * w, o.w += v[k].w * w;   // (NaN != 0)
+    o.x += v[k].x * w, o.y += v[k].y * w, o.z += v[k].z * w, o.w += v[k].w * w;   // (a weight of zero too: what is not a number stays)
   }
   *reinterpret_cast<float4*>(&shared.o[warp][4 * lane]) = o;
   __syncthreads();

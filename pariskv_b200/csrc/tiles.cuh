@@ -49,11 +49,12 @@ __device__ __forceinline__ int share_owner(int64_t x, int64_t total, unsigned sh
   return total < 1 << 22 ? (int)(((unsigned)(x + 1) * shares - 1) / (unsigned)total) : (int)(((x + 1) * shares - 1) / total);
 }
 // Joins n partial results of a query row, record(i) = O rows of 128, then `rows` values m (log2), then `rows` sums l, in the order of i: a block of 128
-// threads.  A warp takes every fourth record, four channels a lane, eight loads in flight; latency is what bounds it.
+// threads.  A warp takes every fourth record, four channels a lane, eight loads in flight; latency is what bounds it.  ALL: a record whose weight is zero counts too, so that what is not a number in it
+// is not lost; every record then has to have been written.
 struct MergeShared {
   float o[4][128], l[4];
 };
-template <class Record>
+template <bool ALL = false, class Record>
 __device__ __forceinline__ void merge_row(MergeShared& s, int n, int rows, int r, Record record, uint16_t* out, float* lse) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   float M = -INFINITY;
@@ -79,7 +80,7 @@ __device__ __forceinline__ void merge_row(MergeShared& s, int n, int rows, int r
 #pragma unroll
       for (int k = 0; k < 8; k++) {
         const float fk = __shfl_sync(0xffffffffu, f, k0 + k);
-        if (k0 + k < cnt && fk != 0.0f) o[0] += v[k].x * fk, o[1] += v[k].y * fk, o[2] += v[k].z * fk, o[3] += v[k].w * fk;   // (NaN != 0)
+        if (k0 + k < cnt && (ALL || fk != 0.0f)) o[0] += v[k].x * fk, o[1] += v[k].y * fk, o[2] += v[k].z * fk, o[3] += v[k].w * fk;   // (NaN != 0)
       }
     }
   }

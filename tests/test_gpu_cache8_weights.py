@@ -1,4 +1,4 @@
-"""Attention over the cache in 8 bits where its numbers cover a wide range: weights far below the largest, values and queries of very different sizes, the smallest codes."""
+"""Attention over the cache in 8 bits where its numbers cover a wide range: weights far below the largest, values and queries of very different sizes, the smallest codes, NaN under weights of next to nothing."""
 import pytest
 import torch
 
@@ -103,3 +103,26 @@ def test_the_smallest_codes(H, G, T, n):
     q = 2 * torch.randn(1, T, H * G, 128, generator=g)
     q[..., 5] = 0.0
     check([x.to(BF).to(DEV)], 64, torch.float8_e4m3fn, q.to(BF).to(DEV), scale=3.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,G,T,n", SHAPES)
+def test_a_block_that_is_not_a_number_under_weights_of_nothing(dtype, H, G, T, n):
+    """A block that holds an infinity reads as NaN: no weight is too small for that, whichever blocks of the grid share the sequence."""
+    for row in (40, n // 2, n - 200):
+        x, q = sink(torch.Generator().manual_seed(6), H, n, 400, (1, T, H * G))
+        x[:, row, 1, 3] = float("inf")
+        cache = filled([x], 16, dtype)
+        assert ops().cache8_attention(q, cache, i32(n)).isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,G,T,n", SHAPES)
+def test_an_infinity_behind_the_blocks_under_weights_of_nothing(dtype, H, G, T, n):
+    """A row in 16 bits by itself: the channel is an infinity, or 0 times one, and the others are as they were."""
+    x, q = sink(torch.Generator().manual_seed(7), H, n, 400, (1, T, H * G))
+    x[:, n - T, 1, 3] = float("inf")   # seen by every token
+    assert (n - T) // 16 == n // 16
+    out = ops().cache8_attention(q, filled([x], 16, dtype), i32(n))
+    assert not out[..., 3].isfinite().any()
+    assert out[..., :3].isfinite().all() and out[..., 4:].isfinite().all()
