@@ -76,7 +76,7 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
   return (uint32_t)lo | (uint32_t)hi << 16;
 }
 // Codes of values whose largest magnitude is amax:  y M / amax to the nearest, ties to the even one, M = 127 (e4m3: 448), as 32-bit arithmetic gives it from (y M / u) / (amax / u) with a power of two
-// u = 128 (512), which keeps the product from overflowing.  A division per value took two thirds of the kernels' instructions.
+// u = 128 (512), which keeps the product from overflowing (amax / u is exact where amax has 16 bits; one of 32 bits has to be above 2^-119 or zero).  A division per value took two thirds of the kernels' instructions.
 constexpr float CODE_MAGIC = 12582912.0f;   // 1.5 2^23: a sum with it ends in the whole number that the other is rounded to
 __device__ __forceinline__ uint32_t code_bytes(const uint32_t* n) { return __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410); }
 template <bool E4M3>

@@ -142,7 +142,14 @@ __global__ void __launch_bounds__(THREADS) rows_i8_kernel(const __grid_constant_
   for (int i = 0; i < THREADS / 32; i++) m = max(m, s_max[i]);
   const bool fine = m < 0x7f800000u;
   const float amax = __uint_as_float(m);
-  const std::conditional_t<MODE == PLAIN, Coder16<false>, Coder32> code(amax);
+  const bool small = MODE != PLAIN && amax < 1e-30f;   // amax / 128 may be no number of 32 bits: the row and its maximum are multiplied by 2^64, which is exact
+  if (small) {
+#pragma unroll
+    for (int k = 0; k < N; k++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) y[k][e] *= 0x1p64f;
+  }
+  const std::conditional_t<MODE == PLAIN, Coder16<false>, Coder32> code(small ? amax * 0x1p64f : amax);
 #pragma unroll
   for (int k = 0; k < N; k++) {
     const int i = (k * THREADS + tid) * 8;
