@@ -58,3 +58,19 @@ def test_a_layer_step_by_step(tokens):
     gate, up = gu.double().chunk(2, -1)
     check_codes(c, s, gate / (1 + torch.exp(-gate)) * up, 16 * 2.0 ** -24)
     product(c, s, w_d)
+
+
+def test_weights_by_rows():
+    """A matrix of 16 bits by quantize_rows_i8, as the integration guide has it: a row of zeros gives zeros, no code is beyond 127, and a product is off by half a code of each operand at most."""
+    g = torch.Generator().manual_seed(2)
+    w = (torch.randn(700, 512, generator=g) * 0.02).to(BF).to(DEV)
+    w[3] = 0
+    codes, scales = ops().quantize_rows_i8(w)
+    assert codes.min() >= -127 and codes.abs().amax(-1).eq(127).sum() == 699 and scales[3] == 0
+    x = torch.randn(9, 512, generator=g).to(BF).to(DEV)
+    cx, sx = ops().quantize_rows_i8(x)
+    y = ops().matmul_i8(cx, sx, codes, scales).double()
+    want = x.double() @ w.double().t()
+    half_x, half_w = sx.double()[:, None] / 2, scales.double()[:, None] / 2
+    bound = half_x * w.double().abs().sum(-1) + (half_w * x.double().abs().sum(-1)).t() + half_x * half_w.t() * 512
+    assert ((y - want).abs() <= bound * (1 + 2.0 ** -20) + 2.0 ** -8 * (want.abs() + bound) * 1.001).all() and not y[:, 3].any()
