@@ -20,6 +20,8 @@ def attend_all(ref, queries, scale):
     out, lse, tol = torch.zeros(queries.shape, dtype=torch.float64, device=DEV), torch.full((bs, T, Hq), float("-inf"), dtype=torch.float64, device=DEV), torch.zeros(queries.shape, dtype=torch.float64, device=DEV)
     for b in range(bs):
         n = ref.rows[b].shape[1]
+        if n == 0:
+            continue
         at = torch.arange(n, device=DEV)
         seen = (at <= n - T + torch.arange(T, device=DEV)[:, None])[:, None]   # [T,1,n]
         for h in range(H):
