@@ -1,10 +1,11 @@
 // Attention of the last tokens of the sequences over the cache in 8 bits:  o = sum_j p_j v_j / sum_j p_j,  p_j = 2^((s_j - max s) scale log2 e),
 //   s_j = ks (q . kc_j),  p_j v_j = (p_j vs) vc_j    with codes kc, vc of a row and the scales ks, vs of its block.
 //
-// HBM bounds a step: 256 bytes a row.  The products run on mma.sync with bf16 operands, which have the range of 32 bits: a code is a bf16 number exactly, a query's value is one (its row is scaled by a power of two, so
-// that no score overflows before it is scaled back), and a weight times the scale of the values is taken as two of them, 17 bits whatever its size.  One fp16 number for it, under a power of two per query row that
-// follows the largest, has 11 bits down to 2^-14 of the largest and none below 2^-25: a long tail behind one key of most of the weight and a value near zero was lost (B200, us, one fp16 | two bf16: 128K keys
-// 53.5 | 54.5, 16 sequences of 16 - 32K 137 | 140, 32 query rows over 8 x 58K 44.5 | 52).  tcgen05, with rows of the cache as the 128 rows of an operand, would want the codes in 16 bits in shared memory first.
+// HBM bounds a step: 256 bytes a row.  The products run on mma.sync, whose operands of 16 bits hold codes and queries exactly: keys and queries as fp16, which takes the fewest instructions, the queries after a power of
+// two per row, or as bf16 where a query's values are too far apart for that (and always from 17 query rows on).  A weight times the scale of the values is taken as two bf16 numbers, 17 bits whatever its size, and the
+// values' codes as bf16: one fp16 number for it, under a power of two per query row that follows the largest, has 11 bits down to 2^-14 of the largest and none below 2^-25, so that a long tail behind one key of most of
+// the weight and a value near zero is lost.  (B200, us, one fp16 | two bf16: 128K keys 53.4 | 53.7, 16 sequences of 16 - 32K 136 | 136, after a second of them 138 | 141, 32 query rows over 8 x 58K 44.5 | 52.5.)
+// tcgen05, with rows of the cache as the 128 rows of an operand, would want the codes in 16 bits in shared memory first.
 // The rows behind the last whole block come from `recent` as bf16, their weights as two bf16 numbers each too.
 //
 // Every warp is by itself: 32 rows a step from global memory into its own stages of shared memory by cp.async, one step ahead, at any strides.  The order of channels in Q K^T and of rows in P V is free, and
@@ -18,6 +19,8 @@
 // Kept: loops by segment with one scaling for the 16 rows that share a scale, 100 -> 60; less code around the loops (run once, it costs its fetching) 97 -> 60 for 32 rows; query rows across and a lazy maximum
 // 56 -> 55, 60 -> 52; ranges that end where the items do 50 -> 47; queries asked for before the rows, two steps of copies at once, all records under way 47.6 -> 44.5.  No better: three stages, two blocks an SM
 // (52 - 54), two ranges a place (58; of long ranges they are kept), two scores an instruction.
+#include <type_traits>
+
 #include "cache8.cuh"
 #include "tiles.cuh"
 
@@ -134,6 +137,16 @@ __device__ __forceinline__ void cp_wait() {
 extern __shared__ __align__(128) unsigned char dyn8[];
 __device__ __forceinline__ uint4 lds16(unsigned off) { return *reinterpret_cast<const uint4*>(dyn8 + off); }
 __device__ __forceinline__ uint2 lds8(unsigned off) { return *reinterpret_cast<const uint2*>(dyn8 + off); }
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -154,9 +167,24 @@ __device__ __forceinline__ uint32_t bytes_of(uint32_t a, uint32_t b) {   // with
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "n"(SELECT));
   return r;
 }
-// K: codes 0 and 2 of w (hi: 1 and 3), of e4m3 2^-120 of them: the queries, which lie in the same order, are multiplied by 2^120
-template <bool E4M3> __device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return E4M3 ? e4m3_pair(bytes_of<0xa280>(w, w)) : i8_pair(w); }
-template <bool E4M3> __device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return E4M3 ? e4m3_pair(bytes_of<0xb391>(w, w)) : i8_pair(w >> 8); }
+// K: two codes of w as fp16 numbers, which takes less than as bf16.  Whole numbers: codes 0 and 2 (hi: 1 and 3) become the last bits of 1024 + (code + 128), and 1152 is taken off.  e4m3: codes 0 and 1 (hi: 2
+// and 3).  WIDE: as bf16 numbers, codes 0 and 2 (hi: 1 and 3), of e4m3 2^-120 of them.  The queries lie in the same order.
+template <bool E4M3, bool WIDE>
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
+  if (WIDE) return E4M3 ? e4m3_pair(bytes_of<0xa280>(w, w)) : i8_pair(w);
+  uint32_t r;
+  if (E4M3) asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(r) : "r"(w));
+  else asm("{\n\t.reg .b32 x;\n\tlop3.b32 x, %1, 0x00ff00ff, 0x64806480, 0x6a;\n\tadd.rn.f16x2 %0, x, %2;\n\t}" : "=r"(r) : "r"(w), "r"(0xe480e480u));
+  return r;
+}
+template <bool E4M3, bool WIDE>
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+  if (WIDE) return E4M3 ? e4m3_pair(bytes_of<0xb391>(w, w)) : i8_pair(w >> 8);
+  uint32_t r;
+  if (E4M3) asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, b;\n\t}" : "=r"(r) : "r"(w));
+  else r = codes_lo<false, false>(w >> 8);
+  return r;
+}
 // V: code I of words a and c, which are of two rows
 template <bool E4M3, int I>
 __device__ __forceinline__ uint32_t codes_of(uint32_t a, uint32_t c) {
@@ -212,11 +240,13 @@ __device__ __forceinline__ float4 remote4(const void* at, int rank) {
 }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-template <bool E4M3, int ROWS, bool DENSE>
+// PAIRED: up to four query rows.  They are columns 0 to 3 of the products and 4 to 7 too, and the second parts of the weights are the weights of the latter, so that one product has both (16 sequences of 16 - 32K, after a second of them, e4m3 146 -> 143 us, int8 157 -> 152).
+template <bool E4M3, int ROWS, bool DENSE, bool PAIRED>
 __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(const __grid_constant__ Attend8 p) {
   constexpr bool ACROSS = A8<ROWS>::across;
   constexpr int MT = ROWS == 32 ? 2 : 1, NR = 2 * MT;   // operands of 16 query rows; query rows that a lane's scores belong to: 8 e + g, across 2 t4 + e
   constexpr int NV = ACROSS ? 4 : 8;                    // its scores of each in a step
+  constexpr bool NARROW = ROWS < 32;                    // queries and keys' codes as fp16 where that is exact (of 32 rows the two forms do not fit into the registers)
   __shared__ float s_m[4][ROWS], s_l[4][ROWS], s_factor[ROWS], s_M[ROWS], s_L[ROWS];   // of the warps; of the block, for its cluster
   __shared__ Way8 s_way;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
@@ -227,7 +257,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
   const int n_rows_all = p.T * p.G, Hq = p.c.H * p.G;
   // 16 channels of query row `row` of an item for this thread, eight of them a row
   auto query = [&](int b, int h, int group, int row, uint4 (&x)[2]) {
-    const int r = group * ROWS + min(row, min(ROWS, n_rows_all - group * ROWS) - 1);
+    const int r = group * ROWS + min(PAIRED ? row & 3 : row, min(ROWS, n_rows_all - group * ROWS) - 1);
     const uint4* from = reinterpret_cast<const uint4*>(p.q + b * p.q_b + (int64_t)(r / p.G) * p.q_t + (int64_t)(h * p.G + r % p.G) * p.q_h + 16 * (tid & 7));
     x[0] = from[0], x[1] = from[1];
   };
@@ -321,46 +351,59 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
     }
     load_step(0);
     load_step(1);
-    // queries: as they are, and after a power of two per row, so that no score overflows before it is scaled back, in the order in which a lane needs them as operands; eight threads a row
+    // queries: as they are, and as fp16 after a power of two per row in the order in which a lane needs them as operands; eight threads a row.  The largest of a row becomes a number from 2^12 to 2^13 (at the ends
+    // of the range less, or up to 2^15), so that all that is not below 2^-29 of it is an fp16 number exactly.  Where a value is, which no model's queries have unless a channel is out of all proportion, the block's
+    // queries and its keys' codes become bf16.
+    auto stage = [&](auto wide) {
+      constexpr bool WIDE = decltype(wide)::value;
+      bool far_below = false;
 #pragma unroll
-    for (int i16 = 0; i16 < (ROWS + 15) / 16; i16++) {
-      const int row = 16 * i16 + (tid >> 3), c = tid & 7;   // 16 channels from 16 c on
-      const uint4 (&x)[2] = q_rows[i16];
-      const uint32_t xw[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
-      uint32_t top = 0;
+      for (int i16 = 0; i16 < (ROWS + 15) / 16; i16++) {
+        const int row = 16 * i16 + (tid >> 3), c = tid & 7;   // 16 channels from 16 c on
+        const uint4 (&x)[2] = q_rows[i16];
+        const uint32_t xw[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+        uint32_t top = 0, low = 0x7fff7fffu;   // low: the smallest that is not zero
 #pragma unroll
-      for (int i = 0; i < 8; i++) top = __vmaxu2(top, xw[i] & 0x7fff7fffu);
-      top = max(top & 0xffffu, top >> 16);
+        for (int i = 0; i < 8; i++) top = __vmaxu2(top, xw[i] & 0x7fff7fffu), low = __vminu2(low, __vsub2(xw[i] & 0x7fff7fffu, 0x00010001u));
+        top = max(top & 0xffffu, top >> 16), low = min(low & 0xffffu, low >> 16) + 1;
 #pragma unroll
-      for (int off = 1; off < 8; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
-      // the largest of the row becomes a number from 1 to 2; a row with an infinity or NaN becomes NaN
-      const unsigned ex = max(min(top >> 7, 252u), 2u);
-      const bool fine = top < 0x7f80u;
-      const float up = fine ? __uint_as_float((254u - ex) << 23) : NAN;
-      if (row < ROWS) {
-        if (c == 0) s_factor[row] = fine ? __uint_as_float(ex << 23) * p.scale_log2 : NAN;
-        uint4* raw = reinterpret_cast<uint4*>(dyn8 + ROWS * 256 + row * A8_QS + 32 * c);
-        raw[0] = x[0], raw[1] = x[1];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          float f[4] = {__uint_as_float(xw[2 * k] << 16) * up, __uint_as_float(xw[2 * k] & 0xffff0000u) * up, __uint_as_float(xw[2 * k + 1] << 16) * up,
-                        __uint_as_float(xw[2 * k + 1] & 0xffff0000u) * up};
-          if (E4M3) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) f[i] *= 0x1p120f;
+        for (int off = 1; off < 8; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+        // a row with an infinity or NaN becomes NaN
+        const unsigned ex = max(min(top >> 7, 252u), 16u);
+        const bool fine = top < 0x7f80u;
+        const float up = fine ? __uint_as_float((254u - ex) << 23) : NAN;
+        far_below |= fine && ex > max(low >> 7, 1u) + 29;
+        if (row < ROWS) {
+          if (c == 0) s_factor[row] = fine ? __uint_as_float((WIDE ? ex : ex - 12) << 23) * p.scale_log2 : NAN;
+          if (!WIDE || !NARROW) {
+            uint4* raw = reinterpret_cast<uint4*>(dyn8 + ROWS * 256 + row * A8_QS + 32 * c);
+            raw[0] = x[0], raw[1] = x[1];
           }
-          const uint32_t lo = pack2(f[0], f[2]), hi = pack2(f[1], f[3]);
-          const int s = 4 * (c & 1) + k, of = 4 * (row & 7) + (c >> 1);   // the lane that it is for
-          if (ROWS == 8) {
-            *reinterpret_cast<uint2*>(dyn8 + s * 256 + of * 8) = make_uint2(lo, hi);
-          } else {   // a0, a1 rows g and g + 8 of the first pair of channels, a2, a3 of the second
-            uint32_t* to = reinterpret_cast<uint32_t*>(dyn8 + ((row >> 4) * 8 + s) * 512 + of * 16) + (row >> 3 & 1);
-            to[0] = lo, to[2] = hi;
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            float f[4] = {__uint_as_float(xw[2 * k] << 16) * up, __uint_as_float(xw[2 * k] & 0xffff0000u) * up, __uint_as_float(xw[2 * k + 1] << 16) * up,
+                          __uint_as_float(xw[2 * k + 1] & 0xffff0000u) * up};
+#pragma unroll
+            for (int i = 0; i < 4; i++) f[i] *= !WIDE ? 0x1p12f : E4M3 ? 0x1p120f : 1.0f;
+            const uint32_t lo = WIDE ? pack2(f[0], f[2]) : half2_of(f[0], f[E4M3 ? 1 : 2]), hi = WIDE ? pack2(f[1], f[3]) : half2_of(f[E4M3 ? 2 : 1], f[3]);
+            const int s = 4 * (c & 1) + k, of = 4 * (row & 7) + (c >> 1);   // the lane that it is for
+            if (ROWS == 8) {
+              *reinterpret_cast<uint2*>(dyn8 + s * 256 + of * 8) = make_uint2(lo, hi);
+            } else {   // a0, a1 rows g and g + 8 of the first pair of channels, a2, a3 of the second
+              uint32_t* to = reinterpret_cast<uint32_t*>(dyn8 + ((row >> 4) * 8 + s) * 512 + of * 16) + (row >> 3 & 1);
+              to[0] = lo, to[2] = hi;
+            }
           }
         }
       }
+      return far_below;
+    };
+    bool wide = true;
+    if constexpr (NARROW) wide = __syncthreads_or(stage(std::false_type()));
+    if (wide) {
+      stage(std::true_type());
+      __syncthreads();
     }
-    __syncthreads();
     // O: operand rows g, g + 8 are query rows, the two columns channels 32 t4 + n and + 16; across: the two columns query rows, operand rows channels 16 g + 2 n, + 1
     constexpr int ON = ACROSS ? 8 : 16;
     float o[MT][ON][4] = {};
@@ -373,7 +416,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
     for (int e = 0; e < NR; e++) {
       st[e] = {-INFINITY, 0.0f};
       factor[e] = s_factor[row_of(e)];
-      last[e] = end + (group * ROWS + min(row_of(e), n_rows - 1)) / p.G;
+      last[e] = end + (group * ROWS + min(PAIRED ? row_of(e) & 3 : row_of(e), n_rows - 1)) / p.G;
     }
     auto scale_row = [&](int e, float f) {
 #pragma unroll
@@ -391,169 +434,188 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
       return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
     };
-    const int lim = min(end + group * ROWS / p.G, whole - 1);   // rows up to here are seen by all
+    const int lim = min(end + group * ROWS / p.G, whole - 1) - 31;   // 32 rows that begin up to here are seen by all
     unsigned at = mine;
-    for (int j = 0; j < n_coded; j++) {
-      const int first = (way.tile + j) * A8_TILE + 32 * warp;
-      at = mine + (j & 1) * A8_SLOT;
-      cp_wait<1>();
-      if (first >= whole) {
-        load_step(j + 2);
-        continue;
-      }
-      // scores of a lane: s[half of the rows][..]: row 8 i + 2 t4 + k of the half (i = c / 4, k = c & 1) and query row g, 8 + g (c >> 1 & 1); across: row g, 8 + g (c >> 1) and query row c & 1
-      float s[MT][2][ACROSS ? 4 : 8];
-#pragma unroll
-      for (int half = 0; half < 2; half++) {
-        uint4 kw[2][2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const unsigned from = at + (8 * (2 * half + i) + g) * 128;
-          kw[i][0] = lds16(from + (((2 * t4) ^ (g & 1)) << 4)), kw[i][1] = lds16(from + (((2 * t4 + 1) ^ (g & 1)) << 4));
+    auto coded_rows = [&](auto wide) {
+      constexpr bool WIDE = decltype(wide)::value;
+      for (int j = 0; j < n_coded; j++) {
+        const int first = (way.tile + j) * A8_TILE + 32 * warp;
+        at = mine + (j & 1) * A8_SLOT;
+        cp_wait<1>();
+        if (first >= whole) {
+          load_step(j + 2);
+          continue;
         }
+        // scores of a lane: s[half of the rows][..]: row 8 i + 2 t4 + k of the half (i = c / 4, k = c & 1) and query row g, 8 + g (c >> 1 & 1); across: row g, 8 + g (c >> 1) and query row c & 1
+        float s[MT][2][ACROSS ? 4 : 8];
+        auto product = [](float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+          if (WIDE) mma_bf16(c, a0, a1, a2, a3, b0, b1);
+          else mma_f16(c, a0, a1, a2, a3, b0, b1);
+        };
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-          for (int c = 0; c < (ACROSS ? 4 : 8); c++) s[mt][half][c] = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < 8; ks++) {
-          uint32_t b[2][2];
+        for (int half = 0; half < 2; half++) {
+          uint4 kw[2][2];
 #pragma unroll
           for (int i = 0; i < 2; i++) {
-            const uint4 v = kw[i][ks >> 2];
-            const uint32_t w = (ks & 3) == 0 ? v.x : (ks & 3) == 1 ? v.y : (ks & 3) == 2 ? v.z : v.w;
-            b[i][0] = codes_lo<E4M3>(w), b[i][1] = codes_hi<E4M3>(w);
+            const unsigned from = at + (8 * (2 * half + i) + g) * 128;
+            kw[i][0] = lds16(from + (((2 * t4) ^ (g & 1)) << 4)), kw[i][1] = lds16(from + (((2 * t4 + 1) ^ (g & 1)) << 4));
           }
-          if (ACROSS) {
-            const uint2 q = lds8(q_off + ks * 256);
-            mma_bf16(s[0][half], b[0][0], b[1][0], b[0][1], b[1][1], q.x, q.y);
-          } else {
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-              const uint4 q = lds16(q_off + (mt * 8 + ks) * 512);
-              mma_bf16(s[mt][half], q.x, q.y, q.z, q.w, b[0][0], b[0][1]);
-              mma_bf16(s[mt][half] + (ACROSS ? 0 : 4), q.x, q.y, q.z, q.w, b[1][0], b[1][1]);
+          for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int c = 0; c < (ACROSS ? 4 : 8); c++) s[mt][half][c] = 0.0f;
+#pragma unroll
+          for (int ks = 0; ks < 8; ks++) {
+            uint32_t b[2][2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const uint4 v = kw[i][ks >> 2];
+              const uint32_t w = (ks & 3) == 0 ? v.x : (ks & 3) == 1 ? v.y : (ks & 3) == 2 ? v.z : v.w;
+              b[i][0] = codes_lo<E4M3, WIDE>(w), b[i][1] = codes_hi<E4M3, WIDE>(w);
+            }
+            if (ACROSS) {
+              const uint2 q = lds8(q_off + ks * 256);
+              product(s[0][half], b[0][0], b[1][0], b[0][1], b[1][1], q.x, q.y);
+            } else {
+#pragma unroll
+              for (int mt = 0; mt < MT; mt++) {
+                const uint4 q = lds16(q_off + (mt * 8 + ks) * 512);
+                product(s[mt][half], q.x, q.y, q.z, q.w, b[0][0], b[0][1]);
+                product(s[mt][half] + (ACROSS ? 0 : 4), q.x, q.y, q.z, q.w, b[1][0], b[1][1]);
+              }
             }
           }
         }
-      }
-      float4 sc;   // scales: K of the first and second 16 rows, V of them
-      {
-        const uint4 x = lds16(at + A8_STAGE);
-        sc = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
-      }
-      // score v of query row e: half v / (NV / 2), and its row in the step
-      auto score = [&](int e, int v) -> float& {
-        if (ACROSS) return s[0][v >> 1][2 * (v & 1) + (e & 1)];
-        return s[e >> 1][v >> 2][4 * (v >> 1 & 1) + 2 * (e & 1) + (v & 1)];
-      };
-      auto row_at = [&](int v) { return ACROSS ? 16 * (v >> 1) + 8 * (v & 1) + g : 16 * (v >> 2) + 8 * (v >> 1 & 1) + 2 * t4 + (v & 1); };
-      uint32_t pw[NR][NV / 2], pl[NR][NV / 2];   // weights as pairs of bf16 numbers, of the columns 2 t4, 2 t4 + 1, and what their rounding left; across: see below
-      float w[NR][NV];
-      const bool all = first + 31 <= lim;
-      bool far = !all;
-      // Two scores at a time: neighbours of a query row; across, the two query rows of a row of the cache.
-#pragma unroll
-      for (int e = 0; e < NR; e += ACROSS ? 2 : 1) {
-        const float k0[2] = {sc.x * factor[e], sc.y * factor[e]}, k1[2] = {ACROSS ? sc.x * factor[e + ACROSS] : k0[0], ACROSS ? sc.y * factor[e + ACROSS] : k0[1]};
-        const float m0 = -st[e].m, m1 = ACROSS ? -st[e + ACROSS].m : m0;
-        float top = -INFINITY;
-#pragma unroll
-        for (int v = 0; v < NV; v += ACROSS ? 1 : 2) {
-          const int h2 = v / (NV / 2);
-          const float2 x = ACROSS ? fma2(score(e, v), score(e + ACROSS, v), k0[h2], k1[h2], m0, m1) : fma2(score(e, v), score(e, v + 1), k0[h2], k0[h2], m0, m0);
-          top = max3(top, x.x, x.y);
-          w[e][v] = x.x;
-          if (ACROSS) w[e + ACROSS][v] = x.y;
-          else w[e][v + 1] = x.y;
+        float4 sc;   // scales: K of the first and second 16 rows, V of them
+        {
+          const uint4 x = lds16(at + A8_STAGE);
+          sc = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
         }
-        far |= top > 8.0f;   // the running maximum may lie 2^8 below the true one: then nothing has to be moved
-      }
-      if (!__any_sync(0xffffffffu, far)) {
+        // score v of query row e: half v / (NV / 2), and its row in the step
+        auto score = [&](int e, int v) -> float& {
+          if (ACROSS) return s[0][v >> 1][2 * (v & 1) + (e & 1)];
+          return s[e >> 1][v >> 2][4 * (v >> 1 & 1) + 2 * (e & 1) + (v & 1)];
+        };
+        auto row_at = [&](int v) { return ACROSS ? 16 * (v >> 1) + 8 * (v & 1) + g : 16 * (v >> 2) + 8 * (v >> 1 & 1) + 2 * t4 + (v & 1); };
+        uint32_t pw[NR][NV / 2], pl[NR][NV / 2];   // weights as pairs of bf16 numbers, of the columns 2 t4, 2 t4 + 1, and what their rounding left; across: see below
+        float w[NR][NV];
+        const bool all = first <= lim;
+        bool far = !all;
+        // Two scores at a time: neighbours of a query row; across, the two query rows of a row of the cache.
 #pragma unroll
         for (int e = 0; e < NR; e += ACROSS ? 2 : 1) {
-          float sum0 = 0.0f, sum1 = 0.0f;
+          const float k0[2] = {sc.x * factor[e], sc.y * factor[e]}, k1[2] = {ACROSS ? sc.x * factor[e + ACROSS] : k0[0], ACROSS ? sc.y * factor[e + ACROSS] : k0[1]};
+          const float m0 = -st[e].m, m1 = ACROSS ? -st[e + ACROSS].m : m0;
+          float top = -INFINITY;
 #pragma unroll
           for (int v = 0; v < NV; v += ACROSS ? 1 : 2) {
-            const float z = v / (NV / 2) ? sc.w : sc.z;
-            float& a = w[e][v];
-            float& c = ACROSS ? w[e + ACROSS][v] : w[e][(v + 1) % NV];
-            a = ex2(a), c = ex2(c);
-            add2(sum0, sum1, a, c);
-            const float2 x = mul2(a, c, z, z);
-            a = x.x, c = x.y;
+            const int h2 = v / (NV / 2);
+            const float2 x = ACROSS ? fma2(score(e, v), score(e + ACROSS, v), k0[h2], k1[h2], m0, m1) : fma2(score(e, v), score(e, v + 1), k0[h2], k0[h2], m0, m0);
+            top = max3(top, x.x, x.y);
+            w[e][v] = x.x;
+            if (ACROSS) w[e + ACROSS][v] = x.y;
+            else w[e][v + 1] = x.y;
           }
-          if (ACROSS) st[e].l += sum0, st[e + ACROSS].l += sum1;
-          else st[e].l += sum0 + sum1;
+          far |= top > 8.0f;   // the running maximum may lie 2^8 below the true one: then nothing has to be moved
         }
-      } else {
+        if (!__any_sync(0xffffffffu, far)) {
 #pragma unroll
-        for (int e = 0; e < NR; e++) {
-          const float kf[2] = {sc.x * factor[e], sc.y * factor[e]}, vs[2] = {sc.z, sc.w};
-          float m = st[e].m, sum = 0.0f;
-          bool seen[NV];
+          for (int e = 0; e < NR; e += ACROSS ? 2 : 1) {
+            float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-          for (int v = 0; v < NV; v++) {
-            seen[v] = all || (first + row_at(v) < whole && first + row_at(v) <= last[e]);
-            if (seen[v]) m = fmaxf(m, score(e, v) * kf[v / (NV / 2)]);
+            for (int v = 0; v < NV; v += ACROSS ? 1 : 2) {
+              const float z = v / (NV / 2) ? sc.w : sc.z;
+              float& a = w[e][v];
+              float& c = ACROSS ? w[e + ACROSS][v] : w[e][(v + 1) % NV];
+              a = ex2(a), c = ex2(c);
+              add2(sum0, sum1, a, c);
+              const float2 x = mul2(a, c, z, z);
+              a = x.x, c = x.y;
+            }
+            if (ACROSS) st[e].l += sum0, st[e + ACROSS].l += sum1;
+            else st[e].l += sum0 + sum1;
           }
-          m = row_max(m);
-          const float least = m == -INFINITY ? 0.0f : m;
+        } else {
 #pragma unroll
-          for (int v = 0; v < NV; v++) {
-            const float y = seen[v] ? ex2(fmaf(score(e, v), kf[v / (NV / 2)], -least)) : 0.0f;
-            sum += y;
-            w[e][v] = seen[v] ? y * vs[v / (NV / 2)] : 0.0f;   // (the scale of a block that it does not see may be NaN)
+          for (int e = 0; e < NR; e++) {
+            const float kf[2] = {sc.x * factor[e], sc.y * factor[e]}, vs[2] = {sc.z, sc.w};
+            float m = st[e].m, sum = 0.0f;
+            bool seen[NV];
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+              seen[v] = all || (first + row_at(v) < whole && first + row_at(v) <= last[e]);
+              if (seen[v]) m = fmaxf(m, score(e, v) * kf[v / (NV / 2)]);
+            }
+            m = row_max(m);
+            const float least = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+              const float y = seen[v] ? ex2(fmaf(score(e, v), kf[v / (NV / 2)], -least)) : 0.0f;
+              sum += y;
+              w[e][v] = seen[v] ? y * vs[v / (NV / 2)] : 0.0f;   // (the scale of a block that it does not see may be NaN)
+            }
+            const float f = move(st[e], m);
+            st[e].l += sum;
+            if (__any_sync(0xffffffffu, f != 1.0f)) scale_row(e, f);
           }
-          const float f = move(st[e], m);
-          st[e].l += sum;
-          if (__any_sync(0xffffffffu, f != 1.0f)) scale_row(e, f);
         }
+        // across: pairs are two query rows of one row of the cache; an exchange of 8 x 8 numbers makes them two rows of one query row
+        if (ACROSS) {
+#pragma unroll
+          for (int v = 0; v < 4; v++) {
+            uint32_t hi, lo;
+            two_of(w[0][v], w[1][v], hi, lo);
+            if (PAIRED) {
+              pw[v >> 1][v & 1] = turn(t4 < 2 ? hi : lo);
+            } else {
+              pw[v >> 1][v & 1] = turn(hi), pl[v >> 1][v & 1] = turn(lo);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < NR; e++)
+#pragma unroll
+            for (int v = 0; v < NV; v += 2) two_of(w[e][v], w[e][v + 1], pw[e][v >> 1], pl[e][v >> 1]);
+        }
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          uint4 v[4];   // rows 2 t4, 2 t4 + 1, and eight further; channels 16 g ..
+#pragma unroll
+          for (int i = 0; i < 4; i++) v[i] = lds16(at + 4096 + (16 * half + 8 * (i >> 1) + 2 * t4 + (i & 1)) * 128 + ((g ^ (2 * t4)) << 4));
+#pragma unroll
+          for (int wd = 0; wd < 4; wd++) {
+            auto word = [&](int i) { return wd == 0 ? v[i].x : wd == 1 ? v[i].y : wd == 2 ? v[i].z : v[i].w; };
+            const uint32_t bs[4][2] = {{codes_of<E4M3, 0>(word(0), word(1)), codes_of<E4M3, 0>(word(2), word(3))}, {codes_of<E4M3, 1>(word(0), word(1)), codes_of<E4M3, 1>(word(2), word(3))},
+                                       {codes_of<E4M3, 2>(word(0), word(1)), codes_of<E4M3, 2>(word(2), word(3))}, {codes_of<E4M3, 3>(word(0), word(1)), codes_of<E4M3, 3>(word(2), word(3))}};
+            if (ACROSS) {
+#pragma unroll
+              for (int i = 0; i < 2; i++) mma_bf16(o[0][2 * wd + i], bs[2 * i][0], bs[2 * i + 1][0], bs[2 * i][1], bs[2 * i + 1][1], pw[half][0], pw[half][1]);
+              if (!PAIRED) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) mma_bf16(o[0][2 * wd + i], bs[2 * i][0], bs[2 * i + 1][0], bs[2 * i][1], bs[2 * i + 1][1], pl[half][0], pl[half][1]);
+              }
+            } else {
+              const int c = 2 * half % (NV / 2), d = (2 * half + 1) % (NV / 2);
+#pragma unroll
+              for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) mma_bf16(o[mt][(4 * wd + i) % ON], pw[2 * mt][c], pw[2 * mt + 1][c], pw[2 * mt][d], pw[2 * mt + 1][d], bs[i][0], bs[i][1]);
+#pragma unroll
+              for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) mma_bf16(o[mt][(4 * wd + i) % ON], pl[2 * mt][c], pl[2 * mt + 1][c], pl[2 * mt][d], pl[2 * mt + 1][d], bs[i][0], bs[i][1]);
+            }
+          }
+        }
+        __syncwarp();
+        load_step(j + 2);
       }
-      // across: pairs are two query rows of one row of the cache; an exchange of 8 x 8 numbers makes them two rows of one query row
-      if (ACROSS) {
-#pragma unroll
-        for (int v = 0; v < 4; v++) {
-          uint32_t hi, lo;
-          two_of(w[0][v], w[1][v], hi, lo);
-          pw[v >> 1][v & 1] = turn(hi), pl[v >> 1][v & 1] = turn(lo);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < NR; e++)
-#pragma unroll
-          for (int v = 0; v < NV; v += 2) two_of(w[e][v], w[e][v + 1], pw[e][v >> 1], pl[e][v >> 1]);
-      }
-#pragma unroll
-      for (int half = 0; half < 2; half++) {
-        uint4 v[4];   // rows 2 t4, 2 t4 + 1, and eight further; channels 16 g ..
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = lds16(at + 4096 + (16 * half + 8 * (i >> 1) + 2 * t4 + (i & 1)) * 128 + ((g ^ (2 * t4)) << 4));
-#pragma unroll
-        for (int wd = 0; wd < 4; wd++) {
-          auto word = [&](int i) { return wd == 0 ? v[i].x : wd == 1 ? v[i].y : wd == 2 ? v[i].z : v[i].w; };
-          const uint32_t bs[4][2] = {{codes_of<E4M3, 0>(word(0), word(1)), codes_of<E4M3, 0>(word(2), word(3))}, {codes_of<E4M3, 1>(word(0), word(1)), codes_of<E4M3, 1>(word(2), word(3))},
-                                     {codes_of<E4M3, 2>(word(0), word(1)), codes_of<E4M3, 2>(word(2), word(3))}, {codes_of<E4M3, 3>(word(0), word(1)), codes_of<E4M3, 3>(word(2), word(3))}};
-          if (ACROSS) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) mma_bf16(o[0][2 * wd + i], bs[2 * i][0], bs[2 * i + 1][0], bs[2 * i][1], bs[2 * i + 1][1], pw[half][0], pw[half][1]);
-#pragma unroll
-            for (int i = 0; i < 2; i++) mma_bf16(o[0][2 * wd + i], bs[2 * i][0], bs[2 * i + 1][0], bs[2 * i][1], bs[2 * i + 1][1], pl[half][0], pl[half][1]);
-          } else {
-            const int c = 2 * half % (NV / 2), d = (2 * half + 1) % (NV / 2);
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-              for (int i = 0; i < 4; i++) mma_bf16(o[mt][(4 * wd + i) % ON], pw[2 * mt][c], pw[2 * mt + 1][c], pw[2 * mt][d], pw[2 * mt + 1][d], bs[i][0], bs[i][1]);
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-              for (int i = 0; i < 4; i++) mma_bf16(o[mt][(4 * wd + i) % ON], pl[2 * mt][c], pl[2 * mt + 1][c], pl[2 * mt][d], pl[2 * mt + 1][d], bs[i][0], bs[i][1]);
-          }
-        }
-      }
-      __syncwarp();
-      load_step(j + 2);
+    };
+    if constexpr (NARROW) {
+      if (!wide) coded_rows(std::false_type());
+      else coded_rows(std::true_type());
+    } else {
+      coded_rows(std::true_type());
     }
     if (recent) {
       // ---- the rows behind the last whole block, 16 bf16 rows of this warp at a time.  Weights are two bf16 numbers each. ----
@@ -626,7 +688,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
           }
         if (ACROSS) {
 #pragma unroll
-          for (int i = 0; i < 2; i++) hi[0][i] = turn(hi[0][i]), lo[0][i] = turn(lo[0][i]);
+          for (int i = 0; i < 2; i++) hi[0][i] = turn(PAIRED && t4 >= 2 ? lo[0][i] : hi[0][i]), lo[0][i] = turn(lo[0][i]);
         }
         // A weight of zero does not keep what is not a number out of a product: it is taken out, and given to the query rows that see it.
         uint4 v[2][4];   // [half of the lane's channels]: rows 2 t4, 2 t4 + 1, and eight further; channels 16 g ..
@@ -682,7 +744,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
                            c1 = __byte_perm(word(2), word(3), 0x7632);
             if (ACROSS) {
               mma_bf16(o[0][4 * part + k], b0, c0, b1, c1, hi[0][0], hi[0][1]);
-              mma_bf16(o[0][4 * part + k], b0, c0, b1, c1, lo[0][0], lo[0][1]);
+              if (!PAIRED) mma_bf16(o[0][4 * part + k], b0, c0, b1, c1, lo[0][0], lo[0][1]);
             } else {
 #pragma unroll
               for (int mt = 0; mt < MT; mt++) {
@@ -745,6 +807,11 @@ __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(con
           const float4* from = reinterpret_cast<const float4*>(parts + w * 2 * A8_SLOT / 4 + A8<ROWS>::place(tid >> 4, c));
           const float4 x = from[0], y = from[1];
           O[0] += x.x, O[1] += x.y, O[2] += x.z, O[3] += x.w, O[4] += y.x, O[5] += y.y, O[6] += y.z, O[7] += y.w;
+          if (PAIRED) {
+            const float4* more = reinterpret_cast<const float4*>(parts + w * 2 * A8_SLOT / 4 + A8<ROWS>::place((tid >> 4) + 4, c));
+            const float4 x = more[0], y = more[1];
+            O[0] += x.x, O[1] += x.y, O[2] += x.z, O[3] += x.w, O[4] += y.x, O[5] += y.y, O[6] += y.z, O[7] += y.w;
+          }
         }
         if (whole_item) {
           const int rr = group * ROWS + row, t = rr / p.G, hq = h * p.G + rr % p.G;
@@ -882,14 +949,14 @@ int a8_cluster(int64_t items, int64_t tiles, int64_t slots) {
   return (tiles + n - 1) / n <= 3 ? (int)n : 0;
 }
 
-template <bool E4M3, int ROWS, bool DENSE>
+template <bool E4M3, int ROWS, bool DENSE, bool PAIRED>
 int launch_as(Attend8 p, cudaStream_t st) {
   p.row_groups = (p.T * p.G + ROWS - 1) / ROWS;
   const int64_t slots = (int64_t)A8<ROWS>::ctas * sm_count(), most = (int64_t)p.bs * p.c.H * p.row_groups * ((p.c.cap + A8_TILE - 1) / A8_TILE + 1);
   const int blocks = (int)(most < slots ? most : slots * a8_waves(most, slots));
   static PerDevice opted;
   if (const unsigned long long bit = first_on_device(opted)) {
-    if (cudaFuncSetAttribute(attend8_kernel<E4M3, ROWS, DENSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, A8<ROWS>::smem) != cudaSuccess)
+    if (cudaFuncSetAttribute(attend8_kernel<E4M3, ROWS, DENSE, PAIRED>, cudaFuncAttributeMaxDynamicSharedMemorySize, A8<ROWS>::smem) != cudaSuccess)
       return fail(PK_ERR_CUDA, "cache8_attention: %s", cudaGetErrorString(cudaGetLastError()));
     mark_on_device(opted, bit);
   }
@@ -903,17 +970,22 @@ int launch_as(Attend8 p, cudaStream_t st) {
     attr[0].id = cudaLaunchAttributeClusterDimension, attr[0].val.clusterDim.x = (unsigned)p.cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr, cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, attend8_kernel<E4M3, ROWS, DENSE>, p);
+    cudaLaunchKernelEx(&cfg, attend8_kernel<E4M3, ROWS, DENSE, PAIRED>, p);
     return check_launch("cache8_attention");
   }
-  launch_chain(attend8_kernel<E4M3, ROWS, DENSE>, dim3((unsigned)blocks), dim3(A8_THREADS), A8<ROWS>::smem, st, p);
+  launch_chain(attend8_kernel<E4M3, ROWS, DENSE, PAIRED>, dim3((unsigned)blocks), dim3(A8_THREADS), A8<ROWS>::smem, st, p);
   launch_chain(attend8_merge_kernel<ROWS>, dim3((unsigned)((int64_t)p.bs * p.T * p.c.H * p.G)), dim3(128), 0, st, p, blocks);
   return check_launch("cache8_attention", 2);
 }
 
-template <bool E4M3, int ROWS>
+template <bool E4M3, int ROWS, bool PAIRED = false>
 int launch(const Attend8& p, cudaStream_t st) {   // K and V of a row side by side, row after row: the copies' addresses are constants apart
-  return p.c.c_l == 256 ? launch_as<E4M3, ROWS, true>(p, st) : launch_as<E4M3, ROWS, false>(p, st);
+  return p.c.c_l == 256 ? launch_as<E4M3, ROWS, true, PAIRED>(p, st) : launch_as<E4M3, ROWS, false, PAIRED>(p, st);
+}
+template <bool E4M3>
+int launch_rows(const Attend8& p, int rows, cudaStream_t st) {
+  if (p.T * p.G <= 4) return launch<E4M3, 8, true>(p, st);
+  return rows == 8 ? launch<E4M3, 8>(p, st) : rows == 16 ? launch<E4M3, 16>(p, st) : launch<E4M3, 32>(p, st);
 }
 
 }  // namespace
@@ -963,6 +1035,5 @@ extern "C" int pk_cache8_attention(const pk_tensor* queries, const pk_cache8* ca
   p.out = (uint16_t*)out->data, p.records = (float*)workspace;
   const cudaStream_t st = (cudaStream_t)stream;
   const int rows = a8_rows(bs * H, p.T * p.G, (p.c.cap + A8_TILE - 1) / A8_TILE + 1, sm_count());
-  if (cache->codes->dtype == PK_E4M3) return rows == 8 ? launch<true, 8>(p, st) : rows == 16 ? launch<true, 16>(p, st) : launch<true, 32>(p, st);
-  return rows == 8 ? launch<false, 8>(p, st) : rows == 16 ? launch<false, 16>(p, st) : launch<false, 32>(p, st);
+  return cache->codes->dtype == PK_E4M3 ? launch_rows<true>(p, rows, st) : launch_rows<false>(p, rows, st);
 }

@@ -76,8 +76,8 @@ def check(n, block, dtype, lengths, H, T, G, item):
 
 
 UNEVEN = [20000, 17, 12001, 0, 128, 19999, 5000, 1, 129, 8192, 300]
-# 12 query rows are items of 16, 24 of 32, 40 two of them; T 1 and 8 heads one of eight
-CASES = [(1, 8, 8), (3, 4, 16), (6, 4, 32), (5, 8, 32)]
+# four and eight query rows are items of eight, 12 of 16, 24 of 32, 40 two of them
+CASES = [(1, 4, 8), (1, 8, 8), (3, 4, 16), (6, 4, 32), (5, 8, 32)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -104,7 +104,7 @@ def test_more_samples_than_lanes(dtype, T, G, rows):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("T,G,rows", CASES[:2])
+@pytest.mark.parametrize("T,G,rows", CASES[:3])
 @pytest.mark.parametrize("lengths", ["even", "uneven"])
 def test_two_ranges_a_place(dtype, T, G, rows, lengths):
     check(20000, 64, dtype, [20000 - 64 * i if lengths == "even" else (20000, 0, 777, 9001)[i % 4] for i in range(36)], 4, T, G, (rows, 2))
