@@ -465,7 +465,7 @@ int launch_vec_as(const MvParams& p, int blocks, cudaStream_t st) {
   launch_chain(matvec_i8_kernel<T, CH, U>, dim3((unsigned)blocks), dim3(MV_THREADS), 0, st, p);
   return check_launch("matmul_i8");
 }
-// Rows at a time: four of 512 columns where a warp has few (B200, us, one token, four | eight at a time: 1024 x 1024 1.9 | 2.7, 6144 x 4096 4.3 | 5.3), eight where it has many (12288 x 4096 11.2 | 10.3,
+// Rows at a time: four of 512 columns where a warp has few (B200, us, one token, one matrix again and again, four | eight at a time: 1024 x 1024 1.9 | 2.7, 6144 x 4096 4.3 | 5.3), eight where it has many (12288 x 4096 11.2 | 10.3,
 // 24576 x 4096 18.9 | 17.5, 151936 x 4096 95 | 91).
 template <int T>
 int launch_vec(MvParams p, cudaStream_t st) {
@@ -475,7 +475,9 @@ int launch_vec(MvParams p, cudaStream_t st) {
   const bool many = p.O / (blocks * groups) >= 32;
   if (per == 1) return many ? launch_vec_as<T, 1, 8>(p, blocks, st) : launch_vec_as<T, 1, 4>(p, blocks, st);
   if (per == 2) return many ? launch_vec_as<T, 2, 4>(p, blocks, st) : launch_vec_as<T, 2, 2>(p, blocks, st);
-  return per == 3 ? launch_vec_as<T, 3, 2>(p, blocks, st) : launch_vec_as<T, 4, 2>(p, blocks, st);
+  if constexpr (T < 4)
+    if (per == 4) return launch_vec_as<T, 4, 2>(p, blocks, st);
+  return launch_vec_as<T, 3, 2>(p, blocks, st);
 }
 constexpr int MV_MOST = 4 * 8 * 512;   // columns
 
@@ -489,7 +491,7 @@ bool bytes_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Blocks that share a tile's columns: as many as there are SMs for, each with so many steps that the sums' way through shared memory is worth it.  B200, us, 4096 columns, by 1 | 2 | 3 | 4 | 6 | 8 blocks:
+// Blocks that share a tile's columns: as many as there are SMs for, each with so many steps that the sums' way through shared memory is worth it.  B200, us, 4096 columns (one matrix again and again), by 1 | 2 | 3 | 4 | 6 | 8 blocks:
 // 16 tokens, 1024 rows 9.6 | 7.6 | 6.3 | 5.5 | 5.6 | 5.2, 6144 rows 10.4 | 8.3 | 7.6 | 7.6 | 12.0 | 11.6, 24576 rows 18.9 | 26 | 30 | 28 | 39 | 42;  128 tokens, 6144 rows 13.4 | 15.5 | 14.2 | 12.8 | 21 | 20.
 int mm_split(int64_t tiles, int chunks, int nt) {
   const int least = nt / 8;
@@ -581,8 +583,10 @@ extern "C" int pk_matmul_i8(const pk_tensor* x, const pk_tensor* x_scales, const
   p.sx = (const float*)x_scales->data, p.so = (const float*)weight_scales->data, p.out = (uint16_t*)out->data, p.out_t = out->stride[0];
   p.T = (int)T, p.O = (int)O, p.chunks = (int)((I + MM_K - 1) / MM_K);
   const cudaStream_t st = (cudaStream_t)stream;
-  // Which kernel, B200, us, without | with tensor cores: 6144 x 4096, one token 4.3 | 8.2, four 7.0 | 8.2; 24576 x 4096, two tokens 18.5 | 19.6, four 20.8 | 19.6.
-  if (I <= MV_MOST && (T <= 2 || (T <= 4 && O * I <= 48 << 20))) {
+  // Which kernel, B200, us, without | with tensor cores, one matrix again and again (from L2): 6144 x 4096, one token 4.3 | 8.2, three 5.8 | 7.6, four 6.5 | 7.5; 24576 x 4096, two tokens 18.5 | 19.6, four 20.8 | 19.6;
+  // 3000 x 16384, three tokens 8.1 | 10.0, but four, whose values and sums do not fit into the registers from 12289 columns on, 12.5 | 10.1.  Matrices of 300 MB in turn: 6144 x 4096, four tokens 8.1 | 9.2,
+  // 4096 x 12288 10.8 | 12.9, 3000 x 16384 15.9 | 14.0.
+  if (I <= MV_MOST && (T <= 2 || (T <= 4 && O * I <= 48 << 20 && (T == 3 || I <= MV_MOST * 3 / 4)))) {
     const MvParams v = {(const int8_t*)weight->data, (const int8_t*)x->data, O > 1 ? weight->stride[0] : I, T > 1 ? x->stride[0] : I, p.sx, p.so, p.out, p.out_t, (int)O, (int)I, 0};
     return T == 1 ? launch_vec<1>(v, st) : T == 2 ? launch_vec<2>(v, st) : T == 3 ? launch_vec<3>(v, st) : launch_vec<4>(v, st);
   }
