@@ -13,10 +13,10 @@
 // Tiles of 128 rows, four warps of a block side by side.  Short caches: a cluster of blocks per item (sample, KV head, group of query rows), one launch.  Others: the tiles of all items, laid end to end, are cut
 // into equal ranges as in attend_few.cu, and attend8_merge_kernel joins the records of items that are cut.
 //
-// B200, us, replayed graphs.  128K keys of 8 heads, a token of four queries each (269 MB) 53: blocks begin their rows 2 us after the start and end after 33 to 49, as fast as their SMs get them (with the products left
-// out the whole takes 46), the joining launch takes 2; 16 sequences of 16 - 32K (e4m3) 135, 6.1 TB/s; 32 query rows a KV head over 8 x 58K keys 44: eight warps an SM by their registers, which wait for one
-// another's turn on the tensor cores 36 % of the time.
-// Kept: loops by segment with one scaling for the 16 rows that share a scale, 100 -> 60; less code around the loops (run once, it costs its fetching) 97 -> 60 for 32 rows; query rows across and a lazy maximum
+// B200, us, replayed graphs.  128K keys of 8 heads, a token of four queries each (269 MB) 53.7: blocks begin their rows 2 us after the start and end after 33 to 49, as fast as their SMs get them (with the products left
+// out the whole takes 46), the joining launch takes 2; 16 sequences of 16 - 32K (e4m3) 136, 6.0 TB/s; 32 query rows a KV head over 8 x 58K keys 52: eight warps an SM by their registers, tensor cores busy 46 % of the
+// time, the rest they wait for one another's turn.
+// Steps of the form with one fp16 number for a weight: loops by segment with one scaling for the 16 rows that share a scale, 100 -> 60; less code around the loops (run once, it costs its fetching) 97 -> 60 for 32 rows; query rows across and a lazy maximum
 // 56 -> 55, 60 -> 52; ranges that end where the items do 50 -> 47; queries asked for before the rows, two steps of copies at once, all records under way 47.6 -> 44.5.  No better: three stages, two blocks an SM
 // (52 - 54), two ranges a place (58; of long ranges they are kept), two scores an instruction.
 #include <type_traits>
@@ -240,7 +240,8 @@ __device__ __forceinline__ float4 remote4(const void* at, int rank) {
 }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// PAIRED: up to four query rows.  They are columns 0 to 3 of the products and 4 to 7 too, and the second parts of the weights are the weights of the latter, so that one product has both (16 sequences of 16 - 32K, after a second of them, e4m3 146 -> 143 us, int8 157 -> 152).
+// PAIRED: up to four query rows.  They are columns 0 to 3 of the products and 4 to 7 too, and the second parts of the weights are the weights of the latter, so that one product has both
+// (16 sequences of 16 - 32K, after a second of them, e4m3 146 -> 143 us, int8 157 -> 152).
 template <bool E4M3, int ROWS, bool DENSE, bool PAIRED>
 __global__ void __launch_bounds__(A8_THREADS, A8<ROWS>::ctas) attend8_kernel(const __grid_constant__ Attend8 p) {
   constexpr bool ACROSS = A8<ROWS>::across;
@@ -933,8 +934,8 @@ int64_t a8_waves(int64_t most, int64_t slots) {
   return most / slots >= 48 ? 2 : 1;
 }
 
-// Query rows of an item.  Few tiles in all: eight, which has the shortest way through its code (B200, us, five tokens of five heads over 43 keys 8.7 | 15.7 with 32 rows, eight tokens of four heads over 1000
-// keys 11.0 | 14.9); then as many as the KV head has, up to 32, because each item reads the cache again.
+// Query rows of an item.  Few tiles in all: eight, which has the shortest way through its code (B200, us, five tokens of five heads over 43 keys 6.1 | 9.4 with 32 rows, eight tokens of four heads over 1000
+// keys 8.3 | 10.9); then as many as the KV head has, up to 32, because each item reads the cache again.
 int a8_rows(int64_t heads, int64_t rows, int64_t tiles, int sms) {
   for (int n = 8; n < 32; n *= 2)
     if (rows <= n || heads * ((rows + n - 1) / n) * tiles <= 6 * sms) return n;
